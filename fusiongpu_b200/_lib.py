@@ -51,6 +51,19 @@ class GraphSearchParams(C.Structure):
                 ("seed", C.c_uint32), ("metric", C.c_int32), ("entry_probes", C.c_int32)]
 
 
+class LinearParams(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("in_dim", C.c_int32), ("out_dim", C.c_int32), ("dtype", C.c_int32),
+                ("activation", C.c_int32), ("x_stride", C.c_int64), ("w_stride", C.c_int64),
+                ("residual_stride", C.c_int64), ("pre_stride", C.c_int64), ("y_stride", C.c_int64)]
+
+
+class PreferenceParams(C.Structure):
+    _fields_ = [("nq", C.c_int32), ("dim", C.c_int32), ("dtype", C.c_int32), ("base_dtype", C.c_int32),
+                ("nbase", C.c_int64), ("n_pairs", C.c_int64), ("metric", C.c_int32), ("beta", C.c_float),
+                ("label_smoothing", C.c_float), ("query_stride", C.c_int64), ("ref_stride", C.c_int64),
+                ("dq_stride", C.c_int64)]
+
+
 # name -> argtypes (all return int status unless noted)
 _P, _I32, _I64, _U32, _F, _SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_uint32, C.c_float, C.c_size_t
 _SIGS = {
@@ -96,6 +109,14 @@ _SIGS = {
                         _P, _P, _SZ, _P],
     "fg_knn": [_P, _I64, _I32, _P, _I32, _I32, _I32, _P, _P, _P, _SZ, _P],
     "fg_knn_exact": [_P, _I64, _I32, _P, _I32, _I32, _P, _P, _P, _SZ, _P],
+    "fg_layer_norm": [_P, _I32, _I64, _I32, _I64, _P, _P, _I32, _F, _P, _I64, _P, _P, _P],
+    "fg_layer_norm_backward_workspace_size": [_I64, _I32, C.POINTER(_SZ)],
+    "fg_layer_norm_backward": [_P, _I64, _P, _I32, _I64, _I32, _I64, _P, _I32, _P, _P, _P, _I64, _P, _P, _P, _SZ, _P],
+    "fg_linear_workspace_size": [C.POINTER(LinearParams), C.POINTER(_SZ)],
+    "fg_linear": [C.POINTER(LinearParams), _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "fg_linear_backward_workspace_size": [C.POINTER(LinearParams), C.POINTER(_SZ)],
+    "fg_linear_backward": [C.POINTER(LinearParams), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "fg_preference_loss": [C.POINTER(PreferenceParams), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
 }
 
 _lib = None

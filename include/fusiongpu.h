@@ -32,10 +32,13 @@ typedef enum {
     FG_METRIC_IP = 1
 } fg_metric;
 
-/* Element type of the graph index's vectors. */
+/* Element types.  The graph index's vectors are F32 or F16; the query
+ * adapter's operators take F32, F16 and BF16, and its documents U8 too. */
 typedef enum {
     FG_DTYPE_F32 = 0,
-    FG_DTYPE_F16 = 1
+    FG_DTYPE_F16 = 1,
+    FG_DTYPE_BF16 = 2,
+    FG_DTYPE_U8 = 3
 } fg_dtype;
 
 typedef enum {
@@ -440,6 +443,109 @@ int fg_knn_exact(const float* base, int64_t nbase, int32_t dim, const float* que
 int fg_knn(const float* base, int64_t nbase, int32_t dim, const float* queries, int32_t nq,
            int32_t k, int32_t metric, int32_t* out_ids, float* out_dists, void* workspace,
            size_t workspace_bytes, void* stream);
+
+/* ---- query adapter (no counterpart in the reference, which searches the
+ * queries as they are): the operators of a small model between an embedding
+ * model and fg_search, and of its training on preferences over the index's
+ * documents.  Element types are fg_dtype values; sums, statistics and
+ * products are held in 32 bits and rounded once, when a result is written.
+ * Matrices are row-major with unit column stride; a row stride counts
+ * elements, and 0 means the row length.  No pointer or stride needs more
+ * alignment than its element type (16-byte aligned rows run faster).  Rows
+ * may number 0.  No call synchronises the host; results do not depend on the
+ * order in which the GPU runs its blocks.  Outputs must not overlap inputs. */
+
+/* Layer norm over each row: y = (x - mean) * rstd * weight + bias, rstd =
+ * 1 / sqrt(variance + eps).  x, y: [rows][dim] of dtype; weight, bias [dim] of
+ * param_dtype (dtype or F32), each NULL for 1 and 0; mean, rstd [rows] float,
+ * both or neither (the backward pass needs them).  1 <= dim <= 16384. */
+int fg_layer_norm(const void* x, int32_t dtype, int64_t rows, int32_t dim, int64_t x_stride, const void* weight,
+                  const void* bias, int32_t param_dtype, float eps, void* y, int64_t y_stride, float* mean,
+                  float* rstd, void* stream);
+
+/* Its gradients: with h = (x - mean) * rstd and a = dy * weight,
+ * dx = rstd * (a - avg(a) - h * avg(a h)); dweight = sum over rows of dy h and
+ * dbias = sum over rows of dy, in param_dtype (0 for no rows).  Any of dx,
+ * dweight, dbias may be NULL.  The workspace holds one partial row of both
+ * sums per resident block, added in block order. */
+int fg_layer_norm_backward_workspace_size(int64_t rows, int32_t dim, size_t* bytes);
+int fg_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int32_t dtype, int64_t rows,
+                           int32_t dim, int64_t x_stride, const void* weight, int32_t param_dtype, const float* mean,
+                           const float* rstd, void* dx, int64_t dx_stride, void* dweight, void* dbias,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Activations of the linear layer: GELU is z * Phi(z) (the erf form), SiLU
+ * z / (1 + exp(-z)). */
+typedef enum {
+    FG_ACT_NONE = 0,
+    FG_ACT_RELU = 1,
+    FG_ACT_GELU = 2,
+    FG_ACT_SILU = 3
+} fg_activation;
+
+/* Linear layer: z = x w^T + bias, y = activation(z) + residual.  x [rows]
+ * [in_dim], w [out_dim][in_dim], bias [out_dim], residual, z and y [rows]
+ * [out_dim], all of one dtype; bias, residual and pre may be NULL; pre receives
+ * z for the backward pass.  z is not rounded before the activation. */
+typedef struct {
+    int64_t rows;
+    int32_t in_dim;
+    int32_t out_dim;
+    int32_t dtype;            /* F32, F16 or BF16                               */
+    int32_t activation;       /* fg_activation                                  */
+    int64_t x_stride;         /* row strides in elements, 0: the row length     */
+    int64_t w_stride;
+    int64_t residual_stride;
+    int64_t pre_stride;
+    int64_t y_stride;         /* y, and dy in the backward pass                 */
+} fg_linear_params;
+
+int fg_linear_workspace_size(const fg_linear_params* params, size_t* bytes);
+int fg_linear(const fg_linear_params* params, const void* x, const void* w, const void* bias, const void* residual,
+              void* pre, void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradients: dz = dy * activation'(pre), dx [rows][in_dim] = dz w,
+ * dw [out_dim][in_dim] = dz^T x, dbias [out_dim] = sum over rows of dz, all
+ * contiguous and of dtype; any may be NULL (w is needed for dx, x for dw, pre
+ * unless the activation is NONE).  The residual's gradient is dy itself.
+ * ReLU's derivative at 0 is 0. */
+int fg_linear_backward_workspace_size(const fg_linear_params* params, size_t* bytes);
+int fg_linear_backward(const fg_linear_params* params, const void* dy, const void* x, const void* w, const void* pre,
+                       void* dx, void* dw, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Preference loss over documents of an index.  The policy of query q prefers
+ * documents by softmax of the search score s (inner product, or minus squared
+ * L2 distance); in the ratio of two documents of one query the normaliser
+ * cancels.  For a pair (pos, neg) of query i, with a reference query r_i (the
+ * unadapted query; ref NULL: a uniform reference),
+ *   margin = beta * (s(q_i, pos) - s(q_i, neg) - s(r_i, pos) + s(r_i, neg)),
+ *   loss = -(1 - label_smoothing) log sigmoid(margin)
+ *          - label_smoothing log sigmoid(-margin),
+ * and dq_i = sum over its pairs of weight * d loss / d q_i, in pair order
+ * within fixed groups.  Pairs of query i are [offsets[i], offsets[i+1]);
+ * offsets ascend from 0 to n_pairs (out-of-range values are clamped).  A pair
+ * with an id outside [0, nbase) is masked: loss and margin 0, no gradient.
+ * base: raw vectors [nbase][dim] (contiguous) of base_dtype; queries, ref, dq
+ * [nq][dim] of dtype; weights [n_pairs] float or NULL for 1; losses [n_pairs],
+ * margins [n_pairs] (or NULL); dq NULL: the loss alone.  dim <= 16384. */
+typedef struct {
+    int32_t nq;
+    int32_t dim;
+    int32_t dtype;            /* queries, ref, dq: F32, F16 or BF16              */
+    int32_t base_dtype;       /* F32, F16, BF16 or U8                            */
+    int64_t nbase;
+    int64_t n_pairs;
+    int32_t metric;           /* fg_metric                                       */
+    float beta;               /* > 0                                             */
+    float label_smoothing;    /* [0, 0.5]                                        */
+    int64_t query_stride;     /* row strides in elements, 0: dim                 */
+    int64_t ref_stride;
+    int64_t dq_stride;
+} fg_preference_params;
+
+int fg_preference_loss(const fg_preference_params* params, const void* queries, const void* ref, const void* base,
+                       const int64_t* offsets, const int32_t* pos_ids, const int32_t* neg_ids, const float* weights,
+                       float* losses, float* margins, void* dq, void* stream);
 
 #ifdef __cplusplus
 }

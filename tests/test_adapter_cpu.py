@@ -1,0 +1,117 @@
+"""CPU tests of the query adapter's C entry points: refusals and workspace
+sizes (host logic; nothing is launched) and the ctypes structures."""
+import ctypes as C
+import os
+import re
+
+import pytest
+
+from fusiongpu_b200 import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P = C.c_void_p(4096)  # stands for a device pointer; refused calls never use it
+
+
+def _struct_fields(name):
+    h = open(os.path.join(ROOT, "include", "fusiongpu.h")).read()
+    h = re.sub(r"/\*.*?\*/", "", h, flags=re.S)
+    body = re.search(r"typedef struct \{([^}]*)\} " + name + ";", h).group(1)
+    types = {"int32_t": C.c_int32, "int64_t": C.c_int64, "float": C.c_float}
+    return [(f, types[t]) for t, f in re.findall(r"(\w+)\s+(\w+);", body)]
+
+
+@pytest.mark.parametrize("name,cls", [("fg_linear_params", _lib.LinearParams),
+                                      ("fg_preference_params", _lib.PreferenceParams)])
+def test_structures_match_the_header(name, cls):
+    assert list(cls._fields_) == _struct_fields(name)
+
+
+def _linear(**kw):
+    v = dict(rows=10, in_dim=8, out_dim=4, dtype=0, activation=0, x_stride=0, w_stride=0, residual_stride=0,
+             pre_stride=0, y_stride=0)
+    v.update(kw)
+    return _lib.LinearParams(*v.values())
+
+
+def _status(name, *args):
+    return getattr(_lib.lib(), name)(*args)
+
+
+def _message():
+    return _lib.lib().fg_last_error().decode()
+
+
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(in_dim=0), dict(out_dim=0), dict(dtype=3), dict(dtype=-1),
+                                dict(activation=4), dict(x_stride=7), dict(w_stride=7), dict(y_stride=3),
+                                dict(pre_stride=3), dict(residual_stride=-4)])
+def test_linear_refuses(kw):
+    p, n = _linear(**kw), C.c_size_t()
+    assert _status("fg_linear", C.byref(p), P, P, None, None, None, P, None, 0, None) == 1 and _message()
+    assert _status("fg_linear_workspace_size", C.byref(p), C.byref(n)) == 1
+    assert _status("fg_linear_backward", C.byref(p), P, P, P, P, P, P, P, None, 0, None) == 1
+    assert _status("fg_linear_backward_workspace_size", C.byref(p), C.byref(n)) == 1
+
+
+def test_linear_null_arguments():
+    p = _linear(activation=2)
+    assert _status("fg_linear", None, P, P, None, None, None, P, None, 0, None) == 1
+    for x, w, y in ((None, P, P), (P, None, P), (P, P, None)):
+        assert _status("fg_linear", C.byref(p), x, w, None, None, None, y, None, 0, None) == 1
+    assert _status("fg_linear_workspace_size", C.byref(p), None) == 1
+    # dy; pre with an activation; w for dx; x for dw
+    for dy, x, w, pre in ((None, P, P, P), (P, P, P, None), (P, P, None, P), (P, None, P, P)):
+        assert _status("fg_linear_backward", C.byref(p), dy, x, w, pre, P, P, P, P, 1 << 40, None) == 1
+    n = _lib.size_query("fg_linear_backward_workspace_size", C.byref(p))
+    assert n >= 10 * 4 * 4  # dz
+    for ws, b in ((None, n), (P, n - 1), (C.c_void_p(4096 + 8), n)):
+        assert _status("fg_linear_backward", C.byref(p), P, P, P, P, P, P, P, ws, b, None) == 3
+    empty = _linear(rows=0)
+    assert _status("fg_linear", C.byref(empty), None, None, None, None, None, None, None, 0, None) == 0
+
+
+def test_layer_norm_refuses():
+    ok = dict(x=P, dtype=0, rows=4, dim=8, ldx=0, w=None, b=None, pd=0, eps=1e-5, y=P, ldy=0, m=None, r=None, s=None)
+
+    def st(**kw):
+        return _status("fg_layer_norm", *{**ok, **kw}.values())
+
+    for kw in (dict(dtype=3), dict(pd=1), dict(dtype=1, pd=2), dict(rows=-1), dict(dim=0), dict(ldx=7), dict(ldy=-8),
+               dict(eps=-1.0), dict(eps=float("nan")), dict(x=None), dict(y=None), dict(m=P), dict(r=P)):
+        assert st(**kw) == 1, kw
+    assert st(dim=16385) == 4
+    assert st(rows=0, x=None, y=None) == 0
+    n = _lib.size_query("fg_layer_norm_backward_workspace_size", 1000, 768)
+    assert n >= 2 * 768 * 4
+    ok = dict(dy=P, lddy=0, x=P, dtype=1, rows=4, dim=8, ldx=0, w=P, pd=0, m=P, r=P, dx=P, lddx=0, dw=P, db=P, ws=P,
+              wb=1 << 40, s=None)
+
+    def st(**kw):
+        return _status("fg_layer_norm_backward", *{**ok, **kw}.values())
+
+    for kw in (dict(dtype=7), dict(pd=2), dict(rows=-1), dict(dim=-3), dict(ldx=3), dict(lddy=3), dict(lddx=3),
+               dict(dy=None), dict(x=None), dict(m=None), dict(r=None)):
+        assert st(**kw) == 1, kw
+    assert st(dim=20000) == 4
+    for kw in (dict(ws=None), dict(wb=8), dict(ws=C.c_void_p(4097))):
+        assert st(**kw) == 3, kw
+
+
+def test_preference_refuses():
+    base = dict(nq=4, dim=8, dtype=0, base_dtype=3, nbase=10, n_pairs=6, metric=0, beta=1.0, label_smoothing=0.0,
+                query_stride=0, ref_stride=0, dq_stride=0)
+
+    def st(args=(P, P, P, P, P, P, P, P, P, P), **kw):
+        p = _lib.PreferenceParams(*{**base, **kw}.values())
+        return _status("fg_preference_loss", C.byref(p), *args, None)
+
+    for kw in (dict(nq=-1), dict(dim=0), dict(dtype=3), dict(base_dtype=4), dict(nbase=-1), dict(n_pairs=-1),
+               dict(metric=2), dict(beta=0.0), dict(beta=-1.0), dict(beta=float("inf")), dict(beta=float("nan")),
+               dict(label_smoothing=0.51), dict(label_smoothing=-0.01), dict(query_stride=7), dict(ref_stride=7),
+               dict(dq_stride=-1)):
+        assert st(**kw) == 1, kw
+    assert st(dim=16385) == 4
+    full = [P] * 10
+    for k in (0, 2, 3, 4, 5, 7):  # queries, base, offsets, pos, neg, losses
+        assert st(full[:k] + [None] + full[k + 1:]) == 1, k
+    assert st([None] * 10, nq=0) == 0
+    assert _status("fg_preference_loss", None, *full, None) == 1

@@ -791,11 +791,7 @@ __global__ void __launch_bounds__(FIN_WARPS * 32) coarse_topk_finish_kernel(
 
 // ---- host side ---------------------------------------------------------------
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
+tc::EncodeTiledFn tc::encode_fn() {
     static EncodeTiledFn fn = nullptr;
     if (!fn) {
         void* p = nullptr;
@@ -808,7 +804,7 @@ static EncodeTiledFn encode_fn() {
 }
 
 static int make_map(CUtensorMap* m, const void* base, long long rows, int kpad, int box_rows) {
-    EncodeTiledFn enc = encode_fn();
+    tc::EncodeTiledFn enc = tc::encode_fn();
     if (!enc) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     if (!aligned(base, 16)) return fail(FG_ERR_INVALID_ARG, "TMA operand not 16-byte aligned");
     cuuint64_t dims[2] = {(cuuint64_t)kpad, (cuuint64_t)rows};

@@ -4,54 +4,11 @@
 //   z = x w^T + bias,  y = act(z) + residual
 //   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  dbias = sum over rows of dz
 #include <algorithm>
+#include <type_traits>
 
-#include "adapter_common.cuh"
+#include "linear.cuh"
 
 namespace fg {
-
-struct Epilogue {
-    const void *bias, *residual;
-    void *pre, *y;
-    long long ldr, ldp, ldy;
-    int act;
-};
-
-// C(m, n) = sum over k of A(m, k) B(n, k); strides per index.
-struct GemmShape {
-    long long m, n, k;
-    long long am, ak, bn, bk;
-};
-
-__device__ __forceinline__ float activate(float z, int act) {
-    switch (act) {
-        case FG_ACT_RELU: return z > 0.0f ? z : (z == z ? 0.0f : z);
-        case FG_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678f));
-        case FG_ACT_SILU: return z / (1.0f + expf(-z));
-        default: return z;
-    }
-}
-
-__device__ __forceinline__ float activate_grad(float z, int act) {
-    switch (act) {
-        case FG_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-        case FG_ACT_GELU:
-            return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * expf(-0.5f * z * z) * 0.39894228f;
-        case FG_ACT_SILU: {
-            const float s = 1.0f / (1.0f + expf(-z));
-            return s * (1.0f + z * (1.0f - s));
-        }
-        default: return 1.0f;
-    }
-}
-
-template <class T>
-__device__ __forceinline__ void epilogue_store(const Epilogue& e, long long m, long long n, float z) {
-    if (e.bias) z += to_f32(static_cast<const T*>(e.bias)[n]);
-    if (e.pre) static_cast<T*>(e.pre)[m * e.ldp + n] = from_f32<T>(z);
-    float y = activate(z, e.act);
-    if (e.residual) y += to_f32(static_cast<const T*>(e.residual)[m * e.ldr + n]);
-    static_cast<T*>(e.y)[m * e.ldy + n] = from_f32<T>(y);
-}
 
 constexpr int SG_T = 64, SG_K = 16;
 
@@ -101,6 +58,8 @@ static int gemm(const void* a, const void* b, const GemmShape& g, const Epilogue
     const long long tiles = ((g.m + SG_T - 1) / SG_T) * ((g.n + SG_T - 1) / SG_T);
     FG_REQUIRE(tiles <= 0x7fffffffll, "%lld x %lld outputs: too many tiles", g.m, g.n);
     if (tiles == 0) return FG_OK;
+    if (sizeof(T) == 2 && tc_gemm_fits(a, b, g))
+        return tc_gemm(std::is_same<T, __half>::value ? FG_DTYPE_F16 : FG_DTYPE_BF16, a, b, g, e, s);
     gemm_simt_kernel<T><<<(unsigned)tiles, 256, 0, s>>>(static_cast<const T*>(a), static_cast<const T*>(b), g, e);
     return check_launch("gemm_simt_kernel");
 }

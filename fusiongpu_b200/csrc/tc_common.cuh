@@ -12,6 +12,12 @@
 namespace fg {
 namespace tc {
 
+// cuTensorMapEncodeTiled, resolved at run time (coarse_tc.cu); null without a driver.
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn();
+
 constexpr uint32_t kWaitLimit = 1u << 20;  // try_wait polls before a wait is declared failed
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -130,6 +136,19 @@ __device__ __forceinline__ uint64_t desc_kmajor_sw128(const void* smem) {
     d |= (uint64_t)(1024 >> 4) << 32;     // stride byte offset: next 8-row atom
     d |= (uint64_t)1 << 46;               // descriptor version (sm_100)
     d |= (uint64_t)2 << 61;               // SWIZZLE_128B
+    return d;
+}
+
+// The same for an MN-major operand: chunks of 64 MN elements, each `chunk` bytes
+// of K rows of 128 bytes; leading offset = next chunk, stride offset = next 8 K.
+__device__ __forceinline__ uint64_t desc_mnmajor_sw128(const void* smem, uint32_t chunk) {
+    const uint32_t a = smem_u32(smem);
+    uint64_t d = 0;
+    d |= (uint64_t)((a >> 4) & 0x3FFFu);
+    d |= (uint64_t)((chunk >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
     return d;
 }
 

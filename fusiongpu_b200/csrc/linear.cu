@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const T* dy, long long lddy, co
     if (j < dim)
         for (long long r = r0 + warp; r < r1; r += 8) {
             float v = to_f32(dy[r * lddy + j]);
-            if (act != FG_ACT_NONE) v *= activate_grad(to_f32(pre[r * ldp + j]), act);
+            if (act != FG_ACT_NONE) v *= activate_grad<sizeof(T) == 2>(to_f32(pre[r * ldp + j]), act);
             if (dz) dz[r * dim + j] = from_f32<T>(v);
             b += v;
         }

@@ -19,23 +19,61 @@ struct GemmShape {
     long long am, ak, bn, bk;
 };
 
+// GELU = z Phi(z).  float32 results: CUDA's erfc, which keeps the small tail.
+// Results rounded to 16 bits (FAST): with a = |z| / sqrt(2), t = 1 / (1 + 0.3275911 a)
+// and e = exp(-a^2), erfc(a) = e t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) + 1.5e-7
+// (Abramowitz and Stegun 7.1.26): two special-function and a dozen other
+// operations, where erff would bound the epilogue.  e also serves the
+// derivative Phi(z) + z exp(-z^2 / 2) / sqrt(2 pi).
+__device__ __forceinline__ float upper_tail(float z, float& e) {  // Phi(-|z|)
+    const float t = __fdividef(1.0f, fmaf(fabsf(z), 0.3275911f * 0.70710678f, 1.0f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * z * (-0.5f * 1.44269504f)));
+    float p = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    p = fmaf(t, p, 0.5f * 1.421413741f);
+    p = fmaf(t, p, 0.5f * -0.284496736f);
+    p = fmaf(t, p, 0.5f * 0.254829592f);
+    return p * t * e;
+}
+
+template <bool FAST>
+__device__ __forceinline__ float sigmoid(float z) {  // z >= -100
+    // below -87 the quotient's divisor would pass 2^126, where __fdividef is 0
+    if (FAST) return __fdividef(z < -87.0f ? 0.0f : 1.0f, 1.0f + __expf(z < -87.0f ? 87.0f : -z));
+    return 1.0f / (1.0f + expf(-z));
+}
+
+template <bool FAST>
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
         case FG_ACT_RELU: return z > 0.0f ? z : (z == z ? 0.0f : z);
-        case FG_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678f));
-        case FG_ACT_SILU: return z / (1.0f + expf(-z));
+        case FG_ACT_GELU: {
+            if (!FAST) return fmaxf(z, -100.0f) * (0.5f * erfcf(z * -0.70710678f));
+            float e;
+            const float q = upper_tail(z, e);
+            return fmaf(-fminf(fabsf(z), 100.0f), q, fmaxf(z, 0.0f));
+        }
+        case FG_ACT_SILU:
+            z = z < -100.0f ? -100.0f : z;  // a NaN stays
+            return z * sigmoid<FAST>(z);
         default: return z;
     }
 }
 
+template <bool FAST>
 __device__ __forceinline__ float activate_grad(float z, int act) {
     switch (act) {
         case FG_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-        case FG_ACT_GELU:
-            return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * expf(-0.5f * z * z) * 0.39894228f;
+        case FG_ACT_GELU: {
+            const float zc = fminf(fmaxf(z, -100.0f), 100.0f);
+            if (!FAST) return fmaf(zc, expf(-0.5f * z * z) * 0.39894228f, 0.5f * erfcf(z * -0.70710678f));
+            float e;
+            const float q = upper_tail(z, e);
+            return fmaf(zc * 0.39894228f, e, z >= 0.0f ? 1.0f - q : q);
+        }
         case FG_ACT_SILU: {
-            const float s = 1.0f / (1.0f + expf(-z));
-            return s * (1.0f + z * (1.0f - s));
+            z = z < -100.0f ? -100.0f : z > 100.0f ? 100.0f : z;
+            const float s = sigmoid<FAST>(z);
+            return s * fmaf(z, 1.0f - s, 1.0f);
         }
         default: return 1.0f;
     }
@@ -45,7 +83,7 @@ template <class T>
 __device__ __forceinline__ void epilogue_store(const Epilogue& e, long long m, long long n, float z) {
     if (e.bias) z += to_f32(static_cast<const T*>(e.bias)[n]);
     if (e.pre) static_cast<T*>(e.pre)[m * e.ldp + n] = from_f32<T>(z);
-    float y = activate(z, e.act);
+    float y = activate<sizeof(T) == 2>(z, e.act);
     if (e.residual) y += to_f32(static_cast<const T*>(e.residual)[m * e.ldr + n]);
     static_cast<T*>(e.y)[m * e.ldy + n] = from_f32<T>(y);
 }

@@ -206,8 +206,8 @@ __global__ void __launch_bounds__(GT_NT, 1)
                 z.w += b.w;
             }
             if (e.pre) store4(static_cast<T*>(e.pre) + row * e.ldp + col, z);
-            float4 y = make_float4(activate(z.x, e.act), activate(z.y, e.act), activate(z.z, e.act),
-                                   activate(z.w, e.act));
+            float4 y = make_float4(activate<true>(z.x, e.act), activate<true>(z.y, e.act), activate<true>(z.z, e.act),
+                                   activate<true>(z.w, e.act));
             if (e.residual) {
                 const float4 b = load4(static_cast<const T*>(e.residual) + row * e.ldr + col);
                 y.x += b.x;
@@ -222,6 +222,270 @@ __global__ void __launch_bounds__(GT_NT, 1)
         }
     }
     if (S > 1) cluster_sync();  // a peer may still read this CTA's partial tile
+}
+
+// ---- many tiles: persistent CTA pairs -----------------------------------------------
+//
+// A cluster of two CTAs takes 256 x BN tiles in turn; each MMA (cta_group::2)
+// spans both: a CTA holds 128 rows of A, half of B and the accumulators of its
+// 128 rows, so a K block brings 32 KB into each CTA instead of the 48 KB that a
+// 128 x 256 tile of its own would need.  TMEM holds two accumulators, and the
+// epilogue of a tile runs while the next one is multiplied: a warp takes its 32
+// rows in chunks of 64 columns through a 4 KB buffer that TMA fills with the
+// residual and stores from (whole 128-byte rows, clipped at the matrix's edge).
+constexpr int GP_STAGES = 5;
+constexpr int GP_A = GT_M * GT_K * 2;
+constexpr int GP_BUF = 4096;   // 32 rows x 128 bytes, 128-byte swizzle
+constexpr int GP_EPI = 8;      // epilogue warps: 4 lane quarters x 2 column halves
+
+template <int BN>
+struct PairOf {
+    static constexpr int B = BN / 2 * GT_K * 2, STAGE = GP_A + B;
+    static constexpr int SMEM = GP_STAGES * STAGE + GP_EPI * 2 * GP_BUF + 1024;
+    static constexpr int CHUNKS = BN / 2 / 64;  // per epilogue warp and tile
+};
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+}
+
+template <class T, int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_NT, 1)
+    gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+                     const __grid_constant__ CUtensorMap ty, const __grid_constant__ CUtensorMap tp,
+                     const __grid_constant__ CUtensorMap tr, const TcArgs g) {
+    using P = PairOf<BN>;
+    extern __shared__ __align__(1024) unsigned char dsmem[];
+    __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], acc_full[2], acc_empty[2], res_full[GP_EPI][2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int s_fail;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = (int)cluster_rank();
+    unsigned char* ring = reinterpret_cast<unsigned char*>(
+        (reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char* bufs = ring + GP_STAGES * P::STAGE;
+    const int pairs = (int)(gridDim.x >> 1), tiles = g.mt * g.nt;
+
+    if (tid == 0) {
+        s_fail = 0;
+        for (int i = 0; i < GP_STAGES; ++i) {
+            tc::mbar_init(&full[i], 1);
+            tc::mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(&acc_full[i], 1);
+            tc::mbar_init(&acc_empty[i], 2 * GP_EPI);
+            for (int w = 0; w < GP_EPI; ++w) tc::mbar_init(&res_full[w][i], 1);
+        }
+        tc::fence_mbar_init();
+    }
+    if (warp == 1) tc::tmem_alloc_pair(&tmem_slot, 2 * BN);
+    tc::fence_before_sync();
+    __syncthreads();
+    cluster_sync();  // the peer's barriers are ready too
+    tc::fence_after_sync();
+    const uint32_t taddr = tmem_slot;
+    volatile int* fail = &s_fail;
+
+    if (warp == 0) {
+        if (lane == 0) {  // ---- TMA producer (each CTA its own halves)
+            int i = 0;
+            bool ok = true;
+            for (int t = blockIdx.x >> 1; t < tiles && ok; t += pairs) {
+                const int m0 = t / g.nt * 2 * GT_M + rank * GT_M, n0 = t % g.nt * BN + rank * (BN / 2);
+                for (int kb = 0; kb < g.kt; ++kb, ++i) {
+                    const int st = i % GP_STAGES;
+                    if (!(ok = tc::mbar_wait_or_fail(&empty[st], ((i / GP_STAGES) & 1) ^ 1, fail))) break;
+                    unsigned char *sa = ring + st * P::STAGE, *sb = sa + GP_A;
+                    if (rank == 0) tc::mbar_arrive_expect_tx(&full[st], 2 * P::STAGE);
+                    const uint32_t bar = tc::leader_addr(&full[st]);
+                    if (g.a_mn) {
+                        for (int c = 0; c < GT_M / 64; ++c)
+                            tc::tma_load_2d_pair(sa + c * 8192, &ta, bar, m0 + c * 64, kb * GT_K);
+                    } else {
+                        tc::tma_load_2d_pair(sa, &ta, bar, kb * GT_K, m0);
+                    }
+                    if (g.b_mn) {
+                        for (int c = 0; c < BN / 128; ++c)
+                            tc::tma_load_2d_pair(sb + c * 8192, &tb, bar, n0 + c * 64, kb * GT_K);
+                    } else {
+                        tc::tma_load_2d_pair(sb, &tb, bar, kb * GT_K, n0);
+                    }
+                }
+            }
+            if (!ok && rank == 0)  // copies in flight land before the blocks end
+                for (int j = i > GP_STAGES ? i - GP_STAGES : 0; j < i; ++j)
+                    tc::mbar_wait(&full[j % GP_STAGES], (j / GP_STAGES) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {  // ---- MMA issuer of the pair
+            int i = 0, li = 0;
+            bool ok = true;
+            for (int t = blockIdx.x >> 1; t < tiles && ok; t += pairs, ++li) {
+                const int acc = li & 1;
+                if (!(ok = tc::mbar_wait_or_fail(&acc_empty[acc], ((li >> 1) & 1) ^ 1, fail))) break;
+                tc::fence_after_sync();
+                for (int kb = 0; kb < g.kt; ++kb, ++i) {
+                    const int st = i % GP_STAGES;
+                    if (!(ok = tc::mbar_wait_or_fail(&full[st], (i / GP_STAGES) & 1, fail))) break;
+                    tc::fence_after_sync();
+                    const unsigned char *sa = ring + st * P::STAGE, *sb = sa + GP_A;
+                    const uint64_t da = g.a_mn ? tc::desc_mnmajor_sw128(sa, 8192) : tc::desc_kmajor_sw128(sa);
+                    const uint64_t db = g.b_mn ? tc::desc_mnmajor_sw128(sb, 8192) : tc::desc_kmajor_sw128(sb);
+                    const uint32_t ka = g.a_mn ? 128 : 2, kbs = g.b_mn ? 128 : 2;
+#pragma unroll
+                    for (int kk = 0; kk < GT_K / 16; ++kk)
+                        tc::umma_pair(taddr + (uint32_t)(acc * BN), da + ka * kk, db + kbs * kk, g.idesc,
+                                      (kb | kk) != 0);
+                    tc::umma_commit_pair(&empty[st]);
+                }
+                if (ok) tc::umma_commit_pair(&acc_full[acc]);
+            }
+        }
+    } else {  // ---- epilogue warps
+        const int q4 = warp & 3, half = (warp - 2) >> 2, w = warp - 2;
+        unsigned char* buf = bufs + w * 2 * GP_BUF;
+        const Epilogue& e = g.e;
+        const int tr_rows = rank * GT_M + q4 * 32;
+        const uint32_t sw = (uint32_t)(lane & 7) << 4, rowoff = (uint32_t)lane * 128;
+        int q = 0, li = 0;  // chunks and tiles so far
+        // with pre, buffer 0 stages pre and buffer 1 the residual and y; else the two alternate
+        auto ybuf = [&](int k) { return e.pre ? 1 : k & 1; };
+        auto fetch_residual = [&](int k, int t, int c) {  // lane 0; the buffer is free
+            tc::mbar_arrive_expect_tx(&res_full[w][ybuf(k)], GP_BUF);
+            tc::tma_load_2d(buf + ybuf(k) * GP_BUF, &tr, &res_full[w][ybuf(k)], t % g.nt * BN + half * (BN / 2) + c * 64,
+                            t / g.nt * 2 * GT_M + tr_rows);
+        };
+        uint32_t res_phase[2] = {0, 0};
+        const int t0 = blockIdx.x >> 1;
+        if (e.residual && t0 < tiles && lane == 0) fetch_residual(0, t0, 0);
+        for (int t = t0; t < tiles; t += pairs, ++li) {
+            const int acc = li & 1;
+            const int n0 = t % g.nt * BN + half * (BN / 2), m0 = t / g.nt * 2 * GT_M + tr_rows;
+            const bool ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&acc_full[acc], (li >> 1) & 1, fail));
+            tc::fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < P::CHUNKS; ++c, ++q) {
+                const int yb = ybuf(q), col = n0 + c * 64;
+                unsigned char* by = buf + yb * GP_BUF;
+                // this chunk's buffers are free, and the next residual is on its way
+                if (lane == 0) {
+                    if (e.pre || e.residual)
+                        tc::bulk_wait_read<0>();
+                    else
+                        tc::bulk_wait_read<1>();
+                    if (e.residual && !e.pre) {
+                        const int c1 = c + 1 < P::CHUNKS ? c + 1 : 0, t1 = c1 ? t : t + pairs;
+                        if (t1 < tiles) fetch_residual(q + 1, t1, c1);
+                    } else if (e.residual && q > 0) {
+                        fetch_residual(q, t, c);
+                    }
+                }
+                __syncwarp();
+                float v[64];
+                const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + half * (BN / 2) + c * 64);
+                tc::tmem_ld_32x32(src, *reinterpret_cast<float(*)[32]>(&v[0]));
+                tc::tmem_ld_32x32(src + 32, *reinterpret_cast<float(*)[32]>(&v[32]));
+                if (c + 1 == P::CHUNKS) {
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
+                }
+                if (!ok) {  // a wait that ran out leaves NaN, not a plausible number
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) v[j] = NAN;
+                }
+                if (e.bias) {
+                    const T* b = static_cast<const T*>(e.bias) + col;
+                    if (col + 64 <= g.n) {
+#pragma unroll
+                        for (int j = 0; j < 64; j += 8) {
+                            const uint4 u = __ldg(reinterpret_cast<const uint4*>(b + j));
+                            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float2 f = unpack2<T>(x[k]);
+                                v[j + 2 * k] += f.x;
+                                v[j + 2 * k + 1] += f.y;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 64; ++j)
+                            if (col + j < g.n) v[j] += to_f32(b[j]);
+                    }
+                }
+                if (e.pre) {
+#pragma unroll
+                    for (int j = 0; j < 64; j += 8)
+                        *reinterpret_cast<uint4*>(buf + rowoff + (((uint32_t)j << 1) ^ sw)) =
+                            make_uint4(pack2<T>(v[j], v[j + 1]), pack2<T>(v[j + 2], v[j + 3]),
+                                       pack2<T>(v[j + 4], v[j + 5]), pack2<T>(v[j + 6], v[j + 7]));
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (m0 < g.m && col < g.n) tc::tma_store_2d(&tp, buf, col, m0);
+                        tc::bulk_commit();
+                    }
+                }
+                if (e.act != FG_ACT_NONE) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) v[j] = activate<true>(v[j], e.act);
+                }
+                if (e.residual) {
+                    tc::mbar_wait_or_fail(&res_full[w][yb], res_phase[yb], fail);
+                    res_phase[yb] ^= 1;
+#pragma unroll
+                    for (int j = 0; j < 64; j += 8) {
+                        const uint4 u = *reinterpret_cast<const uint4*>(by + rowoff + (((uint32_t)j << 1) ^ sw));
+                        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float2 f = unpack2<T>(x[k]);
+                            v[j + 2 * k] += f.x;
+                            v[j + 2 * k + 1] += f.y;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 64; j += 8)
+                    *reinterpret_cast<uint4*>(by + rowoff + (((uint32_t)j << 1) ^ sw)) =
+                        make_uint4(pack2<T>(v[j], v[j + 1]), pack2<T>(v[j + 2], v[j + 3]), pack2<T>(v[j + 4], v[j + 5]),
+                                   pack2<T>(v[j + 6], v[j + 7]));
+                tc::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    if (m0 < g.m && col < g.n) tc::tma_store_2d(&ty, by, col, m0);
+                    tc::bulk_commit();
+                }
+            }
+        }
+        if (lane == 0) tc::bulk_wait_all();
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    cluster_sync();  // no CTA leaves while its peer still reads its memory
+    tc::fence_after_sync();
+    if (warp == 1) tc::tmem_dealloc_pair(taddr, 2 * BN);
 }
 
 // ---- host side ---------------------------------------------------------------
@@ -243,11 +507,11 @@ static int operand_map(CUtensorMap* m, int dtype, const void* p, long long rows,
     return FG_OK;
 }
 
-// Instruction descriptor, kind::f16: f32 accumulators, M = 128.
-static uint32_t instr_desc(int dtype, int n, bool a_mn, bool b_mn) {
+// Instruction descriptor, kind::f16: f32 accumulators.
+static uint32_t instr_desc(int dtype, int m, int n, bool a_mn, bool b_mn) {
     const uint32_t t = dtype == FG_DTYPE_BF16 ? 1 : 0;
     return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(GT_M >> 4) << 24);
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 bool tc_gemm_fits(const void* a, const void* b, const GemmShape& g) {
@@ -262,7 +526,7 @@ static int launch_split(int dtype, const void* a, const void* b, const GemmShape
     int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M);
     if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN);
     if (rc) return rc;
-    g.idesc = instr_desc(dtype, BN, g.a_mn, g.b_mn);
+    g.idesc = instr_desc(dtype, GT_M, BN, g.a_mn, g.b_mn);
     g.nt = (g.n + BN - 1) / BN;
     const long long ctas = (long long)g.mt * g.nt * g.split;
     FG_REQUIRE(ctas <= 0x7fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
@@ -284,6 +548,34 @@ static int launch_split(int dtype, const void* a, const void* b, const GemmShape
     return FG_OK;
 }
 
+// Output or residual [m][n] for TMA: boxes of 32 rows x 64 columns.
+static int tile_map(CUtensorMap* m, int dtype, const void* p, long long rows, long long n, long long ld) {
+    if (!p) return FG_OK;  // the kernel does not touch it
+    return operand_map(m, dtype, p, rows, n, ld, false, 32);
+}
+
+template <class T, int BN>
+static int launch_pair(int dtype, const void* a, const void* b, const GemmShape& s, TcArgs g, cudaStream_t st) {
+    CUtensorMap ta, tb, ty = {}, tp = {}, tr = {};
+    const Epilogue& e = g.e;
+    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M);
+    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN / 2);
+    if (!rc) rc = tile_map(&ty, dtype, e.y, s.m, s.n, e.ldy);
+    if (!rc) rc = tile_map(&tp, dtype, e.pre, s.m, s.n, e.ldp);
+    if (!rc) rc = tile_map(&tr, dtype, e.residual, s.m, s.n, e.ldr);
+    if (rc) return rc;
+    g.idesc = instr_desc(dtype, 2 * GT_M, BN, g.a_mn, g.b_mn);
+    g.mt = (g.m + 2 * GT_M - 1) / (2 * GT_M);
+    g.nt = (g.n + BN - 1) / BN;
+    const long long tiles = (long long)g.mt * g.nt;
+    FG_REQUIRE(tiles <= 0x3fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
+    auto kernel = &gemm_pair_kernel<T, BN>;
+    FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), PairOf<BN>::SMEM));
+    const int pairs = std::max(1, device_attr(cudaDevAttrMultiProcessorCount) / 2);
+    kernel<<<2 * (unsigned)std::min<long long>(tiles, pairs), GT_NT, PairOf<BN>::SMEM, st>>>(ta, tb, ty, tp, tr, g);
+    return check_launch("gemm_pair_kernel");
+}
+
 int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& s, const Epilogue& e, cudaStream_t st) {
     TcArgs g{};
     g.m = (int)s.m;
@@ -293,17 +585,32 @@ int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& s, const E
     g.a_mn = s.ak != 1;
     g.b_mn = s.bk != 1;
     g.e = e;
-    g.vec = aligned(e.y, 8) && e.ldy % 4 == 0 && (!e.bias || aligned(e.bias, 8)) &&
-            (!e.pre || (aligned(e.pre, 8) && e.ldp % 4 == 0)) &&
-            (!e.residual || (aligned(e.residual, 8) && e.ldr % 4 == 0));
-    // The tile width and the split that finish first by this estimate of SM cycles:
-    // a K block's MMAs, the tile's start and end, and the exchange of a split tile.
-    const int sms = std::max(1, device_attr(cudaDevAttrMultiProcessorCount));
+    auto lies = [&](const void* p, long long ld, int bytes) { return !p || (aligned(p, bytes) && ld * 2 % bytes == 0); };
+    g.vec = lies(e.y, e.ldy, 8) && lies(e.bias, 0, 8) && lies(e.pre, e.ldp, 8) && lies(e.residual, e.ldr, 8);
+    const bool tma_out = lies(e.y, e.ldy, 16) && lies(e.bias, 0, 16) && lies(e.pre, e.ldp, 16) && lies(e.residual, e.ldr, 16);
+    // The kernel, tile width and split that finish first by this estimate of SM
+    // cycles: a K block's MMAs (64 x width / 32, or the operands' loads where a
+    // narrow tile waits for them), a tile's epilogue -- behind the next tile's
+    // MMAs in the pair kernel --, start and end, and the exchange of a split tile.
+    const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
     int best_n = 256;
+    bool pair = false;
     double best = 1e300;
+    for (int bn : {256, 128}) {
+        if (!tma_out) break;
+        const long long tiles = (s.m + 2 * GT_M - 1) / (2 * GT_M) * ((g.n + bn - 1) / bn);
+        const double waves = (double)((tiles + sms / 2 - 1) / (sms / 2));
+        const double epi = 16.0 * bn, main = g.kt * (bn == 256 ? 530.0 : 290.0);
+        const double cost = waves * std::max(main, epi) + std::min(main, epi) + 4000;
+        if (cost < best) {
+            best = cost;
+            best_n = bn;
+            pair = true;
+        }
+    }
     for (int bn : {256, 128, 64}) {
         const long long tiles = (long long)g.mt * ((g.n + bn - 1) / bn);
-        const double block = bn == 256 ? 520 : bn == 128 ? 280 : 200;
+        const double block = bn == 256 ? 560 : bn == 128 ? 320 : 220;
         for (int sp : {1, 2, 4, 8}) {
             if (sp > g.kt) break;
             const double waves = (double)((tiles * sp + sms - 1) / sms);
@@ -311,16 +618,19 @@ int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& s, const E
             if (cost < best) {
                 best = cost;
                 best_n = bn;
+                pair = false;
                 g.split = sp;
             }
         }
     }
-#define FG_SPLIT(T)                                                       \
-    (best_n == 256   ? launch_split<T, 256>(dtype, a, b, s, g, st)        \
-     : best_n == 128 ? launch_split<T, 128>(dtype, a, b, s, g, st)        \
-                     : launch_split<T, 64>(dtype, a, b, s, g, st))
-    return dtype == FG_DTYPE_F16 ? FG_SPLIT(__half) : FG_SPLIT(__nv_bfloat16);
-#undef FG_SPLIT
+#define FG_PRODUCT(T)                                                                       \
+    (pair ? (best_n == 256 ? launch_pair<T, 256>(dtype, a, b, s, g, st)                     \
+                           : launch_pair<T, 128>(dtype, a, b, s, g, st))                    \
+          : (best_n == 256   ? launch_split<T, 256>(dtype, a, b, s, g, st)                  \
+             : best_n == 128 ? launch_split<T, 128>(dtype, a, b, s, g, st)                  \
+                             : launch_split<T, 64>(dtype, a, b, s, g, st)))
+    return dtype == FG_DTYPE_F16 ? FG_PRODUCT(__half) : FG_PRODUCT(__nv_bfloat16);
+#undef FG_PRODUCT
 }
 
 }  // namespace fg

@@ -277,6 +277,27 @@ def test_linear_backward(ad, shape, act, t):
     assert ad.linear_backward(dy, x, w, pre=pre, activation=act, input_grad=False)[0] is None
 
 
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("shape", [(40000, 64, 128), (20000, 136, 264), (9000, 520, 1000), (30001, 72, 72),
+                                   (2500, 40, 8200), (19000, 200, 100)])
+@pytest.mark.parametrize("extras", ["", "bias", "pre", "residual", "bias pre residual"])
+def test_linear_many_rows(ad, shape, t, extras):
+    """Sizes of many tiles, with every combination the epilogue treats apart."""
+    n, i, o = shape
+    g = _gen(n)
+    x, w = _randn(g, n, i, t=t), _randn(g, o, i, t=t, scale=i ** -0.5)
+    b = _randn(g, o, t=t) if "bias" in extras else None
+    res = _randn(g, n, o, t=t) if "residual" in extras else None
+    if "pre" in extras:
+        _check_linear(ad, x, w, b, res, "gelu", t)
+        _check_backward(ad, res if res is not None else _randn(g, n, o, t=t), x, w, _randn(g, n, o, t=t), "silu", t)
+        return
+    y = ad.linear(x, w, b, activation="silu", residual=res)
+    ry, rz, mag = _linear_ref(x, w, b, res, "silu")
+    _within(y, ry, 1.2 * (i + 8) * 2 * E32 * mag + ACT[t] * rz.abs().clamp(min=1) + 8 * E32 * (ry.abs() + rz.abs())
+            + U[t] * ry.abs() + TINY[t], "y")
+
+
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("lead", [0, 1, 4, 8])
 def test_linear_strides_and_alignment(ad, t, lead):
@@ -309,6 +330,28 @@ def test_linear_nonfinite_stays_in_its_rows(ad, t, n):
     y = ad.linear(x, w)
     want = torch.where(w[:, 3] > 0, math.inf, -math.inf).to(y.dtype)
     assert torch.equal(y[n // 2], want) and y[keep].isfinite().all()
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_activations_at_their_ends(ad, t):
+    """w = 1: the activations at chosen points, their limits at infinity, NaN."""
+    z = torch.tensor([0.0, -0.0, 1e-3, -1e-3, 3.0, -3.0, 5.5, -5.5, 9.0, -9.0, 40.0, -40.0, 95.0, -95.0, 3e4, -3e4,
+                      math.inf, -math.inf, math.nan], device="cuda", dtype=T[t])[:, None]
+    one = torch.ones(1, 1, device="cuda", dtype=T[t])
+    zd = z.double()
+    for act, at_inf in (("none", (math.inf, -math.inf)), ("relu", (math.inf, 0)), ("gelu", (math.inf, 0)),
+                        ("silu", (math.inf, 0))):
+        y = ad.linear(z, one, activation=act)[:, 0].double()
+        want = _act(zd, act)[:, 0]
+        tol = (ACT[t] if act in ("gelu", "silu") else 0) * zd[:, 0].abs().clamp(min=1) + U[t] * want.abs() + TINY[t]
+        _within(y[:16], want[:16], tol[:16], act)
+        assert (y[16], y[17]) == at_inf and y[18].isnan()
+        d = ad.linear_backward(torch.ones_like(z), z, one, pre=z, activation=act, param_grads=False)[0][:, 0].double()
+        want = _act_grad(zd, act)[:, 0]
+        _within(d[:16], want[:16], ACT[t] * 2 + 3 * U[t] * want[:16].abs() + TINY[t], act + "'")
+        assert d[16] == 1 and d[17] == (act == "none")
+        if act in ("gelu", "silu"):
+            assert d[18].isnan()
 
 
 def test_linear_overflow_and_empty(ad):

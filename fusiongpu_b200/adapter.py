@@ -13,13 +13,15 @@ and the gradients) are the package's own sm_100a kernels behind the C ABI
 (fg_layer_norm, fg_linear, fg_preference_loss in ``include/fusiongpu.h``).
 Tensors are CUDA tensors of float32, float16 or bfloat16; the documents may be
 uint8.  Rows may be strided; a tensor whose last dimension is not contiguous
-is copied.  Every call runs on ``stream`` (default: the current stream), does
-not synchronise, and allocates its results and workspace there.
+is copied.  Every call takes ``stream=`` (default: the current stream of its
+first tensor's device), runs and allocates its results and workspace there, and
+does not synchronise.
 """
 from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -32,8 +34,9 @@ BASE_DTYPES = {**DTYPES, torch.uint8: 3}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 
 
-def _matrix(t: torch.Tensor, name: str, like: torch.Tensor | None = None, shape=None) -> torch.Tensor:
-    """A CUDA matrix with unit column stride, checked against `like`'s type and device."""
+def _matrix(t: torch.Tensor, name: str, like: torch.Tensor | None = None, rows: int = -1, cols: int = -1):
+    """(a CUDA matrix with unit column stride, its row stride), checked against
+    `like`'s type and device and the shape where given."""
     if not t.is_cuda or t.dim() != 2:
         raise ValueError(f"{name} must be a 2-D CUDA tensor")
     if like is None:
@@ -41,89 +44,117 @@ def _matrix(t: torch.Tensor, name: str, like: torch.Tensor | None = None, shape=
             raise TypeError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
     elif t.dtype != like.dtype or t.device != like.device:
         raise TypeError(f"{name} must be {like.dtype} on {like.device}, not {t.dtype} on {t.device}")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
-    rows, cols = t.shape
+    n, d = t.shape
+    if (rows >= 0 and n != rows) or (cols >= 0 and d != cols):
+        raise ValueError(f"{name} has shape {(n, d)}, not {(rows if rows >= 0 else n, cols if cols >= 0 else d)}")
     s0, s1 = t.stride()
-    if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1):
+    if (s1 != 1 and d > 1) or (s0 < d and n > 1):
         t = t.contiguous()
-    return t
+        s0 = d
+    return t, s0 if n > 1 else 0
 
 
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else 0
-
-
-def _vector(t: torch.Tensor | None, name: str, n: int, dtypes, device) -> int | None:
+def _vector(t: torch.Tensor | None, name: str, n: int, dtype, device) -> int | None:
     if t is None:
         return None
-    if t.dtype not in dtypes or t.device != device:
-        raise TypeError(f"{name} must be one of {dtypes} on {device}, not {t.dtype} on {t.device}")
-    if t.shape != (n,) or not t.is_contiguous():
+    if t.dtype != dtype or t.device != device:
+        raise TypeError(f"{name} must be {dtype} on {device}, not {t.dtype} on {t.device}")
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous vector of {n}")
     return t.data_ptr()
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 @contextlib.contextmanager
 def _entered(device, stream):
     with torch.cuda.device(device), torch.cuda.stream(stream):
-        yield stream.cuda_stream
+        yield
 
 
-def _on(t: torch.Tensor, stream):
-    """The stream to launch on, current while results are allocated."""
-    if stream is None and t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext(torch.cuda.current_stream().cuda_stream)
-    return _entered(t.device, stream if stream is not None else torch.cuda.current_stream(t.device))
+def _on(fn):
+    """Runs the function with its `stream` argument and its first tensor's device
+    current, so that results and workspace are allocated for that stream; they
+    already are in the usual call."""
+    @functools.wraps(fn)
+    def call(x, *args, stream: torch.cuda.Stream | None = None, **kw):
+        if stream is None and x.is_cuda and x.device.index == torch.cuda.current_device():
+            return fn(x, *args, **kw)
+        if not x.is_cuda:
+            raise ValueError("CUDA tensors are needed")
+        with _entered(x.device, stream if stream is not None else torch.cuda.current_stream(x.device)):
+            return fn(x, *args, **kw)
+    return call
 
 
+# the current stream's handle; torch.cuda.current_stream() builds an object around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(x: torch.Tensor) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(x.device.index)
+    return torch.cuda.current_stream(x.device).cuda_stream
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_ws(n: int, d: int, device: int) -> int:
+    return _lib.size_query("fg_layer_norm_backward_workspace_size", n, d)
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_ws(query: str, n: int, i: int, o: int, dtype: int, act: int, device: int) -> int:
+    return _lib.size_query(query, C.byref(_lib.LinearParams(n, i, o, dtype, act, 0, 0, 0, 0, 0)))
+
+
+@_on
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
-               eps: float = 1e-5, return_stats: bool = False, stream: torch.cuda.Stream | None = None):
+               eps: float = 1e-5, return_stats: bool = False):
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension
     of x [rows][dim]; weight and bias of x's type or both float32.  With
     return_stats also the rows' mean and 1 / sqrt(variance + eps), which
     :func:`layer_norm_backward` takes."""
-    x = _matrix(x, "x")
+    x, ld = _matrix(x, "x")
     n, d = x.shape
+    t, dev = x.dtype, x.device
     p = weight if weight is not None else bias
-    pd = x.dtype if p is None else p.dtype
-    allowed = (pd,) if pd in (x.dtype, torch.float32) else (x.dtype, torch.float32)
-    w, b = _vector(weight, "weight", d, allowed, x.device), _vector(bias, "bias", d, allowed, x.device)
-    with _on(x, stream) as s:
-        y = torch.empty((n, d), dtype=x.dtype, device=x.device)
-        mean = rstd = None
-        if return_stats:
-            mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device).unbind(0)
-        _lib.call("fg_layer_norm", x.data_ptr(), DTYPES[x.dtype], n, d, _ld(x), w, b, DTYPES[pd], eps, y.data_ptr(),
-                  0, None if mean is None else mean.data_ptr(), None if rstd is None else rstd.data_ptr(), s)
+    pd = torch.float32 if p is not None and p.dtype == torch.float32 else t
+    w, b = _vector(weight, "weight", d, pd, dev), _vector(bias, "bias", d, pd, dev)
+    y = x.new_empty((n, d))
+    mean = rstd = None
+    if return_stats:
+        mean, rstd = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
+    _lib.check(_lib.lib().fg_layer_norm(x.data_ptr(), DTYPES[t], n, d, ld, w, b, DTYPES[pd], eps, y.data_ptr(), 0,
+                                        _ptr(mean), _ptr(rstd), _stream(x)), "fg_layer_norm")
     return (y, mean, rstd) if return_stats else y
 
 
+@_on
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
-                        weight: torch.Tensor | None = None, param_grads: bool = True,
-                        stream: torch.cuda.Stream | None = None):
+                        weight: torch.Tensor | None = None, param_grads: bool = True):
     """Gradients (dx, dweight, dbias) of :func:`layer_norm`; the parameters'
     are of weight's type (x's without one), None when param_grads is false."""
-    x = _matrix(x, "x")
-    dy = _matrix(dy, "dy", x, x.shape)
+    x, ld = _matrix(x, "x")
     n, d = x.shape
-    m, r = (_vector(t, k, n, (torch.float32,), x.device) for t, k in ((mean, "mean"), (rstd, "rstd")))
-    if m is None or r is None:
+    t, dev = x.dtype, x.device
+    dy, lddy = _matrix(dy, "dy", x, n, d)
+    if mean is None or rstd is None:
         raise ValueError("mean and rstd of the forward pass are needed")
-    w = _vector(weight, "weight", d, (x.dtype, torch.float32), x.device)
-    pd = x.dtype if weight is None else weight.dtype
-    with _on(x, stream) as s:
-        dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
-        dw = db = ws = None
-        if param_grads:
-            dw = torch.empty(d, dtype=pd, device=x.device)
-            db = torch.empty(d, dtype=pd, device=x.device)
-            ws = torch.empty(_lib.size_query("fg_layer_norm_backward_workspace_size", n, d), dtype=torch.uint8,
-                             device=x.device)
-        _lib.call("fg_layer_norm_backward", dy.data_ptr(), _ld(dy), x.data_ptr(), DTYPES[x.dtype], n, d, _ld(x), w,
-                  DTYPES[pd], m, r, dx.data_ptr(), 0, None if dw is None else dw.data_ptr(),
-                  None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
-                  0 if ws is None else ws.numel(), s)
+    m, r = _vector(mean, "mean", n, torch.float32, dev), _vector(rstd, "rstd", n, torch.float32, dev)
+    pd = torch.float32 if weight is not None and weight.dtype == torch.float32 else t
+    w = _vector(weight, "weight", d, pd, dev)
+    dx = x.new_empty((n, d))
+    dw = db = ws = None
+    nws = 0
+    if param_grads:
+        dw, db = torch.empty(d, dtype=pd, device=dev), torch.empty(d, dtype=pd, device=dev)
+        nws = _norm_ws(n, d, dev.index)
+        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
+    _lib.check(_lib.lib().fg_layer_norm_backward(dy.data_ptr(), lddy, x.data_ptr(), DTYPES[t], n, d, ld, w, DTYPES[pd],
+                                                 m, r, dx.data_ptr(), 0, _ptr(dw), _ptr(db), _ptr(ws), nws,
+                                                 _stream(x)), "fg_layer_norm_backward")
     return dx, dw, db
 
 
@@ -133,77 +164,67 @@ def _activation(name: str) -> int:
     return ACTIVATIONS[name]
 
 
-def _workspace(query: str, p, device) -> torch.Tensor | None:
-    n = _lib.size_query(query, C.byref(p))
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
-
-
+@_on
 def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
-           residual: torch.Tensor | None = None, return_pre: bool = False,
-           stream: torch.cuda.Stream | None = None):
+           residual: torch.Tensor | None = None, return_pre: bool = False):
     """activation(x w^T + bias) + residual for x [rows][in], w [out][in]; with
     return_pre also x w^T + bias, which :func:`linear_backward` takes.
     activation: "none", "relu", "gelu" (erf) or "silu"."""
     act = _activation(activation)
-    x = _matrix(x, "x")
+    x, ldx = _matrix(x, "x")
     n, i = x.shape
-    w = _matrix(w, "w", x)
+    w, ldw = _matrix(w, "w", x, -1, i)
     o = w.shape[0]
-    if w.shape[1] != i:
-        raise ValueError(f"w has {w.shape[1]} columns, x {i}")
-    b = _vector(bias, "bias", o, (x.dtype,), x.device)
+    t, dev = DTYPES[x.dtype], x.device
+    b = _vector(bias, "bias", o, x.dtype, dev)
+    ldr = 0
     if residual is not None:
-        residual = _matrix(residual, "residual", x, (n, o))
-    with _on(x, stream) as s:
-        y = torch.empty((n, o), dtype=x.dtype, device=x.device)
-        pre = torch.empty((n, o), dtype=x.dtype, device=x.device) if return_pre else None
-        p = _lib.LinearParams(n, i, o, DTYPES[x.dtype], act, _ld(x), _ld(w),
-                              0 if residual is None else _ld(residual), 0, 0)
-        ws = _workspace("fg_linear_workspace_size", p, x.device)
-        _lib.call("fg_linear", C.byref(p), x.data_ptr(), w.data_ptr(), b,
-                  None if residual is None else residual.data_ptr(), None if pre is None else pre.data_ptr(),
-                  y.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), s)
+        residual, ldr = _matrix(residual, "residual", x, n, o)
+    y = x.new_empty((n, o))
+    pre = x.new_empty((n, o)) if return_pre else None
+    p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, ldr, 0, 0)
+    nws = _linear_ws("fg_linear_workspace_size", n, i, o, t, act, dev.index)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    _lib.check(_lib.lib().fg_linear(C.byref(p), x.data_ptr(), w.data_ptr(), b, _ptr(residual), _ptr(pre),
+                                    y.data_ptr(), _ptr(ws), nws, _stream(x)), "fg_linear")
     return (y, pre) if return_pre else y
 
 
+@_on
 def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: torch.Tensor | None = None,
-                    activation: str = "none", input_grad: bool = True, param_grads: bool = True,
-                    stream: torch.cuda.Stream | None = None):
+                    activation: str = "none", input_grad: bool = True, param_grads: bool = True):
     """Gradients (dx, dw, dbias) of :func:`linear`, of x's type; `pre` from the
     forward pass unless the activation is "none".  The residual's gradient is
     dy.  What input_grad and param_grads leave out is None."""
     act = _activation(activation)
-    x = _matrix(x, "x")
+    x, ldx = _matrix(x, "x")
     n, i = x.shape
-    w = _matrix(w, "w", x)
+    w, ldw = _matrix(w, "w", x, -1, i)
     o = w.shape[0]
-    if w.shape[1] != i:
-        raise ValueError(f"w has {w.shape[1]} columns, x {i}")
-    dy = _matrix(dy, "dy", x, (n, o))
-    if act:
-        if pre is None:
-            raise ValueError("the activation's gradient needs pre")
-        pre = _matrix(pre, "pre", x, (n, o))
-    else:
+    t, dev = DTYPES[x.dtype], x.device
+    dy, lddy = _matrix(dy, "dy", x, n, o)
+    ldp = 0
+    if not act:
         pre = None
-    with _on(x, stream) as s:
-        dx = torch.empty((n, i), dtype=x.dtype, device=x.device) if input_grad else None
-        dw = torch.empty((o, i), dtype=x.dtype, device=x.device) if param_grads else None
-        db = torch.empty(o, dtype=x.dtype, device=x.device) if param_grads else None
-        p = _lib.LinearParams(n, i, o, DTYPES[x.dtype], act, _ld(x), _ld(w), 0, 0 if pre is None else _ld(pre),
-                              _ld(dy))
-        ws = _workspace("fg_linear_backward_workspace_size", p, x.device)
-        _lib.call("fg_linear_backward", C.byref(p), dy.data_ptr(), x.data_ptr(), w.data_ptr(),
-                  None if pre is None else pre.data_ptr(), None if dx is None else dx.data_ptr(),
-                  None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
-                  None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), s)
+    elif pre is None:
+        raise ValueError("the activation's gradient needs pre")
+    else:
+        pre, ldp = _matrix(pre, "pre", x, n, o)
+    dx = x.new_empty((n, i)) if input_grad else None
+    dw, db = (x.new_empty((o, i)), x.new_empty(o)) if param_grads else (None, None)
+    p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, 0, ldp, lddy)
+    nws = _linear_ws("fg_linear_backward_workspace_size", n, i, o, t, act, dev.index)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    _lib.check(_lib.lib().fg_linear_backward(C.byref(p), dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(pre),
+                                             _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nws, _stream(x)),
+               "fg_linear_backward")
     return dx, dw, db
 
 
+@_on
 def preference_loss(queries: torch.Tensor, base: torch.Tensor, offsets: torch.Tensor, pos_ids: torch.Tensor,
                     neg_ids: torch.Tensor, ref: torch.Tensor | None = None, weights: torch.Tensor | None = None,
-                    beta: float = 1.0, label_smoothing: float = 0.0, metric: str = "ip", grad: bool = True,
-                    stream: torch.cuda.Stream | None = None):
+                    beta: float = 1.0, label_smoothing: float = 0.0, metric: str = "ip", grad: bool = True):
     """Paired preference loss of queries [nq][dim] over the documents base
     [nbase][dim] (float32, float16, bfloat16 or uint8): query i prefers document
     pos_ids[p] to neg_ids[p] for its pairs p in [offsets[i], offsets[i+1])
@@ -211,29 +232,29 @@ def preference_loss(queries: torch.Tensor, base: torch.Tensor, offsets: torch.Te
     masked).  `ref`: the reference queries the log ratios are taken against
     (the unadapted ones).  Returns (losses [pairs], margins [pairs], dq), dq the
     gradient of sum(weights * losses), or None when grad is false."""
-    q = _matrix(queries, "queries")
+    q, ldq = _matrix(queries, "queries")
     nq, d = q.shape
+    dev = q.device
+    ldr = 0
     if ref is not None:
-        ref = _matrix(ref, "ref", q, q.shape)
+        ref, ldr = _matrix(ref, "ref", q, nq, d)
     if metric not in METRICS:
         raise ValueError(f"metric must be one of {sorted(METRICS)}, not {metric!r}")
-    if base.dtype not in BASE_DTYPES or base.device != q.device:
-        raise TypeError(f"base must be one of {list(BASE_DTYPES)} on {q.device}")
+    if base.dtype not in BASE_DTYPES or base.device != dev:
+        raise TypeError(f"base must be one of {list(BASE_DTYPES)} on {dev}")
     if base.dim() != 2 or base.shape[1] != d or not base.is_contiguous():
         raise ValueError(f"base must be contiguous [nbase][{d}]")
     m = pos_ids.numel()
-    po = _vector(pos_ids, "pos_ids", m, (torch.int32,), q.device)
-    ne = _vector(neg_ids, "neg_ids", m, (torch.int32,), q.device)
-    off = _vector(offsets, "offsets", nq + 1, (torch.int64,), q.device)
-    wt = _vector(weights, "weights", m, (torch.float32,), q.device)
-    with _on(q, stream) as s:
-        losses, margins = torch.empty((2, m), dtype=torch.float32, device=q.device).unbind(0)
-        dq = torch.empty((nq, d), dtype=q.dtype, device=q.device) if grad else None
-        p = _lib.PreferenceParams(nq, d, DTYPES[q.dtype], BASE_DTYPES[base.dtype], base.shape[0], m, METRICS[metric],
-                                  beta, label_smoothing, _ld(q), 0 if ref is None else _ld(ref), 0)
-        _lib.call("fg_preference_loss", C.byref(p), q.data_ptr(), None if ref is None else ref.data_ptr(),
-                  base.data_ptr(), off, po, ne, wt, losses.data_ptr(), margins.data_ptr(),
-                  None if dq is None else dq.data_ptr(), s)
+    po, ne = _vector(pos_ids, "pos_ids", m, torch.int32, dev), _vector(neg_ids, "neg_ids", m, torch.int32, dev)
+    off = _vector(offsets, "offsets", nq + 1, torch.int64, dev)
+    wt = _vector(weights, "weights", m, torch.float32, dev)
+    losses, margins = torch.empty(m, dtype=torch.float32, device=dev), torch.empty(m, dtype=torch.float32, device=dev)
+    dq = q.new_empty((nq, d)) if grad else None
+    p = _lib.PreferenceParams(nq, d, DTYPES[q.dtype], BASE_DTYPES[base.dtype], base.shape[0], m, METRICS[metric], beta,
+                              label_smoothing, ldq, ldr, 0)
+    _lib.check(_lib.lib().fg_preference_loss(C.byref(p), q.data_ptr(), _ptr(ref), base.data_ptr(), off, po, ne, wt,
+                                             losses.data_ptr(), margins.data_ptr(), _ptr(dq), _stream(q)),
+               "fg_preference_loss")
     return losses, margins, dq
 
 

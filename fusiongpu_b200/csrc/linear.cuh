@@ -35,6 +35,55 @@ __device__ __forceinline__ float upper_tail(float z, float& e) {  // Phi(-|z|)
     return p * t * e;
 }
 
+// Two floats in one register pair: fma.rn.f32x2 issues once for both.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t p, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// GELU of two values for results of 16 bits: max(z, 0) - a Phi(-a), a = min(|z|, 30)
+// (Phi(-30) is 0 in float32), the formula of upper_tail in 9 issues a value.
+__device__ __forceinline__ void gelu2(float& z0, float& z1) {
+    const float a0 = fminf(fabsf(z0), 30.0f), a1 = fminf(fabsf(z1), 30.0f);
+    const uint64_t a = pair2(a0, a1);
+    float d0, d1, m0, m1;
+    unpair2(fma2(a, pair2(0.3275911f * 0.70710678f, 0.3275911f * 0.70710678f), pair2(1.0f, 1.0f)), d0, d1);
+    unpair2(mul2(mul2(a, a), pair2(-0.5f * 1.44269504f, -0.5f * 1.44269504f)), m0, m1);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d0));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d1));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(m0));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(m1));
+    const uint64_t t = pair2(d0, d1);
+    uint64_t p = fma2(t, pair2(-0.5f * 1.061405429f, -0.5f * 1.061405429f), pair2(0.5f * 1.453152027f, 0.5f * 1.453152027f));
+    p = fma2(t, p, pair2(-0.5f * 1.421413741f, -0.5f * 1.421413741f));
+    p = fma2(t, p, pair2(0.5f * 0.284496736f, 0.5f * 0.284496736f));
+    p = fma2(t, p, pair2(-0.5f * 0.254829592f, -0.5f * 0.254829592f));
+    p = mul2(mul2(p, t), pair2(m0, m1));
+    float r0, r1;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r0) : "f"(z0));
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r1) : "f"(z1));
+    unpair2(fma2(a, p, pair2(r0, r1)), z0, z1);
+}
+
 template <bool FAST>
 __device__ __forceinline__ float sigmoid(float z) {  // z >= -100
     // below -87 the quotient's divisor would pass 2^126, where __fdividef is 0
@@ -48,9 +97,9 @@ __device__ __forceinline__ float activate(float z, int act) {
         case FG_ACT_RELU: return z > 0.0f ? z : (z == z ? 0.0f : z);
         case FG_ACT_GELU: {
             if (!FAST) return fmaxf(z, -100.0f) * (0.5f * erfcf(z * -0.70710678f));
-            float e;
-            const float q = upper_tail(z, e);
-            return fmaf(-fminf(fabsf(z), 100.0f), q, fmaxf(z, 0.0f));
+            float other = z;
+            gelu2(z, other);
+            return z;
         }
         case FG_ACT_SILU:
             z = z < -100.0f ? -100.0f : z;  // a NaN stays

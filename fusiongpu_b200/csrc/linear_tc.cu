@@ -67,6 +67,29 @@ __device__ __forceinline__ void store4(T* p, float4 f) {
     *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
 }
 
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+}
+
 // One tile of 128 x BN per cluster, its K blocks divided over the cluster's
 // CTAs.  Each CTA's partial tile goes from TMEM to its shared memory (where the
 // operand ring was); then each CTA adds one slice of the columns over the
@@ -178,47 +201,70 @@ __global__ void __launch_bounds__(GT_NT, 1)
         tc::tmem_dealloc(taddr, BN);
     }
 
+    // Four positions per thread and round, their residuals loaded first: one
+    // memory latency a round.
+    constexpr int U = 4;
     const int slice = BN / S, per_row = slice / 4;
     const uint32_t pbase = tc::smem_u32(part);
-    for (int i = tid; i < GT_M * per_row; i += GT_NT) {
-        const int r = i / per_row, c = rank * slice + (i - r * per_row) * 4;
-        const int row = m0 + r, col = n0 + c;
-        if (row >= g.m || col >= g.n) continue;
-        const uint32_t at = pbase + (uint32_t)(r * LDP + c) * 4;
-        float4 z = *reinterpret_cast<const float4*>(part + r * LDP + c);
-        if (S > 1) {
-            z = ld_cluster_f4(at, 0);
-            for (int s = 1; s < S; ++s) {
-                const float4 v = ld_cluster_f4(at, s);
-                z.x += v.x;
-                z.y += v.y;
-                z.z += v.z;
-                z.w += v.w;
-            }
+    const Epilogue& e = g.e;
+    for (int i0 = tid; i0 < GT_M * per_row; i0 += U * GT_NT) {
+        int row[U], col[U];
+        uint32_t at[U];
+        uint2 res[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * GT_NT, r = i / per_row, c = rank * slice + (i - r * per_row) * 4;
+            row[u] = i < GT_M * per_row ? m0 + r : g.m;
+            col[u] = n0 + c;
+            at[u] = (uint32_t)(r * LDP + c) * 4;
+            if (e.residual && g.vec && row[u] < g.m && col[u] + 4 <= g.n)
+                res[u] = *reinterpret_cast<const uint2*>(static_cast<const T*>(e.residual) + row[u] * e.ldr + col[u]);
         }
-        if (g.vec && col + 4 <= g.n) {
-            const Epilogue& e = g.e;
-            if (e.bias) {
-                const float4 b = load4(static_cast<const T*>(e.bias) + col);
-                z.x += b.x;
-                z.y += b.y;
-                z.z += b.z;
-                z.w += b.w;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (row[u] >= g.m || col[u] >= g.n) continue;
+            float4 z;
+            if (S > 1) {
+                z = ld_cluster_f4(pbase + at[u], 0);
+                for (int s = 1; s < S; ++s) {
+                    const float4 v = ld_cluster_f4(pbase + at[u], s);
+                    z.x += v.x;
+                    z.y += v.y;
+                    z.z += v.z;
+                    z.w += v.w;
+                }
+            } else {
+                z = *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(part) + at[u]);
             }
-            if (e.pre) store4(static_cast<T*>(e.pre) + row * e.ldp + col, z);
-            float4 y = make_float4(activate<true>(z.x, e.act), activate<true>(z.y, e.act), activate<true>(z.z, e.act),
-                                   activate<true>(z.w, e.act));
-            if (e.residual) {
-                const float4 b = load4(static_cast<const T*>(e.residual) + row * e.ldr + col);
-                y.x += b.x;
-                y.y += b.y;
-                y.z += b.z;
-                y.w += b.w;
+            if (g.vec && col[u] + 4 <= g.n) {
+                if (e.bias) {
+                    const float4 b = load4(static_cast<const T*>(e.bias) + col[u]);
+                    z.x += b.x;
+                    z.y += b.y;
+                    z.z += b.z;
+                    z.w += b.w;
+                }
+                if (e.pre) store4(static_cast<T*>(e.pre) + row[u] * e.ldp + col[u], z);
+                float4 y = z;
+                if (e.act == FG_ACT_GELU) {
+                    gelu2(y.x, y.y);
+                    gelu2(y.z, y.w);
+                } else if (e.act != FG_ACT_NONE) {
+                    y = make_float4(activate<true>(z.x, e.act), activate<true>(z.y, e.act),
+                                    activate<true>(z.z, e.act), activate<true>(z.w, e.act));
+                }
+                if (e.residual) {
+                    const float2 lo = unpack2<T>(res[u].x), hi = unpack2<T>(res[u].y);
+                    y.x += lo.x;
+                    y.y += lo.y;
+                    y.z += hi.x;
+                    y.w += hi.y;
+                }
+                store4(static_cast<T*>(e.y) + row[u] * e.ldy + col[u], y);
+            } else {
+                const float v[4] = {z.x, z.y, z.z, z.w};
+                for (int j = 0; j < 4 && col[u] + j < g.n; ++j) epilogue_store<T>(e, row[u], col[u] + j, v[j]);
             }
-            store4(static_cast<T*>(e.y) + row * e.ldy + col, y);
-        } else {
-            const float v[4] = {z.x, z.y, z.z, z.w};
-            for (int j = 0; j < 4 && col + j < g.n; ++j) epilogue_store<T>(g.e, row, col + j, v[j]);
         }
     }
     if (S > 1) cluster_sync();  // a peer may still read this CTA's partial tile
@@ -231,51 +277,75 @@ __global__ void __launch_bounds__(GT_NT, 1)
 // 128 rows, so a K block brings 32 KB into each CTA instead of the 48 KB that a
 // 128 x 256 tile of its own would need.  TMEM holds two accumulators, and the
 // epilogue of a tile runs while the next one is multiplied: a warp takes its 32
-// rows in chunks of 64 columns through a 4 KB buffer that TMA fills with the
-// residual and stores from (whole 128-byte rows, clipped at the matrix's edge).
+// rows x 64 columns through a 4 KB buffer that TMA fills with the residual and
+// stores from (whole 128-byte rows, clipped at the matrix's edge).  16 epilogue
+// warps hide the chain TMEM load, residual, fence, store of each: 8 warps of two
+// chunks took 10,200 cycles for a tile of 6,144 cycles of products (width 768).
 constexpr int GP_STAGES = 5;
 constexpr int GP_A = GT_M * GT_K * 2;
 constexpr int GP_BUF = 4096;   // 32 rows x 128 bytes, 128-byte swizzle
-constexpr int GP_EPI = 8;      // epilogue warps: 4 lane quarters x 2 column halves
+constexpr int GP_EPI = 16;     // epilogue warps, each 32 rows x 64 columns of a tile
+constexpr int GP_NT = 64 + GP_EPI * 32;
 
 template <int BN>
 struct PairOf {
     static constexpr int B = BN / 2 * GT_K * 2, STAGE = GP_A + B;
-    static constexpr int SMEM = GP_STAGES * STAGE + GP_EPI * 2 * GP_BUF + 1024;
-    static constexpr int CHUNKS = BN / 2 / 64;  // per epilogue warp and tile
+    static constexpr int SMEM = GP_STAGES * STAGE + GP_EPI * GP_BUF + 1024;
+    static constexpr int WARPS = BN / 64 * 4;         // epilogue warps of a tile
+    static constexpr int GROUPS = GP_EPI / WARPS;     // that take tiles in turn
 };
 
 template <class T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
+__device__ __forceinline__ uint4 pack8(const float* v) {
+    return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
+
 template <class T>
-__device__ __forceinline__ float2 unpack2(uint32_t u);
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+__device__ __forceinline__ void add8(float* v, uint4 u) {
+    const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack2<T>(x[k]);
+        unpair2(add2(pair2(v[2 * k], v[2 * k + 1]), pair2(f.x, f.y)), v[2 * k], v[2 * k + 1]);
+    }
 }
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
+
+template <int ACT>
+__device__ __forceinline__ void activate_all(float (&v)[2][32]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            if (ACT == FG_ACT_GELU) {
+                gelu2(v[h][j], v[h][j + 1]);
+            } else {
+                v[h][j] = activate<true>(v[h][j], ACT);
+                v[h][j + 1] = activate<true>(v[h][j + 1], ACT);
+            }
+        }
+}
+
+// 32 columns of the bias, the same for every lane; `left` of them exist.
+template <class T>
+__device__ __forceinline__ void add_bias(float (&v)[32], const T* b, int left) {
+    if (left >= 32) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) add8<T>(&v[j], __ldg(reinterpret_cast<const uint4*>(b + j)));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < left) v[j] += to_f32(b[j]);
+    }
 }
 
 template <class T, int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_NT, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                      const __grid_constant__ CUtensorMap ty, const __grid_constant__ CUtensorMap tp,
                      const __grid_constant__ CUtensorMap tr, const TcArgs g) {
     using P = PairOf<BN>;
     extern __shared__ __align__(1024) unsigned char dsmem[];
-    __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], acc_full[2], acc_empty[2], res_full[GP_EPI][2];
+    __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], acc_full[2], acc_empty[2], res_full[GP_EPI];
     __shared__ uint32_t tmem_slot;
     __shared__ int s_fail;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -293,9 +363,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_NT, 1)
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&acc_full[i], 1);
-            tc::mbar_init(&acc_empty[i], 2 * GP_EPI);
-            for (int w = 0; w < GP_EPI; ++w) tc::mbar_init(&res_full[w][i], 1);
+            tc::mbar_init(&acc_empty[i], 2 * P::WARPS);
         }
+        for (int w = 0; w < GP_EPI; ++w) tc::mbar_init(&res_full[w], 1);
         tc::fence_mbar_init();
     }
     if (warp == 1) tc::tmem_alloc_pair(&tmem_slot, 2 * BN);
@@ -362,124 +432,96 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_NT, 1)
             }
         }
     } else {  // ---- epilogue warps
-        const int q4 = warp & 3, half = (warp - 2) >> 2, w = warp - 2;
-        unsigned char* buf = bufs + w * 2 * GP_BUF;
+        const int w = warp - 2, q4 = warp & 3, part = w / 4 % (BN / 64), group = w / P::WARPS;
+        unsigned char* buf = bufs + w * GP_BUF;
         const Epilogue& e = g.e;
         const int tr_rows = rank * GT_M + q4 * 32;
-        const uint32_t sw = (uint32_t)(lane & 7) << 4, rowoff = (uint32_t)lane * 128;
-        int q = 0, li = 0;  // chunks and tiles so far
-        // with pre, buffer 0 stages pre and buffer 1 the residual and y; else the two alternate
-        auto ybuf = [&](int k) { return e.pre ? 1 : k & 1; };
-        auto fetch_residual = [&](int k, int t, int c) {  // lane 0; the buffer is free
-            tc::mbar_arrive_expect_tx(&res_full[w][ybuf(k)], GP_BUF);
-            tc::tma_load_2d(buf + ybuf(k) * GP_BUF, &tr, &res_full[w][ybuf(k)], t % g.nt * BN + half * (BN / 2) + c * 64,
-                            t / g.nt * 2 * GT_M + tr_rows);
+        const uint32_t sw = (uint32_t)(lane & 7) << 4;
+        unsigned char* brow = buf + lane * 128;
+        uint32_t res_phase = 0;
+        auto fetch_residual = [&](int t) {  // lane 0, once the buffer is free
+            tc::mbar_arrive_expect_tx(&res_full[w], GP_BUF);
+            tc::tma_load_2d(buf, &tr, &res_full[w], t % g.nt * BN + part * 64, t / g.nt * 2 * GT_M + tr_rows);
         };
-        uint32_t res_phase[2] = {0, 0};
-        const int t0 = blockIdx.x >> 1;
-        if (e.residual && t0 < tiles && lane == 0) fetch_residual(0, t0, 0);
-        for (int t = t0; t < tiles; t += pairs, ++li) {
+        const int step = pairs * P::GROUPS;
+        int t = (blockIdx.x >> 1) + pairs * group, li = group;
+        if (e.residual && !e.pre && t < tiles && lane == 0) fetch_residual(t);
+        for (; t < tiles; t += step, li += P::GROUPS) {
             const int acc = li & 1;
-            const int n0 = t % g.nt * BN + half * (BN / 2), m0 = t / g.nt * 2 * GT_M + tr_rows;
+            const int col = t % g.nt * BN + part * 64, m0 = t / g.nt * 2 * GT_M + tr_rows;
+            const bool inside = m0 < g.m && col < g.n;
             const bool ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&acc_full[acc], (li >> 1) & 1, fail));
             tc::fence_after_sync();
-#pragma unroll 1
-            for (int c = 0; c < P::CHUNKS; ++c, ++q) {
-                const int yb = ybuf(q), col = n0 + c * 64;
-                unsigned char* by = buf + yb * GP_BUF;
-                // this chunk's buffers are free, and the next residual is on its way
-                if (lane == 0) {
-                    if (e.pre || e.residual)
-                        tc::bulk_wait_read<0>();
-                    else
-                        tc::bulk_wait_read<1>();
-                    if (e.residual && !e.pre) {
-                        const int c1 = c + 1 < P::CHUNKS ? c + 1 : 0, t1 = c1 ? t : t + pairs;
-                        if (t1 < tiles) fetch_residual(q + 1, t1, c1);
-                    } else if (e.residual && q > 0) {
-                        fetch_residual(q, t, c);
-                    }
-                }
-                __syncwarp();
-                float v[64];
-                const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + half * (BN / 2) + c * 64);
-                tc::tmem_ld_32x32(src, *reinterpret_cast<float(*)[32]>(&v[0]));
-                tc::tmem_ld_32x32(src + 32, *reinterpret_cast<float(*)[32]>(&v[32]));
-                if (c + 1 == P::CHUNKS) {
-                    tc::fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
-                }
+            const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + part * 64);
+            float v[2][32];
+            tc::tmem_ld_32x32_nowait(src, v[0]);
+            tc::tmem_ld_32x32_nowait(src + 32, v[1]);
+            tc::tmem_ld_wait(v[0]);
+            tc::tmem_ld_wait(v[1]);
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
                 if (!ok) {  // a wait that ran out leaves NaN, not a plausible number
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) v[j] = NAN;
+                    for (int j = 0; j < 32; ++j) v[h][j] = NAN;
                 }
-                if (e.bias) {
-                    const T* b = static_cast<const T*>(e.bias) + col;
-                    if (col + 64 <= g.n) {
+                if (e.bias) add_bias<T>(v[h], static_cast<const T*>(e.bias) + col + 32 * h, g.n - col - 32 * h);
+            }
+            if (e.pre) {
+                if (lane == 0) tc::bulk_wait_read<0>();
+                __syncwarp();
 #pragma unroll
-                        for (int j = 0; j < 64; j += 8) {
-                            const uint4 u = __ldg(reinterpret_cast<const uint4*>(b + j));
-                            const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float2 f = unpack2<T>(x[k]);
-                                v[j + 2 * k] += f.x;
-                                v[j + 2 * k + 1] += f.y;
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 64; ++j)
-                            if (col + j < g.n) v[j] += to_f32(b[j]);
-                    }
-                }
-                if (e.pre) {
-#pragma unroll
-                    for (int j = 0; j < 64; j += 8)
-                        *reinterpret_cast<uint4*>(buf + rowoff + (((uint32_t)j << 1) ^ sw)) =
-                            make_uint4(pack2<T>(v[j], v[j + 1]), pack2<T>(v[j + 2], v[j + 3]),
-                                       pack2<T>(v[j + 4], v[j + 5]), pack2<T>(v[j + 6], v[j + 7]));
-                    tc::fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (m0 < g.m && col < g.n) tc::tma_store_2d(&tp, buf, col, m0);
-                        tc::bulk_commit();
-                    }
-                }
-                if (e.act != FG_ACT_NONE) {
-#pragma unroll
-                    for (int j = 0; j < 64; ++j) v[j] = activate<true>(v[j], e.act);
-                }
-                if (e.residual) {
-                    tc::mbar_wait_or_fail(&res_full[w][yb], res_phase[yb], fail);
-                    res_phase[yb] ^= 1;
-#pragma unroll
-                    for (int j = 0; j < 64; j += 8) {
-                        const uint4 u = *reinterpret_cast<const uint4*>(by + rowoff + (((uint32_t)j << 1) ^ sw));
-                        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float2 f = unpack2<T>(x[k]);
-                            v[j + 2 * k] += f.x;
-                            v[j + 2 * k + 1] += f.y;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 64; j += 8)
-                    *reinterpret_cast<uint4*>(by + rowoff + (((uint32_t)j << 1) ^ sw)) =
-                        make_uint4(pack2<T>(v[j], v[j + 1]), pack2<T>(v[j + 2], v[j + 3]), pack2<T>(v[j + 4], v[j + 5]),
-                                   pack2<T>(v[j + 6], v[j + 7]));
+                    for (int j = 0; j < 32; j += 8)
+                        *reinterpret_cast<uint4*>(brow + (((uint32_t)(32 * h + j) << 1) ^ sw)) = pack8<T>(&v[h][j]);
                 tc::fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) {
-                    if (m0 < g.m && col < g.n) tc::tma_store_2d(&ty, by, col, m0);
+                    if (inside) tc::tma_store_2d(&tp, buf, col, m0);
                     tc::bulk_commit();
                 }
             }
+            switch (e.act) {
+                case FG_ACT_RELU: activate_all<FG_ACT_RELU>(v); break;
+                case FG_ACT_GELU: activate_all<FG_ACT_GELU>(v); break;
+                case FG_ACT_SILU: activate_all<FG_ACT_SILU>(v); break;
+            }
+            if (e.pre || !e.residual) {  // the buffer's last store has read it
+                if (lane == 0) {
+                    tc::bulk_wait_read<0>();
+                    if (e.residual) fetch_residual(t);
+                }
+                __syncwarp();
+            }
+            if (e.residual) {
+                tc::mbar_wait_or_fail(&res_full[w], res_phase, fail);
+                res_phase ^= 1;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        add8<T>(&v[h][j], *reinterpret_cast<const uint4*>(brow + (((uint32_t)(32 * h + j) << 1) ^ sw)));
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 32; j += 8)
+                    *reinterpret_cast<uint4*>(brow + (((uint32_t)(32 * h + j) << 1) ^ sw)) = pack8<T>(&v[h][j]);
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                if (inside) tc::tma_store_2d(&ty, buf, col, m0);
+                tc::bulk_commit();
+                if (e.residual && !e.pre && t + step < tiles) {  // the next tile's residual travels during its products
+                    tc::bulk_wait_read<0>();
+                    fetch_residual(t + step);
+                }
+            }
         }
-        if (lane == 0) tc::bulk_wait_all();
+        if (lane == 0) tc::bulk_wait_read<0>();
     }
     tc::fence_before_sync();
     __syncthreads();
@@ -572,7 +614,7 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
     auto kernel = &gemm_pair_kernel<T, BN>;
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), PairOf<BN>::SMEM));
     const int pairs = std::max(1, device_attr(cudaDevAttrMultiProcessorCount) / 2);
-    kernel<<<2 * (unsigned)std::min<long long>(tiles, pairs), GT_NT, PairOf<BN>::SMEM, st>>>(ta, tb, ty, tp, tr, g);
+    kernel<<<2 * (unsigned)std::min<long long>(tiles, pairs), GP_NT, PairOf<BN>::SMEM, st>>>(ta, tb, ty, tp, tr, g);
     return check_launch("gemm_pair_kernel");
 }
 
@@ -589,19 +631,26 @@ int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& s, const E
     g.vec = lies(e.y, e.ldy, 8) && lies(e.bias, 0, 8) && lies(e.pre, e.ldp, 8) && lies(e.residual, e.ldr, 8);
     const bool tma_out = lies(e.y, e.ldy, 16) && lies(e.bias, 0, 16) && lies(e.pre, e.ldp, 16) && lies(e.residual, e.ldr, 16);
     // The kernel, tile width and split that finish first by this estimate of SM
-    // cycles: a K block's MMAs (64 x width / 32, or the operands' loads where a
-    // narrow tile waits for them), a tile's epilogue -- behind the next tile's
-    // MMAs in the pair kernel --, start and end, and the exchange of a split tile.
+    // cycles.  A K block takes its MMAs (2 x width) or, when many CTAs ask at once,
+    // L2's delivery of their operands: 5,900 bytes a cycle over the GPU (measured:
+    // 11 TB/s, 800 cycles a block for 74 pairs of 256 x 256 tiles, which so reach
+    // 1,450 TFLOP/s; 256 x 128 tiles need 600).  A tile's epilogue runs behind the
+    // next tile's products in the pair kernel, after them in the other.
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
+    auto estimate = [&](long long tiles, int slots, int ctas_per_tile, int bytes, int bn, int blocks, double epi, bool behind) {
+        auto wave = [&](double active) { return blocks * std::max(2.0 * bn, bytes * active * ctas_per_tile / 5900.0); };
+        const double full = (double)(tiles / slots), rest = (double)(tiles % slots);
+        const double w = wave(slots), last = rest > 0 ? wave(rest) : 0.0;
+        if (!behind) return full * (w + epi) + (rest > 0 ? last + epi : 0.0);
+        return full * std::max(w, epi) + (rest > 0 ? std::max(last, epi) : 0.0) + epi;
+    };
     int best_n = 256;
     bool pair = false;
     double best = 1e300;
     for (int bn : {256, 128}) {
         if (!tma_out) break;
         const long long tiles = (s.m + 2 * GT_M - 1) / (2 * GT_M) * ((g.n + bn - 1) / bn);
-        const double waves = (double)((tiles + sms / 2 - 1) / (sms / 2));
-        const double epi = 16.0 * bn, main = g.kt * (bn == 256 ? 530.0 : 290.0);
-        const double cost = waves * std::max(main, epi) + std::min(main, epi) + 4000;
+        const double cost = 5000 + estimate(tiles, sms / 2, 2, GP_A + bn * GT_K, bn, g.kt, 16.0 * bn, true);
         if (cost < best) {
             best = cost;
             best_n = bn;
@@ -610,11 +659,10 @@ int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& s, const E
     }
     for (int bn : {256, 128, 64}) {
         const long long tiles = (long long)g.mt * ((g.n + bn - 1) / bn);
-        const double block = bn == 256 ? 560 : bn == 128 ? 320 : 220;
         for (int sp : {1, 2, 4, 8}) {
             if (sp > g.kt) break;
-            const double waves = (double)((tiles * sp + sms - 1) / sms);
-            const double cost = waves * ((g.kt + sp - 1) / sp * block + 3000 + 12 * bn) + (sp > 1 ? 1000 + 100 * sp : 0);
+            const double epi = 3000 + 25.0 * bn / sp + 4.0 * bn + (sp > 1 ? 1000 + 100 * sp : 0);
+            const double cost = 3000 + estimate(tiles, sms / sp, sp, GP_A + bn * GT_K * 2, bn, (g.kt + sp - 1) / sp, epi, false);
             if (cost < best) {
                 best = cost;
                 best_n = bn;

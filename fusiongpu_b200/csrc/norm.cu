@@ -3,6 +3,16 @@
 //   y = (x - m) r w + b,   m = avg(x),  r = 1 / sqrt(avg((x - m)^2) + eps)
 //   h = (x - m) r,  a = dy w:   dx = r (a - avg(a) - h avg(a h)),
 //   dw = sum over rows of dy h,  db = sum over rows of dy
+//
+// Both are bound by memory: forward reads x and writes y, backward reads x and
+// dy and writes dx, each once.  A row lives in the registers of a group of G
+// threads -- 8 (rows up to 16 elements a thread: four rows to a warp, so that
+// short rows still fill 128-byte requests), 32 (up to 512, or
+// 768 of 16 bits), 128 (up to 4096) or 512 -- and the variance is taken over the centred values, a second pass
+// that costs no memory traffic.  The weight's gradients are summed in registers
+// over the rows a group takes in turn, joined per block in shared memory, and
+// written as one partial row per block, which ln_reduce_kernel adds in block
+// order: no atomics, the same bits every time.  MEASURED
 #include <algorithm>
 
 #include "adapter_common.cuh"
@@ -10,9 +20,6 @@
 namespace fg {
 
 constexpr int LN_MAX_DIM = 16384;
-constexpr int LN_NT = 128;
-constexpr int LN_COLS = 32;    // columns per block of the column sums
-constexpr int LN_SPLIT = 64;   // row ranges of the column sums
 
 struct NormArgs {
     const void *x, *dy, *w, *b;
@@ -21,102 +28,335 @@ struct NormArgs {
     float *out_mean, *out_rstd, *part;
     long long rows, ldx, ldy, lddx;
     int dim, w_f32;
+    int params;  // the weight's gradients are wanted
+    int wide;    // rows and parameters start on 16-byte boundaries
     float eps;
 };
 
-template <class T>
-__device__ __forceinline__ float param(const void* p, int f32, int j) {
-    return f32 ? static_cast<const float*>(p)[j] : to_f32(static_cast<const T*>(p)[j]);
+// VEC elements of a row: one 16-byte access where every row starts on a 16-byte
+// boundary (wide), else single ones, in the same place of the same thread: the
+// results do not depend on alignment.  VEC is 1 where dim is no multiple of 16 bytes.
+template <class T, int VEC>
+struct Chunk {
+    T v[VEC];
+};
+
+template <class T, int VEC>
+__device__ __forceinline__ void load_chunk(Chunk<T, VEC>& c, const T* p, int wide) {
+    if (VEC * sizeof(T) == 16 && wide) {  // read once: not kept in L1, which holds the parameters
+        uint4 u;
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                     : "l"(p));
+        *reinterpret_cast<uint4*>(c.v) = u;
+    } else {
+        // not __ldg: for 16-bit types that is an asm that may be moved above the caller's bounds check
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) c.v[i] = p[i];
+    }
 }
 
-template <class T>
-__global__ void __launch_bounds__(LN_NT) ln_forward_kernel(const NormArgs g) {
-    __shared__ float s[LN_NT / 32];
-    for (long long r = blockIdx.x; r < g.rows; r += gridDim.x) {
-        const T* x = static_cast<const T*>(g.x) + r * g.ldx;
-        T* y = static_cast<T*>(g.y) + r * g.ldy;
-        float t = 0.0f;
-        for (int j = threadIdx.x; j < g.dim; j += LN_NT) t += to_f32(x[j]);
-        const float mean = block_sum<LN_NT>(t, s) / (float)g.dim;
+template <class T, int VEC>
+__device__ __forceinline__ void store_chunk(T* p, const float* f, int wide) {
+    alignas(16) T v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = from_f32<T>(f[i]);
+    if (VEC * sizeof(T) == 16 && wide) {
+        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) p[i] = v[i];
+    }
+}
+
+// VEC parameters from column j: of T or float, `absent` without any.
+template <class T, int VEC>
+__device__ __forceinline__ void load_params(float* f, const void* p, int f32, int wide, int j, float absent) {
+    if (!p) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = absent;
+    } else if (VEC == 1 || !wide) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = f32 ? static_cast<const float*>(p)[j + i] : to_f32(static_cast<const T*>(p)[j + i]);
+    } else if (f32) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + j + i));
+            f[i] = q.x;
+            f[i + 1] = q.y;
+            f[i + 2] = q.z;
+            f[i + 3] = q.w;
+        }
+    } else {
+        alignas(16) T v[VEC];
+        *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + j));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = to_f32(v[i]);
+    }
+}
+
+template <int G>
+constexpr int ln_block() {
+    return G < 128 ? 256 : G;
+}
+
+// Sum over the group's threads, in each of them.
+template <int G>
+__device__ __forceinline__ float group_sum(float v, float* s) {
+    if (G > 32) return block_sum<ln_block<G>()>(v, s);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+template <class T, int VEC, int NCH, int G>
+__global__ void __launch_bounds__(ln_block<G>()) ln_forward_kernel(const NormArgs g) {
+    constexpr int NT = ln_block<G>(), RPB = NT / G;
+    __shared__ float s[NT / 32];
+    const int gl = threadIdx.x % G;
+    const float inv = 1.0f / (float)g.dim;
+    const long long step = (long long)gridDim.x * RPB;
+    // every thread of a warp stays in the loop as long as one of its rows exists
+    for (long long r = (long long)blockIdx.x * RPB + threadIdx.x / G, r0 = r - (threadIdx.x % 32) / G;
+         (G > 32 ? r : r0) < g.rows; r += step, r0 += step) {
+        const bool in = r < g.rows;
+        const T* x = static_cast<const T*>(g.x) + (in ? r : g.rows - 1) * g.ldx;
+        Chunk<T, VEC> c[NCH];
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int j = (k * G + gl) * VEC;
+            if (j < g.dim) load_chunk<T, VEC>(c[k], x + j, g.wide);
+        }
+        float v[NCH * VEC], t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const bool have = (k * G + gl) * VEC < g.dim;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                v[k * VEC + i] = have ? to_f32(c[k].v[i]) : 0.0f;
+                t += v[k * VEC + i];
+            }
+        }
+        const float mean = group_sum<G>(t, s) * inv;
         t = 0.0f;
-        for (int j = threadIdx.x; j < g.dim; j += LN_NT) {
-            const float c = to_f32(x[j]) - mean;
-            t = fmaf(c, c, t);
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const bool have = (k * G + gl) * VEC < g.dim;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                v[k * VEC + i] -= mean;
+                if (have) t = fmaf(v[k * VEC + i], v[k * VEC + i], t);
+            }
         }
-        const float rstd = rsqrtf(block_sum<LN_NT>(t, s) / (float)g.dim + g.eps);
-        for (int j = threadIdx.x; j < g.dim; j += LN_NT) {
-            const float h = __fmul_rn(to_f32(x[j]) - mean, rstd);  // an absent weight or bias is 1 or 0, bit for bit
-            y[j] = from_f32<T>(fmaf(h, g.w ? param<T>(g.w, g.w_f32, j) : 1.0f, g.b ? param<T>(g.b, g.w_f32, j) : 0.0f));
+        const float rstd = 1.0f / sqrtf(group_sum<G>(t, s) * inv + g.eps);
+        if (!in) continue;
+        T* y = static_cast<T*>(g.y) + r * g.ldy;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int j = (k * G + gl) * VEC;
+            if (j < g.dim) {
+                float w[VEC], b[VEC], o[VEC];
+                load_params<T, VEC>(w, g.w, g.w_f32, g.wide, j, 1.0f);
+                load_params<T, VEC>(b, g.b, g.w_f32, g.wide, j, 0.0f);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) o[i] = fmaf(__fmul_rn(v[k * VEC + i], rstd), w[i], b[i]);
+                store_chunk<T, VEC>(y + j, o, g.wide);
+            }
         }
-        if (g.out_mean && threadIdx.x == 0) {
+        if (g.out_mean && gl == 0) {
             g.out_mean[r] = mean;
             g.out_rstd[r] = rstd;
         }
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(LN_NT) ln_dx_kernel(const NormArgs g) {
-    __shared__ float s[LN_NT / 32];
-    for (long long r = blockIdx.x; r < g.rows; r += gridDim.x) {
-        const T* x = static_cast<const T*>(g.x) + r * g.ldx;
-        const T* dy = static_cast<const T*>(g.dy) + r * g.ldy;
-        T* dx = static_cast<T*>(g.dx) + r * g.lddx;
-        const float mean = g.mean[r], rstd = g.rstd[r];
-        float sa = 0.0f, sah = 0.0f;
-        for (int j = threadIdx.x; j < g.dim; j += LN_NT) {
-            const float h = (to_f32(x[j]) - mean) * rstd;
-            const float a = to_f32(dy[j]) * (g.w ? param<T>(g.w, g.w_f32, j) : 1.0f);
-            sa += a;
-            sah = fmaf(a, h, sah);
-        }
-        sa = block_sum<LN_NT>(sa, s) / (float)g.dim;
-        sah = block_sum<LN_NT>(sah, s) / (float)g.dim;
-        for (int j = threadIdx.x; j < g.dim; j += LN_NT) {
-            const float h = (to_f32(x[j]) - mean) * rstd;
-            const float a = to_f32(dy[j]) * (g.w ? param<T>(g.w, g.w_f32, j) : 1.0f);
-            dx[j] = from_f32<T>(rstd * (a - sa - h * sah));
-        }
-    }
-}
+// Blocks of the backward kernel per SM (its registers: two rows ahead packed, two
+// sums a column).
+constexpr int ln_per_sm(int G, int E) { return G == 512 ? 1 : G == 128 ? (E > 16 ? 2 : 4) : 2; }
 
-// Block (c, s): columns [32c, 32c + 32) over the s-th range of rows.
-template <class T>
-__global__ void __launch_bounds__(256) ln_columns_kernel(const NormArgs g) {
-    __shared__ float sw[8][LN_COLS], sb[8][LN_COLS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * LN_COLS + lane;
-    const long long per = (g.rows + gridDim.y - 1) / gridDim.y;
-    const long long r0 = blockIdx.y * per, r1 = r0 + per < g.rows ? r0 + per : g.rows;
-    float w = 0.0f, b = 0.0f;
-    if (j < g.dim)
-        for (long long r = r0 + warp; r < r1; r += 8) {
-            const float d = to_f32(static_cast<const T*>(g.dy)[r * g.ldy + j]);
-            w = fmaf(d, (to_f32(static_cast<const T*>(g.x)[r * g.ldx + j]) - g.mean[r]) * g.rstd[r], w);
-            b += d;
-        }
-    sw[warp][lane] = w;
-    sb[warp][lane] = b;
+// Sums of two values over the group.
+template <int G>
+__device__ __forceinline__ void group_sum2(float& a, float& b, float (*s)[2]) {
+#pragma unroll
+    for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    if (G <= 32) return;
+    __syncthreads();  // the previous call's readers are done with s
+    if ((threadIdx.x & 31) == 0) {
+        s[threadIdx.x >> 5][0] = a;
+        s[threadIdx.x >> 5][1] = b;
+    }
     __syncthreads();
-    if (warp == 0 && j < g.dim) {
-        w = b = 0.0f;
-        for (int i = 0; i < 8; ++i) {
-            w += sw[i][lane];
-            b += sb[i][lane];
-        }
-        g.part[(size_t)blockIdx.y * 2 * g.dim + j] = w;
-        g.part[((size_t)blockIdx.y * 2 + 1) * g.dim + j] = b;
+    a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < G / 32; ++w) {
+        a += s[w][0];
+        b += s[w][1];
     }
 }
 
-// Adds the partial rows in their order.
+// Groups take rows in turn; x and dy of the next row are fetched before this one
+// is worked on (not where a thread holds 32 columns), and stay in their own type
+// until they are used.  The sums for the weight's gradients are in registers (G =
+// 512: in shared memory, each thread its own columns).
+template <class T, int VEC, int NCH, int G>
+__global__ void __launch_bounds__(ln_block<G>(), ln_per_sm(G, NCH * VEC)) ln_backward_kernel(const NormArgs g) {
+    constexpr int NT = ln_block<G>(), RPB = NT / G, E = NCH * VEC;
+    constexpr bool SMEM = G == 512, AHEAD = E <= 24;
+    extern __shared__ float sm[];
+    __shared__ float s[NT / 32][2];
+    const int gl = threadIdx.x % G;
+    const float inv = 1.0f / (float)g.dim;
+    const long long step = (long long)gridDim.x * RPB;
+    float dw[SMEM ? 1 : E], db[SMEM ? 1 : E];
+    if (SMEM) {
+        for (int k = 0; k < NCH; ++k)
+            for (int i = 0; i < VEC; ++i) {
+                const int j = (k * G + gl) * VEC + i;
+                if (j < g.dim) sm[j] = sm[g.dim + j] = 0.0f;
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.0f;
+    }
+    struct Row {
+        Chunk<T, VEC> x[NCH], d[NCH];
+        float mean, rstd;
+    };
+    auto fetch = [&](Row& row, long long r) {
+        if (r >= g.rows) return;
+        const T* x = static_cast<const T*>(g.x) + r * g.ldx;
+        const T* d = static_cast<const T*>(g.dy) + r * g.ldy;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int j = (k * G + gl) * VEC;
+            if (j < g.dim) {
+                load_chunk<T, VEC>(row.x[k], x + j, g.wide);
+                load_chunk<T, VEC>(row.d[k], d + j, g.wide);
+            }
+        }
+        row.mean = __ldg(g.mean + r);
+        row.rstd = __ldg(g.rstd + r);
+    };
+    Row cur, next;
+    const long long first = (long long)blockIdx.x * RPB + threadIdx.x / G;
+    if (AHEAD) fetch(next, first);
+    for (long long r = first, r0 = r - (threadIdx.x % 32) / G; (G > 32 ? r : r0) < g.rows; r += step, r0 += step) {
+        const bool in = r < g.rows;
+        if (AHEAD) {
+            cur = next;
+            fetch(next, r + step);
+        } else {
+            fetch(cur, r);
+        }
+        float sa = 0.0f, sah = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int j = (k * G + gl) * VEC;
+            if (in && j < g.dim) {
+                float w[VEC];
+                load_params<T, VEC>(w, g.w, g.w_f32, g.wide, j, 1.0f);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float d = to_f32(cur.d[k].v[i]), h = (to_f32(cur.x[k].v[i]) - cur.mean) * cur.rstd;
+                    const float a = d * w[i];
+                    if (SMEM) {
+                        sm[j + i] = fmaf(d, h, sm[j + i]);
+                        sm[g.dim + j + i] += d;
+                    } else {
+                        dw[k * VEC + i] = fmaf(d, h, dw[k * VEC + i]);
+                        db[k * VEC + i] += d;
+                    }
+                    sa += a;
+                    sah = fmaf(a, h, sah);
+                }
+            }
+        }
+        if (!g.dx) continue;
+        group_sum2<G>(sa, sah, s);
+        sa *= inv;
+        sah *= inv;
+        if (!in) continue;
+        T* dx = static_cast<T*>(g.dx) + r * g.lddx;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int j = (k * G + gl) * VEC;
+            if (j < g.dim) {
+                float w[VEC], o[VEC];
+                load_params<T, VEC>(w, g.w, g.w_f32, g.wide, j, 1.0f);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float h = (to_f32(cur.x[k].v[i]) - cur.mean) * cur.rstd;
+                    o[i] = cur.rstd * (to_f32(cur.d[k].v[i]) * w[i] - sa - h * sah);
+                }
+                store_chunk<T, VEC>(dx + j, o, g.wide);
+            }
+        }
+    }
+    if (!g.params) return;
+    float* part = g.part + (size_t)blockIdx.x * 2 * g.dim;
+    if (G > 32) {
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int j = (k * G + gl) * VEC + i;
+                if (j < g.dim) {
+                    part[j] = SMEM ? sm[j] : dw[SMEM ? 0 : k * VEC + i];
+                    part[g.dim + j] = SMEM ? sm[g.dim + j] : db[SMEM ? 0 : k * VEC + i];
+                }
+            }
+        return;
+    }
+    // groups of a warp, then the warps of the block
+    float* mine = sm + (threadIdx.x >> 5) * 2 * g.dim;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            float u = dw[SMEM ? 0 : k * VEC + i], v = db[SMEM ? 0 : k * VEC + i];
+#pragma unroll
+            for (int o = G; o < 32; o <<= 1) {
+                u += __shfl_xor_sync(0xffffffffu, u, o);
+                v += __shfl_xor_sync(0xffffffffu, v, o);
+            }
+            const int j = (k * G + gl) * VEC + i;
+            if (j < g.dim && (threadIdx.x & 31) < G) {
+                mine[j] = u;
+                mine[g.dim + j] = v;
+            }
+        }
+    __syncthreads();
+    for (int j = threadIdx.x; j < 2 * g.dim; j += NT) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) v += sm[w * 2 * g.dim + j];
+        part[j] = v;
+    }
+}
+
+// Adds the partial rows: 32 columns per block, warp w the rows w, w + 32, ... in
+// order, then the warps in order.
 template <class P>
-__global__ void ln_reduce_kernel(const float* part, int parts, int dim, P* dw, P* db) {
-    const int j = blockIdx.x * blockDim.x + threadIdx.x;
-    if (j >= 2 * dim) return;
+__global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* part, int parts, int dim, P* dw, P* db) {
+    __shared__ float s[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
     float v = 0.0f;
-    for (int p = 0; p < parts; ++p) v += part[(size_t)p * 2 * dim + j];
-    P* out = j < dim ? dw : db;
-    if (out) out[j < dim ? j : j - dim] = from_f32<P>(v);
+    if (j < 2 * dim) {
+#pragma unroll 8
+        for (int p = warp; p < parts; p += 32) v += part[(size_t)p * 2 * dim + j];
+    }
+    s[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && j < 2 * dim) {
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 32; ++w) v += s[w][lane];
+        P* out = j < dim ? dw : db;
+        if (out) out[j < dim ? j : j - dim] = from_f32<P>(v);
+    }
 }
 
 static int norm_check(int dtype, int param_dtype, long long rows, int dim) {
@@ -129,33 +369,97 @@ static int norm_check(int dtype, int param_dtype, long long rows, int dim) {
     return FG_OK;
 }
 
-static size_t norm_ws(int dim) { return (size_t)LN_SPLIT * 2 * dim * sizeof(float); }
+// Blocks of the backward pass for groups of G threads with E columns each: the SMs
+// filled once, and two rows at least to a group.
+static int norm_parts(long long rows, int G, int E) {
+    const long long rpb = G < 128 ? 256 / G : 1, want = (rows + 2 * rpb - 1) / (2 * rpb);
+    const long long fill = (long long)std::max(1, device_attr(cudaDevAttrMultiProcessorCount)) * ln_per_sm(G, E);
+    return (int)std::min(fill, std::max(want, 1ll));
+}
 
+static size_t norm_ws(long long rows, int dim) {  // for whichever group the alignment selects
+    const int parts = std::max(std::max(norm_parts(rows, 8, 16), norm_parts(rows, 32, 16)),
+                               std::max(norm_parts(rows, 128, 16), norm_parts(rows, 512, 32)));
+    return (size_t)parts * 2 * dim * sizeof(float);
+}
+
+template <class T, int VEC, int NCH, int G>
+static int launch_norm(const NormArgs& g, bool backward, int* parts, cudaStream_t st) {
+    constexpr int NT = ln_block<G>();
+    if (!backward) {
+        const long long blocks = (g.rows + NT / G - 1) / (NT / G);
+        ln_forward_kernel<T, VEC, NCH, G><<<(unsigned)std::min<long long>(blocks, 1 << 24), NT, 0, st>>>(g);
+        return check_launch("ln_forward_kernel");
+    }
+    const int smem = (G == 128 ? 0 : G == 512 ? 1 : NT / 32) * 2 * g.dim * (int)sizeof(float);
+    auto kernel = &ln_backward_kernel<T, VEC, NCH, G>;
+    if (smem > 48 * 1024) FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
+    *parts = norm_parts(g.rows, G, NCH * VEC);
+    kernel<<<*parts, NT, smem, st>>>(g);
+    return check_launch("ln_backward_kernel");
+}
+
+// The group and the chunks per thread that hold a row.
 template <class T>
-static int norm_forward(const NormArgs& g, cudaStream_t s) {
-    ln_forward_kernel<T><<<(unsigned)std::min<long long>(g.rows, 1 << 20), LN_NT, 0, s>>>(g);
-    return check_launch("ln_forward_kernel");
+static int dispatch_norm(NormArgs g, bool backward, int* parts, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    auto lies = [&](const void* p, long long ld) { return !p || (aligned(p, 16) && ld * sizeof(T) % 16 == 0); };
+    const bool vec = g.dim % V == 0;
+    g.wide = lies(g.x, g.ldx) && lies(backward ? g.dy : g.y, g.ldy) && lies(g.dx, g.lddx) &&
+                     lies(g.w, 0) && lies(g.b, 0);
+#define FG_NORM(VEC, NCH, G) \
+    if (g.dim <= (VEC) * (NCH) * (G)) return launch_norm<T, VEC, NCH, G>(g, backward, parts, st)
+    if constexpr (V == 8) {
+        if (vec) {
+            FG_NORM(8, 1, 8);
+            FG_NORM(8, 2, 8);
+            FG_NORM(8, 2, 32);
+            FG_NORM(8, 3, 32);
+            FG_NORM(8, 1, 128);
+            FG_NORM(8, 2, 128);
+            FG_NORM(8, 4, 128);
+            FG_NORM(8, 4, 512);
+        }
+    } else {
+        if (vec) {
+            FG_NORM(4, 2, 8);
+            FG_NORM(4, 4, 8);
+            FG_NORM(4, 2, 32);
+            FG_NORM(4, 4, 32);
+            FG_NORM(4, 2, 128);
+            FG_NORM(4, 4, 128);
+            FG_NORM(4, 8, 128);
+            FG_NORM(4, 8, 512);
+        }
+    }
+    FG_NORM(1, 16, 8);
+    FG_NORM(1, 16, 32);
+    FG_NORM(1, 8, 128);
+    FG_NORM(1, 16, 128);
+    FG_NORM(1, 32, 128);
+    return launch_norm<T, 1, 32, 512>(g, backward, parts, st);
+#undef FG_NORM
 }
 
 template <class T>
-static int norm_backward(const NormArgs& g, void* dw, void* db, cudaStream_t s) {
-    if (g.dx && g.rows) {
-        ln_dx_kernel<T><<<(unsigned)std::min<long long>(g.rows, 1 << 20), LN_NT, 0, s>>>(g);
-        const int rc = check_launch("ln_dx_kernel");
+static int norm_forward(const NormArgs& g, cudaStream_t s) {
+    return dispatch_norm<T>(g, false, nullptr, s);
+}
+
+template <class T>
+static int norm_backward(NormArgs g, void* dw, void* db, cudaStream_t s) {
+    g.params = dw || db;
+    int n = 0;
+    if (g.rows && (g.dx || g.params)) {
+        const int rc = dispatch_norm<T>(g, true, &n, s);
         if (rc) return rc;
     }
-    if (!dw && !db) return FG_OK;
-    const int split = (int)std::min<long long>(LN_SPLIT, (g.rows + 7) / 8);
-    if (split) {
-        ln_columns_kernel<T><<<dim3((g.dim + LN_COLS - 1) / LN_COLS, split), 256, 0, s>>>(g);
-        const int rc = check_launch("ln_columns_kernel");
-        if (rc) return rc;
-    }
-    const int nb = (2 * g.dim + 255) / 256;
+    if (!g.params) return FG_OK;
+    const int nb = (2 * g.dim + 31) / 32;
     if (g.w_f32)
-        ln_reduce_kernel<float><<<nb, 256, 0, s>>>(g.part, split, g.dim, (float*)dw, (float*)db);
+        ln_reduce_kernel<float><<<nb, 1024, 0, s>>>(g.part, n, g.dim, (float*)dw, (float*)db);
     else
-        ln_reduce_kernel<T><<<nb, 256, 0, s>>>(g.part, split, g.dim, (T*)dw, (T*)db);
+        ln_reduce_kernel<T><<<nb, 1024, 0, s>>>(g.part, n, g.dim, (T*)dw, (T*)db);
     return check_launch("ln_reduce_kernel");
 }
 
@@ -201,7 +505,7 @@ int fg_layer_norm_backward_workspace_size(int64_t rows, int32_t dim, size_t* byt
         FG_REQUIRE(bytes, "null bytes");
         const int rc = norm_check(FG_DTYPE_F32, FG_DTYPE_F32, rows, dim);
         if (rc) return rc;
-        *bytes = norm_ws(dim);
+        *bytes = norm_ws(rows, dim);
         return FG_OK;
     });
 }
@@ -219,7 +523,7 @@ int fg_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int
         g.lddx = dx_stride ? dx_stride : dim;
         FG_REQUIRE(g.ldx >= dim && g.ldy >= dim && g.lddx >= dim, "row stride below dim");
         if (rows) FG_REQUIRE(dy && x && mean && rstd, "null buffer");
-        if (dweight || dbias) rc = adapter_ws(workspace, workspace_bytes, norm_ws(dim));
+        if (dweight || dbias) rc = adapter_ws(workspace, workspace_bytes, norm_ws(rows, dim));
         if (rc) return rc;
         g.x = x;
         g.dy = dy;

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "adapter_common.cuh"
+#include "packed.cuh"
 
 namespace fg {
 
@@ -33,31 +34,6 @@ __device__ __forceinline__ float upper_tail(float z, float& e) {  // Phi(-|z|)
     p = fmaf(t, p, 0.5f * -0.284496736f);
     p = fmaf(t, p, 0.5f * 0.254829592f);
     return p * t * e;
-}
-
-// Two floats in one register pair: fma.rn.f32x2 issues once for both.
-__device__ __forceinline__ uint64_t pair2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair2(uint64_t p, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
 }
 
 // GELU of two values for results of 16 bits: max(z, 0) - a Phi(-a), a = min(|z|, 30)

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
         }
     } else {  // ---- epilogue warps: TMEM -> partial tile in shared memory
         const int q4 = warp & 3, half = (warp - 2) >> 2;
-        const bool ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&acc_full, 0, fail));
+        const bool ok = tc::mbar_wait_warp(&acc_full, 0, fail);
         tc::fence_after_sync();
         float* row = part + (q4 * 32 + lane) * LDP;
 #pragma unroll 1
@@ -450,7 +450,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             const int acc = li & 1;
             const int col = t % g.nt * BN + part * 64, m0 = t / g.nt * 2 * GT_M + tr_rows;
             const bool inside = m0 < g.m && col < g.n;
-            const bool ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&acc_full[acc], (li >> 1) & 1, fail));
+            const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
             tc::fence_after_sync();
             const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + part * 64);
             float v[2][32];
@@ -497,7 +497,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 __syncwarp();
             }
             if (e.residual) {
-                tc::mbar_wait_or_fail(&res_full[w], res_phase, fail);
+                tc::mbar_wait_warp(&res_full[w], res_phase, fail);
                 res_phase ^= 1;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)

@@ -393,7 +393,7 @@ static int launch_norm(const NormArgs& g, bool backward, int* parts, cudaStream_
     }
     const int smem = (G == 128 ? 0 : G == 512 ? 1 : NT / 32) * 2 * g.dim * (int)sizeof(float);
     auto kernel = &ln_backward_kernel<T, VEC, NCH, G>;
-    if (smem > 48 * 1024) FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
+    if (smem > 40 * 1024) FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
     *parts = norm_parts(g.rows, G, NCH * VEC);
     kernel<<<*parts, NT, smem, st>>>(g);
     return check_launch("ln_backward_kernel");

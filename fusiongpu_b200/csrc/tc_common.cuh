@@ -67,6 +67,15 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
         : "memory");
 }
 
+// Untiled bulk copy of `bytes` (a multiple of 16, both ends 16-byte aligned) into
+// this block's shared memory, completing on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
                  "r"(ncols)
@@ -265,6 +274,15 @@ __device__ __forceinline__ bool mbar_wait_or_fail(uint64_t* bar, uint32_t parity
     }
     *fail = 1;
     return false;
+}
+
+// The same by a whole warp: one lane polls (the polls of 32 lanes are taken one
+// after another, about 250 cycles even on a completed phase) and tells the others.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* fail) {
+    int ok = 0;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait_or_fail(bar, parity, fail);
+    __syncwarp();  // orders the other lanes' accesses too; the shuffle alone is dropped where its result is not used
+    return __shfl_sync(0xffffffffu, ok, 0);
 }
 
 // Instruction descriptor, kind::f16: bf16 x bf16 -> f32, both K-major.

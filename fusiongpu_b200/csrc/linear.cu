@@ -54,52 +54,152 @@ __global__ void __launch_bounds__(256) gemm_simt_kernel(const T* a, const T* b, 
 }
 
 template <class T>
-static int gemm(const void* a, const void* b, const GemmShape& g, const Epilogue& e, cudaStream_t s) {
+static int gemm(const void* a, const void* b, const GemmShape& g, const Epilogue& e, void* ws, cudaStream_t s) {
     const long long tiles = ((g.m + SG_T - 1) / SG_T) * ((g.n + SG_T - 1) / SG_T);
     FG_REQUIRE(tiles <= 0x7fffffffll, "%lld x %lld outputs: too many tiles", g.m, g.n);
     if (tiles == 0) return FG_OK;
     if (sizeof(T) == 2 && tc_gemm_fits(a, b, g))
-        return tc_gemm(std::is_same<T, __half>::value ? FG_DTYPE_F16 : FG_DTYPE_BF16, a, b, g, e, s);
+        return tc_gemm(std::is_same<T, __half>::value ? FG_DTYPE_F16 : FG_DTYPE_BF16, a, b, g, e, ws, s);
     gemm_simt_kernel<T><<<(unsigned)tiles, 256, 0, s>>>(static_cast<const T*>(a), static_cast<const T*>(b), g, e);
     return check_launch("gemm_simt_kernel");
 }
 
-constexpr int DZ_COLS = 32, DZ_SPLIT = 64;
+// dz = dy act'(pre) and the column sums of dz, in one pass over dy and pre: a warp
+// takes 32 x VEC columns of every eighth row of its block's range, two rows at a
+// time, sums them in registers, and the block writes one partial row.  Memory-bound;
+// DZFIG
+constexpr int DZ_WARPS = 8;
 
-// dz = dy act'(pre) (dz NULL: not stored) and the partial column sums of dz of
-// each row range.
-template <class T>
-__global__ void __launch_bounds__(256) dz_kernel(const T* dy, long long lddy, const T* pre, long long ldp, int act,
-                                                 long long rows, int dim, T* dz, float* part) {
-    __shared__ float sb[8][DZ_COLS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * DZ_COLS + lane;
-    const long long per = (rows + gridDim.y - 1) / gridDim.y;
-    const long long r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
-    float b = 0.0f;
-    if (j < dim)
-        for (long long r = r0 + warp; r < r1; r += 8) {
-            float v = to_f32(dy[r * lddy + j]);
-            if (act != FG_ACT_NONE) v *= activate_grad<sizeof(T) == 2>(to_f32(pre[r * ldp + j]), act);
-            if (dz) dz[r * dim + j] = from_f32<T>(v);
-            b += v;
-        }
-    if (!part) return;
-    sb[warp][lane] = b;
-    __syncthreads();
-    if (warp == 0 && j < dim) {
-        b = 0.0f;
-        for (int i = 0; i < 8; ++i) b += sb[i][lane];
-        part[(size_t)blockIdx.y * dim + j] = b;
+struct DzArgs {
+    const void *dy, *pre;
+    void* dz;     // NULL: not stored
+    float* part;  // NULL: no sums
+    long long lddy, ldp, rows, per;
+    int dim, act, wide;
+};
+
+template <class T, int VEC>
+__device__ __forceinline__ void dz_load(T (&v)[VEC], const T* p, int left, int wide) {
+    if (wide && left >= VEC) {
+        *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < left) v[i] = p[i];
     }
 }
 
+// dy act'(pre) of two columns.
+template <int ACT, bool FAST>
+__device__ __forceinline__ void dz_pair(float& d0, float& d1, float p0, float p1) {
+    if (ACT == FG_ACT_NONE) return;
+    if (ACT == FG_ACT_GELU && FAST) {
+        gelu_grad2(p0, p1);
+    } else {
+        p0 = activate_grad<FAST>(p0, ACT);
+        p1 = activate_grad<FAST>(p1, ACT);
+    }
+    unpair2(mul2(pair2(d0, d1), pair2(p0, p1)), d0, d1);
+}
+
+template <class T, int ACT>
+__global__ void __launch_bounds__(DZ_WARPS * 32) dz_kernel(const DzArgs g) {
+    constexpr int VEC = 16 / sizeof(T), U = 2;
+    __shared__ float s[DZ_WARPS][32 * VEC];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = (blockIdx.x * 32 + lane) * VEC, left = g.dim - j;
+    const long long r0 = blockIdx.y * g.per, r1 = min(r0 + g.per, g.rows);
+    float sum[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+    if (left > 0)
+        for (long long r = r0 + warp; r < r1; r += U * DZ_WARPS) {
+            alignas(16) T d[U][VEC], p[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long long q = r + u * DZ_WARPS;
+                if (q < r1) {
+                    dz_load<T, VEC>(d[u], static_cast<const T*>(g.dy) + q * g.lddy + j, left, g.wide);
+                    if (ACT != FG_ACT_NONE) dz_load<T, VEC>(p[u], static_cast<const T*>(g.pre) + q * g.ldp + j, left, g.wide);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long long q = r + u * DZ_WARPS;
+                if (q >= r1) break;
+                alignas(16) T o[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; i += 2) {
+                    float v0 = to_f32(d[u][i]), v1 = to_f32(d[u][i + 1]);
+                    dz_pair<ACT, sizeof(T) == 2>(v0, v1, to_f32(p[u][i]), to_f32(p[u][i + 1]));
+                    v0 = i < left ? v0 : 0.0f;  // columns past the last
+                    v1 = i + 1 < left ? v1 : 0.0f;
+                    sum[i] += v0;
+                    sum[i + 1] += v1;
+                    o[i] = from_f32<T>(v0);
+                    o[i + 1] = from_f32<T>(v1);
+                }
+                if (g.dz) {  // rows of dz are padded to 16 bytes
+                    T* out = static_cast<T*>(g.dz) + q * ((g.dim + VEC - 1) / VEC * VEC) + j;
+                    *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(o);
+                }
+            }
+        }
+    if (!g.part) return;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s[warp][lane * VEC + i] = sum[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * VEC; c += DZ_WARPS * 32) {
+        const int col = blockIdx.x * 32 * VEC + c;
+        if (col >= g.dim) break;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < DZ_WARPS; ++w) v += s[w][c];
+        g.part[(size_t)blockIdx.y * g.dim + col] = v;
+    }
+}
+
+// Adds the partial rows: 32 columns per block, warp w the rows w, w + 32, ... in
+// order, then the warps in order.
 template <class T>
-__global__ void dz_reduce_kernel(const float* part, int parts, int dim, T* dbias) {
-    const int j = blockIdx.x * blockDim.x + threadIdx.x;
-    if (j >= dim) return;
+__global__ void __launch_bounds__(1024) dz_reduce_kernel(const float* part, int parts, int dim, T* dbias) {
+    __shared__ float s[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
     float v = 0.0f;
-    for (int p = 0; p < parts; ++p) v += part[(size_t)p * dim + j];
-    dbias[j] = from_f32<T>(v);
+    if (j < dim) {
+#pragma unroll 4
+        for (int p = warp; p < parts; p += 32) v += part[(size_t)p * dim + j];
+    }
+    s[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && j < dim) {
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 32; ++w) v += s[w][lane];
+        dbias[j] = from_f32<T>(v);
+    }
+}
+
+// Row ranges: four blocks to an SM over the column tiles, 16 rows at least to a range.
+static int dz_split(long long rows, int dim, int elem) {
+    const int cols = 32 * (16 / elem), tiles = (dim + cols - 1) / cols;
+    const long long fill = std::max(1ll, 4ll * std::max(1, device_attr(cudaDevAttrMultiProcessorCount)) / tiles);
+    return (int)std::max(1ll, std::min(fill, (rows + 15) / 16));
+}
+
+template <class T>
+static int launch_dz(DzArgs g, int split, cudaStream_t s) {
+    constexpr int cols = 32 * (16 / (int)sizeof(T));
+    g.per = (g.rows + split - 1) / split;
+    auto lies = [&](const void* p, long long ld) { return !p || (aligned(p, 16) && ld * (int)sizeof(T) % 16 == 0); };
+    g.wide = lies(g.dy, g.lddy) && lies(g.pre, g.ldp);
+    const dim3 grid((g.dim + cols - 1) / cols, split);
+    switch (g.act) {
+        case FG_ACT_RELU: dz_kernel<T, FG_ACT_RELU><<<grid, DZ_WARPS * 32, 0, s>>>(g); break;
+        case FG_ACT_GELU: dz_kernel<T, FG_ACT_GELU><<<grid, DZ_WARPS * 32, 0, s>>>(g); break;
+        case FG_ACT_SILU: dz_kernel<T, FG_ACT_SILU><<<grid, DZ_WARPS * 32, 0, s>>>(g); break;
+        default: dz_kernel<T, FG_ACT_NONE><<<grid, DZ_WARPS * 32, 0, s>>>(g);
+    }
+    return check_launch("dz_kernel");
 }
 
 struct Strides {
@@ -121,49 +221,66 @@ static int linear_check(const fg_linear_params* p, Strides& t) {
     return FG_OK;
 }
 
+// Products of a layer: z = x w^T, dx = dz w, dw = dz^T x.
+static GemmShape forward_shape(const fg_linear_params* p, const Strides& t) {
+    return {p->rows, p->out_dim, p->in_dim, t.x, 1, t.w, 1};
+}
+static GemmShape dx_shape(const fg_linear_params* p, const Strides& t, long long ldz) {
+    return {p->rows, p->in_dim, p->out_dim, ldz, 1, 1, t.w};
+}
+static GemmShape dw_shape(const fg_linear_params* p, const Strides& t, long long ldz) {
+    return {p->out_dim, p->in_dim, p->rows, 1, ldz, 1, t.x};
+}
+
 struct BackwardWs {
-    void* dz;
+    void *dz, *product;
     float* part;
 };
 
-static size_t backward_carve(const fg_linear_params* p, void* ws, size_t bytes, BackwardWs& w) {
+static long long dz_stride(const fg_linear_params* p) {
+    const int vec = 16 / dtype_size(p->dtype);
+    return (long long)(p->out_dim + vec - 1) / vec * vec;
+}
+
+static size_t backward_carve(const fg_linear_params* p, const Strides& t, void* ws, size_t bytes, BackwardWs& w) {
     Carve c(ws, bytes);
-    w.dz = p->activation == FG_ACT_NONE
-               ? nullptr
-               : c.take<char>((size_t)p->rows * p->out_dim * dtype_size(p->dtype));
-    w.part = c.take<float>((size_t)DZ_SPLIT * p->out_dim);
+    const size_t n = p->dtype == FG_DTYPE_F32 ? 0
+                                              : std::max(tc_gemm_workspace(dx_shape(p, t, t.y)),
+                                                         tc_gemm_workspace(dw_shape(p, t, t.y)));
+    w.product = n ? c.take<char>(n) : nullptr;
+    w.dz = p->activation == FG_ACT_NONE ? nullptr : c.take<char>((size_t)p->rows * dz_stride(p) * dtype_size(p->dtype));
+    w.part = c.take<float>((size_t)dz_split(p->rows, p->out_dim, dtype_size(p->dtype)) * p->out_dim);
     return c.used;
 }
 
 template <class T>
 static int linear_backward(const fg_linear_params* p, const Strides& t, const void* dy, const void* x, const void* w,
                            const void* pre, void* dx, void* dw, void* dbias, const BackwardWs& ws, cudaStream_t s) {
-    const bool act = p->activation != FG_ACT_NONE;
-    const int split = (int)std::min<long long>(DZ_SPLIT, (p->rows + 7) / 8);
+    const bool act = p->activation != FG_ACT_NONE, store = act && (dx || dw);
+    const int split = p->rows ? dz_split(p->rows, p->out_dim, sizeof(T)) : 0;
     int rc;
-    if (split && (act || dbias)) {
-        dz_kernel<T><<<dim3((p->out_dim + DZ_COLS - 1) / DZ_COLS, split), 256, 0, s>>>(
-            (const T*)dy, t.y, (const T*)pre, t.p, p->activation, p->rows, p->out_dim, act ? (T*)ws.dz : nullptr,
-            dbias ? ws.part : nullptr);
-        if ((rc = check_launch("dz_kernel"))) return rc;
+    if (split && (store || dbias)) {
+        const DzArgs g{dy, act ? pre : nullptr, store ? ws.dz : nullptr, dbias ? ws.part : nullptr, t.y, t.p, p->rows, 0,
+                       p->out_dim, p->activation, 0};
+        if ((rc = launch_dz<T>(g, split, s))) return rc;
     }
     if (dbias) {
-        dz_reduce_kernel<T><<<(p->out_dim + 255) / 256, 256, 0, s>>>(ws.part, split, p->out_dim, (T*)dbias);
+        dz_reduce_kernel<T><<<(p->out_dim + 31) / 32, 1024, 0, s>>>(ws.part, split, p->out_dim, (T*)dbias);
         if ((rc = check_launch("dz_reduce_kernel"))) return rc;
     }
     const void* dz = act ? ws.dz : dy;
-    const long long ldz = act ? p->out_dim : t.y;
+    const long long ldz = act ? dz_stride(p) : t.y;
     Epilogue e{};
     if (dx && p->rows) {
         e.y = dx;
         e.ldy = p->in_dim;
-        rc = gemm<T>(dz, w, GemmShape{p->rows, p->in_dim, p->out_dim, ldz, 1, 1, t.w}, e, s);
+        rc = gemm<T>(dz, w, dx_shape(p, t, ldz), e, ws.product, s);
         if (rc) return rc;
     }
     if (dw) {
         e.y = dw;
         e.ldy = p->in_dim;
-        rc = gemm<T>(dz, x, GemmShape{p->out_dim, p->in_dim, p->rows, 1, ldz, 1, t.x}, e, s);
+        rc = gemm<T>(dz, x, dw_shape(p, t, ldz), e, ws.product, s);
         if (rc) return rc;
     }
     return FG_OK;
@@ -181,7 +298,7 @@ int fg_linear_workspace_size(const fg_linear_params* params, size_t* bytes) {
         Strides t;
         const int rc = linear_check(params, t);
         if (rc) return rc;
-        *bytes = 0;
+        *bytes = params->dtype == FG_DTYPE_F32 || params->rows == 0 ? 0 : tc_gemm_workspace(forward_shape(params, t));
         return FG_OK;
     });
 }
@@ -194,14 +311,16 @@ int fg_linear(const fg_linear_params* params, const void* x, const void* w, cons
         if (rc) return rc;
         if (params->rows == 0) return FG_OK;
         FG_REQUIRE(x && w && y, "null buffer");
-        (void)workspace;
-        (void)workspace_bytes;
-        const GemmShape g{params->rows, params->out_dim, params->in_dim, t.x, 1, t.w, 1};
+        const GemmShape g = forward_shape(params, t);
+        if (params->dtype != FG_DTYPE_F32 && tc_gemm_fits(x, w, g)) {
+            const int bad = adapter_ws(workspace, workspace_bytes, tc_gemm_workspace(g));
+            if (bad) return bad;
+        }
         const Epilogue e{bias, residual, pre, y, t.r, t.p, t.y, params->activation};
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        return params->dtype == FG_DTYPE_F32   ? gemm<float>(x, w, g, e, s)
-               : params->dtype == FG_DTYPE_F16 ? gemm<__half>(x, w, g, e, s)
-                                               : gemm<__nv_bfloat16>(x, w, g, e, s);
+        return params->dtype == FG_DTYPE_F32   ? gemm<float>(x, w, g, e, workspace, s)
+               : params->dtype == FG_DTYPE_F16 ? gemm<__half>(x, w, g, e, workspace, s)
+                                               : gemm<__nv_bfloat16>(x, w, g, e, workspace, s);
     });
 }
 
@@ -212,7 +331,7 @@ int fg_linear_backward_workspace_size(const fg_linear_params* params, size_t* by
         const int rc = linear_check(params, t);
         if (rc) return rc;
         BackwardWs w;
-        *bytes = backward_carve(params, nullptr, 0, w);
+        *bytes = backward_carve(params, t, nullptr, 0, w);
         return FG_OK;
     });
 }
@@ -230,9 +349,9 @@ int fg_linear_backward(const fg_linear_params* params, const void* dy, const voi
             FG_REQUIRE(params->activation == FG_ACT_NONE || pre, "the activation's gradient needs pre");
         }
         BackwardWs ws;
-        rc = adapter_ws(workspace, workspace_bytes, backward_carve(params, nullptr, 0, ws));
+        rc = adapter_ws(workspace, workspace_bytes, backward_carve(params, t, nullptr, 0, ws));
         if (rc) return rc;
-        backward_carve(params, workspace, workspace_bytes, ws);
+        backward_carve(params, t, workspace, workspace_bytes, ws);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         return params->dtype == FG_DTYPE_F32 ? linear_backward<float>(params, t, dy, x, w, pre, dx, dw, dbias, ws, s)
                : params->dtype == FG_DTYPE_F16

@@ -21,43 +21,58 @@ struct GemmShape {
 };
 
 // GELU = z Phi(z).  float32 results: CUDA's erfc, which keeps the small tail.
-// Results rounded to 16 bits (FAST): with a = |z| / sqrt(2), t = 1 / (1 + 0.3275911 a)
-// and e = exp(-a^2), erfc(a) = e t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) + 1.5e-7
-// (Abramowitz and Stegun 7.1.26): two special-function and a dozen other
-// operations, where erff would bound the epilogue.  e also serves the
-// derivative Phi(z) + z exp(-z^2 / 2) / sqrt(2 pi).
-__device__ __forceinline__ float upper_tail(float z, float& e) {  // Phi(-|z|)
-    const float t = __fdividef(1.0f, fmaf(fabsf(z), 0.3275911f * 0.70710678f, 1.0f));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * z * (-0.5f * 1.44269504f)));
-    float p = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
-    p = fmaf(t, p, 0.5f * 1.421413741f);
-    p = fmaf(t, p, 0.5f * -0.284496736f);
-    p = fmaf(t, p, 0.5f * 0.254829592f);
-    return p * t * e;
+// Results rounded to 16 bits (FAST): Abramowitz and Stegun's approximations of erfc
+// for x >= 0, which would lose nothing that such a result shows.
+//   7.1.28: (1 + a1 x + ... + a6 x^6)^-16, error 3e-7: one special-function
+//           operation a value, which with the other issues balances the epilogue
+//           (7.1.26 takes two: 4,096 cycles of a tile's 6,144 of products)
+//   7.1.26: exp(-x^2) t (a1 + ... + a5 t^4), t = 1 / (1 + 0.3275911 x), error
+//           1.5e-7: for the derivative, which needs the exponential as well
+// GELU of two values: max(z, 0) - a Phi(-a), a = min(|z|, 30) (Phi(-30) is 0).
+__device__ __forceinline__ void gelu2(float& z0, float& z1) {
+    const uint64_t a = pair2(fminf(fabsf(z0), 30.0f), fminf(fabsf(z1), 30.0f));
+    auto both = [](float c) { return pair2(c, c); };
+    // the coefficients times 2^(-k/2): of a = sqrt(2) x
+    uint64_t p = fma2(a, both(0.0000430638f * 0.125f), both(0.0002765672f * 0.17677670f));
+    p = fma2(a, p, both(0.0001520143f * 0.25f));
+    p = fma2(a, p, both(0.0092705272f * 0.35355339f));
+    p = fma2(a, p, both(0.0422820123f * 0.5f));
+    p = fma2(a, p, both(0.0705230784f * 0.70710678f));
+    p = fma2(a, p, both(1.0f));
+    p = mul2(p, p);
+    p = mul2(p, p);
+    p = mul2(p, p);
+    p = mul2(p, p);
+    float q0, q1, r0, r1;
+    unpair2(p, q0, q1);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(q0));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(q1));
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r0) : "f"(z0));
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r1) : "f"(z1));
+    unpair2(fma2(mul2(a, both(-0.5f)), pair2(q0, q1), pair2(r0, r1)), z0, z1);
 }
 
-// GELU of two values for results of 16 bits: max(z, 0) - a Phi(-a), a = min(|z|, 30)
-// (Phi(-30) is 0 in float32), the formula of upper_tail in 9 issues a value.
-__device__ __forceinline__ void gelu2(float& z0, float& z1) {
-    const float a0 = fminf(fabsf(z0), 30.0f), a1 = fminf(fabsf(z1), 30.0f);
-    const uint64_t a = pair2(a0, a1);
-    float d0, d1, m0, m1;
+// GELU's derivative Phi(z) + z phi(z) of two values, for results of 16 bits: z held
+// to [-30, 30] (a NaN stays), Phi(z) = 1/2 + sign(z) (1/2 - Phi(-|z|)).
+__device__ __forceinline__ void gelu_grad2(float& z0, float& z1) {
+    float c0, c1, d0, d1, m0, m1, q0, q1;
+    asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, 0fC1F00000;\n\tmin.NaN.f32 %0, t, 0f41F00000;\n\t}" : "=f"(c0) : "f"(z0));
+    asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, 0fC1F00000;\n\tmin.NaN.f32 %0, t, 0f41F00000;\n\t}" : "=f"(c1) : "f"(z1));
+    const uint64_t z = pair2(c0, c1), a = pair2(fabsf(c0), fabsf(c1));
     unpair2(fma2(a, pair2(0.3275911f * 0.70710678f, 0.3275911f * 0.70710678f), pair2(1.0f, 1.0f)), d0, d1);
     unpair2(mul2(mul2(a, a), pair2(-0.5f * 1.44269504f, -0.5f * 1.44269504f)), m0, m1);
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d0));
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d1));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(m0));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(m1));
-    const uint64_t t = pair2(d0, d1);
+    const uint64_t t = pair2(d0, d1), e = pair2(m0, m1);
     uint64_t p = fma2(t, pair2(-0.5f * 1.061405429f, -0.5f * 1.061405429f), pair2(0.5f * 1.453152027f, 0.5f * 1.453152027f));
     p = fma2(t, p, pair2(-0.5f * 1.421413741f, -0.5f * 1.421413741f));
     p = fma2(t, p, pair2(0.5f * 0.284496736f, 0.5f * 0.284496736f));
     p = fma2(t, p, pair2(-0.5f * 0.254829592f, -0.5f * 0.254829592f));
-    p = mul2(mul2(p, t), pair2(m0, m1));
-    float r0, r1;
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r0) : "f"(z0));
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r1) : "f"(z1));
-    unpair2(fma2(a, p, pair2(r0, r1)), z0, z1);
+    unpair2(fma2(mul2(p, t), e, pair2(0.5f, 0.5f)), q0, q1);  // 1/2 - Phi(-|z|)
+    const uint64_t phi = pair2(copysignf(q0, c0), copysignf(q1, c1));
+    unpair2(add2(fma2(mul2(z, e), pair2(0.39894228f, 0.39894228f), phi), pair2(0.5f, 0.5f)), z0, z1);
 }
 
 template <bool FAST>
@@ -89,11 +104,13 @@ __device__ __forceinline__ float activate_grad(float z, int act) {
     switch (act) {
         case FG_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
         case FG_ACT_GELU: {
+            if (FAST) {
+                float other = z;
+                gelu_grad2(z, other);
+                return z;
+            }
             const float zc = fminf(fmaxf(z, -100.0f), 100.0f);
-            if (!FAST) return fmaf(zc, expf(-0.5f * z * z) * 0.39894228f, 0.5f * erfcf(z * -0.70710678f));
-            float e;
-            const float q = upper_tail(z, e);
-            return fmaf(zc * 0.39894228f, e, z >= 0.0f ? 1.0f - q : q);
+            return fmaf(zc, expf(-0.5f * z * z) * 0.39894228f, 0.5f * erfcf(z * -0.70710678f));
         }
         case FG_ACT_SILU: {
             z = z < -100.0f ? -100.0f : z > 100.0f ? 100.0f : z;
@@ -116,6 +133,8 @@ __device__ __forceinline__ void epilogue_store(const Epilogue& e, long long m, l
 // Tensor-core product of 16-bit operands (linear_tc.cu).  tc_gemm_fits: the
 // operands' rows start on 16-byte boundaries, as their TMA loads need.
 bool tc_gemm_fits(const void* a, const void* b, const GemmShape& g);
-int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& g, const Epilogue& e, cudaStream_t s);
+// Its workspace (256-byte aligned) holds the partial tiles of a split product.
+size_t tc_gemm_workspace(const GemmShape& g);
+int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& g, const Epilogue& e, void* ws, cudaStream_t s);
 
 }  // namespace fg

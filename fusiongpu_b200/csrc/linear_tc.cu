@@ -19,7 +19,8 @@ struct TcArgs {
     int kt, mt, nt;     // K blocks, row tiles, column tiles
     int m, n;
     int a_mn, b_mn;
-    int split;          // CTAs of a cluster that share a tile's K range
+    int split;          // parts of a tile's K range: CTAs of a cluster, or passes of the pairs
+    int m_pad;          // pairs with split > 1: rows of a part's partial tiles
     int vec;            // outputs, residual and bias allow 4-column accesses
     uint32_t idesc;
     Epilogue e;
@@ -113,6 +114,10 @@ __global__ void __launch_bounds__(GT_NT, 1)
     const int m0 = tile / g.nt * GT_M, n0 = tile % g.nt * BN;
     const int kb0 = (int)((long long)g.kt * rank / S), kb1 = (int)((long long)g.kt * (rank + 1) / S);
 
+    if (warp == 2 && tc::elect_one()) {
+        tc::prefetch_map(&ta);
+        tc::prefetch_map(&tb);
+    }
     if (tid == 0) {
         s_fail = 0;
         for (int i = 0; i < Ring::N; ++i) {
@@ -133,7 +138,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
     volatile int* fail = &s_fail;
 
     if (warp == 0) {
-        if (lane == 0) {  // ---- TMA producer
+        if (tc::elect_one()) {  // ---- TMA producer
             int i = 0;
             bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb, ++i) {
@@ -159,23 +164,26 @@ __global__ void __launch_bounds__(GT_NT, 1)
                     tc::mbar_wait(&full[j % Ring::N], (j / Ring::N) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0) {  // ---- MMA issuer
-            bool ok = true;
-            int i = 0;
-            for (int kb = kb0; kb < kb1; ++kb, ++i) {
-                const int st = i % Ring::N;
-                if (!(ok = tc::mbar_wait_or_fail(&full[st], (i / Ring::N) & 1, fail))) break;
-                tc::fence_after_sync();
-                const unsigned char *sa = ring + st * Ring::STAGE, *sb = sa + Ring::A;
-                const uint64_t da = g.a_mn ? tc::desc_mnmajor_sw128(sa, 8192) : tc::desc_kmajor_sw128(sa);
-                const uint64_t db = g.b_mn ? tc::desc_mnmajor_sw128(sb, 8192) : tc::desc_kmajor_sw128(sb);
-                const uint32_t ka = g.a_mn ? 128 : 2, kbs = g.b_mn ? 128 : 2;  // 16 k, in 16-byte units
+        // ---- MMA issuer: the warp stays together, one elected lane issues
+        bool ok = true;
+        int i = 0;
+        const uint64_t da0 = g.a_mn ? tc::desc_mnmajor_sw128(ring, 8192) : tc::desc_kmajor_sw128(ring);
+        const uint64_t db0 = g.b_mn ? tc::desc_mnmajor_sw128(ring + Ring::A, 8192) : tc::desc_kmajor_sw128(ring + Ring::A);
+        const uint32_t ka = g.a_mn ? 128 : 2, kbs = g.b_mn ? 128 : 2;  // 16 k, in 16-byte units
+        for (int kb = kb0; kb < kb1; ++kb, ++i) {
+            const int st = i % Ring::N;
+            ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&full[st], (i / Ring::N) & 1, fail));
+            if (!ok) break;
+            tc::fence_after_sync();
+            const uint64_t da = da0 + st * (Ring::STAGE / 16), db = db0 + st * (Ring::STAGE / 16);
+            if (tc::elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < GT_K / 16; ++kk)
                     tc::umma_bf16(taddr, da + ka * kk, db + kbs * kk, g.idesc, (i | kk) != 0);
                 tc::umma_commit(&empty[st]);
+                if (kb + 1 == kb1) tc::umma_commit(&acc_full);
             }
-            if (ok) tc::umma_commit(&acc_full);
+            __syncwarp();
         }
     } else {  // ---- epilogue warps: TMEM -> partial tile in shared memory
         const int q4 = warp & 3, half = (warp - 2) >> 2;
@@ -353,8 +361,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     unsigned char* ring = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
     unsigned char* bufs = ring + GP_STAGES * P::STAGE;
-    const int pairs = (int)(gridDim.x >> 1), tiles = g.mt * g.nt;
+    const int pairs = (int)(gridDim.x >> 1), items = g.mt * g.nt * g.split;
+    auto k_begin = [&](int part) { return (int)((long long)g.kt * part / g.split); };
 
+    if (warp == 2 && tc::elect_one()) {
+        tc::prefetch_map(&ta);
+        tc::prefetch_map(&tb);
+        tc::prefetch_map(&ty);
+        if (g.e.pre) tc::prefetch_map(&tp);
+        if (g.e.residual) tc::prefetch_map(&tr);
+    }
     if (tid == 0) {
         s_fail = 0;
         for (int i = 0; i < GP_STAGES; ++i) {
@@ -377,12 +393,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     volatile int* fail = &s_fail;
 
     if (warp == 0) {
-        if (lane == 0) {  // ---- TMA producer (each CTA its own halves)
+        if (tc::elect_one()) {  // ---- TMA producer (each CTA its own halves)
             int i = 0;
             bool ok = true;
-            for (int t = blockIdx.x >> 1; t < tiles && ok; t += pairs) {
+            for (int w = blockIdx.x >> 1; w < items && ok; w += pairs) {
+                const int t = w / g.split, sp = w - t * g.split, k1 = k_begin(sp + 1);
                 const int m0 = t / g.nt * 2 * GT_M + rank * GT_M, n0 = t % g.nt * BN + rank * (BN / 2);
-                for (int kb = 0; kb < g.kt; ++kb, ++i) {
+                for (int kb = k_begin(sp); kb < k1; ++kb, ++i) {
                     const int st = i % GP_STAGES;
                     if (!(ok = tc::mbar_wait_or_fail(&empty[st], ((i / GP_STAGES) & 1) ^ 1, fail))) break;
                     unsigned char *sa = ring + st * P::STAGE, *sb = sa + GP_A;
@@ -407,28 +424,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     tc::mbar_wait(&full[j % GP_STAGES], (j / GP_STAGES) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {  // ---- MMA issuer of the pair
+        if (rank == 0) {  // ---- MMA issuer of the pair: the warp stays together, one elected lane issues
             int i = 0, li = 0;
             bool ok = true;
-            for (int t = blockIdx.x >> 1; t < tiles && ok; t += pairs, ++li) {
-                const int acc = li & 1;
-                if (!(ok = tc::mbar_wait_or_fail(&acc_empty[acc], ((li >> 1) & 1) ^ 1, fail))) break;
+            const uint64_t da0 = g.a_mn ? tc::desc_mnmajor_sw128(ring, 8192) : tc::desc_kmajor_sw128(ring);
+            const uint64_t db0 = g.b_mn ? tc::desc_mnmajor_sw128(ring + GP_A, 8192) : tc::desc_kmajor_sw128(ring + GP_A);
+            const uint32_t ka = g.a_mn ? 128 : 2, kbs = g.b_mn ? 128 : 2;
+            for (int w = blockIdx.x >> 1; w < items && ok; w += pairs, ++li) {
+                const int sp = w % g.split, k0 = k_begin(sp), k1 = k_begin(sp + 1), acc = li & 1;
+                ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&acc_empty[acc], ((li >> 1) & 1) ^ 1, fail));
+                if (!ok) break;
                 tc::fence_after_sync();
-                for (int kb = 0; kb < g.kt; ++kb, ++i) {
+                for (int kb = k0; kb < k1; ++kb, ++i) {
                     const int st = i % GP_STAGES;
-                    if (!(ok = tc::mbar_wait_or_fail(&full[st], (i / GP_STAGES) & 1, fail))) break;
+                    ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&full[st], (i / GP_STAGES) & 1, fail));
+                    if (!ok) break;
                     tc::fence_after_sync();
-                    const unsigned char *sa = ring + st * P::STAGE, *sb = sa + GP_A;
-                    const uint64_t da = g.a_mn ? tc::desc_mnmajor_sw128(sa, 8192) : tc::desc_kmajor_sw128(sa);
-                    const uint64_t db = g.b_mn ? tc::desc_mnmajor_sw128(sb, 8192) : tc::desc_kmajor_sw128(sb);
-                    const uint32_t ka = g.a_mn ? 128 : 2, kbs = g.b_mn ? 128 : 2;
+                    const uint64_t da = da0 + st * (P::STAGE / 16), db = db0 + st * (P::STAGE / 16);
+                    if (tc::elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < GT_K / 16; ++kk)
-                        tc::umma_pair(taddr + (uint32_t)(acc * BN), da + ka * kk, db + kbs * kk, g.idesc,
-                                      (kb | kk) != 0);
-                    tc::umma_commit_pair(&empty[st]);
+                        for (int kk = 0; kk < GT_K / 16; ++kk)
+                            tc::umma_pair(taddr + (uint32_t)(acc * BN), da + ka * kk, db + kbs * kk, g.idesc,
+                                          kb != k0 || kk != 0);
+                        tc::umma_commit_pair(&empty[st]);
+                        if (kb + 1 == k1) tc::umma_commit_pair(&acc_full[acc]);
+                    }
+                    __syncwarp();
                 }
-                if (ok) tc::umma_commit_pair(&acc_full[acc]);
             }
         }
     } else {  // ---- epilogue warps
@@ -444,10 +466,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             tc::tma_load_2d(buf, &tr, &res_full[w], t % g.nt * BN + part * 64, t / g.nt * 2 * GT_M + tr_rows);
         };
         const int step = pairs * P::GROUPS;
-        int t = (blockIdx.x >> 1) + pairs * group, li = group;
-        if (e.residual && !e.pre && t < tiles && lane == 0) fetch_residual(t);
-        for (; t < tiles; t += step, li += P::GROUPS) {
-            const int acc = li & 1;
+        int item = (blockIdx.x >> 1) + pairs * group, li = group;
+        if (e.residual && !e.pre && item < items && tc::elect_one()) fetch_residual(item);
+        for (; item < items; item += step, li += P::GROUPS) {
+            const int acc = li & 1, t = item / g.split;
             const int col = t % g.nt * BN + part * 64, m0 = t / g.nt * 2 * GT_M + tr_rows;
             const bool inside = m0 < g.m && col < g.n;
             const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
@@ -460,7 +482,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             tc::tmem_ld_wait(v[1]);
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
+            if (tc::elect_one()) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
+            if (g.split > 1) {  // this part's sums as they are; finish_kernel adds the parts
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (tc::elect_one()) tc::bulk_wait_read<0>();
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<float4*>(brow + (((uint32_t)j << 2) ^ sw)) =
+                            ok ? make_float4(v[h][j], v[h][j + 1], v[h][j + 2], v[h][j + 3])
+                               : make_float4(NAN, NAN, NAN, NAN);
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                    if (tc::elect_one()) {
+                        if (col + 32 * h < g.n)
+                            tc::tma_store_2d(&ty, buf, col + 32 * h, (item - t * g.split) * g.m_pad + m0);
+                        tc::bulk_commit();
+                    }
+                }
+                continue;
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (!ok) {  // a wait that ran out leaves NaN, not a plausible number
@@ -470,7 +512,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 if (e.bias) add_bias<T>(v[h], static_cast<const T*>(e.bias) + col + 32 * h, g.n - col - 32 * h);
             }
             if (e.pre) {
-                if (lane == 0) tc::bulk_wait_read<0>();
+                if (tc::elect_one()) tc::bulk_wait_read<0>();
                 __syncwarp();
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -479,7 +521,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         *reinterpret_cast<uint4*>(brow + (((uint32_t)(32 * h + j) << 1) ^ sw)) = pack8<T>(&v[h][j]);
                 tc::fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) {
+                if (tc::elect_one()) {
                     if (inside) tc::tma_store_2d(&tp, buf, col, m0);
                     tc::bulk_commit();
                 }
@@ -490,7 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 case FG_ACT_SILU: activate_all<FG_ACT_SILU>(v); break;
             }
             if (e.pre || !e.residual) {  // the buffer's last store has read it
-                if (lane == 0) {
+                if (tc::elect_one()) {
                     tc::bulk_wait_read<0>();
                     if (e.residual) fetch_residual(t);
                 }
@@ -512,22 +554,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     *reinterpret_cast<uint4*>(brow + (((uint32_t)(32 * h + j) << 1) ^ sw)) = pack8<T>(&v[h][j]);
             tc::fence_proxy_async();
             __syncwarp();
-            if (lane == 0) {
+            if (tc::elect_one()) {
                 if (inside) tc::tma_store_2d(&ty, buf, col, m0);
                 tc::bulk_commit();
-                if (e.residual && !e.pre && t + step < tiles) {  // the next tile's residual travels during its products
+                if (e.residual && !e.pre && item + step < items) {  // the next tile's residual travels during its products
                     tc::bulk_wait_read<0>();
-                    fetch_residual(t + step);
+                    fetch_residual(item + step);
                 }
             }
         }
-        if (lane == 0) tc::bulk_wait_read<0>();
+        if (tc::elect_one()) tc::bulk_wait_read<0>();
     }
     tc::fence_before_sync();
     __syncthreads();
     cluster_sync();  // no CTA leaves while its peer still reads its memory
     tc::fence_after_sync();
     if (warp == 1) tc::tmem_dealloc_pair(taddr, 2 * BN);
+}
+
+// The parts of split tiles, added in their order, and the epilogue: four columns a thread.
+template <class T>
+__global__ void __launch_bounds__(256) finish_kernel(const float* part, const TcArgs g, long long ldp) {
+    const int c4 = (g.n + 3) / 4;
+    const long long i = blockIdx.x * 256ll + threadIdx.x, row = i / c4;
+    if (row >= g.m) return;
+    const int col = (int)(i - row * c4) * 4;
+    const float* p = part + row * ldp + col;
+    float4 z = *reinterpret_cast<const float4*>(p);
+    for (int s = 1; s < g.split; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(p + s * (g.m_pad * ldp));
+        z.x += v.x;
+        z.y += v.y;
+        z.z += v.z;
+        z.w += v.w;
+    }
+    const float v[4] = {z.x, z.y, z.z, z.w};
+    if (g.vec && col + 4 <= g.n && !g.e.bias && !g.e.pre && !g.e.residual && g.e.act == FG_ACT_NONE)
+        store4(static_cast<T*>(g.e.y) + row * g.e.ldy + col, z);
+    else
+        for (int j = 0; j < 4 && col + j < g.n; ++j) epilogue_store<T>(g.e, row, col + j, v[j]);
 }
 
 // ---- host side ---------------------------------------------------------------
@@ -596,29 +661,110 @@ static int tile_map(CUtensorMap* m, int dtype, const void* p, long long rows, lo
     return operand_map(m, dtype, p, rows, n, ld, false, 32);
 }
 
+// Partial tiles [split][m_pad][n, padded to 4] of fp32, for the TMA stores of the pairs.
+static int part_map(CUtensorMap* m, const void* p, const TcArgs& g, long long ld) {
+    tc::EncodeTiledFn enc = tc::encode_fn();
+    if (!enc) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    cuuint64_t dims[2] = {(cuuint64_t)ld, (cuuint64_t)g.split * g.m_pad};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 4};
+    cuuint32_t box[2] = {32, 32};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(p), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return FG_OK;
+}
+
 template <class T, int BN>
-static int launch_pair(int dtype, const void* a, const void* b, const GemmShape& s, TcArgs g, cudaStream_t st) {
+static int launch_pair(int dtype, const void* a, const void* b, const GemmShape& s, TcArgs g, void* ws, cudaStream_t st) {
     CUtensorMap ta, tb, ty = {}, tp = {}, tr = {};
     const Epilogue& e = g.e;
-    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M);
-    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN / 2);
-    if (!rc) rc = tile_map(&ty, dtype, e.y, s.m, s.n, e.ldy);
-    if (!rc) rc = tile_map(&tp, dtype, e.pre, s.m, s.n, e.ldp);
-    if (!rc) rc = tile_map(&tr, dtype, e.residual, s.m, s.n, e.ldr);
-    if (rc) return rc;
-    g.idesc = instr_desc(dtype, 2 * GT_M, BN, g.a_mn, g.b_mn);
+    const long long ld = (s.n + 3) / 4 * 4;
     g.mt = (g.m + 2 * GT_M - 1) / (2 * GT_M);
     g.nt = (g.n + BN - 1) / BN;
-    const long long tiles = (long long)g.mt * g.nt;
-    FG_REQUIRE(tiles <= 0x3fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
+    g.m_pad = g.mt * 2 * GT_M;
+    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M);
+    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN / 2);
+    if (g.split > 1) {
+        if (!rc) rc = part_map(&ty, ws, g, ld);
+    } else {
+        if (!rc) rc = tile_map(&ty, dtype, e.y, s.m, s.n, e.ldy);
+        if (!rc) rc = tile_map(&tp, dtype, e.pre, s.m, s.n, e.ldp);
+        if (!rc) rc = tile_map(&tr, dtype, e.residual, s.m, s.n, e.ldr);
+    }
+    if (rc) return rc;
+    g.idesc = instr_desc(dtype, 2 * GT_M, BN, g.a_mn, g.b_mn);
+    const long long items = (long long)g.mt * g.nt * g.split;
+    FG_REQUIRE(items <= 0x3fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
     auto kernel = &gemm_pair_kernel<T, BN>;
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), PairOf<BN>::SMEM));
     const int pairs = std::max(1, device_attr(cudaDevAttrMultiProcessorCount) / 2);
-    kernel<<<2 * (unsigned)std::min<long long>(tiles, pairs), GP_NT, PairOf<BN>::SMEM, st>>>(ta, tb, ty, tp, tr, g);
-    return check_launch("gemm_pair_kernel");
+    TcArgs k = g;
+    if (g.split > 1) k.e.residual = k.e.pre = nullptr;
+    kernel<<<2 * (unsigned)std::min<long long>(items, pairs), GP_NT, PairOf<BN>::SMEM, st>>>(ta, tb, ty, tp, tr, k);
+    rc = check_launch("gemm_pair_kernel");
+    if (rc || g.split == 1) return rc;
+    const long long n4 = (long long)g.m * ((g.n + 3) / 4);
+    finish_kernel<T><<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(static_cast<const float*>(ws), g, ld);
+    return check_launch("finish_kernel");
 }
 
-int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& s, const Epilogue& e, cudaStream_t st) {
+// The kernel, tile width and split that finish first by this estimate in
+// microseconds, fitted to runs of 1 to 7 waves of each (within 15 %): a K block takes
+// a pair 0.39 (256 columns; 512 cycles of products) or 0.34 (128), a CTA of the
+// other kernel 0.43, 0.30 or 0.21 (256, 128, 64); a tile's epilogue runs behind the
+// next tile's products in the pair kernel, after them in the other.  Parts of a tile
+// meet in distributed shared memory (clusters, of which 74, 32 and 14 of two, four
+// and eight CTAs run at once) or, with pairs, in the workspace and one more launch.
+// 10,000 x 768 -> 1536: forward pairs 256 26 us (128: 36; one CTA a tile: 65), dw in
+// 4 parts of pairs 29 us (2 parts 38, clusters of 4 45); 100 x 1536 -> 768: clusters
+// of 4, 64 columns, 8.3 us (unsplit 12, pairs 10).
+struct TcPlan {
+    bool pair;
+    int bn, split;
+    size_t ws;
+};
+
+static TcPlan tc_plan(const GemmShape& s, bool pairs_fit) {
+    const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
+    const int kt = (int)((s.k + GT_K - 1) / GT_K);
+    auto waves = [](long long tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
+    TcPlan best{false, 256, 1, 0};
+    double least = 1e300;
+    auto offer = [&](double cost, const TcPlan& p) {
+        if (cost < least) {
+            least = cost;
+            best = p;
+        }
+    };
+    const long long m2 = (s.m + 2 * GT_M - 1) / (2 * GT_M), m1 = (s.m + GT_M - 1) / GT_M;
+    for (int bn : {256, 128}) {
+        if (!pairs_fit) break;
+        const long long tiles = m2 * ((s.n + bn - 1) / bn);
+        for (int sp : {1, 2, 4, 8, 16}) {
+            if (sp > 1 && (sp > kt / 2 || tiles * sp > sms)) break;
+            const size_t ws = sp > 1 ? (size_t)sp * m2 * 2 * GT_M * ((s.n + 3) / 4 * 4) * 4 : 0;
+            const double epi = bn == 256 ? 2.0 : 1.0, main = (kt + sp - 1) / sp * (bn == 256 ? 0.39 : 0.34);
+            offer(6.0 + waves(tiles * sp, sms / 2) * std::max(main, epi) + epi + (sp > 1 ? 3.0 + 1.5e-6 * ws / 6.0 : 0.0),
+                  TcPlan{true, bn, sp, ws});
+        }
+    }
+    for (int bn : {256, 128, 64}) {
+        const long long tiles = m1 * ((s.n + bn - 1) / bn);
+        for (int sp : {1, 2, 4, 8}) {
+            if (sp > kt) break;
+            const int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
+            const double main = (kt + sp - 1) / sp * (bn == 256 ? 0.43 : bn == 128 ? 0.30 : 0.21);
+            offer(5.0 + waves(tiles, slots) * (main + 2.0 + 0.02 * bn / sp) + (sp == 8 ? 0.7 : 0.0), TcPlan{false, bn, sp, 0});
+        }
+    }
+    return best;
+}
+
+size_t tc_gemm_workspace(const GemmShape& s) { return s.k > 0 ? tc_plan(s, true).ws : 0; }
+
+int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& s, const Epilogue& e, void* ws, cudaStream_t st) {
     TcArgs g{};
     g.m = (int)s.m;
     g.n = (int)s.n;
@@ -630,52 +776,14 @@ int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& s, const E
     auto lies = [&](const void* p, long long ld, int bytes) { return !p || (aligned(p, bytes) && ld * 2 % bytes == 0); };
     g.vec = lies(e.y, e.ldy, 8) && lies(e.bias, 0, 8) && lies(e.pre, e.ldp, 8) && lies(e.residual, e.ldr, 8);
     const bool tma_out = lies(e.y, e.ldy, 16) && lies(e.bias, 0, 16) && lies(e.pre, e.ldp, 16) && lies(e.residual, e.ldr, 16);
-    // The kernel, tile width and split that finish first by this estimate of SM
-    // cycles.  A K block takes its MMAs (2 x width) or, when many CTAs ask at once,
-    // L2's delivery of their operands: 5,900 bytes a cycle over the GPU (measured:
-    // 11 TB/s, 800 cycles a block for 74 pairs of 256 x 256 tiles, which so reach
-    // 1,450 TFLOP/s; 256 x 128 tiles need 600).  A tile's epilogue runs behind the
-    // next tile's products in the pair kernel, after them in the other.
-    const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
-    auto estimate = [&](long long tiles, int slots, int ctas_per_tile, int bytes, int bn, int blocks, double epi, bool behind) {
-        auto wave = [&](double active) { return blocks * std::max(2.0 * bn, bytes * active * ctas_per_tile / 5900.0); };
-        const double full = (double)(tiles / slots), rest = (double)(tiles % slots);
-        const double w = wave(slots), last = rest > 0 ? wave(rest) : 0.0;
-        if (!behind) return full * (w + epi) + (rest > 0 ? last + epi : 0.0);
-        return full * std::max(w, epi) + (rest > 0 ? std::max(last, epi) : 0.0) + epi;
-    };
-    int best_n = 256;
-    bool pair = false;
-    double best = 1e300;
-    for (int bn : {256, 128}) {
-        if (!tma_out) break;
-        const long long tiles = (s.m + 2 * GT_M - 1) / (2 * GT_M) * ((g.n + bn - 1) / bn);
-        const double cost = 5000 + estimate(tiles, sms / 2, 2, GP_A + bn * GT_K, bn, g.kt, 16.0 * bn, true);
-        if (cost < best) {
-            best = cost;
-            best_n = bn;
-            pair = true;
-        }
-    }
-    for (int bn : {256, 128, 64}) {
-        const long long tiles = (long long)g.mt * ((g.n + bn - 1) / bn);
-        for (int sp : {1, 2, 4, 8}) {
-            if (sp > g.kt) break;
-            const double epi = 3000 + 25.0 * bn / sp + 4.0 * bn + (sp > 1 ? 1000 + 100 * sp : 0);
-            const double cost = 3000 + estimate(tiles, sms / sp, sp, GP_A + bn * GT_K * 2, bn, (g.kt + sp - 1) / sp, epi, false);
-            if (cost < best) {
-                best = cost;
-                best_n = bn;
-                pair = false;
-                g.split = sp;
-            }
-        }
-    }
-#define FG_PRODUCT(T)                                                                       \
-    (pair ? (best_n == 256 ? launch_pair<T, 256>(dtype, a, b, s, g, st)                     \
-                           : launch_pair<T, 128>(dtype, a, b, s, g, st))                    \
-          : (best_n == 256   ? launch_split<T, 256>(dtype, a, b, s, g, st)                  \
-             : best_n == 128 ? launch_split<T, 128>(dtype, a, b, s, g, st)                  \
+    TcPlan p = tc_plan(s, true);
+    if (p.pair && p.split == 1 && !tma_out) p = tc_plan(s, false);
+    g.split = p.split;
+#define FG_PRODUCT(T)                                                                     \
+    (p.pair ? (p.bn == 256 ? launch_pair<T, 256>(dtype, a, b, s, g, ws, st)               \
+                           : launch_pair<T, 128>(dtype, a, b, s, g, ws, st))              \
+            : (p.bn == 256   ? launch_split<T, 256>(dtype, a, b, s, g, st)                \
+               : p.bn == 128 ? launch_split<T, 128>(dtype, a, b, s, g, st)                \
                              : launch_split<T, 64>(dtype, a, b, s, g, st)))
     return dtype == FG_DTYPE_F16 ? FG_PRODUCT(__half) : FG_PRODUCT(__nv_bfloat16);
 #undef FG_PRODUCT

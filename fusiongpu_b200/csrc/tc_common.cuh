@@ -58,6 +58,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32
     return false;
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 // 2-D tiled TMA load into shared memory, completing on `bar` (no multicast).
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
     asm volatile(
@@ -96,6 +100,19 @@ __device__ __forceinline__ void fence_before_sync() {
 
 __device__ __forceinline__ void fence_after_sync() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+
+// One lane of a converged warp.  Code under it is known to run in one thread, so the
+// tensor and TMA instructions in it take their operands from uniform registers;
+// under `lane == 0` each costs about 100 cycles more.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, e;\n\t}\n"
+        : "=r"(p));
+    return p != 0;
 }
 
 // ---- CTA pairs (cta_group::2): one MMA over both CTAs' shared and tensor memory ----

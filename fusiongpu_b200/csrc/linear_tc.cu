@@ -298,7 +298,7 @@ constexpr int GP_NT = 64 + GP_EPI * 32;
 template <int BN>
 struct PairOf {
     static constexpr int B = BN / 2 * GT_K * 2, STAGE = GP_A + B;
-    static constexpr int SMEM = GP_STAGES * STAGE + GP_EPI * GP_BUF + 1024;
+    static constexpr int SMEM = GP_STAGES * STAGE + GP_EPI * (GP_BUF + 128);
     static constexpr int WARPS = BN / 64 * 4;         // epilogue warps of a tile
     static constexpr int GROUPS = GP_EPI / WARPS;     // that take tiles in turn
 };
@@ -333,17 +333,22 @@ __device__ __forceinline__ void activate_all(float (&v)[2][32]) {
         }
 }
 
-// 32 columns of the bias, the same for every lane; `left` of them exist.
+// Columns 2 lane and 2 lane + 1 of a 64-column piece of the bias, packed; fetched
+// before the accumulator is waited for (the operand ring leaves no L1 to find it in).
 template <class T>
-__device__ __forceinline__ void add_bias(float (&v)[32], const T* b, int left) {
-    if (left >= 32) {
+__device__ __forceinline__ uint32_t fetch_bias(const T* b, int lane, int left) {
+    if (2 * lane + 2 <= left) return __ldg(reinterpret_cast<const unsigned*>(b) + lane);
+    uint32_t u = 0;
+    if (2 * lane < left) u = *reinterpret_cast<const unsigned short*>(b + 2 * lane);
+    return u;
+}
+
+template <class T>
+__device__ __forceinline__ void add_bias(float (&v)[2][32], const unsigned char* b) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) add8<T>(&v[j], __ldg(reinterpret_cast<const uint4*>(b + j)));
-    } else {
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < left) v[j] += to_f32(b[j]);
-    }
+        for (int j = 0; j < 32; j += 8) add8<T>(&v[h][j], *reinterpret_cast<const uint4*>(b + (32 * h + j) * 2));
 }
 
 template <class T, int BN>
@@ -358,9 +363,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     __shared__ int s_fail;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)cluster_rank();
-    unsigned char* ring = reinterpret_cast<unsigned char*>(
-        (reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
-    unsigned char* bufs = ring + GP_STAGES * P::STAGE;
+    unsigned char *ring = dsmem, *bufs = ring + GP_STAGES * P::STAGE, *biases = bufs + GP_EPI * GP_BUF;
     const int pairs = (int)(gridDim.x >> 1), items = g.mt * g.nt * g.split;
     auto k_begin = [&](int part) { return (int)((long long)g.kt * part / g.split); };
 
@@ -384,6 +387,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
         for (int w = 0; w < GP_EPI; ++w) tc::mbar_init(&res_full[w], 1);
         tc::fence_mbar_init();
     }
+    if (tid == 0 && (tc::smem_u32(dsmem) & 1023)) s_fail = 1;  // swizzled tiles start on 1,024 bytes
     if (warp == 1) tc::tmem_alloc_pair(&tmem_slot, 2 * BN);
     tc::fence_before_sync();
     __syncthreads();
@@ -472,6 +476,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             const int acc = li & 1, t = item / g.split;
             const int col = t % g.nt * BN + part * 64, m0 = t / g.nt * 2 * GT_M + tr_rows;
             const bool inside = m0 < g.m && col < g.n;
+            unsigned char* bias = biases + w * 128;
+            if (e.bias) {
+                reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(static_cast<const T*>(e.bias) + col, lane, g.n - col);
+                __syncwarp();
+            }
             const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
             tc::fence_after_sync();
             const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + part * 64);
@@ -509,8 +518,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[h][j] = NAN;
                 }
-                if (e.bias) add_bias<T>(v[h], static_cast<const T*>(e.bias) + col + 32 * h, g.n - col - 32 * h);
             }
+            if (e.bias) add_bias<T>(v, bias);
             if (e.pre) {
                 if (tc::elect_one()) tc::bulk_wait_read<0>();
                 __syncwarp();

@@ -133,8 +133,10 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
         : "memory");
 }
 
+// For barriers that order tensor memory alone (after fence_before_sync): relaxed,
+// since a release at cluster scope waits for the thread's stores, about 1,000 cycles.
 __device__ __forceinline__ void mbar_arrive_leader(uint32_t leader_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_bar) : "memory");
 }
 
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) {

@@ -105,8 +105,9 @@ def _norm_ws(n: int, d: int, device: int) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-def _linear_ws(query: str, n: int, i: int, o: int, dtype: int, act: int, device: int) -> int:
-    return _lib.size_query(query, C.byref(_lib.LinearParams(n, i, o, dtype, act, 0, 0, 0, 0, 0)))
+def _linear_ws(query: str, n: int, i: int, o: int, dtype: int, act: int, ldx: int, ldw: int, ldy: int,
+               device: int) -> int:
+    return _lib.size_query(query, C.byref(_lib.LinearParams(n, i, o, dtype, act, ldx, ldw, 0, 0, ldy)))
 
 
 @_on
@@ -183,7 +184,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, a
     y = x.new_empty((n, o))
     pre = x.new_empty((n, o)) if return_pre else None
     p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, ldr, 0, 0)
-    nws = _linear_ws("fg_linear_workspace_size", n, i, o, t, act, dev.index)
+    nws = _linear_ws("fg_linear_workspace_size", n, i, o, t, act, ldx, ldw, 0, dev.index)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
     _lib.check(_lib.lib().fg_linear(C.byref(p), x.data_ptr(), w.data_ptr(), b, _ptr(residual), _ptr(pre),
                                     y.data_ptr(), _ptr(ws), nws, _stream(x)), "fg_linear")
@@ -213,7 +214,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: tor
     dx = x.new_empty((n, i)) if input_grad else None
     dw, db = (x.new_empty((o, i)), x.new_empty(o)) if param_grads else (None, None)
     p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, 0, ldp, lddy)
-    nws = _linear_ws("fg_linear_backward_workspace_size", n, i, o, t, act, dev.index)
+    nws = _linear_ws("fg_linear_backward_workspace_size", n, i, o, t, act, ldx, ldw, lddy, dev.index)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
     _lib.check(_lib.lib().fg_linear_backward(C.byref(p), dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(pre),
                                              _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nws, _stream(x)),

@@ -53,14 +53,177 @@ __global__ void __launch_bounds__(256) gemm_simt_kernel(const T* a, const T* b, 
         }
 }
 
+static int simt_gemm_check(const GemmShape& g, long long* tiles) {
+    *tiles = ((g.m + SG_T - 1) / SG_T) * ((g.n + SG_T - 1) / SG_T);
+    FG_REQUIRE(*tiles <= 0x7fffffffll, "%lld x %lld outputs: too many tiles", g.m, g.n);
+    return FG_OK;
+}
+
+// ---- operands as the tensor cores take them ------------------------------------
+//
+// A matrix whose rows do not start on 16-byte boundaries is copied to one whose rows
+// do; a float32 matrix becomes three bf16 planes, x = x0 + x1 + x2, each the rounding
+// of what the ones before leave (a value past bf16's range is cut instead, an infinity
+// or NaN has zeros behind it).  One pass over memory, eight columns a thread.
+struct PackJob {
+    const void* in;
+    void* out;
+    long long rows, ld, plane;
+    int cols;
+};
+struct PackArgs {
+    PackJob job[2];
+    int jobs;
+};
+
+__host__ __device__ inline long long pack_stride(long long cols) { return (cols + 7) / 8 * 8; }
+
+__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
+    p[0] = from_f32<__nv_bfloat16>(x);
+    const bool finite = fabsf(x) <= FLT_MAX;
+    if (finite && !(fabsf(to_f32(p[0])) <= FLT_MAX)) p[0] = from_f32<__nv_bfloat16>(__uint_as_float(__float_as_uint(x) & 0xffff0000u));
+    const float r = x - to_f32(p[0]);
+    p[1] = from_f32<__nv_bfloat16>(finite ? r : 0.0f);
+    p[2] = from_f32<__nv_bfloat16>(finite ? r - to_f32(p[1]) : 0.0f);
+}
+
 template <class T>
-static int gemm(const void* a, const void* b, const GemmShape& g, const Epilogue& e, void* ws, cudaStream_t s) {
-    const long long tiles = ((g.m + SG_T - 1) / SG_T) * ((g.n + SG_T - 1) / SG_T);
-    FG_REQUIRE(tiles <= 0x7fffffffll, "%lld x %lld outputs: too many tiles", g.m, g.n);
-    if (tiles == 0) return FG_OK;
-    if (sizeof(T) == 2 && tc_gemm_fits(a, b, g))
-        return tc_gemm(std::is_same<T, __half>::value ? FG_DTYPE_F16 : FG_DTYPE_BF16, a, b, g, e, ws, s);
-    gemm_simt_kernel<T><<<(unsigned)tiles, 256, 0, s>>>(static_cast<const T*>(a), static_cast<const T*>(b), g, e);
+__global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
+    long long i = blockIdx.x * 256ll + threadIdx.x;
+    for (int k = 0; k < a.jobs; ++k) {
+        const PackJob& j = a.job[k];
+        const long long per_row = pack_stride(j.cols) / 8, n = j.rows * per_row;
+        if (i >= n) {
+            i -= n;
+            continue;
+        }
+        const long long row = i / per_row;
+        const int col = (int)(i - row * per_row) * 8, left = j.cols - col;
+        const T* in = static_cast<const T*>(j.in) + row * j.ld + col;
+        alignas(16) T v[8];
+        if (sizeof(T) == 4 && left >= 8 && (reinterpret_cast<uintptr_t>(in) & 15) == 0) {
+            reinterpret_cast<uint4*>(v)[0] = reinterpret_cast<const uint4*>(in)[0];
+            reinterpret_cast<uint4*>(v)[sizeof(T) / 4] = reinterpret_cast<const uint4*>(in)[sizeof(T) / 4];
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] = c < left ? in[c] : from_f32<T>(0.0f);
+        }
+        if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<uint4*>(static_cast<T*>(j.out) + row * pack_stride(j.cols) + col) = *reinterpret_cast<uint4*>(v);
+        } else {
+            alignas(16) __nv_bfloat16 o[3][8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                __nv_bfloat16 p[3];
+                split3(v[c], p);
+                o[0][c] = p[0];
+                o[1][c] = p[1];
+                o[2][c] = p[2];
+            }
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(j.out) + row * pack_stride(j.cols) + col;
+#pragma unroll
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(out + q * j.plane) = *reinterpret_cast<const uint4*>(o[q]);
+        }
+        return;
+    }
+}
+
+// An operand on its way to a product: as it lies, or packed into the workspace.
+struct Operand {
+    const void* p;
+    long long ld, plane;  // elements
+};
+
+static bool needs_pack(int dtype, long long ld) { return dtype == FG_DTYPE_F32 || ld % 8 != 0; }
+static size_t pack_bytes(int dtype, long long rows, long long cols) {
+    return (size_t)rows * pack_stride(cols) * 2 * (dtype == FG_DTYPE_F32 ? 3 : 1);
+}
+
+template <class T>
+static int pack(const PackArgs& a, cudaStream_t s) {
+    long long n = 0;
+    for (int k = 0; k < a.jobs; ++k) n += a.job[k].rows * (pack_stride(a.job[k].cols) / 8);
+    if (n == 0) return FG_OK;
+    FG_REQUIRE(n <= 0x7fffffffll * 256, "operands too large");
+    pack_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    return check_launch("pack_kernel");
+}
+
+// ---- a few rows: the weights are read once ---------------------------------------
+//
+// A warp takes one output column for all R rows: 32 lanes along k, 16 bytes a lane
+// where the rows allow, then R sums over the warp.  Bound by the weights' bytes; at
+// one row of 768 x 1536 f16 GEMVFIG
+template <class T, int R>
+__global__ void __launch_bounds__(128) gemv_kernel(const T* __restrict__ x, const T* __restrict__ w, const GemmShape g,
+                                                   int wide, const Epilogue e) {
+    constexpr int VEC = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31;
+    const long long n = blockIdx.x * 4ll + (threadIdx.x >> 5);
+    if (n >= g.n) return;
+    const T* wr = w + n * g.bn;
+    float acc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = 0.0f;
+    long long k0 = 0;
+    if (wide) {
+#pragma unroll 4
+        for (long long k = lane * VEC; k + VEC <= g.k; k += 32 * VEC) {
+            alignas(16) T a[VEC], b[VEC];
+            *reinterpret_cast<uint4*>(b) = *reinterpret_cast<const uint4*>(wr + k);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if (r >= g.m) break;
+                *reinterpret_cast<uint4*>(a) = *reinterpret_cast<const uint4*>(x + r * g.am + k);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[r] = fmaf(to_f32(a[i]), to_f32(b[i]), acc[r]);
+            }
+        }
+        k0 = g.k / VEC * VEC;
+    }
+    for (long long k = k0 + lane; k < g.k; k += 32) {
+        const float b = to_f32(wr[k]);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r < g.m) acc[r] = fmaf(to_f32(x[r * g.am + k]), b, acc[r]);
+    }
+    float z = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float t = warp_sum(acc[r]);
+        if (lane == r) z = t;
+    }
+    if (lane < g.m) epilogue_store<T>(e, lane, n, z);
+}
+
+constexpr int GEMV_ROWS = 8;
+
+template <class T>
+static int gemv(const void* x, const void* w, const GemmShape& g, const Epilogue& e, cudaStream_t s) {
+    const T *xp = static_cast<const T*>(x), *wp = static_cast<const T*>(w);
+    auto lies = [&](const void* p, long long ld) { return aligned(p, 16) && ld * (int)sizeof(T) % 16 == 0; };
+    const int wide = lies(x, g.am) && lies(w, g.bn);
+    const unsigned blocks = (unsigned)((g.n + 3) / 4);
+    if (g.m == 1)
+        gemv_kernel<T, 1><<<blocks, 128, 0, s>>>(xp, wp, g, wide, e);
+    else if (g.m == 2)
+        gemv_kernel<T, 2><<<blocks, 128, 0, s>>>(xp, wp, g, wide, e);
+    else if (g.m <= 4)
+        gemv_kernel<T, 4><<<blocks, 128, 0, s>>>(xp, wp, g, wide, e);
+    else
+        gemv_kernel<T, GEMV_ROWS><<<blocks, 128, 0, s>>>(xp, wp, g, wide, e);
+    return check_launch("gemv_kernel");
+}
+
+template <class T>
+static int gemm(const Operand& a, const Operand& b, const GemmShape& g, const Epilogue& e, void* ws, cudaStream_t s) {
+    if (g.m == 0 || g.n == 0) return FG_OK;
+    constexpr int dtype = sizeof(T) == 4 ? FG_DTYPE_F32 : std::is_same<T, __half>::value ? FG_DTYPE_F16 : FG_DTYPE_BF16;
+    if ((sizeof(T) == 2 || a.plane) && tc_gemm_fits(a.p, b.p, g)) return tc_gemm(dtype, a.p, a.plane, b.p, b.plane, g, e, ws, s);
+    long long tiles;
+    const int rc = simt_gemm_check(g, &tiles);
+    if (rc) return rc;
+    gemm_simt_kernel<T><<<(unsigned)tiles, 256, 0, s>>>(static_cast<const T*>(a.p), static_cast<const T*>(b.p), g, e);
     return check_launch("gemm_simt_kernel");
 }
 
@@ -74,7 +237,7 @@ struct DzArgs {
     const void *dy, *pre;
     void* dz;     // NULL: not stored
     float* part;  // NULL: no sums
-    long long lddy, ldp, rows, per;
+    long long lddy, ldp, rows, per, plane;
     int dim, act, wide;
 };
 
@@ -138,9 +301,25 @@ __global__ void __launch_bounds__(DZ_WARPS * 32) dz_kernel(const DzArgs g) {
                     o[i] = from_f32<T>(v0);
                     o[i + 1] = from_f32<T>(v1);
                 }
-                if (g.dz) {  // rows of dz are padded to 16 bytes
-                    T* out = static_cast<T*>(g.dz) + q * ((g.dim + VEC - 1) / VEC * VEC) + j;
-                    *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(o);
+                if (g.dz) {  // an operand as the tensor cores take it: 16 bits, or three planes; padded rows
+                    const long long at = q * pack_stride(g.dim) + j;
+                    if constexpr (sizeof(T) == 2) {
+                        *reinterpret_cast<uint4*>(static_cast<T*>(g.dz) + at) = *reinterpret_cast<const uint4*>(o);
+                    } else {
+                        alignas(8) __nv_bfloat16 pl[3][VEC];
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) {
+                            __nv_bfloat16 w[3];
+                            split3(o[i], w);
+                            pl[0][i] = w[0];
+                            pl[1][i] = w[1];
+                            pl[2][i] = w[2];
+                        }
+#pragma unroll
+                        for (int k = 0; k < 3; ++k)
+                            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(g.dz) + k * g.plane + at) =
+                                *reinterpret_cast<const uint2*>(pl[k]);
+                    }
                 }
             }
         }
@@ -206,9 +385,13 @@ struct Strides {
     long long x, w, r, p, y;
 };
 
+constexpr long long LINEAR_MAX = (1ll << 31) - 1024;  // tensor coordinates are 32 bits
+
 static int linear_check(const fg_linear_params* p, Strides& t) {
     FG_REQUIRE(p, "null params");
     FG_REQUIRE(p->rows >= 0 && p->in_dim >= 1 && p->out_dim >= 1, "bad linear shape");
+    if (p->rows > LINEAR_MAX || p->in_dim > LINEAR_MAX || p->out_dim > LINEAR_MAX)
+        return fail(FG_ERR_UNSUPPORTED, "a dimension above %lld", LINEAR_MAX);
     FG_REQUIRE(float_dtype(p->dtype), "unknown dtype %d", p->dtype);
     FG_REQUIRE(p->activation >= FG_ACT_NONE && p->activation <= FG_ACT_SILU, "unknown activation %d", p->activation);
     t.x = p->x_stride ? p->x_stride : p->in_dim;
@@ -232,23 +415,54 @@ static GemmShape dw_shape(const fg_linear_params* p, const Strides& t, long long
     return {p->out_dim, p->in_dim, p->rows, 1, ldz, 1, t.x};
 }
 
+struct ForwardWs {
+    void *x, *w, *product;
+};
+
+static size_t forward_carve(const fg_linear_params* p, const Strides& t, void* ws, size_t bytes, ForwardWs& f) {
+    Carve c(ws, bytes);
+    f = ForwardWs{};
+    if (p->rows <= GEMV_ROWS) return 0;
+    if (needs_pack(p->dtype, t.x)) f.x = c.take<char>(pack_bytes(p->dtype, p->rows, p->in_dim));
+    if (needs_pack(p->dtype, t.w)) f.w = c.take<char>(pack_bytes(p->dtype, p->out_dim, p->in_dim));
+    const size_t n = tc_gemm_workspace(p->dtype, forward_shape(p, t));
+    if (n) f.product = c.take<char>(n);
+    return c.used;
+}
+
+// x or w: as it lies, or queued to be packed.
+static Operand operand(int dtype, const void* p, long long rows, int cols, long long ld, void* room, PackArgs& a) {
+    if (!needs_pack(dtype, ld)) return {p, ld, 0};
+    const long long stride = pack_stride(cols), plane = dtype == FG_DTYPE_F32 ? rows * stride : 0;
+    a.job[a.jobs++] = PackJob{p, room, rows, ld, plane, cols};
+    return {room, stride, plane};
+}
+
+template <class T>
+static int linear_forward(const fg_linear_params* p, const Strides& t, const void* x, const void* w, const Epilogue& e,
+                          const ForwardWs& f, cudaStream_t s) {
+    if (p->rows <= GEMV_ROWS) return gemv<T>(x, w, forward_shape(p, t), e, s);
+    PackArgs jobs{};
+    const Operand a = operand(p->dtype, x, p->rows, p->in_dim, t.x, f.x, jobs);
+    const Operand b = operand(p->dtype, w, p->out_dim, p->in_dim, t.w, f.w, jobs);
+    const int rc = pack<T>(jobs, s);
+    if (rc) return rc;
+    return gemm<T>(a, b, GemmShape{p->rows, p->out_dim, p->in_dim, a.ld, 1, b.ld, 1}, e, f.product, s);
+}
+
 struct BackwardWs {
-    void *dz, *product;
+    void *dz, *x, *w, *product;
     float* part;
 };
 
-static long long dz_stride(const fg_linear_params* p) {
-    const int vec = 16 / dtype_size(p->dtype);
-    return (long long)(p->out_dim + vec - 1) / vec * vec;
-}
-
 static size_t backward_carve(const fg_linear_params* p, const Strides& t, void* ws, size_t bytes, BackwardWs& w) {
     Carve c(ws, bytes);
-    const size_t n = p->dtype == FG_DTYPE_F32 ? 0
-                                              : std::max(tc_gemm_workspace(dx_shape(p, t, t.y)),
-                                                         tc_gemm_workspace(dw_shape(p, t, t.y)));
-    w.product = n ? c.take<char>(n) : nullptr;
-    w.dz = p->activation == FG_ACT_NONE ? nullptr : c.take<char>((size_t)p->rows * dz_stride(p) * dtype_size(p->dtype));
+    w = BackwardWs{};
+    if (p->activation != FG_ACT_NONE || needs_pack(p->dtype, t.y)) w.dz = c.take<char>(pack_bytes(p->dtype, p->rows, p->out_dim));
+    if (needs_pack(p->dtype, t.x)) w.x = c.take<char>(pack_bytes(p->dtype, p->rows, p->in_dim));
+    if (needs_pack(p->dtype, t.w)) w.w = c.take<char>(pack_bytes(p->dtype, p->out_dim, p->in_dim));
+    const size_t n = std::max(tc_gemm_workspace(p->dtype, dx_shape(p, t, t.y)), tc_gemm_workspace(p->dtype, dw_shape(p, t, t.y)));
+    if (n) w.product = c.take<char>(n);
     w.part = c.take<float>((size_t)dz_split(p->rows, p->out_dim, dtype_size(p->dtype)) * p->out_dim);
     return c.used;
 }
@@ -256,31 +470,35 @@ static size_t backward_carve(const fg_linear_params* p, const Strides& t, void* 
 template <class T>
 static int linear_backward(const fg_linear_params* p, const Strides& t, const void* dy, const void* x, const void* w,
                            const void* pre, void* dx, void* dw, void* dbias, const BackwardWs& ws, cudaStream_t s) {
-    const bool act = p->activation != FG_ACT_NONE, store = act && (dx || dw);
+    const bool act = p->activation != FG_ACT_NONE, store = (act || needs_pack(p->dtype, t.y)) && (dx || dw);
     const int split = p->rows ? dz_split(p->rows, p->out_dim, sizeof(T)) : 0;
+    const long long plane = p->dtype == FG_DTYPE_F32 ? p->rows * pack_stride(p->out_dim) : 0;
     int rc;
     if (split && (store || dbias)) {
         const DzArgs g{dy, act ? pre : nullptr, store ? ws.dz : nullptr, dbias ? ws.part : nullptr, t.y, t.p, p->rows, 0,
-                       p->out_dim, p->activation, 0};
+                       plane, p->out_dim, p->activation, 0};
         if ((rc = launch_dz<T>(g, split, s))) return rc;
     }
     if (dbias) {
         dz_reduce_kernel<T><<<(p->out_dim + 31) / 32, 1024, 0, s>>>(ws.part, split, p->out_dim, (T*)dbias);
         if ((rc = check_launch("dz_reduce_kernel"))) return rc;
     }
-    const void* dz = act ? ws.dz : dy;
-    const long long ldz = act ? dz_stride(p) : t.y;
+    const Operand dz = store ? Operand{ws.dz, pack_stride(p->out_dim), plane} : Operand{dy, t.y, 0};
+    PackArgs jobs{};
+    Operand xo{}, wo{};
+    if (dx && p->rows) wo = operand(p->dtype, w, p->out_dim, p->in_dim, t.w, ws.w, jobs);
+    if (dw && p->rows) xo = operand(p->dtype, x, p->rows, p->in_dim, t.x, ws.x, jobs);
+    if ((rc = pack<T>(jobs, s))) return rc;
     Epilogue e{};
+    e.ldy = p->in_dim;
     if (dx && p->rows) {
         e.y = dx;
-        e.ldy = p->in_dim;
-        rc = gemm<T>(dz, w, dx_shape(p, t, ldz), e, ws.product, s);
+        rc = gemm<T>(dz, wo, GemmShape{p->rows, p->in_dim, p->out_dim, dz.ld, 1, 1, wo.ld}, e, ws.product, s);
         if (rc) return rc;
     }
     if (dw) {
         e.y = dw;
-        e.ldy = p->in_dim;
-        rc = gemm<T>(dz, x, dw_shape(p, t, ldz), e, ws.product, s);
+        rc = gemm<T>(dz, xo, GemmShape{p->out_dim, p->in_dim, p->rows, 1, dz.ld, 1, xo.ld}, e, ws.product, s);
         if (rc) return rc;
     }
     return FG_OK;
@@ -298,7 +516,8 @@ int fg_linear_workspace_size(const fg_linear_params* params, size_t* bytes) {
         Strides t;
         const int rc = linear_check(params, t);
         if (rc) return rc;
-        *bytes = params->dtype == FG_DTYPE_F32 || params->rows == 0 ? 0 : tc_gemm_workspace(forward_shape(params, t));
+        ForwardWs f;
+        *bytes = forward_carve(params, t, nullptr, 0, f);
         return FG_OK;
     });
 }
@@ -311,16 +530,15 @@ int fg_linear(const fg_linear_params* params, const void* x, const void* w, cons
         if (rc) return rc;
         if (params->rows == 0) return FG_OK;
         FG_REQUIRE(x && w && y, "null buffer");
-        const GemmShape g = forward_shape(params, t);
-        if (params->dtype != FG_DTYPE_F32 && tc_gemm_fits(x, w, g)) {
-            const int bad = adapter_ws(workspace, workspace_bytes, tc_gemm_workspace(g));
-            if (bad) return bad;
-        }
+        ForwardWs f;
+        const int bad = adapter_ws(workspace, workspace_bytes, forward_carve(params, t, nullptr, 0, f));
+        if (bad) return bad;
+        forward_carve(params, t, workspace, workspace_bytes, f);
         const Epilogue e{bias, residual, pre, y, t.r, t.p, t.y, params->activation};
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        return params->dtype == FG_DTYPE_F32   ? gemm<float>(x, w, g, e, workspace, s)
-               : params->dtype == FG_DTYPE_F16 ? gemm<__half>(x, w, g, e, workspace, s)
-                                               : gemm<__nv_bfloat16>(x, w, g, e, workspace, s);
+        return params->dtype == FG_DTYPE_F32   ? linear_forward<float>(params, t, x, w, e, f, s)
+               : params->dtype == FG_DTYPE_F16 ? linear_forward<__half>(params, t, x, w, e, f, s)
+                                               : linear_forward<__nv_bfloat16>(params, t, x, w, e, f, s);
     });
 }
 

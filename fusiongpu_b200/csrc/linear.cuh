@@ -130,11 +130,13 @@ __device__ __forceinline__ void epilogue_store(const Epilogue& e, long long m, l
     static_cast<T*>(e.y)[m * e.ldy + n] = from_f32<T>(y);
 }
 
-// Tensor-core product of 16-bit operands (linear_tc.cu).  tc_gemm_fits: the
-// operands' rows start on 16-byte boundaries, as their TMA loads need.
+// Tensor-core product (linear_tc.cu) of 16-bit operands, or for F32 of three bf16
+// planes of each, a_plane and b_plane elements apart.  tc_gemm_fits: the operands'
+// rows start on 16-byte boundaries, as their TMA loads need.  The workspace
+// (256-byte aligned) holds the partial tiles of a split product.
 bool tc_gemm_fits(const void* a, const void* b, const GemmShape& g);
-// Its workspace (256-byte aligned) holds the partial tiles of a split product.
-size_t tc_gemm_workspace(const GemmShape& g);
-int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& g, const Epilogue& e, void* ws, cudaStream_t s);
+size_t tc_gemm_workspace(int dtype, const GemmShape& g);
+int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& g,
+            const Epilogue& e, void* ws, cudaStream_t s);
 
 }  // namespace fg

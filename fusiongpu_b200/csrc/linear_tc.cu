@@ -1,6 +1,12 @@
 // linear_tc.cu -- the linear layer's products on the 5th-generation tensor cores:
 // C(m, n) = sum over k of A(m, k) B(n, k), 16-bit operands, fp32 accumulators in
-// TMEM.  Either operand may have unit stride along k (K-major: x and w of the
+// TMEM.  float32 operands come as three bf16 planes, x = x0 + x1 + x2 (8 bits of
+// the significand each), and the product as the six plane products that reach
+// 2^-24 of it: the same kernels with six times the K blocks.  The tensor cores cut
+// their sums rather than round them, about 1e-8 of the running value for every 16
+// products; so float32 sums are taken from TMEM after at most 512 k, the smallest
+// plane products first, and added in fp32, and 16-bit ones run over 32,768 k at most
+// before they meet other parts.  Either operand may have unit stride along k (K-major: x and w of the
 // forward pass, dz of dx = dz w) or along its rows (MN-major: w of dx, both
 // operands of dw = dz^T x), so no pass over memory transposes anything.
 #include <algorithm>
@@ -14,6 +20,7 @@ constexpr int GT_M = 128;          // UMMA M: rows of a tile, TMEM lanes
 constexpr int GT_K = 64;           // elements of a K block: one 128-byte swizzle row
 constexpr int GT_NT = 64 + 256;    // TMA warp, MMA warp, 8 epilogue warps
 constexpr int GT_RING = 192 * 1024;
+constexpr int GT_RUN = 512;        // K blocks that a 16-bit product's accumulator sums at most
 
 struct TcArgs {
     int kt, mt, nt;     // K blocks, row tiles, column tiles
@@ -22,9 +29,33 @@ struct TcArgs {
     int split;          // parts of a tile's K range: CTAs of a cluster, or passes of the pairs
     int m_pad;          // pairs with split > 1: rows of a part's partial tiles
     int vec;            // outputs, residual and bias allow 4-column accesses
+    int planes;         // 1, or 3: float32
+    GemmShape f;        // planes == 3: the operands as they lie, for results that are not finite
+    const __nv_bfloat16 *fa, *fb;
+    long long a_plane, b_plane;
     uint32_t idesc;
     Epilogue e;
 };
+
+// Planes of the i-th plane product.
+__device__ __forceinline__ int plane_a(int i, int planes) { return planes == 1 ? 0 : (280 >> (2 * i)) & 3; }  // 0 2 1 0 1 0
+__device__ __forceinline__ int plane_b(int i, int planes) { return planes == 1 ? 0 : (82 >> (2 * i)) & 3; }   // 2 0 1 1 0 0
+
+// An infinite operand times the small planes of the other has any sign: a result
+// that is not finite is taken again, one product at a time.
+static __device__ __noinline__ float retake(const TcArgs& g, int m, int n) {
+    float z = 0.0f;
+    auto value = [](const __nv_bfloat16* p, long long step) {
+        return to_f32(p[0]) + to_f32(p[step]) + to_f32(p[2 * step]);
+    };
+    for (long long k = 0; k < g.f.k && z == z; ++k)
+        z = fmaf(value(g.fa + m * g.f.am + k * g.f.ak, g.a_plane), value(g.fb + n * g.f.bn + k * g.f.bk, g.b_plane), z);
+    return z;
+}
+template <class T>
+__device__ __forceinline__ float finite_or_retake(const TcArgs& g, int m, int n, float z) {
+    return sizeof(T) == 4 && !(fabsf(z) <= FLT_MAX) ? retake(g, m, n) : z;
+}
 
 template <int BN>
 struct RingOf {
@@ -62,6 +93,11 @@ __device__ __forceinline__ float4 load4(const T* p) {
     return make_float4(to_f32(v[0]), to_f32(v[1]), to_f32(v[2]), to_f32(v[3]));
 }
 
+template <>
+__device__ __forceinline__ float4 load4<float>(const float* p) {
+    return *reinterpret_cast<const float4*>(p);
+}
+
 template <class T>
 __device__ __forceinline__ void store4(T* p, float4 f) {
     T v[4] = {from_f32<T>(f.x), from_f32<T>(f.y), from_f32<T>(f.z), from_f32<T>(f.w)};
@@ -91,6 +127,11 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
 }
 
+template <>
+__device__ __forceinline__ void store4<float>(float* p, float4 f) {
+    *reinterpret_cast<float4*>(p) = f;
+}
+
 // One tile of 128 x BN per cluster, its K blocks divided over the cluster's
 // CTAs.  Each CTA's partial tile goes from TMEM to its shared memory (where the
 // operand ring was); then each CTA adds one slice of the columns over the
@@ -113,6 +154,9 @@ __global__ void __launch_bounds__(GT_NT, 1)
     const int tile = (int)(blockIdx.x / (unsigned)S);
     const int m0 = tile / g.nt * GT_M, n0 = tile % g.nt * BN;
     const int kb0 = (int)((long long)g.kt * rank / S), kb1 = (int)((long long)g.kt * (rank + 1) / S);
+    // accumulators: one, or for float32 as many as TMEM holds, each for its share of k
+    constexpr int NA = sizeof(T) == 4 ? 512 / BN : 1;
+    const int share = (kb1 - kb0 + NA - 1) / NA, shares = (kb1 - kb0 + share - 1) / share, products = sizeof(T) == 4 ? 6 : 1;
 
     if (warp == 2 && tc::elect_one()) {
         tc::prefetch_map(&ta);
@@ -128,7 +172,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
         tc::fence_mbar_init();
     }
     if (warp == 1) {
-        tc::tmem_alloc(&tmem_slot, BN);
+        tc::tmem_alloc(&tmem_slot, NA * BN);
         tc::tmem_relinquish();
     }
     tc::fence_before_sync();
@@ -141,24 +185,30 @@ __global__ void __launch_bounds__(GT_NT, 1)
         if (tc::elect_one()) {  // ---- TMA producer
             int i = 0;
             bool ok = true;
-            for (int kb = kb0; kb < kb1; ++kb, ++i) {
-                const int st = i % Ring::N;
-                if (!(ok = tc::mbar_wait_or_fail(&empty[st], ((i / Ring::N) & 1) ^ 1, fail))) break;
+            auto load = [&](int kb, int product) {
+                const int st = i % Ring::N, k = kb * GT_K;
+                ok = tc::mbar_wait_or_fail(&empty[st], ((i / Ring::N) & 1) ^ 1, fail);
+                if (!ok) return;
                 unsigned char *sa = ring + st * Ring::STAGE, *sb = sa + Ring::A;
                 tc::mbar_arrive_expect_tx(&full[st], Ring::STAGE);
+                const int pa = plane_a(product, products), pb = plane_b(product, products);
                 if (g.a_mn) {
                     for (int c = 0; c < GT_M / 64; ++c)
-                        tc::tma_load_2d(sa + c * 8192, &ta, &full[st], m0 + c * 64, kb * GT_K);
+                        tc::tma_load_3d(sa + c * 8192, &ta, &full[st], m0 + c * 64, k, pa);
                 } else {
-                    tc::tma_load_2d(sa, &ta, &full[st], kb * GT_K, m0);
+                    tc::tma_load_3d(sa, &ta, &full[st], k, m0, pa);
                 }
                 if (g.b_mn) {
                     for (int c = 0; c < BN / 64; ++c)
-                        tc::tma_load_2d(sb + c * 8192, &tb, &full[st], n0 + c * 64, kb * GT_K);
+                        tc::tma_load_3d(sb + c * 8192, &tb, &full[st], n0 + c * 64, k, pb);
                 } else {
-                    tc::tma_load_2d(sb, &tb, &full[st], kb * GT_K, n0);
+                    tc::tma_load_3d(sb, &tb, &full[st], k, n0, pb);
                 }
-            }
+                ++i;
+            };
+            for (int c0 = kb0; c0 < kb1 && ok; c0 += share)
+                for (int q = 0; q < products && ok; ++q)
+                    for (int kb = c0; kb < min(c0 + share, kb1) && ok; ++kb) load(kb, q);
             if (!ok)  // copies in flight land before the block ends
                 for (int j = i > Ring::N ? i - Ring::N : 0; j < i; ++j)
                     tc::mbar_wait(&full[j % Ring::N], (j / Ring::N) & 1);
@@ -170,20 +220,23 @@ __global__ void __launch_bounds__(GT_NT, 1)
         const uint64_t da0 = g.a_mn ? tc::desc_mnmajor_sw128(ring, 8192) : tc::desc_kmajor_sw128(ring);
         const uint64_t db0 = g.b_mn ? tc::desc_mnmajor_sw128(ring + Ring::A, 8192) : tc::desc_kmajor_sw128(ring + Ring::A);
         const uint32_t ka = g.a_mn ? 128 : 2, kbs = g.b_mn ? 128 : 2;  // 16 k, in 16-byte units
-        for (int kb = kb0; kb < kb1; ++kb, ++i) {
-            const int st = i % Ring::N;
-            ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&full[st], (i / Ring::N) & 1, fail));
-            if (!ok) break;
-            tc::fence_after_sync();
-            const uint64_t da = da0 + st * (Ring::STAGE / 16), db = db0 + st * (Ring::STAGE / 16);
-            if (tc::elect_one()) {
+        for (int c0 = kb0, acc = 0; c0 < kb1 && ok; c0 += share, ++acc) {
+            const int n = (min(c0 + share, kb1) - c0) * products;
+            for (int u = 0; u < n; ++u, ++i) {
+                const int st = i % Ring::N;
+                ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&full[st], (i / Ring::N) & 1, fail));
+                if (!ok) break;
+                tc::fence_after_sync();
+                const uint64_t da = da0 + st * (Ring::STAGE / 16), db = db0 + st * (Ring::STAGE / 16);
+                if (tc::elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < GT_K / 16; ++kk)
-                    tc::umma_bf16(taddr, da + ka * kk, db + kbs * kk, g.idesc, (i | kk) != 0);
-                tc::umma_commit(&empty[st]);
-                if (kb + 1 == kb1) tc::umma_commit(&acc_full);
+                    for (int kk = 0; kk < GT_K / 16; ++kk)
+                        tc::umma_bf16(taddr + (uint32_t)(acc * BN), da + ka * kk, db + kbs * kk, g.idesc, (u | kk) != 0);
+                    tc::umma_commit(&empty[st]);
+                    if (u + 1 == n && c0 + share >= kb1) tc::umma_commit(&acc_full);
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
     } else {  // ---- epilogue warps: TMEM -> partial tile in shared memory
         const int q4 = warp & 3, half = (warp - 2) >> 2;
@@ -194,6 +247,12 @@ __global__ void __launch_bounds__(GT_NT, 1)
         for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
             float v[32];
             tc::tmem_ld_32x32(taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)c, v);
+            for (int a = 1; a < shares; ++a) {
+                float x[32];
+                tc::tmem_ld_32x32(taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(a * BN + c), x);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] += x[j];
+            }
 #pragma unroll
             for (int j = 0; j < 32; j += 4)  // a wait that ran out leaves NaN, not a plausible number
                 *reinterpret_cast<float4*>(row + c + j) =
@@ -206,7 +265,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
     if (S > 1) cluster_sync();
     if (warp == 1) {
         tc::fence_after_sync();
-        tc::tmem_dealloc(taddr, BN);
+        tc::tmem_dealloc(taddr, NA * BN);
     }
 
     // Four positions per thread and round, their residuals loaded first: one
@@ -218,7 +277,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
     for (int i0 = tid; i0 < GT_M * per_row; i0 += U * GT_NT) {
         int row[U], col[U];
         uint32_t at[U];
-        uint2 res[U];
+        float4 res[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * GT_NT, r = i / per_row, c = rank * slice + (i - r * per_row) * 4;
@@ -226,7 +285,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
             col[u] = n0 + c;
             at[u] = (uint32_t)(r * LDP + c) * 4;
             if (e.residual && g.vec && row[u] < g.m && col[u] + 4 <= g.n)
-                res[u] = *reinterpret_cast<const uint2*>(static_cast<const T*>(e.residual) + row[u] * e.ldr + col[u]);
+                res[u] = load4(static_cast<const T*>(e.residual) + row[u] * e.ldr + col[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -244,6 +303,12 @@ __global__ void __launch_bounds__(GT_NT, 1)
             } else {
                 z = *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(part) + at[u]);
             }
+            if (sizeof(T) == 4) {
+                z.x = finite_or_retake<T>(g, row[u], col[u], z.x);
+                if (col[u] + 1 < g.n) z.y = finite_or_retake<T>(g, row[u], col[u] + 1, z.y);
+                if (col[u] + 2 < g.n) z.z = finite_or_retake<T>(g, row[u], col[u] + 2, z.z);
+                if (col[u] + 3 < g.n) z.w = finite_or_retake<T>(g, row[u], col[u] + 3, z.w);
+            }
             if (g.vec && col[u] + 4 <= g.n) {
                 if (e.bias) {
                     const float4 b = load4(static_cast<const T*>(e.bias) + col[u]);
@@ -254,19 +319,19 @@ __global__ void __launch_bounds__(GT_NT, 1)
                 }
                 if (e.pre) store4(static_cast<T*>(e.pre) + row[u] * e.ldp + col[u], z);
                 float4 y = z;
-                if (e.act == FG_ACT_GELU) {
+                if (e.act == FG_ACT_GELU && sizeof(T) == 2) {
                     gelu2(y.x, y.y);
                     gelu2(y.z, y.w);
                 } else if (e.act != FG_ACT_NONE) {
-                    y = make_float4(activate<true>(z.x, e.act), activate<true>(z.y, e.act),
-                                    activate<true>(z.z, e.act), activate<true>(z.w, e.act));
+                    constexpr bool FAST = sizeof(T) == 2;
+                    y = make_float4(activate<FAST>(z.x, e.act), activate<FAST>(z.y, e.act),
+                                    activate<FAST>(z.z, e.act), activate<FAST>(z.w, e.act));
                 }
                 if (e.residual) {
-                    const float2 lo = unpack2<T>(res[u].x), hi = unpack2<T>(res[u].y);
-                    y.x += lo.x;
-                    y.y += lo.y;
-                    y.z += hi.x;
-                    y.w += hi.y;
+                    y.x += res[u].x;
+                    y.y += res[u].y;
+                    y.z += res[u].z;
+                    y.w += res[u].w;
                 }
                 store4(static_cast<T*>(e.y) + row[u] * e.ldy + col[u], y);
             } else {
@@ -289,16 +354,20 @@ __global__ void __launch_bounds__(GT_NT, 1)
 // stores from (whole 128-byte rows, clipped at the matrix's edge).  16 epilogue
 // warps hide the chain TMEM load, residual, fence, store of each: 8 warps of two
 // chunks took 10,200 cycles for a tile of 6,144 cycles of products (width 768).
-constexpr int GP_STAGES = 5;
 constexpr int GP_A = GT_M * GT_K * 2;
 constexpr int GP_BUF = 4096;   // 32 rows x 128 bytes, 128-byte swizzle
 constexpr int GP_EPI = 16;     // epilogue warps, each 32 rows x 64 columns of a tile
 constexpr int GP_NT = 64 + GP_EPI * 32;
 
-template <int BN>
+constexpr int GP_CHUNK = 8;    // K blocks of a float32 accumulator
+
+// Operand stages and the epilogue's buffers: 4 KB a warp, or for float32 8 KB, which
+// hold the running sums of its 32 rows x 64 columns.
+template <class T, int BN>
 struct PairOf {
-    static constexpr int B = BN / 2 * GT_K * 2, STAGE = GP_A + B;
-    static constexpr int SMEM = GP_STAGES * STAGE + GP_EPI * (GP_BUF + 128);
+    static constexpr int B = BN / 2 * GT_K * 2, STAGE = GP_A + B, STAGES = sizeof(T) == 4 ? 3 : 5;
+    static constexpr int BUF = sizeof(T) == 4 ? 2 * GP_BUF : GP_BUF;
+    static constexpr int SMEM = STAGES * STAGE + GP_EPI * (BUF + (sizeof(T) == 4 ? 0 : 128));
     static constexpr int WARPS = BN / 64 * 4;         // epilogue warps of a tile
     static constexpr int GROUPS = GP_EPI / WARPS;     // that take tiles in turn
 };
@@ -356,16 +425,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                      const __grid_constant__ CUtensorMap ty, const __grid_constant__ CUtensorMap tp,
                      const __grid_constant__ CUtensorMap tr, const TcArgs g) {
-    using P = PairOf<BN>;
+    using P = PairOf<T, BN>;
+    constexpr int GP_STAGES = P::STAGES;
+    static_assert(sizeof(T) == 2 || BN == 256, "float32 takes 256 columns");
     extern __shared__ __align__(1024) unsigned char dsmem[];
     __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], acc_full[2], acc_empty[2], res_full[GP_EPI];
     __shared__ uint32_t tmem_slot;
     __shared__ int s_fail;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)cluster_rank();
-    unsigned char *ring = dsmem, *bufs = ring + GP_STAGES * P::STAGE, *biases = bufs + GP_EPI * GP_BUF;
+    unsigned char *ring = dsmem, *bufs = ring + GP_STAGES * P::STAGE, *biases = bufs + GP_EPI * P::BUF;
     const int pairs = (int)(gridDim.x >> 1), items = g.mt * g.nt * g.split;
     auto k_begin = [&](int part) { return (int)((long long)g.kt * part / g.split); };
+    constexpr int products = sizeof(T) == 4 ? 6 : 1, chunk = sizeof(T) == 4 ? GP_CHUNK : 1 << 30;
 
     if (warp == 2 && tc::elect_one()) {
         tc::prefetch_map(&ta);
@@ -403,25 +475,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             for (int w = blockIdx.x >> 1; w < items && ok; w += pairs) {
                 const int t = w / g.split, sp = w - t * g.split, k1 = k_begin(sp + 1);
                 const int m0 = t / g.nt * 2 * GT_M + rank * GT_M, n0 = t % g.nt * BN + rank * (BN / 2);
-                for (int kb = k_begin(sp); kb < k1; ++kb, ++i) {
-                    const int st = i % GP_STAGES;
-                    if (!(ok = tc::mbar_wait_or_fail(&empty[st], ((i / GP_STAGES) & 1) ^ 1, fail))) break;
+                auto load = [&](int kb, int product) {
+                    const int st = i % GP_STAGES, k = kb * GT_K;
+                    ok = tc::mbar_wait_or_fail(&empty[st], ((i / GP_STAGES) & 1) ^ 1, fail);
+                    if (!ok) return;
                     unsigned char *sa = ring + st * P::STAGE, *sb = sa + GP_A;
                     if (rank == 0) tc::mbar_arrive_expect_tx(&full[st], 2 * P::STAGE);
                     const uint32_t bar = tc::leader_addr(&full[st]);
+                    const int pa = plane_a(product, products), pb = plane_b(product, products);
                     if (g.a_mn) {
                         for (int c = 0; c < GT_M / 64; ++c)
-                            tc::tma_load_2d_pair(sa + c * 8192, &ta, bar, m0 + c * 64, kb * GT_K);
+                            tc::tma_load_3d_pair(sa + c * 8192, &ta, bar, m0 + c * 64, k, pa);
                     } else {
-                        tc::tma_load_2d_pair(sa, &ta, bar, kb * GT_K, m0);
+                        tc::tma_load_3d_pair(sa, &ta, bar, k, m0, pa);
                     }
                     if (g.b_mn) {
                         for (int c = 0; c < BN / 128; ++c)
-                            tc::tma_load_2d_pair(sb + c * 8192, &tb, bar, n0 + c * 64, kb * GT_K);
+                            tc::tma_load_3d_pair(sb + c * 8192, &tb, bar, n0 + c * 64, k, pb);
                     } else {
-                        tc::tma_load_2d_pair(sb, &tb, bar, kb * GT_K, n0);
+                        tc::tma_load_3d_pair(sb, &tb, bar, k, n0, pb);
                     }
-                }
+                    ++i;
+                };
+                for (int c0 = k_begin(sp); c0 < k1 && ok; c0 += min(chunk, k1 - c0))
+                    for (int q = 0; q < products && ok; ++q)
+                        for (int kb = c0; kb < c0 + min(chunk, k1 - c0) && ok; ++kb) load(kb, q);
             }
             if (!ok && rank == 0)  // copies in flight land before the blocks end
                 for (int j = i > GP_STAGES ? i - GP_STAGES : 0; j < i; ++j)
@@ -434,32 +512,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             const uint64_t da0 = g.a_mn ? tc::desc_mnmajor_sw128(ring, 8192) : tc::desc_kmajor_sw128(ring);
             const uint64_t db0 = g.b_mn ? tc::desc_mnmajor_sw128(ring + GP_A, 8192) : tc::desc_kmajor_sw128(ring + GP_A);
             const uint32_t ka = g.a_mn ? 128 : 2, kbs = g.b_mn ? 128 : 2;
-            for (int w = blockIdx.x >> 1; w < items && ok; w += pairs, ++li) {
-                const int sp = w % g.split, k0 = k_begin(sp), k1 = k_begin(sp + 1), acc = li & 1;
-                ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&acc_empty[acc], ((li >> 1) & 1) ^ 1, fail));
-                if (!ok) break;
-                tc::fence_after_sync();
-                for (int kb = k0; kb < k1; ++kb, ++i) {
-                    const int st = i % GP_STAGES;
-                    ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&full[st], (i / GP_STAGES) & 1, fail));
+            for (int w = blockIdx.x >> 1; w < items && ok; w += pairs) {
+                const int sp = w % g.split, k1 = k_begin(sp + 1);
+                for (int c0 = k_begin(sp); c0 < k1 && ok; c0 += min(chunk, k1 - c0), ++li) {
+                    const int n = min(chunk, k1 - c0) * products, acc = li & 1;
+                    ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&acc_empty[acc], ((li >> 1) & 1) ^ 1, fail));
                     if (!ok) break;
                     tc::fence_after_sync();
-                    const uint64_t da = da0 + st * (P::STAGE / 16), db = db0 + st * (P::STAGE / 16);
-                    if (tc::elect_one()) {
+                    for (int u = 0; u < n; ++u, ++i) {
+                        const int st = i % GP_STAGES;
+                        ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&full[st], (i / GP_STAGES) & 1, fail));
+                        if (!ok) break;
+                        tc::fence_after_sync();
+                        const uint64_t da = da0 + st * (P::STAGE / 16), db = db0 + st * (P::STAGE / 16);
+                        if (tc::elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < GT_K / 16; ++kk)
-                            tc::umma_pair(taddr + (uint32_t)(acc * BN), da + ka * kk, db + kbs * kk, g.idesc,
-                                          kb != k0 || kk != 0);
-                        tc::umma_commit_pair(&empty[st]);
-                        if (kb + 1 == k1) tc::umma_commit_pair(&acc_full[acc]);
+                            for (int kk = 0; kk < GT_K / 16; ++kk)
+                                tc::umma_pair(taddr + (uint32_t)(acc * BN), da + ka * kk, db + kbs * kk, g.idesc,
+                                              (u | kk) != 0);
+                            tc::umma_commit_pair(&empty[st]);
+                            if (u + 1 == n) tc::umma_commit_pair(&acc_full[acc]);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             }
         }
     } else {  // ---- epilogue warps
         const int w = warp - 2, q4 = warp & 3, part = w / 4 % (BN / 64), group = w / P::WARPS;
-        unsigned char* buf = bufs + w * GP_BUF;
+        unsigned char* buf = bufs + w * P::BUF;
         const Epilogue& e = g.e;
         const int tr_rows = rank * GT_M + q4 * 32;
         const uint32_t sw = (uint32_t)(lane & 7) << 4;
@@ -471,7 +552,126 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
         };
         const int step = pairs * P::GROUPS;
         int item = (blockIdx.x >> 1) + pairs * group, li = group;
-        if (e.residual && !e.pre && item < items && tc::elect_one()) fetch_residual(item);
+        if (sizeof(T) == 2 && e.residual && !e.pre && item < items && tc::elect_one()) fetch_residual(item);
+        if constexpr (sizeof(T) == 4) {
+            // Chunks of k are added to the sums in shared memory, a lane its own row, in
+            // two halves of 32 columns; the last one is followed by the epilogue proper,
+            // one step after the other: six products a K block hide it.
+            for (; item < items; item += step) {
+                const int t = item / g.split, sp = item - t * g.split, k1 = k_begin(sp + 1);
+                const int col = t % g.nt * BN + part * 64, m0 = t / g.nt * 2 * GT_M + tr_rows;
+                bool all_ok = true;
+                if (tc::elect_one()) tc::bulk_wait_read<0>();
+                __syncwarp();
+                for (int c0 = k_begin(sp), first = 1; c0 < k1; c0 += min(chunk, k1 - c0), first = 0, ++li) {
+                    const int acc = li & 1;
+                    all_ok &= tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
+                    tc::fence_after_sync();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v[32];
+                        tc::tmem_ld_32x32(taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + part * 64 + 32 * h), v);
+                        if (h == 1) {
+                            tc::fence_before_sync();
+                            __syncwarp();
+                            if (tc::elect_one()) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            float4* s = reinterpret_cast<float4*>(brow + h * GP_BUF + (((uint32_t)j << 2) ^ sw));
+                            float4 x = first ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *s;
+                            x.x += v[j];
+                            x.y += v[j + 1];
+                            x.z += v[j + 2];
+                            x.w += v[j + 3];
+                            *s = x;
+                        }
+                    }
+                }
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    const int c0 = col + 32 * h;
+                    const bool in = m0 < g.m && c0 < g.n;
+                    unsigned char *hbuf = buf + h * GP_BUF, *hrow = brow + h * GP_BUF;
+                    auto put = [&](const CUtensorMap* map, int y0, bool store) {
+                        tc::fence_proxy_async();
+                        __syncwarp();
+                        if (tc::elect_one()) {
+                            if (store) tc::tma_store_2d(map, hbuf, c0, y0);
+                            tc::bulk_commit();
+                        }
+                    };
+                    if (!all_ok) {  // a wait that ran out leaves NaN, not a plausible number
+                        for (int j = 0; j < 32; ++j) reinterpret_cast<float*>(hrow)[j] = NAN;
+                    }
+                    if (g.split > 1) {  // this part's sums as they are; finish_kernel adds the parts
+                        put(&ty, sp * g.m_pad + m0, c0 < g.n);
+                        continue;
+                    }
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(hrow + (((uint32_t)j << 2) ^ sw));
+                        v[j] = x.x;
+                        v[j + 1] = x.y;
+                        v[j + 2] = x.z;
+                        v[j + 3] = x.w;
+                    }
+                    auto stage = [&] {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<float4*>(hrow + (((uint32_t)j << 2) ^ sw)) =
+                                make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                    };
+                    bool odd = false;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) odd |= !(fabsf(v[j]) <= FLT_MAX);
+                    if (odd && all_ok && m0 + lane < g.m) {
+                        stage();
+                        for (int j = 0; j < 32 && c0 + j < g.n; ++j) {
+                            float* z = reinterpret_cast<float*>(hrow + ((((uint32_t)j << 2) & ~15u) ^ sw)) + (j & 3);
+                            *z = finite_or_retake<T>(g, m0 + lane, c0 + j, *z);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            v[j] = *(reinterpret_cast<float*>(hrow + ((((uint32_t)j << 2) & ~15u) ^ sw)) + (j & 3));
+                    }
+                    if (e.bias) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (c0 + j < g.n) v[j] += __ldg(static_cast<const float*>(e.bias) + c0 + j);
+                    }
+                    if (e.pre) {
+                        stage();
+                        put(&tp, m0, in);
+                    }
+                    if (e.act != FG_ACT_NONE) {
+#pragma unroll 4
+                        for (int j = 0; j < 32; ++j) v[j] = activate<false>(v[j], e.act);
+                    }
+                    if (tc::elect_one()) tc::bulk_wait_read<0>();
+                    __syncwarp();
+                    if (e.residual) {
+                        if (tc::elect_one()) {
+                            tc::mbar_arrive_expect_tx(&res_full[w], GP_BUF);
+                            tc::tma_load_2d(hbuf, &tr, &res_full[w], c0, m0);
+                        }
+                        tc::mbar_wait_warp(&res_full[w], res_phase, fail);
+                        res_phase ^= 1;
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 r = *reinterpret_cast<const float4*>(hrow + (((uint32_t)j << 2) ^ sw));
+                            v[j] += r.x;
+                            v[j + 1] += r.y;
+                            v[j + 2] += r.z;
+                            v[j + 3] += r.w;
+                        }
+                    }
+                    stage();
+                    put(&ty, m0, in);
+                }
+            }
+        } else {
         for (; item < items; item += step, li += P::GROUPS) {
             const int acc = li & 1, t = item / g.split;
             const int col = t % g.nt * BN + part * 64, m0 = t / g.nt * 2 * GT_M + tr_rows;
@@ -572,6 +772,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 }
             }
         }
+        }
         if (tc::elect_one()) tc::bulk_wait_read<0>();
     }
     tc::fence_before_sync();
@@ -597,7 +798,12 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* part, const Tc
         z.z += v.z;
         z.w += v.w;
     }
-    const float v[4] = {z.x, z.y, z.z, z.w};
+    float v[4] = {z.x, z.y, z.z, z.w};
+    if (sizeof(T) == 4) {
+        for (int j = 0; j < 4; ++j)
+            if (col + j < g.n) v[j] = finite_or_retake<T>(g, (int)row, col + j, v[j]);
+        z = make_float4(v[0], v[1], v[2], v[3]);
+    }
     if (g.vec && col + 4 <= g.n && !g.e.bias && !g.e.pre && !g.e.residual && g.e.act == FG_ACT_NONE)
         store4(static_cast<T*>(g.e.y) + row * g.e.ldy + col, z);
     else
@@ -606,17 +812,18 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* part, const Tc
 
 // ---- host side ---------------------------------------------------------------
 
-// Operand of `rows` rows (unit stride along k: [rows][k], else [k][rows]).
+// Operand of `rows` rows (unit stride along k: [rows][k], else [k][rows]), in
+// `planes` planes `plane` elements apart.
 static int operand_map(CUtensorMap* m, int dtype, const void* p, long long rows, long long k, long long ld, bool mn,
-                       int box_rows) {
+                       int box_rows, int planes, long long plane) {
     tc::EncodeTiledFn enc = tc::encode_fn();
     if (!enc) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    cuuint64_t dims[2] = {(cuuint64_t)(mn ? rows : k), (cuuint64_t)(mn ? k : rows)};
-    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    cuuint32_t box[2] = {64, (cuuint32_t)(mn ? GT_K : box_rows)};
-    cuuint32_t estr[2] = {1, 1};
+    cuuint64_t dims[3] = {(cuuint64_t)(mn ? rows : k), (cuuint64_t)(mn ? k : rows), (cuuint64_t)planes};
+    cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)(mn ? GT_K : box_rows), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = enc(m, dtype == FG_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                           2, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           3, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
@@ -625,7 +832,7 @@ static int operand_map(CUtensorMap* m, int dtype, const void* p, long long rows,
 
 // Instruction descriptor, kind::f16: f32 accumulators.
 static uint32_t instr_desc(int dtype, int m, int n, bool a_mn, bool b_mn) {
-    const uint32_t t = dtype == FG_DTYPE_BF16 ? 1 : 0;
+    const uint32_t t = dtype == FG_DTYPE_F16 ? 0 : 1;
     return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
@@ -639,8 +846,8 @@ bool tc_gemm_fits(const void* a, const void* b, const GemmShape& g) {
 template <class T, int BN>
 static int launch_split(int dtype, const void* a, const void* b, const GemmShape& s, TcArgs g, cudaStream_t st) {
     CUtensorMap ta, tb;
-    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M);
-    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN);
+    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M, g.planes, g.a_plane);
+    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN, g.planes, g.b_plane);
     if (rc) return rc;
     g.idesc = instr_desc(dtype, GT_M, BN, g.a_mn, g.b_mn);
     g.nt = (g.n + BN - 1) / BN;
@@ -664,22 +871,21 @@ static int launch_split(int dtype, const void* a, const void* b, const GemmShape
     return FG_OK;
 }
 
-// Output or residual [m][n] for TMA: boxes of 32 rows x 64 columns.
+// Matrix [rows][n] for the epilogue's TMA: boxes of 32 rows of 128 bytes.
 static int tile_map(CUtensorMap* m, int dtype, const void* p, long long rows, long long n, long long ld) {
     if (!p) return FG_OK;  // the kernel does not touch it
-    return operand_map(m, dtype, p, rows, n, ld, false, 32);
-}
-
-// Partial tiles [split][m_pad][n, padded to 4] of fp32, for the TMA stores of the pairs.
-static int part_map(CUtensorMap* m, const void* p, const TcArgs& g, long long ld) {
     tc::EncodeTiledFn enc = tc::encode_fn();
     if (!enc) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    cuuint64_t dims[2] = {(cuuint64_t)ld, (cuuint64_t)g.split * g.m_pad};
-    cuuint64_t strides[1] = {(cuuint64_t)ld * 4};
-    cuuint32_t box[2] = {32, 32};
+    const int es = dtype_size(dtype);
+    cuuint64_t dims[2] = {(cuuint64_t)n, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * es};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32};
     cuuint32_t estr[2] = {1, 1};
-    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(p), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+    const CUtensorMapDataType t = dtype == FG_DTYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : dtype == FG_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUresult r = enc(m, t, 2, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return FG_OK;
@@ -693,10 +899,10 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
     g.mt = (g.m + 2 * GT_M - 1) / (2 * GT_M);
     g.nt = (g.n + BN - 1) / BN;
     g.m_pad = g.mt * 2 * GT_M;
-    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M);
-    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN / 2);
+    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M, g.planes, g.a_plane);
+    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN / 2, g.planes, g.b_plane);
     if (g.split > 1) {
-        if (!rc) rc = part_map(&ty, ws, g, ld);
+        if (!rc) rc = tile_map(&ty, FG_DTYPE_F32, ws, (long long)g.split * g.m_pad, ld, ld);
     } else {
         if (!rc) rc = tile_map(&ty, dtype, e.y, s.m, s.n, e.ldy);
         if (!rc) rc = tile_map(&tp, dtype, e.pre, s.m, s.n, e.ldp);
@@ -707,11 +913,11 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
     const long long items = (long long)g.mt * g.nt * g.split;
     FG_REQUIRE(items <= 0x3fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
     auto kernel = &gemm_pair_kernel<T, BN>;
-    FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), PairOf<BN>::SMEM));
+    FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), PairOf<T, BN>::SMEM));
     const int pairs = std::max(1, device_attr(cudaDevAttrMultiProcessorCount) / 2);
     TcArgs k = g;
     if (g.split > 1) k.e.residual = k.e.pre = nullptr;
-    kernel<<<2 * (unsigned)std::min<long long>(items, pairs), GP_NT, PairOf<BN>::SMEM, st>>>(ta, tb, ty, tp, tr, k);
+    kernel<<<2 * (unsigned)std::min<long long>(items, pairs), GP_NT, PairOf<T, BN>::SMEM, st>>>(ta, tb, ty, tp, tr, k);
     rc = check_launch("gemm_pair_kernel");
     if (rc || g.split == 1) return rc;
     const long long n4 = (long long)g.m * ((g.n + 3) / 4);
@@ -735,9 +941,9 @@ struct TcPlan {
     size_t ws;
 };
 
-static TcPlan tc_plan(const GemmShape& s, bool pairs_fit) {
+static TcPlan tc_plan(const GemmShape& s, int planes, bool pairs_fit) {
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
-    const int kt = (int)((s.k + GT_K - 1) / GT_K);
+    const int kt = (int)((s.k + GT_K - 1) / GT_K) * (planes == 1 ? 1 : 6);
     auto waves = [](long long tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
     TcPlan best{false, 256, 1, 0};
     double least = 1e300;
@@ -748,11 +954,14 @@ static TcPlan tc_plan(const GemmShape& s, bool pairs_fit) {
         }
     };
     const long long m2 = (s.m + 2 * GT_M - 1) / (2 * GT_M), m1 = (s.m + GT_M - 1) / GT_M;
+    const int kb = (int)((s.k + GT_K - 1) / GT_K);
     for (int bn : {256, 128}) {
-        if (!pairs_fit) break;
+        if (planes == 3 && bn == 128) break;
         const long long tiles = m2 * ((s.n + bn - 1) / bn);
-        for (int sp : {1, 2, 4, 8, 16}) {
-            if (sp > 1 && (sp > kt / 2 || tiles * sp > sms)) break;
+        for (int sp : {1, 2, 4, 8, 16, 32}) {
+            if (sp > 1 && (sp > kb / 2 || (tiles * sp > sms && kb * 2 / sp <= GT_RUN))) break;
+            if (planes == 1 && kb > GT_RUN * sp && sp < 32) continue;
+            if (sp == 1 && !pairs_fit) continue;  // parts go through the workspace, whatever the outputs' alignment
             const size_t ws = sp > 1 ? (size_t)sp * m2 * 2 * GT_M * ((s.n + 3) / 4 * 4) * 4 : 0;
             const double epi = bn == 256 ? 2.0 : 1.0, main = (kt + sp - 1) / sp * (bn == 256 ? 0.39 : 0.34);
             offer(6.0 + waves(tiles * sp, sms / 2) * std::max(main, epi) + epi + (sp > 1 ? 3.0 + 1.5e-6 * ws / 6.0 : 0.0),
@@ -762,7 +971,9 @@ static TcPlan tc_plan(const GemmShape& s, bool pairs_fit) {
     for (int bn : {256, 128, 64}) {
         const long long tiles = m1 * ((s.n + bn - 1) / bn);
         for (int sp : {1, 2, 4, 8}) {
-            if (sp > kt) break;
+            if (sp > kb) break;
+            // the sums' length: 512 k for each of float32's 512 / bn accumulators
+            if (kb > (planes == 1 ? GT_RUN : GP_CHUNK * 512 / bn) * sp && kb > 3) continue;
             const int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
             const double main = (kt + sp - 1) / sp * (bn == 256 ? 0.43 : bn == 128 ? 0.30 : 0.21);
             offer(5.0 + waves(tiles, slots) * (main + 2.0 + 0.02 * bn / sp) + (sp == 8 ? 0.7 : 0.0), TcPlan{false, bn, sp, 0});
@@ -771,9 +982,13 @@ static TcPlan tc_plan(const GemmShape& s, bool pairs_fit) {
     return best;
 }
 
-size_t tc_gemm_workspace(const GemmShape& s) { return s.k > 0 ? tc_plan(s, true).ws : 0; }
+size_t tc_gemm_workspace(int dtype, const GemmShape& s) {
+    const int planes = dtype == FG_DTYPE_F32 ? 3 : 1;
+    return s.k > 0 ? std::max(tc_plan(s, planes, true).ws, tc_plan(s, planes, false).ws) : 0;
+}
 
-int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& s, const Epilogue& e, void* ws, cudaStream_t st) {
+int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& s,
+            const Epilogue& e, void* ws, cudaStream_t st) {
     TcArgs g{};
     g.m = (int)s.m;
     g.n = (int)s.n;
@@ -781,20 +996,28 @@ int tc_gemm(int dtype, const void* a, const void* b, const GemmShape& s, const E
     g.mt = (int)((s.m + GT_M - 1) / GT_M);
     g.a_mn = s.ak != 1;
     g.b_mn = s.bk != 1;
+    g.planes = dtype == FG_DTYPE_F32 ? 3 : 1;
+    g.f = s;
+    g.fa = static_cast<const __nv_bfloat16*>(a);
+    g.fb = static_cast<const __nv_bfloat16*>(b);
+    g.a_plane = g.planes == 1 ? 8 : a_plane;  // one plane: any multiple of 16 bytes
+    g.b_plane = g.planes == 1 ? 8 : b_plane;
     g.e = e;
-    auto lies = [&](const void* p, long long ld, int bytes) { return !p || (aligned(p, bytes) && ld * 2 % bytes == 0); };
-    g.vec = lies(e.y, e.ldy, 8) && lies(e.bias, 0, 8) && lies(e.pre, e.ldp, 8) && lies(e.residual, e.ldr, 8);
+    const int es = dtype_size(dtype);
+    auto lies = [&](const void* p, long long ld, int n) { return !p || (aligned(p, n) && ld * es % n == 0); };
+    g.vec = lies(e.y, e.ldy, 4 * es) && lies(e.bias, 0, 4 * es) && lies(e.pre, e.ldp, 4 * es) && lies(e.residual, e.ldr, 4 * es);
     const bool tma_out = lies(e.y, e.ldy, 16) && lies(e.bias, 0, 16) && lies(e.pre, e.ldp, 16) && lies(e.residual, e.ldr, 16);
-    TcPlan p = tc_plan(s, true);
-    if (p.pair && p.split == 1 && !tma_out) p = tc_plan(s, false);
+    TcPlan p = tc_plan(s, g.planes, true);
+    if (p.pair && p.split == 1 && !tma_out) p = tc_plan(s, g.planes, false);
     g.split = p.split;
-#define FG_PRODUCT(T)                                                                     \
-    (p.pair ? (p.bn == 256 ? launch_pair<T, 256>(dtype, a, b, s, g, ws, st)               \
-                           : launch_pair<T, 128>(dtype, a, b, s, g, ws, st))              \
+#define FG_PRODUCT(T)                                                                        \
+    (p.pair ? (sizeof(T) == 4 || p.bn == 256                                              \
+                   ? launch_pair<T, 256>(dtype, a, b, s, g, ws, st)                       \
+                   : launch_pair<T, sizeof(T) == 4 ? 256 : 128>(dtype, a, b, s, g, ws, st)) \
             : (p.bn == 256   ? launch_split<T, 256>(dtype, a, b, s, g, st)                \
                : p.bn == 128 ? launch_split<T, 128>(dtype, a, b, s, g, st)                \
                              : launch_split<T, 64>(dtype, a, b, s, g, st)))
-    return dtype == FG_DTYPE_F16 ? FG_PRODUCT(__half) : FG_PRODUCT(__nv_bfloat16);
+    return dtype == FG_DTYPE_F32 ? FG_PRODUCT(float) : dtype == FG_DTYPE_F16 ? FG_PRODUCT(__half) : FG_PRODUCT(__nv_bfloat16);
 #undef FG_PRODUCT
 }
 

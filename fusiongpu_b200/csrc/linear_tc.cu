@@ -29,6 +29,7 @@ struct TcArgs {
     int split;          // parts of a tile's K range: CTAs of a cluster, or passes of the pairs
     int m_pad;          // pairs with split > 1: rows of a part's partial tiles
     int vec;            // outputs, residual and bias allow 4-column accesses
+    int direct;         // pairs: some of them do not start on 16-byte boundaries, which TMA needs
     int planes;         // 1, or 3: float32
     GemmShape f;        // planes == 3: the operands as they lie, for results that are not finite
     const __nv_bfloat16 *fa, *fb;
@@ -405,11 +406,37 @@ __device__ __forceinline__ void activate_all(float (&v)[2][32]) {
 // Columns 2 lane and 2 lane + 1 of a 64-column piece of the bias, packed; fetched
 // before the accumulator is waited for (the operand ring leaves no L1 to find it in).
 template <class T>
-__device__ __forceinline__ uint32_t fetch_bias(const T* b, int lane, int left) {
-    if (2 * lane + 2 <= left) return __ldg(reinterpret_cast<const unsigned*>(b) + lane);
+__device__ __forceinline__ uint32_t fetch_bias(const T* b, int lane, int left, int direct) {
+    if (2 * lane + 2 <= left && !direct) return __ldg(reinterpret_cast<const unsigned*>(b) + lane);
+    const unsigned short* p = reinterpret_cast<const unsigned short*>(b) + 2 * lane;
     uint32_t u = 0;
-    if (2 * lane < left) u = *reinterpret_cast<const unsigned short*>(b + 2 * lane);
+    if (2 * lane < left) u = p[0];
+    if (2 * lane + 1 < left) u |= (uint32_t)p[1] << 16;
     return u;
+}
+
+// A warp's 32 rows of 128 bytes between its swizzled buffer and a matrix whose rows
+// start anywhere: row by row, neighbouring lanes on neighbouring columns.
+template <class T, bool OUT>
+__device__ __forceinline__ void copy_rows(unsigned char* buf, T* matrix, long long ld, int row0, int col0, int rows, int cols,
+                                          int lane) {
+    constexpr int PER = 128 / 32 / (int)sizeof(T);  // columns a lane
+    __syncwarp();
+    for (int r = 0; r < 32 && row0 + r < rows; ++r) {
+        T* p = matrix + (row0 + r) * ld + col0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = lane + 32 * i;
+            T* q = reinterpret_cast<T*>(buf + r * 128 + ((c * (int)sizeof(T)) ^ ((r & 7) << 4)));
+            if (col0 + c < cols) {
+                if (OUT)
+                    p[c] = *q;
+                else
+                    *q = p[c];
+            }
+        }
+    }
+    __syncwarp();
 }
 
 template <class T>
@@ -552,7 +579,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
         };
         const int step = pairs * P::GROUPS;
         int item = (blockIdx.x >> 1) + pairs * group, li = group;
-        if (sizeof(T) == 2 && e.residual && !e.pre && item < items && tc::elect_one()) fetch_residual(item);
+        const bool ahead = sizeof(T) == 2 && e.residual && !e.pre && !g.direct;  // residuals a tile ahead
+        if (ahead && item < items && tc::elect_one()) fetch_residual(item);
         if constexpr (sizeof(T) == 4) {
             // Chunks of k are added to the sums in shared memory, a lane its own row, in
             // two halves of 32 columns; the last one is followed by the epilogue proper,
@@ -643,7 +671,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     }
                     if (e.pre) {
                         stage();
-                        put(&tp, m0, in);
+                        if (g.direct)
+                            copy_rows<T, true>(hbuf, static_cast<T*>(e.pre), e.ldp, m0, c0, g.m, g.n, lane);
+                        else
+                            put(&tp, m0, in);
                     }
                     if (e.act != FG_ACT_NONE) {
 #pragma unroll 4
@@ -652,12 +683,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     if (tc::elect_one()) tc::bulk_wait_read<0>();
                     __syncwarp();
                     if (e.residual) {
-                        if (tc::elect_one()) {
-                            tc::mbar_arrive_expect_tx(&res_full[w], GP_BUF);
-                            tc::tma_load_2d(hbuf, &tr, &res_full[w], c0, m0);
+                        if (g.direct) {
+                            copy_rows<T, false>(hbuf, const_cast<T*>(static_cast<const T*>(e.residual)), e.ldr, m0, c0, g.m, g.n, lane);
+                        } else {
+                            if (tc::elect_one()) {
+                                tc::mbar_arrive_expect_tx(&res_full[w], GP_BUF);
+                                tc::tma_load_2d(hbuf, &tr, &res_full[w], c0, m0);
+                            }
+                            tc::mbar_wait_warp(&res_full[w], res_phase, fail);
+                            res_phase ^= 1;
                         }
-                        tc::mbar_wait_warp(&res_full[w], res_phase, fail);
-                        res_phase ^= 1;
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
                             const float4 r = *reinterpret_cast<const float4*>(hrow + (((uint32_t)j << 2) ^ sw));
@@ -668,7 +703,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         }
                     }
                     stage();
-                    put(&ty, m0, in);
+                    if (g.direct)
+                        copy_rows<T, true>(hbuf, static_cast<T*>(e.y), e.ldy, m0, c0, g.m, g.n, lane);
+                    else
+                        put(&ty, m0, in);
                 }
             }
         } else {
@@ -678,7 +716,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             const bool inside = m0 < g.m && col < g.n;
             unsigned char* bias = biases + w * 128;
             if (e.bias) {
-                reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(static_cast<const T*>(e.bias) + col, lane, g.n - col);
+                reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(static_cast<const T*>(e.bias) + col, lane, g.n - col, g.direct);
                 __syncwarp();
             }
             const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
@@ -728,11 +766,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
 #pragma unroll
                     for (int j = 0; j < 32; j += 8)
                         *reinterpret_cast<uint4*>(brow + (((uint32_t)(32 * h + j) << 1) ^ sw)) = pack8<T>(&v[h][j]);
-                tc::fence_proxy_async();
-                __syncwarp();
-                if (tc::elect_one()) {
-                    if (inside) tc::tma_store_2d(&tp, buf, col, m0);
-                    tc::bulk_commit();
+                if (g.direct) {
+                    copy_rows<T, true>(buf, static_cast<T*>(e.pre), e.ldp, m0, col, g.m, g.n, lane);
+                } else {
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                    if (tc::elect_one()) {
+                        if (inside) tc::tma_store_2d(&tp, buf, col, m0);
+                        tc::bulk_commit();
+                    }
                 }
             }
             switch (e.act) {
@@ -740,16 +782,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 case FG_ACT_GELU: activate_all<FG_ACT_GELU>(v); break;
                 case FG_ACT_SILU: activate_all<FG_ACT_SILU>(v); break;
             }
-            if (e.pre || !e.residual) {  // the buffer's last store has read it
+            if (g.direct) {
+                if (e.residual)
+                    copy_rows<T, false>(buf, const_cast<T*>(static_cast<const T*>(e.residual)), e.ldr, m0, col, g.m, g.n, lane);
+            } else if (!ahead) {  // the buffer's last store has read it
                 if (tc::elect_one()) {
                     tc::bulk_wait_read<0>();
-                    if (e.residual) fetch_residual(t);
+                    if (e.residual) fetch_residual(item);
                 }
                 __syncwarp();
             }
             if (e.residual) {
-                tc::mbar_wait_warp(&res_full[w], res_phase, fail);
-                res_phase ^= 1;
+                if (!g.direct) {
+                    tc::mbar_wait_warp(&res_full[w], res_phase, fail);
+                    res_phase ^= 1;
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -761,12 +808,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
 #pragma unroll
                 for (int j = 0; j < 32; j += 8)
                     *reinterpret_cast<uint4*>(brow + (((uint32_t)(32 * h + j) << 1) ^ sw)) = pack8<T>(&v[h][j]);
+            if (g.direct) {
+                copy_rows<T, true>(buf, static_cast<T*>(e.y), e.ldy, m0, col, g.m, g.n, lane);
+                continue;
+            }
             tc::fence_proxy_async();
             __syncwarp();
             if (tc::elect_one()) {
                 if (inside) tc::tma_store_2d(&ty, buf, col, m0);
                 tc::bulk_commit();
-                if (e.residual && !e.pre && item + step < items) {  // the next tile's residual travels during its products
+                if (ahead && item + step < items) {  // the next tile's residual travels during its products
                     tc::bulk_wait_read<0>();
                     fetch_residual(item + step);
                 }
@@ -903,7 +954,7 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
     if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN / 2, g.planes, g.b_plane);
     if (g.split > 1) {
         if (!rc) rc = tile_map(&ty, FG_DTYPE_F32, ws, (long long)g.split * g.m_pad, ld, ld);
-    } else {
+    } else if (!g.direct) {
         if (!rc) rc = tile_map(&ty, dtype, e.y, s.m, s.n, e.ldy);
         if (!rc) rc = tile_map(&tp, dtype, e.pre, s.m, s.n, e.ldp);
         if (!rc) rc = tile_map(&tr, dtype, e.residual, s.m, s.n, e.ldr);
@@ -916,7 +967,10 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), PairOf<T, BN>::SMEM));
     const int pairs = std::max(1, device_attr(cudaDevAttrMultiProcessorCount) / 2);
     TcArgs k = g;
-    if (g.split > 1) k.e.residual = k.e.pre = nullptr;
+    if (g.split > 1) {
+        k.e.residual = k.e.pre = nullptr;
+        k.direct = 0;
+    }
     kernel<<<2 * (unsigned)std::min<long long>(items, pairs), GP_NT, PairOf<T, BN>::SMEM, st>>>(ta, tb, ty, tp, tr, k);
     rc = check_launch("gemm_pair_kernel");
     if (rc || g.split == 1) return rc;
@@ -941,7 +995,7 @@ struct TcPlan {
     size_t ws;
 };
 
-static TcPlan tc_plan(const GemmShape& s, int planes, bool pairs_fit) {
+static TcPlan tc_plan(const GemmShape& s, int planes) {
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
     const int kt = (int)((s.k + GT_K - 1) / GT_K) * (planes == 1 ? 1 : 6);
     auto waves = [](long long tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
@@ -961,7 +1015,6 @@ static TcPlan tc_plan(const GemmShape& s, int planes, bool pairs_fit) {
         for (int sp : {1, 2, 4, 8, 16, 32}) {
             if (sp > 1 && (sp > kb / 2 || (tiles * sp > sms && kb * 2 / sp <= GT_RUN))) break;
             if (planes == 1 && kb > GT_RUN * sp && sp < 32) continue;
-            if (sp == 1 && !pairs_fit) continue;  // parts go through the workspace, whatever the outputs' alignment
             const size_t ws = sp > 1 ? (size_t)sp * m2 * 2 * GT_M * ((s.n + 3) / 4 * 4) * 4 : 0;
             const double epi = bn == 256 ? 2.0 : 1.0, main = (kt + sp - 1) / sp * (bn == 256 ? 0.39 : 0.34);
             offer(6.0 + waves(tiles * sp, sms / 2) * std::max(main, epi) + epi + (sp > 1 ? 3.0 + 1.5e-6 * ws / 6.0 : 0.0),
@@ -983,8 +1036,7 @@ static TcPlan tc_plan(const GemmShape& s, int planes, bool pairs_fit) {
 }
 
 size_t tc_gemm_workspace(int dtype, const GemmShape& s) {
-    const int planes = dtype == FG_DTYPE_F32 ? 3 : 1;
-    return s.k > 0 ? std::max(tc_plan(s, planes, true).ws, tc_plan(s, planes, false).ws) : 0;
+    return s.k > 0 ? tc_plan(s, dtype == FG_DTYPE_F32 ? 3 : 1).ws : 0;
 }
 
 int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& s,
@@ -1006,9 +1058,8 @@ int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long lon
     const int es = dtype_size(dtype);
     auto lies = [&](const void* p, long long ld, int n) { return !p || (aligned(p, n) && ld * es % n == 0); };
     g.vec = lies(e.y, e.ldy, 4 * es) && lies(e.bias, 0, 4 * es) && lies(e.pre, e.ldp, 4 * es) && lies(e.residual, e.ldr, 4 * es);
-    const bool tma_out = lies(e.y, e.ldy, 16) && lies(e.bias, 0, 16) && lies(e.pre, e.ldp, 16) && lies(e.residual, e.ldr, 16);
-    TcPlan p = tc_plan(s, g.planes, true);
-    if (p.pair && p.split == 1 && !tma_out) p = tc_plan(s, g.planes, false);
+    g.direct = !(lies(e.y, e.ldy, 16) && lies(e.bias, 0, 16) && lies(e.pre, e.ldp, 16) && lies(e.residual, e.ldr, 16));
+    const TcPlan p = tc_plan(s, g.planes);
     g.split = p.split;
 #define FG_PRODUCT(T)                                                                        \
     (p.pair ? (sizeof(T) == 4 || p.bn == 256                                              \

@@ -64,6 +64,10 @@ def _vector(t: torch.Tensor | None, name: str, n: int, dtype, device) -> int | N
     return t.data_ptr()
 
 
+def _rows(like: torch.Tensor, n: int, d: int) -> torch.Tensor:
+    return torch.empty_strided((n, d), (d, 1), dtype=like.dtype, device=like.device)
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -123,7 +127,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     p = weight if weight is not None else bias
     pd = torch.float32 if p is not None and p.dtype == torch.float32 else t
     w, b = _vector(weight, "weight", d, pd, dev), _vector(bias, "bias", d, pd, dev)
-    y = x.new_empty((n, d))
+    y = _rows(x, n, d)
     mean = rstd = None
     if return_stats:
         mean, rstd = torch.empty(n, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
@@ -146,7 +150,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     m, r = _vector(mean, "mean", n, torch.float32, dev), _vector(rstd, "rstd", n, torch.float32, dev)
     pd = torch.float32 if weight is not None and weight.dtype == torch.float32 else t
     w = _vector(weight, "weight", d, pd, dev)
-    dx = x.new_empty((n, d))
+    dx = _rows(x, n, d)
     dw = db = ws = None
     nws = 0
     if param_grads:
@@ -181,8 +185,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, a
     ldr = 0
     if residual is not None:
         residual, ldr = _matrix(residual, "residual", x, n, o)
-    y = x.new_empty((n, o))
-    pre = x.new_empty((n, o)) if return_pre else None
+    y = _rows(x, n, o)
+    pre = _rows(x, n, o) if return_pre else None
     p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, ldr, 0, 0)
     nws = _linear_ws("fg_linear_workspace_size", n, i, o, t, act, ldx, ldw, 0, dev.index)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
@@ -211,8 +215,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: tor
         raise ValueError("the activation's gradient needs pre")
     else:
         pre, ldp = _matrix(pre, "pre", x, n, o)
-    dx = x.new_empty((n, i)) if input_grad else None
-    dw, db = (x.new_empty((o, i)), x.new_empty(o)) if param_grads else (None, None)
+    dx = _rows(x, n, i) if input_grad else None
+    dw, db = (_rows(x, o, i), torch.empty(o, dtype=x.dtype, device=dev)) if param_grads else (None, None)
     p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, 0, ldp, lddy)
     nws = _linear_ws("fg_linear_backward_workspace_size", n, i, o, t, act, ldx, ldw, lddy, dev.index)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
@@ -250,7 +254,7 @@ def preference_loss(queries: torch.Tensor, base: torch.Tensor, offsets: torch.Te
     off = _vector(offsets, "offsets", nq + 1, torch.int64, dev)
     wt = _vector(weights, "weights", m, torch.float32, dev)
     losses, margins = torch.empty(m, dtype=torch.float32, device=dev), torch.empty(m, dtype=torch.float32, device=dev)
-    dq = q.new_empty((nq, d)) if grad else None
+    dq = _rows(q, nq, d) if grad else None
     p = _lib.PreferenceParams(nq, d, DTYPES[q.dtype], BASE_DTYPES[base.dtype], base.shape[0], m, METRICS[metric], beta,
                               label_smoothing, ldq, ldr, 0)
     _lib.check(_lib.lib().fg_preference_loss(C.byref(p), q.data_ptr(), _ptr(ref), base.data_ptr(), off, po, ne, wt,

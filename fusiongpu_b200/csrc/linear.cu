@@ -266,7 +266,7 @@ __device__ __forceinline__ void dz_pair(float& d0, float& d1, float p0, float p1
 }
 
 template <class T, int ACT>
-__global__ void __launch_bounds__(DZ_WARPS * 32) dz_kernel(const DzArgs g) {
+__global__ void __launch_bounds__(DZ_WARPS * 32, 3) dz_kernel(const DzArgs g) {
     constexpr int VEC = 16 / sizeof(T), U = 2;
     __shared__ float s[DZ_WARPS][32 * VEC];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = (blockIdx.x * 32 + lane) * VEC, left = g.dim - j;
@@ -358,10 +358,10 @@ __global__ void __launch_bounds__(1024) dz_reduce_kernel(const float* part, int 
     }
 }
 
-// Row ranges: four blocks to an SM over the column tiles, 16 rows at least to a range.
+// Row ranges: three blocks to an SM over the column tiles, 16 rows at least to a range.
 static int dz_split(long long rows, int dim, int elem) {
     const int cols = 32 * (16 / elem), tiles = (dim + cols - 1) / cols;
-    const long long fill = std::max(1ll, 4ll * std::max(1, device_attr(cudaDevAttrMultiProcessorCount)) / tiles);
+    const long long fill = std::max(1ll, 3ll * std::max(1, device_attr(cudaDevAttrMultiProcessorCount)) / tiles);
     return (int)std::max(1ll, std::min(fill, (rows + 15) / 16));
 }
 

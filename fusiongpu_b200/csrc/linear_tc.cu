@@ -269,24 +269,41 @@ __global__ void __launch_bounds__(GT_NT, 1)
         tc::tmem_dealloc(taddr, NA * BN);
     }
 
-    // Four positions per thread and round, their residuals loaded first: one
-    // memory latency a round.
+    // Four positions per thread and round, their residuals and biases loaded first:
+    // one memory latency a round.
     constexpr int U = 4;
+    constexpr bool FAST = sizeof(T) == 2;
     const int slice = BN / S, per_row = slice / 4;
     const uint32_t pbase = tc::smem_u32(part);
     const Epilogue& e = g.e;
     for (int i0 = tid; i0 < GT_M * per_row; i0 += U * GT_NT) {
         int row[U], col[U];
         uint32_t at[U];
-        float4 res[U];
+        float4 res[U], bias[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * GT_NT, r = i / per_row, c = rank * slice + (i - r * per_row) * 4;
             row[u] = i < GT_M * per_row ? m0 + r : g.m;
             col[u] = n0 + c;
             at[u] = (uint32_t)(r * LDP + c) * 4;
-            if (e.residual && g.vec && row[u] < g.m && col[u] + 4 <= g.n)
-                res[u] = load4(static_cast<const T*>(e.residual) + row[u] * e.ldr + col[u]);
+            res[u] = bias[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (row[u] < g.m && col[u] < g.n) {
+                const T* rp = static_cast<const T*>(e.residual) + row[u] * e.ldr + col[u];
+                const T* bp = static_cast<const T*>(e.bias) + col[u];
+                if (g.vec && col[u] + 4 <= g.n) {
+                    if (e.residual) res[u] = load4(rp);
+                    if (e.bias) bias[u] = load4(bp);
+                } else {
+                    float* rf = &res[u].x;
+                    float* bf = &bias[u].x;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col[u] + j < g.n) {
+                            if (e.residual) rf[j] = to_f32(rp[j]);
+                            if (e.bias) bf[j] = to_f32(bp[j]);
+                        }
+                }
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -304,41 +321,42 @@ __global__ void __launch_bounds__(GT_NT, 1)
             } else {
                 z = *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(part) + at[u]);
             }
-            if (sizeof(T) == 4) {
+            const bool whole = col[u] + 4 <= g.n;
+            if (!FAST) {
                 z.x = finite_or_retake<T>(g, row[u], col[u], z.x);
                 if (col[u] + 1 < g.n) z.y = finite_or_retake<T>(g, row[u], col[u] + 1, z.y);
                 if (col[u] + 2 < g.n) z.z = finite_or_retake<T>(g, row[u], col[u] + 2, z.z);
                 if (col[u] + 3 < g.n) z.w = finite_or_retake<T>(g, row[u], col[u] + 3, z.w);
             }
-            if (g.vec && col[u] + 4 <= g.n) {
-                if (e.bias) {
-                    const float4 b = load4(static_cast<const T*>(e.bias) + col[u]);
-                    z.x += b.x;
-                    z.y += b.y;
-                    z.z += b.z;
-                    z.w += b.w;
+            z.x += bias[u].x;
+            z.y += bias[u].y;
+            z.z += bias[u].z;
+            z.w += bias[u].w;
+            auto put = [&](void* out, long long ld, const float4& v) {
+                T* p = static_cast<T*>(out) + row[u] * ld + col[u];
+                if (g.vec && whole) {
+                    store4(p, v);
+                } else {
+                    const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col[u] + j < g.n) p[j] = from_f32<T>(f[j]);
                 }
-                if (e.pre) store4(static_cast<T*>(e.pre) + row[u] * e.ldp + col[u], z);
-                float4 y = z;
-                if (e.act == FG_ACT_GELU && sizeof(T) == 2) {
-                    gelu2(y.x, y.y);
-                    gelu2(y.z, y.w);
-                } else if (e.act != FG_ACT_NONE) {
-                    constexpr bool FAST = sizeof(T) == 2;
-                    y = make_float4(activate<FAST>(z.x, e.act), activate<FAST>(z.y, e.act),
-                                    activate<FAST>(z.z, e.act), activate<FAST>(z.w, e.act));
-                }
-                if (e.residual) {
-                    y.x += res[u].x;
-                    y.y += res[u].y;
-                    y.z += res[u].z;
-                    y.w += res[u].w;
-                }
-                store4(static_cast<T*>(e.y) + row[u] * e.ldy + col[u], y);
-            } else {
-                const float v[4] = {z.x, z.y, z.z, z.w};
-                for (int j = 0; j < 4 && col[u] + j < g.n; ++j) epilogue_store<T>(e, row[u], col[u] + j, v[j]);
+            };
+            if (e.pre) put(e.pre, e.ldp, z);
+            float4 y = z;
+            if (e.act == FG_ACT_GELU && FAST) {
+                gelu2(y.x, y.y);
+                gelu2(y.z, y.w);
+            } else if (e.act != FG_ACT_NONE) {
+                y = make_float4(activate<FAST>(z.x, e.act), activate<FAST>(z.y, e.act), activate<FAST>(z.z, e.act),
+                                activate<FAST>(z.w, e.act));
             }
+            y.x += res[u].x;
+            y.y += res[u].y;
+            y.z += res[u].z;
+            y.w += res[u].w;
+            put(e.y, e.ldy, y);
         }
     }
     if (S > 1) cluster_sync();  // a peer may still read this CTA's partial tile
@@ -469,9 +487,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     if (warp == 2 && tc::elect_one()) {
         tc::prefetch_map(&ta);
         tc::prefetch_map(&tb);
-        tc::prefetch_map(&ty);
-        if (g.e.pre) tc::prefetch_map(&tp);
-        if (g.e.residual) tc::prefetch_map(&tr);
+        if (!g.direct) {
+            tc::prefetch_map(&ty);
+            if (g.e.pre) tc::prefetch_map(&tp);
+            if (g.e.residual) tc::prefetch_map(&tr);
+        }
     }
     if (tid == 0) {
         s_fail = 0;

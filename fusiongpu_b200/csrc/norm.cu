@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "adapter_common.cuh"
+#include "packed.cuh"
 
 namespace fg {
 
@@ -197,9 +198,21 @@ __global__ void __launch_bounds__(ln_block<G>(), ln_forward_per_sm(G, NCH* VEC, 
     }
 }
 
-// Blocks of the backward kernel per SM (its registers: two rows ahead packed, two
-// sums a column).
-constexpr int ln_per_sm(int G, int E) { return G == 512 ? 1 : G == 128 ? (E > 16 ? 2 : 4) : 2; }
+// Backward: threads of a block and blocks per SM, by registers: a thread holds two sums
+// and w for each of its E columns, x and dy of a row and, AHEAD, of the next one, in
+// their own type (16-bit ones two to a register, but where VEC is 1).
+constexpr int ln_row_regs(int E, int VEC, int bytes) { return 2 * E * (VEC == 1 ? 4 : bytes) / 4; }
+constexpr bool ln_ahead(int E, int VEC, int bytes) { return ln_row_regs(E, VEC, bytes) <= 32; }
+constexpr int ln_backward_regs(int E, int VEC, int bytes) {
+    return 3 * E + ln_row_regs(E, VEC, bytes) * (ln_ahead(E, VEC, bytes) ? 2 : 1) + 32;
+}
+constexpr int ln_backward_block(int G, int E, int VEC, int bytes) {
+    return G >= 128 ? G : ln_backward_regs(E, VEC, bytes) > 128 ? 384 : 256;
+}
+constexpr int ln_backward_per_sm(int G, int E, int VEC, int bytes) {
+    const int n = 65536 / (128 * ln_backward_regs(E, VEC, bytes));
+    return G == 512 ? 1 : G == 128 ? (n < 4 ? n : 4) : ln_backward_block(G, E, VEC, bytes) == 384 ? 1 : 2;
+}
 
 // Sums of two values over the group.
 template <int G>
@@ -225,19 +238,36 @@ __device__ __forceinline__ void group_sum2(float& a, float& b, float (*s)[2]) {
 }
 
 // Groups take rows in turn; x and dy of the next row are fetched before this one
-// is worked on (not where a thread holds 32 columns), and stay in their own type
-// until they are used.  The sums for the weight's gradients are in registers (G =
-// 512: in shared memory, each thread its own columns).
+// is worked on, and stay in their own type until they are used.  The sums for the
+// weight's gradients are in registers (G = 512: in shared memory, each thread its own
+// columns, and w is read for each row).  Arithmetic is packed, two columns an
+// instruction: BWDFIG
 template <class T, int VEC, int NCH, int G>
-__global__ void __launch_bounds__(ln_block<G>(), ln_per_sm(G, NCH * VEC)) ln_backward_kernel(const NormArgs g) {
-    constexpr int NT = ln_block<G>(), RPB = NT / G, E = NCH * VEC;
-    constexpr bool SMEM = G == 512, AHEAD = E <= 24;
+__global__ void __launch_bounds__(ln_backward_block(G, NCH* VEC, VEC, sizeof(T)),
+                                  ln_backward_per_sm(G, NCH* VEC, VEC, sizeof(T))) ln_backward_kernel(const NormArgs g) {
+    constexpr int E = NCH * VEC, NT = ln_backward_block(G, E, VEC, sizeof(T)), RPB = NT / G;
+    constexpr bool SMEM = G == 512, AHEAD = ln_ahead(E, VEC, sizeof(T));
     extern __shared__ float sm[];
     __shared__ float s[NT / 32][2];
     const int gl = threadIdx.x % G;
     const float inv = 1.0f / (float)g.dim;
     const long long step = (long long)gridDim.x * RPB;
-    float dw[SMEM ? 1 : E], db[SMEM ? 1 : E];
+    uint64_t dw[SMEM ? 1 : E / 2], db[SMEM ? 1 : E / 2];
+    constexpr int P = VEC < 2 ? 2 : VEC;  // columns whose parameters are loaded and results stored together
+    float w[SMEM ? P : E];
+    auto column = [&](int e) { return (e / VEC * G + gl) * VEC + e % VEC; };
+    auto params = [&](int e) {  // of columns e .. e + P - 1
+#pragma unroll
+        for (int i = 0; i < P; i += VEC) {
+            float* at = w + (SMEM ? i : e + i);
+            if (column(e + i) < g.dim)
+                load_params<T, VEC>(at, g.w, g.w_f32, g.wide, column(e + i), 1.0f);
+            else
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) at[k] = 0.0f;
+        }
+    };
+    auto weights = [&](int e) { return pair2(w[SMEM ? e % P : e], w[SMEM ? e % P + 1 : e + 1]); };
     if (SMEM) {
         for (int k = 0; k < NCH; ++k)
             for (int i = 0; i < VEC; ++i) {
@@ -246,14 +276,28 @@ __global__ void __launch_bounds__(ln_block<G>(), ln_per_sm(G, NCH * VEC)) ln_bac
             }
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.0f;
+        for (int i = 0; i < E / 2; ++i) dw[i] = db[i] = 0;
     }
+    // Columns and rows that are not there are zeros, and add nothing.
     struct Row {
         Chunk<T, VEC> x[NCH], d[NCH];
         float mean, rstd;
+        __device__ __forceinline__ float2 get(const Chunk<T, VEC> (&c)[NCH], int e) const {
+            return make_float2(to_f32(c[e / VEC].v[e % VEC]), to_f32(c[(e + 1) / VEC].v[(e + 1) % VEC]));
+        }
+    };
+    auto clear = [&](Row& row) {
+        row.mean = row.rstd = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) row.x[k].v[i] = row.d[k].v[i] = from_f32<T>(0.0f);
     };
     auto fetch = [&](Row& row, long long r) {
-        if (r >= g.rows) return;
+        if (r >= g.rows) {
+            clear(row);
+            return;
+        }
         const T* x = static_cast<const T*>(g.x) + r * g.ldx;
         const T* d = static_cast<const T*>(g.dy) + r * g.ldy;
 #pragma unroll
@@ -269,61 +313,79 @@ __global__ void __launch_bounds__(ln_block<G>(), ln_per_sm(G, NCH * VEC)) ln_bac
     };
     Row cur, next;
     const long long first = (long long)blockIdx.x * RPB + threadIdx.x / G;
+    clear(AHEAD ? next : cur);
     if (AHEAD) fetch(next, first);
+    if (!SMEM) {
+#pragma unroll
+        for (int e = 0; e < E; e += P) params(e);
+    }
     for (long long r = first, r0 = r - (threadIdx.x % 32) / G; (G > 32 ? r : r0) < g.rows; r += step, r0 += step) {
-        const bool in = r < g.rows;
         if (AHEAD) {
             cur = next;
             fetch(next, r + step);
         } else {
             fetch(cur, r);
         }
-        float sa = 0.0f, sah = 0.0f;
+        const uint64_t off = pair2(-cur.mean, -cur.mean), by = pair2(cur.rstd, cur.rstd);
+        uint64_t sa2 = 0, sah2 = 0;
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const int j = (k * G + gl) * VEC;
-            if (in && j < g.dim) {
-                float w[VEC];
-                load_params<T, VEC>(w, g.w, g.w_f32, g.wide, j, 1.0f);
+        for (int e = 0; e < E; e += 2) {
+            const float2 xf = cur.get(cur.x, e), df = cur.get(cur.d, e);
+            const uint64_t d = pair2(df.x, df.y), h = mul2(add2(pair2(xf.x, xf.y), off), by);
+            if (SMEM && e % P == 0) params(e);
+            const uint64_t a = mul2(d, weights(e));
+            if (SMEM) {
+                float dh[2];
+                unpair2(mul2(d, h), dh[0], dh[1]);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float d = to_f32(cur.d[k].v[i]), h = (to_f32(cur.x[k].v[i]) - cur.mean) * cur.rstd;
-                    const float a = d * w[i];
-                    if (SMEM) {
-                        sm[j + i] = fmaf(d, h, sm[j + i]);
-                        sm[g.dim + j + i] += d;
-                    } else {
-                        dw[k * VEC + i] = fmaf(d, h, dw[k * VEC + i]);
-                        db[k * VEC + i] += d;
+                for (int i = 0; i < 2; ++i) {
+                    const int j = column(e + i);
+                    if (j < g.dim) {
+                        sm[j] += dh[i];
+                        sm[g.dim + j] += i ? df.y : df.x;
                     }
-                    sa += a;
-                    sah = fmaf(a, h, sah);
                 }
+            } else {
+                dw[SMEM ? 0 : e / 2] = fma2(d, h, dw[SMEM ? 0 : e / 2]);
+                db[SMEM ? 0 : e / 2] = add2(d, db[SMEM ? 0 : e / 2]);
             }
+            sa2 = add2(sa2, a);
+            sah2 = fma2(a, h, sah2);
         }
         if (!g.dx) continue;
+        float sa, sah, sa1, sah1;
+        unpair2(sa2, sa, sa1);
+        unpair2(sah2, sah, sah1);
+        sa += sa1;
+        sah += sah1;
         group_sum2<G>(sa, sah, s);
-        sa *= inv;
-        sah *= inv;
-        if (!in) continue;
+        if (r >= g.rows) continue;
+        const uint64_t ma = pair2(-sa * inv, -sa * inv), mah = pair2(-sah * inv, -sah * inv);
         T* dx = static_cast<T*>(g.dx) + r * g.lddx;
+        float o[P];
 #pragma unroll
-        for (int k = 0; k < NCH; ++k) {
-            const int j = (k * G + gl) * VEC;
-            if (j < g.dim) {
-                float w[VEC], o[VEC];
-                load_params<T, VEC>(w, g.w, g.w_f32, g.wide, j, 1.0f);
+        for (int e = 0; e < E; e += 2) {
+            if (SMEM && e % P == 0) params(e);
+            const float2 xf = cur.get(cur.x, e), df = cur.get(cur.d, e);
+            const uint64_t h = mul2(add2(pair2(xf.x, xf.y), off), by);
+            const uint64_t a = fma2(pair2(df.x, df.y), weights(e), ma);  // dy w - avg(a)
+            unpair2(mul2(by, fma2(h, mah, a)), o[e % P], o[e % P + 1]);
+            if ((e + 2) % P == 0) {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float h = (to_f32(cur.x[k].v[i]) - cur.mean) * cur.rstd;
-                    o[i] = cur.rstd * (to_f32(cur.d[k].v[i]) * w[i] - sa - h * sah);
+                for (int i = 0; i < P; i += VEC) {
+                    const int j = column(e + 2 - P + i);
+                    if (j < g.dim) store_chunk<T, VEC>(dx + j, o + i, g.wide);
                 }
-                store_chunk<T, VEC>(dx + j, o, g.wide);
             }
         }
     }
     if (!g.params) return;
     float* part = g.part + (size_t)blockIdx.x * 2 * g.dim;
+    auto sum_of = [&](const uint64_t* v, int e) {
+        float f[2];
+        unpair2(v[SMEM ? 0 : e / 2], f[0], f[1]);
+        return f[e & 1];
+    };
     if (G > 32) {
 #pragma unroll
         for (int k = 0; k < NCH; ++k)
@@ -331,8 +393,8 @@ __global__ void __launch_bounds__(ln_block<G>(), ln_per_sm(G, NCH * VEC)) ln_bac
             for (int i = 0; i < VEC; ++i) {
                 const int j = (k * G + gl) * VEC + i;
                 if (j < g.dim) {
-                    part[j] = SMEM ? sm[j] : dw[SMEM ? 0 : k * VEC + i];
-                    part[g.dim + j] = SMEM ? sm[g.dim + j] : db[SMEM ? 0 : k * VEC + i];
+                    part[j] = SMEM ? sm[j] : sum_of(dw, k * VEC + i);
+                    part[g.dim + j] = SMEM ? sm[g.dim + j] : sum_of(db, k * VEC + i);
                 }
             }
         return;
@@ -343,7 +405,7 @@ __global__ void __launch_bounds__(ln_block<G>(), ln_per_sm(G, NCH * VEC)) ln_bac
     for (int k = 0; k < NCH; ++k)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            float u = dw[SMEM ? 0 : k * VEC + i], v = db[SMEM ? 0 : k * VEC + i];
+            float u = sum_of(dw, k * VEC + i), v = sum_of(db, k * VEC + i);
 #pragma unroll
             for (int o = G; o < 32; o <<= 1) {
                 u += __shfl_xor_sync(0xffffffffu, u, o);
@@ -396,18 +458,15 @@ static int norm_check(int dtype, int param_dtype, long long rows, int dim) {
     return FG_OK;
 }
 
-// Blocks of the backward pass for groups of G threads with E columns each: the SMs
-// filled once, and two rows at least to a group.
-static int norm_parts(long long rows, int G, int E) {
-    const long long rpb = G < 128 ? 256 / G : 1, want = (rows + 2 * rpb - 1) / (2 * rpb);
-    const long long fill = (long long)std::max(1, device_attr(cudaDevAttrMultiProcessorCount)) * ln_per_sm(G, E);
+// Blocks of the backward pass: the SMs filled once, and two rows at least to a group.
+static int norm_parts(long long rows, int rows_per_block, int per_sm) {
+    const long long want = (rows + 2ll * rows_per_block - 1) / (2ll * rows_per_block);
+    const long long fill = (long long)std::max(1, device_attr(cudaDevAttrMultiProcessorCount)) * per_sm;
     return (int)std::min(fill, std::max(want, 1ll));
 }
 
-static size_t norm_ws(long long rows, int dim) {  // for whichever group the alignment selects
-    const int parts = std::max(std::max(norm_parts(rows, 8, 16), norm_parts(rows, 32, 16)),
-                               std::max(norm_parts(rows, 128, 16), norm_parts(rows, 512, 32)));
-    return (size_t)parts * 2 * dim * sizeof(float);
+static size_t norm_ws(long long rows, int dim) {  // for whichever group the type selects: at most four blocks an SM
+    return (size_t)norm_parts(rows, 1, 4) * 2 * dim * sizeof(float);
 }
 
 template <class T, int VEC, int NCH, int G>
@@ -420,11 +479,12 @@ static int launch_norm(const NormArgs& g, bool backward, int* parts, cudaStream_
         ln_forward_kernel<T, VEC, NCH, G><<<(unsigned)std::min(blocks, fill), NT, 0, st>>>(g);
         return check_launch("ln_forward_kernel");
     }
-    const int smem = (G == 128 ? 0 : G == 512 ? 1 : NT / 32) * 2 * g.dim * (int)sizeof(float);
+    constexpr int E = NCH * VEC, BT = ln_backward_block(G, E, VEC, sizeof(T));
+    const int smem = (G == 128 ? 0 : G == 512 ? 1 : BT / 32) * 2 * g.dim * (int)sizeof(float);
     auto kernel = &ln_backward_kernel<T, VEC, NCH, G>;
     if (smem > 40 * 1024) FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
-    *parts = norm_parts(g.rows, G, NCH * VEC);
-    kernel<<<*parts, NT, smem, st>>>(g);
+    *parts = norm_parts(g.rows, BT / G, ln_backward_per_sm(G, E, VEC, sizeof(T)));
+    kernel<<<*parts, BT, smem, st>>>(g);
     return check_launch("ln_backward_kernel");
 }
 

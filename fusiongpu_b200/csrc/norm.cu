@@ -30,12 +30,11 @@ struct NormArgs {
     long long rows, ldx, ldy, lddx;
     int dim, w_f32;
     int params;  // the weight's gradients are wanted
-    int wide;    // rows and parameters start on 16-byte boundaries
     float eps;
 };
 
-// VEC elements of a row: one 16-byte access where every row starts on a 16-byte
-// boundary (wide), else single ones, in the same place of the same thread: the
+// VEC elements of a row: one 16-byte access where every row and the parameters start
+// on a 16-byte boundary (wide), else single ones, in the same place of the same thread: the
 // results do not depend on alignment.  VEC is 1 where dim is no multiple of 16 bytes.
 template <class T, int VEC>
 struct Chunk {
@@ -121,7 +120,7 @@ constexpr int ln_forward_per_sm(int G, int E, int bytes) {
 // read from L1 for every row instead, 1,000,000 x 768 f16 with float parameters took
 // 985 us, not FWDFIG: 6 KB of them to a row of 1.5 KB.)  Not so for G = 512, whose
 // registers hold one row: there w and b are read for each.
-template <class T, int VEC, int NCH, int G>
+template <class T, int VEC, int NCH, int G, bool WIDE>
 __global__ void __launch_bounds__(ln_block<G>(), ln_forward_per_sm(G, NCH* VEC, sizeof(T))) ln_forward_kernel(const NormArgs g) {
     constexpr int NT = ln_block<G>(), RPB = NT / G, E = NCH * VEC;
     constexpr bool HOLD = G < 512;
@@ -136,15 +135,15 @@ __global__ void __launch_bounds__(ln_block<G>(), ln_forward_per_sm(G, NCH* VEC, 
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
             const int j = (k * G + gl) * VEC;
-            if (j < g.dim) load_chunk<T, VEC>(c[k], x + j, g.wide);
+            if (j < g.dim) load_chunk<T, VEC>(c[k], x + j, WIDE);
         }
     };
     float w[HOLD ? E : VEC], b[HOLD ? E : VEC];
     auto params = [&](int k, int at) {
         const int j = (k * G + gl) * VEC;
         if (j < g.dim) {
-            load_params<T, VEC>(w + at, g.w, g.w_f32, g.wide, j, 1.0f);
-            load_params<T, VEC>(b + at, g.b, g.w_f32, g.wide, j, 0.0f);
+            load_params<T, VEC>(w + at, g.w, g.w_f32, WIDE, j, 1.0f);
+            load_params<T, VEC>(b + at, g.b, g.w_f32, WIDE, j, 0.0f);
         }
     };
     const long long first = (long long)blockIdx.x * RPB + threadIdx.x / G;
@@ -188,7 +187,7 @@ __global__ void __launch_bounds__(ln_block<G>(), ln_forward_per_sm(G, NCH* VEC, 
                 float o[VEC];
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) o[i] = fmaf(__fmul_rn(v[k * VEC + i], rstd), w[at + i], b[at + i]);
-                store_chunk<T, VEC>(y + j, o, g.wide);
+                store_chunk<T, VEC>(y + j, o, WIDE);
             }
         }
         if (g.out_mean && gl == 0) {
@@ -207,11 +206,12 @@ constexpr int ln_backward_regs(int E, int VEC, int bytes) {
     return 3 * E + ln_row_regs(E, VEC, bytes) * (ln_ahead(E, VEC, bytes) ? 2 : 1) + 32;
 }
 constexpr int ln_backward_block(int G, int E, int VEC, int bytes) {
-    return G >= 128 ? G : ln_backward_regs(E, VEC, bytes) > 128 ? 384 : 256;
+    const int regs = ln_backward_regs(E, VEC, bytes);
+    return G >= 128 ? G : regs > 128 && regs <= 168 ? 384 : 256;
 }
 constexpr int ln_backward_per_sm(int G, int E, int VEC, int bytes) {
     const int n = 65536 / (128 * ln_backward_regs(E, VEC, bytes));
-    return G == 512 ? 1 : G == 128 ? (n < 4 ? n : 4) : ln_backward_block(G, E, VEC, bytes) == 384 ? 1 : 2;
+    return G == 512 ? 1 : G == 128 ? (n < 6 ? n : 6) : ln_backward_regs(E, VEC, bytes) > 128 ? 1 : 2;
 }
 
 // Sums of two values over the group.
@@ -242,7 +242,7 @@ __device__ __forceinline__ void group_sum2(float& a, float& b, float (*s)[2]) {
 // weight's gradients are in registers (G = 512: in shared memory, each thread its own
 // columns, and w is read for each row).  Arithmetic is packed, two columns an
 // instruction: BWDFIG
-template <class T, int VEC, int NCH, int G>
+template <class T, int VEC, int NCH, int G, bool WIDE>
 __global__ void __launch_bounds__(ln_backward_block(G, NCH* VEC, VEC, sizeof(T)),
                                   ln_backward_per_sm(G, NCH* VEC, VEC, sizeof(T))) ln_backward_kernel(const NormArgs g) {
     constexpr int E = NCH * VEC, NT = ln_backward_block(G, E, VEC, sizeof(T)), RPB = NT / G;
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(ln_backward_block(G, NCH* VEC, VEC, sizeof(T))
         for (int i = 0; i < P; i += VEC) {
             float* at = w + (SMEM ? i : e + i);
             if (column(e + i) < g.dim)
-                load_params<T, VEC>(at, g.w, g.w_f32, g.wide, column(e + i), 1.0f);
+                load_params<T, VEC>(at, g.w, g.w_f32, WIDE, column(e + i), 1.0f);
             else
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) at[k] = 0.0f;
@@ -304,8 +304,8 @@ __global__ void __launch_bounds__(ln_backward_block(G, NCH* VEC, VEC, sizeof(T))
         for (int k = 0; k < NCH; ++k) {
             const int j = (k * G + gl) * VEC;
             if (j < g.dim) {
-                load_chunk<T, VEC>(row.x[k], x + j, g.wide);
-                load_chunk<T, VEC>(row.d[k], d + j, g.wide);
+                load_chunk<T, VEC>(row.x[k], x + j, WIDE);
+                load_chunk<T, VEC>(row.d[k], d + j, WIDE);
             }
         }
         row.mean = __ldg(g.mean + r);
@@ -374,77 +374,90 @@ __global__ void __launch_bounds__(ln_backward_block(G, NCH* VEC, VEC, sizeof(T))
 #pragma unroll
                 for (int i = 0; i < P; i += VEC) {
                     const int j = column(e + 2 - P + i);
-                    if (j < g.dim) store_chunk<T, VEC>(dx + j, o + i, g.wide);
+                    if (j < g.dim) store_chunk<T, VEC>(dx + j, o + i, WIDE);
                 }
             }
         }
     }
     if (!g.params) return;
     float* part = g.part + (size_t)blockIdx.x * 2 * g.dim;
-    auto sum_of = [&](const uint64_t* v, int e) {
-        float f[2];
-        unpair2(v[SMEM ? 0 : e / 2], f[0], f[1]);
-        return f[e & 1];
-    };
-    if (G > 32) {
+    // A thread's sums, four columns at a time where its columns come in fours (then
+    // dim is a multiple of 4), to `to`; the groups of a warp are added first.
+    constexpr int Q = VEC >= 4 ? 4 : 1;
+    auto put = [&](float* to) {
 #pragma unroll
-        for (int k = 0; k < NCH; ++k)
+        for (int e = 0; e < E; e += Q) {
+            alignas(16) float f[2][Q];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int j = (k * G + gl) * VEC + i;
-                if (j < g.dim) {
-                    part[j] = SMEM ? sm[j] : sum_of(dw, k * VEC + i);
-                    part[g.dim + j] = SMEM ? sm[g.dim + j] : sum_of(db, k * VEC + i);
+            for (int i = 0; i < Q; ++i) {
+                const int at = SMEM ? 0 : (e + i) / 2;
+                float u[2], v[2];
+                unpair2(dw[at], u[0], u[1]);
+                unpair2(db[at], v[0], v[1]);
+                f[0][i] = u[(e + i) & 1];
+                f[1][i] = v[(e + i) & 1];
+#pragma unroll
+                for (int o = G; o < 32; o <<= 1) {
+                    f[0][i] += __shfl_xor_sync(0xffffffffu, f[0][i], o);
+                    f[1][i] += __shfl_xor_sync(0xffffffffu, f[1][i], o);
                 }
             }
-        return;
-    }
-    // groups of a warp, then the warps of the block
-    float* mine = sm + (threadIdx.x >> 5) * 2 * g.dim;
-#pragma unroll
-    for (int k = 0; k < NCH; ++k)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            float u = sum_of(dw, k * VEC + i), v = sum_of(db, k * VEC + i);
-#pragma unroll
-            for (int o = G; o < 32; o <<= 1) {
-                u += __shfl_xor_sync(0xffffffffu, u, o);
-                v += __shfl_xor_sync(0xffffffffu, v, o);
-            }
-            const int j = (k * G + gl) * VEC + i;
-            if (j < g.dim && (threadIdx.x & 31) < G) {
-                mine[j] = u;
-                mine[g.dim + j] = v;
+            const int j = column(e);
+            if (j < g.dim && (G >= 32 || (threadIdx.x & 31) < G)) {
+                if (Q == 4) {
+                    *reinterpret_cast<float4*>(to + j) = *reinterpret_cast<const float4*>(f[0]);
+                    *reinterpret_cast<float4*>(to + g.dim + j) = *reinterpret_cast<const float4*>(f[1]);
+                } else {
+                    to[j] = f[0][0];
+                    to[g.dim + j] = f[1][0];
+                }
             }
         }
+    };
+    if (G == 128) {
+        put(part);
+        return;
+    }
+    // the warps of the block, in order
+    if (!SMEM) put(sm + (threadIdx.x >> 5) * 2 * g.dim);
     __syncthreads();
     for (int j = threadIdx.x; j < 2 * g.dim; j += NT) {
         float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NT / 32; ++w) v += sm[w * 2 * g.dim + j];
+        for (int w = 0; w < (SMEM ? 1 : NT / 32); ++w) v += sm[w * 2 * g.dim + j];
         part[j] = v;
     }
 }
 
-// Adds the partial rows: 32 columns per block, warp w the rows w, w + 32, ... in
-// order, then the warps in order.
+// Adds the partial rows: 32 columns per block, 16 threads of two along them; group w
+// of 64 takes the rows w, w + 64, ... in order, then the groups are added in order.
 template <class P>
 __global__ void __launch_bounds__(1024) ln_reduce_kernel(const float* part, int parts, int dim, P* dw, P* db) {
-    __shared__ float s[32][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
-    float v = 0.0f;
-    if (j < 2 * dim) {
-#pragma unroll 8
-        for (int p = warp; p < parts; p += 32) v += part[(size_t)p * 2 * dim + j];
+    __shared__ float s[64][33];
+    const int c = threadIdx.x % 16 * 2, group = threadIdx.x / 16, j0 = blockIdx.x * 32;
+    float2 v = make_float2(0.0f, 0.0f);
+    if (j0 + c < 2 * dim) {
+#pragma unroll 16
+        for (int p = group; p < parts; p += 64) {
+            const float2 u = __ldg(reinterpret_cast<const float2*>(part + (size_t)p * 2 * dim + j0 + c));
+            v.x += u.x;
+            v.y += u.y;
+        }
     }
-    s[warp][lane] = v;
+    s[group][c] = v.x;
+    s[group][c + 1] = v.y;
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = j0 + lane;
+    const float two = s[2 * warp][lane] + s[2 * warp + 1][lane];
+    __syncthreads();
+    s[warp][lane] = two;
     __syncthreads();
     if (warp == 0 && j < 2 * dim) {
-        v = 0.0f;
+        float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 32; ++w) v += s[w][lane];
+        for (int w = 0; w < 32; ++w) sum += s[w][lane];
         P* out = j < dim ? dw : db;
-        if (out) out[j < dim ? j : j - dim] = from_f32<P>(v);
+        if (out) out[j < dim ? j : j - dim] = from_f32<P>(sum);
     }
 }
 
@@ -465,23 +478,23 @@ static int norm_parts(long long rows, int rows_per_block, int per_sm) {
     return (int)std::min(fill, std::max(want, 1ll));
 }
 
-static size_t norm_ws(long long rows, int dim) {  // for whichever group the type selects: at most four blocks an SM
-    return (size_t)norm_parts(rows, 1, 4) * 2 * dim * sizeof(float);
+static size_t norm_ws(long long rows, int dim) {  // for whichever group the type selects: at most six blocks an SM
+    return (size_t)norm_parts(rows, 1, 6) * 2 * dim * sizeof(float);
 }
 
-template <class T, int VEC, int NCH, int G>
+template <class T, int VEC, int NCH, int G, bool WIDE>
 static int launch_norm(const NormArgs& g, bool backward, int* parts, cudaStream_t st) {
     constexpr int NT = ln_block<G>();
     if (!backward) {
         const long long blocks = (g.rows + NT / G - 1) / (NT / G);
         const long long fill = (long long)std::max(1, device_attr(cudaDevAttrMultiProcessorCount)) *
                                ln_forward_per_sm(G, NCH * VEC, sizeof(T));
-        ln_forward_kernel<T, VEC, NCH, G><<<(unsigned)std::min(blocks, fill), NT, 0, st>>>(g);
+        ln_forward_kernel<T, VEC, NCH, G, WIDE><<<(unsigned)std::min(blocks, fill), NT, 0, st>>>(g);
         return check_launch("ln_forward_kernel");
     }
     constexpr int E = NCH * VEC, BT = ln_backward_block(G, E, VEC, sizeof(T));
     const int smem = (G == 128 ? 0 : G == 512 ? 1 : BT / 32) * 2 * g.dim * (int)sizeof(float);
-    auto kernel = &ln_backward_kernel<T, VEC, NCH, G>;
+    auto kernel = &ln_backward_kernel<T, VEC, NCH, G, WIDE>;
     if (smem > 40 * 1024) FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
     *parts = norm_parts(g.rows, BT / G, ln_backward_per_sm(G, E, VEC, sizeof(T)));
     kernel<<<*parts, BT, smem, st>>>(g);
@@ -494,16 +507,18 @@ static int dispatch_norm(NormArgs g, bool backward, int* parts, cudaStream_t st)
     constexpr int V = 16 / sizeof(T);
     auto lies = [&](const void* p, long long ld) { return !p || (aligned(p, 16) && ld * sizeof(T) % 16 == 0); };
     const bool vec = g.dim % V == 0;
-    g.wide = lies(g.x, g.ldx) && lies(backward ? g.dy : g.y, g.ldy) && lies(g.dx, g.lddx) &&
-                     lies(g.w, 0) && lies(g.b, 0);
+    const bool wide = lies(g.x, g.ldx) && lies(backward ? g.dy : g.y, g.ldy) && lies(g.dx, g.lddx) && lies(g.w, 0) && lies(g.b, 0);
 #define FG_NORM(VEC, NCH, G) \
-    if (g.dim <= (VEC) * (NCH) * (G)) return launch_norm<T, VEC, NCH, G>(g, backward, parts, st)
+    if (g.dim <= (VEC) * (NCH) * (G))   \
+    return wide && VEC > 1 ? launch_norm<T, VEC, NCH, G, (VEC > 1)>(g, backward, parts, st) \
+                           : launch_norm<T, VEC, NCH, G, false>(g, backward, parts, st)
     if constexpr (V == 8) {
         if (vec) {
             FG_NORM(8, 1, 8);
             FG_NORM(8, 2, 8);
             FG_NORM(8, 2, 32);
             FG_NORM(8, 3, 32);
+            if (backward) FG_NORM(8, 4, 32);
             FG_NORM(8, 1, 128);
             FG_NORM(8, 2, 128);
             FG_NORM(8, 4, 128);
@@ -526,7 +541,7 @@ static int dispatch_norm(NormArgs g, bool backward, int* parts, cudaStream_t st)
     FG_NORM(1, 8, 128);
     FG_NORM(1, 16, 128);
     FG_NORM(1, 32, 128);
-    return launch_norm<T, 1, 32, 512>(g, backward, parts, st);
+    return launch_norm<T, 1, 32, 512, false>(g, backward, parts, st);
 #undef FG_NORM
 }
 

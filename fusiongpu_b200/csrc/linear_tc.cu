@@ -310,9 +310,9 @@ __global__ void __launch_bounds__(GT_NT, 1)
             if (row[u] >= g.m || col[u] >= g.n) continue;
             float4 z;
             if (S > 1) {
-                z = ld_cluster_f4(pbase + at[u], 0);
+                z = ld_cluster_f4(pbase + at[u], rank);
                 for (int s = 1; s < S; ++s) {
-                    const float4 v = ld_cluster_f4(pbase + at[u], s);
+                    const float4 v = ld_cluster_f4(pbase + at[u], (rank + s) & (S - 1));
                     z.x += v.x;
                     z.y += v.y;
                     z.z += v.z;
@@ -434,25 +434,32 @@ __device__ __forceinline__ uint32_t fetch_bias(const T* b, int lane, int left, i
 }
 
 // A warp's 32 rows of 128 bytes between its swizzled buffer and a matrix whose rows
-// start anywhere: row by row, neighbouring lanes on neighbouring columns.
-template <class T, bool OUT>
+// start anywhere: row by row, neighbouring lanes on neighbouring columns, R rows
+// under way at once.
+template <class T, bool OUT, int R>
 __device__ __forceinline__ void copy_rows(unsigned char* buf, T* matrix, long long ld, int row0, int col0, int rows, int cols,
                                           int lane) {
     constexpr int PER = 128 / 32 / (int)sizeof(T);  // columns a lane
     __syncwarp();
-    for (int r = 0; r < 32 && row0 + r < rows; ++r) {
-        T* p = matrix + (row0 + r) * ld + col0;
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32 && row0 + r0 < rows; r0 += R) {
+        T v[R][PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int c = lane + 32 * i;
-            T* q = reinterpret_cast<T*>(buf + r * 128 + ((c * (int)sizeof(T)) ^ ((r & 7) << 4)));
-            if (col0 + c < cols) {
-                if (OUT)
-                    p[c] = *q;
-                else
-                    *q = p[c];
-            }
-        }
+        for (int k = 0; k < 2; ++k)  // read, then write
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int c = lane + 32 * i, at = r0 + r;
+                    T* p = matrix + (row0 + at) * ld + col0 + c;
+                    T* q = reinterpret_cast<T*>(buf + at * 128 + ((c * (int)sizeof(T)) ^ ((at & 7) << 4)));
+                    if (col0 + c < cols && row0 + at < rows) {
+                        if (k == 0)
+                            v[r][i] = OUT ? *q : *p;
+                        else
+                            *(OUT ? p : q) = v[r][i];
+                    }
+                }
     }
     __syncwarp();
 }
@@ -465,7 +472,9 @@ __device__ __forceinline__ void add_bias(float (&v)[2][32], const unsigned char*
         for (int j = 0; j < 32; j += 8) add8<T>(&v[h][j], *reinterpret_cast<const uint4*>(b + (32 * h + j) * 2));
 }
 
-template <class T, int BN>
+// DIRECT: outputs, residual or bias do not start on 16-byte boundaries, which TMA
+// needs: they pass row by row between memory and the buffer.
+template <class T, int BN, bool DIRECT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                      const __grid_constant__ CUtensorMap ty, const __grid_constant__ CUtensorMap tp,
@@ -487,7 +496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     if (warp == 2 && tc::elect_one()) {
         tc::prefetch_map(&ta);
         tc::prefetch_map(&tb);
-        if (!g.direct) {
+        if (!DIRECT) {
             tc::prefetch_map(&ty);
             if (g.e.pre) tc::prefetch_map(&tp);
             if (g.e.residual) tc::prefetch_map(&tr);
@@ -599,8 +608,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
         };
         const int step = pairs * P::GROUPS;
         int item = (blockIdx.x >> 1) + pairs * group, li = group;
-        const bool ahead = sizeof(T) == 2 && e.residual && !e.pre && !g.direct;  // residuals a tile ahead
-        if (ahead && item < items && tc::elect_one()) fetch_residual(item);
+        const bool ahead = sizeof(T) == 2 && e.residual && !e.pre;  // residuals a tile ahead (DIRECT: during its products)
+        if (!DIRECT && ahead && item < items && tc::elect_one()) fetch_residual(item);
         if constexpr (sizeof(T) == 4) {
             // Chunks of k are added to the sums in shared memory, a lane its own row, in
             // two halves of 32 columns; the last one is followed by the epilogue proper,
@@ -691,8 +700,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     }
                     if (e.pre) {
                         stage();
-                        if (g.direct)
-                            copy_rows<T, true>(hbuf, static_cast<T*>(e.pre), e.ldp, m0, c0, g.m, g.n, lane);
+                        if (DIRECT)
+                            copy_rows<T, true, 1>(hbuf, static_cast<T*>(e.pre), e.ldp, m0, c0, g.m, g.n, lane);
                         else
                             put(&tp, m0, in);
                     }
@@ -703,8 +712,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     if (tc::elect_one()) tc::bulk_wait_read<0>();
                     __syncwarp();
                     if (e.residual) {
-                        if (g.direct) {
-                            copy_rows<T, false>(hbuf, const_cast<T*>(static_cast<const T*>(e.residual)), e.ldr, m0, c0, g.m, g.n, lane);
+                        if (DIRECT) {
+                            copy_rows<T, false, 8>(hbuf, const_cast<T*>(static_cast<const T*>(e.residual)), e.ldr, m0, c0, g.m, g.n, lane);
                         } else {
                             if (tc::elect_one()) {
                                 tc::mbar_arrive_expect_tx(&res_full[w], GP_BUF);
@@ -723,8 +732,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         }
                     }
                     stage();
-                    if (g.direct)
-                        copy_rows<T, true>(hbuf, static_cast<T*>(e.y), e.ldy, m0, c0, g.m, g.n, lane);
+                    if (DIRECT)
+                        copy_rows<T, true, 1>(hbuf, static_cast<T*>(e.y), e.ldy, m0, c0, g.m, g.n, lane);
                     else
                         put(&ty, m0, in);
                 }
@@ -736,9 +745,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             const bool inside = m0 < g.m && col < g.n;
             unsigned char* bias = biases + w * 128;
             if (e.bias) {
-                reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(static_cast<const T*>(e.bias) + col, lane, g.n - col, g.direct);
+                reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(static_cast<const T*>(e.bias) + col, lane, g.n - col, DIRECT);
                 __syncwarp();
             }
+            T* residual = const_cast<T*>(static_cast<const T*>(e.residual));
+            if (DIRECT && ahead) copy_rows<T, false, 8>(buf, residual, e.ldr, m0, col, g.m, g.n, lane);
             const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
             tc::fence_after_sync();
             const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + part * 64);
@@ -786,8 +797,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
 #pragma unroll
                     for (int j = 0; j < 32; j += 8)
                         *reinterpret_cast<uint4*>(brow + (((uint32_t)(32 * h + j) << 1) ^ sw)) = pack8<T>(&v[h][j]);
-                if (g.direct) {
-                    copy_rows<T, true>(buf, static_cast<T*>(e.pre), e.ldp, m0, col, g.m, g.n, lane);
+                if (DIRECT) {
+                    copy_rows<T, true, 1>(buf, static_cast<T*>(e.pre), e.ldp, m0, col, g.m, g.n, lane);
                 } else {
                     tc::fence_proxy_async();
                     __syncwarp();
@@ -802,9 +813,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 case FG_ACT_GELU: activate_all<FG_ACT_GELU>(v); break;
                 case FG_ACT_SILU: activate_all<FG_ACT_SILU>(v); break;
             }
-            if (g.direct) {
-                if (e.residual)
-                    copy_rows<T, false>(buf, const_cast<T*>(static_cast<const T*>(e.residual)), e.ldr, m0, col, g.m, g.n, lane);
+            if (DIRECT) {
+                if (e.residual && !ahead) copy_rows<T, false, 4>(buf, residual, e.ldr, m0, col, g.m, g.n, lane);
             } else if (!ahead) {  // the buffer's last store has read it
                 if (tc::elect_one()) {
                     tc::bulk_wait_read<0>();
@@ -813,7 +823,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 __syncwarp();
             }
             if (e.residual) {
-                if (!g.direct) {
+                if (!DIRECT) {
                     tc::mbar_wait_warp(&res_full[w], res_phase, fail);
                     res_phase ^= 1;
                 }
@@ -828,8 +838,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
 #pragma unroll
                 for (int j = 0; j < 32; j += 8)
                     *reinterpret_cast<uint4*>(brow + (((uint32_t)(32 * h + j) << 1) ^ sw)) = pack8<T>(&v[h][j]);
-            if (g.direct) {
-                copy_rows<T, true>(buf, static_cast<T*>(e.y), e.ldy, m0, col, g.m, g.n, lane);
+            if (DIRECT) {
+                copy_rows<T, true, 1>(buf, static_cast<T*>(e.y), e.ldy, m0, col, g.m, g.n, lane);
                 continue;
             }
             tc::fence_proxy_async();
@@ -983,14 +993,11 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
     g.idesc = instr_desc(dtype, 2 * GT_M, BN, g.a_mn, g.b_mn);
     const long long items = (long long)g.mt * g.nt * g.split;
     FG_REQUIRE(items <= 0x3fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
-    auto kernel = &gemm_pair_kernel<T, BN>;
+    auto kernel = g.direct && g.split == 1 ? &gemm_pair_kernel<T, BN, true> : &gemm_pair_kernel<T, BN, false>;
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), PairOf<T, BN>::SMEM));
     const int pairs = std::max(1, device_attr(cudaDevAttrMultiProcessorCount) / 2);
     TcArgs k = g;
-    if (g.split > 1) {
-        k.e.residual = k.e.pre = nullptr;
-        k.direct = 0;
-    }
+    if (g.split > 1) k.e.bias = k.e.residual = k.e.pre = nullptr;  // finish_kernel's
     kernel<<<2 * (unsigned)std::min<long long>(items, pairs), GP_NT, PairOf<T, BN>::SMEM, st>>>(ta, tb, ty, tp, tr, k);
     rc = check_launch("gemm_pair_kernel");
     if (rc || g.split == 1) return rc;

@@ -318,6 +318,21 @@ def test_linear_strides_and_alignment(ad, t, lead):
 
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(300, 8192, 520), (1, 512, 264), (40, 512, 264), (700, 72, 264), (3000, 264, 333)])
+def test_linear_vectors_off_their_alignment(ad, shape, t):
+    """A bias one element off any boundary, residuals of an odd width, few rows to
+    many, sums that are split over k and that are not."""
+    n, i, o = shape
+    g = _gen(n + o)
+    x, w = _randn(g, n, i, t=t), _randn(g, o, i, t=t, scale=i ** -0.5)
+    b, res = _randn(g, o + 1, t=t)[1:], _randn(g, n, o + 3, t=t)[:, 1:1 + o]
+    _check_linear(ad, x, w, b, res, "gelu", t)
+    _check_linear(ad, x, w, b, None, "none", t)
+    y = ad.linear(x, w, b, activation="silu", residual=res)
+    assert torch.equal(y, ad.linear(x, w, b.clone(), activation="silu", residual=res.contiguous()))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n", [1, 5, 40, 300])
 def test_linear_nonfinite_stays_in_its_rows(ad, t, n):
     g = _gen(n)

@@ -151,68 +151,103 @@ static int pack(const PackArgs& a, cudaStream_t s) {
 
 // ---- a few rows: the weights are read once ---------------------------------------
 //
-// A warp takes one output column for all R rows: 32 lanes along k, 16 bytes a lane
-// where the rows allow, then R sums over the warp.  Bound by the weights' bytes; at
-// one row of 768 x 1536 f16 GEMVFIG
-template <class T, int R>
+// A warp takes C output columns for all R rows: 32 lanes along k, 16 bytes a lane
+// where the rows allow, then R C sums over the warp, halved at each step: lane l ends
+// with one of them.  Bound by the latency of the loads, so all of a step's are asked
+// for at once (8 rows of 1536 -> 768 f16: 4.5 us; with a branch on the row between
+// them 11.3), and for one row of a large matrix by its bytes: 768 -> 1536 f16 2.3 us,
+// 4096 -> 4096 5.8 us (5.8 TB/s, of which L2 holds a part).
+template <class T, int R, int C>
 __global__ void __launch_bounds__(128) gemv_kernel(const T* __restrict__ x, const T* __restrict__ w, const GemmShape g,
                                                    int wide, const Epilogue e) {
     constexpr int VEC = 16 / sizeof(T);
     const int lane = threadIdx.x & 31;
-    const long long n = blockIdx.x * 4ll + (threadIdx.x >> 5);
+    const long long n = (blockIdx.x * 4ll + (threadIdx.x >> 5)) * C;
     if (n >= g.n) return;
-    const T* wr = w + n * g.bn;
-    float acc[R];
+    const T *wr[C], *xr[R];  // rows and columns past the last are the last again: no branch keeps loads apart
 #pragma unroll
-    for (int r = 0; r < R; ++r) acc[r] = 0.0f;
+    for (int c = 0; c < C; ++c) wr[c] = w + min(n + c, g.n - 1) * g.bn;
+#pragma unroll
+    for (int r = 0; r < R; ++r) xr[r] = x + min((long long)r, g.m - 1) * g.am;
+    float acc[R * C];
+#pragma unroll
+    for (int i = 0; i < R * C; ++i) acc[i] = 0.0f;
     long long k0 = 0;
     if (wide) {
-#pragma unroll 4
+#pragma unroll(R* C > 4 ? 2 : 4)
         for (long long k = lane * VEC; k + VEC <= g.k; k += 32 * VEC) {
-            alignas(16) T a[VEC], b[VEC];
-            *reinterpret_cast<uint4*>(b) = *reinterpret_cast<const uint4*>(wr + k);
+            alignas(16) T a[R][VEC], b[C][VEC];
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if (r >= g.m) break;
-                *reinterpret_cast<uint4*>(a) = *reinterpret_cast<const uint4*>(x + r * g.am + k);
+            for (int c = 0; c < C; ++c) *reinterpret_cast<uint4*>(b[c]) = *reinterpret_cast<const uint4*>(wr[c] + k);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[r] = fmaf(to_f32(a[i]), to_f32(b[i]), acc[r]);
-            }
+            for (int r = 0; r < R; ++r) *reinterpret_cast<uint4*>(a[r]) = *reinterpret_cast<const uint4*>(xr[r] + k);
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i)
+                        acc[r * C + c] = fmaf(to_f32(a[r][i]), to_f32(b[c][i]), acc[r * C + c]);
         }
         k0 = g.k / VEC * VEC;
     }
     for (long long k = k0 + lane; k < g.k; k += 32) {
-        const float b = to_f32(wr[k]);
+        float b[C];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (r < g.m) acc[r] = fmaf(to_f32(x[r * g.am + k]), b, acc[r]);
-    }
-    float z = 0.0f;
+        for (int c = 0; c < C; ++c) b[c] = to_f32(wr[c][k]);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const float t = warp_sum(acc[r]);
-        if (lane == r) z = t;
+        for (int r = 0; r < R; ++r) {
+            const float a = to_f32(xr[r][k]);
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[r * C + c] = fmaf(a, b[c], acc[r * C + c]);
+        }
     }
-    if (lane < g.m) epilogue_store<T>(e, lane, n, z);
+    int held = 0;  // which sum this lane ends with
+#pragma unroll
+    for (int o = 16, count = R * C; o > 0; o >>= 1) {
+        if (count > 1) {
+            count /= 2;
+            const bool upper = lane & o;
+            held += upper ? count : 0;
+#pragma unroll
+            for (int i = 0; i < R * C / 2; ++i)
+                if (i < count) {
+                    const float keep = upper ? acc[i + count] : acc[i], give = upper ? acc[i] : acc[i + count];
+                    acc[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+                }
+        } else {
+            acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
+        }
+    }
+    const int row = held / C;
+    const long long col = n + held % C;
+    if (lane % (32 / (R * C)) == 0 && row < g.m && col < g.n) epilogue_store<T>(e, row, col, acc[0]);
 }
 
 constexpr int GEMV_ROWS = 8;
 
+template <class T, int R, int C>
+static int gemv_columns(const void* x, const void* w, const GemmShape& g, const Epilogue& e, cudaStream_t s) {
+    auto lies = [&](const void* p, long long ld) { return aligned(p, 16) && ld * (int)sizeof(T) % 16 == 0; };
+    gemv_kernel<T, R, C><<<(unsigned)((g.n + 4 * C - 1) / (4 * C)), 128, 0, s>>>(
+        static_cast<const T*>(x), static_cast<const T*>(w), g, lies(x, g.am) && lies(w, g.bn), e);
+    return check_launch("gemv_kernel");
+}
+
+// Two columns a warp where columns alone give every SM 16 warps (4096 x 4096 f16, 8
+// rows: 14.6 us with two, 18.7 with one; 1536 x 768: 5.5 and 4.5).
+template <class T, int R>
+static int gemv_of(const void* x, const void* w, const GemmShape& g, const Epilogue& e, cudaStream_t s) {
+    return g.n > 16ll * device_attr(cudaDevAttrMultiProcessorCount) ? gemv_columns<T, R, 2>(x, w, g, e, s)
+                                                                    : gemv_columns<T, R, 1>(x, w, g, e, s);
+}
+
 template <class T>
 static int gemv(const void* x, const void* w, const GemmShape& g, const Epilogue& e, cudaStream_t s) {
-    const T *xp = static_cast<const T*>(x), *wp = static_cast<const T*>(w);
-    auto lies = [&](const void* p, long long ld) { return aligned(p, 16) && ld * (int)sizeof(T) % 16 == 0; };
-    const int wide = lies(x, g.am) && lies(w, g.bn);
-    const unsigned blocks = (unsigned)((g.n + 3) / 4);
-    if (g.m == 1)
-        gemv_kernel<T, 1><<<blocks, 128, 0, s>>>(xp, wp, g, wide, e);
-    else if (g.m == 2)
-        gemv_kernel<T, 2><<<blocks, 128, 0, s>>>(xp, wp, g, wide, e);
-    else if (g.m <= 4)
-        gemv_kernel<T, 4><<<blocks, 128, 0, s>>>(xp, wp, g, wide, e);
-    else
-        gemv_kernel<T, GEMV_ROWS><<<blocks, 128, 0, s>>>(xp, wp, g, wide, e);
-    return check_launch("gemv_kernel");
+    return g.m == 1   ? gemv_columns<T, 1, 1>(x, w, g, e, s)
+           : g.m == 2 ? gemv_of<T, 2>(x, w, g, e, s)
+           : g.m <= 4 ? gemv_of<T, 4>(x, w, g, e, s)
+                      : gemv_of<T, GEMV_ROWS>(x, w, g, e, s);
 }
 
 template <class T>

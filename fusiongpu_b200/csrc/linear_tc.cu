@@ -139,7 +139,7 @@ __device__ __forceinline__ void store4<float>(float* p, float4 f) {
 // cluster, in rank order, and finishes it.
 template <class T, int BN>
 __global__ void __launch_bounds__(GT_NT, 1)
-    gemm_split_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const TcArgs g) {
+    gemm_split_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const __grid_constant__ TcArgs g) {
     using Ring = RingOf<BN>;
     constexpr int LDP = BN + 4;  // partial row: 4 floats of padding keep 16-byte stores off each other's banks
     static_assert(GT_M * LDP * 4 <= Ring::N * Ring::STAGE, "the partial tile fits the ring");
@@ -478,7 +478,7 @@ template <class T, int BN, bool DIRECT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                      const __grid_constant__ CUtensorMap ty, const __grid_constant__ CUtensorMap tp,
-                     const __grid_constant__ CUtensorMap tr, const TcArgs g) {
+                     const __grid_constant__ CUtensorMap tr, const __grid_constant__ TcArgs g) {
     using P = PairOf<T, BN>;
     constexpr int GP_STAGES = P::STAGES;
     static_assert(sizeof(T) == 2 || BN == 256, "float32 takes 256 columns");

@@ -21,6 +21,7 @@ constexpr int GT_K = 64;           // elements of a K block: one 128-byte swizzl
 constexpr int GT_NT = 64 + 256;    // TMA warp, MMA warp, 8 epilogue warps
 constexpr int GT_RING = 192 * 1024;
 constexpr int GT_RUN = 512;        // K blocks that a 16-bit product's accumulator sums at most
+constexpr int GP_CHUNK = 8;        // and a float32 one
 
 struct TcArgs {
     int kt, mt, nt;     // K blocks, row tiles, column tiles
@@ -155,9 +156,9 @@ __global__ void __launch_bounds__(GT_NT, 1)
     const int tile = (int)(blockIdx.x / (unsigned)S);
     const int m0 = tile / g.nt * GT_M, n0 = tile % g.nt * BN;
     const int kb0 = (int)((long long)g.kt * rank / S), kb1 = (int)((long long)g.kt * (rank + 1) / S);
-    // accumulators: one, or for float32 as many as TMEM holds, each for its share of k
+    // accumulators: one, or for float32 as many as TMEM holds, each for GP_CHUNK K blocks
     constexpr int NA = sizeof(T) == 4 ? 512 / BN : 1;
-    const int share = (kb1 - kb0 + NA - 1) / NA, shares = (kb1 - kb0 + share - 1) / share, products = sizeof(T) == 4 ? 6 : 1;
+    const int share = sizeof(T) == 4 ? GP_CHUNK : kb1 - kb0, shares = (kb1 - kb0 + share - 1) / share, products = sizeof(T) == 4 ? 6 : 1;
 
     if (warp == 2 && tc::elect_one()) {
         tc::prefetch_map(&ta);
@@ -377,8 +378,6 @@ constexpr int GP_A = GT_M * GT_K * 2;
 constexpr int GP_BUF = 4096;   // 32 rows x 128 bytes, 128-byte swizzle
 constexpr int GP_EPI = 16;     // epilogue warps, each 32 rows x 64 columns of a tile
 constexpr int GP_NT = 64 + GP_EPI * 32;
-
-constexpr int GP_CHUNK = 8;    // K blocks of a float32 accumulator
 
 // Operand stages and the epilogue's buffers: 4 KB a warp, or for float32 8 KB, which
 // hold the running sums of its 32 rows x 64 columns.
@@ -1022,7 +1021,7 @@ struct TcPlan {
     size_t ws;
 };
 
-static TcPlan tc_plan(const GemmShape& s, int planes) {
+static TcPlan tc_plan_of(const GemmShape& s, int planes, bool direct) {
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
     const int kt = (int)((s.k + GT_K - 1) / GT_K) * (planes == 1 ? 1 : 6);
     auto waves = [](long long tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
@@ -1040,30 +1039,42 @@ static TcPlan tc_plan(const GemmShape& s, int planes) {
         if (planes == 3 && bn == 128) break;
         const long long tiles = m2 * ((s.n + bn - 1) / bn);
         for (int sp : {1, 2, 4, 8, 16, 32}) {
+            if (direct && sp > 1) break;
             if (sp > 1 && (sp > kb / 2 || (tiles * sp > sms && kb * 2 / sp <= GT_RUN))) break;
             if (planes == 1 && kb > GT_RUN * sp && sp < 32) continue;
             const size_t ws = sp > 1 ? (size_t)sp * m2 * 2 * GT_M * ((s.n + 3) / 4 * 4) * 4 : 0;
             const double epi = bn == 256 ? 2.0 : 1.0, main = (kt + sp - 1) / sp * (bn == 256 ? 0.39 : 0.34);
-            offer(6.0 + waves(tiles * sp, sms / 2) * std::max(main, epi) + epi + (sp > 1 ? 3.0 + 1.5e-6 * ws / 6.0 : 0.0),
+            const double rows = direct ? (bn == 256 ? 14.0 : 8.0) : 0.0;
+            offer(6.0 + waves(tiles * sp, sms / 2) * (std::max(main, epi) + rows) + epi + (sp > 1 ? 3.0 + 1.5e-6 * ws / 6.0 : 0.0),
                   TcPlan{true, bn, sp, ws});
         }
     }
     for (int bn : {256, 128, 64}) {
         const long long tiles = m1 * ((s.n + bn - 1) / bn);
         for (int sp : {1, 2, 4, 8}) {
-            if (sp > kb) break;
+            if (sp > kb || (direct && sp > 1)) break;
             // the sums' length: 512 k for each of float32's 512 / bn accumulators
             if (kb > (planes == 1 ? GT_RUN : GP_CHUNK * 512 / bn) * sp && kb > 3) continue;
             const int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
             const double main = (kt + sp - 1) / sp * (bn == 256 ? 0.43 : bn == 128 ? 0.30 : 0.21);
-            offer(5.0 + waves(tiles, slots) * (main + 2.0 + 0.02 * bn / sp) + (sp == 8 ? 0.7 : 0.0), TcPlan{false, bn, sp, 0});
+            const double rows = direct ? 0.055 * bn : 0.0;
+            offer(5.0 + waves(tiles, slots) * (main + 2.0 + 0.02 * bn / sp + rows) + (sp == 8 ? 0.7 : 0.0), TcPlan{false, bn, sp, 0});
         }
     }
     return best;
 }
 
+// Outputs that go row by row cost a wave 8 or 14 us more with pairs, less with small
+// tiles (1777 x 101 -> 333 bf16: 27 us with pairs, 12 in tiles of 64 columns).  Only
+// tiles whose sums are not split are chosen anew: those add in one order whichever
+// kernel takes them, so that a result does not depend on its alignment.
+static TcPlan tc_plan(const GemmShape& s, int planes, bool direct) {
+    const TcPlan p = tc_plan_of(s, planes, false);
+    return direct && p.split == 1 ? tc_plan_of(s, planes, true) : p;
+}
+
 size_t tc_gemm_workspace(int dtype, const GemmShape& s) {
-    return s.k > 0 ? tc_plan(s, dtype == FG_DTYPE_F32 ? 3 : 1).ws : 0;
+    return s.k > 0 ? tc_plan(s, dtype == FG_DTYPE_F32 ? 3 : 1, false).ws : 0;
 }
 
 int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& s,
@@ -1086,7 +1097,7 @@ int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long lon
     auto lies = [&](const void* p, long long ld, int n) { return !p || (aligned(p, n) && ld * es % n == 0); };
     g.vec = lies(e.y, e.ldy, 4 * es) && lies(e.bias, 0, 4 * es) && lies(e.pre, e.ldp, 4 * es) && lies(e.residual, e.ldr, 4 * es);
     g.direct = !(lies(e.y, e.ldy, 16) && lies(e.bias, 0, 16) && lies(e.pre, e.ldp, 16) && lies(e.residual, e.ldr, 16));
-    const TcPlan p = tc_plan(s, g.planes);
+    const TcPlan p = tc_plan(s, g.planes, g.direct);
     g.split = p.split;
 #define FG_PRODUCT(T)                                                                        \
     (p.pair ? (sizeof(T) == 4 || p.bn == 256                                              \

@@ -5,8 +5,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <exception>
-
 #include "fg_common.cuh"
 
 namespace fg {

@@ -136,8 +136,9 @@ __device__ __forceinline__ void store4<float>(float* p, float4 f) {
 
 // One tile of 128 x BN per cluster, its K blocks divided over the cluster's
 // CTAs.  Each CTA's partial tile goes from TMEM to its shared memory (where the
-// operand ring was); then each CTA adds one slice of the columns over the
-// cluster, in rank order, and finishes it.
+// operand ring was); then each CTA adds one slice of the columns over the cluster,
+// from its own rank onwards -- were all to begin with rank 0, they would queue for its
+// shared memory: 100 x 1536 -> 768 bf16 8.2 us, so 7.6 -- and finishes it.
 template <class T, int BN>
 __global__ void __launch_bounds__(GT_NT, 1)
     gemm_split_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const __grid_constant__ TcArgs g) {

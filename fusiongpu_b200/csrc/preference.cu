@@ -16,7 +16,9 @@
 // of G threads (8, 32, 128 or 512, by the row's length) takes every (threads / G)-th
 // pair and keeps u and its share of the gradient in registers, the rows of its next
 // pair being loaded meanwhile; at the end the block adds the groups' shares in their
-// order.  MEASURED
+// order.  Rows of 256 columns to 3 KB go to the second kernel below.  Measured: 10,000
+// queries of 16 pairs, documents of 128 f32 72 us (2.3 TB/s), of 768 f16 179 us (2.7
+// TB/s, second kernel), 32 queries of 10 pairs of 128 bytes 5.5 us.
 #include <algorithm>
 
 #include "adapter_common.cuh"
@@ -240,15 +242,16 @@ __global__ void __launch_bounds__(512) preference_kernel(const PrefArgs g) {
     }
 }
 
-// Rows of ROWS_FROM bytes to 4 KB on 16-byte boundaries: a fifth warp brings them
+// Rows of 256 columns to 3 KB on 16-byte boundaries: a fifth warp brings them
 // into a ring in shared memory by bulk copies, as many pairs ahead as the ring holds
-// and on into the block's next query, so the latency of ids and rows is paid once; a
-// warp takes every fourth pair of a query, in the order of the kernel above.  With
-// the copies off the warps' hands the instructions a pair takes bound it next: the
-// producer's lanes issue half a ring at once, the arithmetic is packed in pairs of
-// columns, and a lane writes the loss of one pair in 32.  Each warp has slots of its
-// own: were a slot shared, a warp could ask for its next phase before the last one
-// had come, and a phase's parity cannot tell the two apart.
+// and on into the block's next query, which it asks into L2 before (204 us without, 179
+// with), so the latency of ids and rows is paid once; a
+// warp takes every fourth pair of a query.  With the copies off the warps' hands the
+// instructions a pair takes bound it next: the producer's lanes issue half a ring at
+// once, the arithmetic is packed in pairs of columns, and a lane writes the loss of one
+// pair in 32.  Each warp has slots of its own: were a slot shared, a warp could ask for
+// its next phase before the last one had come, and a phase's parity cannot tell the two
+// apart.
 constexpr int PS_WARPS = 4;
 constexpr int PS_RING = 36 * 1024;
 constexpr int PS_STAGES = 16;
@@ -301,6 +304,8 @@ __device__ __forceinline__ void query_columns(float* f, const void* p, int dtype
         load_query<__nv_bfloat16, VEC>(f, static_cast<const __nv_bfloat16*>(p) + j, wide);
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // MID: squared L2 without a reference, u = q - (d+ + d-) / 2.
 template <class B, int NCH, bool MID>
 __global__ void __launch_bounds__((PS_WARPS + 1) * 32, NCH * 16 / sizeof(B) <= 16 ? 4 : 3)
@@ -331,7 +336,12 @@ __global__ void __launch_bounds__((PS_WARPS + 1) * 32, NCH * 16 / sizeof(B) <= 1
         const int depth = (slots + 1) / 2, batch = PS_WARPS * depth, w0 = (lane % PS_WARPS) * slots;
         RingAt at = {lane < batch ? lane / PS_WARPS : 0, 1};  // the slots start empty
         bool ok = true;
+        const int size = g.dtype == FG_DTYPE_F32 ? 4 : 2;
         for (long long i = i0; i < i1 && ok; ++i) {
+            for (int j = lane * 128; j < g.dim * size; j += 32 * 128) {  // the query comes to L2 meanwhile
+                prefetch_l2(static_cast<const char*>(g.q) + i * g.ldq * size + j);
+                if (g.ref) prefetch_l2(static_cast<const char*>(g.ref) + i * g.ldr * size + j);
+            }
             const long long p0 = first_of(i), p1 = max(first_of(i + 1), p0);
             for (long long base = p0; base < p1; base += batch) {
                 const long long p = base + lane;
@@ -482,9 +492,10 @@ static int preference_stream(const PrefArgs& g, cudaStream_t s) {
     const int smem = PS_WARPS * slots * 2 * row + PS_WARPS * g.dim * (int)sizeof(float);
     auto kernel = g.l2 && !g.ref ? &preference_stream_kernel<B, NCH, true> : &preference_stream_kernel<B, NCH, false>;
     if (smem > 40 * 1024) FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
-    // a few blocks in turn on each SM even out queries of unlike length
+    // 32 blocks in turn on each SM even out queries of unlike length (10,000 queries of 16
+    // pairs on average: 179 us, with 16 186, with 8 192, with 3 266)
     const int sms = std::max(1, device_attr(cudaDevAttrMultiProcessorCount));
-    const int per_block = std::max(1, std::min(16, g.nq / (16 * sms)));
+    const int per_block = std::max(1, std::min(16, g.nq / (32 * sms)));
     kernel<<<(g.nq + per_block - 1) / per_block, (PS_WARPS + 1) * 32, smem, s>>>(g, slots, per_block);
     return check_launch("preference_stream_kernel");
 }
@@ -508,9 +519,12 @@ static int preference_shape(PrefArgs g, cudaStream_t s) {
     g.wide = aligned(g.base, 16);
     auto lies = [&](const void* p, long long ld) { return !p || (aligned(p, 16) && ld * sizeof(T) % 16 == 0); };
     g.qwide = g.dim % V == 0 && lies(g.q, g.ldq) && lies(g.ref, g.ldr);
-    // Both kernels at 10,000 queries of 16 pairs: STREAMFIG
+    // Stream and register kernel at 10,000 queries of 16 pairs: f16 256 columns 110 and
+    // 165 us, 768 179 and 448; u8 512 123 and 173; f32 128 101 and 72, 256 106 and 146,
+    // 768 294 and 296, 1024 357 and 303.  Below 256 columns a warp's lanes have too few
+    // to hide a pair's chain of steps; beyond 768 of f32 the ring holds too few pairs.
     const int row = g.dim * (int)sizeof(B);
-    if (g.dim % V == 0 && g.wide && row >= 512 && g.dim <= 1024) {
+    if (g.dim % V == 0 && g.wide && row >= 512 && g.dim >= 256 && g.dim <= 1024 && row <= 768 * 4) {
         if constexpr (V == 16) {
             return g.dim <= 512 ? preference_stream<B, 1>(g, s) : preference_stream<B, 2>(g, s);
         } else if constexpr (V == 8) {
@@ -520,8 +534,7 @@ static int preference_shape(PrefArgs g, cudaStream_t s) {
         } else {
             return g.dim <= 256   ? preference_stream<B, 2>(g, s)
                    : g.dim <= 512 ? preference_stream<B, 4>(g, s)
-                   : g.dim <= 768 ? preference_stream<B, 6>(g, s)
-                                  : preference_stream<B, 8>(g, s);
+                                  : preference_stream<B, 6>(g, s);
         }
     }
 #define FG_PREF(VEC, NCH, G) \

@@ -295,26 +295,28 @@ class QueryAdapter:
         """The adapted queries [nq][dim], of the adapter's type: what the index
         is searched with."""
         p = self.params
-        q = queries.to(self.dtype)
-        n = layer_norm(q, p["norm_weight"], p["norm_bias"], stream=stream)
-        h = linear(n, p["w1"], p["b1"], activation=self.activation, stream=stream)
-        return linear(h, p["w2"], p["b2"], residual=q, stream=stream)
+        with contextlib.nullcontext() if stream is None else _entered(queries.device, stream):
+            q = queries.to(self.dtype)
+            n = layer_norm(q, p["norm_weight"], p["norm_bias"])
+            h = linear(n, p["w1"], p["b1"], activation=self.activation)
+            return linear(h, p["w2"], p["b2"], residual=q)
 
     def train_step(self, queries: torch.Tensor, base: torch.Tensor, offsets: torch.Tensor, pos_ids: torch.Tensor,
                    neg_ids: torch.Tensor, beta: float = 1.0, label_smoothing: float = 0.0, metric: str = "l2",
-                   weights: torch.Tensor | None = None):
+                   weights: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None):
         """One forward and backward pass on the pairs of `queries`, against the
         unadapted queries as the reference.  Returns (losses, margins) and
         leaves the gradient of sum(weights * losses) in the parameters'
         ``grad``."""
         p = self.params
-        q = queries.to(self.dtype)
-        n, mean, rstd = layer_norm(q, p["norm_weight"], p["norm_bias"], return_stats=True)
-        h, z = linear(n, p["w1"], p["b1"], activation=self.activation, return_pre=True)
-        out = linear(h, p["w2"], p["b2"], residual=q)
-        losses, margins, dout = preference_loss(out, base, offsets, pos_ids, neg_ids, ref=q, weights=weights,
-                                                beta=beta, label_smoothing=label_smoothing, metric=metric)
-        dh, p["w2"].grad, p["b2"].grad = linear_backward(dout, h, p["w2"])
-        dn, p["w1"].grad, p["b1"].grad = linear_backward(dh, n, p["w1"], pre=z, activation=self.activation)
-        _, p["norm_weight"].grad, p["norm_bias"].grad = layer_norm_backward(dn, q, mean, rstd, p["norm_weight"])
+        with contextlib.nullcontext() if stream is None else _entered(queries.device, stream):
+            q = queries.to(self.dtype)
+            n, mean, rstd = layer_norm(q, p["norm_weight"], p["norm_bias"], return_stats=True)
+            h, z = linear(n, p["w1"], p["b1"], activation=self.activation, return_pre=True)
+            out = linear(h, p["w2"], p["b2"], residual=q)
+            losses, margins, dout = preference_loss(out, base, offsets, pos_ids, neg_ids, ref=q, weights=weights,
+                                                    beta=beta, label_smoothing=label_smoothing, metric=metric)
+            dh, p["w2"].grad, p["b2"].grad = linear_backward(dout, h, p["w2"])
+            dn, p["w1"].grad, p["b1"].grad = linear_backward(dh, n, p["w1"], pre=z, activation=self.activation)
+            _, p["norm_weight"].grad, p["norm_bias"].grad = layer_norm_backward(dn, q, mean, rstd, p["norm_weight"])
         return losses, margins

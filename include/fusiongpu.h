@@ -467,7 +467,7 @@ int fg_layer_norm(const void* x, int32_t dtype, int64_t rows, int32_t dim, int64
  * dx = rstd * (a - avg(a) - h * avg(a h)); dweight = sum over rows of dy h and
  * dbias = sum over rows of dy, in param_dtype (0 for no rows).  Any of dx,
  * dweight, dbias may be NULL.  The workspace holds one partial row of both
- * sums per resident block, added in block order. */
+ * sums per resident block, added in one fixed order. */
 int fg_layer_norm_backward_workspace_size(int64_t rows, int32_t dim, size_t* bytes);
 int fg_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int32_t dtype, int64_t rows,
                            int32_t dim, int64_t x_stride, const void* weight, int32_t param_dtype, const float* mean,

@@ -589,6 +589,23 @@ def test_train_step_against_differences(ad, metric, act):
 
 # ---- streams, refusals, the whole -----------------------------------------------------
 
+def test_query_adapter_converts_on_its_stream(ad):
+    """Queries of another type are converted on the stream of the call, not on the
+    current one, which is busy here."""
+    from fusiongpu_b200 import QueryAdapter
+    a = QueryAdapter(96, 160, dtype=torch.float16)
+    a.params["w2"].normal_(generator=_gen(1))
+    q = _randn(_gen(2), 300, 96)
+    want = a(q)
+    torch.empty(300, 96, device="cuda", dtype=torch.float16).fill_(math.nan)  # what an unfinished conversion leaves
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    got = a(q, stream=s)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
 def test_operators_on_another_stream(ad):
     g = _gen(4)
     x, w = _randn(g, 3000, 512, t="bf16"), _randn(g, 256, 512, t="bf16", scale=0.05)

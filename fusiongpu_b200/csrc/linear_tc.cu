@@ -1068,7 +1068,7 @@ static TcPlan tc_plan_of(const GemmShape& s, int planes, bool direct) {
 // Outputs that go row by row cost a wave 8 or 14 us more with pairs, less with small
 // tiles (1777 x 101 -> 333 bf16: 27 us with pairs, 12 in tiles of 64 columns).  Only
 // tiles whose sums are not split are chosen anew: those add in one order whichever
-// kernel takes them, so that a result does not depend on its alignment.
+// kernel takes them, so that a result does not depend on where it is written.
 static TcPlan tc_plan(const GemmShape& s, int planes, bool direct) {
     const TcPlan p = tc_plan_of(s, planes, false);
     return direct && p.split == 1 ? tc_plan_of(s, planes, true) : p;

@@ -141,6 +141,35 @@ def test_layer_norm_strides_and_absent_parameters(ad, t, dim):
         assert ad.layer_norm_backward(c, c, mean, rstd, w, param_grads=False)[1:] == (None, None)
 
 
+@pytest.mark.parametrize("t,p", [("f32", "f32"), ("f16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("dim,rows", [(40, 40001), (128, 21000), (100, 21000), (301, 6000), (512, 6007), (768, 6001),
+                                      (1000, 5003), (1001, 3001), (1536, 3001), (4096, 1501), (5000, 701)])
+def test_layer_norm_more_rows_than_groups(ad, dim, rows, t, p):
+    """Groups that take several rows in turn: every row comes out as it does alone,
+    on 16-byte boundaries and off them, and the weight's gradients hold all rows."""
+    g = _gen(rows)
+    x, dy = _randn(g, rows, dim, t=t, scale=0.7, mean=0.2), _randn(g, rows, dim, t=t, scale=0.3)
+    w, b = _randn(g, dim, t=p, mean=1.0, scale=0.3), _randn(g, dim, t=p, scale=0.3)
+    y, mean, rstd = ad.layer_norm(x, w, b, return_stats=True)
+    dx, dw, db = ad.layer_norm_backward(dy, x, mean, rstd, w)
+    for i in (0, rows // 2 - 11, rows - 23):
+        k = slice(i, i + 23)
+        y1, m1, r1 = ad.layer_norm(x[k], w, b, return_stats=True)
+        assert torch.equal(y1, y[k]) and torch.equal(m1, mean[k]) and torch.equal(r1, rstd[k])
+        assert torch.equal(ad.layer_norm_backward(dy[k], x[k], m1, r1, w, param_grads=False)[0], dx[k])
+    h = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    he = 4 * E32 * ((x.double().abs() + mean.double().abs()[:, None]) * rstd.double()[:, None] + h.abs())
+    deep, d = (rows + 16) * 2 * E32, dy.double()
+    rdw, rdb = (d * h).sum(0), d.sum(0)
+    _within(dw, rdw, deep * (d * h).abs().sum(0) + (d.abs() * he).sum(0) + U[p] * rdw.abs() + TINY[p], "dweight")
+    _within(db, rdb, deep * d.abs().sum(0) + U[p] * rdb.abs() + TINY[p], "dbias")
+    xo = torch.empty(rows, dim + 3, device="cuda", dtype=T[t])[:, 1:1 + dim]
+    xo.copy_(x)
+    assert torch.equal(ad.layer_norm(xo, w, b), y)
+    for u, v in zip(ad.layer_norm_backward(dy, xo, mean, rstd, w), (dx, dw, db)):
+        assert torch.equal(u, v)
+
+
 def test_layer_norm_empty_constant_and_nonfinite_rows(ad):
     x = torch.zeros(0, 64, device="cuda")
     y, mean, rstd = ad.layer_norm(x, return_stats=True)
@@ -330,6 +359,17 @@ def test_linear_vectors_off_their_alignment(ad, shape, t):
     _check_linear(ad, x, w, b, None, "none", t)
     y = ad.linear(x, w, b, activation="silu", residual=res)
     assert torch.equal(y, ad.linear(x, w, b.clone(), activation="silu", residual=res.contiguous()))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 40, 2500), (2, 40, 2500), (3, 64, 2401), (4, 520, 2999), (5, 7, 2999), (8, 136, 4000)])
+def test_linear_few_rows_many_columns(ad, shape, t):
+    n, i, o = shape
+    g = _gen(o + n)
+    x, w = _randn(g, n, i, t=t), _randn(g, o, i, t=t, scale=i ** -0.5)
+    b, res = _randn(g, o, t=t, scale=0.3), _randn(g, n, o, t=t)
+    _check_linear(ad, x, w, b, res, "gelu", t)
+    _check_linear(ad, x, w, None, None, "none", t)
 
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])

@@ -486,6 +486,120 @@ static int linear_forward(const fg_linear_params* p, const Strides& t, const voi
     return gemm<T>(a, b, GemmShape{p->rows, p->out_dim, p->in_dim, a.ld, 1, b.ld, 1}, e, f.product, s);
 }
 
+// ---- gradients of a few rows: one launch -----------------------------------------
+//
+// The first blocks take dx, 64 columns each: w is read once, a warp taking every
+// sixteenth of its rows, and dz of 512 columns at a time is worked out in shared
+// memory; the others take dw and db, four rows of w each.  dz stays in 32 bits: with
+// it rounded to 16 on its way to the tensor cores, as for more rows, one row's dx of
+// 107 -> 56 bf16 was off by 0.0033 where its own rounding is 0.0018.  Bound by the
+// latency of w's loads, 32 rows of it under way in a block.  One row of 768 -> 1536 bf16
+// 10.5 us (with the launches of more rows 15.6), eight 21.7 (15.7, but five launches:
+// a call is 22 us, not 29); float32 9.1 and 20.7 (30 and 34).  Eight rows of 4096 ->
+// 4096 bf16 63 (32): beyond four rows of 2^22 weights the tensor cores take them.
+static bool few(const fg_linear_params* p) {
+    return p->rows >= 1 && p->rows <= GEMV_ROWS && (p->rows <= 4 || (long long)p->in_dim * p->out_dim <= 1 << 22);
+}
+
+constexpr int FEW_NT = 512, FEW_COLS = 64, FEW_OUT = 4;
+
+struct FewArgs {
+    const void *dy, *x, *w, *pre;
+    void *dx, *dw, *db;
+    long long lddy, ldx, ldw, ldp;
+    int rows, in_dim, out_dim, act, dx_blocks;
+};
+
+template <class T>
+__device__ __forceinline__ float dz_of(const FewArgs& g, int r, int o) {
+    const float d = to_f32(static_cast<const T*>(g.dy)[r * g.lddy + o]);
+    return g.act == FG_ACT_NONE ? d : d * activate_grad<false>(to_f32(static_cast<const T*>(g.pre)[r * g.ldp + o]), g.act);
+}
+
+template <class T, int R>
+__global__ void __launch_bounds__(FEW_NT) few_rows_kernel(const FewArgs g) {
+    __shared__ float s[FEW_NT / 32][R][FEW_COLS];  // warps' sums; before, dz of 512 columns
+    float* dz = &s[0][0][0];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if ((int)blockIdx.x < g.dx_blocks) {
+        const int j0 = blockIdx.x * FEW_COLS + lane, j1 = j0 + 32;
+        const T* w = static_cast<const T*>(g.w);
+        float acc[R][2];
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r][0] = acc[r][1] = 0.0f;
+        for (int base = 0; base < g.out_dim; base += FEW_NT) {
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < R; ++r) dz[r * FEW_NT + tid] = r < g.rows && base + tid < g.out_dim ? dz_of<T>(g, r, base + tid) : 0.0f;
+            __syncthreads();
+            const int last = min(FEW_NT, g.out_dim - base) - 1, c0 = min(j0, g.in_dim - 1), c1 = min(j1, g.in_dim - 1);
+#pragma unroll 16
+            for (int o = warp; o < FEW_NT; o += FEW_NT / 32) {
+                if (o > last) break;
+                const T* row = w + (base + o) * g.ldw;
+                const float a = to_f32(row[c0]), b = to_f32(row[c1]);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    acc[r][0] = fmaf(dz[r * FEW_NT + o], a, acc[r][0]);
+                    acc[r][1] = fmaf(dz[r * FEW_NT + o], b, acc[r][1]);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            s[warp][r][lane] = acc[r][0];
+            s[warp][r][lane + 32] = acc[r][1];
+        }
+        __syncthreads();
+        const int r = tid / FEW_COLS, c = tid % FEW_COLS, j = blockIdx.x * FEW_COLS + c;
+        if (r < min(R, g.rows) && j < g.in_dim) {
+            float v = 0.0f;
+#pragma unroll
+            for (int k = 0; k < FEW_NT / 32; ++k) v += s[k][r][c];
+            static_cast<T*>(g.dx)[(long long)r * g.in_dim + j] = from_f32<T>(v);
+        }
+        return;
+    }
+    const int o0 = (blockIdx.x - g.dx_blocks) * FEW_OUT;
+    if (tid < FEW_OUT * R) {
+        const int r = tid / FEW_OUT, o = o0 + tid % FEW_OUT;
+        dz[tid] = r < g.rows && o < g.out_dim ? dz_of<T>(g, r, o) : 0.0f;
+    }
+    __syncthreads();
+    if (g.db && tid < FEW_OUT && o0 + tid < g.out_dim) {
+        float v = 0.0f;
+        for (int r = 0; r < R; ++r) v += dz[r * FEW_OUT + tid];
+        static_cast<T*>(g.db)[o0 + tid] = from_f32<T>(v);
+    }
+    if (!g.dw) return;
+    for (int i = tid; i < g.in_dim; i += FEW_NT) {
+        float v[FEW_OUT] = {};
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float x = r < g.rows ? to_f32(static_cast<const T*>(g.x)[r * g.ldx + i]) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < FEW_OUT; ++k) v[k] = r < g.rows ? fmaf(dz[r * FEW_OUT + k], x, v[k]) : v[k];
+        }
+#pragma unroll
+        for (int k = 0; k < FEW_OUT; ++k)
+            if (o0 + k < g.out_dim) static_cast<T*>(g.dw)[(long long)(o0 + k) * g.in_dim + i] = from_f32<T>(v[k]);
+    }
+}
+
+template <class T>
+static int few_rows(FewArgs g, cudaStream_t s) {
+    g.dx_blocks = g.dx ? (g.in_dim + FEW_COLS - 1) / FEW_COLS : 0;
+    const int blocks = g.dx_blocks + (g.dw || g.db ? (g.out_dim + FEW_OUT - 1) / FEW_OUT : 0);
+    if (!blocks) return FG_OK;
+    auto kernel = g.rows == 1 ? &few_rows_kernel<T, 1>
+                  : g.rows == 2 ? &few_rows_kernel<T, 2>
+                  : g.rows <= 4 ? &few_rows_kernel<T, 4>
+                                : &few_rows_kernel<T, GEMV_ROWS>;
+    kernel<<<blocks, FEW_NT, 0, s>>>(g);
+    return check_launch("few_rows_kernel");
+}
+
 struct BackwardWs {
     void *dz, *x, *w, *product;
     float* part;
@@ -494,6 +608,7 @@ struct BackwardWs {
 static size_t backward_carve(const fg_linear_params* p, const Strides& t, void* ws, size_t bytes, BackwardWs& w) {
     Carve c(ws, bytes);
     w = BackwardWs{};
+    if (few(p)) return 0;
     if (p->activation != FG_ACT_NONE || needs_pack(p->dtype, t.y)) w.dz = c.take<char>(pack_bytes(p->dtype, p->rows, p->out_dim));
     if (needs_pack(p->dtype, t.x)) w.x = c.take<char>(pack_bytes(p->dtype, p->rows, p->in_dim));
     if (needs_pack(p->dtype, t.w)) w.w = c.take<char>(pack_bytes(p->dtype, p->out_dim, p->in_dim));
@@ -506,6 +621,10 @@ static size_t backward_carve(const fg_linear_params* p, const Strides& t, void* 
 template <class T>
 static int linear_backward(const fg_linear_params* p, const Strides& t, const void* dy, const void* x, const void* w,
                            const void* pre, void* dx, void* dw, void* dbias, const BackwardWs& ws, cudaStream_t s) {
+    if (few(p))
+        return few_rows<T>(FewArgs{dy, x, w, pre, dx, dw, dbias, t.y, t.x, t.w, t.p, (int)p->rows, p->in_dim, p->out_dim,
+                                   p->activation, 0},
+                           s);
     const bool act = p->activation != FG_ACT_NONE, store = (act || needs_pack(p->dtype, t.y)) && (dx || dw);
     const int split = p->rows ? dz_split(p->rows, p->out_dim, sizeof(T)) : 0;
     const long long plane = p->dtype == FG_DTYPE_F32 ? p->rows * pack_stride(p->out_dim) : 0;

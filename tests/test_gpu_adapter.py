@@ -306,6 +306,27 @@ def test_linear_backward(ad, shape, act, t):
     assert ad.linear_backward(dy, x, w, pre=pre, activation=act, input_grad=False)[0] is None
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("shape", [(1, 56, 107), (1, 65, 1), (2, 1, 600), (3, 130, 1030), (4, 64, 512), (8, 300, 513), (5, 768, 1536)])
+def test_linear_backward_of_few_rows(ad, shape, act, t):
+    """dz is not rounded before its products: every gradient has one rounding."""
+    n, i, o = shape
+    g = _gen(i + o)
+    x, w = _randn(g, n, i + 3, t=t)[:, 2:2 + i], _randn(g, o, i + 1, t=t, scale=i ** -0.5)[:, 1:]
+    dy, pre = _randn(g, n, o + 5, t=t, scale=0.1)[:, 1:1 + o], _randn(g, n, o, t=t, scale=1.5)
+    dx, dw, db = ad.linear_backward(dy, x, w, pre=None if act == "none" else pre, activation=act)
+    f = torch.ones_like(pre.double()) if act == "none" else _act_grad(pre.double(), act)
+    dz, mag = dy.double() * f, dy.double().abs() * (1 + f.abs())
+    for got, want, m, k in ((dx, dz @ w.double(), mag @ w.double().abs(), o), (db, dz.sum(0), mag.sum(0), n),
+                            (dw, dz.t() @ x.double(), mag.t() @ x.double().abs(), n)):
+        _within(got, want, (k + 32) * 2 * E32 * m + U[t] * want.abs() + TINY[t], "gradient")
+    again = ad.linear_backward(dy, x, w, pre=pre, activation=act, param_grads=False)
+    assert torch.equal(again[0], dx) and again[1] is None
+    only = ad.linear_backward(dy, x, w, pre=pre, activation=act, input_grad=False)
+    assert only[0] is None and torch.equal(only[1], dw) and torch.equal(only[2], db)
+
+
 @pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("shape", [(40000, 64, 128), (20000, 136, 264), (9000, 520, 1000), (30001, 72, 72),
                                    (2500, 40, 8200), (19000, 200, 100)])

@@ -12,9 +12,10 @@ namespace fg {
 
 constexpr int SG_T = 64, SG_K = 16;
 
-// 64 x 64 tile per block of 256 threads, 4 x 4 outputs each, fp32 FMA.
+// 64 x 64 tile per block of 256 threads, 4 x 4 outputs each, fp32 FMA.  a_plane: A in two
+// parts, that many elements apart.
 template <class T>
-__global__ void __launch_bounds__(256) gemm_simt_kernel(const T* a, const T* b, const GemmShape g, const Epilogue e) {
+__global__ void __launch_bounds__(256) gemm_simt_kernel(const T* a, long long a_plane, const T* b, const GemmShape g, const Epilogue e) {
     __shared__ float sa[SG_K][SG_T + 1], sb[SG_K][SG_T + 1];
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const long long nt = (g.n + SG_T - 1) / SG_T;
@@ -25,7 +26,13 @@ __global__ void __launch_bounds__(256) gemm_simt_kernel(const T* a, const T* b, 
             // the fast index follows the unit stride of the operand
             const int ra = g.ak == 1 ? i / SG_K : i % SG_T, ka = g.ak == 1 ? i % SG_K : i / SG_T;
             const int rb = g.bk == 1 ? i / SG_K : i % SG_T, kb = g.bk == 1 ? i % SG_K : i / SG_T;
-            sa[ka][ra] = (m0 + ra < g.m && k0 + ka < g.k) ? to_f32(a[(m0 + ra) * g.am + (k0 + ka) * g.ak]) : 0.0f;
+            float v = 0.0f;
+            if (m0 + ra < g.m && k0 + ka < g.k) {
+                const T* p = a + (m0 + ra) * g.am + (k0 + ka) * g.ak;
+                v = to_f32(p[0]);
+                if (a_plane) v = PartsOf<T>::hi * v + PartsOf<T>::lo * to_f32(p[a_plane]);
+            }
+            sa[ka][ra] = v;
             sb[kb][rb] = (n0 + rb < g.n && k0 + kb < g.k) ? to_f32(b[(n0 + rb) * g.bn + (k0 + kb) * g.bk]) : 0.0f;
         }
         __syncthreads();
@@ -258,8 +265,17 @@ static int gemm(const Operand& a, const Operand& b, const GemmShape& g, const Ep
     long long tiles;
     const int rc = simt_gemm_check(g, &tiles);
     if (rc) return rc;
-    gemm_simt_kernel<T><<<(unsigned)tiles, 256, 0, s>>>(static_cast<const T*>(a.p), static_cast<const T*>(b.p), g, e);
+    gemm_simt_kernel<T><<<(unsigned)tiles, 256, 0, s>>>(static_cast<const T*>(a.p), sizeof(T) == 2 ? a.plane : 0,
+                                                         static_cast<const T*>(b.p), g, e);
     return check_launch("gemm_simt_kernel");
+}
+
+// GELU's and SiLU's dz is worked out in 32 bits, and 16-bit operands take it in two parts
+// (split2): rounded to one, the gradients were off by 0.0023 of their norm, not the 0.0017
+// of their own rounding, and float16 lost terms below 3e-8 and made those past 65504
+// infinite.  ReLU's is dy or 0, exact as it is.
+static bool in_parts(const fg_linear_params* p) {
+    return p->dtype != FG_DTYPE_F32 && (p->activation == FG_ACT_GELU || p->activation == FG_ACT_SILU);
 }
 
 // dz = dy act'(pre) and the column sums of dz, in one pass over dy and pre: a warp
@@ -325,7 +341,8 @@ __global__ void __launch_bounds__(DZ_WARPS * 32, 3) dz_kernel(const DzArgs g) {
             for (int u = 0; u < U; ++u) {
                 const long long q = r + u * DZ_WARPS;
                 if (q >= r1) break;
-                alignas(16) T o[VEC];
+                constexpr bool TWO = sizeof(T) == 2 && (ACT == FG_ACT_GELU || ACT == FG_ACT_SILU);
+                alignas(16) T o[VEC], low[TWO ? VEC : 1];
 #pragma unroll
                 for (int i = 0; i < VEC; i += 2) {
                     float v0 = to_f32(d[u][i]), v1 = to_f32(d[u][i + 1]);
@@ -334,13 +351,20 @@ __global__ void __launch_bounds__(DZ_WARPS * 32, 3) dz_kernel(const DzArgs g) {
                     v1 = i + 1 < left ? v1 : 0.0f;
                     sum[i] += v0;
                     sum[i + 1] += v1;
-                    o[i] = from_f32<T>(v0);
-                    o[i + 1] = from_f32<T>(v1);
+                    if constexpr (TWO) {
+                        split2(v0, o[i], low[i]);
+                        split2(v1, o[i + 1], low[i + 1]);
+                    } else {
+                        o[i] = from_f32<T>(v0);
+                        o[i + 1] = from_f32<T>(v1);
+                    }
                 }
-                if (g.dz) {  // an operand as the tensor cores take it: 16 bits, or three planes; padded rows
+                if (g.dz) {  // an operand as the tensor cores take it: one or two of 16 bits, or three planes; padded rows
                     const long long at = q * pack_stride(g.dim) + j;
                     if constexpr (sizeof(T) == 2) {
                         *reinterpret_cast<uint4*>(static_cast<T*>(g.dz) + at) = *reinterpret_cast<const uint4*>(o);
+                        if constexpr (TWO)
+                            *reinterpret_cast<uint4*>(static_cast<T*>(g.dz) + g.plane + at) = *reinterpret_cast<const uint4*>(low);
                     } else {
                         alignas(8) __nv_bfloat16 pl[3][VEC];
 #pragma unroll
@@ -461,7 +485,7 @@ static size_t forward_carve(const fg_linear_params* p, const Strides& t, void* w
     if (p->rows <= GEMV_ROWS) return 0;
     if (needs_pack(p->dtype, t.x)) f.x = c.take<char>(pack_bytes(p->dtype, p->rows, p->in_dim));
     if (needs_pack(p->dtype, t.w)) f.w = c.take<char>(pack_bytes(p->dtype, p->out_dim, p->in_dim));
-    const size_t n = tc_gemm_workspace(p->dtype, forward_shape(p, t));
+    const size_t n = tc_gemm_workspace(tc_products(p->dtype, false), forward_shape(p, t));
     if (n) f.product = c.take<char>(n);
     return c.used;
 }
@@ -490,9 +514,7 @@ static int linear_forward(const fg_linear_params* p, const Strides& t, const voi
 //
 // The first blocks take dx, 64 columns each: w is read once, a warp taking every
 // sixteenth of its rows, and dz of 512 columns at a time is worked out in shared
-// memory; the others take dw and db, four rows of w each.  dz stays in 32 bits: with
-// it rounded to 16 on its way to the tensor cores, as for more rows, one row's dx of
-// 107 -> 56 bf16 was off by 0.0033 where its own rounding is 0.0018.  Bound by the
+// memory; the others take dw and db, four rows of w each.  dz stays in 32 bits.  Bound by the
 // latency of w's loads, 32 rows of it under way in a block.  One row of 768 -> 1536 bf16
 // 10.5 us (with the launches of more rows 15.6), eight 21.7 (15.7, but five launches:
 // a call is 22 us, not 29); float32 9.1 and 20.7 (30 and 34).  Eight rows of 4096 ->
@@ -609,10 +631,12 @@ static size_t backward_carve(const fg_linear_params* p, const Strides& t, void* 
     Carve c(ws, bytes);
     w = BackwardWs{};
     if (few(p)) return 0;
-    if (p->activation != FG_ACT_NONE || needs_pack(p->dtype, t.y)) w.dz = c.take<char>(pack_bytes(p->dtype, p->rows, p->out_dim));
+    if (p->activation != FG_ACT_NONE || needs_pack(p->dtype, t.y))
+        w.dz = c.take<char>(pack_bytes(p->dtype, p->rows, p->out_dim) * (in_parts(p) ? 2 : 1));
     if (needs_pack(p->dtype, t.x)) w.x = c.take<char>(pack_bytes(p->dtype, p->rows, p->in_dim));
     if (needs_pack(p->dtype, t.w)) w.w = c.take<char>(pack_bytes(p->dtype, p->out_dim, p->in_dim));
-    const size_t n = std::max(tc_gemm_workspace(p->dtype, dx_shape(p, t, t.y)), tc_gemm_workspace(p->dtype, dw_shape(p, t, t.y)));
+    const int products = tc_products(p->dtype, in_parts(p));
+    const size_t n = std::max(tc_gemm_workspace(products, dx_shape(p, t, t.y)), tc_gemm_workspace(products, dw_shape(p, t, t.y)));
     if (n) w.product = c.take<char>(n);
     w.part = c.take<float>((size_t)dz_split(p->rows, p->out_dim, dtype_size(p->dtype)) * p->out_dim);
     return c.used;
@@ -627,7 +651,7 @@ static int linear_backward(const fg_linear_params* p, const Strides& t, const vo
                            s);
     const bool act = p->activation != FG_ACT_NONE, store = (act || needs_pack(p->dtype, t.y)) && (dx || dw);
     const int split = p->rows ? dz_split(p->rows, p->out_dim, sizeof(T)) : 0;
-    const long long plane = p->dtype == FG_DTYPE_F32 ? p->rows * pack_stride(p->out_dim) : 0;
+    const long long plane = p->dtype == FG_DTYPE_F32 || in_parts(p) ? p->rows * pack_stride(p->out_dim) : 0;
     int rc;
     if (split && (store || dbias)) {
         const DzArgs g{dy, act ? pre : nullptr, store ? ws.dz : nullptr, dbias ? ws.part : nullptr, t.y, t.p, p->rows, 0,

@@ -130,12 +130,41 @@ __device__ __forceinline__ void epilogue_store(const Epilogue& e, long long m, l
     static_cast<T*>(e.y)[m * e.ldy + n] = from_f32<T>(y);
 }
 
-// Tensor-core product (linear_tc.cu) of 16-bit operands, or for F32 of three bf16
-// planes of each, a_plane and b_plane elements apart.  tc_gemm_fits: the operands'
-// rows start on 16-byte boundaries, as their TMA loads need.  The workspace
-// (256-byte aligned) holds the partial tiles of a split product.
+// A 32-bit value as two of 16 bits, for an operand that is worked out in 32: the
+// rounding to the type, and the rounding of what that leaves.  bf16: v = p0 + p1, to 16
+// bits of the significand.  f16: v = 2 (p0 + 2^-12 p1), to 22 bits, or 2^-36 where that is
+// more: a gradient may lie below f16's 2^-24 and up to 1.13 times its largest value.  An
+// infinity or NaN has 0 behind it.
+constexpr int F16_PART_SHIFT = 12;
+template <class T>
+struct PartsOf {  // v = hi p0 + lo p1
+    static constexpr float hi = 1.0f, lo = 1.0f;
+};
+template <>
+struct PartsOf<__half> {
+    static constexpr float hi = 2.0f, lo = 2.0f / (1 << F16_PART_SHIFT);
+};
+__device__ __forceinline__ void split2(float v, __nv_bfloat16& p0, __nv_bfloat16& p1) {
+    p0 = from_f32<__nv_bfloat16>(v);
+    const bool finite = fabsf(v) <= FLT_MAX;
+    if (finite && !(fabsf(to_f32(p0)) <= FLT_MAX)) p0 = from_f32<__nv_bfloat16>(__uint_as_float(__float_as_uint(v) & 0xffff0000u));
+    p1 = from_f32<__nv_bfloat16>(finite ? v - to_f32(p0) : 0.0f);
+}
+__device__ __forceinline__ void split2(float v, __half& p0, __half& p1) {
+    const float h = v * 0.5f;
+    p0 = from_f32<__half>(h);
+    const float r = (h - to_f32(p0)) * (float)(1 << F16_PART_SHIFT);
+    p1 = from_f32<__half>(fabsf(v) <= FLT_MAX ? fminf(fmaxf(r, -65504.0f), 65504.0f) : 0.0f);
+}
+
+// Tensor-core product (linear_tc.cu) of 16-bit operands, A possibly in the two parts
+// above, a_plane elements apart (0: as it is), or for F32 of three bf16 planes of each,
+// a_plane and b_plane apart.  tc_gemm_fits: the operands' rows start on 16-byte
+// boundaries, as their TMA loads need.  The workspace (256-byte aligned) holds the
+// partial tiles of a split product; its size goes by the number of plane products.
+inline int tc_products(int dtype, bool parts) { return dtype == FG_DTYPE_F32 ? 6 : parts ? 2 : 1; }
 bool tc_gemm_fits(const void* a, const void* b, const GemmShape& g);
-size_t tc_gemm_workspace(int dtype, const GemmShape& g);
+size_t tc_gemm_workspace(int products, const GemmShape& g);
 int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& g,
             const Epilogue& e, void* ws, cudaStream_t s);
 

@@ -6,10 +6,12 @@
 // their sums rather than round them, about 1e-8 of the running value for every 16
 // products; so float32 sums are taken from TMEM after at most 512 k, the smallest
 // plane products first, and added in fp32, and 16-bit ones run over 32,768 k at most
-// before they meet other parts.  Either operand may have unit stride along k (K-major: x and w of the
+// before they meet other parts.  A 16-bit dz comes as two planes (split2): the lower one's
+// products are summed first, then the upper one's.  Either operand may have unit stride along k (K-major: x and w of the
 // forward pass, dz of dx = dz w) or along its rows (MN-major: w of dx, both
 // operands of dw = dz^T x), so no pass over memory transposes anything.
 #include <algorithm>
+#include <type_traits>
 
 #include "linear.cuh"
 #include "tc_common.cuh"
@@ -31,32 +33,40 @@ struct TcArgs {
     int m_pad;          // pairs with split > 1: rows of a part's partial tiles
     int vec;            // outputs, residual and bias allow 4-column accesses
     int direct;         // pairs: some of them do not start on 16-byte boundaries, which TMA needs
-    int planes;         // 1, or 3: float32
-    GemmShape f;        // planes == 3: the operands as they lie, for results that are not finite
-    const __nv_bfloat16 *fa, *fb;
+    int products;       // plane products: 1; 2: A in two parts; 6: float32, both in three
+    GemmShape f;        // products > 1: the operands as they lie, for results that are not finite
+    const void *fa, *fb;
     long long a_plane, b_plane;
     uint32_t idesc;
     Epilogue e;
 };
 
 // Planes of the i-th plane product.
-__device__ __forceinline__ int plane_a(int i, int planes) { return planes == 1 ? 0 : (280 >> (2 * i)) & 3; }  // 0 2 1 0 1 0
-__device__ __forceinline__ int plane_b(int i, int planes) { return planes == 1 ? 0 : (82 >> (2 * i)) & 3; }   // 2 0 1 1 0 0
+__device__ __forceinline__ int plane_a(int i, int products) {  // 0; 1 0; 0 2 1 0 1 0
+    return products == 1 ? 0 : products == 2 ? 1 - i : (280 >> (2 * i)) & 3;
+}
+__device__ __forceinline__ int plane_b(int i, int products) { return products < 6 ? 0 : (82 >> (2 * i)) & 3; }  // 2 0 1 1 0 0
 
 // An infinite operand times the small planes of the other has any sign: a result
 // that is not finite is taken again, one product at a time.
-static __device__ __noinline__ float retake(const TcArgs& g, int m, int n) {
+template <class T>
+__device__ __noinline__ float retake(const TcArgs& g, int m, int n) {
+    using E = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;  // of a plane
     float z = 0.0f;
-    auto value = [](const __nv_bfloat16* p, long long step) {
-        return to_f32(p[0]) + to_f32(p[step]) + to_f32(p[2 * step]);
-    };
-    for (long long k = 0; k < g.f.k && z == z; ++k)
-        z = fmaf(value(g.fa + m * g.f.am + k * g.f.ak, g.a_plane), value(g.fb + n * g.f.bn + k * g.f.bk, g.b_plane), z);
+    auto whole = [](const E* p, long long step) { return to_f32(p[0]) + to_f32(p[step]) + to_f32(p[2 * step]); };
+    for (long long k = 0; k < g.f.k && z == z; ++k) {
+        const E* a = static_cast<const E*>(g.fa) + m * g.f.am + k * g.f.ak;
+        const E* b = static_cast<const E*>(g.fb) + n * g.f.bn + k * g.f.bk;
+        if constexpr (sizeof(T) == 4)
+            z = fmaf(whole(a, g.a_plane), whole(b, g.b_plane), z);
+        else
+            z = fmaf(PartsOf<T>::hi * to_f32(a[0]) + PartsOf<T>::lo * to_f32(a[g.a_plane]), to_f32(b[0]), z);
+    }
     return z;
 }
 template <class T>
 __device__ __forceinline__ float finite_or_retake(const TcArgs& g, int m, int n, float z) {
-    return sizeof(T) == 4 && !(fabsf(z) <= FLT_MAX) ? retake(g, m, n) : z;
+    return !(fabsf(z) <= FLT_MAX) ? retake<T>(g, m, n) : z;
 }
 
 template <int BN>
@@ -139,7 +149,7 @@ __device__ __forceinline__ void store4<float>(float* p, float4 f) {
 // operand ring was); then each CTA adds one slice of the columns over the cluster,
 // from its own rank onwards -- were all to begin with rank 0, they would queue for its
 // shared memory: 100 x 1536 -> 768 bf16 8.2 us, so 7.6 -- and finishes it.
-template <class T, int BN>
+template <class T, int BN, bool PARTS>
 __global__ void __launch_bounds__(GT_NT, 1)
     gemm_split_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const __grid_constant__ TcArgs g) {
     using Ring = RingOf<BN>;
@@ -159,7 +169,8 @@ __global__ void __launch_bounds__(GT_NT, 1)
     const int kb0 = (int)((long long)g.kt * rank / S), kb1 = (int)((long long)g.kt * (rank + 1) / S);
     // accumulators: one, or for float32 as many as TMEM holds, each for GP_CHUNK K blocks
     constexpr int NA = sizeof(T) == 4 ? 512 / BN : 1;
-    const int share = sizeof(T) == 4 ? GP_CHUNK : kb1 - kb0, shares = (kb1 - kb0 + share - 1) / share, products = sizeof(T) == 4 ? 6 : 1;
+    const int share = sizeof(T) == 4 ? GP_CHUNK : kb1 - kb0, shares = (kb1 - kb0 + share - 1) / share;
+    constexpr int products = sizeof(T) == 4 ? 6 : PARTS ? 2 : 1;
 
     if (warp == 2 && tc::elect_one()) {
         tc::prefetch_map(&ta);
@@ -233,8 +244,13 @@ __global__ void __launch_bounds__(GT_NT, 1)
                 const uint64_t da = da0 + st * (Ring::STAGE / 16), db = db0 + st * (Ring::STAGE / 16);
                 if (tc::elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < GT_K / 16; ++kk)
-                        tc::umma_bf16(taddr + (uint32_t)(acc * BN), da + ka * kk, db + kbs * kk, g.idesc, (u | kk) != 0);
+                    for (int kk = 0; kk < GT_K / 16; ++kk) {
+                        const uint32_t d = taddr + (uint32_t)(acc * BN);
+                        if (std::is_same<T, __half>::value && PARTS && kk == 0 && 2 * u == n)  // on to the upper part
+                            tc::umma_shifted<F16_PART_SHIFT>(d, da, db, g.idesc);
+                        else
+                            tc::umma_bf16(d, da + ka * kk, db + kbs * kk, g.idesc, (u | kk) != 0);
+                    }
                     tc::umma_commit(&empty[st]);
                     if (u + 1 == n && c0 + share >= kb1) tc::umma_commit(&acc_full);
                 }
@@ -275,6 +291,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
     // one memory latency a round.
     constexpr int U = 4;
     constexpr bool FAST = sizeof(T) == 2;
+    constexpr float scale = PartsOf<T>::hi;
     const int slice = BN / S, per_row = slice / 4;
     const uint32_t pbase = tc::smem_u32(part);
     const Epilogue& e = g.e;
@@ -324,7 +341,8 @@ __global__ void __launch_bounds__(GT_NT, 1)
                 z = *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(part) + at[u]);
             }
             const bool whole = col[u] + 4 <= g.n;
-            if (!FAST) {
+            if (PARTS) z = make_float4(z.x * scale, z.y * scale, z.z * scale, z.w * scale);
+            if (products > 1) {
                 z.x = finite_or_retake<T>(g, row[u], col[u], z.x);
                 if (col[u] + 1 < g.n) z.y = finite_or_retake<T>(g, row[u], col[u] + 1, z.y);
                 if (col[u] + 2 < g.n) z.z = finite_or_retake<T>(g, row[u], col[u] + 2, z.z);
@@ -473,8 +491,8 @@ __device__ __forceinline__ void add_bias(float (&v)[2][32], const unsigned char*
 }
 
 // DIRECT: outputs, residual or bias do not start on 16-byte boundaries, which TMA
-// needs: they pass row by row between memory and the buffer.
-template <class T, int BN, bool DIRECT>
+// needs: they pass row by row between memory and the buffer.  PARTS: A in two parts.
+template <class T, int BN, bool DIRECT, bool PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                      const __grid_constant__ CUtensorMap ty, const __grid_constant__ CUtensorMap tp,
@@ -485,13 +503,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     extern __shared__ __align__(1024) unsigned char dsmem[];
     __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], acc_full[2], acc_empty[2], res_full[GP_EPI];
     __shared__ uint32_t tmem_slot;
-    __shared__ int s_fail;
+    __shared__ int s_fail, s_odd;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)cluster_rank();
     unsigned char *ring = dsmem, *bufs = ring + GP_STAGES * P::STAGE, *biases = bufs + GP_EPI * P::BUF;
     const int pairs = (int)(gridDim.x >> 1), items = g.mt * g.nt * g.split;
     auto k_begin = [&](int part) { return (int)((long long)g.kt * part / g.split); };
-    constexpr int products = sizeof(T) == 4 ? 6 : 1, chunk = sizeof(T) == 4 ? GP_CHUNK : 1 << 30;
+    constexpr int chunk = sizeof(T) == 4 ? GP_CHUNK : 1 << 30;
+    constexpr int products = sizeof(T) == 4 ? 6 : PARTS ? 2 : 1;
+    constexpr float scale = PartsOf<T>::hi;
 
     if (warp == 2 && tc::elect_one()) {
         tc::prefetch_map(&ta);
@@ -503,7 +523,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
         }
     }
     if (tid == 0) {
-        s_fail = 0;
+        s_fail = s_odd = 0;
         for (int i = 0; i < GP_STAGES; ++i) {
             tc::mbar_init(&full[i], 1);
             tc::mbar_init(&empty[i], 1);
@@ -583,9 +603,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         const uint64_t da = da0 + st * (P::STAGE / 16), db = db0 + st * (P::STAGE / 16);
                         if (tc::elect_one()) {
 #pragma unroll
-                            for (int kk = 0; kk < GT_K / 16; ++kk)
-                                tc::umma_pair(taddr + (uint32_t)(acc * BN), da + ka * kk, db + kbs * kk, g.idesc,
-                                              (u | kk) != 0);
+                            for (int kk = 0; kk < GT_K / 16; ++kk) {
+                                const uint32_t d = taddr + (uint32_t)(acc * BN);
+                                if (std::is_same<T, __half>::value && PARTS && kk == 0 && 2 * u == n)
+                                    tc::umma_pair_shifted<F16_PART_SHIFT>(d, da, db, g.idesc);  // on to the upper part
+                                else
+                                    tc::umma_pair(d, da + ka * kk, db + kbs * kk, g.idesc, (u | kk) != 0);
+                            }
                             tc::umma_commit_pair(&empty[st]);
                             if (u + 1 == n) tc::umma_commit_pair(&acc_full[acc]);
                         }
@@ -608,6 +632,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
         };
         const int step = pairs * P::GROUPS;
         int item = (blockIdx.x >> 1) + pairs * group, li = group;
+        bool odd_seen = false;  // a result that is not finite, stored as NaN and taken again at the end
         const bool ahead = sizeof(T) == 2 && e.residual && !e.pre;  // residuals a tile ahead (DIRECT: during its products)
         if (!DIRECT && ahead && item < items && tc::elect_one()) fetch_residual(item);
         if constexpr (sizeof(T) == 4) {
@@ -788,6 +813,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     for (int j = 0; j < 32; ++j) v[h][j] = NAN;
                 }
             }
+            if (PARTS) {
+                bool odd = false;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        v[h][j] *= scale;
+                        odd |= !(fabsf(v[h][j]) <= FLT_MAX);
+                    }
+                if (__any_sync(0xffffffffu, odd && ok)) {
+                    odd_seen = true;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[h][j] = fabsf(v[h][j]) <= FLT_MAX ? v[h][j] : NAN;
+                }
+            }
             if (e.bias) add_bias<T>(v, bias);
             if (e.pre) {
                 if (tc::elect_one()) tc::bulk_wait_read<0>();
@@ -854,18 +896,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             }
         }
         }
-        if (tc::elect_one()) tc::bulk_wait_read<0>();
+        if (tc::elect_one()) {
+            if (odd_seen) s_odd = 1;
+            tc::bulk_wait_read<0>();
+        }
     }
     tc::fence_before_sync();
     __syncthreads();
     cluster_sync();  // no CTA leaves while its peer still reads its memory
     tc::fence_after_sync();
     if (warp == 1) tc::tmem_dealloc_pair(taddr, 2 * BN);
+    // Results that are not finite lie in this CTA's tiles as NaN, and are taken again here,
+    // where nothing waits: each is a sum over all of k by one thread.
+    if (!PARTS || !s_odd || s_fail) return;
+    if (warp >= 2 && tc::elect_one()) tc::bulk_wait();  // this block's stores have arrived
+    __syncthreads();
+    const Epilogue& e = g.e;
+    const T* mark = static_cast<const T*>(e.pre ? e.pre : e.y);
+    const long long ld = e.pre ? e.ldp : e.ldy;
+    for (int t = blockIdx.x >> 1; t < items; t += pairs) {
+        const int m0 = t / g.nt * 2 * GT_M + rank * GT_M, n0 = t % g.nt * BN;
+        for (int i = tid; i < GT_M * BN; i += GP_NT) {
+            const int row = m0 + i / BN, col = n0 + i % BN;
+            if (row >= g.m || col >= g.n) continue;
+            const float y = to_f32(__ldcg(mark + row * ld + col));
+            if (y != y) epilogue_store<T>(e, row, col, retake<T>(g, row, col));
+        }
+    }
 }
 
 // The parts of split tiles, added in their order, and the epilogue: four columns a thread.
-template <class T>
-__global__ void __launch_bounds__(256) finish_kernel(const float* part, const TcArgs g, long long ldp) {
+template <class T, bool PARTS>
+__global__ void __launch_bounds__(256) finish_kernel(const float* part, const __grid_constant__ TcArgs g, long long ldp) {
     const int c4 = (g.n + 3) / 4;
     const long long i = blockIdx.x * 256ll + threadIdx.x, row = i / c4;
     if (row >= g.m) return;
@@ -879,8 +941,10 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* part, const Tc
         z.z += v.z;
         z.w += v.w;
     }
+    constexpr float scale = PARTS ? PartsOf<T>::hi : 1.0f;
+    if (PARTS) z = make_float4(z.x * scale, z.y * scale, z.z * scale, z.w * scale);
     float v[4] = {z.x, z.y, z.z, z.w};
-    if (sizeof(T) == 4) {
+    if (sizeof(T) == 4 || PARTS) {
         for (int j = 0; j < 4; ++j)
             if (col + j < g.n) v[j] = finite_or_retake<T>(g, (int)row, col + j, v[j]);
         z = make_float4(v[0], v[1], v[2], v[3]);
@@ -911,6 +975,9 @@ static int operand_map(CUtensorMap* m, int dtype, const void* p, long long rows,
     return FG_OK;
 }
 
+static int a_planes(const TcArgs& g) { return g.products == 6 ? 3 : g.products; }
+static int b_planes(const TcArgs& g) { return g.products == 6 ? 3 : 1; }
+
 // Instruction descriptor, kind::f16: f32 accumulators.
 static uint32_t instr_desc(int dtype, int m, int n, bool a_mn, bool b_mn) {
     const uint32_t t = dtype == FG_DTYPE_F16 ? 0 : 1;
@@ -927,14 +994,16 @@ bool tc_gemm_fits(const void* a, const void* b, const GemmShape& g) {
 template <class T, int BN>
 static int launch_split(int dtype, const void* a, const void* b, const GemmShape& s, TcArgs g, cudaStream_t st) {
     CUtensorMap ta, tb;
-    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M, g.planes, g.a_plane);
-    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN, g.planes, g.b_plane);
+    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M, a_planes(g), g.a_plane);
+    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN, b_planes(g), g.b_plane);
     if (rc) return rc;
     g.idesc = instr_desc(dtype, GT_M, BN, g.a_mn, g.b_mn);
     g.nt = (g.n + BN - 1) / BN;
     const long long ctas = (long long)g.mt * g.nt * g.split;
     FG_REQUIRE(ctas <= 0x7fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
-    auto kernel = &gemm_split_kernel<T, BN>;
+    auto kernel = &gemm_split_kernel<T, BN, false>;
+    if constexpr (sizeof(T) == 2)
+        if (g.products == 2) kernel = &gemm_split_kernel<T, BN, true>;
     const int smem = RingOf<BN>::N * RingOf<BN>::STAGE + 1024;
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
     cudaLaunchConfig_t cfg = {};
@@ -980,8 +1049,8 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
     g.mt = (g.m + 2 * GT_M - 1) / (2 * GT_M);
     g.nt = (g.n + BN - 1) / BN;
     g.m_pad = g.mt * 2 * GT_M;
-    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M, g.planes, g.a_plane);
-    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN / 2, g.planes, g.b_plane);
+    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M, a_planes(g), g.a_plane);
+    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN / 2, b_planes(g), g.b_plane);
     if (g.split > 1) {
         if (!rc) rc = tile_map(&ty, FG_DTYPE_F32, ws, (long long)g.split * g.m_pad, ld, ld);
     } else if (!g.direct) {
@@ -993,7 +1062,10 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
     g.idesc = instr_desc(dtype, 2 * GT_M, BN, g.a_mn, g.b_mn);
     const long long items = (long long)g.mt * g.nt * g.split;
     FG_REQUIRE(items <= 0x3fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
-    auto kernel = g.direct && g.split == 1 ? &gemm_pair_kernel<T, BN, true> : &gemm_pair_kernel<T, BN, false>;
+    const bool direct = g.direct && g.split == 1;
+    auto kernel = direct ? &gemm_pair_kernel<T, BN, true, false> : &gemm_pair_kernel<T, BN, false, false>;
+    if constexpr (sizeof(T) == 2)
+        if (g.products == 2) kernel = direct ? &gemm_pair_kernel<T, BN, true, true> : &gemm_pair_kernel<T, BN, false, true>;
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), PairOf<T, BN>::SMEM));
     const int pairs = std::max(1, device_attr(cudaDevAttrMultiProcessorCount) / 2);
     TcArgs k = g;
@@ -1002,7 +1074,8 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
     rc = check_launch("gemm_pair_kernel");
     if (rc || g.split == 1) return rc;
     const long long n4 = (long long)g.m * ((g.n + 3) / 4);
-    finish_kernel<T><<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(static_cast<const float*>(ws), g, ld);
+    auto finish = sizeof(T) == 2 && g.products == 2 ? &finish_kernel<T, true> : &finish_kernel<T, false>;
+    finish<<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(static_cast<const float*>(ws), g, ld);
     return check_launch("finish_kernel");
 }
 
@@ -1022,9 +1095,9 @@ struct TcPlan {
     size_t ws;
 };
 
-static TcPlan tc_plan_of(const GemmShape& s, int planes, bool direct) {
+static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct) {
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
-    const int kt = (int)((s.k + GT_K - 1) / GT_K) * (planes == 1 ? 1 : 6);
+    const int kt = (int)((s.k + GT_K - 1) / GT_K) * products;
     auto waves = [](long long tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
     TcPlan best{false, 256, 1, 0};
     double least = 1e300;
@@ -1037,12 +1110,12 @@ static TcPlan tc_plan_of(const GemmShape& s, int planes, bool direct) {
     const long long m2 = (s.m + 2 * GT_M - 1) / (2 * GT_M), m1 = (s.m + GT_M - 1) / GT_M;
     const int kb = (int)((s.k + GT_K - 1) / GT_K);
     for (int bn : {256, 128}) {
-        if (planes == 3 && bn == 128) break;
+        if (products == 6 && bn == 128) break;
         const long long tiles = m2 * ((s.n + bn - 1) / bn);
         for (int sp : {1, 2, 4, 8, 16, 32}) {
             if (direct && sp > 1) break;
             if (sp > 1 && (sp > kb / 2 || (tiles * sp > sms && kb * 2 / sp <= GT_RUN))) break;
-            if (planes == 1 && kb > GT_RUN * sp && sp < 32) continue;
+            if (products < 6 && kb > GT_RUN * sp && sp < 32) continue;
             const size_t ws = sp > 1 ? (size_t)sp * m2 * 2 * GT_M * ((s.n + 3) / 4 * 4) * 4 : 0;
             const double epi = bn == 256 ? 2.0 : 1.0, main = (kt + sp - 1) / sp * (bn == 256 ? 0.39 : 0.34);
             const double rows = direct ? (bn == 256 ? 14.0 : 8.0) : 0.0;
@@ -1055,7 +1128,7 @@ static TcPlan tc_plan_of(const GemmShape& s, int planes, bool direct) {
         for (int sp : {1, 2, 4, 8}) {
             if (sp > kb || (direct && sp > 1)) break;
             // the sums' length: 512 k for each of float32's 512 / bn accumulators
-            if (kb > (planes == 1 ? GT_RUN : GP_CHUNK * 512 / bn) * sp && kb > 3) continue;
+            if (kb > (products < 6 ? GT_RUN : GP_CHUNK * 512 / bn) * sp && kb > 3) continue;
             const int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
             const double main = (kt + sp - 1) / sp * (bn == 256 ? 0.43 : bn == 128 ? 0.30 : 0.21);
             const double rows = direct ? 0.055 * bn : 0.0;
@@ -1069,13 +1142,13 @@ static TcPlan tc_plan_of(const GemmShape& s, int planes, bool direct) {
 // tiles (1777 x 101 -> 333 bf16: 27 us with pairs, 12 in tiles of 64 columns).  Only
 // tiles whose sums are not split are chosen anew: those add in one order whichever
 // kernel takes them, so that a result does not depend on where it is written.
-static TcPlan tc_plan(const GemmShape& s, int planes, bool direct) {
-    const TcPlan p = tc_plan_of(s, planes, false);
-    return direct && p.split == 1 ? tc_plan_of(s, planes, true) : p;
+static TcPlan tc_plan(const GemmShape& s, int products, bool direct) {
+    const TcPlan p = tc_plan_of(s, products, false);
+    return direct && p.split == 1 ? tc_plan_of(s, products, true) : p;
 }
 
-size_t tc_gemm_workspace(int dtype, const GemmShape& s) {
-    return s.k > 0 ? tc_plan(s, dtype == FG_DTYPE_F32 ? 3 : 1, false).ws : 0;
+size_t tc_gemm_workspace(int products, const GemmShape& s) {
+    return s.k > 0 ? tc_plan(s, products, false).ws : 0;
 }
 
 int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& s,
@@ -1087,18 +1160,18 @@ int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long lon
     g.mt = (int)((s.m + GT_M - 1) / GT_M);
     g.a_mn = s.ak != 1;
     g.b_mn = s.bk != 1;
-    g.planes = dtype == FG_DTYPE_F32 ? 3 : 1;
+    g.products = tc_products(dtype, a_plane != 0);
     g.f = s;
-    g.fa = static_cast<const __nv_bfloat16*>(a);
-    g.fb = static_cast<const __nv_bfloat16*>(b);
-    g.a_plane = g.planes == 1 ? 8 : a_plane;  // one plane: any multiple of 16 bytes
-    g.b_plane = g.planes == 1 ? 8 : b_plane;
+    g.fa = a;
+    g.fb = b;
+    g.a_plane = a_planes(g) == 1 ? 8 : a_plane;  // one plane: any multiple of 16 bytes
+    g.b_plane = b_planes(g) == 1 ? 8 : b_plane;
     g.e = e;
     const int es = dtype_size(dtype);
     auto lies = [&](const void* p, long long ld, int n) { return !p || (aligned(p, n) && ld * es % n == 0); };
     g.vec = lies(e.y, e.ldy, 4 * es) && lies(e.bias, 0, 4 * es) && lies(e.pre, e.ldp, 4 * es) && lies(e.residual, e.ldr, 4 * es);
     g.direct = !(lies(e.y, e.ldy, 16) && lies(e.bias, 0, 16) && lies(e.pre, e.ldp, 16) && lies(e.residual, e.ldr, 16));
-    const TcPlan p = tc_plan(s, g.planes, g.direct);
+    const TcPlan p = tc_plan(s, g.products, g.direct);
     g.split = p.split;
 #define FG_PRODUCT(T)                                                                        \
     (p.pair ? (sizeof(T) == 4 || p.bn == 256                                              \

@@ -508,7 +508,8 @@ int fg_linear(const fg_linear_params* params, const void* x, const void* w, cons
  * dw [out_dim][in_dim] = dz^T x, dbias [out_dim] = sum over rows of dz, all
  * contiguous and of dtype; any may be NULL (w is needed for dx, x for dw, pre
  * unless the activation is NONE).  The residual's gradient is dy itself.
- * ReLU's derivative at 0 is 0. */
+ * ReLU's derivative at 0 is 0.  GELU's and SiLU's dz of F16 and BF16 enters the
+ * products to 22 and 16 bits of its significand (F16: or to 2^-36). */
 int fg_linear_backward_workspace_size(const fg_linear_params* params, size_t* bytes);
 int fg_linear_backward(const fg_linear_params* params, const void* dy, const void* x, const void* w, const void* pre,
                        void* dx, void* dw, void* dbias, void* workspace, size_t workspace_bytes, void* stream);

@@ -1,0 +1,118 @@
+"""GPU tests of the query adapter's operators where they can lose what the
+definition keeps: gradients of 16-bit layers, the activations' tails, values that
+are not finite, operands off 16-byte boundaries, pairs that no query holds.
+
+Tolerances follow from the arithmetic as in test_gpu_adapter.py, whose helpers
+are used: U[t] is the unit roundoff of a result's type, E32 that of 32-bit sums.
+"""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_adapter import E32, T, TINY, U, _act, _act_grad, _check_backward, _check_linear, _gen, _randn, _within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ad():
+    from fusiongpu_b200 import adapter
+    return adapter
+
+
+# ---- dz of 16-bit layers of more than eight rows ---------------------------------------
+#
+# dz = dy act'(pre) goes to the tensor cores in two parts of the type: together they are
+# off by the product of two unit roundoffs (2^-18 bf16, 2^-24 f16), doubled here, and in
+# float16 by half the lower part's last place, 2^-36.  The derivative's own error is
+# SLOPE: 2^-22 of the fit and a few operations in 32 bits, or of __expf.
+
+PARTS = {"f16": 2.0 ** -23, "bf16": 2.0 ** -17}
+FLOOR = {"f16": 2.0 ** -36, "bf16": 0.0}
+SLOPE = 2.0 ** -19
+
+
+def _check_dz(ad, dy, x, w, pre, act, t):
+    dx, dw, db = ad.linear_backward(dy, x, w, pre=pre, activation=act)
+    d = dy.double()
+    dz = d * _act_grad(pre.double(), act)
+    edz = SLOPE * d.abs() + PARTS[t] * dz.abs() + FLOOR[t]
+    n, o = d.shape
+    for got, want, err, k, mag in (
+            (dx, dz @ w.double(), edz @ w.double().abs(), o, dz.abs() @ w.double().abs()),
+            (dw, dz.t() @ x.double(), edz.t() @ x.double().abs(), n, dz.abs().t() @ x.double().abs()),
+            (db, dz.sum(0), SLOPE * d.abs().sum(0), n, dz.abs().sum(0))):
+        _within(got, want, err + (k + 8) * 2 * E32 * mag + U[t] * want.abs() + TINY[t], f"{tuple(got.shape)}")
+    return dx, dw, db
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("shape", [(9, 56, 107), (40, 264, 520), (300, 768, 1536), (3000, 136, 264), (10000, 768, 1536),
+                                   (20001, 72, 1000), (40000, 520, 72)])
+def test_gradients_have_one_rounding(ad, shape, act, t):
+    n, i, o = shape
+    g = _gen(n + i)
+    x, w = _randn(g, n, i, t=t), _randn(g, o, i, t=t, scale=i ** -0.5)
+    dy, pre = _randn(g, n, o, t=t, scale=0.1), _randn(g, n, o, t=t, scale=1.5)
+    got = _check_dz(ad, dy, x, w, pre, act, t)
+    for u, v in zip(got, ad.linear_backward(dy, x, w, pre=pre, activation=act)):
+        assert torch.equal(u, v)
+    k = slice(0, 8)  # eight rows have a kernel of their own: the same values to 32 bits
+    _check_dz(ad, dy[k], x[k], w, pre[k], act, t)
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("shape", [(16, 40, 72), (4000, 136, 264)])
+def test_float16_gradients_below_and_above_its_range(ad, shape, act):
+    """Terms of dz too small for float16 whose sum is not, and terms past its largest."""
+    n, i, o = shape
+    g = _gen(n)
+    x, w = _randn(g, n, i, t="f16").abs() + 0.5, _randn(g, o, i, t="f16").abs() + 0.5
+    dy = (torch.rand(n, o, generator=g, device="cuda") + 0.5).mul(1e-6).half()
+    pre = (-3.5 - torch.rand(n, o, generator=g, device="cuda")).half()
+    d, p = dy.double(), pre.double()
+    dx, dw, _ = ad.linear_backward(dy, x, w, pre=pre, activation=act)
+    dz = d * _act_grad(p, act)
+    edz = 2.0 ** -15 * dz.abs() + FLOOR["f16"]  # this far out the derivative is right to 2^-16 of itself
+    assert dz.abs().mean() < 2.0 ** -23 and dz.abs().max() > 2.0 ** -34
+    for got, want, err in ((dx, dz @ w.double(), edz @ w.double()), (dw, dz.t() @ x.double(), edz.t() @ x.double())):
+        _within(got, want, err + U["f16"] * want.abs() + TINY["f16"], "small")
+    if n > 1000:
+        assert (dw != 0).all()
+    dy = torch.full((n, o), 62000.0, device="cuda", dtype=torch.float16)
+    pre = torch.full((n, o), 1.40625 if act == "gelu" else 2.40625, device="cuda", dtype=torch.float16)
+    dz = dy.double() * _act_grad(pre.double(), act)
+    assert (dz > 65520).all()
+    x, w = torch.full_like(x, 2.0 ** -7 / n), torch.full_like(w, 2.0 ** -10)
+    dx, dw, _ = ad.linear_backward(dy, x, w, pre=pre, activation=act)
+    edz = 2.0 ** -18 * dz
+    for got, want, err in ((dx, dz @ w.double(), edz @ w.double()), (dw, dz.t() @ x.double(), edz.t() @ x.double())):
+        _within(got, want, err + (n + o) * 2 * E32 * want + U["f16"] * want, "large")
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", [(30, 72, 40), (3000, 264, 520), (30000, 136, 264)])
+def test_gradients_with_infinite_operands(ad, shape, t):
+    """An infinite weight or input times any dz but 0 is infinite, whatever parts dz has."""
+    n, i, o = shape
+    g = _gen(i)
+    x, w = _randn(g, n, i, t=t), _randn(g, o, i, t=t)
+    dy, pre = _randn(g, n, o, t=t), _randn(g, n, o, t=t)
+    dy[:, o // 2] = torch.where(dy[:, o // 2] == 0, 1.0, dy[:, o // 2])
+    w[o // 2, 5] = math.inf
+    x[n // 2, 3] = -math.inf
+    dy[n // 2] = 0.5
+    pre[n // 2] = 1.0
+    dz = dy.double() * _act_grad(pre.double(), "gelu")
+    dx, dw, db = ad.linear_backward(dy, x, w, pre=pre, activation="gelu")
+    assert torch.equal(dx[:, 5].double(), torch.sign(dz[:, o // 2]) * math.inf)
+    assert torch.equal(dw[:, 3].double(), torch.full_like(dz[0], -math.inf))
+    dx[:, 5] = dw[:, 3] = 0
+    assert dx.isfinite().all() and dw.isfinite().all() and db.isfinite().all()
+    dy[1, 2] = math.nan  # poison reaches what depends on it
+    dx, dw, db = ad.linear_backward(dy, x, w, pre=pre, activation="gelu")
+    assert dx[1].isnan().all() and dw[2].isnan().all() and db[2].isnan()
+    keep = torch.arange(n, device="cuda") != 1
+    assert not dx[keep].isnan().any() and not dw[torch.arange(o, device="cuda") != 2].isnan().any()

@@ -734,6 +734,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
 #pragma unroll 4
                         for (int j = 0; j < 32; ++j) v[j] = activate<false>(v[j], e.act);
                     }
+                    // the sums and z were read and written here by ordinary accesses: before a copy lands on them
+                    if (!DIRECT && e.residual) tc::fence_proxy_async();
                     if (tc::elect_one()) tc::bulk_wait_read<0>();
                     __syncwarp();
                     if (e.residual) {

@@ -116,3 +116,20 @@ def test_gradients_with_infinite_operands(ad, shape, t):
     assert dx[1].isnan().all() and dw[2].isnan().all() and db[2].isnan()
     keep = torch.arange(n, device="cuda") != 1
     assert not dx[keep].isnan().any() and not dw[torch.arange(o, device="cuda") != 2].isnan().any()
+
+
+# ---- buffers handed from ordinary accesses to copies ---------------------------------------
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(40000, 64, 128), (20000, 136, 264), (9000, 520, 1000)])
+def test_residual_with_and_without_the_pre_activation(ad, shape, t):
+    """The residual comes through the buffer that held the sums: the same result whether
+    or not the pre-activation left through it in between."""
+    n, i, o = shape
+    g = _gen(o)
+    x, w = _randn(g, n, i, t=t), _randn(g, o, i, t=t, scale=i ** -0.5)
+    b, res = _randn(g, o, t=t), _randn(g, n, o, t=t)
+    for act in ("none", "silu"):
+        want = ad.linear(x, w, b, activation=act, residual=res, return_pre=True)[0]
+        for _ in range(5):
+            assert torch.equal(ad.linear(x, w, b, activation=act, residual=res), want)

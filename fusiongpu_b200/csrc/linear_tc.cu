@@ -490,6 +490,20 @@ __device__ __forceinline__ void add_bias(float (&v)[2][32], const unsigned char*
         for (int j = 0; j < 32; j += 8) add8<T>(&v[h][j], *reinterpret_cast<const uint4*>(b + (32 * h + j) * 2));
 }
 
+// Waits for a copy into a buffer of this warp.  When another role has failed the first
+// wait ends early, and the copy, which may still land, is waited for by itself.
+__device__ __forceinline__ bool copy_landed(uint64_t* bar, uint32_t parity, volatile int* fail) {
+    return tc::mbar_wait_warp(bar, parity, fail) || __all_sync(0xffffffffu, tc::mbar_wait(bar, parity));
+}
+
+// NaN in `cols` columns of a warp's 32 rows, past a buffer that a copy may yet land in.
+template <class T>
+__device__ __noinline__ void store_nan(void* matrix, long long ld, int row0, int col0, int rows, int last, int cols) {
+    const int row = row0 + (int)(threadIdx.x & 31);
+    if (!matrix || row >= rows) return;
+    for (int c = col0; c < min(col0 + cols, last); ++c) static_cast<T*>(matrix)[row * ld + c] = from_f32<T>(NAN);
+}
+
 // DIRECT: outputs, residual or bias do not start on 16-byte boundaries, which TMA
 // needs: they pass row by row between memory and the buffer.  PARTS: A in two parts.
 template <class T, int BN, bool DIRECT, bool PARTS>
@@ -632,6 +646,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
         };
         const int step = pairs * P::GROUPS;
         int item = (blockIdx.x >> 1) + pairs * group, li = group;
+        bool lost = false;      // a residual never came: this warp's results are NaN from there on
         bool odd_seen = false;  // a result that is not finite, stored as NaN and taken again at the end
         const bool ahead = sizeof(T) == 2 && e.residual && !e.pre;  // residuals a tile ahead (DIRECT: during its products)
         if (!DIRECT && ahead && item < items && tc::elect_one()) fetch_residual(item);
@@ -674,6 +689,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 for (int h = 0; h < 2; ++h) {
                     const int c0 = col + 32 * h;
                     const bool in = m0 < g.m && c0 < g.n;
+                    if (lost) {
+                        store_nan<T>(e.pre, e.ldp, m0, c0, g.m, g.n, 32);
+                        store_nan<T>(e.y, e.ldy, m0, c0, g.m, g.n, 32);
+                        continue;
+                    }
                     unsigned char *hbuf = buf + h * GP_BUF, *hrow = brow + h * GP_BUF;
                     auto put = [&](const CUtensorMap* map, int y0, bool store) {
                         tc::fence_proxy_async();
@@ -746,8 +766,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                                 tc::mbar_arrive_expect_tx(&res_full[w], GP_BUF);
                                 tc::tma_load_2d(hbuf, &tr, &res_full[w], c0, m0);
                             }
-                            tc::mbar_wait_warp(&res_full[w], res_phase, fail);
+                            lost = !copy_landed(&res_full[w], res_phase, fail);
                             res_phase ^= 1;
+                            if (lost) {
+                                store_nan<T>(e.y, e.ldy, m0, c0, g.m, g.n, 32);
+                                continue;
+                            }
                         }
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
@@ -770,6 +794,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             const int acc = li & 1, t = item / g.split;
             const int col = t % g.nt * BN + part * 64, m0 = t / g.nt * 2 * GT_M + tr_rows;
             const bool inside = m0 < g.m && col < g.n;
+            if (!DIRECT && lost) {
+                store_nan<T>(e.pre, e.ldp, m0, col, g.m, g.n, 64);
+                store_nan<T>(e.y, e.ldy, m0, col, g.m, g.n, 64);
+                continue;
+            }
             unsigned char* bias = biases + w * 128;
             if (e.bias) {
                 reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(static_cast<const T*>(e.bias) + col, lane, g.n - col, DIRECT);
@@ -868,8 +897,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             }
             if (e.residual) {
                 if (!DIRECT) {
-                    tc::mbar_wait_warp(&res_full[w], res_phase, fail);
+                    lost = !copy_landed(&res_full[w], res_phase, fail);
                     res_phase ^= 1;
+                    if (lost) {
+                        store_nan<T>(e.y, e.ldy, m0, col, g.m, g.n, 64);
+                        continue;
+                    }
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h)

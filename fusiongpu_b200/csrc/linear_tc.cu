@@ -728,15 +728,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     bool odd = false;
 #pragma unroll
                     for (int j = 0; j < 32; ++j) odd |= !(fabsf(v[j]) <= FLT_MAX);
-                    if (odd && all_ok && m0 + lane < g.m) {
-                        stage();
-                        for (int j = 0; j < 32 && c0 + j < g.n; ++j) {
-                            float* z = reinterpret_cast<float*>(hrow + ((((uint32_t)j << 2) & ~15u) ^ sw)) + (j & 3);
-                            *z = finite_or_retake<T>(g, m0 + lane, c0 + j, *z);
-                        }
+                    if (__any_sync(0xffffffffu, odd && all_ok)) {
+                        odd_seen = true;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            v[j] = *(reinterpret_cast<float*>(hrow + ((((uint32_t)j << 2) & ~15u) ^ sw)) + (j & 3));
+                        for (int j = 0; j < 32; ++j) v[j] = fabsf(v[j]) <= FLT_MAX ? v[j] : NAN;
                     }
                     if (e.bias) {
 #pragma unroll
@@ -943,7 +938,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     if (warp == 1) tc::tmem_dealloc_pair(taddr, 2 * BN);
     // Results that are not finite lie in this CTA's tiles as NaN, and are taken again here,
     // where nothing waits: each is a sum over all of k by one thread.
-    if (!PARTS || !s_odd || s_fail) return;
+    if (products == 1 || !s_odd || s_fail) return;
     if (warp >= 2 && tc::elect_one()) tc::bulk_wait();  // this block's stores have arrived
     __syncthreads();
     const Epilogue& e = g.e;

@@ -133,3 +133,49 @@ def test_residual_with_and_without_the_pre_activation(ad, shape, t):
         want = ad.linear(x, w, b, activation=act, residual=res, return_pre=True)[0]
         for _ in range(5):
             assert torch.equal(ad.linear(x, w, b, activation=act, residual=res), want)
+
+
+# ---- float32 sums that are not finite -------------------------------------------------------
+
+@pytest.mark.parametrize("shape,lead", [((9, 40, 72), 0), ((5000, 520, 264), 0), ((5000, 520, 264), 1), ((20000, 72, 1000), 0),
+                                        ((300, 20000, 520), 0)])
+def test_float32_sums_past_its_largest(ad, shape, lead):
+    """Every sum of whole tiles overflows: infinities of the right sign where all products
+    have one, the other rows and columns as without them."""
+    n, i, o = shape
+    g = _gen(i)
+    x, w = _randn(g, n, i), _randn(g, o, i, scale=i ** -0.5)
+    b, res = _randn(g, o), _randn(g, n, o + 4)[:, lead:lead + o]
+    rows, cols = torch.arange(n, device="cuda") % 3 == 0, torch.arange(o, device="cuda") % 5 == 0
+    xl, wl = x.clone(), w.clone()
+    xl[rows], wl[cols] = -2e20, 3e20
+    y, pre = ad.linear(xl, wl, b, activation="silu", residual=res, return_pre=True)
+    big = rows[:, None] & cols
+    assert (pre[big] == -math.inf).all() and torch.equal(y[big], res.expand(n, o)[big])  # silu(-inf) = 0
+    want, wpre = ad.linear(x, w, b, activation="silu", residual=res, return_pre=True)
+    small = ~rows[:, None] & ~cols
+    assert torch.equal(pre[small], wpre[small]) and torch.equal(y[small], want[small])
+    plain = ad.linear(xl, wl)
+    assert (plain[big] == -math.inf).all()
+    assert torch.equal(plain[small], ad.linear(x, w)[small])
+    xl[1::3, 0] = math.nan  # rows that are not all one sign
+    y = ad.linear(xl, wl, residual=res)
+    assert (y[big] == -math.inf).all() and y[1::3].isnan().all() and not y[rows].isnan().any()
+
+
+def test_float32_gradients_past_its_largest(ad):
+    """The same where the sums run over many rows, split and not."""
+    for n, i, o in ((3000, 264, 520), (60000, 136, 264), (30000, 2000, 2100)):
+        g = _gen(n)
+        x, w = _randn(g, n, i).abs() + 0.5, _randn(g, o, i)
+        dy = _randn(g, n, o)
+        x[:, 3], dy[:, 5] = 1e25, -1e25
+        dx, dw, db = ad.linear_backward(dy, x, w, param_grads=True)
+        assert dw[5, 3] == -math.inf
+        assert dw[5, 4:].isfinite().all() and dx.isfinite().all() and db.isfinite().all()
+        dy[n // 2, 7] = math.inf
+        dx, dw, db = ad.linear_backward(dy, x, w)
+        assert (dw[7] == math.inf).all() and db[7] == math.inf
+        assert torch.equal(dx[n // 2], torch.sign(w[7]) * math.inf)
+        keep = torch.arange(o, device="cuda") != 7
+        assert not dw[keep].isnan().any() and dw[keep][:, 8:].isfinite().all()

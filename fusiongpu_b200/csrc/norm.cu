@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(ln_backward_block(G, NCH* VEC, VEC, sizeof(T))
                                   ln_backward_per_sm(G, NCH* VEC, VEC, sizeof(T))) ln_backward_kernel(const NormArgs g) {
     constexpr int E = NCH * VEC, NT = ln_backward_block(G, E, VEC, sizeof(T)), RPB = NT / G;
     constexpr bool SMEM = G == 512, AHEAD = ln_ahead(E, VEC, sizeof(T));
-    extern __shared__ float sm[];
+    extern __shared__ __align__(16) float sm[];  // rows of sums, stored four at a time where dim is a multiple of 4
     __shared__ float s[NT / 32][2];
     const int gl = threadIdx.x % G;
     const float inv = 1.0f / (float)g.dim;

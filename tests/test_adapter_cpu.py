@@ -115,3 +115,12 @@ def test_preference_refuses():
         assert st(full[:k] + [None] + full[k + 1:]) == 1, k
     assert st([None] * 10, nq=0) == 0
     assert _status("fg_preference_loss", None, *full, None) == 1
+
+
+def test_vector_stores_to_shared_memory_are_aligned():
+    """Dynamic shared memory that kernels access 16 bytes at a time is declared so: the
+    compiler places an array of float on 4 bytes where nothing asks for more."""
+    for name in ("norm.cu", "linear_tc.cu"):
+        src = open(os.path.join(ROOT, "fusiongpu_b200", "csrc", name)).read()
+        found = re.findall(r"extern __shared__ (.*?)\w+\[\];", src)
+        assert found and all("__align__" in d for d in found), (name, found)

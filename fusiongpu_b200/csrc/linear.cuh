@@ -20,59 +20,62 @@ struct GemmShape {
     long long am, ak, bn, bk;
 };
 
-// GELU = z Phi(z).  float32 results: CUDA's erfc, which keeps the small tail.
-// Results rounded to 16 bits (FAST): Abramowitz and Stegun's approximations of erfc
-// for x >= 0, which would lose nothing that such a result shows.
-//   7.1.28: (1 + a1 x + ... + a6 x^6)^-16, error 3e-7: one special-function
-//           operation a value, which with the other issues balances the epilogue
-//           (7.1.26 takes two: 4,096 cycles of a tile's 6,144 of products)
-//   7.1.26: exp(-x^2) t (a1 + ... + a5 t^4), t = 1 / (1 + 0.3275911 x), error
-//           1.5e-7: for the derivative, which needs the exponential as well
-// GELU of two values: max(z, 0) - a Phi(-a), a = min(|z|, 30) (Phi(-30) is 0).
+// GELU = z Phi(z).  float32 results: CUDA's erfc.  Results of 16 bits (FAST): fits of our
+// own, least in their largest weighted error over 0 <= a <= 14, that keep the relative
+// accuracy of the tail Phi(-a), as such results show it.
+//   value:      max(z, 0) - a Phi(-a), a = |z|.  Phi(-a) = 2^P(a), P of degree 9: off by
+//               2^-16.7 of the value down to z = -6 (float16's last results) and 2^-12.8
+//               to -13 (bfloat16's).  One special-function operation a value, which with
+//               the other issues balances the epilogue (two are 4,096 cycles of a tile's
+//               6,144 of products)
+//   derivative: T for z < 0, 1 - T otherwise, T = Phi(-a) - a phi(a) = exp(-a^2 / 2) (M -
+//               a / sqrt(2 pi)), M(a) = t Q(t), t = 1 / (1 + 0.26 a), Q of degree 6: off by
+//               2^-22 near 0 and 2^-19 of the value from -1 to -8
+// GELU of two values; 2^24 in P's constant and back keeps Phi(-13) off exp2's underflow.
 __device__ __forceinline__ void gelu2(float& z0, float& z1) {
-    const uint64_t a = pair2(fminf(fabsf(z0), 30.0f), fminf(fabsf(z1), 30.0f));
+    const uint64_t a = pair2(fminf(fabsf(z0), 14.0f), fminf(fabsf(z1), 14.0f));
     auto both = [](float c) { return pair2(c, c); };
-    // the coefficients times 2^(-k/2): of a = sqrt(2) x
-    uint64_t p = fma2(a, both(0.0000430638f * 0.125f), both(0.0002765672f * 0.17677670f));
-    p = fma2(a, p, both(0.0001520143f * 0.25f));
-    p = fma2(a, p, both(0.0092705272f * 0.35355339f));
-    p = fma2(a, p, both(0.0422820123f * 0.5f));
-    p = fma2(a, p, both(0.0705230784f * 0.70710678f));
-    p = fma2(a, p, both(1.0f));
-    p = mul2(p, p);
-    p = mul2(p, p);
-    p = mul2(p, p);
-    p = mul2(p, p);
+    uint64_t p = fma2(a, both(-2.12431917e-09f), both(1.53519707e-07f));
+    p = fma2(a, p, both(-4.85575265e-06f));
+    p = fma2(a, p, both(8.9097688e-05f));
+    p = fma2(a, p, both(-0.00106443313f));
+    p = fma2(a, p, both(0.00886763725f));
+    p = fma2(a, p, both(-0.054471042f));
+    p = fma2(a, p, both(-0.458130389f));
+    p = fma2(a, p, both(-1.15131855f));
+    p = fma2(a, p, both(23.0000038f));
     float q0, q1, r0, r1;
     unpair2(p, q0, q1);
-    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(q0));
-    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(q1));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(q0));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(q1));
     asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r0) : "f"(z0));
     asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r1) : "f"(z1));
-    unpair2(fma2(mul2(a, both(-0.5f)), pair2(q0, q1), pair2(r0, r1)), z0, z1);
+    unpair2(fma2(mul2(a, both(-5.9604645e-08f)), pair2(q0, q1), pair2(r0, r1)), z0, z1);
 }
 
-// GELU's derivative Phi(z) + z phi(z) of two values, for results of 16 bits: z held
-// to [-30, 30] (a NaN stays), Phi(z) = 1/2 + sign(z) (1/2 - Phi(-|z|)).
+// GELU's derivative of two values; z held to [-30, 30], a NaN stays.
 __device__ __forceinline__ void gelu_grad2(float& z0, float& z1) {
-    float c0, c1, d0, d1, m0, m1, q0, q1;
+    float c0, c1, d0, d1, m0, m1, t0, t1;
     asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, 0fC1F00000;\n\tmin.NaN.f32 %0, t, 0f41F00000;\n\t}" : "=f"(c0) : "f"(z0));
     asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, 0fC1F00000;\n\tmin.NaN.f32 %0, t, 0f41F00000;\n\t}" : "=f"(c1) : "f"(z1));
-    const uint64_t z = pair2(c0, c1), a = pair2(fabsf(c0), fabsf(c1));
-    unpair2(fma2(a, pair2(0.3275911f * 0.70710678f, 0.3275911f * 0.70710678f), pair2(1.0f, 1.0f)), d0, d1);
-    unpair2(mul2(mul2(a, a), pair2(-0.5f * 1.44269504f, -0.5f * 1.44269504f)), m0, m1);
+    auto both = [](float c) { return pair2(c, c); };
+    const uint64_t a = pair2(fabsf(c0), fabsf(c1));
+    unpair2(fma2(a, both(0.26f), both(1.0f)), d0, d1);
+    unpair2(mul2(mul2(a, a), both(-0.5f * 1.44269504f)), m0, m1);
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d0));
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d1));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(m0));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(m1));
-    const uint64_t t = pair2(d0, d1), e = pair2(m0, m1);
-    uint64_t p = fma2(t, pair2(-0.5f * 1.061405429f, -0.5f * 1.061405429f), pair2(0.5f * 1.453152027f, 0.5f * 1.453152027f));
-    p = fma2(t, p, pair2(-0.5f * 1.421413741f, -0.5f * 1.421413741f));
-    p = fma2(t, p, pair2(0.5f * 0.284496736f, 0.5f * 0.284496736f));
-    p = fma2(t, p, pair2(-0.5f * 0.254829592f, -0.5f * 0.254829592f));
-    unpair2(fma2(mul2(p, t), e, pair2(0.5f, 0.5f)), q0, q1);  // 1/2 - Phi(-|z|)
-    const uint64_t phi = pair2(copysignf(q0, c0), copysignf(q1, c1));
-    unpair2(add2(fma2(mul2(z, e), pair2(0.39894228f, 0.39894228f), phi), pair2(0.5f, 0.5f)), z0, z1);
+    const uint64_t t = pair2(d0, d1);
+    uint64_t p = fma2(t, both(-0.0721131678f), both(0.225167564f));
+    p = fma2(t, p, both(-0.0996524985f));
+    p = fma2(t, p, both(0.160275265f));
+    p = fma2(t, p, both(0.0762695383f));
+    p = fma2(t, p, both(0.106471479f));
+    p = fma2(t, p, both(0.10358178f));
+    unpair2(mul2(pair2(m0, m1), fma2(a, both(-0.39894228f), mul2(p, t))), t0, t1);
+    z0 = c0 < 0.0f ? t0 : 1.0f - t0;
+    z1 = c1 < 0.0f ? t1 : 1.0f - t1;
 }
 
 template <bool FAST>

@@ -179,3 +179,25 @@ def test_float32_gradients_past_its_largest(ad):
         assert torch.equal(dx[n // 2], torch.sign(w[7]) * math.inf)
         keep = torch.arange(o, device="cuda") != 7
         assert not dw[keep].isnan().any() and dw[keep][:, 8:].isfinite().all()
+
+
+# ---- the tails of the activations ---------------------------------------------------------
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_activation_tails_keep_their_relative_accuracy(ad, act, t):
+    """Results of 16 bits: within their own rounding and 2^-15 of the value (2^-11 below
+    -6, where only bfloat16 has anything to show), not of one."""
+    z = torch.cat([torch.linspace(-13, -2, 4001), torch.linspace(-2, 6, 2001)]).cuda().to(T[t])[:, None]
+    one = torch.ones(1, 1, device="cuda", dtype=T[t])
+    zd = z.double()
+    phi = 0.5 * torch.special.erfc(-zd * math.sqrt(0.5))  # torch's ndtr is (1 + erf) / 2: 0 below -8.3
+    want = zd * phi if act == "gelu" else zd * torch.sigmoid(zd)
+    rel = torch.where(zd < -6, 2.0 ** -11, 2.0 ** -15)
+    tol = (U[t] + rel) * want.abs() + TINY[t]
+    _within(ad.linear(z, one, activation=act), want, tol, "y")
+    _within(ad.linear(z[1000:1003], one, activation=act), want[1000:1003], tol[1000:1003], "y of three rows")
+    d = ad.linear_backward(torch.ones_like(z), z, one, pre=z, activation=act, param_grads=False)[0]
+    want = phi + zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi) if act == "gelu" else _act_grad(zd, act)
+    near = 2.0 ** -19 * (zd > -2.5)  # the derivative passes through 0 there
+    _within(d, want, (U[t] + 2.0 ** -15) * want.abs() + near + TINY[t], "derivative")

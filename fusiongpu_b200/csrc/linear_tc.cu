@@ -1091,7 +1091,8 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
     if (rc) return rc;
     g.idesc = instr_desc(dtype, 2 * GT_M, BN, g.a_mn, g.b_mn);
     const long long items = (long long)g.mt * g.nt * g.split;
-    FG_REQUIRE(items <= 0x3fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
+    FG_REQUIRE(items <= 0x3fffffffll && (long long)g.split * g.m_pad <= 0x7fffffffll, "%d x %d outputs: too many tiles", g.m,
+               g.n);
     const bool direct = g.direct && g.split == 1;
     auto kernel = direct ? &gemm_pair_kernel<T, BN, true, false> : &gemm_pair_kernel<T, BN, false, false>;
     if constexpr (sizeof(T) == 2)
@@ -1142,10 +1143,13 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct) {
     for (int bn : {256, 128}) {
         if (products == 6 && bn == 128) break;
         const long long tiles = m2 * ((s.n + bn - 1) / bn);
-        for (int sp : {1, 2, 4, 8, 16, 32}) {
+        // 16-bit sums run over GT_RUN K blocks at most: parts go on past 32, and past a full
+        // GPU, until they are that short (in 64 bits: kb may be 2^25)
+        auto too_long = [&](int parts) { return products < 6 && kb > (long long)GT_RUN * parts; };
+        for (int sp = 1; sp <= 32 || too_long(sp / 2); sp *= 2) {
             if (direct && sp > 1) break;
-            if (sp > 1 && (sp > kb / 2 || (tiles * sp > sms && kb * 2 / sp <= GT_RUN))) break;
-            if (products < 6 && kb > GT_RUN * sp && sp < 32) continue;
+            if (sp > 1 && (sp > kb / 2 || (tiles * sp > sms && kb <= (long long)GT_RUN * (sp / 2)))) break;
+            if (too_long(sp)) continue;
             const size_t ws = sp > 1 ? (size_t)sp * m2 * 2 * GT_M * ((s.n + 3) / 4 * 4) * 4 : 0;
             const double epi = bn == 256 ? 2.0 : 1.0, main = (kt + sp - 1) / sp * (bn == 256 ? 0.39 : 0.34);
             const double rows = direct ? (bn == 256 ? 14.0 : 8.0) : 0.0;

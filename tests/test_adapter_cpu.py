@@ -124,3 +124,19 @@ def test_vector_stores_to_shared_memory_are_aligned():
         src = open(os.path.join(ROOT, "fusiongpu_b200", "csrc", name)).read()
         found = re.findall(r"extern __shared__ (.*?)\w+\[\];", src)
         assert found and all("__align__" in d for d in found), (name, found)
+
+
+@pytest.mark.parametrize("out_dim,in_dim", [(1536, 768), (2048, 2048), (264, 520), (64, 64)])
+def test_deep_products_are_cut_into_parts(out_dim, in_dim):
+    """dw of 16-bit layers sums over the rows: 32,768 to an accumulator at most, in up to
+    eight parts of a cluster, which need no workspace, or in parts that lie in it."""
+    deep = 512 * 64
+    rows = sorted({deep * 2 ** e + d for e in range(0, 13) for d in (-1, 0, 1, 56, 63, 64, 65, 448, 449, 960, 1000)} |
+                  {deep * m + 1 for m in range(1, 40)})
+    for r in rows:
+        p = _linear(rows=r, in_dim=in_dim, out_dim=out_dim, dtype=2)
+        n = _lib.size_query("fg_linear_backward_workspace_size", C.byref(p))
+        parts = n // ((out_dim + 255) // 256 * 256 * in_dim * 4)
+        blocks = (r + 63) // 64
+        assert blocks <= 512 * (parts if parts else 8), (r, parts)
+        assert parts <= max(32, 2 * blocks / 512), (r, parts)  # and no more than that asks for

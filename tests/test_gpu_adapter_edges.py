@@ -201,3 +201,37 @@ def test_activation_tails_keep_their_relative_accuracy(ad, act, t):
     want = phi + zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi) if act == "gelu" else _act_grad(zd, act)
     near = 2.0 ** -19 * (zd > -2.5)  # the derivative passes through 0 there
     _within(d, want, (U[t] + 2.0 ** -15) * want.abs() + near + TINY[t], "derivative")
+
+
+# ---- sums over very many rows ---------------------------------------------------------------
+
+def _ms(f, n=5):
+    f()
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    for _ in range(n):
+        f()
+    b.record()
+    b.synchronize()
+    return a.elapsed_time(b) / n
+
+
+def test_weight_gradient_of_very_many_rows(ad):
+    """262,200 rows, just past a count whose sums fit one number of parts: still cut into
+    parts, right to 64 bits and no slower than its share."""
+    n, i, o = 262200, 768, 1536
+    g = _gen(1)
+    x, dy = _randn(g, n, i, t="bf16"), _randn(g, n, o, t="bf16")
+    w = _randn(g, o, i, t="bf16")
+    _, dw, db = ad.linear_backward(dy, x, w, input_grad=False)
+    want = torch.zeros(o, i, dtype=torch.float64, device="cuda")
+    for a, b in zip(dy.split(32768), x.split(32768)):
+        want += a.double().t() @ b.double()
+    # 4,097 blocks of 64 k in parts of 512 at most: 2^-24 of the running value (about the
+    # sum's size) for each of 2,048 additions of 16 products, all cut to one side at worst
+    _within(dw, want, 2048 * 2 * E32 * want.abs().max() + U["bf16"] * want.abs(), "dw")
+    _within(db, dy.double().sum(0), (n + 16) * 2 * E32 * dy.double().abs().sum(0), "dbias")
+    k = slice(0, 262144)
+    here, there = (_ms(lambda s=s: ad.linear_backward(dy[s], x[s], w, input_grad=False)) for s in (slice(0, n), k))
+    assert here < 1.6 * there, (here, there)

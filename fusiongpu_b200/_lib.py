@@ -54,7 +54,8 @@ class GraphSearchParams(C.Structure):
 class LinearParams(C.Structure):
     _fields_ = [("rows", C.c_int64), ("in_dim", C.c_int32), ("out_dim", C.c_int32), ("dtype", C.c_int32),
                 ("activation", C.c_int32), ("x_stride", C.c_int64), ("w_stride", C.c_int64),
-                ("residual_stride", C.c_int64), ("pre_stride", C.c_int64), ("y_stride", C.c_int64)]
+                ("residual_stride", C.c_int64), ("pre_stride", C.c_int64), ("y_stride", C.c_int64),
+                ("unaligned", C.c_int32)]
 
 
 class PreferenceParams(C.Structure):

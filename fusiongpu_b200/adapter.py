@@ -109,9 +109,18 @@ def _norm_ws(n: int, d: int, device: int) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-def _linear_ws(query: str, n: int, i: int, o: int, dtype: int, act: int, ldx: int, ldw: int, ldy: int,
+def _linear_ws(query: str, n: int, i: int, o: int, dtype: int, act: int, ldx: int, ldw: int, ldy: int, off: int,
                device: int) -> int:
-    return _lib.size_query(query, C.byref(_lib.LinearParams(n, i, o, dtype, act, ldx, ldw, 0, 0, ldy)))
+    return _lib.size_query(query, C.byref(_lib.LinearParams(n, i, o, dtype, act, ldx, ldw, 0, 0, ldy, off)))
+
+
+def _off16(*pointers: int) -> int:
+    """fg_linear_operand bits of the pointers (x, w, dy) that are off 16 bytes."""
+    off = 0
+    for k, p in enumerate(pointers):
+        if p & 15:
+            off |= 1 << k
+    return off
 
 
 @_on
@@ -187,10 +196,12 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, a
         residual, ldr = _matrix(residual, "residual", x, n, o)
     y = _rows(x, n, o)
     pre = _rows(x, n, o) if return_pre else None
-    p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, ldr, 0, 0)
-    nws = _linear_ws("fg_linear_workspace_size", n, i, o, t, act, ldx, ldw, 0, dev.index)
+    px, pw = x.data_ptr(), w.data_ptr()
+    off = _off16(px, pw)
+    p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, ldr, 0, 0, off)
+    nws = _linear_ws("fg_linear_workspace_size", n, i, o, t, act, ldx, ldw, 0, off, dev.index)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    _lib.check(_lib.lib().fg_linear(C.byref(p), x.data_ptr(), w.data_ptr(), b, _ptr(residual), _ptr(pre),
+    _lib.check(_lib.lib().fg_linear(C.byref(p), px, pw, b, _ptr(residual), _ptr(pre),
                                     y.data_ptr(), _ptr(ws), nws, _stream(x)), "fg_linear")
     return (y, pre) if return_pre else y
 
@@ -217,10 +228,12 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: tor
         pre, ldp = _matrix(pre, "pre", x, n, o)
     dx = _rows(x, n, i) if input_grad else None
     dw, db = (_rows(x, o, i), torch.empty(o, dtype=x.dtype, device=dev)) if param_grads else (None, None)
-    p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, 0, ldp, lddy)
-    nws = _linear_ws("fg_linear_backward_workspace_size", n, i, o, t, act, ldx, ldw, lddy, dev.index)
+    px, pw, pdy = x.data_ptr(), w.data_ptr(), dy.data_ptr()
+    off = _off16(px, pw, pdy)
+    p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, 0, ldp, lddy, off)
+    nws = _linear_ws("fg_linear_backward_workspace_size", n, i, o, t, act, ldx, ldw, lddy, off, dev.index)
     ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    _lib.check(_lib.lib().fg_linear_backward(C.byref(p), dy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(pre),
+    _lib.check(_lib.lib().fg_linear_backward(C.byref(p), pdy, px, pw, _ptr(pre),
                                              _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nws, _stream(x)),
                "fg_linear_backward")
     return dx, dw, db

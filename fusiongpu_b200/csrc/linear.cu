@@ -141,7 +141,9 @@ struct Operand {
     long long ld, plane;  // elements
 };
 
-static bool needs_pack(int dtype, long long ld) { return dtype == FG_DTYPE_F32 || ld % 8 != 0; }
+// `off`: it does not start on a 16-byte boundary either (10,000 x 768 -> 1536 f16: 43 us
+// with x packed, 27 as it lies on one, 1,247 on the CUDA cores).
+static bool needs_pack(int dtype, long long ld, bool off) { return dtype == FG_DTYPE_F32 || ld % 8 != 0 || off; }
 static size_t pack_bytes(int dtype, long long rows, long long cols) {
     return (size_t)rows * pack_stride(cols) * 2 * (dtype == FG_DTYPE_F32 ? 3 : 1);
 }
@@ -453,6 +455,7 @@ static int linear_check(const fg_linear_params* p, Strides& t) {
     if (p->rows > LINEAR_MAX || p->in_dim > LINEAR_MAX || p->out_dim > LINEAR_MAX)
         return fail(FG_ERR_UNSUPPORTED, "a dimension above %lld", LINEAR_MAX);
     FG_REQUIRE(float_dtype(p->dtype), "unknown dtype %d", p->dtype);
+    FG_REQUIRE((p->unaligned & ~(FG_LINEAR_X | FG_LINEAR_W | FG_LINEAR_DY)) == 0, "unknown operand in unaligned %d", p->unaligned);
     FG_REQUIRE(p->activation >= FG_ACT_NONE && p->activation <= FG_ACT_SILU, "unknown activation %d", p->activation);
     t.x = p->x_stride ? p->x_stride : p->in_dim;
     t.w = p->w_stride ? p->w_stride : p->in_dim;
@@ -483,16 +486,16 @@ static size_t forward_carve(const fg_linear_params* p, const Strides& t, void* w
     Carve c(ws, bytes);
     f = ForwardWs{};
     if (p->rows <= GEMV_ROWS) return 0;
-    if (needs_pack(p->dtype, t.x)) f.x = c.take<char>(pack_bytes(p->dtype, p->rows, p->in_dim));
-    if (needs_pack(p->dtype, t.w)) f.w = c.take<char>(pack_bytes(p->dtype, p->out_dim, p->in_dim));
+    if (needs_pack(p->dtype, t.x, p->unaligned & FG_LINEAR_X)) f.x = c.take<char>(pack_bytes(p->dtype, p->rows, p->in_dim));
+    if (needs_pack(p->dtype, t.w, p->unaligned & FG_LINEAR_W)) f.w = c.take<char>(pack_bytes(p->dtype, p->out_dim, p->in_dim));
     const size_t n = tc_gemm_workspace(tc_products(p->dtype, false), forward_shape(p, t));
     if (n) f.product = c.take<char>(n);
     return c.used;
 }
 
 // x or w: as it lies, or queued to be packed.
-static Operand operand(int dtype, const void* p, long long rows, int cols, long long ld, void* room, PackArgs& a) {
-    if (!needs_pack(dtype, ld)) return {p, ld, 0};
+static Operand operand(int dtype, const void* p, long long rows, int cols, long long ld, bool off, void* room, PackArgs& a) {
+    if (!needs_pack(dtype, ld, off)) return {p, ld, 0};
     const long long stride = pack_stride(cols), plane = dtype == FG_DTYPE_F32 ? rows * stride : 0;
     a.job[a.jobs++] = PackJob{p, room, rows, ld, plane, cols};
     return {room, stride, plane};
@@ -503,8 +506,8 @@ static int linear_forward(const fg_linear_params* p, const Strides& t, const voi
                           const ForwardWs& f, cudaStream_t s) {
     if (p->rows <= GEMV_ROWS) return gemv<T>(x, w, forward_shape(p, t), e, s);
     PackArgs jobs{};
-    const Operand a = operand(p->dtype, x, p->rows, p->in_dim, t.x, f.x, jobs);
-    const Operand b = operand(p->dtype, w, p->out_dim, p->in_dim, t.w, f.w, jobs);
+    const Operand a = operand(p->dtype, x, p->rows, p->in_dim, t.x, p->unaligned & FG_LINEAR_X, f.x, jobs);
+    const Operand b = operand(p->dtype, w, p->out_dim, p->in_dim, t.w, p->unaligned & FG_LINEAR_W, f.w, jobs);
     const int rc = pack<T>(jobs, s);
     if (rc) return rc;
     return gemm<T>(a, b, GemmShape{p->rows, p->out_dim, p->in_dim, a.ld, 1, b.ld, 1}, e, f.product, s);
@@ -631,10 +634,10 @@ static size_t backward_carve(const fg_linear_params* p, const Strides& t, void* 
     Carve c(ws, bytes);
     w = BackwardWs{};
     if (few(p)) return 0;
-    if (p->activation != FG_ACT_NONE || needs_pack(p->dtype, t.y))
+    if (p->activation != FG_ACT_NONE || needs_pack(p->dtype, t.y, p->unaligned & FG_LINEAR_DY))
         w.dz = c.take<char>(pack_bytes(p->dtype, p->rows, p->out_dim) * (in_parts(p) ? 2 : 1));
-    if (needs_pack(p->dtype, t.x)) w.x = c.take<char>(pack_bytes(p->dtype, p->rows, p->in_dim));
-    if (needs_pack(p->dtype, t.w)) w.w = c.take<char>(pack_bytes(p->dtype, p->out_dim, p->in_dim));
+    if (needs_pack(p->dtype, t.x, p->unaligned & FG_LINEAR_X)) w.x = c.take<char>(pack_bytes(p->dtype, p->rows, p->in_dim));
+    if (needs_pack(p->dtype, t.w, p->unaligned & FG_LINEAR_W)) w.w = c.take<char>(pack_bytes(p->dtype, p->out_dim, p->in_dim));
     const int products = tc_products(p->dtype, in_parts(p));
     const size_t n = std::max(tc_gemm_workspace(products, dx_shape(p, t, t.y)), tc_gemm_workspace(products, dw_shape(p, t, t.y)));
     if (n) w.product = c.take<char>(n);
@@ -649,7 +652,7 @@ static int linear_backward(const fg_linear_params* p, const Strides& t, const vo
         return few_rows<T>(FewArgs{dy, x, w, pre, dx, dw, dbias, t.y, t.x, t.w, t.p, (int)p->rows, p->in_dim, p->out_dim,
                                    p->activation, 0},
                            s);
-    const bool act = p->activation != FG_ACT_NONE, store = (act || needs_pack(p->dtype, t.y)) && (dx || dw);
+    const bool act = p->activation != FG_ACT_NONE, store = (act || needs_pack(p->dtype, t.y, p->unaligned & FG_LINEAR_DY)) && (dx || dw);
     const int split = p->rows ? dz_split(p->rows, p->out_dim, sizeof(T)) : 0;
     const long long plane = p->dtype == FG_DTYPE_F32 || in_parts(p) ? p->rows * pack_stride(p->out_dim) : 0;
     int rc;
@@ -665,8 +668,8 @@ static int linear_backward(const fg_linear_params* p, const Strides& t, const vo
     const Operand dz = store ? Operand{ws.dz, pack_stride(p->out_dim), plane} : Operand{dy, t.y, 0};
     PackArgs jobs{};
     Operand xo{}, wo{};
-    if (dx && p->rows) wo = operand(p->dtype, w, p->out_dim, p->in_dim, t.w, ws.w, jobs);
-    if (dw && p->rows) xo = operand(p->dtype, x, p->rows, p->in_dim, t.x, ws.x, jobs);
+    if (dx && p->rows) wo = operand(p->dtype, w, p->out_dim, p->in_dim, t.w, p->unaligned & FG_LINEAR_W, ws.w, jobs);
+    if (dw && p->rows) xo = operand(p->dtype, x, p->rows, p->in_dim, t.x, p->unaligned & FG_LINEAR_X, ws.x, jobs);
     if ((rc = pack<T>(jobs, s))) return rc;
     Epilogue e{};
     e.ldy = p->in_dim;

@@ -498,7 +498,19 @@ typedef struct {
     int64_t residual_stride;
     int64_t pre_stride;
     int64_t y_stride;         /* y, and dy in the backward pass                 */
+    int32_t unaligned;        /* fg_linear_operand bits; 0: all on 16 bytes     */
 } fg_linear_params;
+
+/* F16 and BF16 operands whose first element does not lie on a 16-byte boundary.
+ * The workspace has room for a copy of those named here (and of those whose
+ * row stride is off 16 bytes), which the tensor cores read; one that is off and
+ * not named gives the same values from the CUDA cores, at a small part of the
+ * rate. */
+typedef enum {
+    FG_LINEAR_X = 1,
+    FG_LINEAR_W = 2,
+    FG_LINEAR_DY = 4
+} fg_linear_operand;
 
 int fg_linear_workspace_size(const fg_linear_params* params, size_t* bytes);
 int fg_linear(const fg_linear_params* params, const void* x, const void* w, const void* bias, const void* residual,

@@ -140,3 +140,20 @@ def test_deep_products_are_cut_into_parts(out_dim, in_dim):
         blocks = (r + 63) // 64
         assert blocks <= 512 * (parts if parts else 8), (r, parts)
         assert parts <= max(32, 2 * blocks / 512), (r, parts)  # and no more than that asks for
+
+
+def test_linear_room_for_operands_off_16_bytes():
+    """Their copies lie in the workspace; strides off 16 bytes and float32 are copied anyway."""
+    for name, bits in (("fg_linear_workspace_size", 3), ("fg_linear_backward_workspace_size", 7)):
+        for dtype in (1, 2):
+            size = [_lib.size_query(name, C.byref(_linear(rows=500, in_dim=72, out_dim=40, dtype=dtype, unaligned=b)))
+                    for b in range(bits + 1)]
+            for b in range(bits + 1):
+                room = sum(n for k, n in enumerate((500 * 72 * 2, 40 * 72 * 2, 500 * 40 * 2)) if b >> k & 1)
+                assert room <= size[b] - size[0] <= room + 3 * 256
+        both = [_lib.size_query(name, C.byref(_linear(rows=500, in_dim=72, out_dim=40, dtype=1, x_stride=73, w_stride=75,
+                                                      y_stride=41, unaligned=b))) for b in (0, bits)]
+        assert both[0] == both[1]
+    for bits in (8, -1):
+        p, n = _linear(unaligned=bits), C.c_size_t()
+        assert _status("fg_linear_workspace_size", C.byref(p), C.byref(n)) == 1

@@ -235,3 +235,79 @@ def test_weight_gradient_of_very_many_rows(ad):
     k = slice(0, 262144)
     here, there = (_ms(lambda s=s: ad.linear_backward(dy[s], x[s], w, input_grad=False)) for s in (slice(0, n), k))
     assert here < 1.6 * there, (here, there)
+
+
+# ---- operands that do not start on 16-byte boundaries -------------------------------------
+
+def _off(m, lead):
+    """The same matrix, rows a multiple of 16 bytes apart, `lead` elements off a boundary."""
+    n, d = m.shape
+    big = torch.zeros(n, (d + lead + 15) // 8 * 8, device="cuda", dtype=m.dtype)
+    v = big[:, lead:lead + d]
+    v.copy_(m)
+    assert v.stride(0) % 8 == 0 and v.data_ptr() % 16 == lead * m.element_size()
+    return v
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", [(9, 40, 24), (100, 264, 136), (3000, 136, 520), (5001, 768, 264)])
+def test_operands_off_16_bytes(ad, shape, t):
+    n, i, o = shape
+    g = _gen(n + o)
+    x, w = _randn(g, n, i, t=t), _randn(g, o, i, t=t, scale=i ** -0.5)
+    dy, pre = _randn(g, n, o, t=t), _randn(g, n, o, t=t)
+    for lead in (1, 4):
+        for xo, wo, do in ((_off(x, lead), w, dy), (x, _off(w, lead), dy), (_off(x, lead), _off(w, lead), _off(dy, lead))):
+            _check_linear(ad, xo, wo, None, pre, "silu", t)
+            for act in ("none", "gelu"):
+                want = ad.linear_backward(dy, x, w, pre=pre, activation=act)
+                for u, v in zip(ad.linear_backward(do, xo, wo, pre=_off(pre, lead), activation=act), want):
+                    assert torch.equal(u, v)
+                _check_backward(ad, do, xo, wo, _off(pre, lead), act, t)
+            assert torch.equal(ad.linear(xo, wo, activation="gelu"), ad.linear(x, w, activation="gelu"))
+
+
+def test_operands_off_16_bytes_stay_on_the_tensor_cores(ad):
+    """Packing costs a pass over memory, not the FP32 units' twenty to forty times."""
+    g = _gen(1)
+    x, w, dy = _randn(g, 10000, 768, t="f16"), _randn(g, 1536, 768, t="f16"), _randn(g, 10000, 1536, t="f16")
+    xo, wo, do = _off(x, 4), _off(w, 1), _off(dy, 1)
+    here, there = _ms(lambda: ad.linear(x, w)), _ms(lambda: ad.linear(xo, wo))
+    assert there < 5 * here, (here, there)
+    here, there = _ms(lambda: ad.linear_backward(dy, x, w)), _ms(lambda: ad.linear_backward(do, xo, wo))
+    assert there < 5 * here, (here, there)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_operands_off_16_bytes_that_are_not_named(ad, t):
+    """Through the C ABI without the `unaligned` bits: the same values to their rounding,
+    from the CUDA cores."""
+    import ctypes as C
+
+    from fusiongpu_b200 import _lib
+    n, i, o = 150, 136, 72
+    g = _gen(6)
+    x, w = _randn(g, n, i, t=t), _randn(g, o, i, t=t, scale=i ** -0.5)
+    dy, pre = _randn(g, n, o, t=t, scale=0.1), _randn(g, n, o, t=t)
+    xo, wo = _off(x, 1), _off(w, 1)
+    s = torch.cuda.current_stream().cuda_stream
+
+    def call(name, off, *args):
+        p = _lib.LinearParams(n, i, o, ad.DTYPES[T[t]], 2, xo.stride(0), wo.stride(0), 0, 0, 0, off)
+        ws = torch.empty(_lib.size_query(name + "_workspace_size", C.byref(p)), dtype=torch.uint8, device="cuda")
+        _lib.check(getattr(_lib.lib(), name)(C.byref(p), *args, ws.data_ptr(), ws.numel(), s), name)
+
+    ys, dxs, dws = [], [], []
+    for off in (0, 3):
+        y, dx, dw = torch.full_like(dy, math.nan), torch.full_like(x, math.nan), torch.full_like(w, math.nan)
+        call("fg_linear", off, xo.data_ptr(), wo.data_ptr(), None, None, None, y.data_ptr())
+        call("fg_linear_backward", off, dy.data_ptr(), xo.data_ptr(), wo.data_ptr(), pre.data_ptr(), dx.data_ptr(),
+             dw.data_ptr(), None)
+        ys.append(y), dxs.append(dx), dws.append(dw)
+    z = x.double() @ w.double().t()
+    zm = x.double().abs() @ w.double().abs().t()
+    dz = dy.double() * _act_grad(pre.double(), "gelu")
+    for got, want, mag, k in ((ys, _act(z, "gelu"), 1.2 * zm, i), (dxs, dz @ w.double(), dy.double().abs() @ w.double().abs(), o),
+                              (dws, dz.t() @ x.double(), dy.double().abs().t() @ x.double().abs(), n)):
+        for v in got:  # 2^-15: the activation and its derivative
+            _within(v, want, ((k + 8) * 2 * E32 + 2.0 ** -15) * mag + U[t] * want.abs() + TINY[t], str(tuple(v.shape)))

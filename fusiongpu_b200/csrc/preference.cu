@@ -7,8 +7,8 @@
 //   squared L2:     z = 2 beta u . (d+ - d-)         (the norms cancel)
 // and without a reference u = q, for L2 u = q - (d+ + d-) / 2.  The product
 // with the difference is taken as written, which loses nothing to cancellation
-// of four large scores.  loss = softplus(-z) + e z [= (1-e) softplus(-z) +
-// e softplus(z)], d loss / d z = e - sigmoid(-z), dz / dq = k beta (d+ - d-).
+// of four large scores.  loss = (1-e) softplus(-z) + e softplus(z), d loss / d z =
+// e - sigmoid(-z), dz / dq = k beta (d+ - d-).
 //
 // Bound by memory: two document rows a pair, gathered from anywhere in the base,
 // each read once -- the difference stays in registers until the loss's derivative
@@ -78,7 +78,9 @@ __device__ __forceinline__ float pref_group_sum(float v, float* s) {
 
 // Loss of margin z, and d loss / d z times k: the factor of w (d+ - d-) in the gradient.
 __device__ __forceinline__ float pair_value(const PrefArgs& g, float z) {
-    return fmaxf(-z, 0.0f) + log1pf(expf(-fabsf(z))) + (g.smooth > 0.0f ? g.smooth * z : 0.0f);
+    // (1 - e) max(-z, 0) + e max(z, 0), one of them: no infinity less another at infinite margins
+    const float line = z < 0.0f ? (g.smooth - 1.0f) * z : g.smooth > 0.0f ? g.smooth * z : 0.0f;
+    return line + log1pf(expf(-fabsf(z)));
 }
 __device__ __forceinline__ float pair_slope(const PrefArgs& g, float z) {
     const float e = expf(-fabsf(z));

@@ -311,3 +311,20 @@ def test_operands_off_16_bytes_that_are_not_named(ad, t):
                               (dws, dz.t() @ x.double(), dy.double().abs().t() @ x.double().abs(), n)):
         for v in got:  # 2^-15: the activation and its derivative
             _within(v, want, ((k + 8) * 2 * E32 + 2.0 ** -15) * mag + U[t] * want.abs() + TINY[t], str(tuple(v.shape)))
+
+
+# ---- preference loss ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_preference_infinite_margins(ad, dim):
+    """A margin of either infinity under label smoothing: the loss is infinite, not NaN."""
+    base = torch.zeros(2, dim, device="cuda")
+    base[1] = 1e38
+    q = torch.full((2, dim), 1e38, device="cuda")
+    off = torch.tensor([0, 1, 2], device="cuda")
+    pos = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    neg = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    for e, first in ((0.0, 0.0), (0.1, math.inf)):
+        losses, margins, _ = ad.preference_loss(q, base, off, pos, neg, label_smoothing=e)
+        assert margins.tolist() == [math.inf, -math.inf]
+        assert losses.tolist() == [first, math.inf]

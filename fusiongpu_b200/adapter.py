@@ -246,8 +246,8 @@ def preference_loss(queries: torch.Tensor, base: torch.Tensor, offsets: torch.Te
     """Paired preference loss of queries [nq][dim] over the documents base
     [nbase][dim] (float32, float16, bfloat16 or uint8): query i prefers document
     pos_ids[p] to neg_ids[p] for its pairs p in [offsets[i], offsets[i+1])
-    (offsets int64 [nq+1], ids int32; a pair with an id outside the base is
-    masked).  `ref`: the reference queries the log ratios are taken against
+    (offsets int64 [nq+1], ascending, ids int32; a pair with an id outside the
+    base, or that no query holds, is masked: loss and margin 0).  `ref`: the reference queries the log ratios are taken against
     (the unadapted ones).  Returns (losses [pairs], margins [pairs], dq), dq the
     gradient of sum(weights * losses), or None when grad is false."""
     q, ldq = _matrix(queries, "queries")

@@ -87,6 +87,19 @@ __device__ __forceinline__ float pair_slope(const PrefArgs& g, float z) {
     return (g.smooth - __fdividef(z >= 0.0f ? e : 1.0f, 1.0f + e)) * g.k;  // smooth - sigmoid(-z)
 }
 
+// Pairs before the first query's and after the last one's are masked ones: 0, by `nt`
+// threads of the blocks that hold these queries.
+__device__ __forceinline__ void mask_outside(const PrefArgs& g, long long i, long long p0, long long p1, int tid, int nt) {
+    auto clear = [&](long long from, long long to) {
+        for (long long p = from + tid; p < to; p += nt) {
+            g.losses[p] = 0.0f;
+            if (g.margins) g.margins[p] = 0.0f;
+        }
+    };
+    if (i == 0) clear(0, p0);
+    if (i == g.nq - 1) clear(p1, g.n_pairs);
+}
+
 // VEC elements of a query row.
 template <class T, int VEC>
 __device__ __forceinline__ void load_query(float* f, const T* p, int wide) {
@@ -126,6 +139,7 @@ __global__ void __launch_bounds__(512) preference_kernel(const PrefArgs g) {
     for (long long i = blockIdx.x; i < g.nq; i += gridDim.x) {
         const long long p0 = min(max((long long)g.offsets[i], 0ll), g.n_pairs);
         const long long p1 = min(max((long long)g.offsets[i + 1], p0), g.n_pairs);
+        mask_outside(g, i, p0, p1, threadIdx.x, blockDim.x);
         auto ids_of = [&](long long p) {
             Ids d = {-1, -1, 1.0f};
             if (p < p1) {
@@ -382,6 +396,7 @@ __global__ void __launch_bounds__((PS_WARPS + 1) * 32, NCH * 16 / sizeof(B) <= 1
     const uint64_t minus = pair2(-1.0f, -1.0f), half = pair2(-0.5f, -0.5f);
     for (long long i = i0; i < i1; ++i) {
         const long long p0 = first_of(i), p1 = max(first_of(i + 1), p0);
+        mask_outside(g, i, p0, p1, tid, PS_WARPS * 32);
         uint64_t u[E / 2], acc[E / 2];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
@@ -608,7 +623,12 @@ extern "C" int fg_preference_loss(const fg_preference_params* p, const void* que
         g.ldr = p->ref_stride ? p->ref_stride : p->dim;
         g.lddq = p->dq_stride ? p->dq_stride : p->dim;
         FG_REQUIRE(g.ldq >= p->dim && g.ldr >= p->dim && g.lddq >= p->dim, "row stride below dim");
-        if (p->nq == 0) return FG_OK;
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (p->nq == 0) {  // no query holds a pair
+            if (losses && p->n_pairs) FG_CUDA_TRY(cudaMemsetAsync(losses, 0, p->n_pairs * sizeof(float), s));
+            if (margins && p->n_pairs) FG_CUDA_TRY(cudaMemsetAsync(margins, 0, p->n_pairs * sizeof(float), s));
+            return FG_OK;
+        }
         FG_REQUIRE(queries && offsets, "null buffer");
         FG_REQUIRE(p->n_pairs == 0 || (pos_ids && neg_ids && losses), "null buffer");
         FG_REQUIRE(p->nbase == 0 || base, "null base");
@@ -630,7 +650,6 @@ extern "C" int fg_preference_loss(const fg_preference_params* p, const void* que
         g.l2 = p->metric == FG_METRIC_L2;
         g.k = (g.l2 ? 2.0f : 1.0f) * p->beta;
         g.smooth = p->label_smoothing;
-        cudaStream_t s = static_cast<cudaStream_t>(stream);
         return p->dtype == FG_DTYPE_F32   ? preference_base<float>(g, p->base_dtype, s)
                : p->dtype == FG_DTYPE_F16 ? preference_base<__half>(g, p->base_dtype, s)
                                           : preference_base<__nv_bfloat16>(g, p->base_dtype, s);

@@ -536,8 +536,9 @@ int fg_linear_backward(const fg_linear_params* params, const void* dy, const voi
  *          - label_smoothing log sigmoid(-margin),
  * and dq_i = sum over its pairs of weight * d loss / d q_i, in pair order
  * within fixed groups.  Pairs of query i are [offsets[i], offsets[i+1]);
- * offsets ascend from 0 to n_pairs (out-of-range values are clamped).  A pair
- * with an id outside [0, nbase) is masked: loss and margin 0, no gradient.
+ * offsets ascend within [0, n_pairs] (out-of-range values are clamped).  A pair
+ * with an id outside [0, nbase), or before offsets[0] or from offsets[nq] on, is
+ * masked: loss and margin 0, no gradient.
  * base: raw vectors [nbase][dim] (contiguous) of base_dtype; queries, ref, dq
  * [nq][dim] of dtype; weights [n_pairs] float or NULL for 1; losses [n_pairs],
  * margins [n_pairs] (or NULL); dq NULL: the loss alone.  dim <= 16384. */

@@ -328,3 +328,29 @@ def test_preference_infinite_margins(ad, dim):
         losses, margins, _ = ad.preference_loss(q, base, off, pos, neg, label_smoothing=e)
         assert margins.tolist() == [math.inf, -math.inf]
         assert losses.tolist() == [first, math.inf]
+
+
+def _poison(*sizes):
+    """Leaves NaN in the memory that the next allocations of these sizes get."""
+    for t in [torch.full((n,), math.nan, device="cuda") for n in sizes]:
+        del t
+
+
+@pytest.mark.parametrize("dim", [96, 512])
+def test_preference_pairs_outside_the_offsets(ad, dim):
+    """Pairs that no query holds: loss and margin 0, as for masked ones."""
+    g = _gen(dim)
+    base, q = _randn(g, 50, dim), _randn(g, 3, dim)
+    pos = torch.randint(0, 50, (1000,), generator=g, device="cuda", dtype=torch.int32)
+    neg = torch.randint(0, 50, (1000,), generator=g, device="cuda", dtype=torch.int32)
+    for off in ([300, 310, 310, 700], [0, 0, 5, 5], [990, 1000, 1000, 1000], [1000] * 4):
+        _poison(1000, 1000)
+        o = torch.tensor(off, device="cuda")
+        losses, margins, dq = ad.preference_loss(q, base, o, pos, neg, beta=0.1)
+        a, b = off[0], off[-1]
+        assert not losses[:a].any() and not losses[b:].any() and not margins[:a].any() and not margins[b:].any()
+        held = ad.preference_loss(q, base, o - a, pos[a:b], neg[a:b], beta=0.1)
+        assert torch.equal(losses[a:b], held[0]) and torch.equal(margins[a:b], held[1]) and torch.equal(dq, held[2])
+    _poison(1000, 1000)
+    losses, margins, dq = ad.preference_loss(q[:0], base, torch.zeros(1, dtype=torch.int64, device="cuda"), pos, neg)
+    assert dq.shape == (0, dim) and not losses.any() and not margins.any()

@@ -22,6 +22,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
+import inspect
 import math
 
 import torch
@@ -82,14 +83,19 @@ def _on(fn):
     """Runs the function with its `stream` argument and its first tensor's device
     current, so that results and workspace are allocated for that stream; they
     already are in the usual call."""
+    first = next(iter(inspect.signature(fn).parameters))
+
     @functools.wraps(fn)
-    def call(x, *args, stream: torch.cuda.Stream | None = None, **kw):
+    def call(*args, stream: torch.cuda.Stream | None = None, **kw):
+        x = args[0] if args else kw.get(first)
+        if x is None:
+            raise TypeError(f"{fn.__name__}() needs {first}")
         if stream is None and x.is_cuda and x.device.index == torch.cuda.current_device():
-            return fn(x, *args, **kw)
+            return fn(*args, **kw)
         if not x.is_cuda:
             raise ValueError("CUDA tensors are needed")
         with _entered(x.device, stream if stream is not None else torch.cuda.current_stream(x.device)):
-            return fn(x, *args, **kw)
+            return fn(*args, **kw)
     return call
 
 

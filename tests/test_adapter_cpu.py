@@ -157,3 +157,22 @@ def test_linear_room_for_operands_off_16_bytes():
     for bits in (8, -1):
         p, n = _linear(unaligned=bits), C.c_size_t()
         assert _status("fg_linear_workspace_size", C.byref(p), C.byref(n)) == 1
+
+
+def test_operators_take_their_tensors_by_name():
+    """Called with keywords alone, each operator gets as far as its tensors, which here are
+    not on a GPU; a missing one is named."""
+    torch = pytest.importorskip("torch")
+    from fusiongpu_b200 import adapter
+    x = torch.zeros(2, 4)
+    calls = {"layer_norm": dict(x=x), "layer_norm_backward": dict(dy=x, x=x, mean=x[:, 0], rstd=x[:, 0]),
+             "linear": dict(x=x, w=x), "linear_backward": dict(dy=x, x=x, w=x),
+             "preference_loss": dict(queries=x, base=x, offsets=x, pos_ids=x, neg_ids=x)}
+    for name, kw in calls.items():
+        with pytest.raises(ValueError, match="CUDA"):
+            getattr(adapter, name)(**kw)
+        with pytest.raises(ValueError, match="CUDA"):
+            getattr(adapter, name)(*kw.values())
+        first = next(iter(kw))
+        with pytest.raises(TypeError, match=first):
+            getattr(adapter, name)(**{k: v for k, v in kw.items() if k != first})

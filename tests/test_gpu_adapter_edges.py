@@ -354,3 +354,18 @@ def test_preference_pairs_outside_the_offsets(ad, dim):
     _poison(1000, 1000)
     losses, margins, dq = ad.preference_loss(q[:0], base, torch.zeros(1, dtype=torch.int64, device="cuda"), pos, neg)
     assert dq.shape == (0, dim) and not losses.any() and not margins.any()
+
+
+def test_operators_by_keyword(ad):
+    g = _gen(2)
+    x, w, dy = _randn(g, 40, 64), _randn(g, 24, 64), _randn(g, 40, 24)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    y, mean, rstd = ad.layer_norm(x, return_stats=True)
+    for kw in ({}, {"stream": s}):
+        for got, want in ((ad.layer_norm(x=x, **kw), y), (ad.linear(x=x, w=w, **kw), ad.linear(x, w)),
+                          (ad.linear_backward(dy=dy, x=x, w=w, **kw), ad.linear_backward(dy, x, w)),
+                          (ad.layer_norm_backward(dy=x, x=x, mean=mean, rstd=rstd, **kw), ad.layer_norm_backward(x, x, mean, rstd))):
+            s.synchronize()
+            for u, v in zip(got, want):
+                assert torch.equal(u, v)

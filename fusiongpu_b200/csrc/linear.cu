@@ -517,13 +517,18 @@ static int linear_forward(const fg_linear_params* p, const Strides& t, const voi
 //
 // The first blocks take dx, 64 columns each: w is read once, a warp taking every
 // sixteenth of its rows, and dz of 512 columns at a time is worked out in shared
-// memory; the others take dw and db, four rows of w each.  dz stays in 32 bits.  Bound by the
-// latency of w's loads, 32 rows of it under way in a block.  One row of 768 -> 1536 bf16
-// 10.5 us (with the launches of more rows 15.6), eight 21.7 (15.7, but five launches:
-// a call is 22 us, not 29); float32 9.1 and 20.7 (30 and 34).  Eight rows of 4096 ->
-// 4096 bf16 63 (32): beyond four rows of 2^22 weights the tensor cores take them.
+// memory; the others take dw and db, four rows of w each.  dz stays in 32 bits.  Bound by
+// the latency of w's loads, 32 rows of it under way in a block, and so by out_dim; the
+// launches of more rows (dz, its sums, two products) are bound by their number.  Measured,
+// theirs in brackets: bf16 768 -> 1536 one row 10.9 us (17.8), eight 22.2 (18.7, but a call
+// is 25 us, not 29); four rows of 2048 -> 2560 23.6 (27.2), of 1024 -> 4096 36 (23), of
+// 8192 -> 8192 143 (101); eight of 8192 -> 1024 35 (27).  float32, four rows: 1024 -> 4096
+// 38 (53), 64 -> 8192 70 (35).
 static bool few(const fg_linear_params* p) {
-    return p->rows >= 1 && p->rows <= GEMV_ROWS && (p->rows <= 4 || (long long)p->in_dim * p->out_dim <= 1 << 22);
+    const int wide = p->dtype == FG_DTYPE_F32 ? 2 : 1;
+    return p->rows >= 1 && (p->rows <= 4 ? p->out_dim <= 2560 * wide
+                                         : p->rows <= GEMV_ROWS && p->out_dim <= 1536 * wide &&
+                                               (long long)p->in_dim * p->out_dim <= 1 << 22);
 }
 
 constexpr int FEW_NT = 512, FEW_COLS = 64, FEW_OUT = 4;

@@ -369,3 +369,17 @@ def test_operators_by_keyword(ad):
             s.synchronize()
             for u, v in zip(got, want):
                 assert torch.equal(u, v)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 40, 2560), (4, 72, 2561), (4, 33, 5121), (8, 40, 1537), (5, 136, 3200), (8, 4000, 1100)])
+def test_gradients_of_few_rows_of_wide_layers(ad, shape, t):
+    """On both sides of the widths from which the products of more rows take them."""
+    n, i, o = shape
+    g = _gen(o)
+    x, w = _randn(g, n, i, t=t), _randn(g, o, i, t=t, scale=i ** -0.5)
+    dy, pre = _randn(g, n, o, t=t, scale=0.1), _randn(g, n, o, t=t, scale=1.5)
+    for act in ("gelu", "silu"):
+        if t != "f32":
+            _check_dz(ad, dy, x, w, pre, act, t)
+        _check_backward(ad, dy, x, w, pre, act, t)

@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(DZ_WARPS * 32, 3) dz_kernel(const DzArgs g) {
                     sum[i] += v0;
                     sum[i + 1] += v1;
                     if constexpr (TWO) {
-                        split2(v0, o[i], low[i]);
-                        split2(v1, o[i + 1], low[i + 1]);
+                        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+                        split2(v0, v1, *reinterpret_cast<T2*>(o + i), *reinterpret_cast<T2*>(low + i));
                     } else {
                         o[i] = from_f32<T>(v0);
                         o[i + 1] = from_f32<T>(v1);

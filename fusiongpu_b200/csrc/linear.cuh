@@ -160,6 +160,29 @@ __device__ __forceinline__ void split2(float v, __half& p0, __half& p1) {
     p1 = from_f32<__half>(fabsf(v) <= FLT_MAX ? fminf(fmaxf(r, -65504.0f), 65504.0f) : 0.0f);
 }
 
+// The same of two values at once, which are ordinary ones: neither cut nor past the range.
+__device__ __forceinline__ void split2(float v0, float v1, __nv_bfloat162& p0, __nv_bfloat162& p1) {
+    if (!(fabsf(v0) < 3.3e38f && fabsf(v1) < 3.3e38f)) {
+        split2(v0, p0.x, p1.x);
+        split2(v1, p0.y, p1.y);
+        return;
+    }
+    p0 = __floats2bfloat162_rn(v0, v1);
+    const float2 f = __bfloat1622float2(p0);
+    p1 = __floats2bfloat162_rn(v0 - f.x, v1 - f.y);
+}
+__device__ __forceinline__ void split2(float v0, float v1, __half2& p0, __half2& p1) {
+    if (!(fabsf(v0) < 65000.0f && fabsf(v1) < 65000.0f)) {
+        split2(v0, p0.x, p1.x);
+        split2(v1, p0.y, p1.y);
+        return;
+    }
+    constexpr float up = 1 << F16_PART_SHIFT;
+    p0 = __floats2half2_rn(v0 * 0.5f, v1 * 0.5f);
+    const float2 f = __half22float2(p0);  // up (v / 2 - f), exact but for its rounding
+    p1 = __floats2half2_rn(fmaf(v0, 0.5f * up, f.x * -up), fmaf(v1, 0.5f * up, f.y * -up));
+}
+
 // Tensor-core product (linear_tc.cu) of 16-bit operands, A possibly in the two parts
 // above, a_plane elements apart (0: as it is), or for F32 of three bf16 planes of each,
 // a_plane and b_plane apart.  tc_gemm_fits: the operands' rows start on 16-byte

@@ -15,7 +15,10 @@ Tensors are CUDA tensors of float32, float16 or bfloat16; the documents may be
 uint8.  Rows may be strided; a tensor whose last dimension is not contiguous
 is copied.  Every call takes ``stream=`` (default: the current stream of its
 first tensor's device), runs and allocates its results and workspace there, and
-does not synchronise.
+does not synchronise: as with any work on another stream, its tensors are ready
+there before the call and stay until it is done.  Results are no part of an
+autograd graph, whether or not a tensor requires gradients; the backward
+functions are called by hand.
 """
 from __future__ import annotations
 

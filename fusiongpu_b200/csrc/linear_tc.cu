@@ -1111,7 +1111,7 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
 }
 
 // The kernel, tile width and split that finish first by this estimate in
-// microseconds, fitted to runs of 1 to 7 waves of each (within 15 %): a K block takes
+// microseconds, fitted to 16-bit runs of 1 to 7 waves of each (within 15 %): a K block takes
 // a pair 0.39 (256 columns; 512 cycles of products) or 0.34 (128), a CTA of the
 // other kernel 0.43, 0.30 or 0.21 (256, 128, 64); a tile's epilogue runs behind the
 // next tile's products in the pair kernel, after them in the other.  Parts of a tile
@@ -1119,7 +1119,9 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
 // and eight CTAs run at once) or, with pairs, in the workspace and one more launch.
 // 10,000 x 768 -> 1536: forward pairs 256 26 us (128: 36; one CTA a tile: 65), dw in
 // 4 parts of pairs 29 us (2 parts 38, clusters of 4 45); 100 x 1536 -> 768: clusters
-// of 4, 64 columns, 8.3 us (unsplit 12, pairs 10).
+// of 8, 64 columns, 7.8 us (of 4 8.3, unsplit 12, pairs 10).  Float32 counts as six times
+// the K blocks; its epilogue, 32 columns at a time, is not in the estimate, which is
+// therefore far off where k is short (160,930 x 32 -> 524: 69 us, measured 615).
 struct TcPlan {
     bool pair;
     int bn, split;

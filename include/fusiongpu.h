@@ -453,7 +453,9 @@ int fg_knn(const float* base, int64_t nbase, int32_t dim, const float* queries, 
  * elements, and 0 means the row length.  No pointer or stride needs more
  * alignment than its element type (16-byte aligned rows run faster).  Rows
  * may number 0.  No call synchronises the host; results do not depend on the
- * order in which the GPU runs its blocks.  Outputs must not overlap inputs. */
+ * order in which the GPU runs its blocks.  Outputs must not overlap inputs.
+ * Waits inside the kernels are bounded; one that ran out would leave NaN in the
+ * results it concerns, the call's status being long returned. */
 
 /* Layer norm over each row: y = (x - mean) * rstd * weight + bias, rstd =
  * 1 / sqrt(variance + eps).  x, y: [rows][dim] of dtype; weight, bias [dim] of

@@ -383,3 +383,25 @@ def test_gradients_of_few_rows_of_wide_layers(ad, shape, t):
         if t != "f32":
             _check_dz(ad, dy, x, w, pre, act, t)
         _check_backward(ad, dy, x, w, pre, act, t)
+
+
+# ---- layer norm: the parameters' gradients alone ----------------------------------------------
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("dim", [40, 301, 768, 1536, 5000])
+def test_layer_norm_parameter_gradients_alone(ad, t, dim):
+    """Through the C ABI without dx, and without one of the two sums: the same bits."""
+    from fusiongpu_b200 import _lib
+    g = _gen(dim)
+    x, dy, w = _randn(g, 700, dim, t=t), _randn(g, 700, dim, t=t), _randn(g, dim)
+    _, mean, rstd = ad.layer_norm(x, w, return_stats=True)
+    _, dw, db = ad.layer_norm_backward(dy, x, mean, rstd, w)
+    ws = torch.empty(_lib.size_query("fg_layer_norm_backward_workspace_size", 700, dim), dtype=torch.uint8, device="cuda")
+    for want_w, want_b in ((1, 1), (1, 0), (0, 1)):
+        gw, gb = torch.full_like(dw, math.nan), torch.full_like(db, math.nan)
+        _lib.check(_lib.lib().fg_layer_norm_backward(
+            dy.data_ptr(), 0, x.data_ptr(), ad.DTYPES[T[t]], 700, dim, 0, w.data_ptr(), 0, mean.data_ptr(), rstd.data_ptr(),
+            None, 0, gw.data_ptr() if want_w else None, gb.data_ptr() if want_b else None, ws.data_ptr(), ws.numel(),
+            torch.cuda.current_stream().cuda_stream), "fg_layer_norm_backward")
+        assert torch.equal(gw, dw) if want_w else gw.isnan().all()
+        assert torch.equal(gb, db) if want_b else gb.isnan().all()

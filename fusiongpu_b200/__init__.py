@@ -18,8 +18,8 @@ def __getattr__(name):
                 "encode_residuals_to_pq_gpu", "sort_by_list", "recall_at"):
         from . import index
         return getattr(index, name)
-    if name in ("QueryAdapter", "layer_norm", "layer_norm_backward", "linear", "linear_backward",
-                "preference_loss"):
+    if name in ("QueryAdapter", "layer_norm", "layer_norm_backward", "linear", "linear_backward", "gated_linear",
+                "gated_linear_backward", "quantize_rows", "linear_int8", "preference_loss"):
         from . import adapter
         return getattr(adapter, name)
     raise AttributeError(name)

@@ -117,6 +117,13 @@ _SIGS = {
     "fg_linear": [C.POINTER(LinearParams), _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
     "fg_linear_backward_workspace_size": [C.POINTER(LinearParams), C.POINTER(_SZ)],
     "fg_linear_backward": [C.POINTER(LinearParams), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "fg_gated_linear_workspace_size": [C.POINTER(LinearParams), C.POINTER(_SZ)],
+    "fg_gated_linear": [C.POINTER(LinearParams), _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "fg_gated_linear_backward_workspace_size": [C.POINTER(LinearParams), C.POINTER(_SZ)],
+    "fg_gated_linear_backward": [C.POINTER(LinearParams), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "fg_quantize_rows": [_P, _I32, _I64, _I32, _I64, _P, _I64, _P, _P],
+    "fg_linear_int8_workspace_size": [C.POINTER(LinearParams), C.POINTER(_SZ)],
+    "fg_linear_int8": [C.POINTER(LinearParams), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
     "fg_preference_loss": [C.POINTER(PreferenceParams), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
 }
 

@@ -249,6 +249,129 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: tor
 
 
 @_on
+def gated_linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "silu",
+                 return_pre: bool = False):
+    """activation(z) * p for [z p] = x w^T + bias, x [rows][in], w [2 out][in] (the
+    gates' rows, then their partners'), bias [2 out]; with return_pre also [z p]
+    [rows][2 out], which :func:`gated_linear_backward` takes."""
+    act = _activation(activation)
+    x, ldx = _matrix(x, "x")
+    n, i = x.shape
+    w, ldw = _matrix(w, "w", x, -1, i)
+    if w.shape[0] % 2:
+        raise ValueError(f"w must have an even number of rows, not {w.shape[0]}")
+    o = w.shape[0] // 2
+    t, dev = DTYPES[x.dtype], x.device
+    b = _vector(bias, "bias", 2 * o, x.dtype, dev)
+    y = _rows(x, n, o)
+    pre = _rows(x, n, 2 * o) if return_pre else None
+    px, pw = x.data_ptr(), w.data_ptr()
+    off = _off16(px, pw)
+    p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, 0, 0, 0, off)
+    nws = _linear_ws("fg_gated_linear_workspace_size", n, i, o, t, act, ldx, ldw, 0, off, dev.index)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    _lib.check(_lib.lib().fg_gated_linear(C.byref(p), px, pw, b, _ptr(pre), y.data_ptr(), _ptr(ws), nws, _stream(x)),
+               "fg_gated_linear")
+    return (y, pre) if return_pre else y
+
+
+@_on
+def gated_linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: torch.Tensor,
+                          activation: str = "silu", input_grad: bool = True, param_grads: bool = True):
+    """Gradients (dx, dw, dbias) of :func:`gated_linear`, of x's type; `pre` from the
+    forward pass.  What input_grad and param_grads leave out is None."""
+    act = _activation(activation)
+    x, ldx = _matrix(x, "x")
+    n, i = x.shape
+    w, ldw = _matrix(w, "w", x, -1, i)
+    if w.shape[0] % 2:
+        raise ValueError(f"w must have an even number of rows, not {w.shape[0]}")
+    o = w.shape[0] // 2
+    t, dev = DTYPES[x.dtype], x.device
+    dy, lddy = _matrix(dy, "dy", x, n, o)
+    if pre is None:
+        raise ValueError("pre of the forward pass is needed")
+    pre, ldp = _matrix(pre, "pre", x, n, 2 * o)
+    dx = _rows(x, n, i) if input_grad else None
+    dw, db = (_rows(x, 2 * o, i), torch.empty(2 * o, dtype=x.dtype, device=dev)) if param_grads else (None, None)
+    px, pw = x.data_ptr(), w.data_ptr()
+    off = _off16(px, pw)
+    p = _lib.LinearParams(n, i, o, t, act, ldx, ldw, 0, ldp, lddy, off)
+    nws = _linear_ws("fg_gated_linear_backward_workspace_size", n, i, o, t, act, ldx, ldw, lddy, off, dev.index)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    _lib.check(_lib.lib().fg_gated_linear_backward(C.byref(p), dy.data_ptr(), px, pw, pre.data_ptr(), _ptr(dx), _ptr(dw),
+                                                   _ptr(db), _ptr(ws), nws, _stream(x)), "fg_gated_linear_backward")
+    return dx, dw, db
+
+
+def _codes(t: torch.Tensor, name: str, device=None, cols: int = -1):
+    """The same as _matrix for codes of 8 bits."""
+    if not t.is_cuda or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D CUDA tensor")
+    if t.dtype != torch.int8 or (device is not None and t.device != device):
+        raise TypeError(f"{name} must be int8{'' if device is None else f' on {device}'}, not {t.dtype} on {t.device}")
+    n, d = t.shape
+    if cols >= 0 and d != cols:
+        raise ValueError(f"{name} has {d} columns, not {cols}")
+    s0, s1 = t.stride()
+    if (s1 != 1 and d > 1) or (s0 < d and n > 1):
+        t = t.contiguous()
+        s0 = d
+    return t, s0 if n > 1 else 0
+
+
+@_on
+def quantize_rows(x: torch.Tensor):
+    """Codes of 8 bits and their scales for x's rows: scale = max |x| / 127 and
+    q = 127 x / max |x|, rounded to nearest, ties to even.  Returns (q int8
+    [rows][dim], its rows on 16-byte boundaries, so strided where dim is no multiple
+    of 16; scale float32 [rows]).  A row that holds an infinity or a NaN has scale
+    NaN."""
+    x, ld = _matrix(x, "x")
+    n, d = x.shape
+    dev = x.device
+    ldq = (d + 15) // 16 * 16
+    q = torch.empty_strided((n, d), (ldq, 1), dtype=torch.int8, device=dev)
+    scale = torch.empty(n, dtype=torch.float32, device=dev)
+    _lib.check(_lib.lib().fg_quantize_rows(x.data_ptr(), DTYPES[x.dtype], n, d, ld, q.data_ptr(), ldq, scale.data_ptr(),
+                                           _stream(x)), "fg_quantize_rows")
+    return q, scale
+
+
+@_on
+def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                bias: torch.Tensor | None = None, activation: str = "none", residual: torch.Tensor | None = None,
+                dtype: torch.dtype = torch.float32):
+    """activation(x_scale w_scale (x w^T) + bias) + residual for codes x [rows][in]
+    and w [out][in] with a float32 scale per row, as :func:`quantize_rows` gives
+    them; the sums are exact.  bias, residual and the result are of `dtype`."""
+    act = _activation(activation)
+    if dtype not in DTYPES:
+        raise TypeError(f"dtype must be float32, float16 or bfloat16, not {dtype}")
+    x, ldx = _codes(x, "x")
+    n, i = x.shape
+    dev = x.device
+    w, ldw = _codes(w, "w", dev, i)
+    o = w.shape[0]
+    if x_scale is None or w_scale is None:
+        raise ValueError("x_scale and w_scale are needed")
+    xs, wsc = _vector(x_scale, "x_scale", n, torch.float32, dev), _vector(w_scale, "w_scale", o, torch.float32, dev)
+    b = _vector(bias, "bias", o, dtype, dev)
+    y = torch.empty_strided((n, o), (o, 1), dtype=dtype, device=dev)
+    ldr = 0
+    if residual is not None:
+        residual, ldr = _matrix(residual, "residual", y, n, o)
+    px, pw = x.data_ptr(), w.data_ptr()
+    off = _off16(px, pw)
+    p = _lib.LinearParams(n, i, o, DTYPES[dtype], act, ldx, ldw, ldr, 0, 0, off)
+    nws = _linear_ws("fg_linear_int8_workspace_size", n, i, o, DTYPES[dtype], act, ldx, ldw, 0, off, dev.index)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    _lib.check(_lib.lib().fg_linear_int8(C.byref(p), px, xs, pw, wsc, b, _ptr(residual), y.data_ptr(), _ptr(ws), nws,
+                                         _stream(x)), "fg_linear_int8")
+    return y
+
+
+@_on
 def preference_loss(queries: torch.Tensor, base: torch.Tensor, offsets: torch.Tensor, pos_ids: torch.Tensor,
                     neg_ids: torch.Tensor, ref: torch.Tensor | None = None, weights: torch.Tensor | None = None,
                     beta: float = 1.0, label_smoothing: float = 0.0, metric: str = "ip", grad: bool = True):

@@ -73,28 +73,6 @@ static int simt_gemm_check(const GemmShape& g, long long* tiles) {
 // of what the ones before leave (a value past bf16's range is cut instead, an infinity
 // or NaN has zeros behind it; bf16's last place is 2^-133, which values below 2^-109
 // feel).  One pass over memory, eight columns a thread.
-struct PackJob {
-    const void* in;
-    void* out;
-    long long rows, ld, plane;
-    int cols;
-};
-struct PackArgs {
-    PackJob job[2];
-    int jobs;
-};
-
-__host__ __device__ inline long long pack_stride(long long cols) { return (cols + 7) / 8 * 8; }
-
-__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
-    p[0] = from_f32<__nv_bfloat16>(x);
-    const bool finite = fabsf(x) <= FLT_MAX;
-    if (finite && !(fabsf(to_f32(p[0])) <= FLT_MAX)) p[0] = from_f32<__nv_bfloat16>(__uint_as_float(__float_as_uint(x) & 0xffff0000u));
-    const float r = x - to_f32(p[0]);
-    p[1] = from_f32<__nv_bfloat16>(finite ? r : 0.0f);
-    p[2] = from_f32<__nv_bfloat16>(finite ? r - to_f32(p[1]) : 0.0f);
-}
-
 template <class T>
 __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
     long long i = blockIdx.x * 256ll + threadIdx.x;
@@ -136,19 +114,6 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
     }
 }
 
-// An operand on its way to a product: as it lies, or packed into the workspace.
-struct Operand {
-    const void* p;
-    long long ld, plane;  // elements
-};
-
-// `off`: it does not start on a 16-byte boundary either (10,000 x 768 -> 1536 f16: 43 us
-// with x packed, 27 as it lies on one, 1,247 on the CUDA cores).
-static bool needs_pack(int dtype, long long ld, bool off) { return dtype == FG_DTYPE_F32 || ld % 8 != 0 || off; }
-static size_t pack_bytes(int dtype, long long rows, long long cols) {
-    return (size_t)rows * pack_stride(cols) * 2 * (dtype == FG_DTYPE_F32 ? 3 : 1);
-}
-
 template <class T>
 static int pack(const PackArgs& a, cudaStream_t s) {
     long long n = 0;
@@ -167,16 +132,18 @@ static int pack(const PackArgs& a, cudaStream_t s) {
 // for at once (8 rows of 1536 -> 768 f16: 4.5 us; with a branch on the row between
 // them 11.3), and for one row of a large matrix by its bytes: 768 -> 1536 f16 2.3 us,
 // 4096 -> 4096 5.8 us (5.8 TB/s, of which L2 holds a part).
-template <class T, int R, int C>
+//
+// GATED: the two columns are a gate's and its partner's, `up` rows of w apart.
+template <class T, int R, int C, bool GATED>
 __global__ void __launch_bounds__(128) gemv_kernel(const T* __restrict__ x, const T* __restrict__ w, const GemmShape g,
-                                                   int wide, const Epilogue e) {
+                                                   int wide, const Epilogue e, int up) {
     constexpr int VEC = 16 / sizeof(T);
     const int lane = threadIdx.x & 31;
-    const long long n = (blockIdx.x * 4ll + (threadIdx.x >> 5)) * C;
+    const long long n = (blockIdx.x * 4ll + (threadIdx.x >> 5)) * (GATED ? 1 : C);
     if (n >= g.n) return;
     const T *wr[C], *xr[R];  // rows and columns past the last are the last again: no branch keeps loads apart
 #pragma unroll
-    for (int c = 0; c < C; ++c) wr[c] = w + min(n + c, g.n - 1) * g.bn;
+    for (int c = 0; c < C; ++c) wr[c] = w + (GATED ? n + (c ? up : 0) : min(n + c, g.n - 1)) * g.bn;
 #pragma unroll
     for (int r = 0; r < R; ++r) xr[r] = x + min((long long)r, g.m - 1) * g.am;
     float acc[R * C];
@@ -230,17 +197,28 @@ __global__ void __launch_bounds__(128) gemv_kernel(const T* __restrict__ x, cons
         }
     }
     const int row = held / C;
+    if constexpr (GATED) {  // the partner's sum is in the lane of the last halving
+        const float p = __shfl_xor_sync(0xffffffffu, acc[0], 16 / R);
+        if (lane % (32 / (R * C)) == 0 && held % C == 0 && row < g.m) gated_store<T>(e, up, row, n, acc[0], p);
+        return;
+    }
     const long long col = n + held % C;
     if (lane % (32 / (R * C)) == 0 && row < g.m && col < g.n) epilogue_store<T>(e, row, col, acc[0]);
 }
 
-constexpr int GEMV_ROWS = 8;
-
 template <class T, int R, int C>
 static int gemv_columns(const void* x, const void* w, const GemmShape& g, const Epilogue& e, cudaStream_t s) {
     auto lies = [&](const void* p, long long ld) { return aligned(p, 16) && ld * (int)sizeof(T) % 16 == 0; };
-    gemv_kernel<T, R, C><<<(unsigned)((g.n + 4 * C - 1) / (4 * C)), 128, 0, s>>>(
-        static_cast<const T*>(x), static_cast<const T*>(w), g, lies(x, g.am) && lies(w, g.bn), e);
+    gemv_kernel<T, R, C, false><<<(unsigned)((g.n + 4 * C - 1) / (4 * C)), 128, 0, s>>>(
+        static_cast<const T*>(x), static_cast<const T*>(w), g, lies(x, g.am) && lies(w, g.bn), e, 0);
+    return check_launch("gemv_kernel");
+}
+
+template <class T, int R>
+static int gemv_gated(const void* x, const void* w, const GemmShape& g, const Epilogue& e, int up, cudaStream_t s) {
+    auto lies = [&](const void* p, long long ld) { return aligned(p, 16) && ld * (int)sizeof(T) % 16 == 0; };
+    gemv_kernel<T, R, 2, true><<<(unsigned)((up + 3) / 4), 128, 0, s>>>(static_cast<const T*>(x), static_cast<const T*>(w), g,
+                                                                        lies(x, g.am) && lies(w, g.bn), e, up);
     return check_launch("gemv_kernel");
 }
 
@@ -444,13 +422,7 @@ static int launch_dz(DzArgs g, int split, cudaStream_t s) {
     return check_launch("dz_kernel");
 }
 
-struct Strides {
-    long long x, w, r, p, y;
-};
-
-constexpr long long LINEAR_MAX = (1ll << 31) - 1024;  // tensor coordinates are 32 bits
-
-static int linear_check(const fg_linear_params* p, Strides& t) {
+int linear_check(const fg_linear_params* p, Strides& t) {
     FG_REQUIRE(p, "null params");
     FG_REQUIRE(p->rows >= 0 && p->in_dim >= 1 && p->out_dim >= 1, "bad linear shape");
     if (p->rows > LINEAR_MAX || p->in_dim > LINEAR_MAX || p->out_dim > LINEAR_MAX)
@@ -495,7 +467,7 @@ static size_t forward_carve(const fg_linear_params* p, const Strides& t, void* w
 }
 
 // x or w: as it lies, or queued to be packed.
-static Operand operand(int dtype, const void* p, long long rows, int cols, long long ld, bool off, void* room, PackArgs& a) {
+Operand operand(int dtype, const void* p, long long rows, int cols, long long ld, bool off, void* room, PackArgs& a) {
     if (!needs_pack(dtype, ld, off)) return {p, ld, 0};
     const long long stride = pack_stride(cols), plane = dtype == FG_DTYPE_F32 ? rows * stride : 0;
     a.job[a.jobs++] = PackJob{p, room, rows, ld, plane, cols};
@@ -525,7 +497,7 @@ static int linear_forward(const fg_linear_params* p, const Strides& t, const voi
 // is 25 us, not 29); four rows of 2048 -> 2560 23.6 (27.2), of 1024 -> 4096 36 (23), of
 // 8192 -> 8192 143 (101); eight of 8192 -> 1024 35 (27).  float32, four rows: 1024 -> 4096
 // 38 (53), 64 -> 8192 70 (35).
-static bool few(const fg_linear_params* p) {
+bool few(const fg_linear_params* p) {
     const int wide = p->dtype == FG_DTYPE_F32 ? 2 : 1;
     return p->rows >= 1 && (p->rows <= 4 ? p->out_dim <= 2560 * wide
                                          : p->rows <= GEMV_ROWS && p->out_dim <= 1536 * wide &&
@@ -534,15 +506,14 @@ static bool few(const fg_linear_params* p) {
 
 constexpr int FEW_NT = 512, FEW_COLS = 64, FEW_OUT = 4;
 
-struct FewArgs {
-    const void *dy, *x, *w, *pre;
-    void *dx, *dw, *db;
-    long long lddy, ldx, ldw, ldp;
-    int rows, in_dim, out_dim, act, dx_blocks;
-};
-
 template <class T>
 __device__ __forceinline__ float dz_of(const FewArgs& g, int r, int o) {
+    if (g.up) {
+        const int j = o < g.up ? o : o - g.up;
+        const T* pre = static_cast<const T*>(g.pre) + r * g.ldp;
+        const float d = to_f32(static_cast<const T*>(g.dy)[r * g.lddy + j]), z = to_f32(pre[j]);
+        return o < g.up ? d * to_f32(pre[g.up + j]) * activate_grad<false>(z, g.act) : d * activate<false>(z, g.act);
+    }
     const float d = to_f32(static_cast<const T*>(g.dy)[r * g.lddy + o]);
     return g.act == FG_ACT_NONE ? d : d * activate_grad<false>(to_f32(static_cast<const T*>(g.pre)[r * g.ldp + o]), g.act);
 }
@@ -656,7 +627,7 @@ static int linear_backward(const fg_linear_params* p, const Strides& t, const vo
                            const void* pre, void* dx, void* dw, void* dbias, const BackwardWs& ws, cudaStream_t s) {
     if (few(p))
         return few_rows<T>(FewArgs{dy, x, w, pre, dx, dw, dbias, t.y, t.x, t.w, t.p, (int)p->rows, p->in_dim, p->out_dim,
-                                   p->activation, 0},
+                                   p->activation, 0, 0},
                            s);
     const bool act = p->activation != FG_ACT_NONE, store = (act || needs_pack(p->dtype, t.y, p->unaligned & FG_LINEAR_DY)) && (dx || dw);
     const int split = p->rows ? dz_split(p->rows, p->out_dim, sizeof(T)) : 0;
@@ -691,6 +662,48 @@ static int linear_backward(const fg_linear_params* p, const Strides& t, const vo
     }
     return FG_OK;
 }
+
+// ---- for the gated layer ---------------------------------------------------------
+
+#define FG_TYPED(call)                                  \
+    (dtype == FG_DTYPE_F32   ? call(float)              \
+     : dtype == FG_DTYPE_F16 ? call(__half)             \
+                             : call(__nv_bfloat16))
+
+int linear_pack(int dtype, const PackArgs& a, cudaStream_t s) {
+#define FG_CALL(T) pack<T>(a, s)
+    return FG_TYPED(FG_CALL);
+#undef FG_CALL
+}
+
+int linear_gemm(int dtype, const Operand& a, const Operand& b, const GemmShape& g, const Epilogue& e, void* ws, cudaStream_t s) {
+#define FG_CALL(T) gemm<T>(a, b, g, e, ws, s)
+    return FG_TYPED(FG_CALL);
+#undef FG_CALL
+}
+
+int linear_gemv_gated(int dtype, const void* x, const void* w, const GemmShape& g, const Epilogue& e, int up, cudaStream_t s) {
+#define FG_CALL(T)                                        \
+    (g.m == 1   ? gemv_gated<T, 1>(x, w, g, e, up, s)     \
+     : g.m == 2 ? gemv_gated<T, 2>(x, w, g, e, up, s)     \
+     : g.m <= 4 ? gemv_gated<T, 4>(x, w, g, e, up, s)     \
+                : gemv_gated<T, GEMV_ROWS>(x, w, g, e, up, s))
+    return FG_TYPED(FG_CALL);
+#undef FG_CALL
+}
+
+int linear_few_rows(int dtype, const FewArgs& g, cudaStream_t s) {
+#define FG_CALL(T) few_rows<T>(g, s)
+    return FG_TYPED(FG_CALL);
+#undef FG_CALL
+}
+
+int linear_column_sums(int dtype, const float* part, int parts, int dim, void* out, cudaStream_t s) {
+#define FG_CALL(T) (dz_reduce_kernel<T><<<(dim + 31) / 32, 1024, 0, s>>>(part, parts, dim, static_cast<T*>(out)), check_launch("dz_reduce_kernel"))
+    return FG_TYPED(FG_CALL);
+#undef FG_CALL
+}
+#undef FG_TYPED
 
 }  // namespace fg
 

@@ -133,6 +133,20 @@ __device__ __forceinline__ void epilogue_store(const Epilogue& e, long long m, l
     static_cast<T*>(e.y)[m * e.ldy + n] = from_f32<T>(y);
 }
 
+// Gated layer: a gate's z and its partner's, columns n and up + n.
+template <class T>
+__device__ __forceinline__ void gated_store(const Epilogue& e, int up, long long m, long long n, float z, float p) {
+    if (e.bias) {
+        z += to_f32(static_cast<const T*>(e.bias)[n]);
+        p += to_f32(static_cast<const T*>(e.bias)[up + n]);
+    }
+    if (e.pre) {
+        static_cast<T*>(e.pre)[m * e.ldp + n] = from_f32<T>(z);
+        static_cast<T*>(e.pre)[m * e.ldp + up + n] = from_f32<T>(p);
+    }
+    static_cast<T*>(e.y)[m * e.ldy + n] = from_f32<T>(activate<sizeof(T) == 2>(z, e.act) * p);
+}
+
 // A 32-bit value as two of 16 bits, for an operand that is worked out in 32: the
 // rounding to the type, and the rounding of what that leaves.  bf16: v = p0 + p1, to 16
 // bits of the significand.  f16: v = 2 (p0 + 2^-12 p1), to 22 bits, or 2^-36 where that is
@@ -191,7 +205,78 @@ __device__ __forceinline__ void split2(float v0, float v1, __half2& p0, __half2&
 inline int tc_products(int dtype, bool parts) { return dtype == FG_DTYPE_F32 ? 6 : parts ? 2 : 1; }
 bool tc_gemm_fits(const void* a, const void* b, const GemmShape& g);
 size_t tc_gemm_workspace(int products, const GemmShape& g);
+// Gated layer: g.n = 2 up rows of B, up outputs.  Operands as tc_gemm takes them, B K-major,
+// both of at most 32,768 k.
+int tc_gated(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& g,
+             const Epilogue& e, cudaStream_t s);
+// Codes of 8 bits, both K-major, rows on 16-byte boundaries, at most 131,071 k.  dtype: of the
+// epilogue's matrices.
+int tc_int8(int dtype, const void* a, const float* xs, const void* b, const float* ws, const GemmShape& g, const Epilogue& e,
+            cudaStream_t s);
 int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& g,
             const Epilogue& e, void* ws, cudaStream_t s);
+
+// ---- the layer's host side (linear.cu), shared with the gated layer (gated.cu) --------
+
+struct PackJob {
+    const void* in;
+    void* out;
+    long long rows, ld, plane;
+    int cols;
+};
+struct PackArgs {
+    PackJob job[2];
+    int jobs;
+};
+
+__host__ __device__ inline long long pack_stride(long long cols) { return (cols + 7) / 8 * 8; }
+
+__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
+    p[0] = from_f32<__nv_bfloat16>(x);
+    const bool finite = fabsf(x) <= FLT_MAX;
+    if (finite && !(fabsf(to_f32(p[0])) <= FLT_MAX)) p[0] = from_f32<__nv_bfloat16>(__uint_as_float(__float_as_uint(x) & 0xffff0000u));
+    const float r = x - to_f32(p[0]);
+    p[1] = from_f32<__nv_bfloat16>(finite ? r : 0.0f);
+    p[2] = from_f32<__nv_bfloat16>(finite ? r - to_f32(p[1]) : 0.0f);
+}
+
+// An operand on its way to a product: as it lies, or packed into the workspace.
+struct Operand {
+    const void* p;
+    long long ld, plane;  // elements
+};
+
+// `off`: it does not start on a 16-byte boundary either (10,000 x 768 -> 1536 f16: 43 us
+// with x packed, 27 as it lies on one, 1,247 on the CUDA cores).
+inline bool needs_pack(int dtype, long long ld, bool off) { return dtype == FG_DTYPE_F32 || ld % 8 != 0 || off; }
+inline size_t pack_bytes(int dtype, long long rows, long long cols) {
+    return (size_t)rows * pack_stride(cols) * 2 * (dtype == FG_DTYPE_F32 ? 3 : 1);
+}
+
+Operand operand(int dtype, const void* p, long long rows, int cols, long long ld, bool off, void* room, PackArgs& a);
+
+constexpr int GEMV_ROWS = 8;  // rows that go without tensor cores
+
+struct FewArgs {
+    const void *dy, *x, *w, *pre;
+    void *dx, *dw, *db;
+    long long lddy, ldx, ldw, ldp;
+    int rows, in_dim, out_dim, act, dx_blocks;
+    int up;  // gated layer: out_dim / 2, pre [rows][out_dim], dy [rows][up]; else 0
+};
+
+struct Strides {
+    long long x, w, r, p, y;
+};
+
+constexpr long long LINEAR_MAX = (1ll << 31) - 1024;  // tensor coordinates are 32 bits
+
+int linear_check(const fg_linear_params* p, Strides& t);
+bool few(const fg_linear_params* p);
+int linear_pack(int dtype, const PackArgs& a, cudaStream_t s);
+int linear_gemm(int dtype, const Operand& a, const Operand& b, const GemmShape& g, const Epilogue& e, void* ws, cudaStream_t s);
+int linear_gemv_gated(int dtype, const void* x, const void* w, const GemmShape& g, const Epilogue& e, int up, cudaStream_t s);
+int linear_few_rows(int dtype, const FewArgs& g, cudaStream_t s);
+int linear_column_sums(int dtype, const float* part, int parts, int dim, void* out, cudaStream_t s);
 
 }  // namespace fg

@@ -25,6 +25,14 @@ constexpr int GT_RING = 192 * 1024;
 constexpr int GT_RUN = 512;        // K blocks that a 16-bit product's accumulator sums at most
 constexpr int GP_CHUNK = 8;        // and a float32 one
 
+// What the kernels multiply and what becomes of the sums.
+enum {
+    TC_WHOLE,  // A and B as they are
+    TC_PARTS,  // A in two parts
+    TC_GATED,  // B's rows j and up + j together: act(z_j) z_(up + j)
+    TC_INT8    // codes of 8 bits, 32-bit integer sums, times the scales of their row and column
+};
+
 struct TcArgs {
     int kt, mt, nt;     // K blocks, row tiles, column tiles
     int m, n;
@@ -39,6 +47,8 @@ struct TcArgs {
     long long a_plane, b_plane;
     uint32_t idesc;
     Epilogue e;
+    int up;             // TC_GATED: rows of B from a gate's to its partner's
+    const float *xs, *ws;  // TC_INT8: scales of A's and B's rows
 };
 
 // Planes of the i-th plane product.
@@ -98,6 +108,23 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t a, uint32_t rank) {
     return v;
 }
 
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t a, uint32_t rank) {
+    uint32_t v;
+    asm volatile(
+        "{\n\t.reg .b32 p;\n\t"
+        "mapa.shared::cluster.u32 p, %1, %2;\n\t"
+        "ld.shared::cluster.u32 %0, [p];\n\t}\n"
+        : "=r"(v)
+        : "r"(a), "r"(rank)
+        : "memory");
+    return v;
+}
+
+// An integer sum, its bits in a float's place, times its row's and column's scales.
+__device__ __forceinline__ float dequantised(float sum, float xs, float ws) {
+    return (float)__float_as_int(sum) * (xs * ws);
+}
+
 template <class T>
 __device__ __forceinline__ float4 load4(const T* p) {
     T v[4];
@@ -149,35 +176,41 @@ __device__ __forceinline__ void store4<float>(float* p, float4 f) {
 // operand ring was); then each CTA adds one slice of the columns over the cluster,
 // from its own rank onwards -- were all to begin with rank 0, they would queue for its
 // shared memory: 100 x 1536 -> 768 bf16 8.2 us, so 7.6 -- and finishes it.
-template <class T, int BN, bool PARTS>
+//
+// TC_GATED: half of B's rows are gates, the other half their partners, so a tile has BN /
+// 2 outputs.  TC_INT8: integer sums, exact in any order.
+template <class T, int BN, int MODE>
 __global__ void __launch_bounds__(GT_NT, 1)
     gemm_split_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const __grid_constant__ TcArgs g) {
     using Ring = RingOf<BN>;
+    constexpr bool PARTS = MODE == TC_PARTS, PLANES = sizeof(T) == 4 && MODE != TC_INT8;
+    constexpr int BO = MODE == TC_GATED ? BN / 2 : BN;      // outputs of a tile's row
+    constexpr int KB = MODE == TC_INT8 ? 2 * GT_K : GT_K;   // elements of a K block
     constexpr int LDP = BN + 4;  // partial row: 4 floats of padding keep 16-byte stores off each other's banks
     static_assert(GT_M * LDP * 4 <= Ring::N * Ring::STAGE, "the partial tile fits the ring");
     extern __shared__ __align__(1024) unsigned char dsmem[];
     __shared__ __align__(8) uint64_t full[Ring::N], empty[Ring::N], acc_full;
     __shared__ uint32_t tmem_slot;
-    __shared__ int s_fail;
+    __shared__ int s_fail, s_lost;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     unsigned char* ring = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
     float* part = reinterpret_cast<float*>(ring);
     const int S = g.split, rank = S > 1 ? (int)cluster_rank() : 0;
     const int tile = (int)(blockIdx.x / (unsigned)S);
-    const int m0 = tile / g.nt * GT_M, n0 = tile % g.nt * BN;
+    const int m0 = tile / g.nt * GT_M, n0 = tile % g.nt * BO;
     const int kb0 = (int)((long long)g.kt * rank / S), kb1 = (int)((long long)g.kt * (rank + 1) / S);
     // accumulators: one, or for float32 as many as TMEM holds, each for GP_CHUNK K blocks
-    constexpr int NA = sizeof(T) == 4 ? 512 / BN : 1;
-    const int share = sizeof(T) == 4 ? GP_CHUNK : kb1 - kb0, shares = (kb1 - kb0 + share - 1) / share;
-    constexpr int products = sizeof(T) == 4 ? 6 : PARTS ? 2 : 1;
+    constexpr int NA = PLANES ? 512 / BN : 1;
+    const int share = PLANES ? GP_CHUNK : kb1 - kb0, shares = (kb1 - kb0 + share - 1) / share;
+    constexpr int products = PLANES ? 6 : PARTS ? 2 : 1;
 
     if (warp == 2 && tc::elect_one()) {
         tc::prefetch_map(&ta);
         tc::prefetch_map(&tb);
     }
     if (tid == 0) {
-        s_fail = 0;
+        s_fail = s_lost = 0;
         for (int i = 0; i < Ring::N; ++i) {
             tc::mbar_init(&full[i], 1);
             tc::mbar_init(&empty[i], 1);
@@ -200,7 +233,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
             int i = 0;
             bool ok = true;
             auto load = [&](int kb, int product) {
-                const int st = i % Ring::N, k = kb * GT_K;
+                const int st = i % Ring::N, k = kb * KB;
                 ok = tc::mbar_wait_or_fail(&empty[st], ((i / Ring::N) & 1) ^ 1, fail);
                 if (!ok) return;
                 unsigned char *sa = ring + st * Ring::STAGE, *sb = sa + Ring::A;
@@ -215,6 +248,9 @@ __global__ void __launch_bounds__(GT_NT, 1)
                 if (g.b_mn) {
                     for (int c = 0; c < BN / 64; ++c)
                         tc::tma_load_3d(sb + c * 8192, &tb, &full[st], n0 + c * 64, k, pb);
+                } else if (MODE == TC_GATED) {
+                    tc::tma_load_3d(sb, &tb, &full[st], k, n0, pb);
+                    tc::tma_load_3d(sb + BO * 128, &tb, &full[st], k, g.up + n0, pb);
                 } else {
                     tc::tma_load_3d(sb, &tb, &full[st], k, n0, pb);
                 }
@@ -248,6 +284,8 @@ __global__ void __launch_bounds__(GT_NT, 1)
                         const uint32_t d = taddr + (uint32_t)(acc * BN);
                         if (std::is_same<T, __half>::value && PARTS && kk == 0 && 2 * u == n)  // on to the upper part
                             tc::umma_shifted<F16_PART_SHIFT>(d, da, db, g.idesc);
+                        else if (MODE == TC_INT8)
+                            tc::umma_i8(d, da + ka * kk, db + kbs * kk, g.idesc, (u | kk) != 0);
                         else
                             tc::umma_bf16(d, da + ka * kk, db + kbs * kk, g.idesc, (u | kk) != 0);
                     }
@@ -260,6 +298,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
     } else {  // ---- epilogue warps: TMEM -> partial tile in shared memory
         const int q4 = warp & 3, half = (warp - 2) >> 2;
         const bool ok = tc::mbar_wait_warp(&acc_full, 0, fail);
+        if (MODE == TC_INT8 && !ok) s_lost = 1;
         tc::fence_after_sync();
         float* row = part + (q4 * 32 + lane) * LDP;
 #pragma unroll 1
@@ -289,71 +328,96 @@ __global__ void __launch_bounds__(GT_NT, 1)
 
     // Four positions per thread and round, their residuals and biases loaded first:
     // one memory latency a round.
-    constexpr int U = 4;
+    constexpr int U = MODE == TC_GATED ? 2 : 4;
     constexpr bool FAST = sizeof(T) == 2;
     constexpr float scale = PartsOf<T>::hi;
-    const int slice = BN / S, per_row = slice / 4;
+    const int slice = BO / S, per_row = slice / 4;
     const uint32_t pbase = tc::smem_u32(part);
     const Epilogue& e = g.e;
+    bool lost = false;  // an integer sum has no NaN: the CTAs say that theirs never came
+    if (MODE == TC_INT8)
+        for (int s = 0; s < S; ++s) lost |= (S > 1 ? ld_cluster_u32(tc::smem_u32(&s_lost), s) : (uint32_t)s_lost) != 0;
     for (int i0 = tid; i0 < GT_M * per_row; i0 += U * GT_NT) {
         int row[U], col[U];
         uint32_t at[U];
         float4 res[U], bias[U];
+        float4 by[U];  // TC_GATED: the partners' bias; TC_INT8: the columns' scales
+        float xs[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * GT_NT, r = i / per_row, c = rank * slice + (i - r * per_row) * 4;
             row[u] = i < GT_M * per_row ? m0 + r : g.m;
             col[u] = n0 + c;
             at[u] = (uint32_t)(r * LDP + c) * 4;
-            res[u] = bias[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            res[u] = bias[u] = by[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            xs[u] = 0.0f;
             if (row[u] < g.m && col[u] < g.n) {
                 const T* rp = static_cast<const T*>(e.residual) + row[u] * e.ldr + col[u];
                 const T* bp = static_cast<const T*>(e.bias) + col[u];
+                if (MODE == TC_INT8) xs[u] = g.xs[row[u]];
                 if (g.vec && col[u] + 4 <= g.n) {
                     if (e.residual) res[u] = load4(rp);
                     if (e.bias) bias[u] = load4(bp);
+                    if (MODE == TC_GATED && e.bias) by[u] = load4(bp + g.up);
+                    if (MODE == TC_INT8) by[u] = load4(g.ws + col[u]);
                 } else {
                     float* rf = &res[u].x;
                     float* bf = &bias[u].x;
+                    float* yf = &by[u].x;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         if (col[u] + j < g.n) {
                             if (e.residual) rf[j] = to_f32(rp[j]);
                             if (e.bias) bf[j] = to_f32(bp[j]);
+                            if (MODE == TC_GATED && e.bias) yf[j] = to_f32(bp[g.up + j]);
+                            if (MODE == TC_INT8) yf[j] = g.ws[col[u] + j];
                         }
                 }
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (row[u] >= g.m || col[u] >= g.n) continue;
-            float4 z;
-            if (S > 1) {
-                z = ld_cluster_f4(pbase + at[u], rank);
-                for (int s = 1; s < S; ++s) {
-                    const float4 v = ld_cluster_f4(pbase + at[u], (rank + s) & (S - 1));
+        auto sums = [&](uint32_t a) {
+            if (S == 1) return *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(part) + a);
+            float4 z = ld_cluster_f4(pbase + a, rank);
+            for (int s = 1; s < S; ++s) {
+                const float4 v = ld_cluster_f4(pbase + a, (rank + s) & (S - 1));
+                if (MODE == TC_INT8) {
+                    z = make_float4(__int_as_float(__float_as_int(z.x) + __float_as_int(v.x)),
+                                    __int_as_float(__float_as_int(z.y) + __float_as_int(v.y)),
+                                    __int_as_float(__float_as_int(z.z) + __float_as_int(v.z)),
+                                    __int_as_float(__float_as_int(z.w) + __float_as_int(v.w)));
+                } else {
                     z.x += v.x;
                     z.y += v.y;
                     z.z += v.z;
                     z.w += v.w;
                 }
-            } else {
-                z = *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(part) + at[u]);
             }
+            return z;
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (row[u] >= g.m || col[u] >= g.n) continue;
+            float4 z = sums(at[u]);
             const bool whole = col[u] + 4 <= g.n;
             if (PARTS) z = make_float4(z.x * scale, z.y * scale, z.z * scale, z.w * scale);
-            if (products > 1) {
-                z.x = finite_or_retake<T>(g, row[u], col[u], z.x);
-                if (col[u] + 1 < g.n) z.y = finite_or_retake<T>(g, row[u], col[u] + 1, z.y);
-                if (col[u] + 2 < g.n) z.z = finite_or_retake<T>(g, row[u], col[u] + 2, z.z);
-                if (col[u] + 3 < g.n) z.w = finite_or_retake<T>(g, row[u], col[u] + 3, z.w);
+            if (MODE == TC_INT8) {
+                z = make_float4(dequantised(z.x, xs[u], by[u].x), dequantised(z.y, xs[u], by[u].y),
+                                dequantised(z.z, xs[u], by[u].z), dequantised(z.w, xs[u], by[u].w));
+                if (lost) z = make_float4(NAN, NAN, NAN, NAN);
             }
+            auto retaken = [&](float4& z, int c) {
+                z.x = finite_or_retake<T>(g, row[u], c, z.x);
+                if (col[u] + 1 < g.n) z.y = finite_or_retake<T>(g, row[u], c + 1, z.y);
+                if (col[u] + 2 < g.n) z.z = finite_or_retake<T>(g, row[u], c + 2, z.z);
+                if (col[u] + 3 < g.n) z.w = finite_or_retake<T>(g, row[u], c + 3, z.w);
+            };
+            if (products > 1) retaken(z, col[u]);
             z.x += bias[u].x;
             z.y += bias[u].y;
             z.z += bias[u].z;
             z.w += bias[u].w;
-            auto put = [&](void* out, long long ld, const float4& v) {
-                T* p = static_cast<T*>(out) + row[u] * ld + col[u];
+            auto put = [&](void* out, long long at, const float4& v) {
+                T* p = static_cast<T*>(out) + at;
                 if (g.vec && whole) {
                     store4(p, v);
                 } else {
@@ -363,7 +427,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
                         if (col[u] + j < g.n) p[j] = from_f32<T>(f[j]);
                 }
             };
-            if (e.pre) put(e.pre, e.ldp, z);
+            if (e.pre) put(e.pre, row[u] * e.ldp + col[u], z);
             float4 y = z;
             if (e.act == FG_ACT_GELU && FAST) {
                 gelu2(y.x, y.y);
@@ -372,11 +436,21 @@ __global__ void __launch_bounds__(GT_NT, 1)
                 y = make_float4(activate<FAST>(z.x, e.act), activate<FAST>(z.y, e.act), activate<FAST>(z.z, e.act),
                                 activate<FAST>(z.w, e.act));
             }
+            if (MODE == TC_GATED) {
+                float4 p = sums(at[u] + BO * 4);
+                if (products > 1) retaken(p, g.up + col[u]);
+                p.x += by[u].x;
+                p.y += by[u].y;
+                p.z += by[u].z;
+                p.w += by[u].w;
+                if (e.pre) put(e.pre, row[u] * e.ldp + g.up + col[u], p);
+                y = make_float4(y.x * p.x, y.y * p.y, y.z * p.z, y.w * p.w);
+            }
             y.x += res[u].x;
             y.y += res[u].y;
             y.z += res[u].z;
             y.w += res[u].w;
-            put(e.y, e.ldy, y);
+            put(e.y, row[u] * e.ldy + col[u], y);
         }
     }
     if (S > 1) cluster_sync();  // a peer may still read this CTA's partial tile
@@ -400,11 +474,13 @@ constexpr int GP_NT = 64 + GP_EPI * 32;
 
 // Operand stages and the epilogue's buffers: 4 KB a warp, or for float32 8 KB, which
 // hold the running sums of its 32 rows x 64 columns.
-template <class T, int BN>
+template <class T, int BN, int MODE>
 struct PairOf {
-    static constexpr int B = BN / 2 * GT_K * 2, STAGE = GP_A + B, STAGES = sizeof(T) == 4 ? 3 : 5;
+    static constexpr int B = BN / 2 * GT_K * 2, STAGE = GP_A + B;
+    static constexpr int STAGES = sizeof(T) == 4 ? 3 : MODE == TC_INT8 ? 4 : 5;
     static constexpr int BUF = sizeof(T) == 4 ? 2 * GP_BUF : GP_BUF;
-    static constexpr int SMEM = STAGES * STAGE + GP_EPI * (BUF + (sizeof(T) == 4 ? 0 : 128));
+    static constexpr int SCALES = sizeof(T) == 2 && MODE == TC_INT8 ? 256 : 0;  // a warp's 64 columns'
+    static constexpr int SMEM = STAGES * STAGE + GP_EPI * (BUF + (sizeof(T) == 4 ? 0 : 128) + SCALES);
     static constexpr int WARPS = BN / 64 * 4;         // epilogue warps of a tile
     static constexpr int GROUPS = GP_EPI / WARPS;     // that take tiles in turn
 };
@@ -437,6 +513,21 @@ __device__ __forceinline__ void activate_all(float (&v)[2][32]) {
                 v[h][j + 1] = activate<true>(v[h][j + 1], ACT);
             }
         }
+}
+
+// v[0] = act(v[0]) v[1]
+template <int ACT>
+__device__ __forceinline__ void gate_all(float (&v)[2][32]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        if (ACT == FG_ACT_GELU) {
+            gelu2(v[0][j], v[0][j + 1]);
+        } else if (ACT != FG_ACT_NONE) {
+            v[0][j] = activate<true>(v[0][j], ACT);
+            v[0][j + 1] = activate<true>(v[0][j + 1], ACT);
+        }
+        unpair2(mul2(pair2(v[0][j], v[0][j + 1]), pair2(v[1][j], v[1][j + 1])), v[0][j], v[0][j + 1]);
+    }
 }
 
 // Columns 2 lane and 2 lane + 1 of a 64-column piece of the bias, packed; fetched
@@ -505,15 +596,24 @@ __device__ __noinline__ void store_nan(void* matrix, long long ld, int row0, int
 }
 
 // DIRECT: outputs, residual or bias do not start on 16-byte boundaries, which TMA
-// needs: they pass row by row between memory and the buffer.  PARTS: A in two parts.
-template <class T, int BN, bool DIRECT, bool PARTS>
+// needs: they pass row by row between memory and the buffer.
+//
+// TC_GATED: the leader holds 128 gates' rows of B and its peer their partners', so that
+// an accumulator's halves are the two factors of 128 outputs; a warp takes 32 of each.
+// 16-bit results leave in rows of 64 bytes (64-byte swizzle), both pre-activations
+// through the two halves of a warp's buffer.
+template <class T, int BN, bool DIRECT, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                      const __grid_constant__ CUtensorMap ty, const __grid_constant__ CUtensorMap tp,
                      const __grid_constant__ CUtensorMap tr, const __grid_constant__ TcArgs g) {
-    using P = PairOf<T, BN>;
+    using P = PairOf<T, BN, MODE>;
     constexpr int GP_STAGES = P::STAGES;
+    constexpr bool PARTS = MODE == TC_PARTS, PLANES = sizeof(T) == 4 && MODE != TC_INT8;
+    constexpr int BO = MODE == TC_GATED ? BN / 2 : BN, PC = MODE == TC_GATED ? 32 : 64;  // outputs of a tile's row, a warp's
+    constexpr int KB = MODE == TC_INT8 ? 2 * GT_K : GT_K;
     static_assert(sizeof(T) == 2 || BN == 256, "float32 takes 256 columns");
+    static_assert(MODE != TC_GATED || (BN == 256 && !DIRECT), "gated tiles have 128 columns and TMA stores");
     extern __shared__ __align__(1024) unsigned char dsmem[];
     __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], acc_full[2], acc_empty[2], res_full[GP_EPI];
     __shared__ uint32_t tmem_slot;
@@ -523,8 +623,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     unsigned char *ring = dsmem, *bufs = ring + GP_STAGES * P::STAGE, *biases = bufs + GP_EPI * P::BUF;
     const int pairs = (int)(gridDim.x >> 1), items = g.mt * g.nt * g.split;
     auto k_begin = [&](int part) { return (int)((long long)g.kt * part / g.split); };
-    constexpr int chunk = sizeof(T) == 4 ? GP_CHUNK : 1 << 30;
-    constexpr int products = sizeof(T) == 4 ? 6 : PARTS ? 2 : 1;
+    constexpr int chunk = PLANES ? GP_CHUNK : 1 << 30;
+    constexpr int products = PLANES ? 6 : PARTS ? 2 : 1;
     constexpr float scale = PartsOf<T>::hi;
 
     if (warp == 2 && tc::elect_one()) {
@@ -533,7 +633,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
         if (!DIRECT) {
             tc::prefetch_map(&ty);
             if (g.e.pre) tc::prefetch_map(&tp);
-            if (g.e.residual) tc::prefetch_map(&tr);
+            if (MODE == TC_GATED ? g.e.pre != nullptr : g.e.residual != nullptr) tc::prefetch_map(&tr);
         }
     }
     if (tid == 0) {
@@ -564,9 +664,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             bool ok = true;
             for (int w = blockIdx.x >> 1; w < items && ok; w += pairs) {
                 const int t = w / g.split, sp = w - t * g.split, k1 = k_begin(sp + 1);
-                const int m0 = t / g.nt * 2 * GT_M + rank * GT_M, n0 = t % g.nt * BN + rank * (BN / 2);
+                const int m0 = t / g.nt * 2 * GT_M + rank * GT_M;
+                const int n0 = t % g.nt * BO + rank * (MODE == TC_GATED ? g.up : BN / 2);
                 auto load = [&](int kb, int product) {
-                    const int st = i % GP_STAGES, k = kb * GT_K;
+                    const int st = i % GP_STAGES, k = kb * KB;
                     ok = tc::mbar_wait_or_fail(&empty[st], ((i / GP_STAGES) & 1) ^ 1, fail);
                     if (!ok) return;
                     unsigned char *sa = ring + st * P::STAGE, *sb = sa + GP_A;
@@ -621,6 +722,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                                 const uint32_t d = taddr + (uint32_t)(acc * BN);
                                 if (std::is_same<T, __half>::value && PARTS && kk == 0 && 2 * u == n)
                                     tc::umma_pair_shifted<F16_PART_SHIFT>(d, da, db, g.idesc);  // on to the upper part
+                                else if (MODE == TC_INT8)
+                                    tc::umma_pair_i8(d, da + ka * kk, db + kbs * kk, g.idesc, (u | kk) != 0);
                                 else
                                     tc::umma_pair(d, da + ka * kk, db + kbs * kk, g.idesc, (u | kk) != 0);
                             }
@@ -656,8 +759,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             // one step after the other: six products a K block hide it.
             for (; item < items; item += step) {
                 const int t = item / g.split, sp = item - t * g.split, k1 = k_begin(sp + 1);
-                const int col = t % g.nt * BN + part * 64, m0 = t / g.nt * 2 * GT_M + tr_rows;
+                const int col = t % g.nt * BO + part * PC, m0 = t / g.nt * 2 * GT_M + tr_rows;
                 bool all_ok = true;
+                float xs = 0.0f;
+                if (MODE == TC_INT8 && m0 + lane < g.m) xs = g.xs[m0 + lane];
                 if (tc::elect_one()) tc::bulk_wait_read<0>();
                 __syncwarp();
                 for (int c0 = k_begin(sp), first = 1; c0 < k1; c0 += min(chunk, k1 - c0), first = 0, ++li) {
@@ -667,7 +772,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         float v[32];
-                        tc::tmem_ld_32x32(taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + part * 64 + 32 * h), v);
+                        tc::tmem_ld_32x32(taddr + ((uint32_t)(q4 * 32) << 16) +
+                                              (uint32_t)(acc * BN + part * PC + (MODE == TC_GATED ? BO : 32) * h), v);
+                        if (MODE == TC_INT8) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                v[j] = dequantised(v[j], xs, col + 32 * h + j < g.n ? __ldg(g.ws + col + 32 * h + j) : 0.0f);
+                        }
                         if (h == 1) {
                             tc::fence_before_sync();
                             __syncwarp();
@@ -685,8 +796,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         }
                     }
                 }
+                if constexpr (MODE == TC_GATED) {
+                    const bool in = m0 < g.m && col < g.n;
+                    auto put = [&](const CUtensorMap* map, const void* from, bool last) {
+                        tc::fence_proxy_async();
+                        __syncwarp();
+                        if (tc::elect_one()) {
+                            if (in) tc::tma_store_2d(map, from, col, m0);
+                            if (last) tc::bulk_commit();
+                        }
+                    };
+                    // z and its partner: sums, marked where they are not finite, and the bias
+                    bool odd = false;
+#pragma unroll 2
+                    for (int q = 0; q < 16; ++q) {
+                        const int j = q % 8 * 4, c0 = q < 8 ? col : g.up + col;
+                        float4* at = reinterpret_cast<float4*>(brow + q / 8 * GP_BUF + (((uint32_t)j << 2) ^ sw));
+                        const float4 x = *at;
+                        float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool finite = fabsf(v[i]) <= FLT_MAX;
+                            odd |= !finite;
+                            if (!finite || !all_ok) v[i] = NAN;  // a wait that ran out leaves NaN, too
+                            if (e.bias && col + j + i < g.n) v[i] += __ldg(static_cast<const float*>(e.bias) + c0 + j + i);
+                        }
+                        *at = make_float4(v[0], v[1], v[2], v[3]);
+                    }
+                    odd_seen |= __any_sync(0xffffffffu, odd && all_ok);
+                    if (e.pre) {
+                        put(&tp, buf, false);
+                        put(&tr, buf + GP_BUF, true);
+                        if (tc::elect_one()) tc::bulk_wait_read<0>();
+                        __syncwarp();
+                    }
 #pragma unroll 1
-                for (int h = 0; h < 2; ++h) {
+                    for (int j = 0; j < 32; j += 4) {
+                        float4* at = reinterpret_cast<float4*>(brow + (((uint32_t)j << 2) ^ sw));
+                        const float4 z = *at, p = *reinterpret_cast<const float4*>(brow + GP_BUF + (((uint32_t)j << 2) ^ sw));
+                        *at = make_float4(activate<false>(z.x, e.act) * p.x, activate<false>(z.y, e.act) * p.y,
+                                          activate<false>(z.z, e.act) * p.z, activate<false>(z.w, e.act) * p.w);
+                    }
+                    put(&ty, buf, true);
+                }
+#pragma unroll 1
+                for (int h = MODE == TC_GATED ? 2 : 0; h < 2; ++h) {
                     const int c0 = col + 32 * h;
                     const bool in = m0 < g.m && c0 < g.n;
                     if (lost) {
@@ -726,8 +880,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                                 make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                     };
                     bool odd = false;
+                    if (PLANES) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) odd |= !(fabsf(v[j]) <= FLT_MAX);
+                        for (int j = 0; j < 32; ++j) odd |= !(fabsf(v[j]) <= FLT_MAX);
+                    }
                     if (__any_sync(0xffffffffu, odd && all_ok)) {
                         odd_seen = true;
 #pragma unroll
@@ -784,6 +940,72 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         put(&ty, m0, in);
                 }
             }
+        } else if constexpr (MODE == TC_GATED) {
+            const uint32_t sw64 = (uint32_t)(lane >> 1 & 3) << 4;
+            for (; item < items; item += step, li += P::GROUPS) {
+                const int acc = li & 1, col = item % g.nt * BO + part * PC, m0 = item / g.nt * 2 * GT_M + tr_rows;
+                unsigned char* bias = biases + w * 128;
+                if (e.bias) {  // 32 of the gates, 32 of their partners
+                    const T* b = static_cast<const T*>(e.bias) + (lane < 16 ? 0 : g.up) + col;
+                    reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(b, lane & 15, g.n - col, 0);
+                    __syncwarp();
+                }
+                const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
+                tc::fence_after_sync();
+                const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + part * PC);
+                float v[2][32];
+                tc::tmem_ld_32x32_nowait(src, v[0]);
+                tc::tmem_ld_32x32_nowait(src + BO, v[1]);
+                tc::tmem_ld_wait(v[0]);
+                tc::tmem_ld_wait(v[1]);
+                tc::fence_before_sync();
+                __syncwarp();
+                if (tc::elect_one()) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
+                if (!ok) {  // a wait that ran out leaves NaN, not a plausible number
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[0][j] = v[1][j] = NAN;
+                }
+                if (e.bias) add_bias<T>(v, bias);
+                // rows of 64 bytes, 32 of them: a half of the buffer
+                auto stage = [&](const float (&v)[32], int h) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        *reinterpret_cast<uint4*>(buf + h * (GP_BUF / 2) + lane * 64 + (((uint32_t)j << 1) ^ sw64)) = pack8<T>(&v[j]);
+                };
+                const bool inside = m0 < g.m && col < g.n;
+                if (tc::elect_one()) tc::bulk_wait_read<0>();
+                __syncwarp();
+                if (e.pre) {
+                    stage(v[0], 0);
+                    stage(v[1], 1);
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                    if (tc::elect_one()) {
+                        if (inside) {
+                            tc::tma_store_2d(&tp, buf, col, m0);
+                            tc::tma_store_2d(&tr, buf + GP_BUF / 2, col, m0);
+                        }
+                        tc::bulk_commit();
+                    }
+                }
+                switch (e.act) {
+                    case FG_ACT_RELU: gate_all<FG_ACT_RELU>(v); break;
+                    case FG_ACT_GELU: gate_all<FG_ACT_GELU>(v); break;
+                    case FG_ACT_SILU: gate_all<FG_ACT_SILU>(v); break;
+                    default: gate_all<FG_ACT_NONE>(v);
+                }
+                if (e.pre) {
+                    if (tc::elect_one()) tc::bulk_wait_read<0>();
+                    __syncwarp();
+                }
+                stage(v[0], 0);
+                tc::fence_proxy_async();
+                __syncwarp();
+                if (tc::elect_one()) {
+                    if (inside) tc::tma_store_2d(&ty, buf, col, m0);
+                    tc::bulk_commit();
+                }
+            }
         } else {
         for (; item < items; item += step, li += P::GROUPS) {
             const int acc = li & 1, t = item / g.split;
@@ -799,6 +1021,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(static_cast<const T*>(e.bias) + col, lane, g.n - col, DIRECT);
                 __syncwarp();
             }
+            float xs = 0.0f;
+            float* scales = reinterpret_cast<float*>(biases + GP_EPI * 128 + w * P::SCALES);
+            if (MODE == TC_INT8) {
+                if (m0 + lane < g.m) xs = g.xs[m0 + lane];
+                scales[lane] = col + lane < g.n ? g.ws[col + lane] : 0.0f;
+                scales[lane + 32] = col + lane + 32 < g.n ? g.ws[col + lane + 32] : 0.0f;
+                __syncwarp();
+            }
             T* residual = const_cast<T*>(static_cast<const T*>(e.residual));
             if (DIRECT && ahead) copy_rows<T, false, 8>(buf, residual, e.ldr, m0, col, g.m, g.n, lane);
             const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
@@ -812,6 +1042,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             tc::fence_before_sync();
             __syncwarp();
             if (tc::elect_one()) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
+            if (MODE == TC_INT8) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 c = *reinterpret_cast<const float4*>(scales + 32 * h + j);
+                        v[h][j] = dequantised(v[h][j], xs, c.x);
+                        v[h][j + 1] = dequantised(v[h][j + 1], xs, c.y);
+                        v[h][j + 2] = dequantised(v[h][j + 2], xs, c.z);
+                        v[h][j + 3] = dequantised(v[h][j + 3], xs, c.w);
+                    }
+            }
             if (g.split > 1) {  // this part's sums as they are; finish_kernel adds the parts
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -945,12 +1187,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     const T* mark = static_cast<const T*>(e.pre ? e.pre : e.y);
     const long long ld = e.pre ? e.ldp : e.ldy;
     for (int t = blockIdx.x >> 1; t < items; t += pairs) {
-        const int m0 = t / g.nt * 2 * GT_M + rank * GT_M, n0 = t % g.nt * BN;
-        for (int i = tid; i < GT_M * BN; i += GP_NT) {
-            const int row = m0 + i / BN, col = n0 + i % BN;
+        const int m0 = t / g.nt * 2 * GT_M + rank * GT_M, n0 = t % g.nt * BO;
+        for (int i = tid; i < GT_M * BO; i += GP_NT) {
+            const int row = m0 + i / BO, col = n0 + i % BO;
             if (row >= g.m || col >= g.n) continue;
-            const float y = to_f32(__ldcg(mark + row * ld + col));
-            if (y != y) epilogue_store<T>(e, row, col, retake<T>(g, row, col));
+            float y = to_f32(__ldcg(mark + row * ld + col));
+            if (MODE == TC_GATED && e.pre) y += to_f32(__ldcg(mark + row * ld + g.up + col));
+            if (MODE == TC_GATED ? !(fabsf(y) <= FLT_MAX) : y != y) {
+                if (MODE == TC_GATED)
+                    gated_store<T>(e, g.up, row, col, retake<T>(g, row, col), retake<T>(g, row, g.up + col));
+                else
+                    epilogue_store<T>(e, row, col, retake<T>(g, row, col));
+            }
         }
     }
 }
@@ -987,17 +1235,18 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* part, const __
 
 // ---- host side ---------------------------------------------------------------
 
-// Operand of `rows` rows (unit stride along k: [rows][k], else [k][rows]), in
+// Operand of `rows` rows of 16-bit elements, or of bytes (unit stride along k: [rows][k], else [k][rows]), in
 // `planes` planes `plane` elements apart.
 static int operand_map(CUtensorMap* m, int dtype, const void* p, long long rows, long long k, long long ld, bool mn,
-                       int box_rows, int planes, long long plane) {
+                       int box_rows, int planes, long long plane, bool bytes = false) {
     tc::EncodeTiledFn enc = tc::encode_fn();
     if (!enc) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     cuuint64_t dims[3] = {(cuuint64_t)(mn ? rows : k), (cuuint64_t)(mn ? k : rows), (cuuint64_t)planes};
-    cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2};
-    cuuint32_t box[3] = {64, (cuuint32_t)(mn ? GT_K : box_rows), 1};
+    const int es = bytes ? 1 : 2;
+    cuuint64_t strides[2] = {(cuuint64_t)ld * es, (cuuint64_t)plane * es};
+    cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)(mn ? GT_K : box_rows), 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult r = enc(m, dtype == FG_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+    const CUresult r = enc(m, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : dtype == FG_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                            3, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1015,25 +1264,32 @@ static uint32_t instr_desc(int dtype, int m, int n, bool a_mn, bool b_mn) {
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// Of signed bytes, kind::i8: 32-bit integer accumulators.
+static uint32_t instr_desc_i8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
 bool tc_gemm_fits(const void* a, const void* b, const GemmShape& g) {
     const long long lda = g.ak == 1 ? g.am : g.ak, ldb = g.bk == 1 ? g.bn : g.bk;
     return aligned(a, 16) && aligned(b, 16) && lda % 8 == 0 && ldb % 8 == 0 && g.k > 0 && g.m < (1ll << 31) - 512 &&
            g.n < (1ll << 31) - 512 && g.k < (1ll << 31) - 512;
 }
 
-template <class T, int BN>
+template <class T, int BN, int MODE = TC_WHOLE>
 static int launch_split(int dtype, const void* a, const void* b, const GemmShape& s, TcArgs g, cudaStream_t st) {
+    constexpr bool I8 = MODE == TC_INT8;
+    constexpr int BO = MODE == TC_GATED ? BN / 2 : BN;
     CUtensorMap ta, tb;
-    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M, a_planes(g), g.a_plane);
-    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN, b_planes(g), g.b_plane);
+    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M, a_planes(g), g.a_plane, I8);
+    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BO, b_planes(g), g.b_plane, I8);
     if (rc) return rc;
-    g.idesc = instr_desc(dtype, GT_M, BN, g.a_mn, g.b_mn);
-    g.nt = (g.n + BN - 1) / BN;
+    g.idesc = I8 ? instr_desc_i8(GT_M, BN) : instr_desc(dtype, GT_M, BN, g.a_mn, g.b_mn);
+    g.nt = (g.n + BO - 1) / BO;
     const long long ctas = (long long)g.mt * g.nt * g.split;
     FG_REQUIRE(ctas <= 0x7fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
-    auto kernel = &gemm_split_kernel<T, BN, false>;
-    if constexpr (sizeof(T) == 2)
-        if (g.products == 2) kernel = &gemm_split_kernel<T, BN, true>;
+    auto kernel = &gemm_split_kernel<T, BN, MODE>;
+    if constexpr (sizeof(T) == 2 && MODE == TC_WHOLE)
+        if (g.products == 2) kernel = &gemm_split_kernel<T, BN, TC_PARTS>;
     const int smem = RingOf<BN>::N * RingOf<BN>::STAGE + 1024;
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
     cudaLaunchConfig_t cfg = {};
@@ -1051,57 +1307,65 @@ static int launch_split(int dtype, const void* a, const void* b, const GemmShape
     return FG_OK;
 }
 
-// Matrix [rows][n] for the epilogue's TMA: boxes of 32 rows of 128 bytes.
-static int tile_map(CUtensorMap* m, int dtype, const void* p, long long rows, long long n, long long ld) {
+// Matrix [rows][n] for the epilogue's TMA: boxes of 32 rows of 128 or 64 bytes.
+static int tile_map(CUtensorMap* m, int dtype, const void* p, long long rows, long long n, long long ld, int wide = 128) {
     if (!p) return FG_OK;  // the kernel does not touch it
     tc::EncodeTiledFn enc = tc::encode_fn();
     if (!enc) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     const int es = dtype_size(dtype);
     cuuint64_t dims[2] = {(cuuint64_t)n, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)ld * es};
-    cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32};
+    cuuint32_t box[2] = {(cuuint32_t)(wide / es), 32};
     cuuint32_t estr[2] = {1, 1};
     const CUtensorMapDataType t = dtype == FG_DTYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                   : dtype == FG_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const CUresult r = enc(m, t, 2, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                           wide == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return FG_OK;
 }
 
-template <class T, int BN>
+template <class T, int BN, int MODE = TC_WHOLE>
 static int launch_pair(int dtype, const void* a, const void* b, const GemmShape& s, TcArgs g, void* ws, cudaStream_t st) {
+    constexpr bool I8 = MODE == TC_INT8;
+    constexpr int BO = MODE == TC_GATED ? BN / 2 : BN, wide = MODE == TC_GATED && sizeof(T) == 2 ? 64 : 128;
+    using P = PairOf<T, BN, MODE>;
     CUtensorMap ta, tb, ty = {}, tp = {}, tr = {};
     const Epilogue& e = g.e;
     const long long ld = (s.n + 3) / 4 * 4;
     g.mt = (g.m + 2 * GT_M - 1) / (2 * GT_M);
-    g.nt = (g.n + BN - 1) / BN;
+    g.nt = (g.n + BO - 1) / BO;
     g.m_pad = g.mt * 2 * GT_M;
-    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M, a_planes(g), g.a_plane);
-    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN / 2, b_planes(g), g.b_plane);
+    int rc = operand_map(&ta, dtype, a, s.m, s.k, g.a_mn ? s.ak : s.am, g.a_mn, GT_M, a_planes(g), g.a_plane, I8);
+    if (!rc) rc = operand_map(&tb, dtype, b, s.n, s.k, g.b_mn ? s.bk : s.bn, g.b_mn, BN / 2, b_planes(g), g.b_plane, I8);
     if (g.split > 1) {
         if (!rc) rc = tile_map(&ty, FG_DTYPE_F32, ws, (long long)g.split * g.m_pad, ld, ld);
     } else if (!g.direct) {
-        if (!rc) rc = tile_map(&ty, dtype, e.y, s.m, s.n, e.ldy);
-        if (!rc) rc = tile_map(&tp, dtype, e.pre, s.m, s.n, e.ldp);
-        if (!rc) rc = tile_map(&tr, dtype, e.residual, s.m, s.n, e.ldr);
+        if (!rc) rc = tile_map(&ty, dtype, e.y, s.m, g.n, e.ldy, wide);
+        if (!rc) rc = tile_map(&tp, dtype, e.pre, s.m, g.n, e.ldp, wide);
+        // gated: the partners' part of pre, a map of its own, as the gates' ends at its last column
+        if (!rc && MODE == TC_GATED && e.pre)
+            rc = tile_map(&tr, dtype, static_cast<const char*>(e.pre) + (size_t)g.up * dtype_size(dtype), s.m, g.n, e.ldp, wide);
+        if (!rc && MODE != TC_GATED) rc = tile_map(&tr, dtype, e.residual, s.m, s.n, e.ldr, wide);
     }
     if (rc) return rc;
-    g.idesc = instr_desc(dtype, 2 * GT_M, BN, g.a_mn, g.b_mn);
+    g.idesc = I8 ? instr_desc_i8(2 * GT_M, BN) : instr_desc(dtype, 2 * GT_M, BN, g.a_mn, g.b_mn);
     const long long items = (long long)g.mt * g.nt * g.split;
     FG_REQUIRE(items <= 0x3fffffffll && (long long)g.split * g.m_pad <= 0x7fffffffll, "%d x %d outputs: too many tiles", g.m,
                g.n);
     const bool direct = g.direct && g.split == 1;
-    auto kernel = direct ? &gemm_pair_kernel<T, BN, true, false> : &gemm_pair_kernel<T, BN, false, false>;
-    if constexpr (sizeof(T) == 2)
-        if (g.products == 2) kernel = direct ? &gemm_pair_kernel<T, BN, true, true> : &gemm_pair_kernel<T, BN, false, true>;
-    FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), PairOf<T, BN>::SMEM));
+    auto kernel = &gemm_pair_kernel<T, BN, false, MODE>;
+    if constexpr (MODE != TC_GATED)
+        if (direct) kernel = &gemm_pair_kernel<T, BN, true, MODE>;
+    if constexpr (sizeof(T) == 2 && MODE == TC_WHOLE)
+        if (g.products == 2) kernel = direct ? &gemm_pair_kernel<T, BN, true, TC_PARTS> : &gemm_pair_kernel<T, BN, false, TC_PARTS>;
+    FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), P::SMEM));
     const int pairs = std::max(1, device_attr(cudaDevAttrMultiProcessorCount) / 2);
     TcArgs k = g;
     if (g.split > 1) k.e.bias = k.e.residual = k.e.pre = nullptr;  // finish_kernel's
-    kernel<<<2 * (unsigned)std::min<long long>(items, pairs), GP_NT, PairOf<T, BN>::SMEM, st>>>(ta, tb, ty, tp, tr, k);
+    kernel<<<2 * (unsigned)std::min<long long>(items, pairs), GP_NT, P::SMEM, st>>>(ta, tb, ty, tp, tr, k);
     rc = check_launch("gemm_pair_kernel");
     if (rc || g.split == 1) return rc;
     const long long n4 = (long long)g.m * ((g.n + 3) / 4);
@@ -1128,7 +1392,7 @@ struct TcPlan {
     size_t ws;
 };
 
-static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct) {
+static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct, int mode = TC_WHOLE) {
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
     const int kt = (int)((s.k + GT_K - 1) / GT_K) * products;
     auto waves = [](long long tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
@@ -1143,13 +1407,14 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct) {
     const long long m2 = (s.m + 2 * GT_M - 1) / (2 * GT_M), m1 = (s.m + GT_M - 1) / GT_M;
     const int kb = (int)((s.k + GT_K - 1) / GT_K);
     for (int bn : {256, 128}) {
-        if (products == 6 && bn == 128) break;
+        if ((products == 6 || mode == TC_GATED) && bn == 128) break;
+        if (mode == TC_GATED && direct) break;
         const long long tiles = m2 * ((s.n + bn - 1) / bn);
         // 16-bit sums run over GT_RUN K blocks at most: parts go on past 32, and past a full
         // GPU, until they are that short (in 64 bits: kb may be 2^25)
         auto too_long = [&](int parts) { return products < 6 && kb > (long long)GT_RUN * parts; };
         for (int sp = 1; sp <= 32 || too_long(sp / 2); sp *= 2) {
-            if (direct && sp > 1) break;
+            if ((direct || mode != TC_WHOLE) && sp > 1) break;
             if (sp > 1 && (sp > kb / 2 || (tiles * sp > sms && kb <= (long long)GT_RUN * (sp / 2)))) break;
             if (too_long(sp)) continue;
             const size_t ws = sp > 1 ? (size_t)sp * m2 * 2 * GT_M * ((s.n + 3) / 4 * 4) * 4 : 0;
@@ -1183,12 +1448,8 @@ static TcPlan tc_plan(const GemmShape& s, int products, bool direct) {
     return direct && p.split == 1 ? tc_plan_of(s, products, true) : p;
 }
 
-size_t tc_gemm_workspace(int products, const GemmShape& s) {
-    return s.k > 0 ? tc_plan(s, products, false).ws : 0;
-}
-
-int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& s,
-            const Epilogue& e, void* ws, cudaStream_t st) {
+static TcArgs tc_args(const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& s, int products,
+                      const Epilogue& e) {
     TcArgs g{};
     g.m = (int)s.m;
     g.n = (int)s.n;
@@ -1196,17 +1457,32 @@ int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long lon
     g.mt = (int)((s.m + GT_M - 1) / GT_M);
     g.a_mn = s.ak != 1;
     g.b_mn = s.bk != 1;
-    g.products = tc_products(dtype, a_plane != 0);
+    g.products = products;
     g.f = s;
     g.fa = a;
     g.fb = b;
-    g.a_plane = a_planes(g) == 1 ? 8 : a_plane;  // one plane: any multiple of 16 bytes
-    g.b_plane = b_planes(g) == 1 ? 8 : b_plane;
+    g.a_plane = a_planes(g) == 1 ? 16 : a_plane;  // one plane: any multiple of 16 bytes
+    g.b_plane = b_planes(g) == 1 ? 16 : b_plane;
     g.e = e;
+    return g;
+}
+
+// Do all of the epilogue's matrices start their rows on n bytes?
+static bool epilogue_lies(const Epilogue& e, int es, int n) {
+    auto lies = [&](const void* p, long long ld) { return !p || (aligned(p, n) && ld * es % n == 0); };
+    return lies(e.y, e.ldy) && lies(e.bias, 0) && lies(e.pre, e.ldp) && lies(e.residual, e.ldr);
+}
+
+size_t tc_gemm_workspace(int products, const GemmShape& s) {
+    return s.k > 0 ? tc_plan(s, products, false).ws : 0;
+}
+
+int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& s,
+            const Epilogue& e, void* ws, cudaStream_t st) {
+    TcArgs g = tc_args(a, a_plane, b, b_plane, s, tc_products(dtype, a_plane != 0), e);
     const int es = dtype_size(dtype);
-    auto lies = [&](const void* p, long long ld, int n) { return !p || (aligned(p, n) && ld * es % n == 0); };
-    g.vec = lies(e.y, e.ldy, 4 * es) && lies(e.bias, 0, 4 * es) && lies(e.pre, e.ldp, 4 * es) && lies(e.residual, e.ldr, 4 * es);
-    g.direct = !(lies(e.y, e.ldy, 16) && lies(e.bias, 0, 16) && lies(e.pre, e.ldp, 16) && lies(e.residual, e.ldr, 16));
+    g.vec = epilogue_lies(e, es, 4 * es);
+    g.direct = !epilogue_lies(e, es, 16);
     const TcPlan p = tc_plan(s, g.products, g.direct);
     g.split = p.split;
 #define FG_PRODUCT(T)                                                                        \
@@ -1216,6 +1492,50 @@ int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long lon
             : (p.bn == 256   ? launch_split<T, 256>(dtype, a, b, s, g, st)                \
                : p.bn == 128 ? launch_split<T, 128>(dtype, a, b, s, g, st)                \
                              : launch_split<T, 64>(dtype, a, b, s, g, st)))
+    return dtype == FG_DTYPE_F32 ? FG_PRODUCT(float) : dtype == FG_DTYPE_F16 ? FG_PRODUCT(__half) : FG_PRODUCT(__nv_bfloat16);
+#undef FG_PRODUCT
+}
+
+int tc_gated(int dtype, const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& s, const Epilogue& e,
+             cudaStream_t st) {
+    TcArgs g = tc_args(a, a_plane, b, b_plane, s, tc_products(dtype, false), e);
+    const int es = dtype_size(dtype);
+    g.n = g.up = (int)(s.n / 2);
+    // the partners' bias and pre-activations start `up` columns on
+    auto both = [&](int n) { return epilogue_lies(e, es, n) && ((!e.bias && !e.pre) || (long long)g.up * es % n == 0); };
+    g.vec = both(4 * es);
+    g.direct = !both(16);
+    const TcPlan p = tc_plan_of(s, g.products, g.direct, TC_GATED);
+    g.split = p.split;
+#define FG_PRODUCT(T)                                                            \
+    (p.pair        ? launch_pair<T, 256, TC_GATED>(dtype, a, b, s, g, nullptr, st) \
+     : p.bn == 256 ? launch_split<T, 256, TC_GATED>(dtype, a, b, s, g, st)         \
+     : p.bn == 128 ? launch_split<T, 128, TC_GATED>(dtype, a, b, s, g, st)         \
+                   : launch_split<T, 64, TC_GATED>(dtype, a, b, s, g, st))
+    return dtype == FG_DTYPE_F32 ? FG_PRODUCT(float) : dtype == FG_DTYPE_F16 ? FG_PRODUCT(__half) : FG_PRODUCT(__nv_bfloat16);
+#undef FG_PRODUCT
+}
+
+int tc_int8(int dtype, const void* a, const float* xs, const void* b, const float* ws, const GemmShape& s, const Epilogue& e,
+            cudaStream_t st) {
+    TcArgs g = tc_args(a, 0, b, 0, s, 1, e);
+    const int es = dtype_size(dtype);
+    g.kt = (int)((s.k + 2 * GT_K - 1) / (2 * GT_K));
+    g.xs = xs;
+    g.ws = ws;
+    g.vec = epilogue_lies(e, es, 4 * es) && aligned(ws, 16);
+    g.direct = !epilogue_lies(e, es, 16);
+    GemmShape half = s;  // a K block holds 128 codes and takes the time of 64 elements of 16 bits
+    half.k = (s.k + 1) / 2;
+    const TcPlan p = tc_plan_of(half, 1, g.direct, TC_INT8);
+    g.split = p.split;
+#define FG_PRODUCT(T)                                                                       \
+    (p.pair ? (sizeof(T) == 4 || p.bn == 256                                                 \
+                   ? launch_pair<T, 256, TC_INT8>(dtype, a, b, s, g, nullptr, st)            \
+                   : launch_pair<T, sizeof(T) == 4 ? 256 : 128, TC_INT8>(dtype, a, b, s, g, nullptr, st)) \
+     : p.bn == 256 ? launch_split<T, 256, TC_INT8>(dtype, a, b, s, g, st)                    \
+     : p.bn == 128 ? launch_split<T, 128, TC_INT8>(dtype, a, b, s, g, st)                    \
+                   : launch_split<T, 64, TC_INT8>(dtype, a, b, s, g, st))
     return dtype == FG_DTYPE_F32 ? FG_PRODUCT(float) : dtype == FG_DTYPE_F16 ? FG_PRODUCT(__half) : FG_PRODUCT(__nv_bfloat16);
 #undef FG_PRODUCT
 }

@@ -528,6 +528,43 @@ int fg_linear_backward_workspace_size(const fg_linear_params* params, size_t* by
 int fg_linear_backward(const fg_linear_params* params, const void* dy, const void* x, const void* w, const void* pre,
                        void* dx, void* dw, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Gated layer: [z p] = x w^T + bias, y = activation(z) * p.  out_dim is the width
+ * of y; w [2 out_dim][in_dim] holds the gates' rows (z), then their partners' (p),
+ * bias [2 out_dim] likewise (or NULL); pre [rows][2 out_dim] receives z and p for
+ * the backward pass (or NULL; pre_stride 0: 2 out_dim).  z and p are not rounded
+ * before the product.  residual_stride is 0.  in_dim <= 32768, out_dim <= 2^29.
+ * F16 and BF16 x and w that start off a 16-byte boundary have to be named in
+ * `unaligned`. */
+int fg_gated_linear_workspace_size(const fg_linear_params* params, size_t* bytes);
+int fg_gated_linear(const fg_linear_params* params, const void* x, const void* w, const void* bias, void* pre, void* y,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradients: dz = dy p activation'(z), dp = dy activation(z), dx [rows][in_dim]
+ * = [dz dp] w, dw [2 out_dim][in_dim] = [dz dp]^T x, dbias [2 out_dim] = their sums
+ * over the rows, contiguous and of dtype; any may be NULL.  y_stride is dy's.  dz
+ * and dp of F16 and BF16 enter the products as the linear layer's GELU does. */
+int fg_gated_linear_backward_workspace_size(const fg_linear_params* params, size_t* bytes);
+int fg_gated_linear_backward(const fg_linear_params* params, const void* dy, const void* x, const void* w, const void* pre,
+                             void* dx, void* dw, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows as codes of 8 bits: scale = max |x| / 127 of the row, q = 127 x / max |x|
+ * rounded to nearest, ties to even, exactly.  A row of zeros has scale and codes 0;
+ * one that holds an infinity or a NaN has scale NaN and codes 0.  x [rows][dim] of
+ * dtype, q [rows][dim], scale [rows]; rows of q on 16-byte boundaries (address and
+ * stride) are what fg_linear_int8 reads without a copy.  dim <= 2^30. */
+int fg_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t dim, int64_t x_stride, int8_t* q,
+                     int64_t q_stride, float* scale, void* stream);
+
+/* Linear layer of such rows: y = activation(x_scale[i] w_scale[j] (x w^T) + bias) +
+ * residual, x [rows][in_dim] and w [out_dim][in_dim] codes (any of -128 .. 127), their
+ * scales per row; dtype is that of bias, residual and y.  The sums are exact integers.
+ * pre_stride is 0; strides of x and w count codes.  in_dim <= 131071.  Codes that
+ * start off a 16-byte boundary have to be named in `unaligned`. */
+int fg_linear_int8_workspace_size(const fg_linear_params* params, size_t* bytes);
+int fg_linear_int8(const fg_linear_params* params, const int8_t* x, const float* x_scale, const int8_t* w,
+                   const float* w_scale, const void* bias, const void* residual, void* y, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 /* Preference loss over documents of an index.  The policy of query q prefers
  * documents by softmax of the search score s (inner product, or minus squared
  * L2 distance); in the ratio of two documents of one query the normaliser

@@ -19,7 +19,7 @@ def __getattr__(name):
         from . import index
         return getattr(index, name)
     if name in ("QueryAdapter", "layer_norm", "layer_norm_backward", "linear", "linear_backward", "gated_linear",
-                "gated_linear_backward", "quantize_rows", "linear_int8", "preference_loss"):
+                "gated_linear_backward", "quantize_rows", "linear_int8", "orthogonalize", "preference_loss"):
         from . import adapter
         return getattr(adapter, name)
     raise AttributeError(name)

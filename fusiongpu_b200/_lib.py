@@ -58,6 +58,12 @@ class LinearParams(C.Structure):
                 ("unaligned", C.c_int32)]
 
 
+class OrthogonalizeParams(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32), ("dtype", C.c_int32),
+                ("steps", C.c_int32), ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float),
+                ("row_stride", C.c_int64), ("batch_stride", C.c_int64)]
+
+
 class PreferenceParams(C.Structure):
     _fields_ = [("nq", C.c_int32), ("dim", C.c_int32), ("dtype", C.c_int32), ("base_dtype", C.c_int32),
                 ("nbase", C.c_int64), ("n_pairs", C.c_int64), ("metric", C.c_int32), ("beta", C.c_float),
@@ -124,6 +130,8 @@ _SIGS = {
     "fg_quantize_rows": [_P, _I32, _I64, _I32, _I64, _P, _I64, _P, _P],
     "fg_linear_int8_workspace_size": [C.POINTER(LinearParams), C.POINTER(_SZ)],
     "fg_linear_int8": [C.POINTER(LinearParams), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "fg_orthogonalize_workspace_size": [C.POINTER(OrthogonalizeParams), C.POINTER(_SZ)],
+    "fg_orthogonalize": [C.POINTER(OrthogonalizeParams), _P, _P, _P, _SZ, _P],
     "fg_preference_loss": [C.POINTER(PreferenceParams), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
 }
 

@@ -372,6 +372,35 @@ def linear_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
 
 
 @_on
+def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients: tuple[float, float, float] = (3.4445, -4.7750, 2.0315),
+                  eps: float = 1e-7):
+    """The orthogonalised update of g [rows][cols], or of each matrix of g
+    [batch][rows][cols]: X = g / (|g|_F + eps), then `steps` times A = X X^T,
+    X = a X + (b A + c A^2) X.  Of g's type, contiguous."""
+    if not g.is_cuda or g.dim() not in (2, 3):
+        raise ValueError("g must be a 2-D or 3-D CUDA tensor")
+    if g.dtype not in DTYPES:
+        raise TypeError(f"g must be float32, float16 or bfloat16, not {g.dtype}")
+    batch = g.shape[0] if g.dim() == 3 else 1
+    m, n = g.shape[-2:]
+    if not m or not n:
+        raise ValueError(f"g has shape {tuple(g.shape)}")
+    s1, s2 = g.stride(-2), g.stride(-1)
+    if (s2 != 1 and n > 1) or (s1 < n and m > 1) or (batch > 1 and g.stride(0) <= 0):
+        g = g.contiguous()
+        s1 = n
+    ld = s1 if m > 1 else n
+    out = torch.empty_strided(g.shape, (n, 1) if g.dim() == 2 else (m * n, n, 1), dtype=g.dtype, device=g.device)
+    p = _lib.OrthogonalizeParams(batch, m, n, DTYPES[g.dtype], steps, *coefficients, eps, ld,
+                                 g.stride(0) if batch > 1 else 0)
+    nws = _lib.size_query("fg_orthogonalize_workspace_size", C.byref(p))
+    ws = torch.empty(nws, dtype=torch.uint8, device=g.device)
+    _lib.check(_lib.lib().fg_orthogonalize(C.byref(p), g.data_ptr(), out.data_ptr(), _ptr(ws), nws, _stream(g)),
+               "fg_orthogonalize")
+    return out
+
+
+@_on
 def preference_loss(queries: torch.Tensor, base: torch.Tensor, offsets: torch.Tensor, pos_ids: torch.Tensor,
                     neg_ids: torch.Tensor, ref: torch.Tensor | None = None, weights: torch.Tensor | None = None,
                     beta: float = 1.0, label_smoothing: float = 0.0, metric: str = "ip", grad: bool = True):

@@ -565,6 +565,33 @@ int fg_linear_int8(const fg_linear_params* params, const int8_t* x, const float*
                    const float* w_scale, const void* bias, const void* residual, void* y, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/* Orthogonalised update of a matrix: X = G / (|G|_F + eps), then `steps` times
+ * A = X X^T, X = a X + (b A + c A^2) X, which takes the singular values towards one
+ * and keeps the singular vectors.  G: `batch` matrices [rows][cols] of dtype, each on
+ * its own; out [batch][rows][cols] of dtype, contiguous.  Strides count elements
+ * (batch_stride 0: rows * row_stride).  Between the products matrices are held to 22
+ * bits (or 2^-36) as pairs of float16: a, b and c, of at most 16, have to keep
+ * singular values of at most one of order one, as 3.4445, -4.7750, 2.0315 do.  A
+ * matrix that holds an infinity or a NaN is NaN.  steps <= 100, rows and cols <=
+ * 32768, batch <= 65535. */
+typedef struct {
+    int32_t batch;
+    int32_t rows;
+    int32_t cols;
+    int32_t dtype;            /* F32, F16 or BF16                               */
+    int32_t steps;
+    float a;
+    float b;
+    float c;
+    float eps;                /* >= 0                                           */
+    int64_t row_stride;       /* of G, in elements, 0: cols                     */
+    int64_t batch_stride;
+} fg_orthogonalize_params;
+
+int fg_orthogonalize_workspace_size(const fg_orthogonalize_params* params, size_t* bytes);
+int fg_orthogonalize(const fg_orthogonalize_params* params, const void* g, void* out, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 /* Preference loss over documents of an index.  The policy of query q prefers
  * documents by softmax of the search score s (inner product, or minus squared
  * L2 distance); in the ratio of two documents of one query the normaliser

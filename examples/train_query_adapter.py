@@ -5,7 +5,10 @@ whose space is shifted against the base's, so their nearest base vectors are
 often the wrong ones; labelled (preferred, rejected) documents train a
 QueryAdapter, and the adapted queries are searched as usual:
 
-    python examples/train_query_adapter.py
+    python examples/train_query_adapter.py [--gated] [--muon] [--int8]
+
+--gated trains the gated adapter, --muon its matrices by orthogonalised updates,
+and --int8 searches with the trained adapter in 8 bits.
 """
 from __future__ import annotations
 
@@ -17,7 +20,7 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
-from fusiongpu_b200 import IVFPQIndex, QueryAdapter, SearchParams  # noqa: E402
+from fusiongpu_b200 import IVFPQIndex, Muon, QueryAdapter, SearchParams  # noqa: E402
 
 
 def hit_rate(index, queries, wanted, params) -> float:
@@ -26,7 +29,8 @@ def hit_rate(index, queries, wanted, params) -> float:
     return float((ids == wanted[:, None]).any(1).float().mean())
 
 
-def run(nbase=20000, dim=128, nq=2048, nlist=128, pq_m=32, hidden=256, steps=150, negatives=16, seed=0, verbose=True):
+def run(nbase=20000, dim=128, nq=2048, nlist=128, pq_m=32, hidden=256, steps=150, negatives=16, seed=0, verbose=True,
+        gated=False, muon=False, int8=False):
     """Returns the hit rate on held-out queries before and after training."""
     g = torch.Generator(device="cuda").manual_seed(seed)
     base = torch.nn.functional.normalize(torch.randn(nbase, dim, generator=g, device="cuda"), dim=1)
@@ -41,8 +45,9 @@ def run(nbase=20000, dim=128, nq=2048, nlist=128, pq_m=32, hidden=256, steps=150
                           ref_compat=False)
     before = hit_rate(index, queries[test], label[test], params)
 
-    adapter = QueryAdapter(dim, hidden, seed=seed)
-    opt = torch.optim.Adam(adapter.parameters(), lr=3e-3)
+    adapter = QueryAdapter(dim, hidden, seed=seed, gated=gated)
+    opts = ([Muon(adapter.matrices(), lr=0.02), torch.optim.Adam(adapter.vectors(), lr=3e-3)] if muon
+            else [torch.optim.Adam(adapter.parameters(), lr=3e-3)])
     offsets = torch.arange(nq + 1, device="cuda") * negatives
     pos = label[train].repeat_interleave(negatives)
     for step in range(steps):
@@ -54,10 +59,12 @@ def run(nbase=20000, dim=128, nq=2048, nlist=128, pq_m=32, hidden=256, steps=150
         neg = torch.where(neg == pos, -1, neg).contiguous()  # the label itself is no rejected document: masked
         losses, _ = adapter.train_step(queries[train], base, offsets, pos, neg, beta=8.0, metric="l2",
                                        weights=torch.full_like(neg, 1.0 / neg.numel(), dtype=torch.float32))
-        opt.step()
+        for opt in opts:
+            opt.step()
         if verbose and step % 25 == 0:
             print(f"step {step:4d}  loss {float(losses.mean()):.4f}")
-    after = hit_rate(index, adapter(queries[test]), label[test], params)
+    served = adapter.quantized() if int8 else adapter
+    after = hit_rate(index, served(queries[test]), label[test], params)
     if verbose:
         print(f"hit rate at 10 on held-out queries: {before:.3f} -> {after:.3f}")
     return before, after
@@ -66,4 +73,6 @@ def run(nbase=20000, dim=128, nq=2048, nlist=128, pq_m=32, hidden=256, steps=150
 if __name__ == "__main__":
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--steps", type=int, default=150)
-    run(steps=ap.parse_args().steps)
+    for flag in ("gated", "muon", "int8"):
+        ap.add_argument("--" + flag, action="store_true")
+    run(**vars(ap.parse_args()))

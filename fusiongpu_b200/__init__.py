@@ -18,7 +18,7 @@ def __getattr__(name):
                 "encode_residuals_to_pq_gpu", "sort_by_list", "recall_at"):
         from . import index
         return getattr(index, name)
-    if name in ("QueryAdapter", "layer_norm", "layer_norm_backward", "linear", "linear_backward", "gated_linear",
+    if name in ("QueryAdapter", "QuantizedQueryAdapter", "Muon", "layer_norm", "layer_norm_backward", "linear", "linear_backward", "gated_linear",
                 "gated_linear_backward", "quantize_rows", "linear_int8", "orthogonalize", "preference_loss"):
         from . import adapter
         return getattr(adapter, name)

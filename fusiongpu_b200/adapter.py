@@ -8,9 +8,13 @@ residual block
 
     adapted = q + w2 act(w1 layer_norm(q) + b1) + b2
 
-whose operators (:func:`layer_norm`, :func:`linear`, :func:`preference_loss`
-and the gradients) are the package's own sm_100a kernels behind the C ABI
-(fg_layer_norm, fg_linear, fg_preference_loss in ``include/fusiongpu.h``).
+or, gated, with act(z) * p for [z p] = w1 layer_norm(q) + b1 in the inner layer's
+place.  Its operators (:func:`layer_norm`, :func:`linear`, :func:`gated_linear`,
+:func:`preference_loss` and the gradients) are the package's own sm_100a kernels
+behind the C ABI (fg_layer_norm, fg_linear, fg_gated_linear, fg_preference_loss in
+``include/fusiongpu.h``), as are :func:`orthogonalize`, from which :class:`Muon`
+makes the matrices' updates, and :func:`quantize_rows` and :func:`linear_int8`,
+with which :meth:`QueryAdapter.quantized` serves in 8 bits.
 Tensors are CUDA tensors of float32, float16 or bfloat16; the documents may be
 uint8.  Rows may be strided; a tensor whose last dimension is not contiguous
 is copied.  Every call takes ``stream=`` (default: the current stream of its
@@ -438,7 +442,9 @@ def preference_loss(queries: torch.Tensor, base: torch.Tensor, offsets: torch.Te
 
 
 class QueryAdapter:
-    """adapted = q + w2 act(w1 layer_norm(q) + b1) + b2, trained on preferences.
+    """adapted = q + w2 act(w1 layer_norm(q) + b1) + b2, trained on preferences; with
+    gated=True the inner layer is :func:`gated_linear`, w1 [2 hidden][dim] and b1
+    [2 hidden] holding the gates' rows, then their partners'.
 
     `params` holds the tensors (norm_weight, norm_bias in float32, the others in
     `dtype`); w2 and b2 start at zero, so an untrained adapter returns its
@@ -446,24 +452,33 @@ class QueryAdapter:
     where a ``torch.optim`` optimizer over ``parameters()`` finds them."""
 
     def __init__(self, dim: int, hidden: int, activation: str = "gelu", dtype: torch.dtype = torch.float32,
-                 seed: int = 0, device="cuda"):
+                 seed: int = 0, device="cuda", gated: bool = False):
         if dtype not in DTYPES:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, not {dtype}")
         _activation(activation)
-        self.dim, self.hidden, self.activation, self.dtype = dim, hidden, activation, dtype
+        self.dim, self.hidden, self.activation, self.dtype, self.gated = dim, hidden, activation, dtype, gated
         g = torch.Generator().manual_seed(seed)
-        w1 = torch.randn(hidden, dim, generator=g) / math.sqrt(dim)
+        inner = 2 * hidden if gated else hidden
+        w1 = torch.randn(inner, dim, generator=g) / math.sqrt(dim)
         self.params = {
             "norm_weight": torch.ones(dim, device=device),
             "norm_bias": torch.zeros(dim, device=device),
             "w1": w1.to(device=device, dtype=dtype),
-            "b1": torch.zeros(hidden, device=device, dtype=dtype),
+            "b1": torch.zeros(inner, device=device, dtype=dtype),
             "w2": torch.zeros(dim, hidden, device=device, dtype=dtype),
             "b2": torch.zeros(dim, device=device, dtype=dtype),
         }
 
     def parameters(self) -> list[torch.Tensor]:
         return list(self.params.values())
+
+    def matrices(self) -> list[torch.Tensor]:
+        """The parameters that :class:`Muon` takes."""
+        return [p for p in self.params.values() if p.dim() == 2]
+
+    def vectors(self) -> list[torch.Tensor]:
+        """The others."""
+        return [p for p in self.params.values() if p.dim() != 2]
 
     def __call__(self, queries: torch.Tensor, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """The adapted queries [nq][dim], of the adapter's type: what the index
@@ -472,8 +487,12 @@ class QueryAdapter:
         with contextlib.nullcontext() if stream is None else _entered(queries.device, stream):
             q = queries.to(self.dtype)
             n = layer_norm(q, p["norm_weight"], p["norm_bias"])
-            h = linear(n, p["w1"], p["b1"], activation=self.activation)
+            h = (gated_linear if self.gated else linear)(n, p["w1"], p["b1"], activation=self.activation)
             return linear(h, p["w2"], p["b2"], residual=q)
+
+    def quantized(self) -> "QuantizedQueryAdapter":
+        """What this adapter has learned, as it is now, for serving in 8 bits."""
+        return QuantizedQueryAdapter(self)
 
     def train_step(self, queries: torch.Tensor, base: torch.Tensor, offsets: torch.Tensor, pos_ids: torch.Tensor,
                    neg_ids: torch.Tensor, beta: float = 1.0, label_smoothing: float = 0.0, metric: str = "l2",
@@ -483,14 +502,95 @@ class QueryAdapter:
         leaves the gradient of sum(weights * losses) in the parameters'
         ``grad``."""
         p = self.params
+        inner, inner_backward = (gated_linear, gated_linear_backward) if self.gated else (linear, linear_backward)
         with contextlib.nullcontext() if stream is None else _entered(queries.device, stream):
             q = queries.to(self.dtype)
             n, mean, rstd = layer_norm(q, p["norm_weight"], p["norm_bias"], return_stats=True)
-            h, z = linear(n, p["w1"], p["b1"], activation=self.activation, return_pre=True)
+            h, z = inner(n, p["w1"], p["b1"], activation=self.activation, return_pre=True)
             out = linear(h, p["w2"], p["b2"], residual=q)
             losses, margins, dout = preference_loss(out, base, offsets, pos_ids, neg_ids, ref=q, weights=weights,
                                                     beta=beta, label_smoothing=label_smoothing, metric=metric)
             dh, p["w2"].grad, p["b2"].grad = linear_backward(dout, h, p["w2"])
-            dn, p["w1"].grad, p["b1"].grad = linear_backward(dh, n, p["w1"], pre=z, activation=self.activation)
+            dn, p["w1"].grad, p["b1"].grad = inner_backward(dh, n, p["w1"], pre=z, activation=self.activation)
             _, p["norm_weight"].grad, p["norm_bias"].grad = layer_norm_backward(dn, q, mean, rstd, p["norm_weight"])
         return losses, margins
+
+
+class QuantizedQueryAdapter:
+    """A trained :class:`QueryAdapter` whose matrices are codes of 8 bits with a scale
+    per row; the rows that meet them are quantised on the way.  Layer norm, biases,
+    activations and the residual stay as they are.  Keeps copies: the adapter may be
+    trained on."""
+
+    def __init__(self, adapter: QueryAdapter):
+        p = adapter.params
+        self.dim, self.hidden, self.activation, self.dtype = adapter.dim, adapter.hidden, adapter.activation, adapter.dtype
+        self.gated = adapter.gated
+        self.params = {k: p[k].detach().clone() for k in ("norm_weight", "norm_bias", "b1", "b2")}
+        for k in ("w1", "w2"):
+            self.params[k], self.params[k + "_scale"] = quantize_rows(p[k].detach())
+
+    def _inner(self, x: torch.Tensor, x_scale: torch.Tensor, rows: slice, activation: str) -> torch.Tensor:
+        p = self.params
+        return linear_int8(x, x_scale, p["w1"][rows], p["w1_scale"][rows], p["b1"][rows], activation=activation,
+                           dtype=self.dtype)
+
+    def __call__(self, queries: torch.Tensor, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+        """The adapted queries [nq][dim], of the adapter's type."""
+        p, hid = self.params, self.hidden
+        with contextlib.nullcontext() if stream is None else _entered(queries.device, stream):
+            q = queries.to(self.dtype)
+            x, x_scale = quantize_rows(layer_norm(q, p["norm_weight"], p["norm_bias"]))
+            h = self._inner(x, x_scale, slice(0, hid), self.activation)
+            if self.gated:
+                h *= self._inner(x, x_scale, slice(hid, 2 * hid), "none")
+            h, h_scale = quantize_rows(h)
+            return linear_int8(h, h_scale, p["w2"], p["w2_scale"], p["b2"], residual=q, dtype=self.dtype)
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update of a matrix is orthogonalised (:func:`orthogonalize`):
+
+        m = momentum m + grad,   u = grad + momentum m (nesterov) or m
+        p = (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) orthogonalize(u)
+
+    for matrices on the GPU; vectors go to another optimizer.  Matrices of one shape
+    and type are orthogonalised together."""
+
+    def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+                 steps: int = 5, coefficients: tuple[float, float, float] = (3.4445, -4.7750, 2.0315), eps: float = 1e-7):
+        if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
+            raise ValueError("lr and weight_decay must not be negative, momentum must be in [0, 1)")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      coefficients=coefficients, eps=eps))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() != 2 or p.dtype not in DTYPES:
+                    raise ValueError(f"Muon takes matrices of float32, float16 or bfloat16, not {tuple(p.shape)} {p.dtype}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            alike: dict = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if "momentum" not in state:
+                    state["momentum"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                m = state["momentum"].mul_(group["momentum"]).add_(p.grad)
+                u = p.grad.add(m, alpha=group["momentum"]) if group["nesterov"] else m
+                alike.setdefault((p.shape, p.dtype, p.device), []).append((p, u))
+            for (shape, _, _), pairs in alike.items():
+                u = pairs[0][1] if len(pairs) == 1 else torch.stack([u for _, u in pairs])
+                o = orthogonalize(u, steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])
+                scale = math.sqrt(max(1.0, shape[0] / shape[1]))
+                for (p, _), x in zip(pairs, [o] if len(pairs) == 1 else o):
+                    if group["weight_decay"]:
+                        p.mul_(1 - group["lr"] * group["weight_decay"])
+                    p.add_(x, alpha=-group["lr"] * scale)
+        return loss

@@ -21,7 +21,6 @@
 namespace fg {
 
 constexpr int OT_M = 128, OT_K = 64, OT_NT = 64 + 256;
-constexpr int OT_RING = 192 * 1024;
 constexpr int LOW_SHIFT = 11;  // h + 2^-11 l
 constexpr int ORTH_RUN = 8;    // K blocks (512 k) that an accumulator sums before the next one is taken, where TMEM allows
 
@@ -36,100 +35,143 @@ __device__ __forceinline__ float value_of(__half h, __half l) {
 
 // ---- |G|_F and the first X ----------------------------------------------------------
 //
-// Squares are added in 64 bits, in an order that depends on the shape alone: a block sums
-// every ORTH_PARTS-th run of 1,024 elements, and each block of the second launch adds the
-// partial sums again.  Both are bound by memory.
-constexpr int ORTH_PARTS = 128, OI_NT = 256, OI_RUN = 1024;
+// Squares are added in 64 bits, in an order that depends on the shape alone: a warp takes
+// runs of OI_COLS columns of a row, every so many of them; the blocks of the second
+// launch add the blocks' sums again.  Both are bound by memory.
+constexpr int ORTH_PARTS = 592, OI_NT = 256, OI_WARPS = OI_NT / 32, OI_COLS = 1024;
 
 struct OrthIn {
     const void* g;
     double* part;  // [batch][ORTH_PARTS]
-    __half* x;     // planes [2][batch][rows][ld]; NULL: `out` instead
+    __half* x;     // [batch][2 planes][rows][ld]; NULL: `out` instead
     void* out;
-    long long rows, row_stride, batch_stride, ld;
-    int cols, batch, parts;
+    long long row_stride, batch_stride, ld;
+    int rows, cols, batch, parts, runs;  // runs of a row
+    int wide;                            // G's rows start on 16 bytes
     float eps;
 };
 
+// VEC elements of a row from column c on, zeros behind its end.
+template <class T, int VEC>
+__device__ __forceinline__ void orth_load(T (&v)[VEC], const T* row, int c, int cols, int wide) {
+    if (wide && c + VEC <= cols) {
+        *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(row + c);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = c + i < cols ? row[c + i] : from_f32<T>(0.0f);
+    }
+}
+
 template <class T>
 __global__ void __launch_bounds__(OI_NT) orth_norm_kernel(const OrthIn g) {
-    __shared__ double s[OI_NT / 32];
+    constexpr int VEC = 16 / sizeof(T);
+    __shared__ double s[OI_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const T* p = static_cast<const T*>(g.g) + blockIdx.y * g.batch_stride;
-    const long long n = g.rows * g.cols;
+    const int items = g.rows * g.runs;  // at most 2^15 rows of 32 runs
     double sum = 0.0;
-    for (long long r = (long long)blockIdx.x * OI_RUN; r < n; r += (long long)g.parts * OI_RUN) {
+    for (int i = blockIdx.x * OI_WARPS + warp; i < items; i += g.parts * OI_WARPS) {
+        const int row = i / g.runs, c0 = (i - row * g.runs) * OI_COLS, c1 = min(c0 + OI_COLS, g.cols);
+        const T* r = p + row * g.row_stride;
+#pragma unroll 4
+        for (int c = c0 + lane * VEC; c < c1; c += 32 * VEC) {
+            alignas(16) T v[VEC];
+            orth_load<T, VEC>(v, r, c, c1, g.wide);
 #pragma unroll
-        for (int k = 0; k < OI_RUN / OI_NT; ++k) {
-            const long long i = r + k * OI_NT + threadIdx.x;
-            if (i < n) {
-                const long long row = i / g.cols;
-                const double v = (double)to_f32(p[row * g.row_stride + (i - row * g.cols)]);
-                sum = fma(v, v, sum);
+            for (int j = 0; j < VEC; ++j) {
+                const double d = (double)to_f32(v[j]);
+                sum = fma(d, d, sum);
             }
         }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = sum;
+    if (lane == 0) s[warp] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < OI_NT / 32; ++w) sum += s[w];
+        for (int w = 1; w < OI_WARPS; ++w) sum += s[w];
         g.part[blockIdx.y * ORTH_PARTS + blockIdx.x] = sum;
     }
 }
 
 template <class T>
 __global__ void __launch_bounds__(OI_NT) orth_scale_kernel(const OrthIn g) {
-    __shared__ double s;
-    if (threadIdx.x < 32) {
-        double sum = 0.0;
-        for (int i = threadIdx.x; i < g.parts; i += 32) sum += g.part[blockIdx.y * ORTH_PARTS + i];
+    constexpr int VEC = 8;  // of a plane's 16 bytes
+    constexpr int IN = 16 / sizeof(T);
+    __shared__ double s[OI_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < g.parts; i += OI_NT) sum += g.part[blockIdx.y * ORTH_PARTS + i];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (threadIdx.x == 0) s = 1.0 / (sqrt(sum) + (double)g.eps);
-    }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s[warp] = sum;
     __syncthreads();
-    const double inv = s;
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < OI_WARPS; ++w) sum += s[w];
+    const double inv = 1.0 / (sqrt(sum) + (double)g.eps);
     const T* p = static_cast<const T*>(g.g) + blockIdx.y * g.batch_stride;
-    const long long plane = (long long)g.batch * g.rows * g.ld;
-    for (long long i = blockIdx.x * (long long)OI_NT + threadIdx.x; i < g.rows * g.ld; i += (long long)gridDim.x * OI_NT) {
-        const long long row = i / g.ld;
-        const int col = (int)(i - row * g.ld);
-        const float v = col < g.cols ? (float)((double)to_f32(p[row * g.row_stride + col]) * inv) : 0.0f;
-        if (g.x) {
-            __half h, l;
-            planes_of(v, h, l);
-            __half* x = g.x + blockIdx.y * g.rows * g.ld + i;
-            x[0] = h;
-            x[plane] = l;
-        } else if (col < g.cols) {
-            static_cast<T*>(g.out)[(blockIdx.y * g.rows + row) * g.cols + col] = from_f32<T>(v);
+    const long long plane = g.rows * g.ld;
+    const int items = g.rows * g.runs;
+    for (int i = blockIdx.x * OI_WARPS + warp; i < items; i += gridDim.x * OI_WARPS) {
+        const int row = i / g.runs, c0 = (i - row * g.runs) * OI_COLS, c1 = min(c0 + OI_COLS, g.cols);
+        const T* r = p + row * g.row_stride;
+        for (int c = c0 + lane * VEC; c < c1; c += 32 * VEC) {
+            alignas(16) T v[VEC / IN][IN];
+#pragma unroll
+            for (int k = 0; k < VEC / IN; ++k) orth_load<T, IN>(v[k], r, c + k * IN, c1, g.wide);
+            float f[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = (float)((double)to_f32(v[j / IN][j % IN]) * inv);
+            if (g.x) {
+                alignas(16) __half h[VEC], l[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) planes_of(f[j], h[j], l[j]);
+                __half* x = g.x + 2 * blockIdx.y * plane + row * g.ld + c;
+                *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(h);
+                *reinterpret_cast<uint4*>(x + plane) = *reinterpret_cast<const uint4*>(l);
+            } else {
+                T* o = static_cast<T*>(g.out) + ((long long)blockIdx.y * g.rows + row) * g.cols + c;
+                for (int j = 0; j < VEC; ++j)
+                    if (c + j < c1) o[j] = from_f32<T>(f[j]);
+            }
         }
     }
 }
 
 // ---- products ------------------------------------------------------------------------
 //
-// D(m, n) = alpha C(m, n) + beta (sum over k of P(m, k) Q(n, k)): a 128 x BN tile a
+// D(m, n) = beta (sum over k of P(m, k) Q(n, k)) + alpha C(m, n), and `diag` where m = n.  A 128 x BN tile a
 // cluster, its K blocks divided over the cluster's CTAs, partial tiles added through
-// distributed shared memory, as the linear layer's products of few tiles are.
+// distributed shared memory.  A stage of the ring holds both planes of both operands for
+// 64 k, which three products share: h h' into one accumulator, h l' and l h' into
+// another, that counts 2^-11 of it.
+//
+// SYM: D is symmetric.  Tiles above the diagonal are left out; an element below it is
+// written to both its places.
+//
+// The products of one call follow one another by a few microseconds each, so a kernel
+// starts while the one before it ends (griddepcontrol): barriers, tensor memory and
+// tensor maps are ready when that one's results are.
 struct OrthArgs {
-    int kt, mt, nt, m, n;
-    int p_mn, q_mn;       // the operand's unit stride is along its rows
-    int split, batch;
-    float alpha, beta;
-    const __half* c;      // planes, NULL: none
-    __half* d;            // planes, NULL: `out`
-    void* out;
-    long long ldc, ldd, ldo;       // row strides
-    long long c_plane, d_plane;    // from a plane to the next; a matrix to the next: m * ld
+    int kt, mt, nt, m, n, tiles;  // tiles of a matrix
+    int p_mn, q_mn;               // the operand's unit stride is along its rows
+    int split;
+    int sym, vec;                 // vec: `out` allows 4-column stores
+    float alpha, beta, diag;
+    const __half* c;              // NULL: none
+    __half* d;                    // NULL: `out`
+    void* out;                    // [batch][m][n]
+    long long ldc, ldd;
     uint32_t idesc;
 };
 
 template <int BN>
 struct OrthRing {
-    static constexpr int A = OT_M * OT_K * 2, B = BN * OT_K * 2, STAGE = A + B;
-    static constexpr int N = OT_RING / STAGE > 8 ? 8 : OT_RING / STAGE;
+    static constexpr int A = 2 * OT_M * OT_K * 2, B = 2 * BN * OT_K * 2, STAGE = A + B;
+    static constexpr int N = BN == 64 ? 2 : BN == 128 ? 3 : 2;   // 64: two blocks to an SM
+    static constexpr int HIGH = BN == 64 ? 3 : 1, COLS = BN == 256 ? 512 : 256;  // accumulators of h h', columns of TMEM
+    static_assert((HIGH + 1) * BN <= COLS, "accumulators fit");
 };
 
 __device__ __forceinline__ uint32_t orth_rank() {
@@ -152,15 +194,11 @@ __device__ __forceinline__ float4 orth_peer(uint32_t a, uint32_t rank) {
     return v;
 }
 
-// Planes of the i-th of three plane products: l h, h l, h h.
-__device__ __forceinline__ int orth_plane_p(int i) { return i == 0; }
-__device__ __forceinline__ int orth_plane_q(int i) { return i == 1; }
-
 template <class T, int BN>
-__global__ void __launch_bounds__(OT_NT, 1)
+__global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
     orth_product_kernel(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMap tq, const __grid_constant__ OrthArgs g) {
     using Ring = OrthRing<BN>;
-    constexpr int LDP = BN + 4, NA = 512 / BN;
+    constexpr int LDP = BN + 4;
     static_assert(OT_M * LDP * 4 <= Ring::N * Ring::STAGE, "the partial tile fits the ring");
     extern __shared__ __align__(1024) unsigned char dsmem[];
     __shared__ __align__(8) uint64_t full[Ring::N], empty[Ring::N], acc_full;
@@ -171,10 +209,17 @@ __global__ void __launch_bounds__(OT_NT, 1)
         (reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
     float* part = reinterpret_cast<float*>(ring);
     const int S = g.split, rank = S > 1 ? (int)orth_rank() : 0;
-    const int tile = (int)(blockIdx.x / (unsigned)S), b = tile / (g.mt * g.nt), t = tile - b * (g.mt * g.nt);
-    const int m0 = t / g.nt * OT_M, n0 = t % g.nt * BN;
+    const int tile = (int)(blockIdx.x / (unsigned)S), b = tile / g.tiles;
+    int t = tile - b * g.tiles, mi = 0;
+    if (g.sym) {  // row tiles hold the column tiles up to the diagonal
+        for (int in_row; t >= (in_row = min(g.nt, ((mi + 1) * OT_M + BN - 1) / BN)); ++mi) t -= in_row;
+    } else {
+        mi = t / g.nt;
+        t -= mi * g.nt;
+    }
+    const int m0 = mi * OT_M, n0 = t * BN;
     const int kb0 = (int)((long long)g.kt * rank / S), kb1 = (int)((long long)g.kt * (rank + 1) / S);
-    const int share = max(ORTH_RUN, (kb1 - kb0 + NA - 1) / NA), shares = (kb1 - kb0 + share - 1) / share;
+    const int share = max(ORTH_RUN, (kb1 - kb0 + Ring::HIGH - 1) / Ring::HIGH), shares = (kb1 - kb0 + share - 1) / share;
 
     if (warp == 2 && tc::elect_one()) {
         tc::prefetch_map(&tp);
@@ -190,7 +235,7 @@ __global__ void __launch_bounds__(OT_NT, 1)
         tc::fence_mbar_init();
     }
     if (warp == 1) {
-        tc::tmem_alloc(&tmem_slot, 512);
+        tc::tmem_alloc(&tmem_slot, Ring::COLS);
         tc::tmem_relinquish();
     }
     tc::fence_before_sync();
@@ -198,77 +243,80 @@ __global__ void __launch_bounds__(OT_NT, 1)
     tc::fence_after_sync();
     const uint32_t taddr = tmem_slot;
     volatile int* fail = &s_fail;
+    // the next kernel's blocks may come: this block holds its tensor memory
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the last kernel's results are in memory
 
     if (warp == 0) {
         if (tc::elect_one()) {  // ---- TMA producer
-            int i = 0;
+            asm volatile("fence.proxy.async.global;" ::: "memory");  // operands written by ordinary stores
             bool ok = true;
-            for (int c0 = kb0; c0 < kb1 && ok; c0 += share)
-                for (int q = 0; q < 3 && ok; ++q)
-                    for (int kb = c0; kb < min(c0 + share, kb1); ++kb) {
-                        const int st = i % Ring::N, k = kb * OT_K;
-                        ok = tc::mbar_wait_or_fail(&empty[st], ((i / Ring::N) & 1) ^ 1, fail);
-                        if (!ok) break;
-                        unsigned char *sa = ring + st * Ring::STAGE, *sb = sa + Ring::A;
-                        tc::mbar_arrive_expect_tx(&full[st], Ring::STAGE);
-                        const int zp = orth_plane_p(q) * g.batch + b, zq = orth_plane_q(q) * g.batch + b;
-                        if (g.p_mn) {
-                            for (int c = 0; c < OT_M / 64; ++c) tc::tma_load_3d(sa + c * 8192, &tp, &full[st], m0 + c * 64, k, zp);
-                        } else {
-                            tc::tma_load_3d(sa, &tp, &full[st], k, m0, zp);
-                        }
-                        if (g.q_mn) {
-                            for (int c = 0; c < BN / 64; ++c) tc::tma_load_3d(sb + c * 8192, &tq, &full[st], n0 + c * 64, k, zq);
-                        } else {
-                            tc::tma_load_3d(sb, &tq, &full[st], k, n0, zq);
-                        }
-                        ++i;
-                    }
+            int i = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++i) {
+                const int st = i % Ring::N, k = kb * OT_K;
+                ok = tc::mbar_wait_or_fail(&empty[st], ((i / Ring::N) & 1) ^ 1, fail);
+                if (!ok) break;
+                unsigned char *sa = ring + st * Ring::STAGE, *sb = sa + Ring::A;
+                tc::mbar_arrive_expect_tx(&full[st], Ring::STAGE);
+                if (g.p_mn) {
+                    for (int c = 0; c < OT_M / 64; ++c) tc::tma_load_3d(sa + c * 16384, &tp, &full[st], m0 + c * 64, k, 2 * b);
+                } else {
+                    tc::tma_load_3d(sa, &tp, &full[st], k, m0, 2 * b);
+                }
+                if (g.q_mn) {
+                    for (int c = 0; c < BN / 64; ++c) tc::tma_load_3d(sb + c * 16384, &tq, &full[st], n0 + c * 64, k, 2 * b);
+                } else {
+                    tc::tma_load_3d(sb, &tq, &full[st], k, n0, 2 * b);
+                }
+            }
             if (!ok)  // copies in flight land before the block ends
                 for (int j = i > Ring::N ? i - Ring::N : 0; j < i; ++j) tc::mbar_wait(&full[j % Ring::N], (j / Ring::N) & 1);
         }
     } else if (warp == 1) {
         // ---- MMA issuer: the warp stays together, one elected lane issues
         bool ok = true;
-        int i = 0;
-        const uint64_t da0 = g.p_mn ? tc::desc_mnmajor_sw128(ring, 8192) : tc::desc_kmajor_sw128(ring);
-        const uint64_t db0 = g.q_mn ? tc::desc_mnmajor_sw128(ring + Ring::A, 8192) : tc::desc_kmajor_sw128(ring + Ring::A);
-        const uint32_t ka = g.p_mn ? 128 : 2, kbs = g.q_mn ? 128 : 2;  // 16 k, in 16-byte units
-        for (int c0 = kb0, acc = 0; c0 < kb1 && ok; c0 += share, ++acc) {
-            const int n = (min(c0 + share, kb1) - c0) * 3;
-            for (int u = 0; u < n; ++u, ++i) {
-                const int st = i % Ring::N;
-                ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&full[st], (i / Ring::N) & 1, fail));
-                if (!ok) break;
-                tc::fence_after_sync();
-                const uint64_t da = da0 + st * (Ring::STAGE / 16), db = db0 + st * (Ring::STAGE / 16);
-                if (tc::elect_one()) {
+        // planes lie one behind the other: whole (K-major), or in each chunk of 64 rows
+        const uint32_t pa = (g.p_mn ? 8192 : OT_M * 128) / 16, pb = (g.q_mn ? 8192 : BN * 128) / 16;
+        const uint64_t da0 = g.p_mn ? tc::desc_mnmajor_sw128(ring, 16384) : tc::desc_kmajor_sw128(ring);
+        const uint64_t db0 = g.q_mn ? tc::desc_mnmajor_sw128(ring + Ring::A, 16384) : tc::desc_kmajor_sw128(ring + Ring::A);
+        const uint32_t ka = g.p_mn ? 128 : 2, kq = g.q_mn ? 128 : 2;  // 16 k, in 16-byte units
+        for (int kb = kb0, i = 0; kb < kb1; ++kb, ++i) {
+            const int st = i % Ring::N;
+            ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&full[st], (i / Ring::N) & 1, fail));
+            if (!ok) break;
+            tc::fence_after_sync();
+            const uint64_t da = da0 + st * (Ring::STAGE / 16), db = db0 + st * (Ring::STAGE / 16);
+            const uint32_t high = taddr + (uint32_t)((1 + i / share) * BN);
+            if (tc::elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < OT_K / 16; ++kk) {
-                        const uint32_t d = taddr + (uint32_t)(acc * BN);
-                        if (kk == 0 && 3 * u == 2 * n)  // the products of l are done: on to h h
-                            tc::umma_shifted<LOW_SHIFT>(d, da, db, g.idesc);
-                        else
-                            tc::umma_bf16(d, da + ka * kk, db + kbs * kk, g.idesc, (u | kk) != 0);
-                    }
-                    tc::umma_commit(&empty[st]);
-                    if (u + 1 == n && c0 + share >= kb1) tc::umma_commit(&acc_full);
+                for (int kk = 0; kk < OT_K / 16; ++kk) {
+                    const uint64_t a = da + ka * kk, q = db + kq * kk;
+                    tc::umma_bf16(high, a, q, g.idesc, (i % share | kk) != 0);
+                    tc::umma_bf16(taddr, a, q + pb, g.idesc, (i | kk) != 0);
+                    tc::umma_bf16(taddr, a + pa, q, g.idesc, 1);
                 }
-                __syncwarp();
+                tc::umma_commit(&empty[st]);
+                if (kb + 1 == kb1) tc::umma_commit(&acc_full);
             }
+            __syncwarp();
         }
     } else {  // ---- epilogue warps: TMEM -> partial tile in shared memory
         const int q4 = warp & 3, half = (warp - 2) >> 2;
         const bool ok = tc::mbar_wait_warp(&acc_full, 0, fail);
         tc::fence_after_sync();
         float* row = part + (q4 * 32 + lane) * LDP;
+        const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16);
 #pragma unroll 1
         for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-            float v[32];
-            tc::tmem_ld_32x32(taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)c, v);
+            float v[32], x[32];
+            tc::tmem_ld_32x32_nowait(src + (uint32_t)(BN + c), v);
+            tc::tmem_ld_32x32_nowait(src + (uint32_t)c, x);
+            tc::tmem_ld_wait(v);
+            tc::tmem_ld_wait(x);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = fmaf(x[j], 1.0f / (1 << LOW_SHIFT), v[j]);
             for (int a = 1; a < shares; ++a) {
-                float x[32];
-                tc::tmem_ld_32x32(taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(a * BN + c), x);
+                tc::tmem_ld_32x32(src + (uint32_t)((1 + a) * BN + c), x);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] += x[j];
             }
@@ -283,47 +331,126 @@ __global__ void __launch_bounds__(OT_NT, 1)
     if (S > 1) orth_cluster_sync();
     if (warp == 1) {
         tc::fence_after_sync();
-        tc::tmem_dealloc(taddr, 512);
+        tc::tmem_dealloc(taddr, Ring::COLS);
     }
 
-    const int slice = BN / S, per_row = slice / 4;
+    // Two positions of four columns per thread and round, what they read asked for first: one
+    // latency a round.
+    constexpr int U = 2;
+    constexpr int LDT = OT_M + 1;  // SYM: the slice transposed, h and l of an element in one word
+    uint32_t* turned = reinterpret_cast<uint32_t*>(part + OT_M * LDP);
+    const int slice = BN / S, shift = __ffs(slice) - 3;  // columns, and the logarithm of a row's positions
     const uint32_t pbase = tc::smem_u32(part);
-    for (int i = tid; i < OT_M * per_row; i += OT_NT) {
-        const int r = i / per_row, cc = rank * slice + (i - r * per_row) * 4, row = m0 + r, col = n0 + cc;
-        if (row >= g.m || col >= g.n) continue;
-        const uint32_t at = (uint32_t)(r * LDP + cc) * 4;
-        // planes have rows of a multiple of 8 elements, zeros past the last column
-        alignas(8) __half ch[4], cl[4];
-        if (g.c) {
-            const __half* p = g.c + ((long long)b * g.m + row) * g.ldc + col;
-            *reinterpret_cast<uint2*>(ch) = *reinterpret_cast<const uint2*>(p);
-            *reinterpret_cast<uint2*>(cl) = *reinterpret_cast<const uint2*>(p + g.c_plane);
-        }
-        float4 z = S > 1 ? orth_peer(pbase + at, rank) : *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(part) + at);
-        for (int s = 1; s < S; ++s) {
-            const float4 v = orth_peer(pbase + at, (rank + s) & (S - 1));
-            z.x += v.x;
-            z.y += v.y;
-            z.z += v.z;
-            z.w += v.w;
-        }
-        float v[4] = {z.x * g.beta, z.y * g.beta, z.z * g.beta, z.w * g.beta};
-        if (g.c) {
+    const long long c_plane = g.m * g.ldc, d_plane = g.m * g.ldd;
+    for (int i0 = tid; i0 < OT_M << shift; i0 += U * OT_NT) {
+        int r[U], cc[U];
+        bool in[U];
+        float4 z[U];
+        uint2 ch[U], cl[U];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = fmaf(g.alpha, value_of(ch[j], cl[j]), v[j]);
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * OT_NT;
+            r[u] = i >> shift;
+            cc[u] = rank * slice + (i - (r[u] << shift)) * 4;
+            in[u] = r[u] < OT_M && m0 + r[u] < g.m && n0 + cc[u] < g.n;
+            if (!in[u]) continue;
+            const uint32_t at = (uint32_t)(r[u] * LDP + cc[u]) * 4;
+            if (g.c) {  // rows hold a multiple of 8 elements
+                const __half* p = g.c + 2 * b * c_plane + (m0 + r[u]) * g.ldc + n0 + cc[u];
+                ch[u] = *reinterpret_cast<const uint2*>(p);
+                cl[u] = *reinterpret_cast<const uint2*>(p + c_plane);
+            }
+            z[u] = *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(part) + at);
         }
-        if (g.d) {
-            alignas(8) __half h[4], l[4];
+        for (int s0 = 1; s0 < S; s0 += 3) {  // three peers' at a time, this block's own is there
+            float4 x[U][3];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) planes_of(col + j < g.n ? v[j] : 0.0f, h[j], l[j]);
-            __half* p = g.d + ((long long)b * g.m + row) * g.ldd + col;
-            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
-            *reinterpret_cast<uint2*>(p + g.d_plane) = *reinterpret_cast<const uint2*>(l);
-        } else {
-            T* p = static_cast<T*>(g.out) + ((long long)b * g.m + row) * g.ldo + col;
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col + j < g.n) p[j] = from_f32<T>(v[j]);
+                for (int s = 0; s < 3; ++s)
+                    if (in[u] && s0 + s < S) x[u][s] = orth_peer(pbase + (uint32_t)(r[u] * LDP + cc[u]) * 4, (rank + s0 + s) & (S - 1));
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int s = 0; s < 3; ++s)
+                    if (in[u] && s0 + s < S) {
+                        z[u].x += x[u][s].x;
+                        z[u].y += x[u][s].y;
+                        z[u].z += x[u][s].z;
+                        z[u].w += x[u][s].w;
+                    }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (!in[u]) continue;
+            const int row = m0 + r[u], col = n0 + cc[u];
+            float v[4] = {z[u].x * g.beta, z[u].y * g.beta, z[u].z * g.beta, z[u].w * g.beta};
+            if (g.c) {
+                const __half *h = reinterpret_cast<const __half*>(&ch[u]), *l = reinterpret_cast<const __half*>(&cl[u]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = fmaf(g.alpha, value_of(h[j], l[j]), v[j]);
+            }
+            if (g.sym) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col + j == row) v[j] += g.diag;
+            }
+            if (g.d) {
+                alignas(8) __half h[4], l[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) planes_of(v[j], h[j], l[j]);
+                __half* p = g.d + 2 * b * d_plane + row * g.ldd + col;
+                if (!g.sym || col + 3 <= row) {  // elements past the last column lie in the row's padding
+                    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
+                    *reinterpret_cast<uint2*>(p + d_plane) = *reinterpret_cast<const uint2*>(l);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j <= row) {
+                            p[j] = h[j];
+                            p[d_plane + j] = l[j];
+                        }
+                }
+                if (BN < 256 && g.sym) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        turned[(cc[u] - rank * slice + j) * LDT + r[u]] =
+                            (uint32_t)__half_as_ushort(h[j]) | (uint32_t)__half_as_ushort(l[j]) << 16;
+                }
+            } else {
+                T* p = static_cast<T*>(g.out) + ((long long)b * g.m + row) * g.n + col;
+                if (g.vec) {
+                    alignas(16) T o[4] = {from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
+                    if constexpr (sizeof(T) == 4)
+                        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(o);
+                    else
+                        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(o);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j < g.n) p[j] = from_f32<T>(v[j]);
+                }
+            }
+        }
+    }
+    if (BN < 256 && g.sym) {  // a lane takes two rows, which become neighbouring columns
+        static_assert(BN == 256 || (OT_M * LDP + BN * LDT) * 4 <= Ring::N * Ring::STAGE, "the transposed tile fits behind the partial one");
+        __syncthreads();
+        for (int i = tid; i < slice * (OT_M / 2); i += OT_NT) {
+            const int c = i / (OT_M / 2), r = i % (OT_M / 2) * 2, row = m0 + r, col = n0 + rank * slice + c;
+            if (col > row || row >= g.m) continue;  // of a pair on the diagonal the second one counts
+            const uint32_t x = turned[c * LDT + r], y = turned[c * LDT + r + 1];
+            __half* p = g.d + 2 * b * d_plane + col * g.ldd + row;
+            if (col < row && row + 1 < g.m) {
+                *reinterpret_cast<uint32_t*>(p) = __byte_perm(x, y, 0x5410);
+                *reinterpret_cast<uint32_t*>(p + d_plane) = __byte_perm(x, y, 0x7632);
+            } else if (col < row) {
+                p[0] = __ushort_as_half((unsigned short)x);
+                p[d_plane] = __ushort_as_half((unsigned short)(x >> 16));
+            } else if (row + 1 < g.m) {
+                p[1] = __ushort_as_half((unsigned short)y);
+                p[d_plane + 1] = __ushort_as_half((unsigned short)(y >> 16));
+            }
         }
     }
     if (S > 1) orth_cluster_sync();  // a peer may still read this CTA's partial tile
@@ -331,14 +458,14 @@ __global__ void __launch_bounds__(OT_NT, 1)
 
 // ---- host side -----------------------------------------------------------------------
 
-// Planes [2][batch][rows][ld] as an operand of `lead` rows, its k along the memory's rows
-// (lead == rows) or across them (mn).
+// Matrices [batch][2 planes][rows][ld] as an operand: boxes of 64 columns of memory, both
+// planes; mn: its k runs across the rows.
 static int orth_map(CUtensorMap* m, const __half* p, int batch, long long rows, int cols, long long ld, bool mn, int box_rows) {
     tc::EncodeTiledFn enc = tc::encode_fn();
     if (!enc) return fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch * 2};
     cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(rows * ld) * 2};
-    cuuint32_t box[3] = {64, (cuuint32_t)(mn ? OT_K : box_rows), 1};
+    cuuint32_t box[3] = {64, (cuuint32_t)(mn ? OT_K : box_rows), 2};
     cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(p), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -351,18 +478,28 @@ struct OrthPlan {
     int bn, split;
 };
 
-// The tile width and split that finish first by the linear layer's estimate for products
-// of few tiles (microseconds; three products a K block).
-static OrthPlan orth_plan(long long m, long long n, long long k, int batch) {
+static long long orth_tiles(long long m, long long n, int bn, bool sym) {
+    const long long mt = (m + OT_M - 1) / OT_M, nt = (n + bn - 1) / bn;
+    if (!sym) return mt * nt;
+    long long t = 0;
+    for (long long i = 0; i < mt; ++i) t += std::min(nt, ((i + 1) * OT_M + bn - 1) / bn);
+    return t;
+}
+
+// Symmetric products take tiles of up to 128 columns (their transposed copy fits).
+// The tile width and split that finish first by this estimate, in microseconds.
+static OrthPlan orth_plan(long long m, long long n, long long k, int batch, bool sym) {
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount)), kb = (int)((k + OT_K - 1) / OT_K);
     OrthPlan best{128, 1};
     double least = 1e300;
     for (int bn : {256, 128, 64}) {
-        const long long tiles = (m + OT_M - 1) / OT_M * ((n + bn - 1) / bn) * batch;
+        if (sym && bn == 256) continue;
+        const long long tiles = orth_tiles(m, n, bn, sym) * batch;
         for (int sp : {1, 2, 4, 8}) {
             if (sp > kb) break;
-            const int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
-            const double main = (kb + sp - 1) / sp * 3 * (bn == 256 ? 0.43 : bn == 128 ? 0.30 : 0.21);
+            int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
+            if (bn == 64) slots *= 2;
+            const double main = (kb + sp - 1) / sp * (bn == 256 ? 0.85 : bn == 128 ? 0.6 : 0.45);
             const double cost = (double)((tiles + slots - 1) / slots) * (main + 2.0 + 0.02 * bn / sp) + (sp == 8 ? 0.7 : 0.0);
             if (cost < least) {
                 least = cost;
@@ -382,18 +519,19 @@ struct OrthOperand {
 };
 
 template <class T, int BN>
-static int launch_product(const OrthOperand& p, const OrthOperand& q, OrthArgs g, cudaStream_t s) {
+static int launch_product(const OrthOperand& p, const OrthOperand& q, OrthArgs g, int batch, cudaStream_t s) {
     CUtensorMap tp, tq;
-    int rc = orth_map(&tp, p.p, g.batch, p.rows, p.cols, p.ld, p.mn, OT_M);
-    if (!rc) rc = orth_map(&tq, q.p, g.batch, q.rows, q.cols, q.ld, q.mn, BN);
+    int rc = orth_map(&tp, p.p, batch, p.rows, p.cols, p.ld, p.mn, OT_M);
+    if (!rc) rc = orth_map(&tq, q.p, batch, q.rows, q.cols, q.ld, q.mn, BN);
     if (rc) return rc;
     g.p_mn = p.mn;
     g.q_mn = q.mn;
     g.mt = (g.m + OT_M - 1) / OT_M;
     g.nt = (g.n + BN - 1) / BN;
+    g.tiles = (int)orth_tiles(g.m, g.n, BN, g.sym);
     // kind::f16: f16 operands, f32 accumulators
     g.idesc = (1u << 4) | ((uint32_t)p.mn << 15) | ((uint32_t)q.mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(OT_M >> 4) << 24);
-    const long long ctas = (long long)g.mt * g.nt * g.batch * g.split;
+    const long long ctas = (long long)g.tiles * batch * g.split;
     FG_REQUIRE(ctas <= 0x7fffffffll, "too many tiles");
     auto kernel = &orth_product_kernel<T, BN>;
     const int smem = OrthRing<BN>::N * OrthRing<BN>::STAGE + 1024;
@@ -403,24 +541,26 @@ static int launch_product(const OrthOperand& p, const OrthOperand& q, OrthArgs g
     cfg.blockDim = dim3(OT_NT);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = g.split;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tp, tq, g));
     return FG_OK;
 }
 
 template <class T>
-static int product(const OrthOperand& p, const OrthOperand& q, OrthArgs g, long long k, cudaStream_t s) {
-    const OrthPlan plan = orth_plan(g.m, g.n, k, g.batch);
+static int product(const OrthOperand& p, const OrthOperand& q, OrthArgs g, long long k, int batch, cudaStream_t s) {
+    const OrthPlan plan = orth_plan(g.m, g.n, k, batch, g.sym);
     g.split = plan.split;
     g.kt = (int)((k + OT_K - 1) / OT_K);
-    return plan.bn == 256   ? launch_product<T, 256>(p, q, g, s)
-           : plan.bn == 128 ? launch_product<T, 128>(p, q, g, s)
-                            : launch_product<T, 64>(p, q, g, s);
+    return plan.bn == 256   ? launch_product<T, 256>(p, q, g, batch, s)
+           : plan.bn == 128 ? launch_product<T, 128>(p, q, g, batch, s)
+                            : launch_product<T, 64>(p, q, g, batch, s);
 }
 
 struct OrthWs {
@@ -463,7 +603,7 @@ static int orth_check(const fg_orthogonalize_params* p) {
 template <class T>
 static int orthogonalize(const fg_orthogonalize_params* p, const void* g, void* out, const OrthWs& w, cudaStream_t s) {
     const int rows = p->rows, cols = p->cols, batch = p->batch, side = std::min(rows, cols), far = std::max(rows, cols);
-    const long long ldx = orth_ld(cols), lda = orth_ld(side), n = (long long)rows * cols;
+    const long long ldx = orth_ld(cols), lda = orth_ld(side);
     OrthIn in{};
     in.g = g;
     in.part = w.part;
@@ -476,51 +616,55 @@ static int orthogonalize(const fg_orthogonalize_params* p, const void* g, void* 
     in.ld = ldx;
     in.batch = batch;
     in.eps = p->eps;
-    in.parts = (int)std::min<long long>(ORTH_PARTS, (n + OI_RUN - 1) / OI_RUN);
+    in.runs = (cols + OI_COLS - 1) / OI_COLS;
+    in.parts = (int)std::min<long long>(ORTH_PARTS, ((long long)rows * in.runs + OI_WARPS - 1) / OI_WARPS);
+    const int es = sizeof(T);
+    in.wide = aligned(g, 16) && in.row_stride * es % 16 == 0 && (batch == 1 || in.batch_stride * es % 16 == 0);
     orth_norm_kernel<T><<<dim3(in.parts, batch), OI_NT, 0, s>>>(in);
     int rc = check_launch("orth_norm_kernel");
     if (rc) return rc;
-    const int blocks = (int)std::min<long long>((rows * ldx + OI_NT - 1) / OI_NT, 1024);
-    orth_scale_kernel<T><<<dim3(blocks, batch), OI_NT, 0, s>>>(in);
+    orth_scale_kernel<T><<<dim3(in.parts, batch), OI_NT, 0, s>>>(in);
     if ((rc = check_launch("orth_scale_kernel"))) return rc;
     const bool tall = rows > cols;
-    const long long x_plane = (long long)batch * rows * ldx, a_plane = (long long)batch * side * lda;
     for (int k = 0; k < p->steps; ++k) {
         const __half* x = w.x[k & 1];
         const bool last = k + 1 == p->steps;
-        OrthArgs a{};  // A = X X^T
+        // a X + (b A + c A^2) X = Y X with Y = a I + b A + c A^2 = c M^2 + (a - b^2 / 4c) I, M = A +
+        // b / 2c I: neither product reads an addend.  Where b / 2c is large, M^2 would lose what
+        // A^2 is, and A is added as it is; without c, Y comes from the first product.
+        const float ca = p->a, cb = p->b, cc = p->c;
+        const bool square = cc != 0.0f && fabsf(cb) <= 8.0f * fabsf(cc);
+        OrthArgs a{};  // M, A or Y of X X^T
         a.m = a.n = side;
-        a.batch = batch;
-        a.beta = 1.0f;
+        a.sym = 1;
+        a.beta = cc == 0.0f ? cb : 1.0f;
+        a.diag = cc == 0.0f ? ca : square ? cb / (2.0f * cc) : 0.0f;
         a.d = w.a;
         a.ldd = lda;
-        a.d_plane = a_plane;
         const OrthOperand xs{x, rows, cols, ldx, tall};
-        if ((rc = product<T>(xs, xs, a, far, s))) return rc;
-        a.alpha = p->b;  // B = b A + c A A
-        a.beta = p->c;
-        a.c = w.a;
-        a.ldc = lda;
-        a.c_plane = a_plane;
-        a.d = w.b;
-        const OrthOperand as{w.a, side, side, lda, false}, bs{w.b, side, side, lda, false};
-        if ((rc = product<T>(as, as, a, side, s))) return rc;
-        OrthArgs d{};  // X = a X + B X, or a X + X B
+        if ((rc = product<T>(xs, xs, a, far, batch, s))) return rc;
+        const OrthOperand as{w.a, side, side, lda, false}, bs{cc == 0.0f ? w.a : w.b, side, side, lda, false};
+        if (cc != 0.0f) {
+            a.beta = cc;
+            a.diag = square ? (float)((double)ca - (double)cb * cb / (4.0 * cc)) : ca;
+            if (!square) {
+                a.alpha = cb;
+                a.c = w.a;
+                a.ldc = lda;
+            }
+            a.d = w.b;
+            if ((rc = product<T>(as, as, a, side, batch, s))) return rc;
+        }
+        OrthArgs d{};  // X = Y X, or X Y
         d.m = rows;
         d.n = cols;
-        d.batch = batch;
-        d.alpha = p->a;
         d.beta = 1.0f;
-        d.c = x;
-        d.ldc = ldx;
-        d.c_plane = x_plane;
         d.d = last ? nullptr : w.x[(k + 1) & 1];
         d.ldd = ldx;
-        d.d_plane = x_plane;
         d.out = out;
-        d.ldo = cols;
+        d.vec = cols % 4 == 0 && aligned(out, 4 * es);
         const OrthOperand xk{x, rows, cols, ldx, !tall};
-        if ((rc = tall ? product<T>(xk, bs, d, side, s) : product<T>(bs, xk, d, side, s))) return rc;
+        if ((rc = tall ? product<T>(xk, bs, d, side, batch, s) : product<T>(bs, xk, d, side, batch, s))) return rc;
     }
     return FG_OK;
 }

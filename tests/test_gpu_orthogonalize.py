@@ -48,14 +48,22 @@ def _iterate(g, steps=5, coef=COEF, eps=1e-7):
         rms = float((p.square() @ q.square()).sum().sqrt())
         return ROUND * rms + (p.shape[1] / 16 + 16) * 2.0 ** -24 * float((p @ q).norm())
 
+    eye = torch.eye(x.shape[0], device=x.device, dtype=torch.float64)
+    square = c != 0 and abs(b) <= 8 * abs(c)
     for _ in range(steps):
         gram = x @ x.t()
-        poly = b * gram + c * gram @ gram
         top = float(torch.linalg.matrix_norm(x, ord=2))
-        dg = product(x, x.t()) + KEPT * float(gram.norm())
-        dp = abs(b) * dg + abs(c) * (2 * top ** 2 * dg + product(gram, gram)) + KEPT * float(poly.norm())
-        new = a * x + poly @ x
-        dx = top * dp + product(poly, x) + 2 * KEPT * float(new.norm())
+        y = a * eye + b * gram + c * gram @ gram  # the step is y x
+        if square:  # y = c m^2 + (a - b^2 / 4c), m = gram + b / 2c
+            m = gram + b / (2 * c) * eye
+            dm = product(x, x.t()) + KEPT * float(m.norm())
+            dy = abs(c) * (2 * float(torch.linalg.matrix_norm(m, ord=2)) * dm + product(m, m))
+        else:
+            dg = product(x, x.t()) + KEPT * float(gram.norm())
+            dy = abs(b) * dg + abs(c) * (2 * top ** 2 * dg + product(gram, gram))
+        dy += KEPT * float(y.norm())
+        new = y @ x
+        dx = top * dy + product(y, x) + 2 * KEPT * float(new.norm())
         s = torch.linspace(0, top, 200, dtype=torch.float64)
         slope = float((a + 3 * b * s ** 2 + 5 * c * s ** 4).abs().max())
         err = max(slope, float((a + b * s ** 2 + c * s ** 4).abs().max())) * err + dx
@@ -97,7 +105,7 @@ def test_orthogonalize_batches(ad, batch, m, n, t):
 
 
 @pytest.mark.parametrize("steps", [0, 1, 2, 8])
-@pytest.mark.parametrize("coef", [COEF, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5)])
+@pytest.mark.parametrize("coef", [COEF, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (1.5, -0.6, 0.01), (1.9, 0.0, 0.0)])
 def test_orthogonalize_steps_and_coefficients(ad, steps, coef):
     for m, n in ((60, 200), (300, 70)):
         _check(ad, torch.randn(m, n, generator=_gen(m + steps), device="cuda"), "f32", steps, coef)

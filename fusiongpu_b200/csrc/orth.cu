@@ -29,6 +29,13 @@ __device__ __forceinline__ void planes_of(float v, __half& h, __half& l) {
     const float f = __half2float(h);
     l = fabsf(f) <= 65504.0f ? __float2half_rn((v - f) * (float)(1 << LOW_SHIFT)) : __float2half_rn(0.0f);
 }
+// The same of two values; one conversion instruction for both.
+__device__ __forceinline__ void planes_of(float v0, float v1, __half2& h, __half2& l) {
+    h = __floats2half2_rn(v0, v1);
+    const float2 f = __half22float2(h);
+    constexpr float up = 1 << LOW_SHIFT;
+    l = __floats2half2_rn(fabsf(f.x) <= 65504.0f ? (v0 - f.x) * up : 0.0f, fabsf(f.y) <= 65504.0f ? (v1 - f.y) * up : 0.0f);
+}
 __device__ __forceinline__ float value_of(__half h, __half l) {
     return fmaf(__half2float(l), 1.0f / (1 << LOW_SHIFT), __half2float(h));
 }
@@ -126,7 +133,8 @@ __global__ void __launch_bounds__(OI_NT) orth_scale_kernel(const OrthIn g) {
             if (g.x) {
                 alignas(16) __half h[VEC], l[VEC];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) planes_of(f[j], h[j], l[j]);
+                for (int j = 0; j < VEC; j += 2)
+                    planes_of(f[j], f[j + 1], *reinterpret_cast<__half2*>(h + j), *reinterpret_cast<__half2*>(l + j));
                 __half* x = g.x + 2 * blockIdx.y * plane + row * g.ld + c;
                 *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(h);
                 *reinterpret_cast<uint4*>(x + plane) = *reinterpret_cast<const uint4*>(l);
@@ -194,12 +202,11 @@ __device__ __forceinline__ float4 orth_peer(uint32_t a, uint32_t rank) {
     return v;
 }
 
-template <class T, int BN>
+template <class T, int BN, bool SPLIT>
 __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
     orth_product_kernel(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMap tq, const __grid_constant__ OrthArgs g) {
     using Ring = OrthRing<BN>;
-    constexpr int LDP = BN + 4;
-    static_assert(OT_M * LDP * 4 <= Ring::N * Ring::STAGE, "the partial tile fits the ring");
+    constexpr int LDP = BN + 4;  // partial row: 4 floats of padding keep 16-byte stores off each other's banks
     extern __shared__ __align__(1024) unsigned char dsmem[];
     __shared__ __align__(8) uint64_t full[Ring::N], empty[Ring::N], acc_full;
     __shared__ uint32_t tmem_slot;
@@ -208,7 +215,7 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
     unsigned char* ring = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
     float* part = reinterpret_cast<float*>(ring);
-    const int S = g.split, rank = S > 1 ? (int)orth_rank() : 0;
+    const int S = SPLIT ? g.split : 1, rank = SPLIT ? (int)orth_rank() : 0;
     const int tile = (int)(blockIdx.x / (unsigned)S), b = tile / g.tiles;
     int t = tile - b * g.tiles, mi = 0;
     if (g.sym) {  // row tiles hold the column tiles up to the diagonal
@@ -328,84 +335,94 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
         tc::fence_before_sync();
     }
     __syncthreads();
-    if (S > 1) orth_cluster_sync();
+    if (SPLIT) orth_cluster_sync();
     if (warp == 1) {
         tc::fence_after_sync();
         tc::tmem_dealloc(taddr, Ring::COLS);
     }
 
-    // Two positions of four columns per thread and round, what they read asked for first: one
-    // latency a round.
-    constexpr int U = 2;
-    constexpr int LDT = OT_M + 1;  // SYM: the slice transposed, h and l of an element in one word
-    uint32_t* turned = reinterpret_cast<uint32_t*>(part + OT_M * LDP);
-    const int slice = BN / S, shift = __ffs(slice) - 3;  // columns, and the logarithm of a row's positions
+    // W columns a position, two positions a thread and round.  A cluster's exchange waits for
+    // distributed shared memory (a tile of 128 x 64, four CTAs: 2.2 us), of which a round asks
+    // for three peers at once; alone, 16-byte stores count (128 x 256: 4.4 us, with 8 bytes 6.2).
+    constexpr int W = SPLIT ? 4 : 8, U = 2;
+    static_assert((OT_M * LDP + (BN == 256 ? 0 : OT_M * BN)) * 4 <= Ring::N * Ring::STAGE, "the tile, and for SYM its transposed copy, fit the ring");
+    uint32_t* turned = reinterpret_cast<uint32_t*>(part + OT_M * LDP);  // SYM: the slice transposed, h and l in one word,
+    auto turn = [](int c, int r) { return c * OT_M + ((r + c / W) & (OT_M - 1)); };  // turned on by W columns
+    const int slice = BN / S, shift = __ffs(slice / W) - 1;  // columns, and the logarithm of a row's positions
     const uint32_t pbase = tc::smem_u32(part);
     const long long c_plane = g.m * g.ldc, d_plane = g.m * g.ldd;
     for (int i0 = tid; i0 < OT_M << shift; i0 += U * OT_NT) {
         int r[U], cc[U];
         bool in[U];
-        float4 z[U];
-        uint2 ch[U], cl[U];
+        alignas(16) float v[U][W];
+        alignas(16) __half ch[U][W], cl[U][W];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * OT_NT;
             r[u] = i >> shift;
-            cc[u] = rank * slice + (i - (r[u] << shift)) * 4;
-            in[u] = r[u] < OT_M && m0 + r[u] < g.m && n0 + cc[u] < g.n;
+            cc[u] = (i - (r[u] << shift)) * W;
+            in[u] = r[u] < OT_M && m0 + r[u] < g.m && n0 + rank * slice + cc[u] < g.n;
             if (!in[u]) continue;
-            const uint32_t at = (uint32_t)(r[u] * LDP + cc[u]) * 4;
             if (g.c) {  // rows hold a multiple of 8 elements
-                const __half* p = g.c + 2 * b * c_plane + (m0 + r[u]) * g.ldc + n0 + cc[u];
-                ch[u] = *reinterpret_cast<const uint2*>(p);
-                cl[u] = *reinterpret_cast<const uint2*>(p + c_plane);
+                const __half* p = g.c + 2 * b * c_plane + (m0 + r[u]) * g.ldc + n0 + rank * slice + cc[u];
+#pragma unroll
+                for (int j = 0; j < W; j += 4) {
+                    *reinterpret_cast<uint2*>(&ch[u][j]) = *reinterpret_cast<const uint2*>(p + j);
+                    *reinterpret_cast<uint2*>(&cl[u][j]) = *reinterpret_cast<const uint2*>(p + c_plane + j);
+                }
             }
-            z[u] = *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(part) + at);
+            const float* own = part + r[u] * LDP + rank * slice + cc[u];
+#pragma unroll
+            for (int j = 0; j < W; j += 4) *reinterpret_cast<float4*>(&v[u][j]) = *reinterpret_cast<const float4*>(own + j);
         }
-        for (int s0 = 1; s0 < S; s0 += 3) {  // three peers' at a time, this block's own is there
-            float4 x[U][3];
+        if constexpr (SPLIT) {
+            for (int s0 = 1; s0 < S; s0 += 3) {
+                float4 x[U][3];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int s = 0; s < 3; ++s)
-                    if (in[u] && s0 + s < S) x[u][s] = orth_peer(pbase + (uint32_t)(r[u] * LDP + cc[u]) * 4, (rank + s0 + s) & (S - 1));
+                    for (int s = 0; s < 3; ++s)
+                        if (in[u] && s0 + s < S)
+                            x[u][s] = orth_peer(pbase + (uint32_t)(r[u] * LDP + rank * slice + cc[u]) * 4, (rank + s0 + s) & (S - 1));
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int s = 0; s < 3; ++s)
-                    if (in[u] && s0 + s < S) {
-                        z[u].x += x[u][s].x;
-                        z[u].y += x[u][s].y;
-                        z[u].z += x[u][s].z;
-                        z[u].w += x[u][s].w;
-                    }
+                    for (int s = 0; s < 3; ++s)
+                        if (in[u] && s0 + s < S) {
+                            v[u][0] += x[u][s].x;
+                            v[u][1] += x[u][s].y;
+                            v[u][2] += x[u][s].z;
+                            v[u][3] += x[u][s].w;
+                        }
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (!in[u]) continue;
-            const int row = m0 + r[u], col = n0 + cc[u];
-            float v[4] = {z[u].x * g.beta, z[u].y * g.beta, z[u].z * g.beta, z[u].w * g.beta};
+            const int row = m0 + r[u], col = n0 + rank * slice + cc[u];
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[u][j] *= g.beta;
             if (g.c) {
-                const __half *h = reinterpret_cast<const __half*>(&ch[u]), *l = reinterpret_cast<const __half*>(&cl[u]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = fmaf(g.alpha, value_of(h[j], l[j]), v[j]);
+                for (int j = 0; j < W; ++j) v[u][j] = fmaf(g.alpha, value_of(ch[u][j], cl[u][j]), v[u][j]);
             }
-            if (g.sym) {
+            if (g.sym && (unsigned)(row - col) < W) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (col + j == row) v[j] += g.diag;
+                for (int j = 0; j < W; ++j) v[u][j] += col + j == row ? g.diag : 0.0f;
             }
             if (g.d) {
-                alignas(8) __half h[4], l[4];
+                alignas(16) __half h[W], l[W];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) planes_of(v[j], h[j], l[j]);
+                for (int j = 0; j < W; j += 2)
+                    planes_of(v[u][j], v[u][j + 1], *reinterpret_cast<__half2*>(h + j), *reinterpret_cast<__half2*>(l + j));
+                using Wide = typename std::conditional<W == 8, uint4, uint2>::type;
                 __half* p = g.d + 2 * b * d_plane + row * g.ldd + col;
-                if (!g.sym || col + 3 <= row) {  // elements past the last column lie in the row's padding
-                    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
-                    *reinterpret_cast<uint2*>(p + d_plane) = *reinterpret_cast<const uint2*>(l);
+                if (!g.sym || col + W - 1 <= row) {  // elements past the last column lie in the row's padding
+                    *reinterpret_cast<Wide*>(p) = *reinterpret_cast<const Wide*>(h);
+                    *reinterpret_cast<Wide*>(p + d_plane) = *reinterpret_cast<const Wide*>(l);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < W; ++j)
                         if (col + j <= row) {
                             p[j] = h[j];
                             p[d_plane + j] = l[j];
@@ -413,33 +430,35 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
                 }
                 if (BN < 256 && g.sym) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        turned[(cc[u] - rank * slice + j) * LDT + r[u]] =
-                            (uint32_t)__half_as_ushort(h[j]) | (uint32_t)__half_as_ushort(l[j]) << 16;
+                    for (int j = 0; j < W; ++j)
+                        turned[turn(cc[u] + j, r[u])] = (uint32_t)__half_as_ushort(h[j]) | (uint32_t)__half_as_ushort(l[j]) << 16;
                 }
             } else {
                 T* p = static_cast<T*>(g.out) + ((long long)b * g.m + row) * g.n + col;
-                if (g.vec) {
-                    alignas(16) T o[4] = {from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
-                    if constexpr (sizeof(T) == 4)
-                        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(o);
-                    else
-                        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(o);
-                } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (col + j < g.n) p[j] = from_f32<T>(v[j]);
+                for (int k = 0; k < W; k += 4) {
+                    if (g.vec && col + k < g.n) {
+                        alignas(16) T o[4] = {from_f32<T>(v[u][k]), from_f32<T>(v[u][k + 1]), from_f32<T>(v[u][k + 2]), from_f32<T>(v[u][k + 3])};
+                        if constexpr (sizeof(T) == 4)
+                            *reinterpret_cast<uint4*>(p + k) = *reinterpret_cast<const uint4*>(o);
+                        else
+                            *reinterpret_cast<uint2*>(p + k) = *reinterpret_cast<const uint2*>(o);
+                    } else {
+#pragma unroll
+                        for (int j = k; j < k + 4; ++j)
+                            if (col + j < g.n) p[j] = from_f32<T>(v[u][j]);
+                    }
                 }
             }
         }
     }
+    if (SPLIT) asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // this block has read its peers' partial tiles
     if (BN < 256 && g.sym) {  // a lane takes two rows, which become neighbouring columns
-        static_assert(BN == 256 || (OT_M * LDP + BN * LDT) * 4 <= Ring::N * Ring::STAGE, "the transposed tile fits behind the partial one");
         __syncthreads();
         for (int i = tid; i < slice * (OT_M / 2); i += OT_NT) {
             const int c = i / (OT_M / 2), r = i % (OT_M / 2) * 2, row = m0 + r, col = n0 + rank * slice + c;
             if (col > row || row >= g.m) continue;  // of a pair on the diagonal the second one counts
-            const uint32_t x = turned[c * LDT + r], y = turned[c * LDT + r + 1];
+            const uint32_t x = turned[turn(c, r)], y = turned[turn(c, r + 1)];
             __half* p = g.d + 2 * b * d_plane + col * g.ldd + row;
             if (col < row && row + 1 < g.m) {
                 *reinterpret_cast<uint32_t*>(p) = __byte_perm(x, y, 0x5410);
@@ -453,7 +472,7 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
             }
         }
     }
-    if (S > 1) orth_cluster_sync();  // a peer may still read this CTA's partial tile
+    if (SPLIT) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // a peer may still read this CTA's partial tile
 }
 
 // ---- host side -----------------------------------------------------------------------
@@ -533,7 +552,7 @@ static int launch_product(const OrthOperand& p, const OrthOperand& q, OrthArgs g
     g.idesc = (1u << 4) | ((uint32_t)p.mn << 15) | ((uint32_t)q.mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(OT_M >> 4) << 24);
     const long long ctas = (long long)g.tiles * batch * g.split;
     FG_REQUIRE(ctas <= 0x7fffffffll, "too many tiles");
-    auto kernel = &orth_product_kernel<T, BN>;
+    auto kernel = g.split > 1 ? &orth_product_kernel<T, BN, true> : &orth_product_kernel<T, BN, false>;
     const int smem = OrthRing<BN>::N * OrthRing<BN>::STAGE + 1024;
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
     cudaLaunchConfig_t cfg = {};

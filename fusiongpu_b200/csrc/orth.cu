@@ -475,6 +475,235 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
     if (SPLIT) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // a peer may still read this CTA's partial tile
 }
 
+// ---- small matrices: the whole iteration in one block ----------------------------------
+//
+// Up to 128 x 256, whichever way they lie, X and Y (or M) stay in shared memory as the
+// tensor cores read them: chunks of 64 columns, 128 rows of 128 bytes, 128-byte swizzle, a
+// row of X an index of the smaller side.  The same chunk is a K-major operand of X X^T and
+// an MN-major one of Y X.  A product's epilogue writes the next one's operand in place.
+// Bound by the chain of three products and three epilogues a step.
+constexpr int OS_NT = 512, OS_SIDE = 128, OS_FAR = 256, OS_CHUNK = 128 * 128;
+constexpr int OS_X = 4 * OS_CHUNK, OS_Y = 2 * OS_CHUNK;  // bytes of a plane
+constexpr int OS_SMEM = 2 * OS_X + 2 * OS_Y + 1024;
+static_assert(OS_SIDE * (OS_FAR | 1) * 4 <= 2 * OS_X + 2 * OS_Y, "the result's rows fit");
+
+struct OrthSmall {
+    const void* g;
+    void* out;
+    long long row_stride, batch_stride;
+    int rows, cols, steps, square, wide;  // wide: G's rows start on 16 bytes
+    float a, b, c, eps;
+};
+
+__device__ __forceinline__ uint32_t os_at(int row, int col) {  // byte of 8 elements from col on
+    return (uint32_t)((col >> 6) * OS_CHUNK + row * 128 + (((col & 63) * 2) ^ ((row & 7) << 4)));
+}
+
+template <class T>
+__global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g) {
+    extern __shared__ __align__(1024) unsigned char dsmem[];
+    __shared__ __align__(8) uint64_t done;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int s_fail;
+    __shared__ double s_sum[OS_NT / 32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    unsigned char* xs = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
+    unsigned char* ys = xs + 2 * OS_X;
+    const bool tall = g.rows > g.cols;
+    const int side = tall ? g.cols : g.rows, far = tall ? g.rows : g.cols;
+    const int sc = (side + 63) / 64, fc = (far + 63) / 64;  // chunks
+    const T* in = static_cast<const T*>(g.g) + blockIdx.x * g.batch_stride;
+
+    if (tid == 0) {
+        s_fail = 0;
+        tc::mbar_init(&done, 1);
+        tc::fence_mbar_init();
+    }
+    if (warp == 1) {
+        tc::tmem_alloc(&tmem_slot, 512);
+        tc::tmem_relinquish();
+    }
+    // G is read once, 64 elements a thread: |G|_F, then the planes of X
+    constexpr int PIECES = OS_SIDE * OS_FAR / 8 / OS_NT;
+    const int pieces = OS_SIDE * fc * 8;  // eight elements of an index of the smaller side
+    auto piece_of = [&](int k, int& r, int& c) {
+        const int i = k * OS_NT + tid;
+        r = tall ? i & (OS_SIDE - 1) : i / (fc * 8);  // neighbouring lanes on neighbouring columns of memory
+        c = (tall ? i / OS_SIDE : i % (fc * 8)) * 8;
+        return i < pieces;
+    };
+    float v[PIECES][8];
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+        int r, c;
+        const bool in_x = piece_of(k, r, c) && r < side;
+        if (!tall && g.wide && in_x && c + 8 <= far) {
+            alignas(16) T t[8];
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+                reinterpret_cast<uint4*>(t)[j] = reinterpret_cast<const uint4*>(in + r * g.row_stride + c)[j];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[k][j] = to_f32(t[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[k][j] = in_x && c + j < far ? to_f32(in[tall ? (c + j) * g.row_stride + r : r * g.row_stride + c + j]) : 0.0f;
+        }
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fma((double)v[k][j], (double)v[k][j], sum);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t taddr = tmem_slot;
+    volatile int* fail = &s_fail;
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < OS_NT / 32; ++w) sum += s_sum[w];
+    const double inv = 1.0 / (sqrt(sum) + (double)g.eps);
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+        int r, c;
+        if (!piece_of(k, r, c)) continue;
+        alignas(16) __half h[8], l[8];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+            planes_of((float)((double)v[k][j] * inv), (float)((double)v[k][j + 1] * inv), *reinterpret_cast<__half2*>(h + j),
+                      *reinterpret_cast<__half2*>(l + j));
+        const uint32_t at = os_at(r, c);
+        *reinterpret_cast<uint4*>(xs + at) = *reinterpret_cast<const uint4*>(h);
+        *reinterpret_cast<uint4*>(xs + OS_X + at) = *reinterpret_cast<const uint4*>(l);
+    }
+
+    const uint32_t idesc = (1u << 4) | ((uint32_t)(OT_M >> 4) << 24);  // f16 operands, f32 accumulators
+    const int q4 = warp & 3, part = warp >> 2;                         // lanes of TMEM, columns
+    uint32_t phase = 0;
+    bool ok = true;
+    // h h' of columns [0, n) and, 256 on, h l' + l h', over `chunks` of 64 k
+    auto multiply = [&](const unsigned char* p, uint32_t p_low, const unsigned char* q, uint32_t q_low, bool q_mn, int n, int chunks) {
+        tc::fence_proxy_async();  // operands written by ordinary stores
+        tc::fence_before_sync();
+        __syncthreads();
+        tc::fence_after_sync();
+        if (warp == 0) {
+            const uint64_t dp = tc::desc_kmajor_sw128(p), dq = q_mn ? tc::desc_mnmajor_sw128(q, OS_CHUNK) : tc::desc_kmajor_sw128(q);
+            const uint32_t id = idesc | ((uint32_t)q_mn << 16) | ((uint32_t)(n >> 3) << 17);
+            if (tc::elect_one()) {
+                for (int c = 0; c < chunks; ++c)
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint64_t a = dp + c * (OS_CHUNK / 16) + 2 * kk;
+                        const uint64_t b = dq + (q_mn ? c * (64 * 128 / 16) + 128 * kk : c * (OS_CHUNK / 16) + 2 * kk);
+                        const uint32_t more = (c | kk) != 0;
+                        tc::umma_bf16(taddr, a, b, id, more);
+                        tc::umma_bf16(taddr + 256, a, b + q_low / 16, id, more);
+                        tc::umma_bf16(taddr + 256, a + p_low / 16, b, id, 1);
+                    }
+                tc::umma_commit(&done);
+            }
+            __syncwarp();
+        }
+        ok = tc::mbar_wait_warp(&done, phase, fail) && ok;
+        phase ^= 1;
+        tc::fence_after_sync();
+    };
+    // 32 columns of a product from column c on, this lane's row
+    auto take = [&](float (&v)[32], int c) {
+        float x[32];
+        const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)c;
+        tc::tmem_ld_32x32_nowait(src, v);
+        tc::tmem_ld_32x32_nowait(src + 256, x);
+        tc::tmem_ld_wait(v);
+        tc::tmem_ld_wait(x);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = ok ? fmaf(x[j], 1.0f / (1 << LOW_SHIFT), v[j]) : NAN;
+    };
+    auto put = [&](unsigned char* to, uint32_t low, const float (&v)[32], int row, int c) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+            alignas(16) __half h[8], l[8];
+#pragma unroll
+            for (int k = 0; k < 8; k += 2)
+                planes_of(v[j + k], v[j + k + 1], *reinterpret_cast<__half2*>(h + k), *reinterpret_cast<__half2*>(l + k));
+            const uint32_t at = os_at(row, c + j);
+            *reinterpret_cast<uint4*>(to + at) = *reinterpret_cast<const uint4*>(h);
+            *reinterpret_cast<uint4*>(to + low + at) = *reinterpret_cast<const uint4*>(l);
+        }
+    };
+    const int row = q4 * 32 + lane;
+    T* out = static_cast<T*>(g.out) + (long long)blockIdx.x * g.rows * g.cols;
+    // the result: tall, neighbouring lanes on neighbouring columns; else through shared memory,
+    // where X's planes are done with, rows of an odd number of words
+    float* staged = reinterpret_cast<float*>(xs);
+    const int lds = far | 1;
+    auto store = [&](const float (&v)[32], int c) {
+        if (row >= side) return;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (c + j < far) {
+                if (tall)
+                    out[(c + j) * side + row] = from_f32<T>(v[j]);
+                else
+                    staged[row * lds + c + j] = v[j];
+            }
+    };
+#pragma unroll 1
+    for (int step = 0; step < g.steps; ++step) {
+        float v[32];
+        multiply(xs, OS_X, xs, OS_X, false, sc * 64, fc);
+        if (part * 32 < sc * 64) {
+            const float scale = g.c == 0.0f ? g.b : 1.0f, diag = g.c == 0.0f ? g.a : g.square ? g.b / (2.0f * g.c) : 0.0f;
+            take(v, part * 32);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], scale, part * 32 + j == row ? diag : 0.0f);
+            put(ys, OS_Y, v, row, part * 32);
+        }
+        if (g.c != 0.0f) {
+            multiply(ys, OS_Y, ys, OS_Y, false, sc * 64, sc);
+            if (part * 32 < sc * 64) {
+                const float diag = g.square ? (float)((double)g.a - (double)g.b * g.b / (4.0 * g.c)) : g.a;
+                take(v, part * 32);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], g.c, part * 32 + j == row ? diag : 0.0f);
+                if (!g.square) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        alignas(16) __half h[8], l[8];
+                        const uint32_t at = os_at(row, part * 32 + j);
+                        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(ys + at);
+                        *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(ys + OS_Y + at);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[j + k] = fmaf(g.b, value_of(h[k], l[k]), v[j + k]);
+                    }
+                }
+                put(ys, OS_Y, v, row, part * 32);
+            }
+        }
+        multiply(ys, OS_Y, xs, OS_X, true, fc * 64, sc);
+#pragma unroll 1
+        for (int c = part * 32; c < fc * 64; c += 128) {
+            take(v, c);
+            if (step + 1 < g.steps)
+                put(xs, OS_X, v, row, c);
+            else
+                store(v, c);
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    if (warp == 1) tc::tmem_dealloc(taddr, 512);
+    if (!tall)
+        for (int r = warp; r < side; r += OS_NT / 32)
+            for (int c = lane; c < far; c += 32) out[r * far + c] = from_f32<T>(staged[r * lds + c]);
+}
+
 // ---- host side -----------------------------------------------------------------------
 
 // Matrices [batch][2 planes][rows][ld] as an operand: boxes of 64 columns of memory, both
@@ -589,10 +818,15 @@ struct OrthWs {
 
 static long long orth_ld(long long cols) { return (cols + 7) / 8 * 8; }
 
+static bool orth_small(const fg_orthogonalize_params* p) {
+    return p->steps > 0 && std::min(p->rows, p->cols) <= OS_SIDE && std::max(p->rows, p->cols) <= OS_FAR;
+}
+
 static size_t orth_carve(const fg_orthogonalize_params* p, void* ws, size_t bytes, OrthWs& w) {
     Carve c(ws, bytes);
     w = OrthWs{};
     const size_t side = std::min(p->rows, p->cols), batch = p->batch;
+    if (orth_small(p)) return 0;
     w.part = c.take<double>(batch * ORTH_PARTS);
     if (p->steps > 0) {
         for (int k = 0; k < 2; ++k)
@@ -623,6 +857,19 @@ template <class T>
 static int orthogonalize(const fg_orthogonalize_params* p, const void* g, void* out, const OrthWs& w, cudaStream_t s) {
     const int rows = p->rows, cols = p->cols, batch = p->batch, side = std::min(rows, cols), far = std::max(rows, cols);
     const long long ldx = orth_ld(cols), lda = orth_ld(side);
+    const long long row_stride = p->row_stride ? p->row_stride : cols, batch_stride = p->batch_stride ? p->batch_stride : rows * row_stride;
+    // Y = a I + b A + c A^2 = c M^2 + (a - b^2 / 4c) I, M = A + b / 2c I, so that no product of a
+    // X + (b A + c A^2) X = Y X reads an addend.  Where b / 2c is large, M^2 would lose what A^2
+    // is, and A is added as it is; without c, Y comes from the first product.
+    const int es = sizeof(T);
+    const bool wide = aligned(g, 16) && row_stride * es % 16 == 0 && (batch == 1 || batch_stride * es % 16 == 0);
+    const bool square = p->c != 0.0f && fabsf(p->b) <= 8.0f * fabsf(p->c);
+    if (orth_small(p)) {
+        FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(&orth_small_kernel<T>), OS_SMEM));
+        orth_small_kernel<T><<<batch, OS_NT, OS_SMEM, s>>>(
+            OrthSmall{g, out, row_stride, batch_stride, rows, cols, p->steps, square, wide, p->a, p->b, p->c, p->eps});
+        return check_launch("orth_small_kernel");
+    }
     OrthIn in{};
     in.g = g;
     in.part = w.part;
@@ -630,15 +877,14 @@ static int orthogonalize(const fg_orthogonalize_params* p, const void* g, void* 
     in.out = out;
     in.rows = rows;
     in.cols = cols;
-    in.row_stride = p->row_stride ? p->row_stride : cols;
-    in.batch_stride = p->batch_stride ? p->batch_stride : rows * in.row_stride;
+    in.row_stride = row_stride;
+    in.batch_stride = batch_stride;
     in.ld = ldx;
     in.batch = batch;
     in.eps = p->eps;
     in.runs = (cols + OI_COLS - 1) / OI_COLS;
     in.parts = (int)std::min<long long>(ORTH_PARTS, ((long long)rows * in.runs + OI_WARPS - 1) / OI_WARPS);
-    const int es = sizeof(T);
-    in.wide = aligned(g, 16) && in.row_stride * es % 16 == 0 && (batch == 1 || in.batch_stride * es % 16 == 0);
+    in.wide = wide;
     orth_norm_kernel<T><<<dim3(in.parts, batch), OI_NT, 0, s>>>(in);
     int rc = check_launch("orth_norm_kernel");
     if (rc) return rc;
@@ -648,11 +894,7 @@ static int orthogonalize(const fg_orthogonalize_params* p, const void* g, void* 
     for (int k = 0; k < p->steps; ++k) {
         const __half* x = w.x[k & 1];
         const bool last = k + 1 == p->steps;
-        // a X + (b A + c A^2) X = Y X with Y = a I + b A + c A^2 = c M^2 + (a - b^2 / 4c) I, M = A +
-        // b / 2c I: neither product reads an addend.  Where b / 2c is large, M^2 would lose what
-        // A^2 is, and A is added as it is; without c, Y comes from the first product.
         const float ca = p->a, cb = p->b, cc = p->c;
-        const bool square = cc != 0.0f && fabsf(cb) <= 8.0f * fabsf(cc);
         OrthArgs a{};  // M, A or Y of X X^T
         a.m = a.n = side;
         a.sym = 1;

@@ -14,22 +14,92 @@ namespace fg {
 
 // ---- codes of rows -----------------------------------------------------------------
 //
-// A group of threads holds its row in registers, so that memory is read once: a warp up
-// to 1,024 columns, a block of 256 up to 8,192 (16 bits) or 4,096 (32); longer rows are
-// read again from L2.  The largest magnitude is found on the bits, as integers, where a
-// NaN is above all numbers.
+// A group of threads holds its row in registers, so that memory is read once: eight up
+// to 128 columns, a warp up to 2,048 (16 bits) or 1,024 (32), a block of 256 up to 8,192 or
+// 4,096; longer rows are read again from L2.
 constexpr int QR_NT = 256;
 constexpr int QUANTIZE_DIM = 1 << 30;
 
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// Two values' magnitudes against the largest so far, as the type's bits: of two 16-bit
+// values in one instruction, where a NaN wins.
+__device__ __forceinline__ uint32_t larger(uint32_t top, float a, float b) {
+    return max(top, max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
+}
+__device__ __forceinline__ uint32_t larger(uint32_t top, __half a, __half b) {
+    const __half2 t = __hmax2_nan(*reinterpret_cast<const __half2*>(&top), __habs2(__halves2half2(a, b)));
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+__device__ __forceinline__ uint32_t larger(uint32_t top, __nv_bfloat16 a, __nv_bfloat16 b) {
+    const __nv_bfloat162 t = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&top), __habs2(__halves2bfloat162(a, b)));
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+// ... and as the bits of a float, whose order as integers puts a NaN above all numbers.
+template <class T>
+__device__ __forceinline__ uint32_t float_bits(uint32_t top) {
+    if (sizeof(T) == 4) return top;
+    const unsigned short lo = (unsigned short)top, hi = (unsigned short)(top >> 16);
+    const float a = to_f32(*reinterpret_cast<const T*>(&lo)), b = to_f32(*reinterpret_cast<const T*>(&hi));
+    return max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu);
+}
 
-// 127 x / top, rounded to nearest, ties to even.  x inv is off by at most 2^-23 of it
-// (1.6e-5 at 127); next to a half, or where inv is not finite, the quotient in 64 bits,
-// whose distance from a half, if not 0, is at least 2^-25 of it.
-__device__ __forceinline__ int code_of(float x, float top, float inv) {
-    const float t = x * inv, r = rintf(t);
-    if (fabsf(fabsf(t - r) - 0.5f) > 2e-5f && inv <= FLT_MAX) return (int)r;
-    return top > 0.0f ? (int)rint(127.0 * (double)x / (double)top) : 0;
+struct QuantRow {
+    float top, inv, up;  // up: a power of two that brings top to where 127 top and 127 / top are ordinary numbers
+    bool finite;         // no infinity or NaN in the row
+    bool fast;           // inv is an ordinary number
+};
+
+// 127 x / top rounded to nearest, ties to even, for a value near a half between codes: the
+// remainder 127 x - r top of the nearest candidate, as a sum of two floats without an
+// error, against top / 2.  (bfloat16 rows meet exact ties often: their largest value has
+// 8 bits.)
+__device__ __forceinline__ float exact_code(float x, const QuantRow& q) {
+    x *= q.up;
+    const float top = q.top * q.up, half = 0.5f * top;
+    const float r = rintf(x * (127.0f / top)), p = 127.0f * x, t = r * top;
+    const float rest = fmaf(127.0f, x, -p) - fmaf(r, top, -t), e = p - t;  // 127 x - r top = e + rest
+    const float over = (fabsf(e) - half) + (e < 0.0f ? -rest : rest);
+    const bool odd = (int)r & 1;
+    return over > 0.0f || (over == 0.0f && odd) ? r + (e < 0.0f ? -1.0f : 1.0f) : r;
+}
+
+// Codes 127 x / top of N values, rounded to nearest, ties to even.  x times 127 / top plus
+// 1.5 2^23 rounds the product once to an integer, which the sum's low byte holds.  The
+// quotient is taken a little too small and a little too large (by 2^-22 of it, four times
+// its rounding): where both give the same integers, those are right.  Else, 16-bit values:
+// the remainder 127 x - r top is exact in 32 bits, and a code whose remainder reaches top / 2
+// is put right (exact ties are frequent in bfloat16, whose largest value has 8 bits);
+// 32-bit ones are taken again without an error.
+template <class T, int N>
+__device__ __forceinline__ void codes_of(uint32_t (&out)[N / 4], const T (&v)[N], const QuantRow& q) {
+    constexpr float magic = 12582912.0f;
+    const float low = q.inv - q.inv * 2.3841858e-7f, high = q.inv + q.inv * 2.3841858e-7f;
+    const uint64_t l = pair2(low, low), h = pair2(high, high), m = pair2(magic, magic);
+    uint32_t c[N], differ = 0;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const uint64_t x = pair2(to_f32(v[i]), to_f32(v[i + 1]));
+        float a, b, d, e;
+        unpair2(fma2(x, l, m), a, b);
+        unpair2(fma2(x, h, m), d, e);
+        c[i] = __float_as_uint(a);
+        c[i + 1] = __float_as_uint(b);
+        differ |= (c[i] ^ __float_as_uint(d)) | (c[i + 1] ^ __float_as_uint(e));
+    }
+    if (differ || !q.fast) {
+        if (sizeof(T) == 4 || !q.fast) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) c[i] = q.finite && q.top > 0.0f ? __float_as_uint(exact_code(to_f32(v[i]), q) + magic) : 0u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float e = fmaf(__uint_as_float(c[i]) - magic, -q.top, 127.0f * to_f32(v[i])), over = fabsf(e) - 0.5f * q.top;
+                if (over > 0.0f || (over == 0.0f && (c[i] & 1))) c[i] += e < 0.0f ? -1 : 1;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+        out[i / 4] = __byte_perm(__byte_perm(c[i], c[i + 1], 0x0040), __byte_perm(c[i + 2], c[i + 3], 0x0040), 0x5410);
 }
 
 struct QuantArgs {
@@ -37,107 +107,151 @@ struct QuantArgs {
     signed char* q;
     float* scale;
     long long rows, ldx, ldq;
-    int dim, wide;  // wide: rows of x and q start on 16 bytes
+    int dim, unit, wide;  // unit: bytes that x's rows start on, up to 16; wide: q's start on 8
 };
 
+// VEC neighbouring columns, `unit` bytes at a time: what the rows' starts allow.
 template <class T, int VEC>
-__device__ __forceinline__ void qr_store(signed char* p, const T (&v)[VEC], float top, float inv, bool finite, int left, int wide) {
-    alignas(8) signed char c[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) c[i] = finite ? (signed char)code_of(to_f32(v[i]), top, inv) : (signed char)0;
-    if (wide && left >= VEC) {
-        if constexpr (VEC == 8)
-            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(c);
-        else
-            *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(c);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-            if (i < left) p[i] = c[i];
-    }
-}
-
-template <class T, int VEC>
-__device__ __forceinline__ void qr_load(T (&v)[VEC], const T* p, int left, int wide) {
-    if (wide && left >= VEC) {
+__device__ __forceinline__ void qr_load(T (&v)[VEC], const T* p, int left, int unit) {
+    if (unit == 16 && left >= VEC) {
         *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
+    } else if (unit >= 8 && left >= VEC) {
+        reinterpret_cast<uint2*>(v)[0] = reinterpret_cast<const uint2*>(p)[0];
+        reinterpret_cast<uint2*>(v)[1] = reinterpret_cast<const uint2*>(p)[1];
+    } else if (unit >= 4 && left >= VEC) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(v)[i] = reinterpret_cast<const uint32_t*>(p)[i];
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[i] = i < left ? p[i] : from_f32<T>(0.0f);
     }
 }
 
-// L threads a row (32, or the block), PER pieces of 16 bytes each; PER 0: rows of any
-// length, read twice.
-template <class T, int L, int PER>
-__global__ void __launch_bounds__(QR_NT) quantize_kernel(const QuantArgs g) {
-    constexpr int VEC = 16 / sizeof(T), HELD = PER ? PER : 1;
-    __shared__ uint32_t s[QR_NT / 32];
-    const int lane = threadIdx.x % L;
-    const long long row = blockIdx.x * (long long)(QR_NT / L) + threadIdx.x / L;
-    if (row >= g.rows) return;  // L == 32: whole warps; L == QR_NT: none
-    const T* x = static_cast<const T*>(g.x) + row * g.ldx;
-    signed char* q = g.q + row * g.ldq;
-    alignas(16) T v[HELD][VEC];
-    uint32_t top = 0;
-    auto more = [&](const T (&v)[VEC]) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) top = max(top, magnitude(to_f32(v[i])));
-    };
-    if (PER) {
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int c = (k * L + lane) * VEC;
-            qr_load<T, VEC>(v[k], x + c, g.dim - c, g.wide);
-        }
-#pragma unroll
-        for (int k = 0; k < PER; ++k) more(v[k]);
+template <class T, int VEC>
+__device__ __forceinline__ void qr_store(signed char* p, const T (&v)[VEC], const QuantRow& q, int left, int wide) {
+    uint32_t codes[VEC / 4];
+    codes_of<T, VEC>(codes, v, q);
+    if (wide && left >= VEC) {
+        if constexpr (VEC == 8)
+            *reinterpret_cast<uint2*>(p) = make_uint2(codes[0], codes[1]);
+        else
+            *reinterpret_cast<uint32_t*>(p) = codes[0];
     } else {
-        for (int c = lane * VEC; c < g.dim; c += L * VEC) {
-            qr_load<T, VEC>(v[0], x + c, g.dim - c, g.wide);
-            more(v[0]);
-        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i < left) p[i] = (signed char)(codes[i / 4] >> (i % 4 * 8));
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+}
+
+// The row's largest magnitude, in all of its L threads.
+template <class T, int L>
+__device__ __forceinline__ QuantRow row_of(uint32_t top, uint32_t* s) {
+    top = float_bits<T>(top);
+    if (L < 32) {
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    } else {
+        top = __reduce_max_sync(0xffffffffu, top);
+    }
     if (L > 32) {
+        __syncthreads();  // the last row's readers are done with s
         if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = top;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < QR_NT / 32; ++w) top = max(top, s[w]);
+        for (int w = 0; w < L / 32; ++w) top = max(top, s[w]);
     }
-    const bool finite = top < 0x7f800000u;
-    const float most = __uint_as_float(top), inv = 127.0f / most;
-    if (lane == 0) g.scale[row] = finite ? most / 127.0f : NAN;
-    if (PER) {
+    QuantRow q;
+    q.finite = top < 0x7f800000u;
+    q.top = __uint_as_float(top);
+    q.inv = 127.0f / q.top;
+    q.up = q.top < 1e-18f ? 18446744073709551616.0f : q.top > 1e30f ? 1.0f / 65536.0f : 1.0f;  // 2^64, 2^-16
+    q.fast = q.finite && q.up == 1.0f;
+    return q;
+}
+__device__ __forceinline__ float scale_of(const QuantRow& q) { return q.finite ? q.top / 127.0f : NAN; }
+
+// L threads a row (8, 32 or the block), PER pieces of 16 bytes each.  Groups take rows in
+// turn and ask for the next one before they work on this one (1M x 768 float16: 376 us, 6.1
+// TB/s; with a group a row 501).
+template <class T, int L, int PER>
+__global__ void __launch_bounds__(QR_NT, PER <= 4 ? 4 : 2) quantize_kernel(const QuantArgs g) {
+    constexpr int VEC = 16 / sizeof(T), GROUPS = QR_NT / L;
+    __shared__ uint32_t s[QR_NT / 32];
+    const int lane = threadIdx.x % L;
+    const long long step = (long long)gridDim.x * GROUPS;
+    alignas(16) T next[PER][VEC];
+    auto fetch = [&](long long r) {
+        const T* x = static_cast<const T*>(g.x) + min(r, g.rows - 1) * g.ldx;  // a group past the last row takes it again
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int c = (k * L + lane) * VEC;
-            qr_store<T, VEC>(q + c, v[k], most, inv, finite, g.dim - c, g.wide);
-        }
-    } else {
-        for (int c = lane * VEC; c < g.dim; c += L * VEC) {
-            qr_load<T, VEC>(v[0], x + c, g.dim - c, g.wide);
-            qr_store<T, VEC>(q + c, v[0], most, inv, finite, g.dim - c, g.wide);
-        }
+        for (int k = 0; k < PER; ++k) qr_load<T, VEC>(next[k], x + (k * L + lane) * VEC, g.dim - (k * L + lane) * VEC, g.unit);
+    };
+    long long first = (long long)blockIdx.x * GROUPS, row = first + threadIdx.x / L;  // `first`: the block's, so that its threads stay together
+    fetch(row);
+    for (; first < g.rows; first += step, row += step) {
+        alignas(16) T v[PER][VEC];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) *reinterpret_cast<uint4*>(v[k]) = *reinterpret_cast<const uint4*>(next[k]);
+        if (first + step < g.rows) fetch(row + step);
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) top = larger(top, v[k][i], v[k][i + 1]);
+        const QuantRow q = row_of<T, L>(top, s);
+        if (row >= g.rows) continue;
+        if (lane == 0) g.scale[row] = scale_of(q);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) qr_store<T, VEC>(g.q + row * g.ldq + (k * L + lane) * VEC, v[k], q, g.dim - (k * L + lane) * VEC, g.wide);
+    }
+}
+
+// Rows of any length, read twice.
+template <class T>
+__global__ void __launch_bounds__(QR_NT) quantize_long_kernel(const QuantArgs g) {
+    constexpr int VEC = 16 / sizeof(T);
+    __shared__ uint32_t s[QR_NT / 32];
+    const long long row = blockIdx.x;
+    const T* x = static_cast<const T*>(g.x) + row * g.ldx;
+    alignas(16) T v[VEC];
+    uint32_t top = 0;
+#pragma unroll 4
+    for (int c = threadIdx.x * VEC; c < g.dim; c += QR_NT * VEC) {
+        qr_load<T, VEC>(v, x + c, g.dim - c, g.unit);
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) top = larger(top, v[i], v[i + 1]);
+    }
+    const QuantRow q = row_of<T, QR_NT>(top, s);
+    if (threadIdx.x == 0) g.scale[row] = scale_of(q);
+    for (int c = threadIdx.x * VEC; c < g.dim; c += QR_NT * VEC) {
+        qr_load<T, VEC>(v, x + c, g.dim - c, g.unit);
+        qr_store<T, VEC>(g.q + row * g.ldq + c, v, q, g.dim - c, g.wide);
     }
 }
 
 template <class T>
 static int launch_quantize(QuantArgs g, cudaStream_t s) {
     constexpr int VEC = 16 / (int)sizeof(T);
-    g.wide = aligned(g.x, 16) && g.ldx * (int)sizeof(T) % 16 == 0 && aligned(g.q, 16) && g.ldq % 16 == 0;
+    g.unit = 16;
+    while (g.unit > (int)sizeof(T) && !(aligned(g.x, g.unit) && g.ldx * (int)sizeof(T) % g.unit == 0)) g.unit /= 2;
+    g.wide = aligned(g.q, 8) && g.ldq % 8 == 0;
     const long long pieces = (g.dim + VEC - 1) / VEC;
-    const bool warps = pieces <= 32 * (sizeof(T) == 2 ? 4 : 8);
-    const long long blocks = warps ? (g.rows + QR_NT / 32 - 1) / (QR_NT / 32) : g.rows;
-    FG_REQUIRE(blocks <= 0x7fffffffll, "too many rows");
-    const int per = (int)std::min<long long>(8, (pieces + (warps ? 32 : QR_NT) - 1) / (warps ? 32 : QR_NT));
-    auto kernel = &quantize_kernel<T, QR_NT, 0>;
-    if (warps)
-        kernel = per <= 1 ? &quantize_kernel<T, 32, 1> : per <= 2 ? &quantize_kernel<T, 32, 2> : per <= 3 ? &quantize_kernel<T, 32, 3>
-                 : per <= 4 ? &quantize_kernel<T, 32, 4> : per <= 6 ? &quantize_kernel<T, 32, 6> : &quantize_kernel<T, 32, 8>;
-    else if (pieces <= 4 * QR_NT)
-        kernel = per <= 1 ? &quantize_kernel<T, QR_NT, 1> : per <= 2 ? &quantize_kernel<T, QR_NT, 2> : &quantize_kernel<T, QR_NT, 4>;
-    kernel<<<(unsigned)blocks, QR_NT, 0, s>>>(g);
+    const bool warps = pieces <= 32 * 8;
+    if (!warps && pieces > 4 * QR_NT) {
+        FG_REQUIRE(g.rows <= 0x7fffffffll, "too many rows");
+        quantize_long_kernel<T><<<(unsigned)g.rows, QR_NT, 0, s>>>(g);
+        return check_launch("quantize_long_kernel");
+    }
+    const bool eights = pieces <= 8 * (sizeof(T) == 2 ? 2 : 4);
+    const int lanes = eights ? 8 : warps ? 32 : QR_NT, per = (int)((pieces + lanes - 1) / lanes);
+    auto of = [&](auto l) {
+        constexpr int L = decltype(l)::value;
+        return per <= 1 ? &quantize_kernel<T, L, 1> : per <= 2 ? &quantize_kernel<T, L, 2> : per <= 3 ? &quantize_kernel<T, L, 3> : &quantize_kernel<T, L, 4>;
+    };
+    auto kernel = eights ? of(std::integral_constant<int, 8>()) : warps ? of(std::integral_constant<int, 32>()) : of(std::integral_constant<int, QR_NT>());
+    if (per > 4) kernel = per <= 6 ? &quantize_kernel<T, 32, 6> : &quantize_kernel<T, 32, 8>;
+    const long long blocks = (g.rows + QR_NT / lanes - 1) / (QR_NT / lanes);
+    const long long most = (long long)(per <= 4 ? 4 : 2) * std::max(1, device_attr(cudaDevAttrMultiProcessorCount));
+    kernel<<<(unsigned)std::min(blocks, most), QR_NT, 0, s>>>(g);
     return check_launch("quantize_kernel");
 }
 
@@ -260,7 +374,7 @@ int fg_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t dim, in
         if (dim > QUANTIZE_DIM) return fail(FG_ERR_UNSUPPORTED, "dim above %d", QUANTIZE_DIM);
         if (rows == 0) return FG_OK;
         FG_REQUIRE(x && q && scale, "null buffer");
-        const QuantArgs g{x, reinterpret_cast<signed char*>(q), scale, rows, ldx, ldq, dim, 0};
+        const QuantArgs g{x, reinterpret_cast<signed char*>(q), scale, rows, ldx, ldq, dim, 0, 0};
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         return dtype == FG_DTYPE_F32   ? launch_quantize<float>(g, s)
                : dtype == FG_DTYPE_F16 ? launch_quantize<__half>(g, s)

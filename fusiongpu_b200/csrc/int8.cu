@@ -299,7 +299,11 @@ __global__ void __launch_bounds__(128) gemv_int8_kernel(const signed char* __res
         const int v = __reduce_add_sync(0xffffffffu, acc[r]);
         if (lane == r) mine = v;
     }
-    if (lane < R && lane < g.m) epilogue_store<T>(e, lane, n, (float)mine * (xs[lane] * ws[n]));
+    if (lane < R && lane < g.m) {
+        Epilogue rest = e;  // the bias is in the product with the scales
+        rest.bias = nullptr;
+        epilogue_store<T>(rest, lane, n, fmaf((float)mine * ws[n], xs[lane], e.bias ? to_f32(static_cast<const T*>(e.bias)[n]) : 0.0f));
+    }
 }
 
 template <class T>

@@ -49,6 +49,7 @@ struct TcArgs {
     Epilogue e;
     int up;             // TC_GATED: rows of B from a gate's to its partner's
     const float *xs, *ws;  // TC_INT8: scales of A's and B's rows
+    int quads;             // ws on 16 bytes, n a multiple of 4
 };
 
 // Planes of the i-th plane product.
@@ -120,9 +121,9 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t a, uint32_t rank) {
     return v;
 }
 
-// An integer sum, its bits in a float's place, times its row's and column's scales.
-__device__ __forceinline__ float dequantised(float sum, float xs, float ws) {
-    return (float)__float_as_int(sum) * (xs * ws);
+// An integer sum, its bits in a float's place, times its column's and row's scales, and the bias.
+__device__ __forceinline__ float dequantised(float sum, float xs, float ws, float bias) {
+    return fmaf((float)__float_as_int(sum) * ws, xs, bias);
 }
 
 template <class T>
@@ -401,8 +402,8 @@ __global__ void __launch_bounds__(GT_NT, 1)
             const bool whole = col[u] + 4 <= g.n;
             if (PARTS) z = make_float4(z.x * scale, z.y * scale, z.z * scale, z.w * scale);
             if (MODE == TC_INT8) {
-                z = make_float4(dequantised(z.x, xs[u], by[u].x), dequantised(z.y, xs[u], by[u].y),
-                                dequantised(z.z, xs[u], by[u].z), dequantised(z.w, xs[u], by[u].w));
+                z = make_float4(dequantised(z.x, xs[u], by[u].x, bias[u].x), dequantised(z.y, xs[u], by[u].y, bias[u].y),
+                                dequantised(z.z, xs[u], by[u].z, bias[u].z), dequantised(z.w, xs[u], by[u].w, bias[u].w));
                 if (lost) z = make_float4(NAN, NAN, NAN, NAN);
             }
             auto retaken = [&](float4& z, int c) {
@@ -412,10 +413,12 @@ __global__ void __launch_bounds__(GT_NT, 1)
                 if (col[u] + 3 < g.n) z.w = finite_or_retake<T>(g, row[u], c + 3, z.w);
             };
             if (products > 1) retaken(z, col[u]);
-            z.x += bias[u].x;
-            z.y += bias[u].y;
-            z.z += bias[u].z;
-            z.w += bias[u].w;
+            if (MODE != TC_INT8) {
+                z.x += bias[u].x;
+                z.y += bias[u].y;
+                z.z += bias[u].z;
+                z.w += bias[u].w;
+            }
             auto put = [&](void* out, long long at, const float4& v) {
                 T* p = static_cast<T*>(out) + at;
                 if (g.vec && whole) {
@@ -477,10 +480,10 @@ constexpr int GP_NT = 64 + GP_EPI * 32;
 template <class T, int BN, int MODE>
 struct PairOf {
     static constexpr int B = BN / 2 * GT_K * 2, STAGE = GP_A + B;
-    static constexpr int STAGES = sizeof(T) == 4 ? 3 : MODE == TC_INT8 ? 4 : 5;
-    static constexpr int BUF = sizeof(T) == 4 ? 2 * GP_BUF : GP_BUF;
-    static constexpr int SCALES = sizeof(T) == 2 && MODE == TC_INT8 ? 256 : 0;  // a warp's 64 columns'
-    static constexpr int SMEM = STAGES * STAGE + GP_EPI * (BUF + (sizeof(T) == 4 ? 0 : 128) + SCALES);
+    static constexpr bool TWO = sizeof(T) == 4 || MODE == TC_INT8;  // buffers a warp
+    static constexpr int STAGES = TWO ? 3 : 5;
+    static constexpr int BUF = TWO ? 2 * GP_BUF : GP_BUF;
+    static constexpr int SMEM = STAGES * STAGE + GP_EPI * (BUF + (sizeof(T) == 4 ? 0 : 128));
     static constexpr int WARPS = BN / 64 * 4;         // epilogue warps of a tile
     static constexpr int GROUPS = GP_EPI / WARPS;     // that take tiles in turn
 };
@@ -581,6 +584,47 @@ __device__ __forceinline__ void add_bias(float (&v)[2][32], const unsigned char*
         for (int j = 0; j < 32; j += 8) add8<T>(&v[h][j], *reinterpret_cast<const uint4*>(b + (32 * h + j) * 2));
 }
 
+// Integer sums of 64 columns, times their scales and the row's, and the bias.  Columns past
+// the last take the last one's scale; they are not stored.  QUADS: scales on 16 bytes, their
+// number a multiple of 4.
+template <class T, bool QUADS>
+__device__ __forceinline__ void dequantise_all(float (&v)[2][32], const float* ws, int col, int n, float xs, const unsigned char* bias) {
+    const uint64_t x = pair2(xs, xs);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+            const int c = col + 32 * h + j;
+            float s[8], b[8];
+            if (QUADS) {
+                *reinterpret_cast<float4*>(s) = __ldg(reinterpret_cast<const float4*>(ws + min(c, n - 4)));
+                *reinterpret_cast<float4*>(s + 4) = __ldg(reinterpret_cast<const float4*>(ws + min(c + 4, n - 4)));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] = __ldg(ws + min(c + i, n - 1));
+            }
+            if (bias) {
+                const uint4 u = *reinterpret_cast<const uint4*>(bias + (32 * h + j) * 2);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = unpack2<T>(w[i]);
+                    b[2 * i] = f.x;
+                    b[2 * i + 1] = f.y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                float &p = v[h][j + i], &q = v[h][j + i + 1];
+                const uint64_t sum = pair2((float)__float_as_int(p), (float)__float_as_int(q));
+                unpair2(fma2(mul2(sum, pair2(s[i], s[i + 1])), x, pair2(b[i], b[i + 1])), p, q);
+            }
+        }
+}
+
 // Waits for a copy into a buffer of this warp.  When another role has failed the first
 // wait ends early, and the copy, which may still land, is waited for by itself.
 __device__ __forceinline__ bool copy_landed(uint64_t* bar, uint32_t parity, volatile int* fail) {
@@ -615,7 +659,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     static_assert(sizeof(T) == 2 || BN == 256, "float32 takes 256 columns");
     static_assert(MODE != TC_GATED || (BN == 256 && !DIRECT), "gated tiles have 128 columns and TMA stores");
     extern __shared__ __align__(1024) unsigned char dsmem[];
-    __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], acc_full[2], acc_empty[2], res_full[GP_EPI];
+    __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], acc_full[2], acc_empty[2], res_full[MODE == TC_INT8 ? 2 * GP_EPI : GP_EPI];
     __shared__ uint32_t tmem_slot;
     __shared__ int s_fail, s_odd;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -646,7 +690,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             tc::mbar_init(&acc_full[i], 1);
             tc::mbar_init(&acc_empty[i], 2 * P::WARPS);
         }
-        for (int w = 0; w < GP_EPI; ++w) tc::mbar_init(&res_full[w], 1);
+        for (int w = 0; w < (MODE == TC_INT8 ? 2 * GP_EPI : GP_EPI); ++w) tc::mbar_init(&res_full[w], 1);
         tc::fence_mbar_init();
     }
     if (tid == 0 && (tc::smem_u32(dsmem) & 1023)) s_fail = 1;  // swizzled tiles start on 1,024 bytes
@@ -751,7 +795,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
         int item = (blockIdx.x >> 1) + pairs * group, li = group;
         bool lost = false;      // a residual never came: this warp's results are NaN from there on
         bool odd_seen = false;  // a result that is not finite, stored as NaN and taken again at the end
-        const bool ahead = sizeof(T) == 2 && e.residual && !e.pre;  // residuals a tile ahead (DIRECT: during its products)
+        const bool ahead = sizeof(T) == 2 && MODE != TC_INT8 && e.residual && !e.pre;  // residuals a tile ahead (DIRECT: during its products)
         if (!DIRECT && ahead && item < items && tc::elect_one()) fetch_residual(item);
         if constexpr (sizeof(T) == 4) {
             // Chunks of k are added to the sums in shared memory, a lane its own row, in
@@ -775,9 +819,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         tc::tmem_ld_32x32(taddr + ((uint32_t)(q4 * 32) << 16) +
                                               (uint32_t)(acc * BN + part * PC + (MODE == TC_GATED ? BO : 32) * h), v);
                         if (MODE == TC_INT8) {
+                            const float* bias = static_cast<const float*>(e.bias);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                v[j] = dequantised(v[j], xs, col + 32 * h + j < g.n ? __ldg(g.ws + col + 32 * h + j) : 0.0f);
+                            for (int j = 0; j < 32; ++j) {
+                                const int c = min(col + 32 * h + j, g.n - 1);  // columns past the last are not stored
+                                v[j] = dequantised(v[j], xs, __ldg(g.ws + c), bias ? __ldg(bias + c) : 0.0f);
+                            }
                         }
                         if (h == 1) {
                             tc::fence_before_sync();
@@ -889,7 +936,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = fabsf(v[j]) <= FLT_MAX ? v[j] : NAN;
                     }
-                    if (e.bias) {
+                    if (MODE != TC_INT8 && e.bias) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
                             if (c0 + j < g.n) v[j] += __ldg(static_cast<const float*>(e.bias) + c0 + j);
@@ -1006,6 +1053,96 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     tc::bulk_commit();
                 }
             }
+        } else if constexpr (MODE == TC_INT8) {
+            // The products of a tile take 512 cycles for 128 k, so that the epilogue bounds it: two
+            // buffers a warp, and the next tile's residual travels during this one's epilogue (1M x
+            // 768 -> 768 float16 with residual: 946 us with one buffer).  The columns' scales come
+            // from L1, which the operands pass by.
+            T* residual = const_cast<T*>(static_cast<const T*>(e.residual));
+            auto fetch = [&](int it, int i) {  // lane 0, once the buffer is free
+                tc::mbar_arrive_expect_tx(&res_full[2 * w + (i & 1)], GP_BUF);
+                tc::tma_load_2d(buf + (i & 1) * GP_BUF, &tr, &res_full[2 * w + (i & 1)], it % g.nt * BN + part * 64,
+                                it / g.nt * 2 * GT_M + tr_rows);
+            };
+            if (!DIRECT && e.residual && item < items && tc::elect_one()) fetch(item, 0);
+            bool flying = false;  // after a copy that never came: the next one is under way, and lands before the block ends
+            for (int i = 0; item < items; item += step, li += P::GROUPS, ++i) {
+                const int acc = li & 1, col = item % g.nt * BN + part * 64, m0 = item / g.nt * 2 * GT_M + tr_rows;
+                unsigned char *ibuf = buf + (i & 1) * GP_BUF, *irow = ibuf + lane * 128;
+                if (lost) {
+                    if (flying) tc::mbar_wait(&res_full[2 * w + (i & 1)], (i >> 1) & 1);
+                    flying = false;
+                    store_nan<T>(e.y, e.ldy, m0, col, g.m, g.n, 64);
+                    continue;
+                }
+                if (!DIRECT) {
+                    if (tc::elect_one()) {
+                        tc::bulk_wait_read<0>();  // the last tile's results have left the other buffer
+                        if (e.residual && item + step < items) fetch(item + step, i + 1);
+                    }
+                    __syncwarp();
+                }
+                unsigned char* bias = biases + w * 128;
+                if (e.bias) {
+                    reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(static_cast<const T*>(e.bias) + col, lane, g.n - col, DIRECT);
+                    __syncwarp();
+                }
+                if (DIRECT && e.residual) copy_rows<T, false, 8>(ibuf, residual, e.ldr, m0, col, g.m, g.n, lane);
+                const float xs = m0 + lane < g.m ? __ldg(g.xs + m0 + lane) : 0.0f;
+                const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
+                tc::fence_after_sync();
+                const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + part * 64);
+                float v[2][32];
+                tc::tmem_ld_32x32_nowait(src, v[0]);
+                tc::tmem_ld_32x32_nowait(src + 32, v[1]);
+                tc::tmem_ld_wait(v[0]);
+                tc::tmem_ld_wait(v[1]);
+                tc::fence_before_sync();
+                __syncwarp();
+                if (tc::elect_one()) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
+                if (g.quads)
+                    dequantise_all<T, true>(v, g.ws, col, g.n, xs, e.bias ? bias : nullptr);
+                else
+                    dequantise_all<T, false>(v, g.ws, col, g.n, xs, e.bias ? bias : nullptr);
+                if (!ok) {  // a wait that ran out leaves NaN, not a plausible number
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[0][j] = v[1][j] = NAN;
+                }
+                switch (e.act) {
+                    case FG_ACT_RELU: activate_all<FG_ACT_RELU>(v); break;
+                    case FG_ACT_GELU: activate_all<FG_ACT_GELU>(v); break;
+                    case FG_ACT_SILU: activate_all<FG_ACT_SILU>(v); break;
+                }
+                if (e.residual) {
+                    if (!DIRECT) {
+                        lost = flying = !copy_landed(&res_full[2 * w + (i & 1)], (i >> 1) & 1, fail);
+                        if (lost) {
+                            store_nan<T>(e.y, e.ldy, m0, col, g.m, g.n, 64);
+                            continue;
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8)
+                            add8<T>(&v[h][j], *reinterpret_cast<const uint4*>(irow + (((uint32_t)(32 * h + j) << 1) ^ sw)));
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        *reinterpret_cast<uint4*>(irow + (((uint32_t)(32 * h + j) << 1) ^ sw)) = pack8<T>(&v[h][j]);
+                if (DIRECT) {
+                    copy_rows<T, true, 1>(ibuf, static_cast<T*>(e.y), e.ldy, m0, col, g.m, g.n, lane);
+                    continue;
+                }
+                tc::fence_proxy_async();
+                __syncwarp();
+                if (tc::elect_one()) {
+                    if (m0 < g.m && col < g.n) tc::tma_store_2d(&ty, ibuf, col, m0);
+                    tc::bulk_commit();
+                }
+            }
         } else {
         for (; item < items; item += step, li += P::GROUPS) {
             const int acc = li & 1, t = item / g.split;
@@ -1021,14 +1158,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(static_cast<const T*>(e.bias) + col, lane, g.n - col, DIRECT);
                 __syncwarp();
             }
-            float xs = 0.0f;
-            float* scales = reinterpret_cast<float*>(biases + GP_EPI * 128 + w * P::SCALES);
-            if (MODE == TC_INT8) {
-                if (m0 + lane < g.m) xs = g.xs[m0 + lane];
-                scales[lane] = col + lane < g.n ? g.ws[col + lane] : 0.0f;
-                scales[lane + 32] = col + lane + 32 < g.n ? g.ws[col + lane + 32] : 0.0f;
-                __syncwarp();
-            }
             T* residual = const_cast<T*>(static_cast<const T*>(e.residual));
             if (DIRECT && ahead) copy_rows<T, false, 8>(buf, residual, e.ldr, m0, col, g.m, g.n, lane);
             const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
@@ -1042,18 +1171,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
             tc::fence_before_sync();
             __syncwarp();
             if (tc::elect_one()) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
-            if (MODE == TC_INT8) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 c = *reinterpret_cast<const float4*>(scales + 32 * h + j);
-                        v[h][j] = dequantised(v[h][j], xs, c.x);
-                        v[h][j + 1] = dequantised(v[h][j + 1], xs, c.y);
-                        v[h][j + 2] = dequantised(v[h][j + 2], xs, c.z);
-                        v[h][j + 3] = dequantised(v[h][j + 3], xs, c.w);
-                    }
-            }
             if (g.split > 1) {  // this part's sums as they are; finish_kernel adds the parts
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -1524,6 +1641,7 @@ int tc_int8(int dtype, const void* a, const float* xs, const void* b, const floa
     g.xs = xs;
     g.ws = ws;
     g.vec = epilogue_lies(e, es, 4 * es) && aligned(ws, 16);
+    g.quads = aligned(ws, 16) && s.n % 4 == 0;
     g.direct = !epilogue_lies(e, es, 16);
     GemmShape half = s;  // a K block holds 128 codes and takes the time of 64 elements of 16 bits
     half.k = (s.k + 1) / 2;

@@ -49,7 +49,7 @@ struct TcArgs {
     Epilogue e;
     int up;             // TC_GATED: rows of B from a gate's to its partner's
     const float *xs, *ws;  // TC_INT8: scales of A's and B's rows
-    int quads;             // ws on 16 bytes, n a multiple of 4
+    int quads;             // ws (and a 32-bit bias) on 16 bytes, n a multiple of 4
 };
 
 // Planes of the i-th plane product.
@@ -503,17 +503,17 @@ __device__ __forceinline__ void add8(float* v, uint4 u) {
     }
 }
 
-template <int ACT>
+template <int ACT, bool FAST = true>
 __device__ __forceinline__ void activate_all(float (&v)[2][32]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
-            if (ACT == FG_ACT_GELU) {
+            if (ACT == FG_ACT_GELU && FAST) {
                 gelu2(v[h][j], v[h][j + 1]);
             } else {
-                v[h][j] = activate<true>(v[h][j], ACT);
-                v[h][j + 1] = activate<true>(v[h][j + 1], ACT);
+                v[h][j] = activate<FAST>(v[h][j], ACT);
+                v[h][j + 1] = activate<FAST>(v[h][j + 1], ACT);
             }
         }
 }
@@ -585,8 +585,8 @@ __device__ __forceinline__ void add_bias(float (&v)[2][32], const unsigned char*
 }
 
 // Integer sums of 64 columns, times their scales and the row's, and the bias.  Columns past
-// the last take the last one's scale; they are not stored.  QUADS: scales on 16 bytes, their
-// number a multiple of 4.
+// the last take the last one's scale; they are not stored.  QUADS: scales (and a bias of 32
+// bits, which lies in global memory) on 16 bytes, their number a multiple of 4.
 template <class T, bool QUADS>
 __device__ __forceinline__ void dequantise_all(float (&v)[2][32], const float* ws, int col, int n, float xs, const unsigned char* bias) {
     const uint64_t x = pair2(xs, xs);
@@ -603,12 +603,21 @@ __device__ __forceinline__ void dequantise_all(float (&v)[2][32], const float* w
 #pragma unroll
                 for (int i = 0; i < 8; ++i) s[i] = __ldg(ws + min(c + i, n - 1));
             }
-            if (bias) {
+            if (bias && sizeof(T) == 4) {
+                const float* f = reinterpret_cast<const float*>(bias);
+                if (QUADS) {
+                    *reinterpret_cast<float4*>(b) = __ldg(reinterpret_cast<const float4*>(f + min(c, n - 4)));
+                    *reinterpret_cast<float4*>(b + 4) = __ldg(reinterpret_cast<const float4*>(f + min(c + 4, n - 4)));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b[i] = __ldg(f + min(c + i, n - 1));
+                }
+            } else if (bias) {
                 const uint4 u = *reinterpret_cast<const uint4*>(bias + (32 * h + j) * 2);
                 const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 f = unpack2<T>(w[i]);
+                    const float2 f = unpack2<typename std::conditional<sizeof(T) == 4, __half, T>::type>(w[i]);
                     b[2 * i] = f.x;
                     b[2 * i + 1] = f.y;
                 }
@@ -797,7 +806,93 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
         bool odd_seen = false;  // a result that is not finite, stored as NaN and taken again at the end
         const bool ahead = sizeof(T) == 2 && MODE != TC_INT8 && e.residual && !e.pre;  // residuals a tile ahead (DIRECT: during its products)
         if (!DIRECT && ahead && item < items && tc::elect_one()) fetch_residual(item);
-        if constexpr (sizeof(T) == 4) {
+        if constexpr (MODE == TC_INT8 && sizeof(T) == 4) {
+            // Bound by the results' bytes; both halves of 32 columns have a buffer, which the residual
+            // fills during the products.
+            float* residual = const_cast<float*>(static_cast<const float*>(e.residual));
+            for (int i = 0; item < items; item += step, li += P::GROUPS, ++i) {
+                const int acc = li & 1, col = item % g.nt * BN + part * 64, m0 = item / g.nt * 2 * GT_M + tr_rows;
+                if (lost) {
+                    store_nan<T>(e.y, e.ldy, m0, col, g.m, g.n, 64);
+                    continue;
+                }
+                if (!DIRECT) {
+                    if (tc::elect_one()) {
+                        if (e.residual) {
+                            tc::bulk_wait_read<0>();
+                            tc::mbar_arrive_expect_tx(&res_full[w], 2 * GP_BUF);
+                            for (int h = 0; h < 2; ++h) tc::tma_load_2d(buf + h * GP_BUF, &tr, &res_full[w], col + 32 * h, m0);
+                        }
+                    }
+                    __syncwarp();
+                } else if (e.residual) {
+                    for (int h = 0; h < 2; ++h)
+                        copy_rows<T, false, 8>(buf + h * GP_BUF, residual, e.ldr, m0, col + 32 * h, g.m, g.n, lane);
+                }
+                const float xs = m0 + lane < g.m ? __ldg(g.xs + m0 + lane) : 0.0f;
+                const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
+                tc::fence_after_sync();
+                const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(acc * BN + part * 64);
+                float v[2][32];
+                tc::tmem_ld_32x32_nowait(src, v[0]);
+                tc::tmem_ld_32x32_nowait(src + 32, v[1]);
+                tc::tmem_ld_wait(v[0]);
+                tc::tmem_ld_wait(v[1]);
+                tc::fence_before_sync();
+                __syncwarp();
+                if (tc::elect_one()) tc::mbar_arrive_leader(tc::leader_addr(&acc_empty[acc]));
+                if (g.quads)
+                    dequantise_all<T, true>(v, g.ws, col, g.n, xs, static_cast<const unsigned char*>(e.bias));
+                else
+                    dequantise_all<T, false>(v, g.ws, col, g.n, xs, static_cast<const unsigned char*>(e.bias));
+                if (!ok) {  // a wait that ran out leaves NaN, not a plausible number
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[0][j] = v[1][j] = NAN;
+                }
+                switch (e.act) {
+                    case FG_ACT_RELU: activate_all<FG_ACT_RELU, false>(v); break;
+                    case FG_ACT_GELU: activate_all<FG_ACT_GELU, false>(v); break;
+                    case FG_ACT_SILU: activate_all<FG_ACT_SILU, false>(v); break;
+                }
+                if (e.residual && !DIRECT) {
+                    lost = !copy_landed(&res_full[w], i & 1, fail);
+                    if (lost) {
+                        store_nan<T>(e.y, e.ldy, m0, col, g.m, g.n, 64);
+                        continue;
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    unsigned char* hrow = brow + h * GP_BUF;
+                    if (e.residual) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 r = *reinterpret_cast<const float4*>(hrow + (((uint32_t)j << 2) ^ sw));
+                            v[h][j] += r.x;
+                            v[h][j + 1] += r.y;
+                            v[h][j + 2] += r.z;
+                            v[h][j + 3] += r.w;
+                        }
+                    } else if (!DIRECT) {  // this half's results of the last tile have left it
+                        if (tc::elect_one()) tc::bulk_wait_read<1>();
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<float4*>(hrow + (((uint32_t)j << 2) ^ sw)) = make_float4(v[h][j], v[h][j + 1], v[h][j + 2], v[h][j + 3]);
+                    if (DIRECT) {
+                        copy_rows<T, true, 1>(buf + h * GP_BUF, static_cast<T*>(e.y), e.ldy, m0, col + 32 * h, g.m, g.n, lane);
+                        continue;
+                    }
+                    tc::fence_proxy_async();
+                    __syncwarp();
+                    if (tc::elect_one()) {
+                        if (m0 < g.m && col + 32 * h < g.n) tc::tma_store_2d(&ty, buf + h * GP_BUF, col + 32 * h, m0);
+                        tc::bulk_commit();
+                    }
+                }
+            }
+        } else if constexpr (sizeof(T) == 4) {
             // Chunks of k are added to the sums in shared memory, a lane its own row, in
             // two halves of 32 columns; the last one is followed by the epilogue proper,
             // one step after the other: six products a K block hide it.
@@ -805,8 +900,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 const int t = item / g.split, sp = item - t * g.split, k1 = k_begin(sp + 1);
                 const int col = t % g.nt * BO + part * PC, m0 = t / g.nt * 2 * GT_M + tr_rows;
                 bool all_ok = true;
-                float xs = 0.0f;
-                if (MODE == TC_INT8 && m0 + lane < g.m) xs = g.xs[m0 + lane];
                 if (tc::elect_one()) tc::bulk_wait_read<0>();
                 __syncwarp();
                 for (int c0 = k_begin(sp), first = 1; c0 < k1; c0 += min(chunk, k1 - c0), first = 0, ++li) {
@@ -818,14 +911,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         float v[32];
                         tc::tmem_ld_32x32(taddr + ((uint32_t)(q4 * 32) << 16) +
                                               (uint32_t)(acc * BN + part * PC + (MODE == TC_GATED ? BO : 32) * h), v);
-                        if (MODE == TC_INT8) {
-                            const float* bias = static_cast<const float*>(e.bias);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const int c = min(col + 32 * h + j, g.n - 1);  // columns past the last are not stored
-                                v[j] = dequantised(v[j], xs, __ldg(g.ws + c), bias ? __ldg(bias + c) : 0.0f);
-                            }
-                        }
                         if (h == 1) {
                             tc::fence_before_sync();
                             __syncwarp();
@@ -927,16 +1012,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                                 make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                     };
                     bool odd = false;
-                    if (PLANES) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) odd |= !(fabsf(v[j]) <= FLT_MAX);
-                    }
+                    for (int j = 0; j < 32; ++j) odd |= !(fabsf(v[j]) <= FLT_MAX);
                     if (__any_sync(0xffffffffu, odd && all_ok)) {
                         odd_seen = true;
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = fabsf(v[j]) <= FLT_MAX ? v[j] : NAN;
                     }
-                    if (MODE != TC_INT8 && e.bias) {
+                    if (e.bias) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
                             if (c0 + j < g.n) v[j] += __ldg(static_cast<const float*>(e.bias) + c0 + j);
@@ -1641,7 +1724,7 @@ int tc_int8(int dtype, const void* a, const float* xs, const void* b, const floa
     g.xs = xs;
     g.ws = ws;
     g.vec = epilogue_lies(e, es, 4 * es) && aligned(ws, 16);
-    g.quads = aligned(ws, 16) && s.n % 4 == 0;
+    g.quads = aligned(ws, 16) && s.n % 4 == 0 && (es == 2 || aligned(e.bias, 16));
     g.direct = !epilogue_lies(e, es, 16);
     GemmShape half = s;  // a K block holds 128 codes and takes the time of 64 elements of 16 bits
     half.k = (s.k + 1) / 2;

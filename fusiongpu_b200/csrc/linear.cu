@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(128) gemv_kernel(const T* __restrict__ x, cons
     constexpr int VEC = 16 / sizeof(T);
     const int lane = threadIdx.x & 31;
     const long long n = (blockIdx.x * 4ll + (threadIdx.x >> 5)) * (GATED ? 1 : C);
-    if (n >= g.n) return;
+    if (n >= (GATED ? up : g.n)) return;
     const T *wr[C], *xr[R];  // rows and columns past the last are the last again: no branch keeps loads apart
 #pragma unroll
     for (int c = 0; c < C; ++c) wr[c] = w + (GATED ? n + (c ? up : 0) : min(n + c, g.n - 1)) * g.bn;

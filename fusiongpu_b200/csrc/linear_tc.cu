@@ -481,8 +481,9 @@ template <class T, int BN, int MODE>
 struct PairOf {
     static constexpr int B = BN / 2 * GT_K * 2, STAGE = GP_A + B;
     static constexpr bool TWO = sizeof(T) == 4 || MODE == TC_INT8;  // buffers a warp
-    static constexpr int STAGES = TWO ? 3 : 5;
-    static constexpr int BUF = TWO ? 2 * GP_BUF : GP_BUF;
+    static constexpr bool GATED = sizeof(T) == 2 && MODE == TC_GATED;  // room for both pre-activations and the result
+    static constexpr int STAGES = TWO ? 3 : GATED ? 4 : 5;
+    static constexpr int BUF = TWO ? 2 * GP_BUF : GATED ? GP_BUF * 3 / 2 : GP_BUF;
     static constexpr int SMEM = STAGES * STAGE + GP_EPI * (BUF + (sizeof(T) == 4 ? 0 : 128));
     static constexpr int WARPS = BN / 64 * 4;         // epilogue warps of a tile
     static constexpr int GROUPS = GP_EPI / WARPS;     // that take tiles in turn
@@ -653,8 +654,8 @@ __device__ __noinline__ void store_nan(void* matrix, long long ld, int row0, int
 //
 // TC_GATED: the leader holds 128 gates' rows of B and its peer their partners', so that
 // an accumulator's halves are the two factors of 128 outputs; a warp takes 32 of each.
-// 16-bit results leave in rows of 64 bytes (64-byte swizzle), both pre-activations
-// through the two halves of a warp's buffer.
+// 16-bit results leave in rows of 64 bytes (64-byte swizzle); both pre-activations and the
+// result have 2 KB each of a warp's buffer, so that none waits for another's store.
 template <class T, int BN, bool DIRECT, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
@@ -1103,9 +1104,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         *reinterpret_cast<uint4*>(buf + h * (GP_BUF / 2) + lane * 64 + (((uint32_t)j << 1) ^ sw64)) = pack8<T>(&v[j]);
                 };
                 const bool inside = m0 < g.m && col < g.n;
-                if (tc::elect_one()) tc::bulk_wait_read<0>();
-                __syncwarp();
                 if (e.pre) {
+                    if (tc::elect_one()) tc::bulk_wait_read<1>();  // the last tile's: its result may still leave
+                    __syncwarp();
                     stage(v[0], 0);
                     stage(v[1], 1);
                     tc::fence_proxy_async();
@@ -1124,15 +1125,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     case FG_ACT_SILU: gate_all<FG_ACT_SILU>(v); break;
                     default: gate_all<FG_ACT_NONE>(v);
                 }
-                if (e.pre) {
-                    if (tc::elect_one()) tc::bulk_wait_read<0>();
-                    __syncwarp();
+                if (tc::elect_one()) {  // the last tile's result has left; this one's pre-activations may yet
+                    if (e.pre)
+                        tc::bulk_wait_read<1>();
+                    else
+                        tc::bulk_wait_read<0>();
                 }
-                stage(v[0], 0);
+                __syncwarp();
+                stage(v[0], 2);
                 tc::fence_proxy_async();
                 __syncwarp();
                 if (tc::elect_one()) {
-                    if (inside) tc::tma_store_2d(&ty, buf, col, m0);
+                    if (inside) tc::tma_store_2d(&ty, buf + GP_BUF, col, m0);
                     tc::bulk_commit();
                 }
             }
@@ -1643,9 +1647,9 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct, int mode
 // tiles (1777 x 101 -> 333 bf16: 27 us with pairs, 12 in tiles of 64 columns).  Only
 // tiles whose sums are not split are chosen anew: those add in one order whichever
 // kernel takes them, so that a result does not depend on where it is written.
-static TcPlan tc_plan(const GemmShape& s, int products, bool direct) {
-    const TcPlan p = tc_plan_of(s, products, false);
-    return direct && p.split == 1 ? tc_plan_of(s, products, true) : p;
+static TcPlan tc_plan(const GemmShape& s, int products, bool direct, int mode = TC_WHOLE) {
+    const TcPlan p = tc_plan_of(s, products, false, mode);
+    return direct && p.split == 1 ? tc_plan_of(s, products, true, mode) : p;
 }
 
 static TcArgs tc_args(const void* a, long long a_plane, const void* b, long long b_plane, const GemmShape& s, int products,
@@ -1705,7 +1709,7 @@ int tc_gated(int dtype, const void* a, long long a_plane, const void* b, long lo
     auto both = [&](int n) { return epilogue_lies(e, es, n) && ((!e.bias && !e.pre) || (long long)g.up * es % n == 0); };
     g.vec = both(4 * es);
     g.direct = !both(16);
-    const TcPlan p = tc_plan_of(s, g.products, g.direct, TC_GATED);
+    const TcPlan p = tc_plan(s, g.products, g.direct, TC_GATED);
     g.split = p.split;
 #define FG_PRODUCT(T)                                                            \
     (p.pair        ? launch_pair<T, 256, TC_GATED>(dtype, a, b, s, g, nullptr, st) \

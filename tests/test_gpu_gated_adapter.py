@@ -436,6 +436,65 @@ def test_linear_int8_beyond_32_bit_offsets(ad):
     assert torch.equal(y[:300], small) and torch.equal(y[-300:], small)
 
 
+def _framed(rows, cols, t, lead=3, tail=5, above=2):
+    """A matrix within a larger one of a value that no result takes, and the larger one."""
+    frame = torch.full((rows + 2 * above, lead + cols + tail), 77.0, device="cuda").to(t)
+    return frame[above:above + rows, lead:lead + cols], frame
+
+
+def _frame_stayed(frame, view):
+    clean = frame.clone()
+    off = (view.data_ptr() - frame.data_ptr()) // frame.element_size()
+    r, c = off // frame.shape[1], off % frame.shape[1]
+    clean[r:r + view.shape[0], c:c + view.shape[1]] = 77
+    return bool((clean == 77).all())
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 8, 9, 130, 700, 20000])
+@pytest.mark.parametrize("i,o", [(33, 17), (40, 1), (64, 130), (72, 200), (16, 66)])
+def test_results_stay_within_their_matrices(ad, n, i, o, t):
+    """Through the C ABI, into the middle of larger matrices: what lies around the results
+    is left as it was, and they are the values of the Python call."""
+    import ctypes as C
+
+    from fusiongpu_b200 import _lib
+    L, s = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(1 << 27, dtype=torch.uint8, device="cuda")
+    g = _gen(n + o)
+    x, w, b = _randn(g, n, i, t=t), _randn(g, 2 * o, i, t=t, scale=0.2), _randn(g, 2 * o, t=t)
+    for lead in (3, 8):
+        y, fy = _framed(n, o, T[t], lead)
+        pre, fp = _framed(n, 2 * o, T[t], lead)
+        p = _lib.LinearParams(n, i, o, ad.DTYPES[T[t]], 3, 0, 0, 0, pre.stride(0), y.stride(0), 0)
+        _lib.check(L.fg_gated_linear(C.byref(p), x.data_ptr(), w.data_ptr(), b.data_ptr(), pre.data_ptr(), y.data_ptr(),
+                                     ws.data_ptr(), ws.numel(), s), "fg_gated_linear")
+        ry, rp = ad.gated_linear(x, w, b, return_pre=True)
+        assert torch.equal(y, ry) and torch.equal(pre, rp)
+        assert _frame_stayed(fy, y) and _frame_stayed(fp, pre)
+        q, xs = ad.quantize_rows(x)
+        wq, wsc = ad.quantize_rows(w)
+        y, fy = _framed(n, 2 * o, T[t], lead)
+        p = _lib.LinearParams(n, i, 2 * o, ad.DTYPES[T[t]], 2, q.stride(0), wq.stride(0), 0, 0, y.stride(0), 0)
+        _lib.check(L.fg_linear_int8(C.byref(p), q.data_ptr(), xs.data_ptr(), wq.data_ptr(), wsc.data_ptr(), b.data_ptr(), None,
+                                    y.data_ptr(), ws.data_ptr(), ws.numel(), s), "fg_linear_int8")
+        assert torch.equal(y, ad.linear_int8(q, xs, wq, wsc, b, activation="gelu", dtype=T[t])) and _frame_stayed(fy, y)
+        codes, fc = _framed(n, i, torch.int8, lead)
+        scale, fs = _framed(1, n, torch.float32, lead)
+        _lib.check(L.fg_quantize_rows(x.data_ptr(), ad.DTYPES[T[t]], n, i, 0, codes.data_ptr(), codes.stride(0),
+                                      scale.data_ptr(), s), "fg_quantize_rows")
+        assert torch.equal(codes, q) and torch.equal(scale[0], xs) and _frame_stayed(fc, codes) and _frame_stayed(fs, scale)
+    dy = _randn(g, n, o, t=t)
+    want = ad.gated_linear_backward(dy, x, w, rp)
+    frames = [_framed(1, v.numel(), T[t]) for v in want]
+    p = _lib.LinearParams(n, i, o, ad.DTYPES[T[t]], 3, 0, 0, 0, 0, 0, 7)
+    off = [v.data_ptr() for v, _ in frames]
+    _lib.check(L.fg_gated_linear_backward(C.byref(p), dy.data_ptr(), x.data_ptr(), w.data_ptr(), rp.data_ptr(), *off,
+                                          ws.data_ptr(), ws.numel(), s), "fg_gated_linear_backward")
+    for (v, f), r in zip(frames, want):
+        assert torch.equal(v.view(r.shape), r) and _frame_stayed(f, v)
+
+
 def test_refusals(ad):
     x, w = torch.zeros(4, 32, device="cuda"), torch.zeros(20, 32, device="cuda")
     with pytest.raises(ValueError):

@@ -159,6 +159,28 @@ def test_orthogonalize_ends(ad):
     assert ad.orthogonalize(torch.zeros(0, 5, 4, device="cuda")).shape == (0, 5, 4)
 
 
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("batch,m,n", [(1, 5, 7), (2, 100, 33), (3, 33, 257), (1, 300, 129), (2, 131, 515)])
+def test_orthogonalize_stays_within_its_matrices(ad, batch, m, n, t):
+    """Through the C ABI: what lies around the result and the workspace is left as it was."""
+    import ctypes as C
+
+    from fusiongpu_b200 import _lib
+    g = torch.randn(batch, m, n, generator=_gen(n), device="cuda").to(T[t])
+    for steps in (0, 1, 5):
+        p = _lib.OrthogonalizeParams(batch, m, n, ad.DTYPES[T[t]], steps, *COEF, 1e-7, 0, 0)
+        need = _lib.size_query("fg_orthogonalize_workspace_size", C.byref(p))
+        ws = torch.full((need + 512,), 77, dtype=torch.uint8, device="cuda")
+        frame = torch.full((batch * m * n + 14,), 77.0, device="cuda").to(T[t])
+        _lib.check(_lib.lib().fg_orthogonalize(C.byref(p), g.data_ptr(), frame[7:].data_ptr(), ws[256:].data_ptr(), need,
+                                               torch.cuda.current_stream().cuda_stream), "fg_orthogonalize")
+        got = frame[7:-7].view(batch, m, n)
+        want = ad.orthogonalize(g, steps=steps)
+        assert torch.equal(got, want)
+        assert (frame[:7] == 77).all() and (frame[-7:] == 77).all()
+        assert (ws[:256] == 77).all() and (ws[256 + need:] == 77).all()
+
+
 def test_orthogonalize_refusals(ad):
     from fusiongpu_b200._lib import FgError
     x = torch.ones(4, 6, device="cuda")

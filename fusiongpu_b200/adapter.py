@@ -127,6 +127,12 @@ def _linear_ws(query: str, n: int, i: int, o: int, dtype: int, act: int, ldx: in
     return _lib.size_query(query, C.byref(_lib.LinearParams(n, i, o, dtype, act, ldx, ldw, 0, 0, ldy, off)))
 
 
+@functools.lru_cache(maxsize=1024)
+def _orthogonalize_ws(batch: int, m: int, n: int, dtype: int, steps: int) -> int:
+    return _lib.size_query("fg_orthogonalize_workspace_size",
+                           C.byref(_lib.OrthogonalizeParams(batch, m, n, dtype, steps, 0, 0, 0, 0, 0, 0)))
+
+
 def _off16(*pointers: int) -> int:
     """fg_linear_operand bits of the pointers (x, w, dy) that are off 16 bytes."""
     off = 0
@@ -395,10 +401,10 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients: tuple[float, fl
         s1 = n
     ld = s1 if m > 1 else n
     out = torch.empty_strided(g.shape, (n, 1) if g.dim() == 2 else (m * n, n, 1), dtype=g.dtype, device=g.device)
-    p = _lib.OrthogonalizeParams(batch, m, n, DTYPES[g.dtype], steps, *coefficients, eps, ld,
-                                 g.stride(0) if batch > 1 else 0)
-    nws = _lib.size_query("fg_orthogonalize_workspace_size", C.byref(p))
-    ws = torch.empty(nws, dtype=torch.uint8, device=g.device)
+    a, b, c = coefficients
+    p = _lib.OrthogonalizeParams(batch, m, n, DTYPES[g.dtype], steps, a, b, c, eps, ld, g.stride(0) if batch > 1 else 0)
+    nws = _orthogonalize_ws(batch, m, n, DTYPES[g.dtype], steps)
+    ws = torch.empty(nws, dtype=torch.uint8, device=g.device) if nws else None
     _lib.check(_lib.lib().fg_orthogonalize(C.byref(p), g.data_ptr(), out.data_ptr(), _ptr(ws), nws, _stream(g)),
                "fg_orthogonalize")
     return out

@@ -12,6 +12,12 @@
 // to a^steps, and with one float16 plane the result was off by 2.4e-3 of its norm, with
 // one bfloat16 plane by 1.8e-2, with two by 6e-7 (float32 throughout: 2e-6).  Singular
 // values stay of order one, so that float16's range holds them.
+//
+// The tensor cores cut their sums, always towards zero: 1,024 k in one accumulator, and a I
+// as part of Y in X = Y X (or the completed square c (A + b / 2c)^2, which spares B's
+// addend), left 1.4e-5 of float32 results.  So a X and b A are added behind the products,
+// and sums are taken from the accumulators after ORTH_RUN blocks of 64 k and added in
+// fp32.
 #include <algorithm>
 #include <type_traits>
 
@@ -22,7 +28,7 @@ namespace fg {
 
 constexpr int OT_M = 128, OT_K = 64, OT_NT = 64 + 256;
 constexpr int LOW_SHIFT = 11;  // h + 2^-11 l
-constexpr int ORTH_RUN = 8;    // K blocks (512 k) that an accumulator sums before the next one is taken, where TMEM allows
+constexpr int ORTH_RUN = 4;    // K blocks (256 k) that an accumulator sums
 
 __device__ __forceinline__ void planes_of(float v, __half& h, __half& l) {
     h = __float2half_rn(v);
@@ -149,11 +155,13 @@ __global__ void __launch_bounds__(OI_NT) orth_scale_kernel(const OrthIn g) {
 
 // ---- products ------------------------------------------------------------------------
 //
-// D(m, n) = beta (sum over k of P(m, k) Q(n, k)) + alpha C(m, n), and `diag` where m = n.  A 128 x BN tile a
+// D(m, n) = beta (sum over k of P(m, k) Q(n, k)) + alpha C(m, n).  A 128 x BN tile a
 // cluster, its K blocks divided over the cluster's CTAs, partial tiles added through
 // distributed shared memory.  A stage of the ring holds both planes of both operands for
 // 64 k, which three products share: h h' into one accumulator, h l' and l h' into
-// another, that counts 2^-11 of it.
+// another, that counts 2^-11 of it.  The epilogue warps take the first one's sums into
+// registers after each run; the next run's products of l come first, behind which that
+// hides.
 //
 // SYM: D is symmetric.  Tiles above the diagonal are left out; an element below it is
 // written to both its places.
@@ -166,7 +174,7 @@ struct OrthArgs {
     int p_mn, q_mn;               // the operand's unit stride is along its rows
     int split;
     int sym, vec;                 // vec: `out` allows 4-column stores
-    float alpha, beta, diag;
+    float alpha, beta;
     const __half* c;              // NULL: none
     __half* d;                    // NULL: `out`
     void* out;                    // [batch][m][n]
@@ -177,9 +185,8 @@ struct OrthArgs {
 template <int BN>
 struct OrthRing {
     static constexpr int A = 2 * OT_M * OT_K * 2, B = 2 * BN * OT_K * 2, STAGE = A + B;
-    static constexpr int N = BN == 64 ? 2 : BN == 128 ? 3 : 2;   // 64: two blocks to an SM
-    static constexpr int HIGH = BN == 64 ? 3 : 1, COLS = BN == 256 ? 512 : 256;  // accumulators of h h', columns of TMEM
-    static_assert((HIGH + 1) * BN <= COLS, "accumulators fit");
+    static constexpr int N = BN == 64 ? 2 : 3;                   // 64: two blocks to an SM
+    static constexpr int COLS = 2 * BN;                          // of TMEM: h h', and the others
 };
 
 __device__ __forceinline__ uint32_t orth_rank() {
@@ -208,7 +215,7 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
     using Ring = OrthRing<BN>;
     constexpr int LDP = BN + 4;  // partial row: 4 floats of padding keep 16-byte stores off each other's banks
     extern __shared__ __align__(1024) unsigned char dsmem[];
-    __shared__ __align__(8) uint64_t full[Ring::N], empty[Ring::N], acc_full;
+    __shared__ __align__(8) uint64_t full[Ring::N], empty[Ring::N], acc_full, acc_empty;
     __shared__ uint32_t tmem_slot;
     __shared__ int s_fail;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
     }
     const int m0 = mi * OT_M, n0 = t * BN;
     const int kb0 = (int)((long long)g.kt * rank / S), kb1 = (int)((long long)g.kt * (rank + 1) / S);
-    const int share = max(ORTH_RUN, (kb1 - kb0 + Ring::HIGH - 1) / Ring::HIGH), shares = (kb1 - kb0 + share - 1) / share;
+    const int runs = (kb1 - kb0 + ORTH_RUN - 1) / ORTH_RUN;
 
     if (warp == 2 && tc::elect_one()) {
         tc::prefetch_map(&tp);
@@ -239,6 +246,7 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
             tc::mbar_init(&empty[i], 1);
         }
         tc::mbar_init(&acc_full, 1);
+        tc::mbar_init(&acc_empty, 8);
         tc::fence_mbar_init();
     }
     if (warp == 1) {
@@ -253,6 +261,32 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
     // the next kernel's blocks may come: this block holds its tensor memory
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the last kernel's results are in memory
+
+    // The finishing pass: W columns a position, two positions a thread and round, their
+    // addends a round ahead, the first one's before the products.  A cluster's exchange waits
+    // for distributed shared memory (a tile of 128 x 64, four CTAs: 2.2 us), of which a round
+    // asks for three peers at once; alone, 16-byte stores count.
+    constexpr int W = SPLIT ? 4 : 8, U = 2;
+    using Wide = typename std::conditional<W == 8, uint4, uint2>::type;
+    const int slice = BN / S, shift = __ffs(slice / W) - 1;  // columns, and the logarithm of a row's positions
+    const long long c_plane = g.m * g.ldc, d_plane = g.m * g.ldd;
+    auto place = [&](int i, int& r, int& c) {
+        r = i >> shift;
+        c = (i - (r << shift)) * W;
+        return r < OT_M && m0 + r < g.m && n0 + rank * slice + c < g.n;
+    };
+    Wide next_h[U], next_l[U];
+    auto addends = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            int r, c;
+            if (!g.c || !place(i0 + u * OT_NT, r, c)) continue;
+            const __half* p = g.c + 2 * b * c_plane + (m0 + r) * g.ldc + n0 + rank * slice + c;  // rows hold a multiple of 8 elements
+            next_h[u] = *reinterpret_cast<const Wide*>(p);
+            next_l[u] = *reinterpret_cast<const Wide*>(p + c_plane);
+        }
+    };
+    addends(tid);
 
     if (warp == 0) {
         if (tc::elect_one()) {  // ---- TMA producer
@@ -293,44 +327,59 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
             if (!ok) break;
             tc::fence_after_sync();
             const uint64_t da = da0 + st * (Ring::STAGE / 16), db = db0 + st * (Ring::STAGE / 16);
-            const uint32_t high = taddr + (uint32_t)((1 + i / share) * BN);
+            const bool run = i % ORTH_RUN == 0;
             if (tc::elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < OT_K / 16; ++kk) {
-                    const uint64_t a = da + ka * kk, q = db + kq * kk;
-                    tc::umma_bf16(high, a, q, g.idesc, (i % share | kk) != 0);
-                    tc::umma_bf16(taddr, a, q + pb, g.idesc, (i | kk) != 0);
-                    tc::umma_bf16(taddr, a + pa, q, g.idesc, 1);
+                    tc::umma_bf16(taddr, da + ka * kk, db + kq * kk + pb, g.idesc, (i | kk) != 0);
+                    tc::umma_bf16(taddr, da + ka * kk + pa, db + kq * kk, g.idesc, 1);
                 }
+            }
+            __syncwarp();
+            if (run && i > 0) {  // the last run's sums have been taken
+                ok = __all_sync(0xffffffffu, tc::mbar_wait_or_fail(&acc_empty, (i / ORTH_RUN - 1) & 1, fail));
+                if (!ok) break;
+                tc::fence_after_sync();
+            }
+            if (tc::elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < OT_K / 16; ++kk)
+                    tc::umma_bf16(taddr + BN, da + ka * kk, db + kq * kk, g.idesc, !run || kk != 0);
                 tc::umma_commit(&empty[st]);
-                if (kb + 1 == kb1) tc::umma_commit(&acc_full);
+                if (kb + 1 == kb1 || (i + 1) % ORTH_RUN == 0) tc::umma_commit(&acc_full);
             }
             __syncwarp();
         }
     } else {  // ---- epilogue warps: TMEM -> partial tile in shared memory
-        const int q4 = warp & 3, half = (warp - 2) >> 2;
-        const bool ok = tc::mbar_wait_warp(&acc_full, 0, fail);
-        tc::fence_after_sync();
+        constexpr int COLUMNS = BN / 2, G = COLUMNS / 32;  // of a warp
+        const int q4 = warp & 3, c0 = ((warp - 2) >> 2) * COLUMNS;
         float* row = part + (q4 * 32 + lane) * LDP;
-        const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16);
-#pragma unroll 1
-        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-            float v[32], x[32];
-            tc::tmem_ld_32x32_nowait(src + (uint32_t)(BN + c), v);
-            tc::tmem_ld_32x32_nowait(src + (uint32_t)c, x);
-            tc::tmem_ld_wait(v);
-            tc::tmem_ld_wait(x);
+        const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)c0;
+        bool ok = true;
+        float sum[G][32];
+        for (int r = 0; r < runs; ++r) {
+            ok = tc::mbar_wait_warp(&acc_full, r & 1, fail) && ok;
+            tc::fence_after_sync();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = fmaf(x[j], 1.0f / (1 << LOW_SHIFT), v[j]);
-            for (int a = 1; a < shares; ++a) {
-                tc::tmem_ld_32x32(src + (uint32_t)((1 + a) * BN + c), x);
+            for (int c = 0; c < G; ++c) {
+                float v[32];
+                tc::tmem_ld_32x32(src + (uint32_t)(BN + 32 * c), v);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] += x[j];
+                for (int j = 0; j < 32; ++j) sum[c][j] = r ? sum[c][j] + v[j] : v[j];
             }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (tc::elect_one()) tc::mbar_arrive(&acc_empty);
+        }
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)  // a wait that ran out leaves NaN, not a plausible number
-                *reinterpret_cast<float4*>(row + c + j) =
-                    ok ? make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]) : make_float4(NAN, NAN, NAN, NAN);
+        for (int c = 0; c < G; ++c) {
+            float v[32];
+            tc::tmem_ld_32x32(src + (uint32_t)(32 * c), v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = ok ? fmaf(v[j], 1.0f / (1 << LOW_SHIFT), sum[c][j]) : NAN;  // a wait that ran out
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+                *reinterpret_cast<float4*>(row + c0 + 32 * c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         }
         tc::fence_before_sync();
     }
@@ -341,40 +390,26 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
         tc::tmem_dealloc(taddr, Ring::COLS);
     }
 
-    // W columns a position, two positions a thread and round.  A cluster's exchange waits for
-    // distributed shared memory (a tile of 128 x 64, four CTAs: 2.2 us), of which a round asks
-    // for three peers at once; alone, 16-byte stores count (128 x 256: 4.4 us, with 8 bytes 6.2).
-    constexpr int W = SPLIT ? 4 : 8, U = 2;
-    static_assert((OT_M * LDP + (BN == 256 ? 0 : OT_M * BN)) * 4 <= Ring::N * Ring::STAGE, "the tile, and for SYM its transposed copy, fit the ring");
+    static_assert((OT_M * LDP + OT_M * BN) * 4 <= Ring::N * Ring::STAGE, "the tile, and for SYM its transposed copy, fit the ring");
     uint32_t* turned = reinterpret_cast<uint32_t*>(part + OT_M * LDP);  // SYM: the slice transposed, h and l in one word,
     auto turn = [](int c, int r) { return c * OT_M + ((r + c / W) & (OT_M - 1)); };  // turned on by W columns
-    const int slice = BN / S, shift = __ffs(slice / W) - 1;  // columns, and the logarithm of a row's positions
     const uint32_t pbase = tc::smem_u32(part);
-    const long long c_plane = g.m * g.ldc, d_plane = g.m * g.ldd;
     for (int i0 = tid; i0 < OT_M << shift; i0 += U * OT_NT) {
         int r[U], cc[U];
         bool in[U];
         alignas(16) float v[U][W];
-        alignas(16) __half ch[U][W], cl[U][W];
+        Wide ch[U], cl[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * OT_NT;
-            r[u] = i >> shift;
-            cc[u] = (i - (r[u] << shift)) * W;
-            in[u] = r[u] < OT_M && m0 + r[u] < g.m && n0 + rank * slice + cc[u] < g.n;
+            ch[u] = next_h[u];
+            cl[u] = next_l[u];
+            in[u] = place(i0 + u * OT_NT, r[u], cc[u]);
             if (!in[u]) continue;
-            if (g.c) {  // rows hold a multiple of 8 elements
-                const __half* p = g.c + 2 * b * c_plane + (m0 + r[u]) * g.ldc + n0 + rank * slice + cc[u];
-#pragma unroll
-                for (int j = 0; j < W; j += 4) {
-                    *reinterpret_cast<uint2*>(&ch[u][j]) = *reinterpret_cast<const uint2*>(p + j);
-                    *reinterpret_cast<uint2*>(&cl[u][j]) = *reinterpret_cast<const uint2*>(p + c_plane + j);
-                }
-            }
             const float* own = part + r[u] * LDP + rank * slice + cc[u];
 #pragma unroll
             for (int j = 0; j < W; j += 4) *reinterpret_cast<float4*>(&v[u][j]) = *reinterpret_cast<const float4*>(own + j);
         }
+        addends(i0 + U * OT_NT);
         if constexpr (SPLIT) {
             for (int s0 = 1; s0 < S; s0 += 3) {
                 float4 x[U][3];
@@ -404,18 +439,14 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
             for (int j = 0; j < W; ++j) v[u][j] *= g.beta;
             if (g.c) {
 #pragma unroll
-                for (int j = 0; j < W; ++j) v[u][j] = fmaf(g.alpha, value_of(ch[u][j], cl[u][j]), v[u][j]);
-            }
-            if (g.sym && (unsigned)(row - col) < W) {
-#pragma unroll
-                for (int j = 0; j < W; ++j) v[u][j] += col + j == row ? g.diag : 0.0f;
+                for (int j = 0; j < W; ++j)
+                    v[u][j] = fmaf(g.alpha, value_of(reinterpret_cast<const __half*>(&ch[u])[j], reinterpret_cast<const __half*>(&cl[u])[j]), v[u][j]);
             }
             if (g.d) {
                 alignas(16) __half h[W], l[W];
 #pragma unroll
                 for (int j = 0; j < W; j += 2)
                     planes_of(v[u][j], v[u][j + 1], *reinterpret_cast<__half2*>(h + j), *reinterpret_cast<__half2*>(l + j));
-                using Wide = typename std::conditional<W == 8, uint4, uint2>::type;
                 __half* p = g.d + 2 * b * d_plane + row * g.ldd + col;
                 if (!g.sym || col + W - 1 <= row) {  // elements past the last column lie in the row's padding
                     *reinterpret_cast<Wide*>(p) = *reinterpret_cast<const Wide*>(h);
@@ -428,7 +459,7 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
                             p[d_plane + j] = l[j];
                         }
                 }
-                if (BN < 256 && g.sym) {
+                if (g.sym) {
 #pragma unroll
                     for (int j = 0; j < W; ++j)
                         turned[turn(cc[u] + j, r[u])] = (uint32_t)__half_as_ushort(h[j]) | (uint32_t)__half_as_ushort(l[j]) << 16;
@@ -453,7 +484,7 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
         }
     }
     if (SPLIT) asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // this block has read its peers' partial tiles
-    if (BN < 256 && g.sym) {  // a lane takes two rows, which become neighbouring columns
+    if (g.sym) {  // a lane takes two rows, which become neighbouring columns
         __syncthreads();
         for (int i = tid; i < slice * (OT_M / 2); i += OT_NT) {
             const int c = i / (OT_M / 2), r = i % (OT_M / 2) * 2, row = m0 + r, col = n0 + rank * slice + c;
@@ -485,13 +516,12 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
 constexpr int OS_NT = 512, OS_SIDE = 128, OS_FAR = 256, OS_CHUNK = 128 * 128;
 constexpr int OS_X = 4 * OS_CHUNK, OS_Y = 2 * OS_CHUNK;  // bytes of a plane
 constexpr int OS_SMEM = 2 * OS_X + 2 * OS_Y + 1024;
-static_assert(OS_SIDE * (OS_FAR | 1) * 4 <= 2 * OS_X + 2 * OS_Y, "the result's rows fit");
 
 struct OrthSmall {
     const void* g;
     void* out;
     long long row_stride, batch_stride;
-    int rows, cols, steps, square, wide;  // wide: G's rows start on 16 bytes
+    int rows, cols, steps, wide;  // wide: G's rows start on 16 bytes
     float a, b, c, eps;
 };
 
@@ -585,8 +615,9 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
     const int q4 = warp & 3, part = warp >> 2;                         // lanes of TMEM, columns
     uint32_t phase = 0;
     bool ok = true;
-    // h h' of columns [0, n) and, 256 on, h l' + l h', over `chunks` of 64 k
-    auto multiply = [&](const unsigned char* p, uint32_t p_low, const unsigned char* q, uint32_t q_low, bool q_mn, int n, int chunks) {
+    // h h' of columns [0, n) and, 256 on, h l' + l h', over `chunks` of 64 k; with `two`, the
+    // second half of the chunks into columns from 128 on
+    auto multiply = [&](const unsigned char* p, uint32_t p_low, const unsigned char* q, uint32_t q_low, bool q_mn, int n, int chunks, bool two) {
         tc::fence_proxy_async();  // operands written by ordinary stores
         tc::fence_before_sync();
         __syncthreads();
@@ -600,9 +631,9 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
                     for (int kk = 0; kk < 4; ++kk) {
                         const uint64_t a = dp + c * (OS_CHUNK / 16) + 2 * kk;
                         const uint64_t b = dq + (q_mn ? c * (64 * 128 / 16) + 128 * kk : c * (OS_CHUNK / 16) + 2 * kk);
-                        const uint32_t more = (c | kk) != 0;
-                        tc::umma_bf16(taddr, a, b, id, more);
-                        tc::umma_bf16(taddr + 256, a, b + q_low / 16, id, more);
+                        const int later = two && 2 * c >= chunks, first = later ? (chunks + 1) / 2 : 0;
+                        tc::umma_bf16(taddr + 128 * later, a, b, id, c > first || kk != 0);
+                        tc::umma_bf16(taddr + 256, a, b + q_low / 16, id, (c | kk) != 0);
                         tc::umma_bf16(taddr + 256, a + p_low / 16, b, id, 1);
                     }
                 tc::umma_commit(&done);
@@ -614,7 +645,7 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
         tc::fence_after_sync();
     };
     // 32 columns of a product from column c on, this lane's row
-    auto take = [&](float (&v)[32], int c) {
+    auto take = [&](float (&v)[32], int c, bool two) {
         float x[32];
         const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)c;
         tc::tmem_ld_32x32_nowait(src, v);
@@ -623,6 +654,23 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
         tc::tmem_ld_wait(x);
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = ok ? fmaf(x[j], 1.0f / (1 << LOW_SHIFT), v[j]) : NAN;
+        if (two) {
+            tc::tmem_ld_32x32(src + 128, x);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += x[j];
+        }
+    };
+    // v = scale v + w times the matrix's own columns from c on
+    auto add = [&](float (&v)[32], float scale, float w, const unsigned char* from, uint32_t low, int row, int c) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+            alignas(16) __half h[8], l[8];
+            const uint32_t at = os_at(row, c + j);
+            *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(from + at);
+            *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(from + low + at);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[j + k] = fmaf(v[j + k], scale, w * value_of(h[k], l[k]));
+        }
     };
     auto put = [&](unsigned char* to, uint32_t low, const float (&v)[32], int row, int c) {
 #pragma unroll
@@ -639,56 +687,47 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
     const int row = q4 * 32 + lane;
     T* out = static_cast<T*>(g.out) + (long long)blockIdx.x * g.rows * g.cols;
     // the result: tall, neighbouring lanes on neighbouring columns; else through shared memory,
-    // where X's planes are done with, rows of an odd number of words
-    float* staged = reinterpret_cast<float*>(xs);
-    const int lds = far | 1;
+    // eight elements where their own planes were: the first four in h's place, then l's
     auto store = [&](const float (&v)[32], int c) {
-        if (row >= side) return;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (c + j < far) {
-                if (tall)
-                    out[(c + j) * side + row] = from_f32<T>(v[j]);
-                else
-                    staged[row * lds + c + j] = v[j];
+        for (int j = 0; j < 32; j += 8) {
+            if (tall) {
+#pragma unroll
+                for (int k = j; k < j + 8; ++k)
+                    if (row < side && c + k < far) out[(c + k) * side + row] = from_f32<T>(v[k]);
+            } else {
+                const uint32_t at = os_at(row, c + j);
+                *reinterpret_cast<float4*>(xs + at) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                *reinterpret_cast<float4*>(xs + OS_X + at) = make_float4(v[j + 4], v[j + 5], v[j + 6], v[j + 7]);
             }
+        }
     };
 #pragma unroll 1
     for (int step = 0; step < g.steps; ++step) {
         float v[32];
-        multiply(xs, OS_X, xs, OS_X, false, sc * 64, fc);
-        if (part * 32 < sc * 64) {
-            const float scale = g.c == 0.0f ? g.b : 1.0f, diag = g.c == 0.0f ? g.a : g.square ? g.b / (2.0f * g.c) : 0.0f;
-            take(v, part * 32);
+        const int c0 = part * 32;
+        multiply(xs, OS_X, xs, OS_X, false, sc * 64, fc, fc > 1);
+        if (c0 < sc * 64) {
+            take(v, c0, fc > 1);
+            if (g.c == 0.0f) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], scale, part * 32 + j == row ? diag : 0.0f);
-            put(ys, OS_Y, v, row, part * 32);
+                for (int j = 0; j < 32; ++j) v[j] *= g.b;
+            }
+            put(ys, OS_Y, v, row, c0);
         }
         if (g.c != 0.0f) {
-            multiply(ys, OS_Y, ys, OS_Y, false, sc * 64, sc);
-            if (part * 32 < sc * 64) {
-                const float diag = g.square ? (float)((double)g.a - (double)g.b * g.b / (4.0 * g.c)) : g.a;
-                take(v, part * 32);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], g.c, part * 32 + j == row ? diag : 0.0f);
-                if (!g.square) {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        alignas(16) __half h[8], l[8];
-                        const uint32_t at = os_at(row, part * 32 + j);
-                        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(ys + at);
-                        *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(ys + OS_Y + at);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) v[j + k] = fmaf(g.b, value_of(h[k], l[k]), v[j + k]);
-                    }
-                }
-                put(ys, OS_Y, v, row, part * 32);
+            multiply(ys, OS_Y, ys, OS_Y, false, sc * 64, sc, sc > 1);
+            if (c0 < sc * 64) {
+                take(v, c0, sc > 1);
+                add(v, g.c, g.b, ys, OS_Y, row, c0);
+                put(ys, OS_Y, v, row, c0);
             }
         }
-        multiply(ys, OS_Y, xs, OS_X, true, fc * 64, sc);
+        multiply(ys, OS_Y, xs, OS_X, true, fc * 64, sc, false);
 #pragma unroll 1
-        for (int c = part * 32; c < fc * 64; c += 128) {
-            take(v, c);
+        for (int c = c0; c < fc * 64; c += 128) {
+            take(v, c, false);
+            add(v, 1.0f, g.a, xs, OS_X, row, c);
             if (step + 1 < g.steps)
                 put(xs, OS_X, v, row, c);
             else
@@ -701,7 +740,8 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
     if (warp == 1) tc::tmem_dealloc(taddr, 512);
     if (!tall)
         for (int r = warp; r < side; r += OS_NT / 32)
-            for (int c = lane; c < far; c += 32) out[r * far + c] = from_f32<T>(staged[r * lds + c]);
+            for (int c = lane; c < far; c += 32)
+                out[r * far + c] = from_f32<T>(*reinterpret_cast<const float*>(xs + (c & 4 ? OS_X : 0) + os_at(r, c & ~7) + (c & 3) * 4));
 }
 
 // ---- host side -----------------------------------------------------------------------
@@ -734,21 +774,24 @@ static long long orth_tiles(long long m, long long n, int bn, bool sym) {
     return t;
 }
 
-// Symmetric products take tiles of up to 128 columns (their transposed copy fits).
-// The tile width and split that finish first by this estimate, in microseconds.
+// The tile width and split that finish first by this estimate, in microseconds: a K block
+// takes 0.75 in tiles of 64 columns, of which two blocks share an SM, and 0.7 in tiles of
+// 128, what follows the products 3 and 3.5, and an exchange over the cluster 1, 2 or 4 more.
+// Measured for the sizes 512 x 256 to 2048 x 2048, each product with each choice: within 1 us
+// of the best one.  (Tiles of 256 columns, whose accumulators fill TMEM, took 95 us where
+// these take 77: 2048 x 1024 from the right, four matrices.)
 static OrthPlan orth_plan(long long m, long long n, long long k, int batch, bool sym) {
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount)), kb = (int)((k + OT_K - 1) / OT_K);
     OrthPlan best{128, 1};
     double least = 1e300;
-    for (int bn : {256, 128, 64}) {
-        if (sym && bn == 256) continue;
+    for (int bn : {128, 64}) {
         const long long tiles = orth_tiles(m, n, bn, sym) * batch;
         for (int sp : {1, 2, 4, 8}) {
             if (sp > kb) break;
             int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
             if (bn == 64) slots *= 2;
-            const double main = (kb + sp - 1) / sp * (bn == 256 ? 0.85 : bn == 128 ? 0.6 : 0.45);
-            const double cost = (double)((tiles + slots - 1) / slots) * (main + 2.0 + 0.02 * bn / sp) + (sp == 8 ? 0.7 : 0.0);
+            const double each = (kb + sp - 1) / sp * (bn == 128 ? 0.7 : 0.75) + (bn == 128 ? 3.5 : 3.0) + (sp == 8 ? 4 : sp == 4 ? 2 : sp - 1);
+            const double cost = (double)((tiles + slots - 1) / slots) * each;
             if (cost < least) {
                 least = cost;
                 best = OrthPlan{bn, sp};
@@ -806,9 +849,7 @@ static int product(const OrthOperand& p, const OrthOperand& q, OrthArgs g, long 
     const OrthPlan plan = orth_plan(g.m, g.n, k, batch, g.sym);
     g.split = plan.split;
     g.kt = (int)((k + OT_K - 1) / OT_K);
-    return plan.bn == 256   ? launch_product<T, 256>(p, q, g, batch, s)
-           : plan.bn == 128 ? launch_product<T, 128>(p, q, g, batch, s)
-                            : launch_product<T, 64>(p, q, g, batch, s);
+    return plan.bn == 128 ? launch_product<T, 128>(p, q, g, batch, s) : launch_product<T, 64>(p, q, g, batch, s);
 }
 
 struct OrthWs {
@@ -858,16 +899,12 @@ static int orthogonalize(const fg_orthogonalize_params* p, const void* g, void* 
     const int rows = p->rows, cols = p->cols, batch = p->batch, side = std::min(rows, cols), far = std::max(rows, cols);
     const long long ldx = orth_ld(cols), lda = orth_ld(side);
     const long long row_stride = p->row_stride ? p->row_stride : cols, batch_stride = p->batch_stride ? p->batch_stride : rows * row_stride;
-    // Y = a I + b A + c A^2 = c M^2 + (a - b^2 / 4c) I, M = A + b / 2c I, so that no product of a
-    // X + (b A + c A^2) X = Y X reads an addend.  Where b / 2c is large, M^2 would lose what A^2
-    // is, and A is added as it is; without c, Y comes from the first product.
     const int es = sizeof(T);
     const bool wide = aligned(g, 16) && row_stride * es % 16 == 0 && (batch == 1 || batch_stride * es % 16 == 0);
-    const bool square = p->c != 0.0f && fabsf(p->b) <= 8.0f * fabsf(p->c);
     if (orth_small(p)) {
         FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(&orth_small_kernel<T>), OS_SMEM));
         orth_small_kernel<T><<<batch, OS_NT, OS_SMEM, s>>>(
-            OrthSmall{g, out, row_stride, batch_stride, rows, cols, p->steps, square, wide, p->a, p->b, p->c, p->eps});
+            OrthSmall{g, out, row_stride, batch_stride, rows, cols, p->steps, wide, p->a, p->b, p->c, p->eps});
         return check_launch("orth_small_kernel");
     }
     OrthIn in{};
@@ -894,32 +931,30 @@ static int orthogonalize(const fg_orthogonalize_params* p, const void* g, void* 
     for (int k = 0; k < p->steps; ++k) {
         const __half* x = w.x[k & 1];
         const bool last = k + 1 == p->steps;
-        const float ca = p->a, cb = p->b, cc = p->c;
-        OrthArgs a{};  // M, A or Y of X X^T
+        OrthArgs a{};  // A = X X^T, or without c already B = b A
         a.m = a.n = side;
         a.sym = 1;
-        a.beta = cc == 0.0f ? cb : 1.0f;
-        a.diag = cc == 0.0f ? ca : square ? cb / (2.0f * cc) : 0.0f;
+        a.beta = p->c == 0.0f ? p->b : 1.0f;
         a.d = w.a;
         a.ldd = lda;
         const OrthOperand xs{x, rows, cols, ldx, tall};
         if ((rc = product<T>(xs, xs, a, far, batch, s))) return rc;
-        const OrthOperand as{w.a, side, side, lda, false}, bs{cc == 0.0f ? w.a : w.b, side, side, lda, false};
-        if (cc != 0.0f) {
-            a.beta = cc;
-            a.diag = square ? (float)((double)ca - (double)cb * cb / (4.0 * cc)) : ca;
-            if (!square) {
-                a.alpha = cb;
-                a.c = w.a;
-                a.ldc = lda;
-            }
+        const OrthOperand as{w.a, side, side, lda, false}, bs{p->c == 0.0f ? w.a : w.b, side, side, lda, false};
+        if (p->c != 0.0f) {  // B = b A + c A A
+            a.alpha = p->b;
+            a.beta = p->c;
+            a.c = w.a;
+            a.ldc = lda;
             a.d = w.b;
             if ((rc = product<T>(as, as, a, side, batch, s))) return rc;
         }
-        OrthArgs d{};  // X = Y X, or X Y
+        OrthArgs d{};  // X = a X + B X, or a X + X B
         d.m = rows;
         d.n = cols;
+        d.alpha = p->a;
         d.beta = 1.0f;
+        d.c = x;
+        d.ldc = ldx;
         d.d = last ? nullptr : w.x[(k + 1) & 1];
         d.ldd = ldx;
         d.out = out;

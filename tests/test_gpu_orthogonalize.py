@@ -3,8 +3,9 @@
 Tolerances are on the Frobenius norm of the error and follow the iteration.  A
 product of P and Q is off by ROUND for each of its terms, independently (two
 operands' roundings to 22 bits and the product of their low planes, which is left
-out), so by ROUND * sqrt(sum of the terms' squares), and by what 32-bit sums that
-are cut rather than rounded lose, (k / 16 + 16) * 2^-24 of the result; a matrix
+out), so by ROUND * sqrt(sum of the terms' squares), and by what 32-bit sums lose: cut every
+16 k in runs of at most 256, 16 * 2^-24 of the result, and rounded when runs are added,
+another 8 * 2^-24; a matrix
 kept between products adds 2^-22 of its norm.  An error of X grows in a step by
 the largest slope of a s + b s^3 + c s^5 over the singular values, chords through
 the origin among them.  Three times the sum of these is allowed, the terms being
@@ -46,24 +47,16 @@ def _iterate(g, steps=5, coef=COEF, eps=1e-7):
 
     def product(p, q):
         rms = float((p.square() @ q.square()).sum().sqrt())
-        return ROUND * rms + (p.shape[1] / 16 + 16) * 2.0 ** -24 * float((p @ q).norm())
+        return ROUND * rms + 24 * 2.0 ** -24 * float((p @ q).norm())
 
-    eye = torch.eye(x.shape[0], device=x.device, dtype=torch.float64)
-    square = c != 0 and abs(b) <= 8 * abs(c)
     for _ in range(steps):
         gram = x @ x.t()
+        poly = b * gram + c * gram @ gram
         top = float(torch.linalg.matrix_norm(x, ord=2))
-        y = a * eye + b * gram + c * gram @ gram  # the step is y x
-        if square:  # y = c m^2 + (a - b^2 / 4c), m = gram + b / 2c
-            m = gram + b / (2 * c) * eye
-            dm = product(x, x.t()) + KEPT * float(m.norm())
-            dy = abs(c) * (2 * float(torch.linalg.matrix_norm(m, ord=2)) * dm + product(m, m))
-        else:
-            dg = product(x, x.t()) + KEPT * float(gram.norm())
-            dy = abs(b) * dg + abs(c) * (2 * top ** 2 * dg + product(gram, gram))
-        dy += KEPT * float(y.norm())
-        new = y @ x
-        dx = top * dy + product(y, x) + 2 * KEPT * float(new.norm())
+        dg = product(x, x.t()) + KEPT * float(gram.norm())
+        dp = abs(b) * dg + abs(c) * (2 * top ** 2 * dg + product(gram, gram)) + KEPT * float(poly.norm())
+        new = a * x + poly @ x
+        dx = top * dp + product(poly, x) + 2 * KEPT * float(new.norm())
         s = torch.linspace(0, top, 200, dtype=torch.float64)
         slope = float((a + 3 * b * s ** 2 + 5 * c * s ** 4).abs().max())
         err = max(slope, float((a + b * s ** 2 + c * s ** 4).abs().max())) * err + dx

@@ -128,7 +128,7 @@ def _linear_ws(query: str, n: int, i: int, o: int, dtype: int, act: int, ldx: in
 
 
 @functools.lru_cache(maxsize=1024)
-def _orthogonalize_ws(batch: int, m: int, n: int, dtype: int, steps: int) -> int:
+def _orthogonalize_ws(batch: int, m: int, n: int, dtype: int, steps: int, device: int) -> int:
     return _lib.size_query("fg_orthogonalize_workspace_size",
                            C.byref(_lib.OrthogonalizeParams(batch, m, n, dtype, steps, 0, 0, 0, 0, 0, 0)))
 
@@ -403,7 +403,7 @@ def orthogonalize(g: torch.Tensor, steps: int = 5, coefficients: tuple[float, fl
     out = torch.empty_strided(g.shape, (n, 1) if g.dim() == 2 else (m * n, n, 1), dtype=g.dtype, device=g.device)
     a, b, c = coefficients
     p = _lib.OrthogonalizeParams(batch, m, n, DTYPES[g.dtype], steps, a, b, c, eps, ld, g.stride(0) if batch > 1 else 0)
-    nws = _orthogonalize_ws(batch, m, n, DTYPES[g.dtype], steps)
+    nws = _orthogonalize_ws(batch, m, n, DTYPES[g.dtype], steps, g.device.index)
     ws = torch.empty(nws, dtype=torch.uint8, device=g.device) if nws else None
     _lib.check(_lib.lib().fg_orthogonalize(C.byref(p), g.data_ptr(), out.data_ptr(), _ptr(ws), nws, _stream(g)),
                "fg_orthogonalize")

@@ -28,7 +28,7 @@ namespace fg {
 
 constexpr int OT_M = 128, OT_K = 64, OT_NT = 64 + 256;
 constexpr int LOW_SHIFT = 11;  // h + 2^-11 l
-constexpr int ORTH_RUN = 4;    // K blocks (256 k) that an accumulator sums
+constexpr int ORTH_RUN = 2;    // K blocks (128 k) that an accumulator sums
 
 __device__ __forceinline__ void planes_of(float v, __half& h, __half& l) {
     h = __float2half_rn(v);
@@ -506,14 +506,20 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
     if (SPLIT) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // a peer may still read this CTA's partial tile
 }
 
-// ---- small matrices: the whole iteration in one block ----------------------------------
+// ---- up to 128 on the smaller side: the whole iteration in one launch --------------------
 //
-// Up to 128 x 256, whichever way they lie, X and Y (or M) stay in shared memory as the
+// A block holds 256 columns of X (rows, where they lie that way) in shared memory as the
 // tensor cores read them: chunks of 64 columns, 128 rows of 128 bytes, 128-byte swizzle, a
 // row of X an index of the smaller side.  The same chunk is a K-major operand of X X^T and
-// an MN-major one of Y X.  A product's epilogue writes the next one's operand in place.
-// Bound by the chain of three products and three epilogues a step.
-constexpr int OS_NT = 512, OS_SIDE = 128, OS_FAR = 256, OS_CHUNK = 128 * 128;
+// an MN-major one of B X.  A product's epilogue writes the next one's operand in place.
+//
+// Up to 256 on the longer side one block does; up to 2,048 a cluster of two, four or eight,
+// whose parts of A meet in the workspace (L2 carries them faster than distributed shared
+// memory): each block adds a slice of them and writes its planes, of which all take a
+// copy.  B is worked out by every block for itself, B X is its own.  Bound by the chain of
+// three products and three epilogues a step, 9.4 us for 128 x 256 in one block (products
+// 2.0, 1.2 and 1.9).
+constexpr int OS_NT = 512, OS_SIDE = 128, OS_FAR = 256, OS_CHUNK = 128 * 128, OS_MOST = 8;  // OS_FAR: of a block; blocks
 constexpr int OS_X = 4 * OS_CHUNK, OS_Y = 2 * OS_CHUNK;  // bytes of a plane
 constexpr int OS_SMEM = 2 * OS_X + 2 * OS_Y + 1024;
 
@@ -521,9 +527,15 @@ struct OrthSmall {
     const void* g;
     void* out;
     long long row_stride, batch_stride;
-    int rows, cols, steps, wide;  // wide: G's rows start on 16 bytes
+    int rows, cols, steps, wide, split;  // wide: G's rows start on 16 bytes; split: blocks a matrix
     float a, b, c, eps;
+    double* sums;         // split > 1: [batch][split]
+    float4* part;         // [batch][split][columns of A / 4][128]
+    unsigned char* image; // [batch][2 planes of Y]
 };
+
+static_assert(OS_SIDE * OS_SIDE / 4 / OS_NT == OS_MOST, "pieces of A that a thread adds");
+__device__ __forceinline__ float4 os_add(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 
 __device__ __forceinline__ uint32_t os_at(int row, int col) {  // byte of 8 elements from col on
     return (uint32_t)((col >> 6) * OS_CHUNK + row * 128 + (((col & 63) * 2) ^ ((row & 7) << 4)));
@@ -532,7 +544,7 @@ __device__ __forceinline__ uint32_t os_at(int row, int col) {  // byte of 8 elem
 template <class T>
 __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g) {
     extern __shared__ __align__(1024) unsigned char dsmem[];
-    __shared__ __align__(8) uint64_t done;
+    __shared__ __align__(8) uint64_t done, copied;
     __shared__ uint32_t tmem_slot;
     __shared__ int s_fail;
     __shared__ double s_sum[OS_NT / 32];
@@ -540,13 +552,16 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
     unsigned char* xs = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
     unsigned char* ys = xs + 2 * OS_X;
     const bool tall = g.rows > g.cols;
-    const int side = tall ? g.cols : g.rows, far = tall ? g.rows : g.cols;
-    const int sc = (side + 63) / 64, fc = (far + 63) / 64;  // chunks
-    const T* in = static_cast<const T*>(g.g) + blockIdx.x * g.batch_stride;
+    const int S = g.split, rank = S > 1 ? (int)orth_rank() : 0, matrix = (int)(blockIdx.x / (unsigned)S);
+    const int side = tall ? g.cols : g.rows, whole = tall ? g.rows : g.cols, chunks_of_all = (whole + 63) / 64;
+    const int chunk0 = chunks_of_all * rank / S, f0 = chunk0 * 64;  // this block's part of the longer side
+    const int sc = (side + 63) / 64, fc = chunks_of_all * (rank + 1) / S - chunk0, far = min(whole - f0, fc * 64);
+    const T* in = static_cast<const T*>(g.g) + matrix * g.batch_stride + (tall ? f0 * g.row_stride : (long long)f0);
 
     if (tid == 0) {
         s_fail = 0;
         tc::mbar_init(&done, 1);
+        tc::mbar_init(&copied, 1);
         tc::fence_mbar_init();
     }
     if (warp == 1) {
@@ -596,6 +611,12 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
     sum = 0.0;
 #pragma unroll
     for (int w = 0; w < OS_NT / 32; ++w) sum += s_sum[w];
+    if (S > 1) {
+        if (tid == 0) g.sums[matrix * S + rank] = sum;
+        orth_cluster_sync();
+        sum = 0.0;
+        for (int r = 0; r < S; ++r) sum += __ldcg(g.sums + matrix * S + r);
+    }
     const double inv = 1.0 / (sqrt(sum) + (double)g.eps);
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
@@ -685,7 +706,7 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
         }
     };
     const int row = q4 * 32 + lane;
-    T* out = static_cast<T*>(g.out) + (long long)blockIdx.x * g.rows * g.cols;
+    T* out = static_cast<T*>(g.out) + (long long)matrix * g.rows * g.cols + (tall ? (long long)f0 * side : (long long)f0);
     // the result: tall, neighbouring lanes on neighbouring columns; else through shared memory,
     // eight elements where their own planes were: the first four in h's place, then l's
     auto store = [&](const float (&v)[32], int c) {
@@ -694,7 +715,7 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
             if (tall) {
 #pragma unroll
                 for (int k = j; k < j + 8; ++k)
-                    if (row < side && c + k < far) out[(c + k) * side + row] = from_f32<T>(v[k]);
+                    if (row < side && c + k < far) out[(long long)(c + k) * side + row] = from_f32<T>(v[k]);
             } else {
                 const uint32_t at = os_at(row, c + j);
                 *reinterpret_cast<float4*>(xs + at) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
@@ -702,6 +723,8 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
             }
         }
     };
+    float4* parts = g.part + (size_t)matrix * S * sc * 16 * OS_SIDE;
+    unsigned char* image = g.image + (size_t)matrix * 2 * OS_Y;
 #pragma unroll 1
     for (int step = 0; step < g.steps; ++step) {
         float v[32];
@@ -713,7 +736,45 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] *= g.b;
             }
-            put(ys, OS_Y, v, row, c0);
+            if (S == 1) {
+                put(ys, OS_Y, v, row, c0);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    parts[(rank * sc * 16 + (c0 + j) / 4) * OS_SIDE + row] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            }
+        }
+        if (S > 1) {
+            orth_cluster_sync();
+            // eight pieces of four columns a thread at most, all asked for at once
+            const int pieces = sc * 16 * OS_SIDE, per = pieces / S, loads = (per + OS_NT - 1) / OS_NT * S;
+            float4 p[OS_MOST];
+#pragma unroll
+            for (int k = 0; k < OS_MOST; ++k)
+                if (k < loads && tid < per) p[k] = __ldcg(parts + (k & (S - 1)) * pieces + rank * per + k / S * OS_NT + tid);
+#pragma unroll
+            for (int k = 0; k < OS_MOST; ++k) {
+                if (k >= loads || tid >= per) break;
+                if ((k & (S - 1)) != 0) p[k] = os_add(p[k - 1], p[k]);  // the blocks' in their order
+                if (((k + 1) & (S - 1)) != 0) continue;
+                alignas(8) __half h[4], l[4];
+                planes_of(p[k].x, p[k].y, *reinterpret_cast<__half2*>(h), *reinterpret_cast<__half2*>(l));
+                planes_of(p[k].z, p[k].w, *reinterpret_cast<__half2*>(h + 2), *reinterpret_cast<__half2*>(l + 2));
+                const int i = rank * per + k / S * OS_NT + tid, col = i / OS_SIDE * 4;
+                unsigned char* at = image + os_at(i & (OS_SIDE - 1), col & ~7) + (col & 4) * 2;
+                *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(h);
+                *reinterpret_cast<uint2*>(at + OS_Y) = *reinterpret_cast<const uint2*>(l);
+            }
+            orth_cluster_sync();
+            if (tid == 0) {
+                asm volatile("fence.proxy.async.global;" ::: "memory");  // written by ordinary stores
+                tc::mbar_arrive_expect_tx(&copied, 2 * sc * OS_CHUNK);
+                for (int k = 0; k < 2 * sc; ++k) {
+                    const int at = (k & 1) * OS_Y + (k >> 1) * OS_CHUNK;
+                    tc::bulk_load(ys + at, image + at, OS_CHUNK, &copied);
+                }
+            }
+            ok = tc::mbar_wait_warp(&copied, step & 1, fail) && ok;
         }
         if (g.c != 0.0f) {
             multiply(ys, OS_Y, ys, OS_Y, false, sc * 64, sc, sc > 1);
@@ -741,7 +802,7 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
     if (!tall)
         for (int r = warp; r < side; r += OS_NT / 32)
             for (int c = lane; c < far; c += 32)
-                out[r * far + c] = from_f32<T>(*reinterpret_cast<const float*>(xs + (c & 4 ? OS_X : 0) + os_at(r, c & ~7) + (c & 3) * 4));
+                out[(long long)r * whole + c] = from_f32<T>(*reinterpret_cast<const float*>(xs + (c & 4 ? OS_X : 0) + os_at(r, c & ~7) + (c & 3) * 4));
 }
 
 // ---- host side -----------------------------------------------------------------------
@@ -855,19 +916,36 @@ static int product(const OrthOperand& p, const OrthOperand& q, OrthArgs g, long 
 struct OrthWs {
     __half *x[2], *a, *b;
     double* part;
+    float4* parts;
+    unsigned char* image;
 };
 
 static long long orth_ld(long long cols) { return (cols + 7) / 8 * 8; }
 
-static bool orth_small(const fg_orthogonalize_params* p) {
-    return p->steps > 0 && std::min(p->rows, p->cols) <= OS_SIDE && std::max(p->rows, p->cols) <= OS_FAR;
+// Blocks a matrix for the one launch above, or 0: it does not fit, or so many matrices take
+// more than two rounds of clusters (74, 32 and 14 of two, four and eight blocks run at once),
+// where the products one by one are as fast.
+static int orth_small(const fg_orthogonalize_params* p) {
+    const int far = std::max(p->rows, p->cols);
+    if (p->steps == 0 || std::min(p->rows, p->cols) > OS_SIDE || far > OS_FAR * OS_MOST) return 0;
+    int split = 1;
+    while (far > OS_FAR * split) split *= 2;
+    const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
+    const int slots = split == 2 ? sms / 2 : std::max(1, split == 4 ? sms * 32 / 148 : sms * 14 / 148);
+    return split == 1 || p->batch <= 2 * slots ? split : 0;
 }
 
 static size_t orth_carve(const fg_orthogonalize_params* p, void* ws, size_t bytes, OrthWs& w) {
     Carve c(ws, bytes);
     w = OrthWs{};
     const size_t side = std::min(p->rows, p->cols), batch = p->batch;
-    if (orth_small(p)) return 0;
+    if (const int split = orth_small(p)) {
+        if (split == 1) return 0;
+        w.part = c.take<double>(batch * split);
+        w.parts = c.take<float4>(batch * split * ((side + 63) / 64) * 16 * OS_SIDE);
+        w.image = c.take<unsigned char>(batch * 2 * OS_Y);
+        return c.used;
+    }
     w.part = c.take<double>(batch * ORTH_PARTS);
     if (p->steps > 0) {
         for (int k = 0; k < 2; ++k)
@@ -901,11 +979,23 @@ static int orthogonalize(const fg_orthogonalize_params* p, const void* g, void* 
     const long long row_stride = p->row_stride ? p->row_stride : cols, batch_stride = p->batch_stride ? p->batch_stride : rows * row_stride;
     const int es = sizeof(T);
     const bool wide = aligned(g, 16) && row_stride * es % 16 == 0 && (batch == 1 || batch_stride * es % 16 == 0);
-    if (orth_small(p)) {
+    if (const int split = orth_small(p)) {
         FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(&orth_small_kernel<T>), OS_SMEM));
-        orth_small_kernel<T><<<batch, OS_NT, OS_SMEM, s>>>(
-            OrthSmall{g, out, row_stride, batch_stride, rows, cols, p->steps, wide, p->a, p->b, p->c, p->eps});
-        return check_launch("orth_small_kernel");
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)batch * split);
+        cfg.blockDim = dim3(OS_NT);
+        cfg.dynamicSmemBytes = OS_SMEM;
+        cfg.stream = s;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = split;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, &orth_small_kernel<T>,
+                                       OrthSmall{g, out, row_stride, batch_stride, rows, cols, p->steps, wide, split, p->a, p->b, p->c,
+                                                 p->eps, w.part, w.parts, w.image}));
+        return FG_OK;
     }
     OrthIn in{};
     in.g = g;

@@ -3,10 +3,9 @@
 Tolerances are on the Frobenius norm of the error and follow the iteration.  A
 product of P and Q is off by ROUND for each of its terms, independently (two
 operands' roundings to 22 bits and the product of their low planes, which is left
-out), so by ROUND * sqrt(sum of the terms' squares), and by what 32-bit sums lose: cut every
-16 k in runs of at most 256, 16 * 2^-24 of the result, and rounded when runs are added,
-another 8 * 2^-24; a matrix
-kept between products adds 2^-22 of its norm.  An error of X grows in a step by
+out), so by ROUND * sqrt(sum of the terms' squares), and by what 32-bit sums lose: 16 * 2^-24 of
+the result for the cuts within runs of at most 128 k (twice what their eight additions make)
+and 8 * 2^-24 for the runs' additions; a matrix kept between products adds 2^-22 of its norm.  An error of X grows in a step by
 the largest slope of a s + b s^3 + c s^5 over the singular values, chords through
 the origin among them.  Three times the sum of these is allowed, the terms being
 standard deviations, and the rounding of the result to its type.
@@ -76,7 +75,8 @@ def _check(ad, g, t, steps=5, coef=COEF, eps=1e-7):
     return got
 
 
-SHAPES = [(1, 1), (1, 50), (50, 1), (7, 5), (5, 7), (64, 64), (100, 257), (128, 256), (256, 128), (129, 127), (333, 101),
+SHAPES = [(128, 257), (600, 100), (40, 511), (128, 512), (513, 128), (70, 1000), (1024, 128), (3, 1025), (128, 2000), (2048, 65),
+          (100, 2049), (1, 2048), (1, 1), (1, 50), (50, 1), (7, 5), (5, 7), (64, 64), (100, 257), (128, 256), (256, 128), (129, 127), (333, 101),
           (101, 333), (768, 300), (1000, 1000), (64, 3000), (3000, 60), (2000, 520), (768, 1536)]
 
 
@@ -88,7 +88,8 @@ def test_orthogonalize(ad, shape, t):
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16"])
-@pytest.mark.parametrize("batch,m,n", [(2, 40, 24), (3, 100, 257), (8, 256, 128), (5, 128, 700), (4, 1024, 600)])
+@pytest.mark.parametrize("batch,m,n", [(2, 40, 24), (3, 100, 257), (8, 256, 128), (5, 128, 700), (4, 1024, 600),
+                                       (30, 64, 1500), (29, 700, 120), (200, 30, 300)])
 def test_orthogonalize_batches(ad, batch, m, n, t):
     x = (torch.randn(batch, m, n, generator=_gen(m), device="cuda") * torch.logspace(-6, 3, batch, device="cuda")[:, None, None]).to(T[t])
     got = _check(ad, x, t)
@@ -100,7 +101,7 @@ def test_orthogonalize_batches(ad, batch, m, n, t):
 @pytest.mark.parametrize("steps", [0, 1, 2, 8])
 @pytest.mark.parametrize("coef", [COEF, (1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (1.5, -0.6, 0.01), (1.9, 0.0, 0.0)])
 def test_orthogonalize_steps_and_coefficients(ad, steps, coef):
-    for m, n in ((60, 200), (300, 70)):
+    for m, n in ((60, 200), (300, 70), (100, 1100), (300, 260)):
         _check(ad, torch.randn(m, n, generator=_gen(m + steps), device="cuda"), "f32", steps, coef)
 
 
@@ -135,7 +136,7 @@ def test_orthogonalize_strides(ad, t):
 
 
 def test_orthogonalize_ends(ad):
-    for m, n in ((40, 100), (100, 40), (300, 300)):
+    for m, n in ((40, 100), (100, 40), (120, 900), (600, 50), (300, 300)):
         z = torch.zeros(3, m, n, device="cuda")
         z[1] = torch.randn(m, n, generator=_gen(m), device="cuda")
         alone = ad.orthogonalize(z[1])
@@ -153,7 +154,7 @@ def test_orthogonalize_ends(ad):
 
 
 @pytest.mark.parametrize("t", ["f32", "f16"])
-@pytest.mark.parametrize("batch,m,n", [(1, 5, 7), (2, 100, 33), (3, 33, 257), (1, 300, 129), (2, 131, 515)])
+@pytest.mark.parametrize("batch,m,n", [(1, 5, 7), (2, 100, 33), (3, 33, 257), (1, 300, 129), (2, 131, 515), (2, 1111, 97)])
 def test_orthogonalize_stays_within_its_matrices(ad, batch, m, n, t):
     """Through the C ABI: what lies around the result and the workspace is left as it was."""
     import ctypes as C
@@ -172,6 +173,32 @@ def test_orthogonalize_stays_within_its_matrices(ad, batch, m, n, t):
         assert torch.equal(got, want)
         assert (frame[:7] == 77).all() and (frame[-7:] == 77).all()
         assert (ws[:256] == 77).all() and (ws[256 + need:] == 77).all()
+
+
+@pytest.mark.parametrize("m,n", [(90, 200), (100, 900), (300, 260)])
+def test_orthogonalize_at_once_and_captured(ad, m, n):
+    """Calls on several streams at once, and two captured graphs beside them, each with its
+    workspace."""
+    xs = [torch.randn(m, n, generator=_gen(k), device="cuda") for k in range(4)]
+    want = [ad.orthogonalize(x) for x in xs]
+    torch.cuda.synchronize()
+    graphs = []
+    for x in xs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ad.orthogonalize(x)
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(5):
+        got = []
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                if k < 2:
+                    graphs[k][0].replay()
+                got.append(graphs[k][1] if k < 2 else ad.orthogonalize(xs[k]))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
 
 
 def test_orthogonalize_refusals(ad):

@@ -182,10 +182,11 @@ struct OrthArgs {
     uint32_t idesc;
 };
 
-template <int BN>
+// DEEP: twice the stages, for products whose blocks have an SM each.
+template <int BN, bool DEEP>
 struct OrthRing {
     static constexpr int A = 2 * OT_M * OT_K * 2, B = 2 * BN * OT_K * 2, STAGE = A + B;
-    static constexpr int N = BN == 64 ? 2 : 3;                   // 64: two blocks to an SM
+    static constexpr int N = BN == 128 ? 3 : DEEP ? 4 : 2;       // 2: two blocks to an SM
     static constexpr int COLS = 2 * BN;                          // of TMEM: h h', and the others
 };
 
@@ -209,10 +210,10 @@ __device__ __forceinline__ float4 orth_peer(uint32_t a, uint32_t rank) {
     return v;
 }
 
-template <class T, int BN, bool SPLIT>
-__global__ void __launch_bounds__(OT_NT, BN == 64 ? 2 : 1)
+template <class T, int BN, bool SPLIT, bool DEEP>
+__global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
     orth_product_kernel(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMap tq, const __grid_constant__ OrthArgs g) {
-    using Ring = OrthRing<BN>;
+    using Ring = OrthRing<BN, DEEP>;
     constexpr int LDP = BN + 4;  // partial row: 4 floats of padding keep 16-byte stores off each other's banks
     extern __shared__ __align__(1024) unsigned char dsmem[];
     __shared__ __align__(8) uint64_t full[Ring::N], empty[Ring::N], acc_full, acc_empty;
@@ -825,6 +826,7 @@ static int orth_map(CUtensorMap* m, const __half* p, int batch, long long rows, 
 
 struct OrthPlan {
     int bn, split;
+    bool deep;
 };
 
 static long long orth_tiles(long long m, long long n, int bn, bool sym) {
@@ -836,26 +838,29 @@ static long long orth_tiles(long long m, long long n, int bn, bool sym) {
 }
 
 // The tile width and split that finish first by this estimate, in microseconds: a K block
-// takes 0.75 in tiles of 64 columns, of which two blocks share an SM, and 0.7 in tiles of
-// 128, what follows the products 3 and 3.5, and an exchange over the cluster 1, 2 or 4 more.
-// Measured for the sizes 512 x 256 to 2048 x 2048, each product with each choice: within 1 us
-// of the best one.  (Tiles of 256 columns, whose accumulators fill TMEM, took 95 us where
-// these take 77: 2048 x 1024 from the right, four matrices.)
+// takes 0.75 in tiles of 64 columns, of which two blocks share an SM, 0.4 in such tiles with
+// the SM and twice the stages to themselves, 0.7 in tiles of 128; what follows the products 3,
+// 3 and 3.7; and an exchange over the cluster, by what each CTA has left to finish, 1.8 of
+// two, and of four 0.5 where results go to two places (SYM), else 2.  Measured for 400 x 300
+// to 2048 x 2048, each product with each choice: within 1.5 us of the best one.  (Tiles of
+// 256 columns, whose accumulators fill TMEM, took 95 us where these take 77: 2048 x 1024 from
+// the right, four matrices.)
 static OrthPlan orth_plan(long long m, long long n, long long k, int batch, bool sym) {
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount)), kb = (int)((k + OT_K - 1) / OT_K);
-    OrthPlan best{128, 1};
+    OrthPlan best{128, 1, false};
     double least = 1e300;
-    for (int bn : {128, 64}) {
-        const long long tiles = orth_tiles(m, n, bn, sym) * batch;
+    for (const OrthPlan& way : {OrthPlan{128, 1, false}, OrthPlan{64, 1, false}, OrthPlan{64, 1, true}}) {
+        const long long tiles = orth_tiles(m, n, way.bn, sym) * batch;
         for (int sp : {1, 2, 4, 8}) {
             if (sp > kb) break;
             int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
-            if (bn == 64) slots *= 2;
-            const double each = (kb + sp - 1) / sp * (bn == 128 ? 0.7 : 0.75) + (bn == 128 ? 3.5 : 3.0) + (sp == 8 ? 4 : sp == 4 ? 2 : sp - 1);
+            if (way.bn == 64 && !way.deep) slots *= 2;
+            const double each = (kb + sp - 1) / sp * (way.bn == 128 ? 0.7 : way.deep ? 0.4 : 0.75) + (way.bn == 128 ? 3.7 : 3.0) +
+                                (sp == 1 ? 0.0 : sp == 2 ? 1.8 : sp == 4 ? (sym ? 0.5 : 2.0) : 4.0);
             const double cost = (double)((tiles + slots - 1) / slots) * each;
             if (cost < least) {
                 least = cost;
-                best = OrthPlan{bn, sp};
+                best = OrthPlan{way.bn, sp, way.deep};
             }
         }
     }
@@ -870,7 +875,7 @@ struct OrthOperand {
     bool mn;
 };
 
-template <class T, int BN>
+template <class T, int BN, bool DEEP>
 static int launch_product(const OrthOperand& p, const OrthOperand& q, OrthArgs g, int batch, cudaStream_t s) {
     CUtensorMap tp, tq;
     int rc = orth_map(&tp, p.p, batch, p.rows, p.cols, p.ld, p.mn, OT_M);
@@ -885,8 +890,8 @@ static int launch_product(const OrthOperand& p, const OrthOperand& q, OrthArgs g
     g.idesc = (1u << 4) | ((uint32_t)p.mn << 15) | ((uint32_t)q.mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(OT_M >> 4) << 24);
     const long long ctas = (long long)g.tiles * batch * g.split;
     FG_REQUIRE(ctas <= 0x7fffffffll, "too many tiles");
-    auto kernel = g.split > 1 ? &orth_product_kernel<T, BN, true> : &orth_product_kernel<T, BN, false>;
-    const int smem = OrthRing<BN>::N * OrthRing<BN>::STAGE + 1024;
+    auto kernel = g.split > 1 ? &orth_product_kernel<T, BN, true, DEEP> : &orth_product_kernel<T, BN, false, DEEP>;
+    const int smem = OrthRing<BN, DEEP>::N * OrthRing<BN, DEEP>::STAGE + 1024;
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
@@ -910,7 +915,9 @@ static int product(const OrthOperand& p, const OrthOperand& q, OrthArgs g, long 
     const OrthPlan plan = orth_plan(g.m, g.n, k, batch, g.sym);
     g.split = plan.split;
     g.kt = (int)((k + OT_K - 1) / OT_K);
-    return plan.bn == 128 ? launch_product<T, 128>(p, q, g, batch, s) : launch_product<T, 64>(p, q, g, batch, s);
+    return plan.bn == 128 ? launch_product<T, 128, false>(p, q, g, batch, s)
+           : plan.deep    ? launch_product<T, 64, true>(p, q, g, batch, s)
+                          : launch_product<T, 64, false>(p, q, g, batch, s);
 }
 
 struct OrthWs {

@@ -875,49 +875,65 @@ struct OrthOperand {
     bool mn;
 };
 
-template <class T, int BN, bool DEEP>
-static int launch_product(const OrthOperand& p, const OrthOperand& q, OrthArgs g, int batch, cudaStream_t s) {
+// A product ready to launch: a step's are the last step's but for the buffers of X, so they
+// are made once a call (each tensor map takes the host a microsecond).
+struct OrthProduct {
     CUtensorMap tp, tq;
-    int rc = orth_map(&tp, p.p, batch, p.rows, p.cols, p.ld, p.mn, OT_M);
-    if (!rc) rc = orth_map(&tq, q.p, batch, q.rows, q.cols, q.ld, q.mn, BN);
+    OrthArgs g;
+    OrthPlan plan;
+    unsigned ctas;
+};
+
+static int make_product(const OrthOperand& p, const OrthOperand& q, const OrthArgs& args, long long k, int batch, OrthProduct& o) {
+    o.plan = orth_plan(args.m, args.n, k, batch, args.sym);
+    const int bn = o.plan.bn;
+    int rc = orth_map(&o.tp, p.p, batch, p.rows, p.cols, p.ld, p.mn, OT_M);
+    if (!rc) rc = orth_map(&o.tq, q.p, batch, q.rows, q.cols, q.ld, q.mn, bn);
     if (rc) return rc;
+    OrthArgs& g = o.g;
+    g = args;
+    g.split = o.plan.split;
+    g.kt = (int)((k + OT_K - 1) / OT_K);
     g.p_mn = p.mn;
     g.q_mn = q.mn;
     g.mt = (g.m + OT_M - 1) / OT_M;
-    g.nt = (g.n + BN - 1) / BN;
-    g.tiles = (int)orth_tiles(g.m, g.n, BN, g.sym);
+    g.nt = (g.n + bn - 1) / bn;
+    g.tiles = (int)orth_tiles(g.m, g.n, bn, g.sym);
     // kind::f16: f16 operands, f32 accumulators
-    g.idesc = (1u << 4) | ((uint32_t)p.mn << 15) | ((uint32_t)q.mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(OT_M >> 4) << 24);
+    g.idesc = (1u << 4) | ((uint32_t)p.mn << 15) | ((uint32_t)q.mn << 16) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(OT_M >> 4) << 24);
     const long long ctas = (long long)g.tiles * batch * g.split;
     FG_REQUIRE(ctas <= 0x7fffffffll, "too many tiles");
-    auto kernel = g.split > 1 ? &orth_product_kernel<T, BN, true, DEEP> : &orth_product_kernel<T, BN, false, DEEP>;
+    o.ctas = (unsigned)ctas;
+    return FG_OK;
+}
+
+template <class T, int BN, bool DEEP>
+static int launch_product(const OrthProduct& o, cudaStream_t s) {
+    auto kernel = o.plan.split > 1 ? &orth_product_kernel<T, BN, true, DEEP> : &orth_product_kernel<T, BN, false, DEEP>;
     const int smem = OrthRing<BN, DEEP>::N * OrthRing<BN, DEEP>::STAGE + 1024;
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.gridDim = dim3(o.ctas);
     cfg.blockDim = dim3(OT_NT);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = g.split;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = o.plan.split;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 2;
-    FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tp, tq, g));
+    cfg.numAttrs = o.plan.split > 1 ? 2 : 1;
+    FG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, o.tp, o.tq, o.g));
     return FG_OK;
 }
 
 template <class T>
-static int product(const OrthOperand& p, const OrthOperand& q, OrthArgs g, long long k, int batch, cudaStream_t s) {
-    const OrthPlan plan = orth_plan(g.m, g.n, k, batch, g.sym);
-    g.split = plan.split;
-    g.kt = (int)((k + OT_K - 1) / OT_K);
-    return plan.bn == 128 ? launch_product<T, 128, false>(p, q, g, batch, s)
-           : plan.deep    ? launch_product<T, 64, true>(p, q, g, batch, s)
-                          : launch_product<T, 64, false>(p, q, g, batch, s);
+static int product(const OrthProduct& o, cudaStream_t s) {
+    return o.plan.bn == 128 ? launch_product<T, 128, false>(o, s)
+           : o.plan.deep    ? launch_product<T, 64, true>(o, s)
+                            : launch_product<T, 64, false>(o, s);
 }
 
 struct OrthWs {
@@ -1024,40 +1040,50 @@ static int orthogonalize(const fg_orthogonalize_params* p, const void* g, void* 
     if (rc) return rc;
     orth_scale_kernel<T><<<dim3(in.parts, batch), OI_NT, 0, s>>>(in);
     if ((rc = check_launch("orth_scale_kernel"))) return rc;
+    if (p->steps == 0) return FG_OK;
     const bool tall = rows > cols;
-    for (int k = 0; k < p->steps; ++k) {
-        const __half* x = w.x[k & 1];
-        const bool last = k + 1 == p->steps;
+    OrthProduct first[2], second, third[2];  // by the buffer that X lies in
+    const OrthOperand as{w.a, side, side, lda, false}, bs{p->c == 0.0f ? w.a : w.b, side, side, lda, false};
+    for (int k = 0; k < std::min(2, p->steps); ++k) {
         OrthArgs a{};  // A = X X^T, or without c already B = b A
         a.m = a.n = side;
         a.sym = 1;
         a.beta = p->c == 0.0f ? p->b : 1.0f;
         a.d = w.a;
         a.ldd = lda;
-        const OrthOperand xs{x, rows, cols, ldx, tall};
-        if ((rc = product<T>(xs, xs, a, far, batch, s))) return rc;
-        const OrthOperand as{w.a, side, side, lda, false}, bs{p->c == 0.0f ? w.a : w.b, side, side, lda, false};
-        if (p->c != 0.0f) {  // B = b A + c A A
-            a.alpha = p->b;
-            a.beta = p->c;
-            a.c = w.a;
-            a.ldc = lda;
-            a.d = w.b;
-            if ((rc = product<T>(as, as, a, side, batch, s))) return rc;
-        }
+        const OrthOperand xs{w.x[k], rows, cols, ldx, tall};
+        if ((rc = make_product(xs, xs, a, far, batch, first[k]))) return rc;
         OrthArgs d{};  // X = a X + B X, or a X + X B
         d.m = rows;
         d.n = cols;
         d.alpha = p->a;
         d.beta = 1.0f;
-        d.c = x;
+        d.c = w.x[k];
         d.ldc = ldx;
-        d.d = last ? nullptr : w.x[(k + 1) & 1];
+        d.d = w.x[k ^ 1];
         d.ldd = ldx;
         d.out = out;
         d.vec = cols % 4 == 0 && aligned(out, 4 * es);
-        const OrthOperand xk{x, rows, cols, ldx, !tall};
-        if ((rc = tall ? product<T>(xk, bs, d, side, batch, s) : product<T>(bs, xk, d, side, batch, s))) return rc;
+        const OrthOperand xk{w.x[k], rows, cols, ldx, !tall};
+        if ((rc = make_product(tall ? xk : bs, tall ? bs : xk, d, side, batch, third[k]))) return rc;
+    }
+    if (p->c != 0.0f) {  // B = b A + c A A
+        OrthArgs a{};
+        a.m = a.n = side;
+        a.sym = 1;
+        a.alpha = p->b;
+        a.beta = p->c;
+        a.c = w.a;
+        a.ldc = lda;
+        a.d = w.b;
+        a.ldd = lda;
+        if ((rc = make_product(as, as, a, side, batch, second))) return rc;
+    }
+    for (int k = 0; k < p->steps; ++k) {
+        if ((rc = product<T>(first[k & 1], s))) return rc;
+        if (p->c != 0.0f && (rc = product<T>(second, s))) return rc;
+        if (k + 1 == p->steps) third[k & 1].g.d = nullptr;  // to `out`
+        if ((rc = product<T>(third[k & 1], s))) return rc;
     }
     return FG_OK;
 }

@@ -83,7 +83,7 @@ __device__ __forceinline__ void gd_store(E* p, const E (&v)[VEC], int left, int 
 }
 
 template <class T, int ACT>
-__global__ void __launch_bounds__(GD_WARPS * 32, 2) gated_dz_kernel(const GatedDz g) {
+__global__ void __launch_bounds__(GD_WARPS * 32, 3) gated_dz_kernel(const GatedDz g) {
     constexpr int VEC = 16 / sizeof(T);
     constexpr bool FAST = sizeof(T) == 2;
     using E = typename std::conditional<FAST, T, __nv_bfloat16>::type;  // of an operand
@@ -158,10 +158,10 @@ __global__ void __launch_bounds__(GD_WARPS * 32, 2) gated_dz_kernel(const GatedD
     }
 }
 
-// Row ranges: two blocks to an SM over the column tiles, 16 rows at least to a range.
+// Row ranges: three blocks to an SM over the column tiles, 16 rows at least to a range.
 static int gated_dz_split(long long rows, int up, int elem) {
     const int cols = 32 * (16 / elem), tiles = (up + cols - 1) / cols;
-    const long long fill = std::max(1ll, 2ll * std::max(1, device_attr(cudaDevAttrMultiProcessorCount)) / tiles);
+    const long long fill = std::max(1ll, 3ll * std::max(1, device_attr(cudaDevAttrMultiProcessorCount)) / tiles);
     return (int)std::max(1ll, std::min(fill, (rows + 15) / 16));
 }
 

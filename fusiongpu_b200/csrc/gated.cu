@@ -19,7 +19,8 @@ namespace fg {
 // A warp takes 32 x VEC gates of every eighth row of its block's range and sums its
 // columns in registers; the block writes one partial row.  Both factors are products of
 // values of the layer's type, so 16-bit ones enter the products in two parts (split2)
-// whatever the activation.
+// whatever the activation.  Bound by the latency of its loads and by memory: 10,000 x 1024
+// bfloat16 30 us (143 MB, 4.8 TB/s), float16 28, float32 45 (55 with two blocks an SM).
 constexpr int GD_WARPS = 8;
 
 struct GatedDz {

@@ -171,8 +171,8 @@ __device__ __forceinline__ QuantRow row_of(uint32_t top, uint32_t* s) {
 __device__ __forceinline__ float scale_of(const QuantRow& q) { return q.finite ? q.top / 127.0f : NAN; }
 
 // L threads a row (8, 32 or the block), PER pieces of 16 bytes each.  Groups take rows in
-// turn and ask for the next one before they work on this one (1M x 768 float16: 376 us, 6.1
-// TB/s; with a group a row 501).
+// turn and ask for the next one before they work on this one.  Bound by memory, and nearly
+// by issue slots (70 %): 1M x 768 float16 363 to 417 us, 5.5 to 6.3 TB/s (a group a row: 501).
 template <class T, int L, int PER>
 __global__ void __launch_bounds__(QR_NT, PER <= 4 ? 4 : 2) quantize_kernel(const QuantArgs g) {
     constexpr int VEC = 16 / sizeof(T), GROUPS = QR_NT / L;
@@ -256,6 +256,8 @@ static int launch_quantize(QuantArgs g, cudaStream_t s) {
 }
 
 // ---- a few rows: a warp a column, four codes at a time -----------------------------
+//
+// Bound by the latency of the loads: 768 -> 1536 2.6 us for one row, 3.1 for eight.
 template <class T, int R>
 __global__ void __launch_bounds__(128) gemv_int8_kernel(const signed char* __restrict__ x, const signed char* __restrict__ w,
                                                         const GemmShape g, int wide, const float* xs, const float* ws, const Epilogue e) {

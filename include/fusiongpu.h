@@ -572,7 +572,7 @@ int fg_linear_int8(const fg_linear_params* params, const int8_t* x, const float*
  * (batch_stride 0: rows * row_stride).  Between the products matrices are held to 22
  * bits (or 2^-36) as pairs of float16: a, b and c, of at most 16, have to keep
  * singular values of at most one of order one, as 3.4445, -4.7750, 2.0315 do.  A
- * matrix that holds an infinity or a NaN is NaN.  steps <= 100, rows and cols <=
+ * matrix that holds an infinity or a NaN is NaN after a step.  steps <= 100, rows and cols <=
  * 32768, batch <= 65535. */
 typedef struct {
     int32_t batch;

@@ -17,7 +17,9 @@ namespace fg {
 // ---- dz and dp, and their column sums ----------------------------------------------
 //
 // A warp takes 32 x VEC gates of every eighth row of its block's range and sums its
-// columns in registers; the block writes one partial row.  Both factors are products of
+// columns in registers; the block writes one partial row.  A lane's VEC gates lie beside each
+// other where the operand's halves start on 16 bytes, else 32 apart, so that a warp's
+// accesses of one element are in order (1,777 x 333 bfloat16: 14.1 us beside each other).  Both factors are products of
 // values of the layer's type, so 16-bit ones enter the products in two parts (split2)
 // whatever the activation.  Bound by the latency of its loads and by memory: 10,000 x 1024
 // bfloat16 30 us (143 MB, 4.8 TB/s), float16 28, float32 45 (55 with two blocks an SM).
@@ -40,6 +42,10 @@ __device__ __forceinline__ void act_both(float z, float& a, float& d) {
         a = c * s;
         d = s * fmaf(fminf(c, 100.0f), 1.0f - s, 1.0f);
         if (z != z) d = z;
+    } else if (ACT == FG_ACT_GELU && !FAST) {  // one Phi for both
+        const float c = fminf(fmaxf(z, -100.0f), 100.0f), phi = 0.5f * erfcf(z * -0.70710678f);
+        a = fmaxf(z, -100.0f) * phi;
+        d = fmaf(c, expf(-0.5f * z * z) * 0.39894228f, phi);
     } else {
         a = activate<FAST>(z, ACT);
         d = activate_grad<FAST>(z, ACT);
@@ -58,19 +64,18 @@ __device__ __forceinline__ void act_both2(float z0, float z1, float& a0, float& 
     }
 }
 
+// VEC values of a row: from p on, or 32 apart.
 template <class T, int VEC>
-__device__ __forceinline__ void gd_load(T (&v)[VEC], const T* p, int left, int wide) {
+__device__ __forceinline__ void gd_load(T (&v)[VEC], const T* p, int left, int wide, int step) {
     if (wide && left >= VEC) {
         *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
     } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = i < left ? p[i] : from_f32<T>(0.0f);
+        for (int i = 0; i < VEC; ++i) v[i] = i * step < left ? p[i * step] : from_f32<T>(0.0f);
     }
 }
-
-// VEC values of `step`-bit operands at p: whole where rows and halves allow.
 template <class E, int VEC>
-__device__ __forceinline__ void gd_store(E* p, const E (&v)[VEC], int left, int wide) {
+__device__ __forceinline__ void gd_store(E* p, const E (&v)[VEC], int left, int wide, int step) {
     if (wide && left >= VEC) {
         if constexpr (sizeof(E) * VEC == 16)
             *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
@@ -79,7 +84,7 @@ __device__ __forceinline__ void gd_store(E* p, const E (&v)[VEC], int left, int 
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
-            if (i < left) p[i] = v[i];
+            if (i * step < left) p[i * step] = v[i];
     }
 }
 
@@ -89,7 +94,8 @@ __global__ void __launch_bounds__(GD_WARPS * 32, 3) gated_dz_kernel(const GatedD
     constexpr bool FAST = sizeof(T) == 2;
     using E = typename std::conditional<FAST, T, __nv_bfloat16>::type;  // of an operand
     __shared__ float s[GD_WARPS][32 * VEC];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = (blockIdx.x * 32 + lane) * VEC, left = g.up - j;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int step = g.out_wide ? 1 : 32, j = blockIdx.x * 32 * VEC + lane * (g.out_wide ? VEC : 1), left = g.up - j;
     const long long r0 = blockIdx.y * g.per, r1 = min(r0 + g.per, g.rows), ldz = pack_stride(2ll * g.up);
     float sum[2][VEC];
 #pragma unroll
@@ -98,9 +104,9 @@ __global__ void __launch_bounds__(GD_WARPS * 32, 3) gated_dz_kernel(const GatedD
         for (long long r = r0 + warp; r < r1; r += GD_WARPS) {
             alignas(16) T d[VEC], z[VEC], p[VEC];
             const T* pre = static_cast<const T*>(g.pre) + r * g.ldp + j;
-            gd_load<T, VEC>(d, static_cast<const T*>(g.dy) + r * g.lddy + j, left, g.in_wide);
-            gd_load<T, VEC>(z, pre, left, g.in_wide);
-            gd_load<T, VEC>(p, pre + g.up, left, g.in_wide);
+            gd_load<T, VEC>(d, static_cast<const T*>(g.dy) + r * g.lddy + j, left, g.in_wide, step);
+            gd_load<T, VEC>(z, pre, left, g.in_wide, step);
+            gd_load<T, VEC>(p, pre + g.up, left, g.in_wide, step);
             float o[2][VEC];
 #pragma unroll
             for (int i = 0; i < VEC; i += 2) {
@@ -124,8 +130,8 @@ __global__ void __launch_bounds__(GD_WARPS * 32, 3) gated_dz_kernel(const GatedD
 #pragma unroll
                     for (int i = 0; i < VEC; i += 2)
                         split2(o[h][i], o[h][i + 1], *reinterpret_cast<T2*>(hi + i), *reinterpret_cast<T2*>(low + i));
-                    gd_store<T, VEC>(out, hi, left, g.out_wide);
-                    gd_store<T, VEC>(out + g.plane, low, left, g.out_wide);
+                    gd_store<T, VEC>(out, hi, left, g.out_wide, step);
+                    gd_store<T, VEC>(out + g.plane, low, left, g.out_wide, step);
                 } else {
                     alignas(8) __nv_bfloat16 pl[3][VEC];
 #pragma unroll
@@ -137,7 +143,7 @@ __global__ void __launch_bounds__(GD_WARPS * 32, 3) gated_dz_kernel(const GatedD
                         pl[2][i] = w[2];
                     }
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) gd_store<__nv_bfloat16, VEC>(out + k * g.plane, pl[k], left, g.out_wide);
+                    for (int k = 0; k < 3; ++k) gd_store<__nv_bfloat16, VEC>(out + k * g.plane, pl[k], left, g.out_wide, step);
                 }
             }
         }
@@ -146,7 +152,7 @@ __global__ void __launch_bounds__(GD_WARPS * 32, 3) gated_dz_kernel(const GatedD
     for (int h = 0; h < 2; ++h) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s[warp][lane * VEC + i] = h ? sum[1][i] : sum[0][i];
+        for (int i = 0; i < VEC; ++i) s[warp][lane * (g.out_wide ? VEC : 1) + i * step] = h ? sum[1][i] : sum[0][i];
         __syncthreads();
         for (int c = threadIdx.x; c < 32 * VEC; c += GD_WARPS * 32) {
             const int col = blockIdx.x * 32 * VEC + c;

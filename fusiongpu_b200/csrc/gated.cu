@@ -16,9 +16,10 @@ namespace fg {
 
 // ---- dz and dp, and their column sums ----------------------------------------------
 //
-// A warp takes 32 x VEC gates of every eighth row of its block's range and sums its
-// columns in registers; the block writes one partial row.  A lane's VEC gates lie beside each
-// other where the operand's halves start on 16 bytes, else 32 apart, so that a warp's
+// A group of L lanes takes L x VEC gates of every so many rows of its block's range and
+// sums its columns in registers; the block writes one partial row.  L is 32, or 16 or 8 for
+// layers as narrow as that (100,000 x 40 float16: 64 us with whole warps).  A lane's VEC gates lie beside each
+// other where the operand's halves start on 16 bytes, else L apart, so that a group's
 // accesses of one element are in order (1,777 x 333 bfloat16: 14.1 us beside each other).  Both factors are products of
 // values of the layer's type, so 16-bit ones enter the products in two parts (split2)
 // whatever the activation.  Bound by the latency of its loads and by memory: 10,000 x 1024
@@ -64,7 +65,7 @@ __device__ __forceinline__ void act_both2(float z0, float z1, float& a0, float& 
     }
 }
 
-// VEC values of a row: from p on, or 32 apart.
+// VEC values of a row: from p on, or `step` apart.
 template <class T, int VEC>
 __device__ __forceinline__ void gd_load(T (&v)[VEC], const T* p, int left, int wide, int step) {
     if (wide && left >= VEC) {
@@ -88,20 +89,21 @@ __device__ __forceinline__ void gd_store(E* p, const E (&v)[VEC], int left, int 
     }
 }
 
-template <class T, int ACT>
+template <class T, int ACT, int L>
 __global__ void __launch_bounds__(GD_WARPS * 32, 3) gated_dz_kernel(const GatedDz g) {
     constexpr int VEC = 16 / sizeof(T);
     constexpr bool FAST = sizeof(T) == 2;
     using E = typename std::conditional<FAST, T, __nv_bfloat16>::type;  // of an operand
-    __shared__ float s[GD_WARPS][32 * VEC];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int step = g.out_wide ? 1 : 32, j = blockIdx.x * 32 * VEC + lane * (g.out_wide ? VEC : 1), left = g.up - j;
+    constexpr int GROUPS = GD_WARPS * 32 / L;
+    __shared__ float s[GROUPS][L * VEC];
+    const int lane = threadIdx.x % L, group = threadIdx.x / L;
+    const int step = g.out_wide ? 1 : L, j = blockIdx.x * L * VEC + lane * (g.out_wide ? VEC : 1), left = g.up - j;
     const long long r0 = blockIdx.y * g.per, r1 = min(r0 + g.per, g.rows), ldz = pack_stride(2ll * g.up);
     float sum[2][VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum[0][i] = sum[1][i] = 0.0f;
     if (left > 0)
-        for (long long r = r0 + warp; r < r1; r += GD_WARPS) {
+        for (long long r = r0 + group; r < r1; r += GROUPS) {
             alignas(16) T d[VEC], z[VEC], p[VEC];
             const T* pre = static_cast<const T*>(g.pre) + r * g.ldp + j;
             gd_load<T, VEC>(d, static_cast<const T*>(g.dy) + r * g.lddy + j, left, g.in_wide, step);
@@ -152,39 +154,55 @@ __global__ void __launch_bounds__(GD_WARPS * 32, 3) gated_dz_kernel(const GatedD
     for (int h = 0; h < 2; ++h) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s[warp][lane * (g.out_wide ? VEC : 1) + i * step] = h ? sum[1][i] : sum[0][i];
+        for (int i = 0; i < VEC; ++i) s[group][lane * (g.out_wide ? VEC : 1) + i * step] = h ? sum[1][i] : sum[0][i];
         __syncthreads();
-        for (int c = threadIdx.x; c < 32 * VEC; c += GD_WARPS * 32) {
-            const int col = blockIdx.x * 32 * VEC + c;
+        for (int c = threadIdx.x; c < L * VEC; c += GD_WARPS * 32) {
+            const int col = blockIdx.x * L * VEC + c;
             if (col >= g.up) break;
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < GD_WARPS; ++w) v += s[w][c];
+            for (int w = 0; w < GROUPS; ++w) v += s[w][c];
             g.part[(size_t)blockIdx.y * 2 * g.up + (size_t)h * g.up + col] = v;
         }
     }
 }
 
-// Row ranges: three blocks to an SM over the column tiles, 16 rows at least to a range.
+// Lanes of a group: as few as hold the layer's width.
+static int gated_dz_lanes(int up, int elem) {
+    const int pieces = (up + 16 / elem - 1) / (16 / elem);
+    return pieces <= 8 ? 8 : pieces <= 16 ? 16 : 32;
+}
+
+// Row ranges: three blocks to an SM over the column tiles, two rows to a group at least.
 static int gated_dz_split(long long rows, int up, int elem) {
-    const int cols = 32 * (16 / elem), tiles = (up + cols - 1) / cols;
+    const int lanes = gated_dz_lanes(up, elem), cols = lanes * (16 / elem), least = 2 * GD_WARPS * 32 / lanes, tiles = (up + cols - 1) / cols;
     const long long fill = std::max(1ll, 3ll * std::max(1, device_attr(cudaDevAttrMultiProcessorCount)) / tiles);
-    return (int)std::max(1ll, std::min(fill, (rows + 15) / 16));
+    return (int)std::max(1ll, std::min(fill, (rows + least - 1) / least));
+}
+
+template <class T, int L>
+static void launch_gated_dz_of(const GatedDz& g, int split, cudaStream_t s) {
+    constexpr int cols = L * (16 / (int)sizeof(T));
+    const dim3 grid((g.up + cols - 1) / cols, split);
+    switch (g.act) {
+        case FG_ACT_RELU: gated_dz_kernel<T, FG_ACT_RELU, L><<<grid, GD_WARPS * 32, 0, s>>>(g); break;
+        case FG_ACT_GELU: gated_dz_kernel<T, FG_ACT_GELU, L><<<grid, GD_WARPS * 32, 0, s>>>(g); break;
+        case FG_ACT_SILU: gated_dz_kernel<T, FG_ACT_SILU, L><<<grid, GD_WARPS * 32, 0, s>>>(g); break;
+        default: gated_dz_kernel<T, FG_ACT_NONE, L><<<grid, GD_WARPS * 32, 0, s>>>(g);
+    }
 }
 
 template <class T>
 static int launch_gated_dz(GatedDz g, int split, cudaStream_t s) {
-    constexpr int VEC = 16 / (int)sizeof(T), cols = 32 * VEC;
+    constexpr int VEC = 16 / (int)sizeof(T);
     g.per = (g.rows + split - 1) / split;
     auto lies = [&](const void* p, long long ld) { return aligned(p, 16) && ld * (int)sizeof(T) % 16 == 0; };
     g.in_wide = lies(g.dy, g.lddy) && lies(g.pre, g.ldp) && g.up % VEC == 0;
     g.out_wide = g.up % VEC == 0;
-    const dim3 grid((g.up + cols - 1) / cols, split);
-    switch (g.act) {
-        case FG_ACT_RELU: gated_dz_kernel<T, FG_ACT_RELU><<<grid, GD_WARPS * 32, 0, s>>>(g); break;
-        case FG_ACT_GELU: gated_dz_kernel<T, FG_ACT_GELU><<<grid, GD_WARPS * 32, 0, s>>>(g); break;
-        case FG_ACT_SILU: gated_dz_kernel<T, FG_ACT_SILU><<<grid, GD_WARPS * 32, 0, s>>>(g); break;
-        default: gated_dz_kernel<T, FG_ACT_NONE><<<grid, GD_WARPS * 32, 0, s>>>(g);
+    switch (gated_dz_lanes(g.up, sizeof(T))) {
+        case 8: launch_gated_dz_of<T, 8>(g, split, s); break;
+        case 16: launch_gated_dz_of<T, 16>(g, split, s); break;
+        default: launch_gated_dz_of<T, 32>(g, split, s);
     }
     return check_launch("gated_dz_kernel");
 }

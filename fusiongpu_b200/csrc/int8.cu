@@ -321,12 +321,22 @@ static int gemv_int8(const void* x, const void* w, const GemmShape& g, const flo
 // ---- rows off 16 bytes, copied to rows on them --------------------------------------
 __global__ void __launch_bounds__(256) pack_int8_kernel(const signed char* in, signed char* out, long long rows, long long ld, int cols,
                                                         long long stride) {
-    const long long i = blockIdx.x * 256ll + threadIdx.x, per = stride / 16, row = i / per;
+    const long long i = blockIdx.x * 256ll + threadIdx.x, per = stride / 16;
+    const long long row = i <= 0x7fffffff ? (long long)((unsigned)i / (unsigned)per) : i / per;  // 64 bits take a long division
     if (row >= rows) return;
     const int c0 = (int)(i - row * per) * 16;
+    const signed char* from = in + row * ld + c0;
+    const uintptr_t start = reinterpret_cast<uintptr_t>(from);
     alignas(16) signed char v[16];
+    if (c0 + 16 <= cols && (start & 15) == 0) {
+        *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(from);
+    } else if (c0 + 16 <= cols && (start & 3) == 0) {
 #pragma unroll
-    for (int c = 0; c < 16; ++c) v[c] = c0 + c < cols ? in[row * ld + c0 + c] : (signed char)0;
+        for (int c = 0; c < 4; ++c) reinterpret_cast<uint32_t*>(v)[c] = reinterpret_cast<const uint32_t*>(from)[c];
+    } else {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) v[c] = c0 + c < cols ? from[c] : (signed char)0;
+    }
     *reinterpret_cast<uint4*>(out + row * stride + c0) = *reinterpret_cast<const uint4*>(v);
 }
 

@@ -74,7 +74,7 @@ static int simt_gemm_check(const GemmShape& g, long long* tiles) {
 // or NaN has zeros behind it; bf16's last place is 2^-133, which values below 2^-109
 // feel).  One pass over memory, eight columns a thread.
 template <class T>
-__global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackArgs a) {
     long long i = blockIdx.x * 256ll + threadIdx.x;
     for (int k = 0; k < a.jobs; ++k) {
         const PackJob& j = a.job[k];
@@ -83,13 +83,23 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
             i -= n;
             continue;
         }
-        const long long row = i / per_row;
+        // 64 bits take a division of a hundred instructions
+        const long long row = i <= 0x7fffffff ? (long long)((unsigned)i / (unsigned)per_row) : i / per_row;
         const int col = (int)(i - row * per_row) * 8, left = j.cols - col;
         const T* in = static_cast<const T*>(j.in) + row * j.ld + col;
         alignas(16) T v[8];
-        if (sizeof(T) == 4 && left >= 8 && (reinterpret_cast<uintptr_t>(in) & 15) == 0) {
-            reinterpret_cast<uint4*>(v)[0] = reinterpret_cast<const uint4*>(in)[0];
-            reinterpret_cast<uint4*>(v)[sizeof(T) / 4] = reinterpret_cast<const uint4*>(in)[sizeof(T) / 4];
+        // as many bytes at a time as the row's start allows (rows on 8: 40,000 x 500
+        // bfloat16)
+        const uintptr_t start = reinterpret_cast<uintptr_t>(in);
+        if (left >= 8 && (start & 15) == 0) {
+#pragma unroll
+            for (int c = 0; c < (int)sizeof(T) / 2; ++c) reinterpret_cast<uint4*>(v)[c] = reinterpret_cast<const uint4*>(in)[c];
+        } else if (left >= 8 && (start & 7) == 0) {
+#pragma unroll
+            for (int c = 0; c < (int)sizeof(T); ++c) reinterpret_cast<uint2*>(v)[c] = reinterpret_cast<const uint2*>(in)[c];
+        } else if (left >= 8 && (start & 3) == 0) {
+#pragma unroll
+            for (int c = 0; c < 2 * (int)sizeof(T); ++c) reinterpret_cast<uint32_t*>(v)[c] = reinterpret_cast<const uint32_t*>(in)[c];
         } else {
 #pragma unroll
             for (int c = 0; c < 8; ++c) v[c] = c < left ? in[c] : from_f32<T>(0.0f);

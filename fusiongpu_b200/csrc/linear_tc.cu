@@ -582,6 +582,20 @@ __device__ __forceinline__ void copy_rows(unsigned char* buf, T* matrix, long lo
     __syncwarp();
 }
 
+// A warp's 32 rows of 64 bytes from its buffer (64-byte swizzle) to a matrix whose rows start
+// anywhere, as copy_rows does.
+template <class T>
+__device__ __forceinline__ void store_half(const unsigned char* buf, T* matrix, long long ld, int row0, int col0, int rows, int cols, int lane) {
+    __syncwarp();
+    if (col0 + lane < cols) {
+        T* p = matrix + row0 * ld + col0 + lane;
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r)
+            if (row0 + r < rows) p[r * ld] = *reinterpret_cast<const T*>(buf + r * 64 + ((lane * 2) ^ ((r >> 1 & 3) << 4)));
+    }
+    __syncwarp();
+}
+
 template <class T>
 __device__ __forceinline__ void add_bias(float (&v)[2][32], const unsigned char* b) {
 #pragma unroll
@@ -672,7 +686,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     constexpr int BO = MODE == TC_GATED ? BN / 2 : BN, PC = MODE == TC_GATED ? 32 : 64;  // outputs of a tile's row, a warp's
     constexpr int KB = MODE == TC_INT8 ? 2 * GT_K : GT_K;
     static_assert(sizeof(T) == 2 || BN == 256, "float32 takes 256 columns");
-    static_assert(MODE != TC_GATED || (BN == 256 && !DIRECT), "gated tiles have 128 columns and TMA stores");
+    static_assert(MODE != TC_GATED || BN == 256, "gated tiles have 128 columns");
     extern __shared__ __align__(1024) unsigned char dsmem[];
     __shared__ __align__(8) uint64_t full[GP_STAGES], empty[GP_STAGES], acc_full[2], acc_empty[2], res_full[MODE == TC_INT8 ? 2 * GP_EPI : GP_EPI];
     __shared__ uint32_t tmem_slot;
@@ -962,7 +976,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         *at = make_float4(v[0], v[1], v[2], v[3]);
                     }
                     odd_seen |= __any_sync(0xffffffffu, odd && all_ok);
-                    if (e.pre) {
+                    if (e.pre && DIRECT) {
+                        copy_rows<T, true, 1>(buf, static_cast<T*>(e.pre), e.ldp, m0, col, g.m, g.n, lane);
+                        copy_rows<T, true, 1>(buf + GP_BUF, static_cast<T*>(e.pre) + g.up, e.ldp, m0, col, g.m, g.n, lane);
+                    } else if (e.pre) {
                         put(&tp, buf, false);
                         put(&tr, buf + GP_BUF, true);
                         if (tc::elect_one()) tc::bulk_wait_read<0>();
@@ -975,7 +992,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         *at = make_float4(activate<false>(z.x, e.act) * p.x, activate<false>(z.y, e.act) * p.y,
                                           activate<false>(z.z, e.act) * p.z, activate<false>(z.w, e.act) * p.w);
                     }
-                    put(&ty, buf, true);
+                    if (DIRECT)
+                        copy_rows<T, true, 1>(buf, static_cast<T*>(e.y), e.ldy, m0, col, g.m, g.n, lane);
+                    else
+                        put(&ty, buf, true);
                 }
 #pragma unroll 1
                 for (int h = MODE == TC_GATED ? 2 : 0; h < 2; ++h) {
@@ -1083,7 +1103,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 unsigned char* bias = biases + w * 128;
                 if (e.bias) {  // 32 of the gates, 32 of their partners
                     const T* b = static_cast<const T*>(e.bias) + (lane < 16 ? 0 : g.up) + col;
-                    reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(b, lane & 15, g.n - col, 0);
+                    reinterpret_cast<uint32_t*>(bias)[lane] = fetch_bias<T>(b, lane & 15, g.n - col, DIRECT);
                     __syncwarp();
                 }
                 const bool ok = tc::mbar_wait_warp(&acc_full[acc], (li >> 1) & 1, fail);
@@ -1109,7 +1129,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                         *reinterpret_cast<uint4*>(buf + h * (GP_BUF / 2) + lane * 64 + (((uint32_t)j << 1) ^ sw64)) = pack8<T>(&v[j]);
                 };
                 const bool inside = m0 < g.m && col < g.n;
-                if (e.pre) {
+                if (e.pre && DIRECT) {
+                    stage(v[0], 0);
+                    stage(v[1], 1);
+                    store_half<T>(buf, static_cast<T*>(e.pre), e.ldp, m0, col, g.m, g.n, lane);
+                    store_half<T>(buf + GP_BUF / 2, static_cast<T*>(e.pre) + g.up, e.ldp, m0, col, g.m, g.n, lane);
+                } else if (e.pre) {
                     if (tc::elect_one()) tc::bulk_wait_read<1>();  // the last tile's: its result may still leave
                     __syncwarp();
                     stage(v[0], 0);
@@ -1129,6 +1154,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                     case FG_ACT_GELU: gate_all<FG_ACT_GELU>(v); break;
                     case FG_ACT_SILU: gate_all<FG_ACT_SILU>(v); break;
                     default: gate_all<FG_ACT_NONE>(v);
+                }
+                if (DIRECT) {
+                    stage(v[0], 2);
+                    store_half<T>(buf + GP_BUF, static_cast<T*>(e.y), e.ldy, m0, col, g.m, g.n, lane);
+                    continue;
                 }
                 if (tc::elect_one()) {  // the last tile's result has left; this one's pre-activations may yet
                     if (e.pre)
@@ -1567,8 +1597,7 @@ static int launch_pair(int dtype, const void* a, const void* b, const GemmShape&
                g.n);
     const bool direct = g.direct && g.split == 1;
     auto kernel = &gemm_pair_kernel<T, BN, false, MODE>;
-    if constexpr (MODE != TC_GATED)
-        if (direct) kernel = &gemm_pair_kernel<T, BN, true, MODE>;
+    if (direct) kernel = &gemm_pair_kernel<T, BN, true, MODE>;
     if constexpr (sizeof(T) == 2 && MODE == TC_WHOLE)
         if (g.products == 2) kernel = direct ? &gemm_pair_kernel<T, BN, true, TC_PARTS> : &gemm_pair_kernel<T, BN, false, TC_PARTS>;
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), P::SMEM));
@@ -1618,7 +1647,6 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct, int mode
     const int kb = (int)((s.k + GT_K - 1) / GT_K);
     for (int bn : {256, 128}) {
         if ((products == 6 || mode == TC_GATED) && bn == 128) break;
-        if (mode == TC_GATED && direct) break;
         const long long tiles = m2 * ((s.n + bn - 1) / bn);
         // 16-bit sums run over GT_RUN K blocks at most: parts go on past 32, and past a full
         // GPU, until they are that short (in 64 bits: kb may be 2^25)
@@ -1629,7 +1657,7 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct, int mode
             if (too_long(sp)) continue;
             const size_t ws = sp > 1 ? (size_t)sp * m2 * 2 * GT_M * ((s.n + 3) / 4 * 4) * 4 : 0;
             const double epi = bn == 256 ? 2.0 : 1.0, main = (kt + sp - 1) / sp * (bn == 256 ? 0.39 : 0.34);
-            const double rows = direct ? (bn == 256 ? 14.0 : 8.0) : 0.0;
+            const double rows = !direct ? 0.0 : mode == TC_GATED ? 9.0 : bn == 256 ? 14.0 : 8.0;
             offer(6.0 + waves(tiles * sp, sms / 2) * (std::max(main, epi) + rows) + epi + (sp > 1 ? 3.0 + 1.5e-6 * ws / 6.0 : 0.0),
                   TcPlan{true, bn, sp, ws});
         }

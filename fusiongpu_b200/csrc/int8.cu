@@ -43,7 +43,7 @@ __device__ __forceinline__ uint32_t float_bits(uint32_t top) {
 }
 
 struct QuantRow {
-    float top, inv, up;  // up: a power of two that brings top to where 127 top and 127 / top are ordinary numbers
+    float top, inv, up;  // inv: 127 / top, nearly; up: a power of two that brings top to where 127 top and 127 / top are ordinary numbers
     bool finite;         // no infinity or NaN in the row
     bool fast;           // inv is an ordinary number
 };
@@ -63,27 +63,47 @@ __device__ __forceinline__ float exact_code(float x, const QuantRow& q) {
 }
 
 // Codes 127 x / top of N values, rounded to nearest, ties to even.  x times 127 / top plus
-// 1.5 2^23 rounds the product once to an integer, which the sum's low byte holds.  The
-// quotient is taken a little too small and a little too large (by 2^-22 of it, four times
-// its rounding): where both give the same integers, those are right.  Else, 16-bit values:
-// the remainder 127 x - r top is exact in 32 bits, and a code whose remainder reaches top / 2
-// is put right (exact ties are frequent in bfloat16, whose largest value has 8 bits);
-// 32-bit ones are taken again without an error.
+// 1.5 2^23 rounds the product once to an integer, which the sum's low byte holds; the
+// quotient is off by 1.5 2^-23 of it.
+//   bfloat16: exact ties are frequent (the largest value has 8 bits), and nothing else comes
+//   near a half: with t = 127 m 2^-e / n, m and n of 8 bits, a value that is none is 2^-e / 255
+//   from it at least, t at most 254 2^-e.  So what lies within 2^-22 t of a half is a tie, and
+//   goes to twice the rounded half of the quotient, which is even.
+//   float16 and float32: the quotient is taken 2^-21 too small and too large; where both give
+//   the same integers, those are right.  Else, float16: the remainder 127 x - r top is exact
+//   in 32 bits, and a code whose remainder reaches top / 2 is put right.  float32: again
+//   without an error.
 template <class T, int N>
 __device__ __forceinline__ void codes_of(uint32_t (&out)[N / 4], const T (&v)[N], const QuantRow& q) {
     constexpr float magic = 12582912.0f;
-    const float low = q.inv - q.inv * 2.3841858e-7f, high = q.inv + q.inv * 2.3841858e-7f;
-    const uint64_t l = pair2(low, low), h = pair2(high, high), m = pair2(magic, magic);
     uint32_t c[N], differ = 0;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const uint64_t inv = pair2(q.inv, q.inv), half = pair2(0.5f * q.inv, 0.5f * q.inv), m = pair2(magic, magic), minus = pair2(-magic, -magic);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-        const uint64_t x = pair2(to_f32(v[i]), to_f32(v[i + 1]));
-        float a, b, d, e;
-        unpair2(fma2(x, l, m), a, b);
-        unpair2(fma2(x, h, m), d, e);
-        c[i] = __float_as_uint(a);
-        c[i + 1] = __float_as_uint(b);
-        differ |= (c[i] ^ __float_as_uint(d)) | (c[i + 1] ^ __float_as_uint(e));
+        for (int i = 0; i < N; i += 2) {
+            const uint64_t x = pair2(to_f32(v[i]), to_f32(v[i + 1])), r = fma2(x, inv, m), back = add2(r, minus);
+            float a, b, d, e, s, t;
+            unpair2(back, a, b);
+            unpair2(fma2(x, inv, pair2(-a, -b)), d, e);
+            unpair2(fma2(x, half, m), s, t);
+            const bool tie0 = fmaf(fabsf(a), 2.3841858e-7f, fabsf(d)) >= 0.5f, tie1 = fmaf(fabsf(b), 2.3841858e-7f, fabsf(e)) >= 0.5f;
+            unpair2(r, a, b);
+            c[i] = tie0 ? __float_as_uint(s) * 2 : __float_as_uint(a);
+            c[i + 1] = tie1 ? __float_as_uint(t) * 2 : __float_as_uint(b);
+        }
+    } else {
+        const float low = q.inv - q.inv * 4.7683716e-7f, high = q.inv + q.inv * 4.7683716e-7f;
+        const uint64_t l = pair2(low, low), h = pair2(high, high), m = pair2(magic, magic);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const uint64_t x = pair2(to_f32(v[i]), to_f32(v[i + 1]));
+            float a, b, d, e;
+            unpair2(fma2(x, l, m), a, b);
+            unpair2(fma2(x, h, m), d, e);
+            c[i] = __float_as_uint(a);
+            c[i + 1] = __float_as_uint(b);
+            differ |= (c[i] ^ __float_as_uint(d)) | (c[i + 1] ^ __float_as_uint(e));
+        }
     }
     if (differ || !q.fast) {
         if (sizeof(T) == 4 || !q.fast) {
@@ -113,7 +133,9 @@ struct QuantArgs {
 // VEC neighbouring columns, `unit` bytes at a time: what the rows' starts allow.
 template <class T, int VEC>
 __device__ __forceinline__ void qr_load(T (&v)[VEC], const T* p, int left, int unit) {
-    if (unit == 16 && left >= VEC) {
+    if (left <= 0) {  // behind the row's end
+        *reinterpret_cast<uint4*>(v) = make_uint4(0, 0, 0, 0);
+    } else if (unit == 16 && left >= VEC) {
         *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
     } else if (unit >= 8 && left >= VEC) {
         reinterpret_cast<uint2*>(v)[0] = reinterpret_cast<const uint2*>(p)[0];
@@ -129,6 +151,7 @@ __device__ __forceinline__ void qr_load(T (&v)[VEC], const T* p, int left, int u
 
 template <class T, int VEC>
 __device__ __forceinline__ void qr_store(signed char* p, const T (&v)[VEC], const QuantRow& q, int left, int wide) {
+    if (left <= 0) return;
     uint32_t codes[VEC / 4];
     codes_of<T, VEC>(codes, v, q);
     if (wide && left >= VEC) {
@@ -163,18 +186,28 @@ __device__ __forceinline__ QuantRow row_of(uint32_t top, uint32_t* s) {
     QuantRow q;
     q.finite = top < 0x7f800000u;
     q.top = __uint_as_float(top);
-    q.inv = 127.0f / q.top;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q.inv) : "f"(q.top));
+    q.inv *= 127.0f;
     q.up = q.top < 1e-18f ? 18446744073709551616.0f : q.top > 1e30f ? 1.0f / 65536.0f : 1.0f;  // 2^64, 2^-16
     q.fast = q.finite && q.up == 1.0f;
     return q;
 }
-__device__ __forceinline__ float scale_of(const QuantRow& q) { return q.finite ? q.top / 127.0f : NAN; }
+// top / 127, correctly rounded: one correction of the product with the rounded 1 / 127, which
+// gives the division's bits for all significands; tiny and huge rows divide.
+__device__ __forceinline__ float scale_of(const QuantRow& q) {
+    if (!q.fast) return q.finite ? q.top / 127.0f : NAN;
+    constexpr float y = 1.0f / 127.0f;
+    const float r = q.top * y;
+    return fmaf(fmaf(r, -127.0f, q.top), y, r);
+}
+
+__host__ __device__ constexpr int qr_blocks(int per) { return per <= 4 ? 4 : 2; }  // an SM
 
 // L threads a row (8, 32 or the block), PER pieces of 16 bytes each.  Groups take rows in
 // turn and ask for the next one before they work on this one.  Bound by memory, and nearly
 // by issue slots (70 %): 1M x 768 float16 363 to 417 us, 5.5 to 6.3 TB/s (a group a row: 501).
 template <class T, int L, int PER>
-__global__ void __launch_bounds__(QR_NT, PER <= 4 ? 4 : 2) quantize_kernel(const QuantArgs g) {
+__global__ void __launch_bounds__(QR_NT, qr_blocks(PER)) quantize_kernel(const QuantArgs g) {
     constexpr int VEC = 16 / sizeof(T), GROUPS = QR_NT / L;
     __shared__ uint32_t s[QR_NT / 32];
     const int lane = threadIdx.x % L;
@@ -250,7 +283,7 @@ static int launch_quantize(QuantArgs g, cudaStream_t s) {
     auto kernel = eights ? of(std::integral_constant<int, 8>()) : warps ? of(std::integral_constant<int, 32>()) : of(std::integral_constant<int, QR_NT>());
     if (per > 4) kernel = per <= 6 ? &quantize_kernel<T, 32, 6> : &quantize_kernel<T, 32, 8>;
     const long long blocks = (g.rows + QR_NT / lanes - 1) / (QR_NT / lanes);
-    const long long most = (long long)(per <= 4 ? 4 : 2) * std::max(1, device_attr(cudaDevAttrMultiProcessorCount));
+    const long long most = (long long)qr_blocks(per) * std::max(1, device_attr(cudaDevAttrMultiProcessorCount));
     kernel<<<(unsigned)std::min(blocks, most), QR_NT, 0, s>>>(g);
     return check_launch("quantize_kernel");
 }

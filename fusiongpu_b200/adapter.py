@@ -561,7 +561,8 @@ class Muon(torch.optim.Optimizer):
         p = (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) orthogonalize(u)
 
     for matrices on the GPU; vectors go to another optimizer.  Matrices of one shape
-    and type are orthogonalised together."""
+    and type are orthogonalised together.  m is of the parameter's type, as torch's
+    optimizers keep their states."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  steps: int = 5, coefficients: tuple[float, float, float] = (3.4445, -4.7750, 2.0315), eps: float = 1e-7):

@@ -16,7 +16,7 @@ namespace fg {
 
 // ---- dz and dp, and their column sums ----------------------------------------------
 //
-// A group of L lanes takes L x VEC gates of every so many rows of its block's range and
+// A group of L lanes takes L x VEC gates of every so many rows and
 // sums its columns in registers; the block writes one partial row.  L is 32, or 16 or 8 for
 // layers as narrow as that (100,000 x 40 float16: 64 us with whole warps).  A lane's VEC gates lie beside each
 // other where the operand's halves start on 16 bytes, else L apart, so that a group's
@@ -30,7 +30,7 @@ struct GatedDz {
     const void *dy, *pre;
     void* dz;     // [rows][2 up] of operands, stride pack_stride(2 up); NULL: not stored
     float* part;  // NULL: no sums
-    long long lddy, ldp, rows, per, plane;
+    long long lddy, ldp, rows, plane;
     int up, act;
     int in_wide, out_wide;  // all rows and halves start on 16 bytes
 };
@@ -98,12 +98,12 @@ __global__ void __launch_bounds__(GD_WARPS * 32, 3) gated_dz_kernel(const GatedD
     __shared__ float s[GROUPS][L * VEC];
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
     const int step = g.out_wide ? 1 : L, j = blockIdx.x * L * VEC + lane * (g.out_wide ? VEC : 1), left = g.up - j;
-    const long long r0 = blockIdx.y * g.per, r1 = min(r0 + g.per, g.rows), ldz = pack_stride(2ll * g.up);
+    const long long ldz = pack_stride(2ll * g.up);
     float sum[2][VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum[0][i] = sum[1][i] = 0.0f;
     if (left > 0)
-        for (long long r = r0 + group; r < r1; r += GROUPS) {
+        for (long long r = (long long)blockIdx.y * GROUPS + group; r < g.rows; r += (long long)gridDim.y * GROUPS) {
             alignas(16) T d[VEC], z[VEC], p[VEC];
             const T* pre = static_cast<const T*>(g.pre) + r * g.ldp + j;
             gd_load<T, VEC>(d, static_cast<const T*>(g.dy) + r * g.lddy + j, left, g.in_wide, step);
@@ -195,7 +195,6 @@ static void launch_gated_dz_of(const GatedDz& g, int split, cudaStream_t s) {
 template <class T>
 static int launch_gated_dz(GatedDz g, int split, cudaStream_t s) {
     constexpr int VEC = 16 / (int)sizeof(T);
-    g.per = (g.rows + split - 1) / split;
     auto lies = [&](const void* p, long long ld) { return aligned(p, 16) && ld * (int)sizeof(T) % 16 == 0; };
     g.in_wide = lies(g.dy, g.lddy) && lies(g.pre, g.ldp) && g.up % VEC == 0;
     g.out_wide = g.up % VEC == 0;
@@ -295,7 +294,7 @@ static int gated_backward(const fg_linear_params& q, const Strides& t, const voi
     const long long plane = q.rows * pack_stride(q.out_dim);
     int rc;
     if (split && (dx || dw || dbias)) {
-        const GatedDz g{dy, pre, dx || dw ? ws.dz : nullptr, dbias ? ws.part : nullptr, t.y, t.p, q.rows, 0, plane, up, q.activation, 0, 0};
+        const GatedDz g{dy, pre, dx || dw ? ws.dz : nullptr, dbias ? ws.part : nullptr, t.y, t.p, q.rows, plane, up, q.activation, 0, 0};
         rc = q.dtype == FG_DTYPE_F32   ? launch_gated_dz<float>(g, split, s)
              : q.dtype == FG_DTYPE_F16 ? launch_gated_dz<__half>(g, split, s)
                                        : launch_gated_dz<__nv_bfloat16>(g, split, s);

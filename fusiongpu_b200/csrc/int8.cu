@@ -17,7 +17,7 @@ namespace fg {
 // A group of threads holds its row in registers, so that memory is read once: eight up
 // to 128 columns, a warp up to 2,048 (16 bits) or 1,024 (32), a block of 256 up to 8,192 or
 // 4,096; longer rows are read again from L2.
-constexpr int QR_NT = 256;
+constexpr int QR_NT = 256, QR_TURNS = 8;
 constexpr int QUANTIZE_DIM = 1 << 30;
 
 // Two values' magnitudes against the largest so far, as the type's bits: of two 16-bit
@@ -50,8 +50,7 @@ struct QuantRow {
 
 // 127 x / top rounded to nearest, ties to even, for a value near a half between codes: the
 // remainder 127 x - r top of the nearest candidate, as a sum of two floats without an
-// error, against top / 2.  (bfloat16 rows meet exact ties often: their largest value has
-// 8 bits.)
+// error, against top / 2.
 __device__ __forceinline__ float exact_code(float x, const QuantRow& q) {
     x *= q.up;
     const float top = q.top * q.up, half = 0.5f * top;
@@ -127,15 +126,15 @@ struct QuantArgs {
     signed char* q;
     float* scale;
     long long rows, ldx, ldq;
-    int dim, unit, wide;  // unit: bytes that x's rows start on, up to 16; wide: q's start on 8
+    int dim, turns, unit, wide;  // turns: rows of a group; unit: bytes that x's rows start on, up to 16; wide: q's start on 8
 };
 
 // VEC neighbouring columns, `unit` bytes at a time: what the rows' starts allow.
 template <class T, int VEC>
-__device__ __forceinline__ void qr_load(T (&v)[VEC], const T* p, int left, int unit) {
+__device__ __forceinline__ void qr_load(T (&v)[VEC], const T* p, int left, int unit, bool whole = false) {
     if (left <= 0) {  // behind the row's end
         *reinterpret_cast<uint4*>(v) = make_uint4(0, 0, 0, 0);
-    } else if (unit == 16 && left >= VEC) {
+    } else if (whole || (unit == 16 && left >= VEC)) {
         *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
     } else if (unit >= 8 && left >= VEC) {
         reinterpret_cast<uint2*>(v)[0] = reinterpret_cast<const uint2*>(p)[0];
@@ -150,11 +149,11 @@ __device__ __forceinline__ void qr_load(T (&v)[VEC], const T* p, int left, int u
 }
 
 template <class T, int VEC>
-__device__ __forceinline__ void qr_store(signed char* p, const T (&v)[VEC], const QuantRow& q, int left, int wide) {
+__device__ __forceinline__ void qr_store(signed char* p, const T (&v)[VEC], const QuantRow& q, int left, int wide, bool whole = false) {
     if (left <= 0) return;
     uint32_t codes[VEC / 4];
     codes_of<T, VEC>(codes, v, q);
-    if (wide && left >= VEC) {
+    if (whole || (wide && left >= VEC)) {
         if constexpr (VEC == 8)
             *reinterpret_cast<uint2*>(p) = make_uint2(codes[0], codes[1]);
         else
@@ -203,28 +202,38 @@ __device__ __forceinline__ float scale_of(const QuantRow& q) {
 
 __host__ __device__ constexpr int qr_blocks(int per) { return per <= 4 ? 4 : 2; }  // an SM
 
-// L threads a row (8, 32 or the block), PER pieces of 16 bytes each.  Groups take rows in
-// turn and ask for the next one before they work on this one.  Bound by memory, and nearly
-// by issue slots (70 %): 1M x 768 float16 363 to 417 us, 5.5 to 6.3 TB/s (a group a row: 501).
-template <class T, int L, int PER>
+// L threads a row (8, 32 or the block), PER pieces of 16 bytes each.  A block takes as many
+// rows at a time as it has groups, QR_TURNS times or, of few rows, as one round of blocks
+// needs; a group asks for its next row before it works on this one.  Bound by memory, and
+// nearly by issue slots (70 %): 1M x 768 float16 342 us, 6.7 TB/s (a row a group: 501; 32 rows
+// a group 351, one round of blocks 390: they drift apart, and memory serves neighbours
+// best); 2M x 128 bfloat16 147 (202 with a remainder for its ties).  Narrow rows are bound by
+// issue slots: 3M x 40 float16 138.
+//
+// WHOLE: all pieces are loaded and stored whole.
+template <class T, int L, int PER, bool WHOLE>
 __global__ void __launch_bounds__(QR_NT, qr_blocks(PER)) quantize_kernel(const QuantArgs g) {
     constexpr int VEC = 16 / sizeof(T), GROUPS = QR_NT / L;
     __shared__ uint32_t s[QR_NT / 32];
     const int lane = threadIdx.x % L;
-    const long long step = (long long)gridDim.x * GROUPS;
+    const long long x_step = GROUPS * g.ldx, q_step = GROUPS * g.ldq;
+    long long first = (long long)blockIdx.x * g.turns * GROUPS, row = first + threadIdx.x / L;  // `first`: the block's, so that its threads stay together
+    const long long end = min(first + (long long)g.turns * GROUPS, g.rows);
+    const T* x = static_cast<const T*>(g.x) + row * g.ldx + lane * VEC;  // of the next row
+    signed char* out = g.q + row * g.ldq + lane * VEC;
     alignas(16) T next[PER][VEC];
-    auto fetch = [&](long long r) {
-        const T* x = static_cast<const T*>(g.x) + min(r, g.rows - 1) * g.ldx;  // a group past the last row takes it again
+    auto fetch = [&](bool here) {
 #pragma unroll
-        for (int k = 0; k < PER; ++k) qr_load<T, VEC>(next[k], x + (k * L + lane) * VEC, g.dim - (k * L + lane) * VEC, g.unit);
+        for (int k = 0; k < PER; ++k)
+            qr_load<T, VEC>(next[k], x + k * L * VEC, here ? g.dim - (k * L + lane) * VEC : 0, WHOLE ? 16 : g.unit, WHOLE);
+        x += x_step;
     };
-    long long first = (long long)blockIdx.x * GROUPS, row = first + threadIdx.x / L;  // `first`: the block's, so that its threads stay together
-    fetch(row);
-    for (; first < g.rows; first += step, row += step) {
+    fetch(row < g.rows);
+    for (; first < end; first += GROUPS, row += GROUPS, out += q_step) {
         alignas(16) T v[PER][VEC];
 #pragma unroll
         for (int k = 0; k < PER; ++k) *reinterpret_cast<uint4*>(v[k]) = *reinterpret_cast<const uint4*>(next[k]);
-        if (first + step < g.rows) fetch(row + step);
+        if (first + GROUPS < end) fetch(row + GROUPS < g.rows);
         uint32_t top = 0;
 #pragma unroll
         for (int k = 0; k < PER; ++k)
@@ -234,7 +243,7 @@ __global__ void __launch_bounds__(QR_NT, qr_blocks(PER)) quantize_kernel(const Q
         if (row >= g.rows) continue;
         if (lane == 0) g.scale[row] = scale_of(q);
 #pragma unroll
-        for (int k = 0; k < PER; ++k) qr_store<T, VEC>(g.q + row * g.ldq + (k * L + lane) * VEC, v[k], q, g.dim - (k * L + lane) * VEC, g.wide);
+        for (int k = 0; k < PER; ++k) qr_store<T, VEC>(out + k * L * VEC, v[k], q, g.dim - (k * L + lane) * VEC, WHOLE ? 1 : g.wide, WHOLE);
     }
 }
 
@@ -276,15 +285,21 @@ static int launch_quantize(QuantArgs g, cudaStream_t s) {
     }
     const bool eights = pieces <= 8 * (sizeof(T) == 2 ? 2 : 4);
     const int lanes = eights ? 8 : warps ? 32 : QR_NT, per = (int)((pieces + lanes - 1) / lanes);
-    auto of = [&](auto l) {
+    auto of = [&](auto l, auto whole) {
         constexpr int L = decltype(l)::value;
-        return per <= 1 ? &quantize_kernel<T, L, 1> : per <= 2 ? &quantize_kernel<T, L, 2> : per <= 3 ? &quantize_kernel<T, L, 3> : &quantize_kernel<T, L, 4>;
+        constexpr bool W = decltype(whole)::value;
+        return per <= 1 ? &quantize_kernel<T, L, 1, W> : per <= 2 ? &quantize_kernel<T, L, 2, W> : per <= 3 ? &quantize_kernel<T, L, 3, W> : &quantize_kernel<T, L, 4, W>;
     };
-    auto kernel = eights ? of(std::integral_constant<int, 8>()) : warps ? of(std::integral_constant<int, 32>()) : of(std::integral_constant<int, QR_NT>());
-    if (per > 4) kernel = per <= 6 ? &quantize_kernel<T, 32, 6> : &quantize_kernel<T, 32, 8>;
+    auto way = [&](auto whole) {
+        constexpr bool W = decltype(whole)::value;
+        if (per > 4) return per <= 6 ? &quantize_kernel<T, 32, 6, W> : &quantize_kernel<T, 32, 8, W>;
+        return eights ? of(std::integral_constant<int, 8>(), whole) : warps ? of(std::integral_constant<int, 32>(), whole) : of(std::integral_constant<int, QR_NT>(), whole);
+    };
+    auto kernel = g.unit == 16 && g.wide && g.dim % VEC == 0 ? way(std::true_type()) : way(std::false_type());
     const long long blocks = (g.rows + QR_NT / lanes - 1) / (QR_NT / lanes);
     const long long most = (long long)qr_blocks(per) * std::max(1, device_attr(cudaDevAttrMultiProcessorCount));
-    kernel<<<(unsigned)std::min(blocks, most), QR_NT, 0, s>>>(g);
+    g.turns = (int)std::min<long long>(QR_TURNS, (blocks + most - 1) / most);
+    kernel<<<(unsigned)((blocks + g.turns - 1) / g.turns), QR_NT, 0, s>>>(g);
     return check_launch("quantize_kernel");
 }
 
@@ -423,7 +438,7 @@ int fg_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t dim, in
         if (dim > QUANTIZE_DIM) return fail(FG_ERR_UNSUPPORTED, "dim above %d", QUANTIZE_DIM);
         if (rows == 0) return FG_OK;
         FG_REQUIRE(x && q && scale, "null buffer");
-        const QuantArgs g{x, reinterpret_cast<signed char*>(q), scale, rows, ldx, ldq, dim, 0, 0};
+        const QuantArgs g{x, reinterpret_cast<signed char*>(q), scale, rows, ldx, ldq, dim, 0, 0, 0};
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         return dtype == FG_DTYPE_F32   ? launch_quantize<float>(g, s)
                : dtype == FG_DTYPE_F16 ? launch_quantize<__half>(g, s)

@@ -139,6 +139,22 @@ def test_gated_backward(ad, shape, act, t):
     assert dx is None and torch.equal(dw, got[1]) and torch.equal(db, got[2])
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(30000, 24, 1), (20001, 16, 9), (30000, 40, 32), (12345, 33, 40), (9999, 17, 64), (20000, 24, 65),
+                                   (5001, 65, 128), (4000, 40, 129), (10000, 8, 333)])
+def test_gated_backward_narrow(ad, shape, t):
+    """Layers as narrow as a part of a warp, on rows that more than fill the GPU."""
+    n, i, o = shape
+    g = _gen(n + o)
+    x, w = _randn(g, n, i, t=t), _randn(g, 2 * o, i, t=t, scale=i ** -0.5)
+    dy, pre = _randn(g, n, o, t=t, scale=0.1), _randn(g, n, 2 * o, t=t, scale=1.5)
+    got = _check_gated_backward(ad, dy, x, w, pre, "silu", t)
+    wide = _randn(g, n, o + 11, t=t)  # the same from rows that start anywhere
+    wide[:, 3:3 + o] = dy
+    for u, v in zip(got, ad.gated_linear_backward(wide[:, 3:3 + o], x, w, pre, activation="silu")):
+        assert torch.equal(u, v)
+
+
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("n", [5, 200])
 def test_gated_backward_against_differences(ad, act, n):
@@ -260,6 +276,19 @@ def test_quantize_rows(ad, dim, t):
             rq, rs = _quantised(view)
             assert q.dtype == torch.int8 and torch.equal(q, rq) and torch.equal(s, rs)
             assert q.data_ptr() % 16 == 0 and (rows < 2 or q.stride(0) % 16 == 0)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,dim", [(100_001, 1), (60_000, 9), (50_001, 40), (40_000, 100), (20_001, 129), (20_000, 333),
+                                      (9_001, 600), (3_001, 1025), (2_501, 3001)])
+def test_quantize_more_rows_than_groups(ad, rows, dim, t):
+    x = _randn(_gen(rows), rows, dim, t=t)
+    x[rows // 2] = math.nan
+    q, s = ad.quantize_rows(x)
+    good = torch.arange(rows, device="cuda") != rows // 2
+    rq, rs = _quantised(x[good])
+    assert torch.equal(q[good], rq) and torch.equal(s[good], rs)
+    assert s[rows // 2].isnan() and not q[rows // 2].any()
 
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])

@@ -88,6 +88,12 @@ def test_orthogonalize(ad, shape, t):
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 5000), (5000, 3), (1, 32768), (32768, 2), (17, 4001), (9001, 130)])
+def test_orthogonalize_long_and_thin(ad, shape, t):
+    _check(ad, torch.randn(*shape, generator=_gen(shape[0]), device="cuda").to(T[t]), t)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
 @pytest.mark.parametrize("batch,m,n", [(2, 40, 24), (3, 100, 257), (8, 256, 128), (5, 128, 700), (4, 1024, 600),
                                        (30, 64, 1500), (29, 700, 120), (200, 30, 300)])
 def test_orthogonalize_batches(ad, batch, m, n, t):

@@ -16,14 +16,15 @@ namespace fg {
 
 // ---- dz and dp, and their column sums ----------------------------------------------
 //
-// A group of L lanes takes L x VEC gates of every so many rows and
-// sums its columns in registers; the block writes one partial row.  L is 32, or 16 or 8 for
-// layers as narrow as that (100,000 x 40 float16: 64 us with whole warps).  A lane's VEC gates lie beside each
+// A group of L lanes takes L x VEC gates of every so many rows and sums its columns in
+// registers; the block writes one partial row.  L is 32, or 16 or 8 for layers as narrow as
+// that (100,000 x 40 float16 19 us, 64 with whole warps).  A lane's VEC gates lie beside each
 // other where the operand's halves start on 16 bytes, else L apart, so that a group's
-// accesses of one element are in order (1,777 x 333 bfloat16: 14.1 us beside each other).  Both factors are products of
-// values of the layer's type, so 16-bit ones enter the products in two parts (split2)
-// whatever the activation.  Bound by the latency of its loads and by memory: 10,000 x 1024
-// bfloat16 30 us (143 MB, 4.8 TB/s), float16 28, float32 45 (55 with two blocks an SM).
+// accesses of one element are in order (1,777 x 333 bfloat16 6.8 us, 14.1 beside each
+// other).  Both factors are products of values of the layer's type, so 16-bit ones enter the
+// products in two parts (split2) whatever the activation.  Bound by the latency of its loads
+// and by memory: 10,000 x 1024 bfloat16 28 us (143 MB, 5.1 TB/s), float16 30, float32 46 (55
+// with two blocks an SM).
 constexpr int GD_WARPS = 8;
 
 struct GatedDz {

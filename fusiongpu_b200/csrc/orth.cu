@@ -22,28 +22,30 @@
 #include <type_traits>
 
 #include "adapter_common.cuh"
+#include "packed.cuh"
 #include "tc_common.cuh"
 
 namespace fg {
 
-constexpr int OT_M = 128, OT_K = 64, OT_NT = 64 + 256;
+constexpr int OT_M = 128, OT_K = 64;
 constexpr int LOW_SHIFT = 11;  // h + 2^-11 l
 constexpr int ORTH_RUN = 2;    // K blocks (128 k) that an accumulator sums
 
-__device__ __forceinline__ void planes_of(float v, __half& h, __half& l) {
-    h = __float2half_rn(v);
-    const float f = __half2float(h);
-    l = fabsf(f) <= 65504.0f ? __float2half_rn((v - f) * (float)(1 << LOW_SHIFT)) : __float2half_rn(0.0f);
-}
-// The same of two values; one conversion instruction for both.
-__device__ __forceinline__ void planes_of(float v0, float v1, __half2& h, __half2& l) {
-    h = __floats2half2_rn(v0, v1);
-    const float2 f = __half22float2(h);
+// Two values, on the instructions for two.  What is past float16's range becomes NaN.
+__device__ __forceinline__ uint64_t both(float c) { return pair2(c, c); }
+__device__ __forceinline__ void planes_of(uint64_t v, __half2& h, __half2& l) {
     constexpr float up = 1 << LOW_SHIFT;
-    l = __floats2half2_rn(fabsf(f.x) <= 65504.0f ? (v0 - f.x) * up : 0.0f, fabsf(f.y) <= 65504.0f ? (v1 - f.y) * up : 0.0f);
+    float a, b;
+    unpair2(v, a, b);
+    h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    unpair2(fma2(pair2(f.x, f.y), both(-up), mul2(v, both(up))), a, b);  // exact
+    l = __floats2half2_rn(a, b);
 }
-__device__ __forceinline__ float value_of(__half h, __half l) {
-    return fmaf(__half2float(l), 1.0f / (1 << LOW_SHIFT), __half2float(h));
+__device__ __forceinline__ void planes_of(float v0, float v1, __half2& h, __half2& l) { planes_of(pair2(v0, v1), h, l); }
+__device__ __forceinline__ uint64_t value_of(__half2 h, __half2 l) {
+    const float2 a = __half22float2(h), b = __half22float2(l);
+    return fma2(pair2(b.x, b.y), both(1.0f / (1 << LOW_SHIFT)), pair2(a.x, a.y));
 }
 
 // ---- |G|_F and the first X ----------------------------------------------------------
@@ -188,6 +190,9 @@ struct OrthRing {
     static constexpr int A = 2 * OT_M * OT_K * 2, B = 2 * BN * OT_K * 2, STAGE = A + B;
     static constexpr int N = BN == 128 ? 3 : DEEP ? 4 : 2;       // 2: two blocks to an SM
     static constexpr int COLS = 2 * BN;                          // of TMEM: h h', and the others
+    // warps that empty the accumulators; threads: a block with the SM to itself has eight more
+    // warps for its finish
+    static constexpr int WARPS = 8, NT = BN == 64 && DEEP ? 576 : 320;
 };
 
 __device__ __forceinline__ uint32_t orth_rank() {
@@ -211,10 +216,10 @@ __device__ __forceinline__ float4 orth_peer(uint32_t a, uint32_t rank) {
 }
 
 template <class T, int BN, bool SPLIT, bool DEEP>
-__global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
+__global__ void __launch_bounds__(OrthRing<BN, DEEP>::NT, BN == 64 && !DEEP ? 2 : 1)
     orth_product_kernel(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMap tq, const __grid_constant__ OrthArgs g) {
     using Ring = OrthRing<BN, DEEP>;
-    constexpr int LDP = BN + 4;  // partial row: 4 floats of padding keep 16-byte stores off each other's banks
+    constexpr int NT = Ring::NT, LDP = BN + 4;  // partial row: 4 floats of padding keep 16-byte stores off each other's banks
     extern __shared__ __align__(1024) unsigned char dsmem[];
     __shared__ __align__(8) uint64_t full[Ring::N], empty[Ring::N], acc_full, acc_empty;
     __shared__ uint32_t tmem_slot;
@@ -247,7 +252,7 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
             tc::mbar_init(&empty[i], 1);
         }
         tc::mbar_init(&acc_full, 1);
-        tc::mbar_init(&acc_empty, 8);
+        tc::mbar_init(&acc_empty, Ring::WARPS);
         tc::fence_mbar_init();
     }
     if (warp == 1) {
@@ -281,13 +286,13 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             int r, c;
-            if (!g.c || !place(i0 + u * OT_NT, r, c)) continue;
+            if (!g.c || !place(i0 + u * NT, r, c)) continue;
             const __half* p = g.c + 2 * b * c_plane + (m0 + r) * g.ldc + n0 + rank * slice + c;  // rows hold a multiple of 8 elements
             next_h[u] = *reinterpret_cast<const Wide*>(p);
             next_l[u] = *reinterpret_cast<const Wide*>(p + c_plane);
         }
     };
-    addends(tid);
+    if (warp > 0) addends(tid);  // the producer's behind its work: its fence waits for loads
 
     if (warp == 0) {
         if (tc::elect_one()) {  // ---- TMA producer
@@ -314,6 +319,8 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
             if (!ok)  // copies in flight land before the block ends
                 for (int j = i > Ring::N ? i - Ring::N : 0; j < i; ++j) tc::mbar_wait(&full[j % Ring::N], (j / Ring::N) & 1);
         }
+        __syncwarp();
+        addends(tid);
     } else if (warp == 1) {
         // ---- MMA issuer: the warp stays together, one elected lane issues
         bool ok = true;
@@ -351,8 +358,8 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
             }
             __syncwarp();
         }
-    } else {  // ---- epilogue warps: TMEM -> partial tile in shared memory
-        constexpr int COLUMNS = BN / 2, G = COLUMNS / 32;  // of a warp
+    } else if (warp < 2 + Ring::WARPS) {  // ---- epilogue warps: TMEM -> partial tile in shared memory
+        constexpr int COLUMNS = BN / (Ring::WARPS / 4), G = COLUMNS / 32;  // of a warp
         const int q4 = warp & 3, c0 = ((warp - 2) >> 2) * COLUMNS;
         float* row = part + (q4 * 32 + lane) * LDP;
         const uint32_t src = taddr + ((uint32_t)(q4 * 32) << 16) + (uint32_t)c0;
@@ -393,9 +400,9 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
 
     static_assert((OT_M * LDP + OT_M * BN) * 4 <= Ring::N * Ring::STAGE, "the tile, and for SYM its transposed copy, fit the ring");
     uint32_t* turned = reinterpret_cast<uint32_t*>(part + OT_M * LDP);  // SYM: the slice transposed, h and l in one word,
-    auto turn = [](int c, int r) { return c * OT_M + ((r + c / W) & (OT_M - 1)); };  // turned on by W columns
+    auto turn = [](int c, int r) { return c * OT_M + ((r + c / W * 4) & (OT_M - 1)); };  // turned on by 4 rows every W columns
     const uint32_t pbase = tc::smem_u32(part);
-    for (int i0 = tid; i0 < OT_M << shift; i0 += U * OT_NT) {
+    for (int i0 = tid; i0 < OT_M << shift; i0 += U * NT) {
         int r[U], cc[U];
         bool in[U];
         alignas(16) float v[U][W];
@@ -404,13 +411,13 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
         for (int u = 0; u < U; ++u) {
             ch[u] = next_h[u];
             cl[u] = next_l[u];
-            in[u] = place(i0 + u * OT_NT, r[u], cc[u]);
+            in[u] = place(i0 + u * NT, r[u], cc[u]);
             if (!in[u]) continue;
             const float* own = part + r[u] * LDP + rank * slice + cc[u];
 #pragma unroll
             for (int j = 0; j < W; j += 4) *reinterpret_cast<float4*>(&v[u][j]) = *reinterpret_cast<const float4*>(own + j);
         }
-        addends(i0 + U * OT_NT);
+        addends(i0 + U * NT);
         if constexpr (SPLIT) {
             for (int s0 = 1; s0 < S; s0 += 3) {
                 float4 x[U][3];
@@ -436,18 +443,18 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
         for (int u = 0; u < U; ++u) {
             if (!in[u]) continue;
             const int row = m0 + r[u], col = n0 + rank * slice + cc[u];
+            uint64_t z[W / 2];
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[u][j] *= g.beta;
+            for (int j = 0; j < W / 2; ++j) z[j] = mul2(pair2(v[u][2 * j], v[u][2 * j + 1]), both(g.beta));
             if (g.c) {
 #pragma unroll
-                for (int j = 0; j < W; ++j)
-                    v[u][j] = fmaf(g.alpha, value_of(reinterpret_cast<const __half*>(&ch[u])[j], reinterpret_cast<const __half*>(&cl[u])[j]), v[u][j]);
+                for (int j = 0; j < W / 2; ++j)
+                    z[j] = fma2(both(g.alpha), value_of(reinterpret_cast<const __half2*>(&ch[u])[j], reinterpret_cast<const __half2*>(&cl[u])[j]), z[j]);
             }
             if (g.d) {
                 alignas(16) __half h[W], l[W];
 #pragma unroll
-                for (int j = 0; j < W; j += 2)
-                    planes_of(v[u][j], v[u][j + 1], *reinterpret_cast<__half2*>(h + j), *reinterpret_cast<__half2*>(l + j));
+                for (int j = 0; j < W; j += 2) planes_of(z[j / 2], *reinterpret_cast<__half2*>(h + j), *reinterpret_cast<__half2*>(l + j));
                 __half* p = g.d + 2 * b * d_plane + row * g.ldd + col;
                 if (!g.sym || col + W - 1 <= row) {  // elements past the last column lie in the row's padding
                     *reinterpret_cast<Wide*>(p) = *reinterpret_cast<const Wide*>(h);
@@ -468,6 +475,8 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
             } else {
                 T* p = static_cast<T*>(g.out) + ((long long)b * g.m + row) * g.n + col;
 #pragma unroll
+                for (int j = 0; j < W; j += 2) unpair2(z[j / 2], v[u][j], v[u][j + 1]);
+#pragma unroll
                 for (int k = 0; k < W; k += 4) {
                     if (g.vec && col + k < g.n) {
                         alignas(16) T o[4] = {from_f32<T>(v[u][k]), from_f32<T>(v[u][k + 1]), from_f32<T>(v[u][k + 2]), from_f32<T>(v[u][k + 3])};
@@ -484,23 +493,27 @@ __global__ void __launch_bounds__(OT_NT, BN == 64 && !DEEP ? 2 : 1)
             }
         }
     }
-    if (SPLIT) asm volatile("barrier.cluster.arrive.release;" ::: "memory");  // this block has read its peers' partial tiles
-    if (g.sym) {  // a lane takes two rows, which become neighbouring columns
+    if (SPLIT) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // this block has read its peers' partial tiles: nothing of its own to show them
+    if (g.sym) {  // a lane takes four rows, which become neighbouring columns; what is past the last one lies in the padding
         __syncthreads();
-        for (int i = tid; i < slice * (OT_M / 2); i += OT_NT) {
-            const int c = i / (OT_M / 2), r = i % (OT_M / 2) * 2, row = m0 + r, col = n0 + rank * slice + c;
-            if (col > row || row >= g.m) continue;  // of a pair on the diagonal the second one counts
-            const uint32_t x = turned[turn(c, r)], y = turned[turn(c, r + 1)];
+        for (int i = tid; i < slice * (OT_M / 4); i += NT) {
+            const int c = i / (OT_M / 4), r = i % (OT_M / 4) * 4, row = m0 + r, col = n0 + rank * slice + c;
+            if (col > row + 3 || col >= g.n || row >= g.m) continue;
+            const uint4 x = *reinterpret_cast<const uint4*>(turned + turn(c, r));
+            const uint2 h = make_uint2(__byte_perm(x.x, x.y, 0x5410), __byte_perm(x.z, x.w, 0x5410));
+            const uint2 l = make_uint2(__byte_perm(x.x, x.y, 0x7632), __byte_perm(x.z, x.w, 0x7632));
             __half* p = g.d + 2 * b * d_plane + col * g.ldd + row;
-            if (col < row && row + 1 < g.m) {
-                *reinterpret_cast<uint32_t*>(p) = __byte_perm(x, y, 0x5410);
-                *reinterpret_cast<uint32_t*>(p + d_plane) = __byte_perm(x, y, 0x7632);
-            } else if (col < row) {
-                p[0] = __ushort_as_half((unsigned short)x);
-                p[d_plane] = __ushort_as_half((unsigned short)(x >> 16));
-            } else if (row + 1 < g.m) {
-                p[1] = __ushort_as_half((unsigned short)y);
-                p[d_plane + 1] = __ushort_as_half((unsigned short)(y >> 16));
+            if (col <= row) {
+                *reinterpret_cast<uint2*>(p) = h;
+                *reinterpret_cast<uint2*>(p + d_plane) = l;
+            } else {  // on the diagonal
+                const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int j = 1; j < 4; ++j)
+                    if (row + j >= col) {
+                        p[j] = __ushort_as_half((unsigned short)v[j]);
+                        p[d_plane + j] = __ushort_as_half((unsigned short)(v[j] >> 16));
+                    }
             }
         }
     }
@@ -686,12 +699,13 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
     auto add = [&](float (&v)[32], float scale, float w, const unsigned char* from, uint32_t low, int row, int c) {
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
-            alignas(16) __half h[8], l[8];
+            alignas(16) __half2 h[4], l[4];
             const uint32_t at = os_at(row, c + j);
             *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(from + at);
             *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(from + low + at);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[j + k] = fmaf(v[j + k], scale, w * value_of(h[k], l[k]));
+            for (int k = 0; k < 8; k += 2)
+                unpair2(fma2(pair2(v[j + k], v[j + k + 1]), both(scale), mul2(both(w), value_of(h[k / 2], l[k / 2]))), v[j + k], v[j + k + 1]);
         }
     };
     auto put = [&](unsigned char* to, uint32_t low, const float (&v)[32], int row, int c) {
@@ -914,7 +928,7 @@ static int launch_product(const OrthProduct& o, cudaStream_t s) {
     FG_CUDA_TRY(ensure_smem(reinterpret_cast<const void*>(kernel), smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(o.ctas);
-    cfg.blockDim = dim3(OT_NT);
+    cfg.blockDim = dim3(OrthRing<BN, DEEP>::NT);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[2];

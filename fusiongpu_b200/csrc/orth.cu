@@ -852,13 +852,14 @@ static long long orth_tiles(long long m, long long n, int bn, bool sym) {
 }
 
 // The tile width and split that finish first by this estimate, in microseconds: a K block
-// takes 0.75 in tiles of 64 columns, of which two blocks share an SM, 0.4 in such tiles with
-// the SM and twice the stages to themselves, 0.7 in tiles of 128; what follows the products 3,
-// 3 and 3.7; and an exchange over the cluster, by what each CTA has left to finish, 1.8 of
-// two, and of four 0.5 where results go to two places (SYM), else 2.  Measured for 400 x 300
-// to 2048 x 2048, each product with each choice: within 1.5 us of the best one.  (Tiles of
-// 256 columns, whose accumulators fill TMEM, took 95 us where these take 77: 2048 x 1024 from
-// the right, four matrices.)
+// takes 0.75 in tiles of 64 columns, of which two blocks share an SM, 0.45 in such tiles with
+// the SM and twice the stages to themselves, 0.7 in tiles of 128; what follows the products 3
+// (4 with neighbours on their SMs), 2.5 and 3.7; and an exchange over the cluster, by what
+// each CTA has left to finish, 1.8 of two, and of four 0.5 where results go to two places
+// (SYM), else 2; with the SM to itself 0.2 and none, else 0.9 and 1.1.  Measured for 130 x 130
+// to four of 2048 x 1024, each product with each choice: within 1.6 us of the best one.
+// (Tiles of 256 columns, whose accumulators fill TMEM, took 95 us where these take 77: 2048 x
+// 1024 from the right, four matrices.)
 static OrthPlan orth_plan(long long m, long long n, long long k, int batch, bool sym) {
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount)), kb = (int)((k + OT_K - 1) / OT_K);
     OrthPlan best{128, 1, false};
@@ -869,8 +870,10 @@ static OrthPlan orth_plan(long long m, long long n, long long k, int batch, bool
             if (sp > kb) break;
             int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
             if (way.bn == 64 && !way.deep) slots *= 2;
-            const double each = (kb + sp - 1) / sp * (way.bn == 128 ? 0.7 : way.deep ? 0.4 : 0.75) + (way.bn == 128 ? 3.7 : 3.0) +
-                                (sp == 1 ? 0.0 : sp == 2 ? 1.8 : sp == 4 ? (sym ? 0.5 : 2.0) : 4.0);
+            const double exchange = sp == 1 ? 0.0 : sp == 8 ? 4.0 : way.deep ? (sp == 2 ? (sym ? 0.2 : 0.9) : sym ? 0.0 : 1.1)
+                                                                             : (sp == 2 ? 1.8 : sym ? 0.5 : 2.0);
+            const double each = (kb + sp - 1) / sp * (way.bn == 128 ? 0.7 : way.deep ? 0.45 : 0.75) +
+                                (way.bn == 128 ? 3.7 : way.deep ? 2.5 : tiles * sp > sms ? 4.0 : 3.0) + exchange;
             const double cost = (double)((tiles + slots - 1) / slots) * each;
             if (cost < least) {
                 least = cost;

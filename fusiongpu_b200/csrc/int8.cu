@@ -205,7 +205,7 @@ __host__ __device__ constexpr int qr_blocks(int per) { return per <= 4 ? 4 : 2; 
 // L threads a row (8, 32 or the block), PER pieces of 16 bytes each.  A block takes as many
 // rows at a time as it has groups, QR_TURNS times or, of few rows, as one round of blocks
 // needs; a group asks for its next row before it works on this one.  Bound by memory, and
-// nearly by issue slots (70 %): 1M x 768 float16 342 us, 6.7 TB/s (a row a group: 501; 32 rows
+// nearly by issue slots (66 %): 1M x 768 float16 342 us, 6.7 TB/s (a row a group: 501; 32 rows
 // a group 351, one round of blocks 390: they drift apart, and memory serves neighbours
 // best); 2M x 128 bfloat16 147 (202 with a remainder for its ties).  Narrow rows are bound by
 // issue slots: 3M x 40 float16 138.

@@ -270,8 +270,9 @@ __global__ void __launch_bounds__(OrthRing<BN, DEEP>::NT, BN == 64 && !DEEP ? 2 
 
     // The finishing pass: W columns a position, two positions a thread and round, their
     // addends a round ahead, the first one's before the products.  A cluster's exchange waits
-    // for distributed shared memory (a tile of 128 x 64, four CTAs: 2.2 us), of which a round
-    // asks for three peers at once; alone, 16-byte stores count.
+    // for distributed shared memory (a tile of 128 x 64, four CTAs, finished in 2 us), of which
+    // a round asks for three peers at once; alone, instructions count, and 16-byte stores (with
+    // 16 warps 1.1 us, with ten 1.5; four positions a thread are no faster).
     constexpr int W = SPLIT ? 4 : 8, U = 2;
     using Wide = typename std::conditional<W == 8, uint4, uint2>::type;
     const int slice = BN / S, shift = __ffs(slice / W) - 1;  // columns, and the logarithm of a row's positions

@@ -262,12 +262,13 @@ static int gated_forward(const fg_linear_params& q, const Strides& t, const void
     return tc_gated(q.dtype, a.p, a.plane, b.p, b.plane, GemmShape{q.rows, q.out_dim, q.in_dim, a.ld, 1, b.ld, 1}, e, s);
 }
 
-// dx = dz w and dw = dz^T x of both halves at once.
+// dx = dz w and dw = dz^T x of both halves at once, in as many parts as fill the GPU (dw of
+// 10,000 x 768 -> 1024, 24 tiles: three parts 47 us, two 64; float32 140 and 196).
 static GemmShape gated_dx(const fg_linear_params& q, long long ldw) {
-    return {q.rows, q.in_dim, q.out_dim, pack_stride(q.out_dim), 1, 1, ldw};
+    return {q.rows, q.in_dim, q.out_dim, pack_stride(q.out_dim), 1, 1, ldw, true};
 }
 static GemmShape gated_dw(const fg_linear_params& q, long long ldx) {
-    return {q.out_dim, q.in_dim, q.rows, 1, pack_stride(q.out_dim), 1, ldx};
+    return {q.out_dim, q.in_dim, q.rows, 1, pack_stride(q.out_dim), 1, ldx, true};
 }
 
 static size_t gated_backward_carve(const fg_linear_params& q, const Strides& t, void* ws, size_t bytes, GatedWs& w) {

@@ -18,6 +18,7 @@ struct Epilogue {
 struct GemmShape {
     long long m, n, k;
     long long am, ak, bn, bk;
+    bool any_parts = false;  // k may be split among pairs into 3, 5, ... parts as well as powers of two
 };
 
 // GELU = z Phi(z).  float32 results: CUDA's erfc.  Results of 16 bits (FAST): fits of our

@@ -1651,7 +1651,7 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct, int mode
         // 16-bit sums run over GT_RUN K blocks at most: parts go on past 32, and past a full
         // GPU, until they are that short (in 64 bits: kb may be 2^25)
         auto too_long = [&](int parts) { return products < 6 && kb > (long long)GT_RUN * parts; };
-        for (int sp = 1; sp <= 32 || too_long(sp / 2); sp *= 2) {
+        for (int sp = 1; sp <= 32 || too_long(sp / 2); sp = s.any_parts && sp < 32 ? sp + 1 : sp * 2) {
             if ((direct || mode != TC_WHOLE) && sp > 1) break;
             if (sp > 1 && (sp > kb / 2 || (tiles * sp > sms && kb <= (long long)GT_RUN * (sp / 2)))) break;
             if (too_long(sp)) continue;

@@ -155,6 +155,19 @@ def test_gated_backward_narrow(ad, shape, t):
         assert torch.equal(u, v)
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(10000, 768, 1024), (3000, 256, 256), (5000, 700, 450), (2500, 520, 300), (20000, 256, 640)])
+def test_gated_backward_in_parts(ad, shape, t):
+    """Sums over rows in three, five, ... parts, whichever fill the GPU."""
+    n, i, o = shape
+    g = _gen(n + i)
+    x, w = _randn(g, n, i, t=t), _randn(g, 2 * o, i, t=t, scale=i ** -0.5)
+    dy, pre = _randn(g, n, o, t=t, scale=0.1), _randn(g, n, 2 * o, t=t, scale=1.5)
+    got = _check_gated_backward(ad, dy, x, w, pre, "gelu", t)
+    for u, v in zip(got, ad.gated_linear_backward(dy, x, w, pre, activation="gelu")):
+        assert torch.equal(u, v)
+
+
 @pytest.mark.parametrize("act", ["gelu", "silu"])
 @pytest.mark.parametrize("n", [5, 200])
 def test_gated_backward_against_differences(ad, act, n):

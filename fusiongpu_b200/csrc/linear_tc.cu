@@ -1525,6 +1525,8 @@ static int launch_split(int dtype, const void* a, const void* b, const GemmShape
     if (rc) return rc;
     g.idesc = I8 ? instr_desc_i8(GT_M, BN) : instr_desc(dtype, GT_M, BN, g.a_mn, g.b_mn);
     g.nt = (g.n + BO - 1) / BO;
+    if (sizeof(T) == 4 && !I8)  // the plan's: each run of GP_CHUNK K blocks has its accumulator
+        FG_REQUIRE((g.kt + g.split - 1) / g.split <= GP_CHUNK * (512 / BN), "%d K blocks: too many for a tile's accumulators", g.kt);
     const long long ctas = (long long)g.mt * g.nt * g.split;
     FG_REQUIRE(ctas <= 0x7fffffffll, "%d x %d outputs: too many tiles", g.m, g.n);
     auto kernel = &gemm_split_kernel<T, BN, MODE>;
@@ -1669,6 +1671,9 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct, int mode
             // the sums' length: 512 k for each of float32's 512 / bn accumulators
             if (kb > (products < 6 ? GT_RUN : GP_CHUNK * 512 / bn) * sp && kb > 3) continue;
             const int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
+            // a second wave of clusters costs more than this estimate: gated 20,000 x 768 -> 100
+            // float32 in fours 105 us, in pairs 77 (plain layers keep the order of their sums)
+            if (mode != TC_WHOLE && sp > 1 && tiles > slots) break;
             const double main = (kt + sp - 1) / sp * (bn == 256 ? 0.43 : bn == 128 ? 0.30 : 0.21);
             const double rows = direct ? 0.055 * bn : 0.0;
             offer(5.0 + waves(tiles, slots) * (main + 2.0 + 0.02 * bn / sp + rows) + (sp == 8 ? 0.7 : 0.0), TcPlan{false, bn, sp, 0});

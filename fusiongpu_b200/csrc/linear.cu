@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(256) gemm_simt_kernel(const T* a, long long a_
             if (m0 + ra < g.m && k0 + ka < g.k) {
                 const T* p = a + (m0 + ra) * g.am + (k0 + ka) * g.ak;
                 v = to_f32(p[0]);
-                if (a_plane) v = PartsOf<T>::hi * v + PartsOf<T>::lo * to_f32(p[a_plane]);
+                if (a_plane) v = of_parts<T>(p[0], p[a_plane]);
             }
             sa[ka][ra] = v;
             sb[kb][rb] = (n0 + rb < g.n && k0 + kb < g.k) ? to_f32(b[(n0 + rb) * g.bn + (k0 + kb) * g.bk]) : 0.0f;

@@ -153,7 +153,13 @@ __device__ __forceinline__ void gated_store(const Epilogue& e, int up, long long
 // bits of the significand.  f16: v = 2 (p0 + 2^-12 p1), to 22 bits, or 2^-36 where that is
 // more: a gradient may lie below f16's 2^-24 and up to 1.13 times its largest value.  An
 // infinity or NaN has 0 behind it.
+//
+// A gated layer's dz = dy p act'(z) may pass that range as well, up to 2^32.2.  Such an f16
+// value is a NaN, whose payload and lower part hold its bits from F16_FAR on, rounded to
+// 2^-21 of it; the results that it enters come out as NaN and are taken again one product
+// at a time, from of_parts.
 constexpr int F16_PART_SHIFT = 12;
+constexpr uint32_t F16_FAR = 0x47800000u;  // 2^16
 template <class T>
 struct PartsOf {  // v = hi p0 + lo p1
     static constexpr float hi = 1.0f, lo = 1.0f;
@@ -171,8 +177,29 @@ __device__ __forceinline__ void split2(float v, __nv_bfloat16& p0, __nv_bfloat16
 __device__ __forceinline__ void split2(float v, __half& p0, __half& p1) {
     const float h = v * 0.5f;
     p0 = from_f32<__half>(h);
+    if (fabsf(v) <= FLT_MAX && fabsf(to_f32(p0)) > 65504.0f) {
+        const uint32_t u = ((__float_as_uint(v) & 0x7fffffffu) - F16_FAR + 4) >> 3;  // below 2^25 - 2^16, a plain NaN's
+        p0 = __ushort_as_half((unsigned short)(0x7e00u | (u >> 16) | (v < 0.0f ? 0x8000u : 0u)));
+        p1 = __ushort_as_half((unsigned short)u);
+        return;
+    }
     const float r = (h - to_f32(p0)) * (float)(1 << F16_PART_SHIFT);
     p1 = from_f32<__half>(fabsf(v) <= FLT_MAX ? fminf(fmaxf(r, -65504.0f), 65504.0f) : 0.0f);
+}
+
+// What the parts stand for.
+template <class T>
+__device__ __forceinline__ float of_parts(T p0, T p1) {
+    return PartsOf<T>::hi * to_f32(p0) + PartsOf<T>::lo * to_f32(p1);
+}
+template <>
+__device__ __forceinline__ float of_parts<__half>(__half p0, __half p1) {
+    const uint32_t b = __half_as_ushort(p0);
+    if ((b & 0x7e00u) == 0x7e00u && (b & 0x7fffu) != 0x7fffu) {
+        const float v = __uint_as_float(F16_FAR + (((b & 0x1ffu) << 16 | __half_as_ushort(p1)) << 3));
+        return b & 0x8000u ? -v : v;
+    }
+    return PartsOf<__half>::hi * to_f32(p0) + PartsOf<__half>::lo * to_f32(p1);
 }
 
 // The same of two values at once, which are ordinary ones: neither cut nor past the range.

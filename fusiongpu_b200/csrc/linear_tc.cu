@@ -63,8 +63,8 @@ __device__ __forceinline__ int plane_a(int i, int products) {  // 0; 1 0; 0 2 1 
 }
 __device__ __forceinline__ int plane_b(int i, int products) { return products < 6 ? 0 : (82 >> (2 * i)) & 3; }  // 2 0 1 1 0 0
 
-// An infinite operand times the small planes of the other has any sign: a result
-// that is not finite is taken again, one product at a time.
+// An infinite operand times the small planes of the other has any sign, and an f16 part past
+// its range is a NaN: a result that is not finite is taken again, one product at a time.
 template <class T>
 __device__ __noinline__ float retake(const TcArgs& g, int m, int n) {
     using E = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;  // of a plane
@@ -76,7 +76,7 @@ __device__ __noinline__ float retake(const TcArgs& g, int m, int n) {
         if constexpr (sizeof(T) == 4)
             z = fmaf(whole(a, g.a_plane), whole(b, g.b_plane), z);
         else
-            z = fmaf(PartsOf<T>::hi * to_f32(a[0]) + PartsOf<T>::lo * to_f32(a[g.a_plane]), to_f32(b[0]), z);
+            z = fmaf(of_parts<T>(a[0], a[g.a_plane]), to_f32(b[0]), z);
     }
     return z;
 }

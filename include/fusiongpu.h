@@ -542,7 +542,8 @@ int fg_gated_linear(const fg_linear_params* params, const void* x, const void* w
 /* Its gradients: dz = dy p activation'(z), dp = dy activation(z), dx [rows][in_dim]
  * = [dz dp] w, dw [2 out_dim][in_dim] = [dz dp]^T x, dbias [2 out_dim] = their sums
  * over the rows, contiguous and of dtype; any may be NULL.  y_stride is dy's.  dz
- * and dp of F16 and BF16 enter the products as the linear layer's GELU does. */
+ * and dp of F16 and BF16 enter the products as the linear layer's GELU does; those of
+ * F16 that pass its range (up to 2^32.2) with 2^-21 of themselves. */
 int fg_gated_linear_backward_workspace_size(const fg_linear_params* params, size_t* bytes);
 int fg_gated_linear_backward(const fg_linear_params* params, const void* dy, const void* x, const void* w, const void* pre,
                              void* dx, void* dw, void* dbias, void* workspace, size_t workspace_bytes, void* stream);

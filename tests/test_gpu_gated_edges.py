@@ -1,0 +1,119 @@
+"""GPU tests of the gated adapter's operators at the ends of their ranges, against plain
+implementations in 64 bits.
+
+Tolerances are those of the operators' own tests: U[t] the unit roundoff of a result's
+type, E32 = 2^-24 that of 32-bit sums, (n + 8) * 2 * E32 of the magnitudes for a sum of n
+products, ACT for the activation functions.  A gradient of a pre-activation that passes
+float16's range enters the products with 2^-21 of it (20 bits behind the leading one,
+rounded), any other with PART of it.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+T = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TINY = {"f32": 2.0 ** -149, "f16": 2.0 ** -25, "bf16": 2.0 ** -134}
+ACT = {"f32": 2.0 ** -20, "f16": 2.0 ** -18, "bf16": 2.0 ** -18}
+PART = {"f32": 2.0 ** -23, "f16": 2.0 ** -21, "bf16": 2.0 ** -16}
+LOW = {"f32": 2.0 ** -130, "f16": 2.0 ** -36, "bf16": 2.0 ** -130}
+E32 = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ad():
+    from fusiongpu_b200 import adapter
+    return adapter
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(g, *shape, t="f32", scale=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(T[t])
+
+
+def _within(got, want, tol, t, what):
+    """A value past the type's range is infinite in it, as its rounding is."""
+    round_ = want.to(T[t]).double()
+    past = round_.isinf()
+    assert torch.equal(got.double()[past], round_[past]), what
+    bad = ~((got.double() - want).abs() <= tol) & ~past
+    assert not bad.any(), f"{what}: {int(bad.sum())} off, worst {float(((got.double() - want).abs() / tol)[bad].max()):.3g} x tolerance"
+
+
+def _backward(dy, x, w, pre, act):
+    """The gradients and what their operands' and sums' errors make of them at most, but
+    for the results' rounding."""
+    h = dy.shape[1]
+    d, z, p = dy.double(), pre[:, :h].double(), pre[:, h:].double()
+    s = torch.sigmoid(z)
+    f, a = {"none": lambda: (torch.ones_like(z), z), "silu": lambda: (s * (1 + z * (1 - s)), z * s),
+            "gelu": lambda: (torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi), z * torch.special.ndtr(z))}[act]()
+    return torch.cat([d * p * f, d * a], 1), torch.cat([(d * p).abs(), d.abs() * z.abs().clamp(min=1)], 1)
+
+
+def _check_backward(ad, dy, x, w, pre, act, t):
+    dx, dw, db = ad.gated_linear_backward(dy, x, w, pre, activation=act)
+    dz, mag = _backward(dy, x, w, pre, act)
+    edz = (ACT[t] * mag if act != "none" else 0) + 4 * E32 * dz.abs()
+    part = edz + PART[t] * dz.abs() + LOW[t]
+    n, k = dz.shape
+    rdx, rdw, rdb = dz @ w.double(), dz.t() @ x.double(), dz.sum(0)
+    _within(dx, rdx, part @ w.double().abs() + (k + 8) * 2 * E32 * (dz.abs() @ w.double().abs()) + U[t] * rdx.abs() + TINY[t], t, "dx")
+    _within(dw, rdw, part.t() @ x.double().abs() + (n + 8) * 2 * E32 * (dz.abs().t() @ x.double().abs()) + U[t] * rdw.abs()
+            + TINY[t], t, "dw")
+    _within(db, rdb, edz.sum(0) + (n + 8) * 2 * E32 * dz.abs().sum(0) + U[t] * rdb.abs() + TINY[t], t, "dbias")
+    return dx, dw, db
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("act", ["none", "silu", "gelu"])
+@pytest.mark.parametrize("n,i,o", [(2, 40, 24), (8, 64, 900), (40, 72, 48), (300, 64, 130), (3000, 264, 333), (20000, 128, 256)])
+def test_gated_backward_past_the_range_of_its_type(ad, n, i, o, t, act):
+    """dz = dy p act'(z) and dp = dy act(z) of values that float16 holds may lie past its
+    range while the gradients do not."""
+    g = _gen(n + o)
+    x, w = _randn(g, n, i, t=t, scale=2.0 ** -8), _randn(g, 2 * o, i, t=t, scale=2.0 ** -9)
+    dy, pre = _randn(g, n, o, t=t, scale=0.1), _randn(g, n, 2 * o, t=t, scale=1.5)
+    rows = torch.randint(0, n, (6,), generator=g, device="cuda")
+    cols = torch.randint(0, o, (6,), generator=g, device="cuda")
+    dy[rows, cols] = torch.tensor([3000, -3000, 50000, 1312, -400, 1310], device="cuda").to(T[t])
+    pre[rows, cols] = torch.tensor([2, 1.5, 300, 30, 1000, 100], device="cuda").to(T[t])
+    pre[rows, o + cols] = torch.tensor([100, 200, -80, 100, 1000, -100], device="cuda").to(T[t])
+    _check_backward(ad, dy, x, w, pre, act, t)  # the largest, of 50000 * 300 * 2^-9 and more, may round to an infinity
+
+
+@pytest.mark.parametrize("n", [5, 60, 5000])
+def test_gated_backward_of_the_largest_values(ad, n):
+    """float16's largest dy and p: dz of 2^32."""
+    top = 65504.0
+    x = torch.zeros(n, 40, device="cuda", dtype=torch.float16)
+    w = torch.zeros(64, 40, device="cuda", dtype=torch.float16)
+    dy, pre = torch.zeros(n, 32, device="cuda", dtype=torch.float16), torch.zeros(n, 64, device="cuda", dtype=torch.float16)
+    dy[n // 2, 3], pre[n // 2, 3], pre[n // 2, 35] = -top, top, top
+    x[n // 2, 7], w[3, 5], w[35, 6] = 2.0 ** -20, 2.0 ** -24, 3 * 2.0 ** -24
+    dx, dw, _ = _check_backward(ad, dy, x, w, pre, "silu", "f16")
+    assert abs(float(dx[n // 2, 5]) + top * top * 2.0 ** -24) <= 1 and abs(float(dx[n // 2, 6]) + 3 * top * top * 2.0 ** -24) <= 2
+    assert int((dx != 0).sum()) == 2 and int((dw != 0).sum()) == 2
+
+
+@pytest.mark.parametrize("n", [60, 5000])
+def test_gated_backward_keeps_infinities_and_nan(ad, n):
+    """A dy that is infinite or NaN, beside one whose dz passes the range."""
+    g = _gen(n)
+    x, w = _randn(g, n, 64, t="f16", scale=2.0 ** -8), _randn(g, 96, 64, t="f16", scale=2.0 ** -9)
+    dy, pre = _randn(g, n, 48, t="f16"), _randn(g, n, 96, t="f16")
+    pre[1, 48 + 4], dy[1, 4], pre[1, 4] = 1000, 1000, 3
+    clean = ad.gated_linear_backward(dy, x, w, pre, activation="none", param_grads=False)[0]
+    dy[2, 5], dy[3, 6] = math.nan, math.inf
+    dx = ad.gated_linear_backward(dy, x, w, pre, activation="none", param_grads=False)[0]
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[2:4] = False
+    assert dx[2].isnan().all() and torch.equal(dx[keep], clean[keep]) and clean.isfinite().all()
+    dz, _ = _backward(dy[3:4], x, w, pre[3:4], "none")
+    torch.testing.assert_close(dx[3].double(), dz[0, [6, 54]] @ w[[6, 54]].double(), rtol=0, atol=0, equal_nan=True)

@@ -117,3 +117,25 @@ def test_gated_backward_keeps_infinities_and_nan(ad, n):
     assert dx[2].isnan().all() and torch.equal(dx[keep], clean[keep]) and clean.isfinite().all()
     dz, _ = _backward(dy[3:4], x, w, pre[3:4], "none")
     torch.testing.assert_close(dx[3].double(), dz[0, [6, 54]] @ w[[6, 54]].double(), rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_muon_keeps_a_small_decay(ad, dtype, monkeypatch):
+    """The usual lr and a weight decay of 0.05 over a thousand steps without a gradient:
+    each factor off by half a step, eps / 2, where at least 4 eps (or the step's decay, if
+    that is eps or more) is taken at a time, and less than 4 eps held back."""
+    eps, d, n = torch.finfo(dtype).eps, 0.02 * 0.05, 1000
+    p = (torch.rand(50, 70, generator=_gen(3), device="cuda") + 0.5).to(dtype)
+    start = p.double()
+    p.grad = torch.zeros_like(p)
+    opt = ad.Muon([p], lr=0.02, weight_decay=0.05)
+    for _ in range(n):
+        opt.step()
+    want, due = n * math.log1p(-d), d if d >= eps else 4 * eps
+    assert float((torch.log(p.double() / start) - want).abs().max()) <= 1.02 * eps / 2 / due * abs(want) + 4 * eps + d
+    if d < eps:
+        while 1 - opt.state[p].get("decay", 1.0) + d >= 4 * eps:  # off the step that takes it
+            opt.step()
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()

@@ -133,6 +133,11 @@ def _orthogonalize_ws(batch: int, m: int, n: int, dtype: int, steps: int, device
                            C.byref(_lib.OrthogonalizeParams(batch, m, n, dtype, steps, 0, 0, 0, 0, 0, 0)))
 
 
+@functools.lru_cache(maxsize=1024)
+def _orthogonalize_check(m: int, n: int, dtype: int, steps: int, a: float, b: float, c: float, eps: float) -> None:
+    _lib.size_query("fg_orthogonalize_workspace_size", C.byref(_lib.OrthogonalizeParams(1, m, n, dtype, steps, a, b, c, eps, 0, 0)))
+
+
 def _off16(*pointers: int) -> int:
     """fg_linear_operand bits of the pointers (x, w, dy) that are off 16 bytes."""
     off = 0
@@ -571,14 +576,39 @@ class Muon(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  steps: int = 5, coefficients: tuple[float, float, float] = (3.4445, -4.7750, 2.0315), eps: float = 1e-7):
-        if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
-            raise ValueError("lr and weight_decay must not be negative, momentum must be in [0, 1)")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                                       coefficients=coefficients, eps=eps))
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        try:
+            self._check(self.param_groups[-1])
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check(group: dict) -> None:
+        """Refuses what a step could not finish."""
+        if not group["lr"] >= 0 or not 0 <= group["momentum"] < 1 or not group["weight_decay"] >= 0:
+            raise ValueError("lr and weight_decay must not be negative, momentum must be in [0, 1)")
+        for p in group["params"]:
+            if p.dim() != 2 or p.dtype not in DTYPES:
+                raise ValueError(f"Muon takes matrices of float32, float16 or bfloat16, not {tuple(p.shape)} {p.dtype}")
+            _orthogonalize_check(*p.shape, DTYPES[p.dtype], group["steps"], *group["coefficients"], group["eps"])
+
+    def _check_step(self) -> None:
+        """The same of the whole step, before anything moves."""
         for group in self.param_groups:
+            self._check(group)
+            d = group["lr"] * group["weight_decay"]
             for p in group["params"]:
-                if p.dim() != 2 or p.dtype not in DTYPES:
-                    raise ValueError(f"Muon takes matrices of float32, float16 or bfloat16, not {tuple(p.shape)} {p.dtype}")
+                if p.grad is None:
+                    continue
+                if not p.is_cuda or p.grad.layout != torch.strided:
+                    raise ValueError(f"Muon takes matrices on the GPU with dense gradients, not on {p.device} with {p.grad.layout}")
+                if 0 < d < torch.finfo(p.dtype).eps and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(f"a decay of {d:g} a step, which {p.dtype} does not resolve, cannot be captured into a CUDA graph")
 
     def _decay(self, p: torch.Tensor, d: float) -> None:
         """p = (1 - d) p, or held back.  A factor of 1 - d is off by half a step, eps / 2 of
@@ -587,10 +617,8 @@ class Muon(torch.optim.Optimizer):
         keep = state.pop("decay", 1.0) * (1 - d)
         if d >= eps or 1 - keep >= 4 * eps:
             p.mul_(keep)
-            return
-        if p.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError(f"a decay of {d:g} a step, which {p.dtype} does not resolve, cannot be captured into a CUDA graph")
-        state["decay"] = keep
+        else:
+            state["decay"] = keep
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -598,6 +626,7 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self._check_step()
         for group in self.param_groups:
             alike: dict = {}
             for p in group["params"]:

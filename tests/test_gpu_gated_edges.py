@@ -139,3 +139,16 @@ def test_muon_keeps_a_small_decay(ad, dtype, monkeypatch):
         monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
         with pytest.raises(RuntimeError, match="captured"):
             opt.step()
+
+
+def test_muon_refused_step_moves_nothing(ad):
+    """What one parameter is refused for is found before another one moves."""
+    here, there = torch.ones(4, 8, device="cuda"), torch.ones(4, 8)
+    here.grad, there.grad = torch.ones_like(here), torch.ones_like(there)
+    opt = ad.Muon([dict(params=[here]), dict(params=[there])], weight_decay=0.1)
+    with pytest.raises(ValueError, match="GPU"):
+        opt.step()
+    assert (here == 1).all() and not opt.state[here]
+    there.grad = None
+    opt.step()
+    assert (here != 1).all()

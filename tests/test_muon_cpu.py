@@ -44,3 +44,45 @@ def test_decay_held_back_is_saved_with_the_state():
     again = Muon([p])
     again.load_state_dict(opt.state_dict())
     assert again.state[p]["decay"] == opt.state[p]["decay"] == 1 - 1e-3
+
+
+def _matrix(*shape, **kw):
+    p = torch.nn.Parameter(torch.ones(*shape, **kw))
+    p.grad = torch.ones_like(p)
+    return p
+
+
+def test_added_groups_are_checked():
+    from fusiongpu_b200._lib import FgError
+    opt = Muon([_matrix(4, 8)])
+    for bad in (_matrix(8), _matrix(2, 3, 4), _matrix(4, 8, dtype=torch.float64)):
+        with pytest.raises(ValueError):
+            opt.add_param_group(dict(params=[bad]))
+        with pytest.raises(ValueError):
+            Muon([dict(params=[_matrix(4, 8)]), dict(params=[bad])])
+    for kw in (dict(lr=-1.0), dict(lr=math.nan), dict(momentum=1.0), dict(weight_decay=-0.1)):
+        with pytest.raises(ValueError):
+            opt.add_param_group(dict(params=[_matrix(4, 8)], **kw))
+        with pytest.raises(ValueError):
+            Muon([dict(params=[_matrix(4, 8)], **kw)])
+    for kw in (dict(steps=101), dict(eps=-1.0), dict(coefficients=(17.0, 0.0, 0.0))):
+        with pytest.raises(FgError):
+            opt.add_param_group(dict(params=[_matrix(4, 8)], **kw))
+    for shape in ((0, 8), (1, 32769)):
+        with pytest.raises(FgError):
+            opt.add_param_group(dict(params=[_matrix(*shape)]))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[_matrix(4, 8)], lr=0.1))
+    assert len(opt.param_groups) == 2 and opt.param_groups[1]["lr"] == 0.1
+
+
+def test_a_refused_step_moves_nothing():
+    """Parameters that are not on the GPU, and settings changed since."""
+    p = _matrix(4, 8)
+    opt = Muon([p], weight_decay=0.1)
+    with pytest.raises(ValueError, match="GPU"):
+        opt.step()
+    opt.param_groups[0]["momentum"] = 1.5
+    with pytest.raises(ValueError, match="momentum"):
+        opt.step()
+    assert (p == 1).all() and not opt.state[p]

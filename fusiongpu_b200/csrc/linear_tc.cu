@@ -91,41 +91,6 @@ struct RingOf {
     static constexpr int N = GT_RING / STAGE > 8 ? 8 : GT_RING / STAGE;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-
-// 16 bytes at shared address `a` of CTA `rank` of the cluster.
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t a, uint32_t rank) {
-    float4 v;
-    asm volatile(
-        "{\n\t.reg .b32 p;\n\t"
-        "mapa.shared::cluster.u32 p, %4, %5;\n\t"
-        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [p];\n\t}\n"
-        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-        : "r"(a), "r"(rank)
-        : "memory");
-    return v;
-}
-
-__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t a, uint32_t rank) {
-    uint32_t v;
-    asm volatile(
-        "{\n\t.reg .b32 p;\n\t"
-        "mapa.shared::cluster.u32 p, %1, %2;\n\t"
-        "ld.shared::cluster.u32 %0, [p];\n\t}\n"
-        : "=r"(v)
-        : "r"(a), "r"(rank)
-        : "memory");
-    return v;
-}
-
 // An integer sum, its bits in a float's place, times its column's and row's scales, and the bias.
 __device__ __forceinline__ float dequantised(float sum, float xs, float ws, float bias) {
     return fmaf((float)__float_as_int(sum) * ws, xs, bias);
@@ -202,7 +167,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
     unsigned char* ring = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
     float* part = reinterpret_cast<float*>(ring);
-    const int S = g.split, rank = S > 1 ? (int)cluster_rank() : 0;
+    const int S = g.split, rank = S > 1 ? (int)tc::cluster_rank() : 0;
     const int tile = (int)(blockIdx.x / (unsigned)S);
     const int m0 = tile / g.nt * GT_M, n0 = tile % g.nt * BO;
     const int kb0 = (int)((long long)g.kt * rank / S), kb1 = (int)((long long)g.kt * (rank + 1) / S);
@@ -326,7 +291,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
         tc::fence_before_sync();
     }
     __syncthreads();
-    if (S > 1) cluster_sync();
+    if (S > 1) tc::cluster_sync();
     if (warp == 1) {
         tc::fence_after_sync();
         tc::tmem_dealloc(taddr, NA * BN);
@@ -342,7 +307,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
     const Epilogue& e = g.e;
     bool lost = false;  // an integer sum has no NaN: the CTAs say that theirs never came
     if (MODE == TC_INT8)
-        for (int s = 0; s < S; ++s) lost |= (S > 1 ? ld_cluster_u32(tc::smem_u32(&s_lost), s) : (uint32_t)s_lost) != 0;
+        for (int s = 0; s < S; ++s) lost |= (S > 1 ? tc::ld_cluster_u32(tc::smem_u32(&s_lost), s) : (uint32_t)s_lost) != 0;
     for (int i0 = tid; i0 < GT_M * per_row; i0 += U * GT_NT) {
         int row[U], col[U];
         uint32_t at[U];
@@ -383,9 +348,9 @@ __global__ void __launch_bounds__(GT_NT, 1)
         }
         auto sums = [&](uint32_t a) {
             if (S == 1) return *reinterpret_cast<const float4*>(reinterpret_cast<const char*>(part) + a);
-            float4 z = ld_cluster_f4(pbase + a, rank);
+            float4 z = tc::ld_cluster_f4(pbase + a, rank);
             for (int s = 1; s < S; ++s) {
-                const float4 v = ld_cluster_f4(pbase + a, (rank + s) & (S - 1));
+                const float4 v = tc::ld_cluster_f4(pbase + a, (rank + s) & (S - 1));
                 if (MODE == TC_INT8) {
                     z = make_float4(__int_as_float(__float_as_int(z.x) + __float_as_int(v.x)),
                                     __int_as_float(__float_as_int(z.y) + __float_as_int(v.y)),
@@ -461,7 +426,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
             put(e.y, row[u] * e.ldy + col[u], y);
         }
     }
-    if (S > 1) cluster_sync();  // a peer may still read this CTA's partial tile
+    if (S > 1) tc::cluster_sync();  // a peer may still read this CTA's partial tile
 }
 
 // ---- many tiles: persistent CTA pairs -----------------------------------------------
@@ -692,7 +657,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     __shared__ uint32_t tmem_slot;
     __shared__ int s_fail, s_odd;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rank = (int)cluster_rank();
+    const int rank = (int)tc::cluster_rank();
     unsigned char *ring = dsmem, *bufs = ring + GP_STAGES * P::STAGE, *biases = bufs + GP_EPI * P::BUF;
     const int pairs = (int)(gridDim.x >> 1), items = g.mt * g.nt * g.split;
     auto k_begin = [&](int part) { return (int)((long long)g.kt * part / g.split); };
@@ -726,7 +691,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     if (warp == 1) tc::tmem_alloc_pair(&tmem_slot, 2 * BN);
     tc::fence_before_sync();
     __syncthreads();
-    cluster_sync();  // the peer's barriers are ready too
+    tc::cluster_sync();  // the peer's barriers are ready too
     tc::fence_after_sync();
     const uint32_t taddr = tmem_slot;
     volatile int* fail = &s_fail;
@@ -1415,7 +1380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
     }
     tc::fence_before_sync();
     __syncthreads();
-    cluster_sync();  // no CTA leaves while its peer still reads its memory
+    tc::cluster_sync();  // no CTA leaves while its peer still reads its memory
     tc::fence_after_sync();
     if (warp == 1) tc::tmem_dealloc_pair(taddr, 2 * BN);
     // Results that are not finite lie in this CTA's tiles as NaN, and are taken again here,

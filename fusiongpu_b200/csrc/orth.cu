@@ -195,26 +195,6 @@ struct OrthRing {
     static constexpr int WARPS = 8, NT = BN == 64 && DEEP ? 576 : 320;
 };
 
-__device__ __forceinline__ uint32_t orth_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void orth_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ float4 orth_peer(uint32_t a, uint32_t rank) {
-    float4 v;
-    asm volatile(
-        "{\n\t.reg .b32 p;\n\t"
-        "mapa.shared::cluster.u32 p, %4, %5;\n\t"
-        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [p];\n\t}\n"
-        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-        : "r"(a), "r"(rank)
-        : "memory");
-    return v;
-}
-
 template <class T, int BN, bool SPLIT, bool DEEP>
 __global__ void __launch_bounds__(OrthRing<BN, DEEP>::NT, BN == 64 && !DEEP ? 2 : 1)
     orth_product_kernel(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMap tq, const __grid_constant__ OrthArgs g) {
@@ -228,7 +208,7 @@ __global__ void __launch_bounds__(OrthRing<BN, DEEP>::NT, BN == 64 && !DEEP ? 2 
     unsigned char* ring = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
     float* part = reinterpret_cast<float*>(ring);
-    const int S = SPLIT ? g.split : 1, rank = SPLIT ? (int)orth_rank() : 0;
+    const int S = SPLIT ? g.split : 1, rank = SPLIT ? (int)tc::cluster_rank() : 0;
     const int tile = (int)(blockIdx.x / (unsigned)S), b = tile / g.tiles;
     int t = tile - b * g.tiles, mi = 0;
     if (g.sym) {  // row tiles hold the column tiles up to the diagonal
@@ -393,7 +373,7 @@ __global__ void __launch_bounds__(OrthRing<BN, DEEP>::NT, BN == 64 && !DEEP ? 2 
         tc::fence_before_sync();
     }
     __syncthreads();
-    if (SPLIT) orth_cluster_sync();
+    if (SPLIT) tc::cluster_sync();
     if (warp == 1) {
         tc::fence_after_sync();
         tc::tmem_dealloc(taddr, Ring::COLS);
@@ -427,7 +407,7 @@ __global__ void __launch_bounds__(OrthRing<BN, DEEP>::NT, BN == 64 && !DEEP ? 2 
 #pragma unroll
                     for (int s = 0; s < 3; ++s)
                         if (in[u] && s0 + s < S)
-                            x[u][s] = orth_peer(pbase + (uint32_t)(r[u] * LDP + rank * slice + cc[u]) * 4, (rank + s0 + s) & (S - 1));
+                            x[u][s] = tc::ld_cluster_f4(pbase + (uint32_t)(r[u] * LDP + rank * slice + cc[u]) * 4, (rank + s0 + s) & (S - 1));
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -567,7 +547,7 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
     unsigned char* xs = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dsmem) + 1023) & ~static_cast<uintptr_t>(1023));
     unsigned char* ys = xs + 2 * OS_X;
     const bool tall = g.rows > g.cols;
-    const int S = g.split, rank = S > 1 ? (int)orth_rank() : 0, matrix = (int)(blockIdx.x / (unsigned)S);
+    const int S = g.split, rank = S > 1 ? (int)tc::cluster_rank() : 0, matrix = (int)(blockIdx.x / (unsigned)S);
     const int side = tall ? g.cols : g.rows, whole = tall ? g.rows : g.cols, chunks_of_all = (whole + 63) / 64;
     const int chunk0 = chunks_of_all * rank / S, f0 = chunk0 * 64;  // this block's part of the longer side
     const int sc = (side + 63) / 64, fc = chunks_of_all * (rank + 1) / S - chunk0, far = min(whole - f0, fc * 64);
@@ -628,7 +608,7 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
     for (int w = 0; w < OS_NT / 32; ++w) sum += s_sum[w];
     if (S > 1) {
         if (tid == 0) g.sums[matrix * S + rank] = sum;
-        orth_cluster_sync();
+        tc::cluster_sync();
         sum = 0.0;
         for (int r = 0; r < S; ++r) sum += __ldcg(g.sums + matrix * S + r);
     }
@@ -761,7 +741,7 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
             }
         }
         if (S > 1) {
-            orth_cluster_sync();
+            tc::cluster_sync();
             // eight pieces of four columns a thread at most, all asked for at once
             const int pieces = sc * 16 * OS_SIDE, per = pieces / S, loads = (per + OS_NT - 1) / OS_NT * S;
             float4 p[OS_MOST];
@@ -781,7 +761,7 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
                 *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(h);
                 *reinterpret_cast<uint2*>(at + OS_Y) = *reinterpret_cast<const uint2*>(l);
             }
-            orth_cluster_sync();
+            tc::cluster_sync();
             if (tid == 0) {
                 asm volatile("fence.proxy.async.global;" ::: "memory");  // written by ordinary stores
                 tc::mbar_arrive_expect_tx(&copied, 2 * sc * OS_CHUNK);

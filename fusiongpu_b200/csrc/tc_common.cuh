@@ -123,6 +123,43 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
+// ---- clusters ---------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// 16 bytes at shared address `a` of CTA `rank` of the cluster.
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t a, uint32_t rank) {
+    float4 v;
+    asm volatile(
+        "{\n\t.reg .b32 p;\n\t"
+        "mapa.shared::cluster.u32 p, %4, %5;\n\t"
+        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [p];\n\t}\n"
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+        : "r"(a), "r"(rank)
+        : "memory");
+    return v;
+}
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t a, uint32_t rank) {
+    uint32_t v;
+    asm volatile(
+        "{\n\t.reg .b32 p;\n\t"
+        "mapa.shared::cluster.u32 p, %1, %2;\n\t"
+        "ld.shared::cluster.u32 %0, [p];\n\t}\n"
+        : "=r"(v)
+        : "r"(a), "r"(rank)
+        : "memory");
+    return v;
+}
+
 // ---- CTA pairs (cta_group::2): one MMA over both CTAs' shared and tensor memory ----
 
 // Shared-cluster address of a variable of the pair's leader (rank 0 of a cluster of 2).

@@ -273,6 +273,7 @@ __global__ void __launch_bounds__(OrthRing<BN, DEEP>::NT, BN == 64 && !DEEP ? 2 
             next_l[u] = *reinterpret_cast<const Wide*>(p + c_plane);
         }
     };
+    int lost = 0;
     if (warp > 0) addends(tid);  // the producer's behind its work: its fence waits for loads
 
     if (warp == 0) {
@@ -365,14 +366,18 @@ __global__ void __launch_bounds__(OrthRing<BN, DEEP>::NT, BN == 64 && !DEEP ? 2 
             float v[32];
             tc::tmem_ld_32x32(src + (uint32_t)(32 * c), v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = ok ? fmaf(v[j], 1.0f / (1 << LOW_SHIFT), sum[c][j]) : NAN;  // a wait that ran out
+            for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], 1.0f / (1 << LOW_SHIFT), sum[c][j]);
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
                 *reinterpret_cast<float4*>(row + c0 + 32 * c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         }
+        lost = !ok;
         tc::fence_before_sync();
     }
-    __syncthreads();
+    if (__syncthreads_or(lost)) {  // a wait that ran out leaves NaN, not a plausible number, once no copy is under way to the ring
+        for (int i = tid; i < OT_M * LDP; i += NT) part[i] = NAN;
+        __syncthreads();
+    }
     if (SPLIT) tc::cluster_sync();
     if (warp == 1) {
         tc::fence_after_sync();
@@ -631,6 +636,14 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
     const int q4 = warp & 3, part = warp >> 2;                         // lanes of TMEM, columns
     uint32_t phase = 0;
     bool ok = true;
+    // A wait that another warp's failure ended early is taken again by itself: neither products
+    // nor copies are left under way at the block's end, and what was waited for in vain is NaN.
+    auto landed = [&](uint64_t* bar, uint32_t parity) {
+        if (tc::mbar_wait_warp(bar, parity, fail)) return true;
+        tc::mbar_wait(bar, parity);
+        __syncwarp();
+        return false;
+    };
     // h h' of columns [0, n) and, 256 on, h l' + l h', over `chunks` of 64 k; with `two`, the
     // second half of the chunks into columns from 128 on
     auto multiply = [&](const unsigned char* p, uint32_t p_low, const unsigned char* q, uint32_t q_low, bool q_mn, int n, int chunks, bool two) {
@@ -656,7 +669,7 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
             }
             __syncwarp();
         }
-        ok = tc::mbar_wait_warp(&done, phase, fail) && ok;
+        ok = landed(&done, phase) && ok;
         phase ^= 1;
         tc::fence_after_sync();
     };
@@ -770,7 +783,7 @@ __global__ void __launch_bounds__(OS_NT, 1) orth_small_kernel(const OrthSmall g)
                     tc::bulk_load(ys + at, image + at, OS_CHUNK, &copied);
                 }
             }
-            ok = tc::mbar_wait_warp(&copied, step & 1, fail) && ok;
+            ok = landed(&copied, step & 1) && ok;
         }
         if (g.c != 0.0f) {
             multiply(ys, OS_Y, ys, OS_Y, false, sc * 64, sc, sc > 1);

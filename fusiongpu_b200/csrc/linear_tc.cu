@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
     tc::fence_after_sync();
     const uint32_t taddr = tmem_slot;
     volatile int* fail = &s_fail;
+    int gone = 0;
 
     if (warp == 0) {
         if (tc::elect_one()) {  // ---- TMA producer
@@ -269,6 +270,7 @@ __global__ void __launch_bounds__(GT_NT, 1)
     } else {  // ---- epilogue warps: TMEM -> partial tile in shared memory
         const int q4 = warp & 3, half = (warp - 2) >> 2;
         const bool ok = tc::mbar_wait_warp(&acc_full, 0, fail);
+        gone = !ok;
         if (MODE == TC_INT8 && !ok) s_lost = 1;
         tc::fence_after_sync();
         float* row = part + (q4 * 32 + lane) * LDP;
@@ -283,14 +285,14 @@ __global__ void __launch_bounds__(GT_NT, 1)
                 for (int j = 0; j < 32; ++j) v[j] += x[j];
             }
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)  // a wait that ran out leaves NaN, not a plausible number
-                *reinterpret_cast<float4*>(row + c + j) =
-                    ok ? make_float4(v[j], v[j + 1], v[j + 2], v[j + 3])
-                       : make_float4(NAN, NAN, NAN, NAN);
+            for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(row + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         }
         tc::fence_before_sync();
     }
-    __syncthreads();
+    if (__syncthreads_or(gone) && MODE != TC_INT8) {  // a wait that ran out leaves NaN, not a plausible number, once no copy is under way to the ring
+        for (int i = tid; i < GT_M * LDP; i += GT_NT) part[i] = NAN;
+        __syncthreads();
+    }
     if (S > 1) tc::cluster_sync();
     if (warp == 1) {
         tc::fence_after_sync();

@@ -7,8 +7,6 @@ which the producer has waited for its copies, or the loss is told by a flag."""
 import os
 import re
 
-import pytest
-
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fusiongpu_b200", "csrc")
 
 
@@ -24,10 +22,10 @@ def _kernel(file, name):
     raise AssertionError(name)
 
 
-def _products(file, name):
+def _products(file, name, word="lost"):
     k = _kernel(file, name)
-    told = k.index("lost = !ok")
-    barrier = k.index("__syncthreads_or(lost)", told)
+    told = k.index(word + " = !ok")
+    barrier = k.index(f"__syncthreads_or({word})", told)
     cluster = k.index("tc::cluster_sync()", barrier)
     filled = k.index("part[i] = NAN", barrier)
     assert told < barrier < filled < cluster
@@ -38,6 +36,12 @@ def _products(file, name):
 
 def test_orthogonalised_update():
     _products("orth.cu", "orth_product_kernel")
+
+
+def test_split_tiles_of_the_linear_and_gated_layers():
+    _products("linear_tc.cu", "gemm_split_kernel", "gone")
+    k = _kernel("linear_tc.cu", "gemm_split_kernel")  # integer sums have no NaN: a flag, which all of the cluster read
+    assert "if (MODE == TC_INT8 && !ok) s_lost = 1;" in k and "if (lost) z = make_float4(NAN, NAN, NAN, NAN);" in k
 
 
 def test_one_launch_update_ends_with_nothing_under_way():

@@ -1604,7 +1604,7 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct, int mode
     const int sms = std::max(2, device_attr(cudaDevAttrMultiProcessorCount));
     const int kt = (int)((s.k + GT_K - 1) / GT_K) * products;
     auto waves = [](long long tiles, int slots) { return (double)((tiles + slots - 1) / slots); };
-    TcPlan best{false, 256, 1, 0};
+    TcPlan best{false, 0, 1, 0};  // bn 0: none
     double least = 1e300;
     auto offer = [&](double cost, const TcPlan& p) {
         if (cost < least) {
@@ -1618,8 +1618,9 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct, int mode
         if ((products == 6 || mode == TC_GATED) && bn == 128) break;
         const long long tiles = m2 * ((s.n + bn - 1) / bn);
         // 16-bit sums run over GT_RUN K blocks at most: parts go on past 32, and past a full
-        // GPU, until they are that short (in 64 bits: kb may be 2^25)
-        auto too_long = [&](int parts) { return products < 6 && kb > (long long)GT_RUN * parts; };
+        // GPU, until they are that short (in 64 bits: kb may be 2^25).  Integer ones are exact at
+        // any length (4,096 x 65,552 -> 4,096 8 bits 1,127 us with pairs, 1,228 a CTA a tile).
+        auto too_long = [&](int parts) { return products < 6 && mode != TC_INT8 && kb > (long long)GT_RUN * parts; };
         for (int sp = 1; sp <= 32 || too_long(sp / 2); sp = s.any_parts && sp < 32 ? sp + 1 : sp * 2) {
             if ((direct || mode != TC_WHOLE) && sp > 1) break;
             if (sp > 1 && (sp > kb / 2 || (tiles * sp > sms && kb <= (long long)GT_RUN * (sp / 2)))) break;
@@ -1636,7 +1637,7 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct, int mode
         for (int sp : {1, 2, 4, 8}) {
             if (sp > kb || (direct && sp > 1)) break;
             // the sums' length: 512 k for each of float32's 512 / bn accumulators
-            if (kb > (products < 6 ? GT_RUN : GP_CHUNK * 512 / bn) * sp && kb > 3) continue;
+            if (mode != TC_INT8 && kb > (products < 6 ? GT_RUN : GP_CHUNK * 512 / bn) * sp && kb > 3) continue;
             const int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
             // a second wave of clusters costs more than this estimate: gated 20,000 x 768 -> 100
             // float32 in fours 105 us, in pairs 77 (plain layers keep the order of their sums)
@@ -1677,6 +1678,10 @@ static TcArgs tc_args(const void* a, long long a_plane, const void* b, long long
     return g;
 }
 
+static int no_plan(const GemmShape& s) {
+    return fail(FG_ERR_UNSUPPORTED, "%lld x %lld outputs of %lld products: no tiles hold their sums", s.m, s.n, s.k);
+}
+
 // Do all of the epilogue's matrices start their rows on n bytes?
 static bool epilogue_lies(const Epilogue& e, int es, int n) {
     auto lies = [&](const void* p, long long ld) { return !p || (aligned(p, n) && ld * es % n == 0); };
@@ -1694,6 +1699,7 @@ int tc_gemm(int dtype, const void* a, long long a_plane, const void* b, long lon
     g.vec = epilogue_lies(e, es, 4 * es);
     g.direct = !epilogue_lies(e, es, 16);
     const TcPlan p = tc_plan(s, g.products, g.direct);
+    if (!p.bn) return no_plan(s);
     g.split = p.split;
 #define FG_PRODUCT(T)                                                                        \
     (p.pair ? (sizeof(T) == 4 || p.bn == 256                                              \
@@ -1716,6 +1722,7 @@ int tc_gated(int dtype, const void* a, long long a_plane, const void* b, long lo
     g.vec = both(4 * es);
     g.direct = !both(16);
     const TcPlan p = tc_plan(s, g.products, g.direct, TC_GATED);
+    if (!p.bn) return no_plan(s);
     g.split = p.split;
 #define FG_PRODUCT(T)                                                            \
     (p.pair        ? launch_pair<T, 256, TC_GATED>(dtype, a, b, s, g, nullptr, st) \
@@ -1739,6 +1746,7 @@ int tc_int8(int dtype, const void* a, const float* xs, const void* b, const floa
     GemmShape half = s;  // a K block holds 128 codes and takes the time of 64 elements of 16 bits
     half.k = (s.k + 1) / 2;
     const TcPlan p = tc_plan_of(half, 1, g.direct, TC_INT8);
+    if (!p.bn) return no_plan(s);
     g.split = p.split;
 #define FG_PRODUCT(T)                                                                       \
     (p.pair ? (sizeof(T) == 4 || p.bn == 256                                                 \

@@ -152,3 +152,38 @@ def test_muon_refused_step_moves_nothing(ad):
     there.grad = None
     opt.step()
     assert (here != 1).all()
+
+
+@pytest.mark.parametrize("n,o", [(2500, 2001), (2500, 2000), (700, 33)])
+def test_linear_int8_of_long_rows(ad, n, o):
+    """Sums past 65,536 codes are integers like any other: exact, and of the same tiles as
+    shorter ones.  2^-22 of the result: the sum's rounding to 32 bits, those of the two
+    products with the scales, and the result's."""
+    i = 65552
+    g = _gen(o)
+    x, w = (torch.randint(-128, 128, (k, i), generator=g, device="cuda", dtype=torch.int8) for k in (n, o))
+    xs, ws = (torch.rand(k, generator=g, device="cuda") + 0.5 for k in (n, o))
+    y = ad.linear_int8(x, xs, w, ws)
+    rows = torch.randint(0, n, (64,), generator=g, device="cuda")
+    want = (x[rows].double() @ w.double().t()) * xs[rows].double()[:, None] * ws.double()
+    assert bool(((y[rows].double() - want).abs() <= 2.0 ** -22 * want.abs()).all())
+
+
+def _kernels(f):
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        f()
+        torch.cuda.synchronize()
+    return [e.key for e in prof.key_averages()]
+
+
+@pytest.mark.parametrize("o", [2000, 2001])
+def test_linear_int8_of_long_rows_takes_pairs(ad, o):
+    """The kernel that takes rows of 65,536 codes takes longer ones too."""
+    xs, ws = torch.ones(2500, device="cuda"), torch.ones(o, device="cuda")
+    names = []
+    for i in (65536, 65552):
+        x, w = (torch.ones(k, i, device="cuda", dtype=torch.int8) for k in (2500, o))
+        names.append([k.split("<")[0] for k in _kernels(lambda: ad.linear_int8(x, xs, w, ws)) if "gemm_" in k])
+    if not names[0]:
+        pytest.skip("no kernels recorded")
+    assert names[0] == names[1]

@@ -1639,12 +1639,14 @@ static TcPlan tc_plan_of(const GemmShape& s, int products, bool direct, int mode
             // the sums' length: 512 k for each of float32's 512 / bn accumulators
             if (mode != TC_INT8 && kb > (products < 6 ? GT_RUN : GP_CHUNK * 512 / bn) * sp && kb > 3) continue;
             const int slots = sp == 1 ? sms : sp == 2 ? sms / 2 : std::max(1, sp == 4 ? sms * 32 / 148 : sms * 14 / 148);
-            // a second wave of clusters costs more than this estimate: gated 20,000 x 768 -> 100
-            // float32 in fours 105 us, in pairs 77 (plain layers keep the order of their sums)
-            if (mode != TC_WHOLE && sp > 1 && tiles > slots) break;
+            // waves of clusters cost 1.3 times this estimate: gated float32 20,000 x 768 -> 100 in fours
+            // 105 us, in pairs 77; 390 x 5,113 -> 620 in eights 72, in pairs 190; of 110 gated and
+            // 8-bit layers, where the two choices differ, the better one but for three (at most 12
+            // %).  Plain layers keep the order of their sums.
+            const double again = mode != TC_WHOLE && sp > 1 && tiles > slots ? 1.3 : 1.0;
             const double main = (kt + sp - 1) / sp * (bn == 256 ? 0.43 : bn == 128 ? 0.30 : 0.21);
             const double rows = direct ? 0.055 * bn : 0.0;
-            offer(5.0 + waves(tiles, slots) * (main + 2.0 + 0.02 * bn / sp + rows) + (sp == 8 ? 0.7 : 0.0), TcPlan{false, bn, sp, 0});
+            offer(again * (5.0 + waves(tiles, slots) * (main + 2.0 + 0.02 * bn / sp + rows)) + (sp == 8 ? 0.7 : 0.0), TcPlan{false, bn, sp, 0});
         }
     }
     return best;

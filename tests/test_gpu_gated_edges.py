@@ -187,3 +187,27 @@ def test_linear_int8_of_long_rows_takes_pairs(ad, o):
     if not names[0]:
         pytest.skip("no kernels recorded")
     assert names[0] == names[1]
+
+
+def _us(f, n=20):
+    for _ in range(3):
+        f()
+    best = math.inf
+    for _ in range(3):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(n):
+            f()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) * 1e3 / n)
+    return best
+
+
+@pytest.mark.parametrize("n,i,o", [(390, 5113, 620), (1882, 5504, 207), (6606, 5479, 54)])
+def test_gated_deep_sums_take_no_longer_than_plain_ones(ad, n, i, o):
+    """float32 layers of few tiles and long sums: the gated layer against the plain one of
+    as many columns, the same products (1.0 to 1.1 times as long; 1.8 is allowed)."""
+    g = _gen(n)
+    x, w = _randn(g, n, i), _randn(g, 2 * o, i, scale=i ** -0.5)
+    assert _us(lambda: ad.gated_linear(x, w)) <= 1.8 * _us(lambda: ad.linear(x, w))

@@ -211,3 +211,26 @@ def test_gated_deep_sums_take_no_longer_than_plain_ones(ad, n, i, o):
     g = _gen(n)
     x, w = _randn(g, n, i), _randn(g, 2 * o, i, scale=i ** -0.5)
     assert _us(lambda: ad.gated_linear(x, w)) <= 1.8 * _us(lambda: ad.linear(x, w))
+
+
+@pytest.mark.parametrize("nesterov,decay", [(True, 0.0), (True, 0.1), (False, 0.01)])
+@pytest.mark.parametrize("shape", [(60, 40), (30, 100), (300, 200)])
+def test_muon_against_its_formula_in_64_bits(ad, shape, nesterov, decay):
+    """Three float32 steps.  u is off by eight roundings at most of three times its own
+    magnitude (three gradients, as large each), and the iteration multiplies what X is off
+    by 3.4445, its largest slope, a step; the operator adds its own error (three standard
+    deviations).  p is rounded twice a step."""
+    from tests.test_gpu_orthogonalize import _iterate
+    g = _gen(shape[0])
+    p = _randn(g, *shape)
+    want, m, off = p.double(), torch.zeros_like(p).double(), 0.0
+    opt = ad.Muon([p], lr=0.05, momentum=0.9, nesterov=nesterov, weight_decay=decay)
+    scale = 0.05 * math.sqrt(max(1.0, shape[0] / shape[1]))
+    for _ in range(3):
+        p.grad = _randn(g, *shape)
+        opt.step()
+        m = 0.9 * m + p.grad.double()
+        o, err = _iterate(p.grad.double() + 0.9 * m if nesterov else m)
+        want = (1 - 0.05 * decay) * want - scale * o
+        off += scale * (3 * err + 3.4445 ** 5 * 24 * E32) + 2 * E32 * float(want.norm())
+        assert float((p.double() - want).norm()) <= off

@@ -531,7 +531,12 @@ class QuantizedQueryAdapter:
     """A trained :class:`QueryAdapter` whose matrices are codes of 8 bits with a scale
     per row; the rows that meet them are quantised on the way.  Layer norm, biases,
     activations and the residual stay as they are.  Keeps copies: the adapter may be
-    trained on."""
+    trained on.
+
+    Its matrices take a quarter of float32's bytes.  float32 adapters are faster so from
+    about a hundred queries on (768 wide, 10,000 queries: 153 us on the device, 343),
+    those of 16 bits only where they are plain and the queries very many (1,000,000:
+    4.3 ms, 4.7): the codes of the rows are passes of their own."""
 
     def __init__(self, adapter: QueryAdapter):
         p = adapter.params
@@ -553,6 +558,8 @@ class QuantizedQueryAdapter:
             q = queries.to(self.dtype)
             x, x_scale = quantize_rows(layer_norm(q, p["norm_weight"], p["norm_bias"]))
             h = self._inner(x, x_scale, slice(0, hid), self.activation)
+            # both factors and their product are of the adapter's type: the update is off by 2.67 % in
+            # bfloat16, with 32 bits there 2.66 %, since the codes make the error (768 -> 1024)
             if self.gated:
                 h *= self._inner(x, x_scale, slice(hid, 2 * hid), "none")
             h, h_scale = quantize_rows(h)
@@ -566,8 +573,12 @@ class Muon(torch.optim.Optimizer):
         p = (1 - lr weight_decay) p - lr sqrt(max(1, rows / cols)) orthogonalize(u)
 
     for matrices on the GPU; vectors go to another optimizer.  Matrices of one shape
-    and type are orthogonalised together.  m is of the parameter's type, as torch's
-    optimizers keep their states.
+    and type are orthogonalised together.  (K. Jordan and others, "Muon: An optimizer
+    for hidden layers in neural networks", 2024.)
+
+    m is of the parameter's type, as torch's optimizers keep their states: rounded twice
+    a step, it is off by 0.7 % of its norm in bfloat16 and 0.1 % in float16 (momentum
+    0.95).  Parameters of float32 keep all of it in 32 bits.
 
     A decay smaller than the type resolves (lr weight_decay below 2^-7 in bfloat16,
     2^-10 in float16) would be rounded away step by step, so it is held back, in the

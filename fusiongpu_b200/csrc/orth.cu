@@ -3,17 +3,18 @@
 //   X = G / (|G|_F + eps);  a number of times  A = X X^T,  B = b A + c A^2,  X = a X + B X
 //
 // (K. Jordan and others, "Muon: An optimizer for hidden layers in neural networks", 2024,
-// whose coefficients are the default; from the smaller side: for more rows than columns A = X^T X and X = a X + X B, without
-// a transposition in memory: the operands' layouts say which index runs along k).  Each
-// step maps the singular values s to a s + b s^3 + c s^5 and leaves the singular vectors.
+// whose coefficients are the default; from the smaller side: for more rows than columns A =
+// X^T X and X = a X + X B, without a transposition in memory: the operands' layouts say which
+// index runs along k).  Each step maps the singular values s to a s + b s^3 + c s^5 and
+// leaves the singular vectors.
 //
 // Matrices between the products are held as two float16 planes, x = h + 2^-11 l, 22 bits
 // of the significand or 2^-36, and a product is the three plane products that reach 2^-22
 // of it, with fp32 sums: the iteration multiplies what an operand's rounding leaves by up
 // to a^steps, and with one float16 plane the result was off by 2.4e-3 of its norm, with
-// one bfloat16 plane by 1.8e-2, with two by 1.1e-6 (four of 2048 x 1024) to 2.4e-6 (float32
-// throughout: 3.1e-6, 1.2e-6 to 3.5e-6 over the sizes).  Singular values stay of order one,
-// so that float16's range holds them.
+// one bfloat16 plane by 1.8e-2, with two by 1.1e-6 to 2.4e-6 (float32 throughout: 1.2e-6 to
+// 3.5e-6; four of 2048 x 1024 1.1e-6 and 3.1e-6).  Singular values stay of order one, so
+// that float16's range holds them.
 //
 // The tensor cores cut their sums, always towards zero: 1,024 k in one accumulator, and a I
 // as part of Y in X = Y X (or the completed square c (A + b / 2c)^2, which spares B's
